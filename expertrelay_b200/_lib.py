@@ -78,6 +78,53 @@ class MoeRowsIO(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    """struct er_kv_cache."""
+
+    _fields_ = [
+        ("k", _vp),
+        ("v", _vp),
+        ("dtype", _i),
+        ("num_pages", _i),
+        ("page_size", _i),
+        ("kv_heads", _i),
+        ("head_dim", _i),
+        ("page_stride", C.c_longlong),
+        ("head_stride", C.c_longlong),
+        ("slot_stride", C.c_longlong),
+        ("table", _vp),
+        ("seqs", _i),
+        ("table_width", _i),
+        ("table_stride", C.c_longlong),
+    ]
+
+
+class KvAttendIO(C.Structure):
+    """struct er_kv_attend_io."""
+
+    _fields_ = [
+        ("q", _vp),
+        ("q_dtype", _i),
+        ("q_stride", C.c_longlong),
+        ("out", _vp),
+        ("rows", _i),
+        ("heads", _i),
+        ("seqs", _vp),
+        ("lens", _vp),
+        ("scale", C.c_float),
+        ("pages", _vp),
+        ("counts", _vp),
+        ("max_pages", _i),
+        ("mass", _vp),
+        ("mass_row_stride", C.c_longlong),
+        ("mass_head_stride", C.c_longlong),
+        ("mass_len", _i),
+        ("status", _vp),
+    ]
+
+
+KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_SEQ = 1, 2, 4
+
 MOE_STAGES = ("router", "plan", "gate_up", "down", "combine")
 
 CACHE_DRY = 1
@@ -146,6 +193,15 @@ SIGNATURES: dict[str, tuple] = {
     "er_cache_resize": (_i, [_vp, _i, _vp, C.POINTER(_i)]),
     "er_cache_lookup": (_i, [_vp, _i, _i, C.POINTER(_i), C.POINTER(_i)]),
     "er_cache_stats_get": (_i, [_vp, C.POINTER(CacheStats)]),
+    "er_kv_append": (_i, [C.POINTER(KvCache), _vp, _i, C.c_longlong, _vp, _vp, _i, _i, C.c_double, _vp, _i, _vp, _vp]),
+    "er_kv_attend_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvAttendIO)]),
+    "er_kv_attend": (_i, [C.POINTER(KvCache), C.POINTER(KvAttendIO), _vp, C.c_size_t, _vp]),
+    "er_kv_page_bounds": (_i, [C.POINTER(KvCache), _vp, _vp, _vp, _vp, _vp, _vp]),
+    "er_kv_select_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), _i]),
+    "er_kv_select": (_i, [C.POINTER(KvCache), _vp, _i, C.c_longlong, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp,
+                          _vp, _vp, C.c_size_t, _vp]),
+    "er_kv_evict": (_i, [C.POINTER(KvCache), C.POINTER(KvCache), _vp, _vp, C.c_longlong, C.c_longlong, _i, _vp,
+                         C.c_longlong, C.c_longlong, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "er_trace_record_bytes": (C.c_size_t, [_i, _i]),
     "er_rms_norm": (_i, [_vp, _vp, _vp, C.c_float, _i, _i, _vp, _vp, _vp]),
     "er_rope_kv": (_i, [_vp, C.c_longlong, _vp, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _i, _vp]),

@@ -1,0 +1,245 @@
+// er_kv_append.cu -- new tokens into the paged key-value cache, and the
+// int8 bounds of its pages.
+//
+// Append: rotate-half RoPE (runtime/qwen_moe.py:126-138, 255-262) on the q
+// and k heads of a token's projection row and the write of k and v into the
+// token's page. The angle position * theta^(-2j/d) and its sine and cosine
+// are taken in 64 bits and rounded once: in 32 bits the product alone loses
+// 2^-24 of the angle, 0.004 rad at position 65536 of the fastest channel.
+#include "er_kv.cuh"
+
+namespace er {
+
+struct InvFreq {
+  double f[128];
+};
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// One CTA per token. The products and sums of the rotation are rounded one
+// by one (no fused multiply-add), so a key's bits do not depend on which
+// half of the pair it is, and the pages' codes follow from the formula alone.
+template <typename TX, typename TQ, typename TC>
+__global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
+                                                        const int32_t* __restrict__ seqs,
+                                                        const int32_t* __restrict__ positions, int heads,
+                                                        const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
+                                                        int* status) {
+  __shared__ float cs[256];  // [d/2] cos, then [d/2] sin
+  chain_wait();
+  const int t = blockIdx.x, d = kv.d, half = d / 2, kvh = kv.kv_heads;
+  const int pos = positions[t], seq = seqs ? seqs[t] : t;
+  for (int j = threadIdx.x; j < half; j += blockDim.x) {
+    double s, c;
+    sincos((double)pos * inv.f[j], &s, &c);
+    cs[j] = (float)c;
+    cs[half + j] = (float)s;
+  }
+  char *kp = nullptr, *vp = nullptr;
+  int bad = 0;
+  if (seq < 0 || seq >= kv.seqs) {
+    bad = ER_KV_BAD_SEQ;
+  } else if (pos < 0 || pos >= kv.capacity()) {
+    bad = ER_KV_BAD_LENGTH;
+  } else {
+    const int page = kv.pages_of(seq)[pos / kv.page_size];
+    if (page < 0 || page >= kv.num_pages) {
+      bad = ER_KV_BAD_PAGE;
+    } else {
+      const long long off = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride;
+      kp = kv.k + off;
+      vp = kv.v + off;
+    }
+  }
+  if (bad && threadIdx.x == 0) kv_report(status, bad);
+  __syncthreads();
+  const TX* row = qkv + (long long)t * ld;
+  for (int i = threadIdx.x; i < (heads + kvh) * half; i += blockDim.x) {
+    const int head = i / half, j = i % half;
+    const float c = cs[j], s = cs[half + j];
+    const float a = to_f32(row[(long long)head * d + j]), b = to_f32(row[(long long)head * d + j + half]);
+    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), y = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+    if (head < heads) {
+      TQ* qo = q_out + ((long long)t * heads + head) * d;
+      qo[j] = from_f32<TQ>(x);
+      qo[j + half] = from_f32<TQ>(y);
+    } else if (!bad) {
+      const long long h = head - heads;
+      TC* ko = reinterpret_cast<TC*>(kp + h * kv.head_stride);
+      ko[j] = from_f32<TC>(x);
+      ko[j + half] = from_f32<TC>(y);
+      TC* vo = reinterpret_cast<TC*>(vp + h * kv.head_stride);
+      const TX* vr = row + (long long)(head + kvh) * d;
+      vo[j] = from_f32<TC>(to_f32(vr[j]));
+      vo[j + half] = from_f32<TC>(to_f32(vr[j + half]));
+    }
+  }
+}
+
+// Least and greatest key of every channel of a page, a warp per (page, key
+// head): the lanes split a slot's 16-byte columns, lane groups the slots.
+template <typename TC>
+__global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t* __restrict__ lens,
+                                                        const int32_t* __restrict__ start, int8_t* __restrict__ codes,
+                                                        float* __restrict__ scales, int* status) {
+  constexpr int V = 16 / sizeof(TC);
+  chain_wait();
+  const int seq = blockIdx.y, h = blockIdx.z, lane = threadIdx.x & 31;
+  const int len = lens[seq], from = start[seq], ps = kv.page_size, d = kv.d;
+  if (len < 0 || len > kv.capacity() || from < 0) {
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) kv_report(status, ER_KV_BAD_LENGTH);
+    return;
+  }
+  if (from >= len) return;
+  const int cols = d / V;  // 1 .. 64
+  int wide = 1;            // lanes across a slot
+  while (wide < cols && wide < 32) wide *= 2;
+  const int col = lane % wide, group = lane / wide, groups = 32 / wide;
+  const int last = (len - 1) / ps;
+  for (int o = from / ps + blockIdx.x * 4 + (threadIdx.x >> 5); o <= last; o += gridDim.x * 4) {
+    const int page = kv.pages_of(seq)[o];
+    if (page < 0 || page >= kv.num_pages) {
+      if (lane == 0) kv_report(status, ER_KV_BAD_PAGE);
+      continue;
+    }
+    const int slots = min(ps, len - o * ps);
+    const char* base = kv.k + page * kv.page_stride + h * kv.head_stride;
+    float lo[2][V], hi[2][V];
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < V; ++e) lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int c = col + 32 * w;
+      if (c < cols) {
+#pragma unroll 4
+        for (int s = group; s < slots; s += groups) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(base + s * kv.slot_stride + c * 16);
+          const TC* x = reinterpret_cast<const TC*>(&raw);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float f = to_f32(x[e]);
+            lo[w][e] = fminf(lo[w][e], f);
+            hi[w][e] = fmaxf(hi[w][e], f);
+          }
+        }
+      }
+    }
+    float top = 0.f;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        for (int x = wide; x < 32; x *= 2) {
+          lo[w][e] = fminf(lo[w][e], __shfl_xor_sync(0xffffffffu, lo[w][e], x));
+          hi[w][e] = fmaxf(hi[w][e], __shfl_xor_sync(0xffffffffu, hi[w][e], x));
+        }
+        if (col + 32 * w < cols && lo[w][e] <= hi[w][e]) top = fmaxf(top, fmaxf(fabsf(lo[w][e]), fabsf(hi[w][e])));
+      }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float scale = top * kCodeStep;
+    const long long at = ((long long)page * kv.kv_heads + h) * 2 * d;
+    if (lane == 0) scales[(long long)page * kv.kv_heads + h] = scale;
+    if (group == 0) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int c = col + 32 * w;
+        if (c < cols) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            float a = 0.f, b = 0.f;
+            if (scale > 0.f && lo[w][e] <= hi[w][e]) {
+              a = rintf(lo[w][e] / scale);
+              b = rintf(hi[w][e] / scale);
+            }
+            codes[at + c * V + e] = (int8_t)(a == a ? (int)fminf(fmaxf(a, -127.f), 127.f) : 0);
+            codes[at + d + c * V + e] = (int8_t)(b == b ? (int)fminf(fmaxf(b, -127.f), 127.f) : 0);
+          }
+        }
+      }
+    }
+  }
+}
+
+namespace {
+
+// theta^(-2j/d), kept for the last (theta, d) of the calling thread
+const InvFreq& inv_freq(double theta, int d) {
+  static thread_local InvFreq f;
+  static thread_local double last_theta = 0.0;
+  static thread_local int last_d = 0;
+  if (theta != last_theta || d != last_d) {
+    for (int j = 0; j < d / 2; ++j) f.f[j] = pow(theta, -2.0 * j / d);
+    last_theta = theta;
+    last_d = d;
+  }
+  return f;
+}
+
+template <typename TX, typename TQ, typename TC>
+int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* seqs, const int32_t* positions, int n,
+              int heads, double theta, void* q_out, int* status, cudaStream_t st) {
+  return launch_chained(kv_append_kernel<TX, TQ, TC>, dim3(n), dim3(256), 0, st, "kv_append_kernel", kv,
+                        (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
+}
+
+}  // namespace
+}  // namespace er
+
+using namespace er;
+
+extern "C" int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype, long long ld,
+                            const int32_t* seqs, const int32_t* positions, int n, int heads, double theta, void* q_out,
+                            int q_dtype, int* status, void* stream) {
+  if (int rc = kv_check("er_kv_append", cache)) return rc;
+  if (n < 0 || heads <= 0 || !(theta > 0))
+    return fail(ER_EINVAL, "er_kv_append: n %d, heads %d, theta %g", n, heads, theta);
+  if ((qkv_dtype != ER_DTYPE_F32 && qkv_dtype != ER_DTYPE_BF16) || (q_dtype != ER_DTYPE_F32 && q_dtype != ER_DTYPE_BF16))
+    return fail(ER_EINVAL, "er_kv_append: dtypes %d, %d", qkv_dtype, q_dtype);
+  if (ld < (long long)(heads + 2 * cache->kv_heads) * cache->head_dim)
+    return fail(ER_EINVAL, "er_kv_append: row stride %lld shorter than q|k|v (%lld)", ld,
+                (long long)(heads + 2 * cache->kv_heads) * cache->head_dim);
+  if (n == 0) return ER_OK;
+  if (!qkv || !positions || !q_out) return fail(ER_EINVAL, "er_kv_append: null pointer");
+  const KvView kv = kv_view(*cache);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int sel = (qkv_dtype == ER_DTYPE_BF16) * 4 + (q_dtype == ER_DTYPE_BF16) * 2 + (cache->dtype == ER_DTYPE_BF16);
+  using bf = __nv_bfloat16;
+  switch (sel) {
+    case 0: return append_go<float, float, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 1: return append_go<float, float, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 2: return append_go<float, bf, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 3: return append_go<float, bf, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 4: return append_go<bf, float, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 5: return append_go<bf, float, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 6: return append_go<bf, bf, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    default: return append_go<bf, bf, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+  }
+}
+
+extern "C" int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, const int32_t* start, int8_t* codes,
+                                 float* scales, int* status, void* stream) {
+  if (int rc = kv_check("er_kv_page_bounds", cache)) return rc;
+  if (cache->seqs == 0 || cache->table_width == 0) return ER_OK;
+  if (!lens || !start || !codes || !scales) return fail(ER_EINVAL, "er_kv_page_bounds: null pointer");
+  if (cache->seqs > 65535 || cache->kv_heads > 65535)
+    return fail(ER_EINVAL, "er_kv_page_bounds: %d sequences, %d key heads", cache->seqs, cache->kv_heads);
+  const KvView kv = kv_view(*cache);
+  // a step touches one page a sequence, a prompt all of them: the CTAs of a
+  // (sequence, key head) walk its pages, about 16 CTAs an SM in all
+  const long long want = 148 * 16 / ((long long)kv.seqs * kv.kv_heads), most = (kv.width + 3) / 4;
+  const unsigned gx = (unsigned)(want < 1 ? 1 : want > most ? most : want);
+  const dim3 grid(gx, kv.seqs, kv.kv_heads);
+  if (cache->dtype == ER_DTYPE_BF16)
+    return launch_chained(kv_bounds_kernel<__nv_bfloat16>, grid, dim3(128), 0, (cudaStream_t)stream,
+                          "kv_bounds_kernel", kv, lens, start, codes, scales, status);
+  return launch_chained(kv_bounds_kernel<float>, grid, dim3(128), 0, (cudaStream_t)stream, "kv_bounds_kernel", kv,
+                        lens, start, codes, scales, status);
+}

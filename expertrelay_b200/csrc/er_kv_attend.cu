@@ -1,0 +1,499 @@
+// er_kv_attend.cu -- attention of rows of queries over the paged key-value
+// cache: the fp32 kernel, the join of split rows, the accumulated attention
+// weight, and the entry point.
+#include "er_kv_attend.cuh"
+
+namespace er {
+
+constexpr int kSimtStages = 3;
+
+struct SimtShape {
+  int warps, pitch, smem;
+};
+
+// Shared memory of the fp32 kernel: queries, the warps' pieces, probabilities
+// and key masks, then per warp a ring of kSimtStages chunks of keys and values.
+inline SimtShape simt_shape(int d, int es, int gb) {
+  SimtShape s;
+  s.pitch = d * es + ((d * es / 16) % 2 ? 0 : 16);  // an odd number of 16-byte columns: no bank conflicts across keys
+  for (s.warps = 4; s.warps >= 1; s.warps /= 2) {
+    s.smem = gb * d * 4 + s.warps * gb * (d + 2) * 4 + s.warps * gb * kKvChunk * 4 + 64 +
+             s.warps * kSimtStages * (2 * kKvChunk * s.pitch);
+    if (s.smem <= 220 * 1024) break;
+  }
+  return s;
+}
+
+// fp32 throughout: a warp takes 16 keys at a time, from its own ring of
+// asynchronous copies. Scores: lane l holds key l % 16 and half of the
+// columns. Values: the lanes split a row's 16-byte columns, lane groups the
+// keys. GB queries of the group at a time share each key that is read.
+template <typename TC, typename TQ, int GB>
+__global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_constant__ AttendArgs a, int pitch) {
+  constexpr int V = 16 / sizeof(TC);
+  extern __shared__ __align__(16) char sm[];
+  __shared__ long long sums[129];
+  __shared__ int where[3], spoiled;
+  const int d = a.kv.d, warps = blockDim.x / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* qs = reinterpret_cast<float*>(sm);                // [GB][d]
+  float* merge = qs + GB * d;                              // [warps][GB][d + 2]: m, l, o
+  float* prob = merge + warps * GB * (d + 2) + warp * GB * kKvChunk;  // [16][GB]
+  char* ring0 = sm + ((GB * d + warps * GB * (d + 2) + warps * GB * kKvChunk) * 4 + 15) / 16 * 16;
+  char* ring = ring0 + warp * kSimtStages * 2 * kKvChunk * pitch;
+  const int cols = d / V;
+  int wide = 2;  // lanes across a row; at most 16 rows at a time, so every lane group has as many
+  while (wide < cols && wide < 32) wide *= 2;
+  const int col = lane % wide, kg = lane / wide, kgs = 32 / wide;
+  const int cw = cols > 32 ? 2 : 1;  // columns a lane
+
+  chain_wait();
+  Place c;
+  long long left;
+  const long long begin = kv_run(a, sums, where, c, &left);
+  (void)begin;
+  if (left == 0) return;
+
+  uint32_t live[kSimtStages];  // keys of a stage that exist, bad ones in the upper half
+  Place f = c;
+  long long ahead = left;
+  auto fetch = [&](int st) {
+    uint32_t mask = 0;
+    if (ahead > 0) {
+      const int j0 = f.t * a.tile + warp * kKvChunk;
+      const int h = f.head(a);
+      const long long off = lane < kKvChunk ? kv_locate(a, f, h, j0 + lane) : -1;
+      mask = __ballot_sync(0xffffffffu, off >= 0) | (__ballot_sync(0xffffffffu, off == -2) << 16);
+      const uint32_t kd = smem_addr(ring + st * 2 * kKvChunk * pitch), vd = kd + kKvChunk * pitch;
+      for (int r = kg; r < kKvChunk; r += kgs) {
+        const long long o = __shfl_sync(0xffffffffu, off, r);
+        const int bytes = o >= 0 ? 16 : 0;
+        const long long at = o >= 0 ? o : 0;
+        for (int w = 0; w < cw; ++w) {
+          const int cc = col + 32 * w;
+          if (cc < cols) {
+            copy16(kd + r * pitch + cc * 16, a.kv.k + at + cc * 16, bytes);
+            copy16(vd + r * pitch + cc * 16, a.kv.v + at + cc * 16, bytes);
+          }
+        }
+      }
+      if (--ahead > 0) f.next(a);
+    }
+    copy_commit();
+    return mask;
+  };
+#pragma unroll
+  for (int s = 0; s < kSimtStages; ++s) live[s] = fetch(s);
+
+  float m[GB], l[GB], o[GB][8];
+  bool fresh = true;
+  int st = 0, first_t = 0;
+  bool bad = false;
+  while (left > 0) {
+    const int h = c.head(a), blk = c.block(a), row = c.row(a);
+    const int g0 = blk * GB, live_g = min(GB, a.group - g0);
+    if (fresh) {  // a new unit: its queries
+      fresh = false;
+      bad = false;
+      first_t = c.t;
+      const TQ* q = (const TQ*)a.q + (long long)row * a.q_stride + (long long)(h * a.group + g0) * d;
+      for (int i = threadIdx.x; i < GB * d; i += blockDim.x) qs[i] = i < live_g * d ? to_f32(q[i]) : 0.f;
+      if (threadIdx.x == 0) spoiled = 0;
+      __syncthreads();
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[g][e] = 0.f;
+      }
+    }
+    copy_wait<kSimtStages - 1>();
+    __syncwarp();
+    uint32_t mask = live[0];
+#pragma unroll
+    for (int s = 1; s < kSimtStages; ++s)
+      if (s == st) mask = live[s];
+    if (mask >> 16) bad = true;
+    if (mask & 0xffff) {
+      const char* kc = ring + st * 2 * kKvChunk * pitch;
+      const char* vc = kc + kKvChunk * pitch;
+      const int key = lane & 15;
+      const bool on = (mask >> key) & 1;
+      float s[GB];
+#pragma unroll
+      for (int g = 0; g < GB; ++g) s[g] = 0.f;
+      for (int cc = lane >> 4; cc < cols; cc += 2) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(kc + key * pitch + cc * 16);
+        const TC* kx = reinterpret_cast<const TC*>(&raw);
+        float kf[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) kf[e] = to_f32(kx[e]);
+#pragma unroll
+        for (int g = 0; g < GB; ++g)
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            const float4 qv = *reinterpret_cast<const float4*>(qs + g * d + cc * V + e);
+            s[g] = fmaf(qv.x, kf[e], fmaf(qv.y, kf[e + 1], fmaf(qv.z, kf[e + 2], fmaf(qv.w, kf[e + 3], s[g]))));
+          }
+      }
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        s[g] = (s[g] + __shfl_xor_sync(0xffffffffu, s[g], 16)) * a.scale;
+        if (!on) s[g] = -INFINITY;
+      }
+      if (a.scores && on && lane < 16) {
+        float* to = a.scores + (((long long)row * a.kv.kv_heads + h) * a.mass_len + c.t * a.tile + warp * kKvChunk + key) *
+                                   a.group + g0;
+#pragma unroll
+        for (int g = 0; g < GB; ++g)
+          if (g < live_g) to[g] = s[g];
+      }
+#pragma unroll
+      for (int g = 0; g < GB; ++g) {
+        float top = s[g];
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float now = fmaxf(m[g], top);
+        const float base = now == -INFINITY ? 0.f : now;  // scores of -inf alone weigh nothing
+        const float keep = exp2f(m[g] - base);
+        m[g] = now;
+        const float p = on ? exp2f(s[g] - base) : 0.f;
+        l[g] = l[g] * keep + (lane < 16 ? p : 0.f);
+        if (lane < 16) prob[key * GB + g] = p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[g][e] *= keep;
+      }
+      __syncwarp();
+      for (int r = kg; r < kKvChunk; r += kgs) {
+        float p[GB];
+#pragma unroll
+        for (int g = 0; g < GB; ++g) p[g] = prob[r * GB + g];
+#pragma unroll
+        for (int w = 0; w < 8 / V; ++w) {
+          const int cc = col + 32 * w;
+          if (cc < cols) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(vc + r * pitch + cc * 16);
+            const TC* vx = reinterpret_cast<const TC*>(&raw);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float f = to_f32(vx[e]);
+#pragma unroll
+              for (int g = 0; g < GB; ++g) o[g][w * V + e] = fmaf(p[g], f, o[g][w * V + e]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    const uint32_t got = fetch(st);
+#pragma unroll
+    for (int s = 0; s < kSimtStages; ++s)
+      if (s == st) live[s] = got;
+    st = st + 1 == kSimtStages ? 0 : st + 1;
+    --left;
+    const int t = c.t, tiles = c.tiles;
+    if (t + 1 < tiles && left > 0) {
+      ++c.t;
+      continue;
+    }
+    // the unit ends here, or the CTA's part of it: the warps' pieces join
+#pragma unroll
+    for (int g = 0; g < GB; ++g) {
+      l[g] = warp_sum(l[g]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        for (int x = wide; x < 32; x *= 2) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], x);
+      float* to = merge + (warp * GB + g) * (d + 2);
+      if (lane == 0) {
+        to[0] = m[g];
+        to[1] = l[g];
+      }
+      if (kg == 0) {
+#pragma unroll
+        for (int w = 0; w < 8 / V; ++w)
+          if (col + 32 * w < cols) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) to[2 + (col + 32 * w) * V + e] = o[g][w * V + e];
+          }
+      }
+    }
+    if (bad && lane == 0) spoiled = 1;
+    __syncthreads();
+    const bool whole = first_t == 0 && t + 1 == tiles;
+    const bool nan = spoiled != 0;
+    if (nan && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
+    for (int i = threadIdx.x; i < GB * d; i += blockDim.x) {
+      const int g = i / d, cc = i % d;
+      if (g >= live_g) continue;
+      const float* from = merge + g * (d + 2);
+      float top = -INFINITY, sum = 0.f, acc = 0.f;
+      for (int w = 0; w < warps; ++w) top = fmaxf(top, from[w * GB * (d + 2)]);
+      for (int w = 0; w < warps; ++w) {
+        const float* p = from + w * GB * (d + 2);
+        const float by = piece_weight(p[0], top);
+        sum = fmaf(p[1], by, sum);
+        acc = fmaf(p[2 + cc], by, acc);
+      }
+      if (nan) sum = acc = __int_as_float(0x7fc00000);
+      if (whole) {
+        const long long at = (long long)row * a.heads + h * a.group + g0 + g;
+        ((TQ*)a.out)[at * d + cc] = kv_round<TQ>(sum == 0.f ? 0.f : acc / sum);
+        if (a.scores && cc == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
+      } else {
+        const long long slot = (long long)blockIdx.x * 2 + (first_t != 0 ? 0 : 1);
+        a.part_o[(slot * GB + g) * d + cc] = acc;
+        if (cc == 0) {
+          a.part_ml[(slot * GB + g) * 2] = top;
+          a.part_ml[(slot * GB + g) * 2 + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    fresh = true;
+    if (left > 0) c.next(a);
+  }
+}
+
+// One CTA per (row, key head, head block): rows without keys get zeros, bad
+// ones NaN, split ones the join of their pieces. The pieces of a unit are the
+// CTAs whose runs meet it, in order: the first piece of a CTA that began
+// before the unit's start is impossible, so a CTA's piece is its first one
+// when the unit began before the CTA's run, its last one otherwise.
+template <typename TQ>
+__global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ AttendArgs a, int gb) {
+  chain_wait();
+  const int per_row = a.kv.kv_heads * a.blocks;
+  const int row = blockIdx.x / per_row, rest = blockIdx.x % per_row, h = rest / a.blocks, blk = rest % a.blocks;
+  const int x = a.pages ? row * a.kv.kv_heads + h : row, u = a.pages ? blk : rest;
+  const int d = a.kv.d, g0 = blk * gb, live_g = min(gb, a.group - g0);
+  const long long total = a.prefix[a.entries] * a.units, c = a.prefix[x + 1] - a.prefix[x];
+  const long long at = (long long)row * a.heads + h * a.group + g0;
+  TQ* out = (TQ*)a.out + at * d;
+  if (c == 0) {
+    const float v = kv_entry(a, x).bad ? __int_as_float(0x7fc00000) : 0.f;
+    for (int i = threadIdx.x; i < live_g * d; i += blockDim.x) out[i] = kv_round<TQ>(v);
+    return;
+  }
+  const long long begin = a.prefix[x] * a.units + (long long)u * c;
+  const int shares = kv_shares(a, total);
+  const int i0 = kv_share_of(total, shares, begin), i1 = kv_share_of(total, shares, begin + c - 1);
+  if (i0 == i1) return;  // written whole
+  for (int i = threadIdx.x; i < live_g * d; i += blockDim.x) {
+    const int g = i / d, cc = i % d;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+    for (int k = i0; k <= i1; ++k) {
+      const long long slot = (long long)k * 2 + (kv_share_start(total, shares, k) > begin ? 0 : 1);
+      top = fmaxf(top, a.part_ml[(slot * gb + g) * 2]);
+    }
+    for (int k = i0; k <= i1; ++k) {
+      const long long slot = (long long)k * 2 + (kv_share_start(total, shares, k) > begin ? 0 : 1);
+      const float mi = a.part_ml[(slot * gb + g) * 2], li = a.part_ml[(slot * gb + g) * 2 + 1];
+      const float by = li != li ? 1.f : piece_weight(mi, top);  // a spoiled piece spoils the row
+      sum = fmaf(li, by, sum);
+      acc = fmaf(a.part_o[(slot * gb + g) * d + cc], by, acc);
+    }
+    out[i] = kv_round<TQ>(sum == 0.f ? 0.f : acc / sum);
+    if (a.scores && cc == 0) a.lse[at + g] = sum == 0.f ? INFINITY : top + log2f(sum);
+  }
+}
+
+// mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position.
+__global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ AttendArgs a) {
+  chain_wait();
+  const int unit = blockIdx.y, row = unit / a.kv.kv_heads, h = unit % a.kv.kv_heads;
+  const Entry e = kv_entry(a, row);
+  float* to = a.mass + row * a.mass_row_stride + h * a.mass_head_stride;
+  const float* s = a.scores + (long long)unit * a.mass_len * a.group;
+  const float* lse = a.lse + (long long)row * a.heads + h * a.group;
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < e.n; j += gridDim.x * 256) {
+    float sum = 0.f;
+    for (int g = 0; g < a.group; ++g) sum += exp2f(s[(long long)j * a.group + g] - lse[g]);
+    to[j] += sum;
+  }
+}
+
+namespace {
+
+template <typename TC, typename TQ, int GB>
+int simt_go(const AttendArgs& a, cudaStream_t st) {
+  const SimtShape s = simt_shape(a.kv.d, sizeof(TC), GB);
+  auto kernel = kv_attend_simt_kernel<TC, TQ, GB>;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem),
+                          "kv_attend smem attribute"))
+    return rc;
+  return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a, s.pitch);
+}
+
+template <typename TC, typename TQ>
+int simt_gb(const AttendArgs& a, int gb, cudaStream_t st) {
+  switch (gb) {
+    case 1: return simt_go<TC, TQ, 1>(a, st);
+    case 2: return simt_go<TC, TQ, 2>(a, st);
+    case 4: return simt_go<TC, TQ, 4>(a, st);
+    default: return simt_go<TC, TQ, 8>(a, st);
+  }
+}
+
+// queries of a group that a CTA takes together
+inline int head_block(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
+
+constexpr int kMaxEntries = 4096;  // scan entries a launch takes; more rows go in several launches
+
+struct Layout {
+  int gb, blocks, warps, grid, rows;  // rows: of one launch
+  size_t prefix, ml, o, lse, scores, bytes;
+};
+
+Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
+  Layout L;
+  const int group = io.heads / c.kv_heads;
+  L.gb = head_block(group);
+  L.blocks = (group + L.gb - 1) / L.gb;
+  const SimtShape s = simt_shape(c.head_dim, c.dtype == ER_DTYPE_BF16 ? 2 : 4, L.gb);
+  L.warps = s.warps;
+  const int per_sm = 227 * 1024 / (s.smem + 2048);
+  L.grid = sms * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+  L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
+  if (L.rows < 1) L.rows = 1;
+  if (L.rows > io.rows) L.rows = io.rows;
+  const size_t entries = io.pages ? (size_t)L.rows * c.kv_heads : L.rows;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes, 256);
+    return here;
+  };
+  L.prefix = take((entries + 1) * 8);
+  L.ml = take((size_t)L.grid * 2 * L.gb * 2 * 4);
+  L.o = take((size_t)L.grid * 2 * L.gb * c.head_dim * 4);
+  L.lse = take(io.mass ? (size_t)L.rows * io.heads * 4 : 0);
+  L.scores = take(io.mass ? (size_t)L.rows * io.heads * io.mass_len * 4 : 0);
+  L.bytes = at;
+  return L;
+}
+
+int attend_check(const er_kv_cache* c, const er_kv_attend_io* io) {
+  if (int rc = kv_check("er_kv_attend", c)) return rc;
+  if (!io) return fail(ER_EINVAL, "er_kv_attend: null io");
+  if (io->rows < 0 || io->heads <= 0 || io->heads % c->kv_heads)
+    return fail(ER_EINVAL, "er_kv_attend: rows %d, heads %d / %d", io->rows, io->heads, c->kv_heads);
+  if (io->q_dtype != ER_DTYPE_F32 && io->q_dtype != ER_DTYPE_BF16)
+    return fail(ER_EINVAL, "er_kv_attend: q dtype %d", io->q_dtype);
+  if (io->q_stride < (long long)io->heads * c->head_dim)
+    return fail(ER_EINVAL, "er_kv_attend: row stride %lld shorter than the queries", io->q_stride);
+  if (io->pages && (io->max_pages <= 0 || !io->counts))
+    return fail(ER_EINVAL, "er_kv_attend: page lists of %d without counts or room", io->max_pages);
+  if (io->pages && io->mass) return fail(ER_EINVAL, "er_kv_attend: mass is not accumulated over page lists");
+  if (io->mass && io->mass_len < 0) return fail(ER_EINVAL, "er_kv_attend: mass_len %d", io->mass_len);
+  if (!io->seqs && io->rows > c->seqs)
+    return fail(ER_EINVAL, "er_kv_attend: %d rows, %d sequences", io->rows, c->seqs);
+  if (io->pages && c->kv_heads > kMaxEntries) return fail(ER_EINVAL, "er_kv_attend: %d key heads", c->kv_heads);
+  return ER_OK;
+}
+
+int device_sms(int* sms) {
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  return cuda_check(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
+}
+
+}  // namespace
+}  // namespace er
+
+using namespace er;
+
+extern "C" size_t er_kv_attend_workspace_bytes(const er_kv_cache* cache, const er_kv_attend_io* io) {
+  int sms = 0;
+  if (attend_check(cache, io) || io->rows == 0 || device_sms(&sms)) return 0;
+  return attend_layout(*cache, *io, sms).bytes;
+}
+
+extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  if (int rc = attend_check(cache, io)) return rc;
+  if (io->rows == 0) return ER_OK;
+  if (!io->q || !io->out || !io->lens) return fail(ER_EINVAL, "er_kv_attend: null pointer");
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const Layout L = attend_layout(*cache, *io, sms);
+  if (!workspace || workspace_bytes < L.bytes)
+    return fail(ER_ENOSPACE, "er_kv_attend: workspace %zu bytes, need %zu", workspace_bytes, L.bytes);
+  cudaStream_t st = (cudaStream_t)stream;
+  char* ws = (char*)workspace;
+  const size_t qs = io->q_dtype == ER_DTYPE_BF16 ? 2 : 4;
+  for (int r0 = 0; r0 < io->rows; r0 += L.rows) {
+    AttendArgs a = {};
+    a.kv = kv_view(*cache);
+    a.rows = io->rows - r0 < L.rows ? io->rows - r0 : L.rows;
+    if (!io->seqs) {  // the launch's rows are sequences r0 ..
+      a.kv.table += r0 * a.kv.table_stride;
+      a.kv.seqs -= r0;
+    }
+    a.q = (const char*)io->q + (size_t)r0 * io->q_stride * qs;
+    a.q_stride = io->q_stride;
+    a.out = (char*)io->out + (size_t)r0 * io->heads * cache->head_dim * qs;
+    a.heads = io->heads;
+    a.group = io->heads / cache->kv_heads;
+    a.blocks = L.blocks;
+    a.seqs = io->seqs ? io->seqs + r0 : nullptr;
+    a.lens = io->lens + r0;
+    a.scale = io->scale * 1.4426950408889634f;
+    a.max_pages = io->max_pages;
+    if (io->pages) {
+      a.pages = io->pages + (size_t)r0 * cache->kv_heads * io->max_pages;
+      a.counts = io->counts + (size_t)r0 * cache->kv_heads;
+    }
+    a.tile = L.warps * kKvChunk;
+    a.min_tiles = 2;
+    a.status = io->status;
+    a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;
+    a.units = io->pages ? L.blocks : cache->kv_heads * L.blocks;
+    a.prefix = (long long*)(ws + L.prefix);
+    a.part_ml = (float*)(ws + L.ml);
+    a.part_o = (float*)(ws + L.o);
+    a.grid = L.grid;
+    if (io->mass) {
+      a.lse = (float*)(ws + L.lse);
+      a.scores = (float*)(ws + L.scores);
+      a.mass = io->mass + r0 * io->mass_row_stride;
+      a.mass_row_stride = io->mass_row_stride;
+      a.mass_head_stride = io->mass_head_stride;
+      a.mass_len = io->mass_len;
+    }
+    int rc;
+    using bf = __nv_bfloat16;
+    const bool cb = cache->dtype == ER_DTYPE_BF16, qb = io->q_dtype == ER_DTYPE_BF16;
+    if (cb)
+      rc = qb ? simt_gb<bf, bf>(a, L.gb, st) : simt_gb<bf, float>(a, L.gb, st);
+    else
+      rc = qb ? simt_gb<float, bf>(a, L.gb, st) : simt_gb<float, float>(a, L.gb, st);
+    if (rc) return rc;
+    const unsigned units = (unsigned)a.rows * cache->kv_heads * L.blocks;
+    rc = qb ? launch_chained(kv_join_kernel<bf>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, L.gb)
+            : launch_chained(kv_join_kernel<float>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, L.gb);
+    if (rc) return rc;
+    if (io->mass && io->mass_len > 0) {
+      const int pairs = a.rows * cache->kv_heads;
+      for (int p0 = 0; p0 < pairs; p0 += 65535 / cache->kv_heads * cache->kv_heads) {
+        AttendArgs b = a;  // whole rows at a time: the grid's y extent is 16 bits
+        const int r = p0 / cache->kv_heads, n = pairs - p0 < 65535 / cache->kv_heads * cache->kv_heads
+                                                    ? pairs - p0
+                                                    : 65535 / cache->kv_heads * cache->kv_heads;
+        b.lens += r;
+        if (b.seqs) {
+          b.seqs += r;
+        } else {
+          b.kv.table += r * b.kv.table_stride;
+          b.kv.seqs -= r;
+        }
+        b.mass += r * b.mass_row_stride;
+        b.scores += (size_t)p0 * b.mass_len * b.group;
+        b.lse += (size_t)r * b.heads;
+        const int most = (io->mass_len + 255) / 256, want = sms * 8 / n + 1;
+        rc = launch_chained(kv_mass_kernel, dim3(most < want ? most : want, n), dim3(256), 0, st, "kv_mass_kernel", b);
+        if (rc) return rc;
+      }
+    }
+  }
+  return ER_OK;
+}

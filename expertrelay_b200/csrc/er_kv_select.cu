@@ -1,0 +1,292 @@
+// er_kv_select.cu -- the pages worth reading for each query, and the
+// positions worth keeping in a cache that grows too long.
+//
+// Both rank by a score and take the best: a radix select by the whole CTA
+// (er_kv.cuh) finds the score of the last one taken, a second pass in
+// position order writes the taken ones ascending, equal scores to the lower
+// position.
+#include "er_kv.cuh"
+
+namespace er {
+
+constexpr int kScoreThreads = 256;
+
+// Page scores of one (row, key head): the group's queries as int8 codes
+// against the pages' int8 bounds. 8 codes of each bound per lane, `wide`
+// lanes a page. The dot products are exact integers (|I| <= 256 * 127^2 <
+// 2^24, so float(I) is exact too) and the two roundings after them are in a
+// fixed order: the scores, and so the choice, are the same on any grid.
+template <typename TQ>
+__global__ void __launch_bounds__(kScoreThreads)
+    kv_score_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
+                    const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
+                    const float* __restrict__ scales, float* __restrict__ scores, int* status) {
+  extern __shared__ __align__(16) int8_t qc[];  // [group][2][d]: negative codes, positive codes; then [group] floats t
+  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
+  chain_wait();
+  const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads, d = kv.d;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int seq = seqs ? seqs[row] : row, len = lens[row];
+  if (seq < 0 || seq >= kv.seqs || len < 0 || len > kv.capacity()) return;  // reported by the selection
+  const int np = (len + kv.page_size - 1) / kv.page_size;
+  for (int g = warp; g < group; g += kScoreThreads / 32) {
+    const TQ* qr = q + (long long)row * q_stride + (long long)(h * group + g) * d;
+    float top = 0.f;
+    bool nan = false;
+    for (int c = lane; c < d; c += 32) {
+      const float x = to_f32(qr[c]);
+      nan |= x != x;
+      top = fmaxf(top, fabsf(x));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float t = top * kCodeStep;
+    if (__any_sync(0xffffffffu, nan)) t = __int_as_float(0x7fc00000);
+    for (int c = lane; c < d; c += 32) {
+      float r = t == 0.f ? 0.f : rintf(to_f32(qr[c]) / t);
+      r = r == r ? fminf(fmaxf(r, -127.f), 127.f) : 0.f;
+      qc[(g * 2 + 0) * d + c] = (int8_t)fminf(r, 0.f);
+      qc[(g * 2 + 1) * d + c] = (int8_t)fmaxf(r, 0.f);
+    }
+    if (lane == 0) qt[g] = t;
+  }
+  __syncthreads();
+  const int cols = d / 8;  // 1 .. 32
+  int wide = 1;
+  while (wide < cols) wide *= 2;
+  const int col = lane % wide, per = 32 / wide;
+  float* out = scores + (long long)blockIdx.y * kv.width;
+  for (int o0 = (blockIdx.x * (kScoreThreads / 32) + warp) * per; o0 < np; o0 += gridDim.x * (kScoreThreads / 32) * per) {
+    const int o = o0 + lane / wide;
+    const int page = o < np ? kv.pages_of(seq)[o] : -1;
+    const bool ok = page >= 0 && page < kv.num_pages;
+    if (o < np && !ok && col == 0) kv_report(status, ER_KV_BAD_PAGE);
+    uint2 lo = make_uint2(0, 0), hi = lo;
+    float scale = 0.f;
+    if (ok) {
+      const long long at = (long long)page * kv.kv_heads + h;
+      scale = scales[at];
+      if (col < cols) {
+        lo = *reinterpret_cast<const uint2*>(codes + at * 2 * d + col * 8);
+        hi = *reinterpret_cast<const uint2*>(codes + at * 2 * d + d + col * 8);
+      }
+    }
+    float best = -INFINITY;
+    bool nan = !ok;
+    for (int g = 0; g < group; ++g) {
+      int sum = 0;
+      if (col < cols) {
+        const uint2 neg = *reinterpret_cast<const uint2*>(qc + (g * 2 + 0) * d + col * 8);
+        const uint2 pos = *reinterpret_cast<const uint2*>(qc + (g * 2 + 1) * d + col * 8);
+        sum = __dp4a((int)neg.x, (int)lo.x, sum);
+        sum = __dp4a((int)neg.y, (int)lo.y, sum);
+        sum = __dp4a((int)pos.x, (int)hi.x, sum);
+        sum = __dp4a((int)pos.y, (int)hi.y, sum);
+      }
+      for (int x = wide / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      const float v = __fmul_rn((float)sum, qt[g]);
+      nan |= v != v;
+      best = fmaxf(best, v);
+    }
+    if (o < np && col == 0) out[o] = nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale);
+  }
+}
+
+// Writes, ascending, the `take` of n positions that are forced (the first
+// `sinks`, the last `recent`) or rank best; emit(slot, i) for each.
+template <typename Key, typename Emit>
+__device__ void take_best(Key key, int n, int take, int sinks, int recent, int* hist, int* red, Emit emit) {
+  if (n <= take) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) emit(i, i);
+    return;
+  }
+  const int lo = sinks, hi = n - recent, want = take - sinks - recent;
+  uint32_t least = 0xffffffffu;
+  int equal = 0;
+  if (want > 0) least = block_select(key, lo, hi, want, hist, red, &equal);
+  int above = 0, same = 0;  // taken outright, and equal to the threshold, so far
+  for (int i0 = 0; i0 < n; i0 += blockDim.x) {
+    const int i = i0 + threadIdx.x;
+    bool sure = false, tie = false;
+    if (i < n) {
+      if (i < lo || i >= hi) {
+        sure = true;
+      } else if (want > 0) {
+        const uint32_t k = key(i);
+        sure = k > least;
+        tie = k == least;
+      }
+    }
+    int total;
+    const int before = block_scan((int)sure | ((int)tie << 16), red, &total);
+    const int ties = same + (before >> 16);
+    if (sure || (tie && ties < equal)) emit(above + (before & 0xffff) + min(ties, equal), i);
+    above += total & 0xffff;
+    same += total >> 16;
+  }
+}
+
+constexpr int kTakeThreads = 512;
+
+__global__ void __launch_bounds__(kTakeThreads)
+    kv_choose_kernel(KvView kv, const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
+                     const float* __restrict__ scores, int budget, int sinks, int recent, int32_t* __restrict__ pages,
+                     int32_t* __restrict__ counts, int* status) {
+  __shared__ int hist[256], red[kTakeThreads / 32];
+  chain_wait();
+  const int row = blockIdx.x / kv.kv_heads;
+  const int seq = seqs ? seqs[row] : row, len = lens[row];
+  const bool bad_seq = seq < 0 || seq >= kv.seqs, bad_len = len < 0 || len > kv.capacity();
+  if ((bad_seq || bad_len) && threadIdx.x == 0) kv_report(status, bad_seq ? ER_KV_BAD_SEQ : ER_KV_BAD_LENGTH);
+  const int n = bad_seq || bad_len ? 0 : (len + kv.page_size - 1) / kv.page_size;
+  const int take = min(n, budget);
+  const float* s = scores + (long long)blockIdx.x * kv.width;
+  int32_t* out = pages + (long long)blockIdx.x * budget;
+  take_best([&](int i) { return rank_key(s[i]); }, n, budget, sinks, recent, hist, red,
+            [&](int slot, int i) { out[slot] = i; });
+  for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
+  if (threadIdx.x == 0) counts[blockIdx.x] = take;
+}
+
+struct MassView {
+  const float* mass;
+  float* to_mass;
+  long long seq_stride, head_stride, to_seq_stride, to_head_stride;
+  int len, to_len;
+};
+
+__global__ void __launch_bounds__(kTakeThreads)
+    kv_keep_kernel(KvView kv, MassView m, const int32_t* __restrict__ lens, int budget, int sinks, int recent,
+                   int32_t* __restrict__ kept, int32_t* __restrict__ lens_out, int* status) {
+  __shared__ int hist[256], red[kTakeThreads / 32];
+  chain_wait();
+  const int seq = blockIdx.x / kv.kv_heads, h = blockIdx.x % kv.kv_heads;
+  int n = lens[seq];
+  if (n < 0 || n > kv.capacity() || n > m.len) {
+    if (threadIdx.x == 0 && h == 0) kv_report(status, ER_KV_BAD_LENGTH);
+    n = 0;
+  }
+  const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
+  float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
+  int32_t* out = kept + (long long)blockIdx.x * budget;
+  take_best([&](int i) { return rank_key(w[i]); }, n, budget, sinks, recent, hist, red, [&](int slot, int i) {
+    out[slot] = i;
+    to[slot] = w[i];
+  });
+  const int take = min(n, budget);
+  for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
+  if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
+}
+
+// Rows of the kept positions, 16 bytes a lane, into the destination's pages.
+__global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, const int32_t* __restrict__ kept,
+                                                      int budget, int row_bytes, int* status) {
+  chain_wait();
+  const int seq = blockIdx.y, h = blockIdx.z;
+  const int cols = row_bytes / 16;
+  const int32_t* list = kept + ((long long)seq * from.kv_heads + h) * budget;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < (long long)budget * cols; i += gridDim.x * 256LL) {
+    const int slot = (int)(i / cols), c = (int)(i % cols);
+    const int src = list[slot];
+    if (src < 0) continue;
+    const int a = from.pages_of(seq)[src / from.page_size], b = to.pages_of(seq)[slot / to.page_size];
+    if (a < 0 || a >= from.num_pages || b < 0 || b >= to.num_pages) {
+      if (c == 0) kv_report(status, ER_KV_BAD_PAGE);
+      continue;
+    }
+    const long long so = a * from.page_stride + h * from.head_stride + (src % from.page_size) * from.slot_stride;
+    const long long de = b * to.page_stride + h * to.head_stride + (slot % to.page_size) * to.slot_stride;
+    const uint4 x = *reinterpret_cast<const uint4*>(from.k + so + c * 16);
+    const uint4 y = *reinterpret_cast<const uint4*>(from.v + so + c * 16);
+    *reinterpret_cast<uint4*>(to.k + de + c * 16) = x;
+    *reinterpret_cast<uint4*>(to.v + de + c * 16) = y;
+  }
+}
+
+}  // namespace er
+
+using namespace er;
+
+extern "C" size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows) {
+  if (!cache || rows <= 0 || cache->kv_heads <= 0 || cache->table_width <= 0) return 0;
+  return align_up((size_t)rows * cache->kv_heads * cache->table_width * sizeof(float), 256);
+}
+
+extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, long long q_stride, int rows,
+                            int heads, const int32_t* seqs, const int32_t* lens, const int8_t* codes,
+                            const float* scales, int budget, int sinks, int recent, int32_t* pages_out,
+                            int32_t* counts_out, int* status, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = kv_check("er_kv_select", cache)) return rc;
+  if (rows < 0 || heads <= 0 || heads % cache->kv_heads)
+    return fail(ER_EINVAL, "er_kv_select: rows %d, heads %d / %d", rows, heads, cache->kv_heads);
+  if (q_dtype != ER_DTYPE_F32 && q_dtype != ER_DTYPE_BF16) return fail(ER_EINVAL, "er_kv_select: q dtype %d", q_dtype);
+  if (budget <= 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)
+    return fail(ER_EINVAL, "er_kv_select: budget %d with %d first and %d last pages", budget, sinks, recent);
+  if (q_stride < (long long)heads * cache->head_dim)
+    return fail(ER_EINVAL, "er_kv_select: row stride %lld shorter than the queries", q_stride);
+  if (!seqs && rows > cache->seqs) return fail(ER_EINVAL, "er_kv_select: %d rows, %d sequences", rows, cache->seqs);
+  if (rows == 0) return ER_OK;
+  if (!q || !lens || !codes || !scales || !pages_out || !counts_out) return fail(ER_EINVAL, "er_kv_select: null pointer");
+  if (((uintptr_t)codes & 7)) return fail(ER_EINVAL, "er_kv_select: codes must be 8-byte aligned");
+  const int group = heads / cache->kv_heads;
+  const size_t smem = (size_t)group * (2 * cache->head_dim + 4);
+  if (smem > 48 * 1024) return fail(ER_EINVAL, "er_kv_select: %d queries a key head", group);
+  if ((long long)rows * cache->kv_heads > 65535)
+    return fail(ER_EINVAL, "er_kv_select: %d rows of %d key heads (at most 65535 in all)", rows, cache->kv_heads);
+  const size_t need = er_kv_select_workspace_bytes(cache, rows);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(ER_ENOSPACE, "er_kv_select: workspace %zu bytes, need %zu", workspace_bytes, need);
+  const KvView kv = kv_view(*cache);
+  cudaStream_t st = (cudaStream_t)stream;
+  const int units = rows * kv.kv_heads;
+  int wide = 1;
+  while (wide < kv.d / 8) wide *= 2;
+  const int per = kScoreThreads / wide;  // pages a CTA scores at a time
+  const long long most = (kv.width + per - 1) / per, want = 148 * 8 / units + 1;
+  const unsigned gx = (unsigned)(most < 1 ? 1 : most < want ? most : want);
+  int rc;
+  if (q_dtype == ER_DTYPE_BF16)
+    rc = launch_chained(kv_score_kernel<__nv_bfloat16>, dim3(gx, units), dim3(kScoreThreads), smem, st,
+                        "kv_score_kernel", kv, (const __nv_bfloat16*)q, q_stride, group, seqs, lens, codes, scales,
+                        (float*)workspace, status);
+  else
+    rc = launch_chained(kv_score_kernel<float>, dim3(gx, units), dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
+                        (const float*)q, q_stride, group, seqs, lens, codes, scales, (float*)workspace, status);
+  if (rc) return rc;
+  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), 0, st, "kv_choose_kernel", kv, seqs, lens,
+                        (const float*)workspace, budget, sinks, recent, pages_out, counts_out, status);
+}
+
+extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
+                           long long mass_seq_stride, long long mass_head_stride, int mass_len, float* to_mass,
+                           long long to_mass_seq_stride, long long to_mass_head_stride, int to_mass_len, int budget,
+                           int sinks, int recent, int32_t* kept_out, int32_t* lens_out, int* status, void* stream) {
+  if (int rc = kv_check("er_kv_evict", from)) return rc;
+  if (int rc = kv_check("er_kv_evict", to)) return rc;
+  if (from->dtype != to->dtype || from->kv_heads != to->kv_heads || from->head_dim != to->head_dim ||
+      from->seqs != to->seqs)
+    return fail(ER_EINVAL, "er_kv_evict: the two caches differ in type, key heads, head_dim or sequences");
+  if (budget <= 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)
+    return fail(ER_EINVAL, "er_kv_evict: budget %d with %d first and %d last positions", budget, sinks, recent);
+  if (mass_len < 0 || to_mass_len < budget || (long long)to->table_width * to->page_size < budget)
+    return fail(ER_EINVAL, "er_kv_evict: budget %d, but the destination holds %lld positions and %d weights", budget,
+                (long long)to->table_width * to->page_size, to_mass_len);
+  if (from->seqs == 0) return ER_OK;
+  if (!lens || !mass || !to_mass || !kept_out || !lens_out) return fail(ER_EINVAL, "er_kv_evict: null pointer");
+  if (lens == lens_out) return fail(ER_EINVAL, "er_kv_evict: lens_out is lens");
+  if (from->seqs > 65535 || from->kv_heads > 65535)
+    return fail(ER_EINVAL, "er_kv_evict: %d sequences, %d key heads", from->seqs, from->kv_heads);
+  const KvView a = kv_view(*from), b = kv_view(*to);
+  const MassView m{mass,        to_mass,  mass_seq_stride, mass_head_stride, to_mass_seq_stride, to_mass_head_stride,
+                   mass_len, to_mass_len};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (int rc = launch_chained(kv_keep_kernel, dim3(a.seqs * a.kv_heads), dim3(kTakeThreads), 0, st, "kv_keep_kernel", a,
+                              m, lens, budget, sinks, recent, kept_out, lens_out, status))
+    return rc;
+  const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4);
+  const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;
+  const long long most = ((long long)budget * (row_bytes / 16) + 255) / 256;
+  const dim3 grid((unsigned)(most < want ? most : want), a.seqs, a.kv_heads);
+  return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, (const int32_t*)kept_out,
+                        budget, row_bytes, status);
+}

@@ -30,6 +30,9 @@
  *                                                         decoder-layer norm, RoPE + KV cache, embedding
  *   er_store_*         store/unbuffered_io.py:135-149,    one aligned read per expert record
  *                      store/expert_reader.py:92-101      (ExpertStoreReader.read_into)
+ * er_kv_* (the paged key-value cache) have no counterpart in the reference,
+ * which keeps one sequence's keys and values in one array
+ * (runtime/qwen_moe.py:90-106, 250-291).
  */
 #ifndef EXPERTRELAY_B200_H
 #define EXPERTRELAY_B200_H
@@ -369,6 +372,119 @@ ER_API int er_rope_kv(const float* qkv, long long ld, float* q_out, int n, int h
  * runtime/weights.py:62-64); an id outside [0, vocab) sets *bad and a NaN row */
 ER_API int er_embed_int8(const int8_t* q, const float* scales, long long vocab, int hidden, const int64_t* ids, int n,
                          float* out, int* bad, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key-value cache of many sequences, one layer of it: pages of
+ * page_size positions for every key head, in any order in two pools, and per
+ * sequence a table of page ids. Position t of sequence s lies in page
+ * table[s * table_stride + t / page_size], slot t % page_size. k and v have
+ * the same strides (in elements; the head_dim values of a slot contiguous,
+ * every slot on a 16-byte boundary). No counterpart in the reference.
+ *
+ * Lengths, positions and tables live on the device and are checked there: a
+ * bad one (a page id outside [0, num_pages), a length or position outside the
+ * table, a sequence outside [0, seqs)) is never followed; it sets a bit of
+ * *status (int32 on the device, may be NULL) and spoils the rows that needed
+ * it (NaN attention rows, positions not written). Slots behind a sequence's
+ * length are never read as keys or values, whatever they hold.
+ */
+typedef struct er_kv_cache {
+  void* k;                     /* [num_pages, kv_heads, page_size, head_dim] by the strides below */
+  void* v;
+  int dtype;                   /* ER_DTYPE_F32 / ER_DTYPE_BF16 */
+  int num_pages, page_size, kv_heads;
+  int head_dim;                /* a multiple of 8, <= 256 */
+  long long page_stride, head_stride, slot_stride;
+  const int32_t* table;        /* device [seqs, table_width], row stride table_stride */
+  int seqs, table_width;
+  long long table_stride;
+} er_kv_cache;
+
+#define ER_KV_BAD_PAGE 1       /* status bits: a page id outside the pool */
+#define ER_KV_BAD_LENGTH 2     /* a length, position or count outside its table */
+#define ER_KV_BAD_SEQ 4        /* a sequence index outside [0, seqs) */
+
+/* RoPE and the write of new tokens' rows into the pages: row i of qkv
+ * [n, (heads + 2 kv_heads) head_dim] (q | k | v, dtype qkv_dtype, row stride
+ * ld) belongs to position positions[i] of sequence seqs[i] (seqs NULL: i).
+ * Its q heads are rotated into q_out [n, heads, head_dim] (q_dtype), its k
+ * heads rotated into the page, its v heads copied there. Angles are
+ * position * theta^(-2j/head_dim) in 64 bits, rotate-half. A (sequence,
+ * position) pair may occur once per call. */
+ER_API int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype, long long ld, const int32_t* seqs,
+                        const int32_t* positions, int n, int heads, double theta, void* q_out, int q_dtype,
+                        int* status, void* stream);
+
+/* Attention of rows of queries over the pages: row r has `heads` queries
+ * (heads / kv_heads of them per key head) that see the first lens[r]
+ * positions of sequence seqs[r] (seqs NULL: r; several rows may read one
+ * sequence, as the tokens of a prompt do):
+ *   out = softmax(scale q k^T) v, in fp32 sums; zeros where there is no key
+ *   or every score is -inf.
+ * With pages/counts, key head h of row r reads only the pages whose ordinals
+ * are pages[(r * kv_heads + h) * max_pages + i], i < counts[r * kv_heads + h]
+ * (distinct; positions behind lens[r] are left out).
+ * With mass, mass[r * mass_row_stride + h * mass_head_stride + j] grows by
+ * key head h's attention weight on position j, summed over its queries
+ * (not together with pages). */
+typedef struct er_kv_attend_io {
+  const void* q;               /* [rows, heads, head_dim], row stride q_stride elements */
+  int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */
+  long long q_stride;
+  void* out;                   /* [rows, heads, head_dim] contiguous */
+  int rows, heads;
+  const int32_t* seqs;         /* optional [rows] */
+  const int32_t* lens;         /* [rows] */
+  float scale;
+  const int32_t* pages;        /* optional [rows, kv_heads, max_pages] */
+  const int32_t* counts;       /* [rows, kv_heads], with pages */
+  int max_pages;
+  float* mass;                 /* optional, mass_len positions for each (row, key head) */
+  long long mass_row_stride, mass_head_stride;
+  int mass_len;
+  int* status;                 /* optional */
+} er_kv_attend_io;
+ER_API size_t er_kv_attend_workspace_bytes(const er_kv_cache* cache, const er_kv_attend_io* io);
+ER_API int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Bounds of the pages that hold positions [start[s], lens[s]) of each
+ * sequence, renewed from the whole page up to lens[s]: per page and key head,
+ * the least and the greatest key of every channel as int8 codes
+ * codes[(page * kv_heads + h) * 2 * head_dim + {0, head_dim} + c] =
+ * rint(x / scale) with scale[page * kv_heads + h] = max |x| * (1/127), the
+ * factor rounded to 32 bits (code 0 where that is no number; NaN keys are
+ * passed over). */
+ER_API int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, const int32_t* start, int8_t* codes,
+                             float* scales, int* status, void* stream);
+
+/* For each row and key head, up to `budget` pages: the first `sinks` and the
+ * last `recent` of its sequence, then those with the best score
+ *   max over the group's queries of (float(I) * t) * scale,
+ *   I = sum_c (c_c > 0 ? c_c * greatest_c : c_c * least_c), c_c = rint(q_c / t), t = max |q| * (1/127)
+ * (I exact, the products rounded in this order; ties to the lower page, NaN
+ * last). pages_out [rows, kv_heads, budget]: ordinals ascending, -1 behind
+ * them; counts_out [rows, kv_heads]. lens, seqs as for er_kv_attend. */
+ER_API size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows);
+ER_API int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, long long q_stride, int rows, int heads,
+                        const int32_t* seqs, const int32_t* lens, const int8_t* codes, const float* scales, int budget,
+                        int sinks, int recent, int32_t* pages_out, int32_t* counts_out, int* status, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Eviction by accumulated attention weight: each key head of each sequence
+ * keeps min(lens[s], budget) positions: the first `sinks`, the last `recent`,
+ * then those of the greatest mass[s * mass_seq_stride + h * mass_head_stride
+ * + j] (ties to the lower position, NaN last). They are copied, in order, to
+ * positions 0, 1, ... of sequence s in `to` (another cache of the same type,
+ * heads and head_dim, or other pages of the same pool: no page of `to` may be
+ * one that `from` reads), their mass to to_mass (same kind of strides).
+ * kept_out [seqs, kv_heads, budget]: the positions, -1 behind them;
+ * lens_out [seqs]. What lies behind the kept positions in `to` and to_mass
+ * stays as it was. A sequence with a bad length keeps nothing. */
+ER_API int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
+                       long long mass_seq_stride, long long mass_head_stride, int mass_len, float* to_mass,
+                       long long to_mass_seq_stride, long long to_mass_head_stride, int to_mass_len, int budget,
+                       int sinks, int recent, int32_t* kept_out, int32_t* lens_out, int* status, void* stream);
 
 /* ---- expert store reads (store/unbuffered_io.py, store/expert_reader.py) ----
  * experts.bin opened for reads that bypass the page cache (O_DIRECT; with

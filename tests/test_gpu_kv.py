@@ -1,0 +1,509 @@
+"""GPU: the paged key-value cache's operators against their definitions in
+64 bits (tests/kv_ref.py), at the lengths, pages, strides and masks where
+they can go wrong."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from kv_ref import attend_row, attend_tolerance, bounds_of, choose, half_step, make_cache, page_scores, tokens
+
+from expertrelay_b200 import kv
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _i32(x, device="cuda"):
+    return torch.tensor(x, dtype=torch.int32, device=device)
+
+
+def _case(seed, lens, kv_heads, group, d, ps, cache_dtype, q_dtype, layout="hnd", rows=None):
+    gen = torch.Generator().manual_seed(seed)
+    k, v, table = make_cache(gen, lens, kv_heads, d, ps, cache_dtype, layout=layout)
+    q = torch.randn((len(lens) if rows is None else rows, kv_heads * group, d), generator=gen).to(q_dtype).cuda()
+    return kv.PagedKV(k, v, table), q
+
+
+def _check_attend(cache, q, lens, out, *, seqs=None, scale=None, mass=None, mass0=None, picks=None):
+    d = cache.head_dim
+    scale = d ** -0.5 if scale is None else scale
+    table = cache.table.cpu()
+    for r, n in enumerate(lens):
+        s = r if seqs is None else seqs[r]
+        kk, vv = tokens(cache.k, table, s, n), tokens(cache.v, table, s, n)
+        want, weight, spread, size = attend_row(q[r].double().cpu().numpy(), kk, vv, scale,
+                                                None if picks is None else picks[r])
+        tol = attend_tolerance(want, spread, size, d, n, out.dtype)
+        got = out[r].double().cpu().numpy()
+        assert np.all(np.abs(got - want) <= tol), \
+            f"row {r} of {n}: off by {np.max(np.abs(got - want) / tol):.3g} of the tolerance"
+        if mass is not None:
+            grown = mass[r, :, :n].double().cpu().numpy() - mass0[r, :, :n].double().cpu().numpy()
+            eps = 2 * (d + 4) * 2.0 ** -23 * size + (2 * n + 16) * 2.0 ** -23
+            slack = eps * weight + half_step(F32) * np.abs(mass[r, :, :n].double().cpu().numpy()) + 1e-30
+            assert np.all(np.abs(grown - weight) <= slack), f"mass of row {r}"
+            assert torch.equal(mass[r, :, n:], mass0[r, :, n:])
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)])
+@pytest.mark.parametrize(("kv_heads", "group", "d", "ps"), [
+    (16, 1, 128, 16), (4, 8, 128, 64), (2, 3, 64, 24), (3, 2, 80, 7), (1, 16, 96, 1), (2, 5, 256, 32), (1, 4, 8, 5),
+    (2, 1, 192, 128), (1, 33, 64, 16),
+])
+def test_attend_matches_the_definition(cuda, cache_dtype, q_dtype, kv_heads, group, d, ps):
+    # empty, one, around a chunk of 16 keys, around a tile, a page's end inside a tile, odd and long
+    lens = [0, 1, 15, 16, 17, 63, 64, 65, 129, 333, 1501]
+    cache, q = _case(d + group, lens, kv_heads, group, d, ps, cache_dtype, q_dtype)
+    out = kv.attend(cache, q, _i32(lens))
+    assert out.dtype == q_dtype and tuple(out.shape) == tuple(q.shape)
+    assert torch.all(out[0] == 0)
+    _check_attend(cache, q, lens, out)
+    cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("length", [1, 2, 31, 640, 5000, 40001])
+def test_attend_one_row(cuda, dtype, length):
+    cache, q = _case(length, [length], 2, 4, 128, 16, dtype, dtype)
+    out = kv.attend(cache, q, _i32([length]))
+    _check_attend(cache, q, [length], out)
+    assert torch.equal(out, kv.attend(cache, q, _i32([length])))  # bit for bit again
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("layout", ["nhd", "wide"])
+def test_attend_strides(cuda, dtype, layout):
+    lens = [200, 0, 77, 1]
+    cache, q = _case(5, lens, 3, 2, 64, 16, dtype, dtype, layout=layout)
+    wide = torch.randn((4, 6 * 64 + 40)).to(dtype).cuda()
+    wide[:, 8:8 + 6 * 64] = q.reshape(4, -1)
+    qs = wide[:, 8:8 + 6 * 64].view(4, 6, 64)
+    assert not qs.is_contiguous()
+    _check_attend(cache, q, lens, kv.attend(cache, qs, _i32(lens)))
+    # a table whose rows lie apart, a scale of one's own, an output given
+    table = torch.full((4, cache.width + 3), -7, dtype=torch.int32, device="cuda")
+    table[:, :cache.width] = cache.table
+    other = kv.PagedKV(cache.k, cache.v, table[:, :cache.width])
+    out = torch.empty_like(q)
+    assert kv.attend(other, qs, _i32(lens), scale=0.3, out=out) is out
+    _check_attend(cache, q, lens, out, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attend_rows_of_one_sequence(cuda, dtype):
+    """A prompt's tokens as rows that share their sequence, in any order."""
+    lens = [150, 90]
+    seqs = [0] * 150 + [1, 0, 1]
+    rows = list(range(1, 151)) + [90, 3, 41]
+    cache, q = _case(6, lens, 2, 2, 64, 16, dtype, dtype, rows=len(rows))
+    out = kv.attend(cache, q, _i32(rows), seqs=_i32(seqs))
+    _check_attend(cache, q, rows, out, seqs=seqs)
+
+
+def test_attend_more_rows_than_a_launch_takes(cuda):
+    """More than 4096 rows go in several launches."""
+    lens = [33, 70]
+    cache, _ = _case(7, lens, 1, 2, 32, 16, F32, F32)
+    rows = 4100
+    q = torch.randn((rows, 2, 32), device="cuda")
+    seqs = torch.arange(rows, device="cuda", dtype=torch.int32) % 2
+    ns = (torch.arange(rows, device="cuda", dtype=torch.int32) * 7) % 34
+    mass = torch.zeros((rows, 1, 40), device="cuda")
+    out = kv.attend(cache, q, ns, seqs=seqs, mass=mass)
+    at = [0, 1, 2, 4094, 4095, 4096, 4097, 4099]
+    _check_attend(cache, q[at], ns[at].tolist(), out[at], seqs=seqs[at].tolist(), mass=mass[at],
+                  mass0=torch.zeros_like(mass[at]))
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), [(F32, F32), (BF16, BF16)])
+@pytest.mark.parametrize("group", [1, 3, 8, 12])
+def test_attend_accumulates_mass(cuda, cache_dtype, q_dtype, group):
+    lens = [300, 0, 1, 64, 2049]
+    cache, q = _case(group, lens, 2, group, 64, 16, cache_dtype, q_dtype)
+    mass = torch.rand((5, 2, 2100), device="cuda")[:, :, :2060]  # rows apart
+    mass0 = mass.clone()
+    out = kv.attend(cache, q, _i32(lens), mass=mass)
+    _check_attend(cache, q, lens, out, mass=mass, mass0=mass0)
+    assert torch.equal(out, kv.attend(cache, q, _i32(lens)))  # the same with and without
+
+
+def test_attend_infinite_scores(cuda):
+    """-inf scores weigh nothing, a row of them alone is a row without keys; +inf and NaN come out as NaN."""
+    for dtype in (F32, BF16):
+        cache, q = _case(8, [40, 40, 40, 40], 1, 1, 64, 16, dtype, dtype)
+        big = torch.finfo(dtype).max
+        q[:] = 1.0
+        for r, at in ((0, list(range(40))), (1, list(range(20))), (2, [30]), (3, [5])):
+            for t in at:
+                cache.k[int(cache.table[r, t // 16]), 0, t % 16] = {0: -big, 1: -big, 2: big, 3: float("nan")}[r]
+        out = kv.attend(cache, q, _i32([40] * 4)).float()
+        assert torch.all(out[0] == 0)
+        v = torch.from_numpy(tokens(cache.v, cache.table, 1, 40))
+        k = torch.from_numpy(tokens(cache.k, cache.table, 1, 40))
+        p = torch.softmax(k[0, 20:].sum(-1) / 8, 0)
+        want = p @ v[0, 20:]
+        spread = (p @ v[0, 20:].abs()).numpy()
+        tol = attend_tolerance(want.numpy(), spread, float(k[0, 20:].abs().sum(-1).max() / 8), 64, 40, dtype)
+        assert np.all(np.abs(out[1, 0].double().cpu().numpy() - want.numpy()) <= tol)
+        assert torch.isnan(out[2]).all() and torch.isnan(out[3]).all()
+
+
+def test_attend_bad_pages_and_lengths_spoil_their_rows_alone(cuda):
+    for dtype in (F32, BF16):
+        lens = [200, 200, 200, 200, 200, 200]
+        cache, q = _case(9, lens, 2, 2, 64, 16, dtype, dtype)
+        table = cache.table.clone()
+        table[1, 5] = cache.num_pages
+        table[2, 0] = -1
+        cache = kv.PagedKV(cache.k, cache.v, table)
+        given = [200, 200, 200, -3, cache.width * 16 + 1, 190]
+        out = kv.attend(cache, q, _i32(given))
+        for r in (1, 2, 3, 4):
+            assert torch.isnan(out[r]).all(), r
+        for r in (0, 5):
+            _check_attend(cache, q[r:r + 1], [given[r]], out[r:r + 1], seqs=[r])
+        with pytest.raises(ValueError, match="page id outside the pool, a length"):
+            cache.check()
+        cache.check()
+        out = kv.attend(cache, q, _i32([200] * 6), seqs=_i32([0, 6, -1, 0, 0, 0]))
+        assert torch.isnan(out[1:3]).all() and not torch.isnan(out[[0, 3, 4, 5]]).any()
+        with pytest.raises(ValueError, match="sequence outside the table"):
+            cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attend_over_page_lists(cuda, dtype):
+    lens = [500, 31, 0, 64]
+    cache, q = _case(10, lens, 2, 3, 64, 16, dtype, dtype)
+    lists = {(0, 0): [0, 4, 31], (0, 1): [31], (1, 0): [0, 1], (1, 1): [], (2, 0): [], (2, 1): [], (3, 0): [3, 1], (3, 1): [2]}
+    pages, counts = torch.full((4, 2, 5), -1, dtype=torch.int32), torch.zeros((4, 2), dtype=torch.int32)
+    picks = [[None, None] for _ in lens]
+    for (r, h), ids in lists.items():
+        pages[r, h, :len(ids)] = torch.tensor(ids, dtype=torch.int32)
+        counts[r, h] = len(ids)
+        picks[r][h] = [t for p in ids for t in range(p * 16, min(lens[r], p * 16 + 16))]
+    out = kv.attend(cache, q, _i32(lens), pages=pages.cuda(), counts=counts.cuda())
+    _check_attend(cache, q, lens, out, picks=picks)
+    cache.check()
+    # an ordinal outside the table, a count outside the list: those key heads alone are spoilt
+    pages[0, 0, 1], counts[3, 1] = cache.width, 6
+    out = kv.attend(cache, q, _i32(lens), pages=pages.cuda(), counts=counts.cuda())
+    assert torch.isnan(out[0, :3]).all() and torch.isnan(out[3, 3:]).all()
+    _check_attend(cache, q[1:3], lens[1:3], out[1:3], seqs=[1, 2], picks=picks[1:3])
+    assert not torch.isnan(out[0, 3:]).any() and not torch.isnan(out[3, :3]).any()
+
+
+def test_attend_offsets_past_32_bits(cuda):
+    """A pool whose later pages lie more than 2^32 bytes in."""
+    pages, ps, d = 70000, 128, 128  # 2.3 GB a pool of one key head in bf16: byte offsets past 2^31
+    k = torch.empty((pages, 2, ps, d), dtype=BF16, device="cuda")
+    v = torch.empty_like(k)
+    assert k.numel() * 2 > 2 ** 32
+    ids = [pages - 1, 0, pages - 2, 65536]
+    gen = torch.Generator().manual_seed(1)
+    for p in ids:
+        k[p] = torch.randn((2, ps, d), generator=gen).to(BF16).cuda()
+        v[p] = torch.randn((2, ps, d), generator=gen).to(BF16).cuda()
+    cache = kv.PagedKV(k, v, _i32([ids]))
+    q = torch.randn((1, 4, d), generator=gen).to(BF16).cuda()
+    _check_attend(cache, q, [500], kv.attend(cache, q, _i32([500])))
+
+
+@pytest.mark.parametrize("cache_dtype", [F32, BF16])
+@pytest.mark.parametrize(("q_dtype", "heads", "kv_heads", "d", "ps"), [
+    (F32, 16, 16, 128, 16), (BF16, 8, 2, 64, 24), (F32, 3, 1, 80, 1), (BF16, 2, 2, 256, 64), (F32, 1, 1, 8, 3),
+])
+def test_append(cuda, cache_dtype, q_dtype, heads, kv_heads, d, ps):
+    gen = torch.Generator().manual_seed(d)
+    lens = [100, 9, 40]
+    k, v, table = make_cache(gen, lens, kv_heads, d, ps, cache_dtype)
+    cache = kv.PagedKV(k, v, table)
+    seqs = [0, 1, 0, 2, 0]
+    pos = [99, 0, 50, 39, 51]
+    theta = 10000.0
+    wide = torch.randn((5, (heads + 2 * kv_heads) * d + 24), generator=gen).to(q_dtype).cuda()
+    qkv = wide[:, : (heads + 2 * kv_heads) * d]
+    k0, v0 = k.clone(), v.clone()
+    q = kv.append(cache, qkv, _i32(pos), heads, theta, seqs=_i32(seqs))
+    assert q.dtype == q_dtype
+    x = qkv.double().cpu().numpy().reshape(5, heads + 2 * kv_heads, d)
+    ang = np.array(pos)[:, None] * theta ** (-2.0 * np.arange(d // 2) / d)
+    c, s = np.cos(ang)[:, None], np.sin(ang)[:, None]
+    a, b = x[..., :d // 2], x[..., d // 2:]
+    turned = np.concatenate([a * c - b * s, b * c + a * s], -1)
+    size = np.concatenate([np.abs(a * c) + np.abs(b * s), np.abs(b * c) + np.abs(a * s)], -1)
+    # cos, sin, product and sum are rounded to 32 bits, then the result to its type
+    def near(got, want, by, dtype):
+        assert np.all(np.abs(got - want) <= 3.01 * 2.0 ** -24 * by + half_step(dtype) * (np.abs(want) + 3.01 * 2.0 ** -24 * by) * (dtype != F32))
+    near(q.double().cpu().numpy(), turned[:, :heads], size[:, :heads], q_dtype)
+    for i in range(5):
+        page, slot = int(table[seqs[i], pos[i] // ps]), pos[i] % ps
+        near(k[page, :, slot].double().cpu().numpy(), turned[i, heads:heads + kv_heads], size[i, heads:heads + kv_heads],
+             cache_dtype)
+        assert torch.equal(v[page, :, slot], qkv[i].reshape(-1, d)[heads + kv_heads:].to(cache_dtype))
+        k0[page, :, slot], v0[page, :, slot] = k[page, :, slot], v[page, :, slot]
+    assert torch.equal(k.nan_to_num(7), k0.nan_to_num(7)) and torch.equal(v.nan_to_num(7), v0.nan_to_num(7))
+    cache.check()
+
+
+def test_append_far_positions_and_other_q_type(cuda):
+    """Angles of far positions, where a 32-bit product would lose them."""
+    k = torch.zeros((1, 1, 1, 64), dtype=F32, device="cuda")
+    cache = kv.PagedKV(k, k.clone(), torch.zeros((1, 2_000_000), dtype=torch.int32, device="cuda"))
+    x = torch.randn((1, 3 * 64), device="cuda")
+    q = kv.append(cache, x, _i32([1_999_999]), 1, 1e6, q_dtype=BF16)
+    ang = 1_999_999 * 1e6 ** (-2.0 * np.arange(32) / 64)
+    a, b = x[0, 64:96].double().cpu().numpy(), x[0, 96:128].double().cpu().numpy()
+    want = np.concatenate([a * np.cos(ang) - b * np.sin(ang), b * np.cos(ang) + a * np.sin(ang)])
+    size = np.abs(np.concatenate([a, b])) + np.abs(np.concatenate([b, a]))
+    assert np.all(np.abs(k[0, 0, 0].double().cpu().numpy() - want) <= 3.01 * 2.0 ** -24 * size)
+    assert q.dtype == BF16
+
+
+def test_append_leaves_bad_rows_unwritten(cuda):
+    gen = torch.Generator().manual_seed(3)
+    k, v, table = make_cache(gen, [32, 32], 1, 64, 16, F32)
+    table[1, 1] = 99
+    cache = kv.PagedKV(k, v, table)
+    k0 = k.clone()
+    kv.append(cache, torch.randn((5, 3 * 64), device="cuda"), _i32([32, -1, 16, 0, 0]), 1, 1e4, seqs=_i32([0, 0, 1, 2, -1]))
+    assert torch.equal(k.nan_to_num(7), k0.nan_to_num(7))
+    with pytest.raises(ValueError, match="page id outside the pool, a length.*, a sequence"):
+        cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize(("d", "ps"), [(128, 16), (64, 24), (80, 5), (256, 64), (8, 1)])
+def test_page_bounds(cuda, dtype, d, ps):
+    gen = torch.Generator().manual_seed(d)
+    lens, start = [100, 0, 33, 7], [0, 0, 32, 7]
+    k, v, table = make_cache(gen, lens, 2, d, ps, dtype)
+    k[int(table[0, 0])] = 0  # a page of zeros: codes and scale 0
+    cache = kv.PagedKV(k, v, table)
+    bounds = kv.PageBounds.new(cache)
+    bounds.codes.fill_(11)
+    bounds.scales.fill_(-1)
+    kv.page_bounds(cache, bounds, _i32(lens), _i32(start))
+    cache.check()
+    touched = set()
+    for s, n in enumerate(lens):
+        if start[s] >= n:
+            continue
+        for o in range(start[s] // ps, -(-n // ps)):
+            page = int(table[s, o])
+            for h in range(2):
+                lo, hi, scale = bounds_of(k[page, h, : min(ps, n - o * ps)].float().cpu().numpy())
+                assert bounds.scales[page, h].item() == scale
+                assert np.array_equal(bounds.codes[page, h, 0].cpu().numpy(), lo)
+                assert np.array_equal(bounds.codes[page, h, 1].cpu().numpy(), hi)
+                touched.add(page)
+    rest = [p for p in range(cache.num_pages) if p not in touched]
+    assert torch.all(bounds.codes[rest] == 11) and torch.all(bounds.scales[rest] == -1)
+
+
+def _select_case(seed, lens, kv_heads, group, d, ps, dtype):
+    cache, q = _case(seed, lens, kv_heads, group, d, ps, dtype, dtype)
+    bounds = kv.PageBounds.new(cache)
+    kv.page_bounds(cache, bounds, _i32(lens), _i32([0] * len(lens)))
+    return cache, q, bounds
+
+
+def _want_pages(cache, bounds, q, lens, budget, sinks, recent):
+    want = []
+    table, group = cache.table.cpu(), q.shape[1] // cache.kv_heads
+    codes, scales = bounds.codes.cpu().numpy(), bounds.scales.cpu().numpy()
+    for r, n in enumerate(lens):
+        ids = table[r, : -(-n // cache.page_size)].numpy()
+        row = []
+        for h in range(cache.kv_heads):
+            sc = page_scores(q[r, h * group:(h + 1) * group].float().cpu().numpy(), codes[ids, h, 0], codes[ids, h, 1],
+                             scales[ids, h]) if len(ids) else np.zeros(0)
+            row.append(choose(sc, len(ids), budget, sinks, recent))
+        want.append(row)
+    return want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize(("group", "d", "ps", "budget", "sinks", "recent"), [
+    (1, 128, 16, 8, 1, 2), (8, 64, 4, 64, 0, 0), (3, 80, 1, 33, 2, 3), (2, 256, 16, 1, 0, 1), (5, 8, 2, 5, 2, 3),
+])
+def test_select_pages(cuda, dtype, group, d, ps, budget, sinks, recent):
+    lens = [1500, 0, 1, 16 * 8, 700, 333]
+    cache, q, bounds = _select_case(group, lens, 2, group, d, ps, dtype)
+    pages, counts = kv.select_pages(cache, bounds, q, _i32(lens), budget, sinks=sinks, recent=recent)
+    cache.check()
+    for r, row in enumerate(_want_pages(cache, bounds, q, lens, budget, sinks, recent)):
+        for h, ids in enumerate(row):
+            assert counts[r, h].item() == len(ids)
+            assert pages[r, h].tolist() == ids + [-1] * (budget - len(ids)), (r, h)
+    out = kv.attend(cache, q, _i32(lens), pages=pages, counts=counts)
+    picks = [[[t for p in ids for t in range(p * ps, min(n, (p + 1) * ps))] for ids in row]
+             for n, row in zip(lens, _want_pages(cache, bounds, q, lens, budget, sinks, recent))]
+    _check_attend(cache, q, lens, out, picks=picks)
+
+
+def test_select_ties_zeros_and_bad_rows(cuda):
+    lens = [640, 640, 640, 640]
+    cache, q, bounds = _select_case(4, lens, 1, 2, 64, 16, F32)
+    bounds.codes[:] = 5  # every page alike: the lowest win
+    bounds.scales[:] = 1.0
+    q[1] = 0
+    q[2, 1, 3] = float("nan")  # no page ranks
+    given = [640, 640, 640, cache.width * 16 + 1]
+    pages, counts = kv.select_pages(cache, bounds, q, _i32(given), 6, sinks=1, recent=1)
+    for r in range(3):
+        assert pages[r, 0].tolist() == [0, 1, 2, 3, 4, 39]
+    assert counts[3, 0].item() == 0 and pages[3, 0].tolist() == [-1] * 6
+    with pytest.raises(ValueError, match="length"):
+        cache.check()
+    # a bad page id is never followed, and ranks last
+    table = cache.table.clone()
+    table[0, 1] = -5
+    cache = kv.PagedKV(cache.k, cache.v, table)
+    pages, _ = kv.select_pages(cache, bounds, q, _i32([640] * 4), 6, sinks=1, recent=1)
+    assert pages[0, 0].tolist() == [0, 2, 3, 4, 5, 39]
+    with pytest.raises(ValueError, match="page id"):
+        cache.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize(("d", "ps", "to_ps", "budget", "sinks", "recent"), [
+    (128, 16, 16, 100, 4, 20), (64, 24, 16, 1, 0, 0), (80, 5, 7, 300, 0, 300), (256, 64, 32, 513, 4, 0), (8, 1, 3, 64, 64, 0),
+])
+def test_evict(cuda, dtype, d, ps, to_ps, budget, sinks, recent):
+    gen = torch.Generator().manual_seed(d)
+    lens = [1200, 0, 1, budget, budget + 1, 777]
+    k, v, table = make_cache(gen, lens, 2, d, ps, dtype)
+    cache = kv.PagedKV(k, v, table)
+    width = -(-budget // to_ps)
+    tk, tv = (torch.full((6 * width, 2, to_ps, d), 9.0, dtype=dtype, device="cuda") for _ in range(2))
+    to = kv.PagedKV(tk, tv, torch.randperm(6 * width, generator=gen).to(torch.int32).reshape(6, width).cuda())
+    mass = torch.rand((6, 2, 1250), generator=gen)
+    mass = torch.where(mass < 0.4, torch.zeros(()), mass ** 3)  # many exact ties
+    mass[0, 0, 100:110] = float("nan")
+    mass[0, 1, 100:110] = float("inf")
+    mass[5, 0, 50] = -0.0
+    mass = mass.cuda()
+    to_mass = torch.full((6, 2, width * to_ps), -3.0, device="cuda")
+    kept, new = kv.evict(cache, _i32(lens), mass, to, to_mass, budget, sinks=sinks, recent=recent)
+    cache.check()
+    assert new.tolist() == [min(n, budget) for n in lens]
+    host = mass.cpu().numpy()
+    for s, n in enumerate(lens):
+        kk, vv = tokens(k, table, s, n), tokens(v, table, s, n)
+        m = min(n, budget)
+        for h in range(2):
+            ids = choose(host[s, h], n, budget, sinks, recent)
+            assert kept[s, h].tolist() == ids + [-1] * (budget - m), (s, h)
+            got_k = np.concatenate([tk[int(p), h].double().cpu().numpy() for p in to.table[s]])
+            got_v = np.concatenate([tv[int(p), h].double().cpu().numpy() for p in to.table[s]])
+            assert np.array_equal(got_k[:m], kk[h][ids]) and np.array_equal(got_v[:m], vv[h][ids])
+            assert np.all(got_k[m:] == 9) and np.all(got_v[m:] == 9)  # behind them as it was
+            assert np.array_equal(to_mass[s, h, :m].cpu().numpy(), host[s, h][ids], equal_nan=True)
+            assert torch.all(to_mass[s, h, m:] == -3)
+
+
+def test_evict_bad_lengths_and_pages(cuda):
+    gen = torch.Generator().manual_seed(2)
+    lens = [64, 64, 64]
+    k, v, table = make_cache(gen, lens, 1, 64, 16, F32)
+    table[2, 3] = 1000
+    cache = kv.PagedKV(k, v, table)
+    tk = torch.zeros((6, 1, 16, 64), device="cuda")
+    to = kv.PagedKV(tk, tk.clone(), torch.arange(6, dtype=torch.int32, device="cuda").reshape(3, 2))
+    mass, to_mass = torch.rand((3, 1, 64), device="cuda"), torch.zeros((3, 1, 32), device="cuda")
+    kept, new = kv.evict(cache, _i32([64, 65, 64]), mass, to, to_mass, 32, sinks=0, recent=32)
+    assert new.tolist() == [32, 0, 32] and kept[1, 0].tolist() == [-1] * 32
+    assert kept[2, 0].tolist() == list(range(32, 64))
+    assert torch.equal(tk[5], torch.zeros_like(tk[5])) and not torch.equal(tk[4], torch.zeros_like(tk[4]))
+    with pytest.raises(ValueError, match="page id outside the pool, a length"):
+        cache.check()
+
+
+def test_refusals(cuda):
+    cache, q = _case(1, [64, 64], 2, 2, 64, 16, F32, F32)
+    lens = _i32([64, 64])
+    bad = [
+        (lambda: kv.PagedKV(cache.k.double(), cache.v.double(), cache.table), "float32 or bfloat16"),
+        (lambda: kv.PagedKV(cache.k.cpu(), cache.v.cpu(), cache.table.cpu()), "CUDA tensor"),
+        (lambda: kv.PagedKV(cache.k, cache.v.to(BF16), cache.table), "v: expected"),
+        (lambda: kv.PagedKV(cache.k, cache.v.transpose(1, 2).contiguous().transpose(1, 2), cache.table), "strides"),
+        (lambda: kv.PagedKV(cache.k, cache.v, cache.table.long()), "table"),
+        (lambda: kv.PagedKV(cache.k, cache.v, cache.table.t()), "contiguous rows"),
+        (lambda: kv.attend(cache, q[:, :3], lens), "3 heads over 2"),
+        (lambda: kv.attend(cache, q.half(), lens), "q: expected"),
+        (lambda: kv.attend(cache, q[..., :32], lens), "q: expected"),
+        (lambda: kv.attend(cache, q.transpose(0, 1).contiguous().transpose(0, 1), lens), "strides"),
+        (lambda: kv.attend(cache, q, lens.long()), "lens"),
+        (lambda: kv.attend(cache, q, lens[:1]), "lens"),
+        (lambda: kv.attend(cache, torch.cat([q, q]), _i32([1] * 4)), "4 rows over 2 sequences"),
+        (lambda: kv.attend(cache, q, lens, out=q[:1]), "out"),
+        (lambda: kv.attend(cache, q, lens, pages=_i32([[[0], [0]]] * 2)), "together"),
+        (lambda: kv.attend(cache, q, lens, mass=torch.zeros((2, 1, 64), device="cuda")), "mass"),
+        (lambda: kv.attend(cache, q, lens, pages=_i32([[[0], [0]]] * 2), counts=_i32([[1, 1]] * 2),
+                           mass=torch.zeros((2, 2, 64), device="cuda")), "not accumulated"),
+        (lambda: kv.attend(cache, q, lens, workspace=torch.empty(16, dtype=torch.uint8, device="cuda")), "workspace"),
+        (lambda: kv.append(cache, torch.zeros((2, 64), device="cuda"), lens, 4, 1e4), "qkv"),
+        (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens, 4, 0.0), "theta"),
+        (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens, 4, 1e4, q_dtype=torch.half), "q_dtype"),
+        (lambda: kv.select_pages(cache, kv.PageBounds.new(cache), q, lens, 2, sinks=2, recent=1), "budget"),
+        (lambda: kv.select_pages(cache, kv.PageBounds(torch.zeros((1, 2, 2, 64), dtype=torch.int8, device="cuda"),
+                                                      torch.zeros((1, 2), device="cuda")), q, lens, 2), "not this cache's"),
+        (lambda: kv.evict(cache, lens, torch.zeros((2, 2, 64), device="cuda"), cache,
+                          torch.zeros((2, 2, 64), device="cuda"), 8, recent=2), "own pages"),
+    ]
+    for call, words in bad:
+        with pytest.raises(ValueError, match=words):
+            call()
+    mass = torch.zeros((2, 2, 64), device="cuda")
+    to = kv.PagedKV(torch.zeros_like(cache.k), torch.zeros_like(cache.v), cache.table.clone())
+    with pytest.raises(ValueError, match="to_mass"):
+        kv.evict(cache, lens, mass, to, mass, 8, recent=2)
+    with pytest.raises(ValueError, match="destination holds"):
+        kv.evict(cache, lens, mass, to, torch.zeros((2, 2, 65), device="cuda"), 65, recent=2)
+    unaligned = torch.zeros(cache.k.numel() + 2, device="cuda")[2:].view(cache.k.shape)
+    with pytest.raises(ValueError, match="16-byte"):
+        kv.attend(kv.PagedKV(unaligned, unaligned, cache.table), q, lens)
+
+
+def test_empty_calls(cuda):
+    cache, q = _case(1, [64, 64], 2, 2, 64, 16, F32, F32)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert kv.attend(cache, q[:0], none).shape == (0, 4, 64)
+    assert kv.append(cache, torch.zeros((0, 512), device="cuda"), none, 4, 1e4).shape == (0, 4, 64)
+    pages, counts = kv.select_pages(cache, kv.PageBounds.new(cache), q[:0], none, 4)
+    assert pages.shape == (0, 2, 4) and counts.shape == (0, 2)
+    out = kv.attend(cache, q, _i32([0, 0]))
+    assert torch.all(out == 0)
+
+
+def test_streams_and_graph_replay(cuda):
+    """Captured once, replayed with other lengths, tables and queries; two graphs that share nothing; another stream."""
+    lens = [300, 45]
+    cache, q = _case(12, lens, 2, 4, 128, 16, BF16, BF16)
+    ns = _i32(lens)
+    kv.attend(cache, q, ns)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kv.attend(cache, q, ns))
+        graphs.append(g)
+    for new in ([300, 45], [17, 0], [1, 33]):
+        ns.copy_(_i32(new))
+        q.copy_(torch.randn(q.shape).to(BF16))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            _check_attend(cache, q, new, out)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = kv.attend(cache, q, ns)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, outs[0])

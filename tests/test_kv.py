@@ -1,0 +1,99 @@
+"""The paged cache's C entry points without a GPU: every refusal comes before the device is touched."""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import pytest
+
+from expertrelay_b200 import _lib
+
+P = 0x1000  # an address that is never followed
+
+
+def _cache(**kw):
+    base = dict(k=P, v=P, dtype=_lib.DTYPE_BF16, num_pages=8, page_size=16, kv_heads=2, head_dim=64,
+                page_stride=2 * 16 * 64, head_stride=16 * 64, slot_stride=64, table=P, seqs=3, table_width=4,
+                table_stride=4)
+    return _lib.KvCache(**{**base, **kw})
+
+
+def _io(**kw):
+    base = dict(q=P, q_dtype=_lib.DTYPE_BF16, q_stride=4 * 64, out=P, rows=3, heads=4, lens=P, scale=0.1)
+    return _lib.KvAttendIO(**{**base, **kw})
+
+
+def _fails(rc, words):
+    assert rc == _lib.ER_EINVAL
+    assert words in _lib.last_error(), _lib.last_error()
+
+
+@pytest.mark.parametrize(("change", "words"), [
+    ({"dtype": 2}, "dtype 2"), ({"num_pages": 0}, "0 pages"), ({"page_size": -1}, "-1 positions"),
+    ({"kv_heads": 0}, "0 key heads"), ({"head_dim": 60}, "head_dim 60"), ({"head_dim": 264}, "head_dim 264"),
+    ({"head_dim": 0}, "head_dim 0"), ({"k": None}, "null"), ({"table": None}, "null"), ({"k": P + 8}, "16-byte"),
+    ({"slot_stride": 68}, "16-byte"), ({"seqs": -1}, "-1 x 4"),
+])
+def test_cache_refusals(change, words):
+    L, c = _lib.lib(), _cache(**change)
+    _fails(L.er_kv_attend(C.byref(c), C.byref(_io()), None, 0, None), words)
+    _fails(L.er_kv_append(C.byref(c), P, 1, 8 * 64, None, P, 1, 4, 1e4, P, 1, None, None), words)
+    _fails(L.er_kv_page_bounds(C.byref(c), P, P, P, P, None, None), words)
+    _fails(L.er_kv_select(C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 0, 0, P, P, None, None, 0, None), words)
+    _fails(L.er_kv_evict(C.byref(c), C.byref(_cache()), P, P, 1, 1, 64, P, 1, 1, 64, 8, 0, 0, P, P, None, None), words)
+
+
+@pytest.mark.parametrize(("change", "words"), [
+    ({"rows": -1}, "rows -1"), ({"heads": 3}, "heads 3 / 2"), ({"heads": 0}, "heads 0"), ({"q_dtype": 7}, "q dtype 7"),
+    ({"q_stride": 255}, "row stride 255"), ({"pages": P}, "page lists"), ({"pages": P, "max_pages": 4}, "page lists"),
+    ({"pages": P, "counts": P, "max_pages": 4, "mass": P}, "page lists"), ({"mass": P, "mass_len": -1}, "mass_len"),
+    ({"rows": 4}, "4 rows, 3 sequences"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lens": None}, "null"),
+])
+def test_attend_refusals(change, words):
+    _fails(_lib.lib().er_kv_attend(C.byref(_cache()), C.byref(_io(**change)), None, 0, None), words)
+
+
+def test_append_refusals():
+    L, c = _lib.lib(), _cache()
+    args = [C.byref(c), P, 1, 8 * 64, None, P, 1, 4, 1e4, P, 1, None, None]
+    for at, value, words in [(1, None, "null"), (2, 5, "dtypes 5"), (3, 8 * 64 - 1, "row stride"), (5, None, "null"),
+                             (6, -1, "n -1"), (7, 0, "heads 0"), (8, 0.0, "theta 0"), (8, float("nan"), "theta"),
+                             (9, None, "null"), (10, 9, "9")]:
+        _fails(L.er_kv_append(*[value if i == at else x for i, x in enumerate(args)]), words)
+
+
+def test_select_refusals():
+    L, c = _lib.lib(), _cache()
+    args = [C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 1, 1, P, P, None, None, 0, None]
+    for at, value, words in [(1, None, "null"), (2, 3, "q dtype"), (3, 8, "row stride"), (4, -2, "rows -2"),
+                             (5, 5, "heads 5"), (7, None, "null"), (8, P + 4, "8-byte"), (10, 0, "budget 0"),
+                             (11, 4, "budget 4"), (12, -1, "budget 4"), (4, 4, "4 rows, 3 sequences")]:
+        _fails(L.er_kv_select(*[value if i == at else x for i, x in enumerate(args)]), words)
+    assert L.er_kv_select(*args) == _lib.ER_ENOSPACE and "workspace 0 bytes" in _lib.last_error()
+    assert L.er_kv_select_workspace_bytes(C.byref(c), 3) >= 3 * 2 * 4 * 4
+
+
+def test_evict_refusals():
+    L = _lib.lib()
+    def call(frm=None, to=None, **kw):
+        a = dict(lens=P, mass=P, mass_len=64, to_mass=P, to_mass_len=64, budget=8, sinks=1, recent=1, kept=P, out=P + 64)
+        a.update(kw)
+        return L.er_kv_evict(C.byref(frm or _cache()), C.byref(to or _cache()), a["lens"], a["mass"], 1, 1,
+                             a["mass_len"], a["to_mass"], 1, 1, a["to_mass_len"], a["budget"], a["sinks"], a["recent"],
+                             a["kept"], a["out"], None, None)
+    for other in ({"dtype": 0, "slot_stride": 64}, {"kv_heads": 1}, {"head_dim": 32}, {"seqs": 2}):
+        _fails(call(to=_cache(**other)), "differ")
+    _fails(call(budget=0), "budget 0")
+    _fails(call(sinks=8), "budget 8")
+    _fails(call(budget=65), "destination holds 64")
+    _fails(call(to_mass_len=7), "7 weights")
+    _fails(call(out=P), "lens_out is lens")
+    for name in ("lens", "mass", "to_mass", "kept", "out"):
+        _fails(call(**{name: None}), "null")
+
+
+def test_nothing_to_do_is_fine():
+    L = _lib.lib()
+    assert L.er_kv_attend(C.byref(_cache()), C.byref(_io(rows=0)), None, 0, None) == _lib.ER_OK
+    assert L.er_kv_append(C.byref(_cache()), P, 1, 512, None, P, 0, 4, 1e4, P, 1, None, None) == _lib.ER_OK
+    assert L.er_kv_page_bounds(C.byref(_cache(seqs=0)), P, P, P, P, None, None) == _lib.ER_OK
