@@ -7,20 +7,20 @@ namespace er {
 
 constexpr int kSimtStages = 3;
 
-struct SimtShape {
-  int warps, pitch, smem;
-};
-
-// Shared memory of the fp32 kernel: queries, the warps' pieces, probabilities
-// and key masks, then per warp a ring of kSimtStages chunks of keys and values.
-inline SimtShape simt_shape(int d, int es, int gb) {
-  SimtShape s;
-  s.pitch = d * es + ((d * es / 16) % 2 ? 0 : 16);  // an odd number of 16-byte columns: no bank conflicts across keys
-  for (s.warps = 4; s.warps >= 1; s.warps /= 2) {
-    s.smem = gb * d * 4 + s.warps * gb * (d + 2) * 4 + s.warps * gb * kKvChunk * 4 + 64 +
-             s.warps * kSimtStages * (2 * kKvChunk * s.pitch);
+// Shared memory of the fp32 kernel: queries, the warps' pieces, probabilities,
+// then per warp a ring of kSimtStages chunks of keys and values, their rows
+// an odd number of 16-byte columns apart (no bank conflicts across keys).
+inline int simt_pitch(int d) { return d * 4 + ((d / 4) % 2 ? 0 : 16); }
+inline KernelShape simt_shape(int d, int group) {
+  KernelShape s;
+  s.heads = group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
+  for (s.warps = 4; s.warps > 1; s.warps /= 2) {
+    s.smem = s.heads * d * 4 + s.warps * s.heads * (d + 2) * 4 + s.warps * s.heads * kKvChunk * 4 + 64 +
+             s.warps * kSimtStages * (2 * kKvChunk * simt_pitch(d));
     if (s.smem <= 220 * 1024) break;
   }
+  s.per_sm = 227 * 1024 / (s.smem + 3072);
+  if (s.per_sm > 4) s.per_sm = 4;
   return s;
 }
 
@@ -28,8 +28,9 @@ inline SimtShape simt_shape(int d, int es, int gb) {
 // asynchronous copies. Scores: lane l holds key l % 16 and half of the
 // columns. Values: the lanes split a row's 16-byte columns, lane groups the
 // keys. GB queries of the group at a time share each key that is read.
-template <typename TC, typename TQ, int GB>
+template <typename TQ, int GB>
 __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_constant__ AttendArgs a, int pitch) {
+  using TC = float;
   constexpr int V = 16 / sizeof(TC);
   extern __shared__ __align__(16) char sm[];
   __shared__ long long sums[129];
@@ -314,45 +315,40 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
 
 namespace {
 
-template <typename TC, typename TQ, int GB>
-int simt_go(const AttendArgs& a, cudaStream_t st) {
-  const SimtShape s = simt_shape(a.kv.d, sizeof(TC), GB);
-  auto kernel = kv_attend_simt_kernel<TC, TQ, GB>;
+template <typename TQ, int GB>
+int simt_go(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
+  auto kernel = kv_attend_simt_kernel<TQ, GB>;
   if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem),
                           "kv_attend smem attribute"))
     return rc;
-  return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a, s.pitch);
+  return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a,
+                        simt_pitch(a.kv.d));
 }
 
-template <typename TC, typename TQ>
-int simt_gb(const AttendArgs& a, int gb, cudaStream_t st) {
-  switch (gb) {
-    case 1: return simt_go<TC, TQ, 1>(a, st);
-    case 2: return simt_go<TC, TQ, 2>(a, st);
-    case 4: return simt_go<TC, TQ, 4>(a, st);
-    default: return simt_go<TC, TQ, 8>(a, st);
+template <typename TQ>
+int attend_simt(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
+  switch (s.heads) {
+    case 1: return simt_go<TQ, 1>(a, s, st);
+    case 2: return simt_go<TQ, 2>(a, s, st);
+    case 4: return simt_go<TQ, 4>(a, s, st);
+    default: return simt_go<TQ, 8>(a, s, st);
   }
 }
-
-// queries of a group that a CTA takes together
-inline int head_block(int group) { return group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8; }
 
 constexpr int kMaxEntries = 4096;  // scan entries a launch takes; more rows go in several launches
 
 struct Layout {
-  int gb, blocks, warps, grid, rows;  // rows: of one launch
+  KernelShape shape;
+  int blocks, grid, rows;  // rows: of one launch
   size_t prefix, ml, o, lse, scores, bytes;
 };
 
 Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   Layout L;
   const int group = io.heads / c.kv_heads;
-  L.gb = head_block(group);
-  L.blocks = (group + L.gb - 1) / L.gb;
-  const SimtShape s = simt_shape(c.head_dim, c.dtype == ER_DTYPE_BF16 ? 2 : 4, L.gb);
-  L.warps = s.warps;
-  const int per_sm = 227 * 1024 / (s.smem + 2048);
-  L.grid = sms * (per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm);
+  L.shape = c.dtype == ER_DTYPE_BF16 ? mma_shape(c.head_dim, group, io.q_dtype) : simt_shape(c.head_dim, group);
+  L.blocks = (group + L.shape.heads - 1) / L.shape.heads;
+  L.grid = sms * L.shape.per_sm;
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
   if (L.rows < 1) L.rows = 1;
   if (L.rows > io.rows) L.rows = io.rows;
@@ -364,8 +360,8 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
     return here;
   };
   L.prefix = take((entries + 1) * 8);
-  L.ml = take((size_t)L.grid * 2 * L.gb * 2 * 4);
-  L.o = take((size_t)L.grid * 2 * L.gb * c.head_dim * 4);
+  L.ml = take((size_t)L.grid * 2 * L.shape.heads * 2 * 4);
+  L.o = take((size_t)L.grid * 2 * L.shape.heads * c.head_dim * 4);
   L.lse = take(io.mass ? (size_t)L.rows * io.heads * 4 : 0);
   L.scores = take(io.mass ? (size_t)L.rows * io.heads * io.mass_len * 4 : 0);
   L.bytes = at;
@@ -443,7 +439,10 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
       a.pages = io->pages + (size_t)r0 * cache->kv_heads * io->max_pages;
       a.counts = io->counts + (size_t)r0 * cache->kv_heads;
     }
-    a.tile = L.warps * kKvChunk;
+    a.tile = L.shape.warps * kKvChunk;
+    a.shift = -1;
+    for (int b = 0; b < 31; ++b)
+      if (cache->page_size == 1 << b) a.shift = b;
     a.min_tiles = 2;
     a.status = io->status;
     a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;
@@ -464,13 +463,14 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     using bf = __nv_bfloat16;
     const bool cb = cache->dtype == ER_DTYPE_BF16, qb = io->q_dtype == ER_DTYPE_BF16;
     if (cb)
-      rc = qb ? simt_gb<bf, bf>(a, L.gb, st) : simt_gb<bf, float>(a, L.gb, st);
+      rc = attend_mma(a, io->q_dtype, st);
     else
-      rc = qb ? simt_gb<float, bf>(a, L.gb, st) : simt_gb<float, float>(a, L.gb, st);
+      rc = qb ? attend_simt<bf>(a, L.shape, st) : attend_simt<float>(a, L.shape, st);
     if (rc) return rc;
     const unsigned units = (unsigned)a.rows * cache->kv_heads * L.blocks;
-    rc = qb ? launch_chained(kv_join_kernel<bf>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, L.gb)
-            : launch_chained(kv_join_kernel<float>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, L.gb);
+    const int gb = L.shape.heads;
+    rc = qb ? launch_chained(kv_join_kernel<bf>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, gb)
+            : launch_chained(kv_join_kernel<float>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, gb);
     if (rc) return rc;
     if (io->mass && io->mass_len > 0) {
       const int pairs = a.rows * cache->kv_heads;

@@ -33,6 +33,7 @@ struct AttendArgs {
   const int32_t* counts;
   int max_pages;
   int tile;                    // keys a tile: warps a CTA * kKvChunk
+  int shift;                   // log2 of page_size, -1 when it is no power of two
   int min_tiles;               // fewest tiles worth a CTA
   int* status;
   // scan entries: rows, or (row, key head) pairs when each has its own page list
@@ -225,5 +226,14 @@ __device__ __forceinline__ __nv_bfloat16 kv_round<__nv_bfloat16>(float v) { retu
 // 2^(m_i - m) of a piece, 0 for a piece without keys or of -inf scores alone.
 __device__ __forceinline__ float piece_weight(float mi, float m) { return mi == -INFINITY ? 0.f : exp2f(mi - m); }
 
+
+// What a launch of an attention kernel takes: queries of a group together,
+// warps and shared memory of a CTA, CTAs an SM.
+struct KernelShape {
+  int heads, warps, smem, per_sm;
+};
+// the tensor-core kernel for bf16 caches (er_kv_attend_mma.cu)
+KernelShape mma_shape(int d, int group, int q_dtype);
+int attend_mma(const AttendArgs& a, int q_dtype, cudaStream_t st);
 
 }  // namespace er
