@@ -49,9 +49,8 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
 
   chain_wait();
   Place c;
-  long long left;
-  const long long begin = kv_run(a, sums, where, c, &left);
-  (void)begin;
+  const Run run = kv_run(a, sums, where, c);
+  long long left = run.left;
   if (left == 0) return;
 
   uint32_t live[kSimtStages];  // keys of a stage that exist, bad ones in the upper half
@@ -221,6 +220,8 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     if (bad && lane == 0) spoiled = 1;
     __syncthreads();
     const bool whole = first_t == 0 && t + 1 == tiles;
+    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind (the run's last tile is tile t)
+      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, run.begin + run.left - (t + 1), run.total};
     const bool nan = spoiled != 0;
     if (nan && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
     for (int i = threadIdx.x; i < GB * d; i += blockDim.x) {
@@ -255,47 +256,88 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   }
 }
 
-// One CTA per (row, key head, head block): rows without keys get zeros, bad
-// ones NaN, split ones the join of their pieces. The pieces of a unit are the
-// CTAs whose runs meet it, in order: the first piece of a CTA that began
-// before the unit's start is impossible, so a CTA's piece is its first one
-// when the unit began before the CTA's run, its last one otherwise.
+// Joins the units that several CTAs share: CTA (i, g) query g of the unit
+// that begins in CTA i's run and ends behind it. The pieces are that CTA's
+// last one and the first ones of the CTAs after it. A piece's weights are
+// found once, then threads split the pieces and the channels (four each).
+// The CTAs of g = 0 also write the rows without keys (zeros) and the bad
+// ones (NaN), which no attention CTA meets.
+constexpr int kJoinThreads = 256;
+
 template <typename TQ>
-__global__ void __launch_bounds__(128) kv_join_kernel(const __grid_constant__ AttendArgs a, int gb) {
+__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttendArgs a, int gb) {
+  extern __shared__ float wt[];  // [grid] weights, then [kJoinThreads][4] partial sums
+  __shared__ float red[2][kJoinThreads / 32];
   chain_wait();
-  const int per_row = a.kv.kv_heads * a.blocks;
-  const int row = blockIdx.x / per_row, rest = blockIdx.x % per_row, h = rest / a.blocks, blk = rest % a.blocks;
-  const int x = a.pages ? row * a.kv.kv_heads + h : row, u = a.pages ? blk : rest;
-  const int d = a.kv.d, g0 = blk * gb, live_g = min(gb, a.group - g0);
-  const long long total = a.prefix[a.entries] * a.units, c = a.prefix[x + 1] - a.prefix[x];
-  const long long at = (long long)row * a.heads + h * a.group + g0;
-  TQ* out = (TQ*)a.out + at * d;
-  if (c == 0) {
-    const float v = kv_entry(a, x).bad ? __int_as_float(0x7fc00000) : 0.f;
-    for (int i = threadIdx.x; i < live_g * d; i += blockDim.x) out[i] = kv_round<TQ>(v);
-    return;
-  }
-  const long long begin = a.prefix[x] * a.units + (long long)u * c;
-  const int shares = kv_shares(a, total);
-  const int i0 = kv_share_of(total, shares, begin), i1 = kv_share_of(total, shares, begin + c - 1);
-  if (i0 == i1) return;  // written whole
-  for (int i = threadIdx.x; i < live_g * d; i += blockDim.x) {
-    const int g = i / d, cc = i % d;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int k = i0; k <= i1; ++k) {
-      const long long slot = (long long)k * 2 + (kv_share_start(total, shares, k) > begin ? 0 : 1);
-      top = fmaxf(top, a.part_ml[(slot * gb + g) * 2]);
+  const int g = blockIdx.y, d = a.kv.d;
+  if (g == 0) {
+    for (int x = blockIdx.x; x < a.entries; x += a.grid) {
+      const Entry e = kv_entry(a, x);
+      if (e.n > 0) continue;
+      const TQ v = kv_round<TQ>(e.bad ? __int_as_float(0x7fc00000) : 0.f);
+      const int per = (a.pages ? a.group : a.heads) * d;  // an entry is a row, or a key head of one
+      TQ* out = (TQ*)a.out + (long long)x * per;
+      for (int i = threadIdx.x; i < per; i += kJoinThreads) out[i] = v;
     }
-    for (int k = i0; k <= i1; ++k) {
-      const long long slot = (long long)k * 2 + (kv_share_start(total, shares, k) > begin ? 0 : 1);
-      const float mi = a.part_ml[(slot * gb + g) * 2], li = a.part_ml[(slot * gb + g) * 2 + 1];
-      const float by = li != li ? 1.f : piece_weight(mi, top);  // a spoiled piece spoils the row
-      sum = fmaf(li, by, sum);
-      acc = fmaf(a.part_o[(slot * gb + g) * d + cc], by, acc);
-    }
-    out[i] = kv_round<TQ>(sum == 0.f ? 0.f : acc / sum);
-    if (a.scores && cc == 0) a.lse[at + g] = sum == 0.f ? INFINITY : top + log2f(sum);
   }
+  const CutUnit c = a.cut[blockIdx.x];
+  if (c.row < 0 || c.g0 + g >= a.group) return;
+  const int shares = kv_shares(a, c.total), i0 = blockIdx.x;
+  const int n = kv_share_of(c.total, shares, c.begin + c.tiles - 1) - i0 + 1;  // pieces
+  auto piece = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * gb + g; };
+  float top = -INFINITY, sum = 0.f;
+  for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, a.part_ml[piece(k) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (threadIdx.x % 32 == 0) red[0][threadIdx.x / 32] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[0][w]);
+  for (int k = threadIdx.x; k < n; k += kJoinThreads) {
+    const float li = a.part_ml[piece(k) * 2 + 1];
+    const float by = li != li ? 1.f : piece_weight(a.part_ml[piece(k) * 2], top);  // a spoiled piece spoils the row
+    wt[k] = by;
+    sum = fmaf(li, by, sum);
+  }
+  sum = warp_sum(sum);
+  if (threadIdx.x % 32 == 0) red[1][threadIdx.x / 32] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) sum += red[1][w];
+  const int cols = d / 4, groups = kJoinThreads / cols;  // 2 .. 64 columns of 4 channels
+  const int col = threadIdx.x % cols, grp = threadIdx.x / cols;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (grp < groups) {
+#pragma unroll 4
+    for (int k = grp; k < n; k += groups) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + piece(k) * d + col * 4);
+      const float by = wt[k];
+      acc.x = fmaf(x.x, by, acc.x);
+      acc.y = fmaf(x.y, by, acc.y);
+      acc.z = fmaf(x.z, by, acc.z);
+      acc.w = fmaf(x.w, by, acc.w);
+    }
+  }
+  float4* part = reinterpret_cast<float4*>(wt + (a.grid + 3) / 4 * 4);
+  part[threadIdx.x] = acc;
+  __syncthreads();
+  const long long at = (long long)c.row * a.heads + c.head * a.group + c.g0 + g;
+  if (threadIdx.x < cols) {
+    for (int q = 1; q < groups; ++q) {
+      const float4 x = part[q * cols + col];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+    }
+    TQ* out = (TQ*)a.out + at * d + col * 4;
+    out[0] = kv_round<TQ>(sum == 0.f ? 0.f : acc.x / sum);
+    out[1] = kv_round<TQ>(sum == 0.f ? 0.f : acc.y / sum);
+    out[2] = kv_round<TQ>(sum == 0.f ? 0.f : acc.z / sum);
+    out[3] = kv_round<TQ>(sum == 0.f ? 0.f : acc.w / sum);
+  }
+  if (a.scores && threadIdx.x == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
 // mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position.
@@ -340,7 +382,7 @@ constexpr int kMaxEntries = 4096;  // scan entries a launch takes; more rows go 
 struct Layout {
   KernelShape shape;
   int blocks, grid, rows;  // rows: of one launch
-  size_t prefix, ml, o, lse, scores, bytes;
+  size_t cut, ml, o, lse, scores, bytes;
 };
 
 Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
@@ -352,14 +394,13 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
   if (L.rows < 1) L.rows = 1;
   if (L.rows > io.rows) L.rows = io.rows;
-  const size_t entries = io.pages ? (size_t)L.rows * c.kv_heads : L.rows;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += align_up(bytes, 256);
     return here;
   };
-  L.prefix = take((entries + 1) * 8);
+  L.cut = take((size_t)L.grid * sizeof(CutUnit));
   L.ml = take((size_t)L.grid * 2 * L.shape.heads * 2 * 4);
   L.o = take((size_t)L.grid * 2 * L.shape.heads * c.head_dim * 4);
   L.lse = take(io.mass ? (size_t)L.rows * io.heads * 4 : 0);
@@ -447,7 +488,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     a.status = io->status;
     a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;
     a.units = io->pages ? L.blocks : cache->kv_heads * L.blocks;
-    a.prefix = (long long*)(ws + L.prefix);
+    a.cut = (CutUnit*)(ws + L.cut);
     a.part_ml = (float*)(ws + L.ml);
     a.part_o = (float*)(ws + L.o);
     a.grid = L.grid;
@@ -467,10 +508,11 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     else
       rc = qb ? attend_simt<bf>(a, L.shape, st) : attend_simt<float>(a, L.shape, st);
     if (rc) return rc;
-    const unsigned units = (unsigned)a.rows * cache->kv_heads * L.blocks;
     const int gb = L.shape.heads;
-    rc = qb ? launch_chained(kv_join_kernel<bf>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, gb)
-            : launch_chained(kv_join_kernel<float>, dim3(units), dim3(128), 0, st, "kv_join_kernel", a, gb);
+    const dim3 grid(L.grid, gb < a.group ? gb : a.group);
+    const size_t smem = (size_t)(L.grid + 3) / 4 * 16 + kJoinThreads * 16;
+    rc = qb ? launch_chained(kv_join_kernel<bf>, grid, dim3(kJoinThreads), smem, st, "kv_join_kernel", a, gb)
+            : launch_chained(kv_join_kernel<float>, grid, dim3(kJoinThreads), smem, st, "kv_join_kernel", a, gb);
     if (rc) return rc;
     if (io->mass && io->mass_len > 0) {
       const int pairs = a.rows * cache->kv_heads;

@@ -19,6 +19,13 @@ namespace er {
 constexpr int kKvMaxLen = 0x7fff0000;  // positions stay ints with a tile's keys added
 constexpr int kKvChunk = 16;  // keys a warp takes at a time
 
+// A unit whose tiles several CTAs share: the first of them writes it, the join reads it.
+struct CutUnit {
+  int row, head, g0;  // row -1: none begins here and ends behind
+  int tiles;
+  long long begin, total;  // its first tile, and all tiles of the launch
+};
+
 struct AttendArgs {
   KvView kv;
   const void* q;
@@ -38,7 +45,7 @@ struct AttendArgs {
   int* status;
   // scan entries: rows, or (row, key head) pairs when each has its own page list
   int entries, units;          // units of one entry: the tiles repeat that often
-  long long* prefix;           // [entries + 1] tiles of one unit before an entry; written by CTA 0
+  CutUnit* cut;                // [grid] the unit that begins in a CTA's run and ends behind it
   float* part_ml;              // [2 grid][GB][2]: m, l of a CTA's first and last piece
   float* part_o;               // [2 grid][GB][d]
   int grid;                    // CTAs of the attention kernel
@@ -116,10 +123,12 @@ struct Place {
 };
 
 // The CTA's run of tiles: its first place and how many tiles it has. Every
-// CTA sums the entries' tiles itself (a few loads a thread); CTA 0 leaves the
-// prefix for the join. `sums`: blockDim.x + 1 long longs, shared.
-__device__ __forceinline__ long long kv_run(const AttendArgs& a, long long* sums, int* where, Place& p,
-                                            long long* left) {
+// CTA sums the entries' tiles itself (a few loads a thread). `sums`: blockDim.x + 1 long longs, shared.
+struct Run {
+  long long begin, left, total;
+};
+__device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int* where, Place& p) {
+  if (threadIdx.x == 0) a.cut[blockIdx.x].row = -1;
   const int per = (a.entries + blockDim.x - 1) / blockDim.x;
   const int x0 = min(a.entries, (int)threadIdx.x * per), x1 = min(a.entries, x0 + per);
   long long mine = 0;
@@ -149,18 +158,9 @@ __device__ __forceinline__ long long kv_run(const AttendArgs& a, long long* sums
   }
   __syncthreads();
   const long long per_unit = sums[blockDim.x], total = per_unit * a.units;
-  if (blockIdx.x == 0) {
-    long long run = sums[threadIdx.x];
-    for (int x = x0; x < x1; ++x) {
-      a.prefix[x] = run;
-      run += kv_tiles(a, kv_entry(a, x).n);
-    }
-    if (threadIdx.x == 0) a.prefix[a.entries] = per_unit;
-  }
-  *left = 0;
-  if (total == 0) return 0;
+  if (total == 0) return Run{0, 0, 0};
   const int shares = kv_shares(a, total);
-  if ((int)blockIdx.x >= shares) return 0;
+  if ((int)blockIdx.x >= shares) return Run{0, 0, total};
   const long long begin = kv_share_start(total, shares, blockIdx.x);
   const long long end = kv_share_start(total, shares, blockIdx.x + 1);
   // the entry whose units hold tile `begin`: all units of the entries before it are passed
@@ -182,8 +182,7 @@ __device__ __forceinline__ long long kv_run(const AttendArgs& a, long long* sums
   p.load(a, where[0]);
   p.u = where[1];
   p.t = where[2];
-  *left = end - begin;
-  return begin;
+  return Run{begin, end - begin, total};
 }
 
 // Where key j of a place lies: byte offset of its slot (key head included)

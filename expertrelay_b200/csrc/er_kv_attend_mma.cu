@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
   }
   chain_wait();
   Place c;
-  long long left;
-  kv_run(a, sums, where, c, &left);
+  const Run run = kv_run(a, sums, where, c);
+  long long left = run.left;
   if (left == 0) return;
 
   Place f = c;
@@ -231,6 +231,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     if (mask & 0xffff) {
       const uint32_t kc = smem_addr(ring + st * 2 * Ring::kChunkBytes), vc = kc + Ring::kChunkBytes;
       const int mi = lane / 8, mr = lane % 8;  // the 8x8 matrix and its row that this lane addresses
+      // two chains of products: their latencies overlap, and each is summed
+      // over half as many steps (the parts below the leading one in the second)
       float s2[2][NT][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint2 b = qf[((ks * QS + p) * NT + nt) * 32 + lane];
-            mma(s2[ks & 1][nt], kf, b.x, b.y);
+            mma(s2[QS == 1 ? ks & 1 : p > 0][nt], kf, b.x, b.y);
           }
       }
       const bool on0 = (mask >> (lane / 4)) & 1, on1 = (mask >> (lane / 4 + 8)) & 1;
@@ -324,9 +326,18 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         uint32_t vf[4];
         ldsm_t(vf, vc + swz<DP>((mi >> 1) * 8 + mr, k * 2 + (mi & 1)));
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          if (QS == 1) {
 #pragma unroll
-          for (int i = PS - 1; i >= 0; --i) mma(o[k][nt], vf, b[i][nt][0], b[i][nt][1]);
+            for (int i = PS - 1; i >= 0; --i) mma(o[k][nt], vf, b[i][nt][0], b[i][nt][1]);
+          } else {  // the tensor cores cut their sums: a chunk's alone there, the running sum rounded here
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = PS - 1; i >= 0; --i) mma(x, vf, b[i][nt][0], b[i][nt][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][nt][e] += x[e];
+          }
+        }
       }
     }
     __syncwarp();
@@ -356,6 +367,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       }
     if (bad && lane == 0) spoiled = 1;
     const bool whole = first_t == 0 && t + 1 == tiles;
+    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind (the run's last tile is tile t)
+      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, run.begin + run.left - (t + 1), run.total};
 #pragma unroll
     for (int q4 = 0; q4 < NT * 8 / kMergeHeads; ++q4) {
       if (q4 * kMergeHeads >= live_g) break;
