@@ -1,6 +1,8 @@
 // er_kv.cuh -- the paged key-value cache as the er_kv_* kernels see it.
 #pragma once
 
+#include <atomic>
+
 #include "er_internal.cuh"
 
 namespace er {
@@ -42,6 +44,33 @@ inline int kv_check(const char* who, const er_kv_cache* c) {
   return ER_OK;
 }
 
+// The current device, and its SMs (asked once a device).
+inline int device_sms(int* sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  if (dev < 64 && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return ER_OK;
+  if (int rc = cuda_check(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute"))
+    return rc;
+  if (dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
+  return ER_OK;
+}
+
+// Lets `kernel` take up to `bytes` of dynamic shared memory (set once a
+// device; `done`: one word per kernel, a bit per device).
+template <typename K>
+inline int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return ER_OK;
+  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                          "shared memory attribute"))
+    return rc;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return ER_OK;
+}
+
 __device__ __forceinline__ void kv_report(int* status, int bit) {
   if (status) atomicOr(status, bit);
 }
@@ -79,47 +108,67 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   return before + inc - v;
 }
 
-// The `want`-th largest of key(i), i in [lo, hi), by the whole block: 8 bits
-// a pass from the top. Returns the threshold; *equal is how many of the keys
-// equal to it belong to the `want` largest (the lowest i first). want >= 1,
-// want <= hi - lo. `hist`: 256 ints, `red`: 2 ints, shared.
-template <typename Key>
-__device__ uint32_t block_select(Key key, int lo, int hi, int want, int* hist, int* red, int* equal) {
+// Positions ranked by a score: their rank keys in shared memory where they
+// fit (a key behind every 32 is left out, so that runs of any length start in
+// different banks), else read from the scores each time.
+struct RankKeys {
+  uint32_t* held;
+  const float* scores;
+
+  __device__ __forceinline__ static int at(int i) { return i + (i >> 5); }
+  __device__ __forceinline__ uint32_t operator()(int i) const { return held ? held[at(i)] : rank_key(scores[i]); }
+};
+inline size_t rank_keys_bytes(long long n) { return (size_t)(n + n / 32 + 1) * 4; }
+
+// Bins of one pass of the select: 11, 11, then 10 bits. Four copies of the
+// histogram, by lane, where there are many keys: scores crowd into few bins
+// (a sum that is still zero, one binade) and shared-memory atomics on one
+// address run one by one.
+constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
+constexpr size_t kSelectBytes = (size_t)kSelectBins * kSelectCopies * 4;
+
+// The `want`-th largest of key(i), i in [lo, hi), by the whole block.
+// Returns the threshold; *equal is how many of the keys equal to it belong to
+// the `want` largest (the lowest i first). 1 <= want <= hi - lo. `hist`:
+// kSelectBytes, `red`: one int per warp and two more, shared.
+__device__ __forceinline__ uint32_t block_select(const RankKeys& key, int lo, int hi, int want, int* hist, int* red,
+                                                 int* equal) {
+  const int copies = hi - lo >= kSelectMany ? kSelectCopies : 1, warps = blockDim.x >> 5;
+  int* mine = hist + (copies > 1 ? (threadIdx.x & (kSelectCopies - 1)) * kSelectBins : 0);
   uint32_t prefix = 0, mask = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int b = threadIdx.x; b < 256; b += blockDim.x) hist[b] = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    for (int b = threadIdx.x; b < copies * kSelectBins; b += blockDim.x) hist[b] = 0;
     __syncthreads();
     for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) {
       const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    if (threadIdx.x < 32) {  // lane l: bins 255 - 8 l .. 248 - 8 l, from the top
-      int c[8], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += c[j] = hist[255 - 8 * (int)threadIdx.x - j];
-      int inc = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((int)threadIdx.x >= o) inc += up;
-      }
-      int above = inc - sum;
-      if (above < want && want <= inc) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (above < want && want <= above + c[j]) {
-            red[0] = 255 - 8 * (int)threadIdx.x - j;
-            red[1] = want - above;
-          }
-          above += c[j];
+    // thread t: `per` bins from the top
+    const int per = (bins + blockDim.x - 1) / blockDim.x, top = bins - 1 - (int)threadIdx.x * per;
+    int sum = 0;
+    for (int j = 0; j < per; ++j)
+      if (top - j >= 0)
+        for (int c = 0; c < copies; ++c) sum += hist[c * kSelectBins + top - j];
+    int total;
+    int above = block_scan(sum, red, &total);
+    if (above < want && want <= above + sum) {
+      for (int j = 0; j < per; ++j) {
+        int n = 0;
+        for (int c = 0; c < copies; ++c) n += hist[c * kSelectBins + top - j];
+        if (above < want && want <= above + n) {
+          red[warps] = top - j;
+          red[warps + 1] = want - above;
         }
+        above += n;
       }
     }
     __syncthreads();
-    prefix |= (uint32_t)red[0] << shift;
-    mask |= 255u << shift;
-    want = red[1];
+    prefix |= (uint32_t)red[warps] << shift;
+    mask |= (uint32_t)(bins - 1) << shift;
+    want = red[warps + 1];
   }
   *equal = want;
   return prefix;

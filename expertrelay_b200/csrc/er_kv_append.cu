@@ -21,16 +21,52 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// One CTA per token. The products and sums of the rotation are rounded one
-// by one (no fused multiply-add), so a key's bits do not depend on which
-// half of the pair it is, and the pages' codes follow from the formula alone.
-template <typename TX, typename TQ, typename TC>
+// VEC values as fp32, by 16-byte loads and stores where VEC is 8.
+template <int VEC, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&x)[VEC]) {
+  if constexpr (VEC == 1) {
+    x[0] = to_f32(*p);
+  } else {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      const uint4 raw = ld_stream_u4(p + i);
+      const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[i + e] = to_f32(v[e]);
+    }
+  }
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(x[0]);
+  } else {
+    constexpr int N = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < VEC; i += N) {
+      uint4 raw;
+      T* v = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = from_f32<T>(x[i + e]);
+      *reinterpret_cast<uint4*>(p + i) = raw;
+    }
+  }
+}
+
+// One CTA per token; a thread turns VEC pairs (j, j + d/2) of a head, or
+// copies two VECs of a v head. The products and sums of the rotation are
+// rounded one by one (no fused multiply-add), so a key's bits do not depend
+// on which half of the pair it is, and the pages' codes follow from the
+// formula alone. Memory-bound; the angles' sines (64 bits, half a row of
+// threads) run while the other CTAs of the SM have their rows in flight.
+template <typename TX, typename TQ, typename TC, int VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
                                                         const int32_t* __restrict__ seqs,
                                                         const int32_t* __restrict__ positions, int heads,
                                                         const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
                                                         int* status) {
-  __shared__ float cs[256];  // [d/2] cos, then [d/2] sin
+  __shared__ __align__(16) float cs[256];  // [d/2] cos, then [d/2] sin
   chain_wait();
   const int t = blockIdx.x, d = kv.d, half = d / 2, kvh = kv.kv_heads;
   const int pos = positions[t], seq = seqs ? seqs[t] : t;
@@ -59,24 +95,30 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __r
   if (bad && threadIdx.x == 0) kv_report(status, bad);
   __syncthreads();
   const TX* row = qkv + (long long)t * ld;
-  for (int i = threadIdx.x; i < (heads + kvh) * half; i += blockDim.x) {
-    const int head = i / half, j = i % half;
-    const float c = cs[j], s = cs[half + j];
-    const float a = to_f32(row[(long long)head * d + j]), b = to_f32(row[(long long)head * d + j + half]);
-    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), y = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+  const int per = half / VEC;
+  for (int i = threadIdx.x; i < (heads + 2 * kvh) * per; i += blockDim.x) {
+    const int head = i / per, j = i % per * VEC;
+    float a[VEC], b[VEC];
+    load_vec<VEC>(row + (long long)head * d + j, a);
+    load_vec<VEC>(row + (long long)head * d + j + half, b);
+    if (head < heads + kvh) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float c = cs[j + e], s = cs[half + j + e], x = a[e], y = b[e];
+        a[e] = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+        b[e] = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+      }
+    }
     if (head < heads) {
-      TQ* qo = q_out + ((long long)t * heads + head) * d;
-      qo[j] = from_f32<TQ>(x);
-      qo[j + half] = from_f32<TQ>(y);
+      TQ* o = q_out + ((long long)t * heads + head) * d + j;
+      store_vec<VEC>(o, a);
+      store_vec<VEC>(o + half, b);
     } else if (!bad) {
-      const long long h = head - heads;
-      TC* ko = reinterpret_cast<TC*>(kp + h * kv.head_stride);
-      ko[j] = from_f32<TC>(x);
-      ko[j + half] = from_f32<TC>(y);
-      TC* vo = reinterpret_cast<TC*>(vp + h * kv.head_stride);
-      const TX* vr = row + (long long)(head + kvh) * d;
-      vo[j] = from_f32<TC>(to_f32(vr[j]));
-      vo[j + half] = from_f32<TC>(to_f32(vr[j + half]));
+      const bool key = head < heads + kvh;
+      TC* o = reinterpret_cast<TC*>((key ? kp + (head - heads) * kv.head_stride
+                                         : vp + (head - heads - kvh) * kv.head_stride)) + j;
+      store_vec<VEC>(o, a);
+      store_vec<VEC>(o + half, b);
     }
   }
 }
@@ -186,8 +228,11 @@ const InvFreq& inv_freq(double theta, int d) {
 template <typename TX, typename TQ, typename TC>
 int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* seqs, const int32_t* positions, int n,
               int heads, double theta, void* q_out, int* status, cudaStream_t st) {
-  return launch_chained(kv_append_kernel<TX, TQ, TC>, dim3(n), dim3(256), 0, st, "kv_append_kernel", kv,
-                        (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
+  // 16-byte accesses need half a head in whole VECs and aligned rows
+  const bool vec = kv.d % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)(ld * sizeof(TX))) & 15);
+  return launch_chained(vec ? kv_append_kernel<TX, TQ, TC, 8> : kv_append_kernel<TX, TQ, TC, 1>, dim3(n), dim3(256), 0,
+                        st, "kv_append_kernel", kv, (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d),
+                        (TQ*)q_out, status);
 }
 
 }  // namespace

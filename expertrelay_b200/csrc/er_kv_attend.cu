@@ -360,9 +360,8 @@ namespace {
 template <typename TQ, int GB>
 int simt_go(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
   auto kernel = kv_attend_simt_kernel<TQ, GB>;
-  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, s.smem),
-                          "kv_attend smem attribute"))
-    return rc;
+  static std::atomic<unsigned long long> done;
+  if (int rc = allow_smem(kernel, 224 * 1024, done)) return rc;
   return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a,
                         simt_pitch(a.kv.d));
 }
@@ -428,12 +427,6 @@ int attend_check(const er_kv_cache* c, const er_kv_attend_io* io) {
   return ER_OK;
 }
 
-int device_sms(int* sms) {
-  int dev = 0;
-  if (int rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
-  return cuda_check(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), "cudaDeviceGetAttribute");
-}
-
 }  // namespace
 }  // namespace er
 
@@ -455,6 +448,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
   const Layout L = attend_layout(*cache, *io, sms);
   if (!workspace || workspace_bytes < L.bytes)
     return fail(ER_ENOSPACE, "er_kv_attend: workspace %zu bytes, need %zu", workspace_bytes, L.bytes);
+  if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_kv_attend: workspace must be 256-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;
   char* ws = (char*)workspace;
   const size_t qs = io->q_dtype == ER_DTYPE_BF16 ? 2 : 4;

@@ -427,9 +427,8 @@ template <int DP, int NT, int QS>
 int mma_go(const AttendArgs& a, cudaStream_t st) {
   auto kernel = kv_attend_mma_kernel<DP, NT, QS>;
   constexpr int smem = mma_smem<DP, NT, QS>();
-  if (int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                          "kv_attend smem attribute"))
-    return rc;
+  static std::atomic<unsigned long long> done;
+  if (int rc = allow_smem(kernel, smem, done)) return rc;
   return launch_chained(kernel, dim3(a.grid), dim3(kMmaWarps * 32), smem, st, "kv_attend_mma_kernel", a);
 }
 

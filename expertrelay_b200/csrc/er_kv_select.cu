@@ -93,46 +93,72 @@ __global__ void __launch_bounds__(kScoreThreads)
 }
 
 // Writes, ascending, the `take` of n positions that are forced (the first
-// `sinks`, the last `recent`) or rank best; emit(slot, i) for each.
-template <typename Key, typename Emit>
-__device__ void take_best(Key key, int n, int take, int sinks, int recent, int* hist, int* red, Emit emit) {
+// `sinks`, the last `recent`) or rank best; emit(slot, i) for each. `held`:
+// room for the n keys in shared memory, or NULL.
+template <typename Emit>
+__device__ __forceinline__ void take_best(const float* scores, uint32_t* held, int n, int take, int sinks, int recent,
+                                          int* hist, int* red, Emit emit) {
   if (n <= take) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) emit(i, i);
     return;
   }
   const int lo = sinks, hi = n - recent, want = take - sinks - recent;
+  if (held) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
+    __syncthreads();
+  }
+  const RankKeys key{held, scores};
   uint32_t least = 0xffffffffu;
   int equal = 0;
   if (want > 0) least = block_select(key, lo, hi, want, hist, red, &equal);
+  // in rounds of a run of positions a thread: one run takes them all when they are held
+  const int run = held ? (n + blockDim.x - 1) / blockDim.x : 8;
   int above = 0, same = 0;  // taken outright, and equal to the threshold, so far
-  for (int i0 = 0; i0 < n; i0 += blockDim.x) {
-    const int i = i0 + threadIdx.x;
-    bool sure = false, tie = false;
-    if (i < n) {
-      if (i < lo || i >= hi) {
-        sure = true;
-      } else if (want > 0) {
-        const uint32_t k = key(i);
-        sure = k > least;
-        tie = k == least;
+  for (int i0 = 0; i0 < n; i0 += run * blockDim.x) {
+    const int b = min(n, i0 + (int)threadIdx.x * run), e = min(n, b + run);
+    int sure = 0, ties = 0;
+    for (int i = b; i < e; ++i) {
+      const bool forced = i < lo || i >= hi;
+      const uint32_t k = key(i);
+      sure += forced || (want > 0 && k > least);
+      ties += !forced && want > 0 && k == least;
+    }
+    int all_sure, all_ties;
+    int at = above + block_scan(sure, red, &all_sure);
+    int tie = same + block_scan(ties, red, &all_ties);
+    for (int i = b; i < e; ++i) {
+      const bool forced = i < lo || i >= hi;
+      const uint32_t k = key(i);
+      if (forced || (want > 0 && k > least)) {
+        emit(at + min(tie, equal), i);
+        ++at;
+      } else if (want > 0 && k == least) {
+        if (tie < equal) emit(at + tie, i);
+        ++tie;
       }
     }
-    int total;
-    const int before = block_scan((int)sure | ((int)tie << 16), red, &total);
-    const int ties = same + (before >> 16);
-    if (sure || (tie && ties < equal)) emit(above + (before & 0xffff) + min(ties, equal), i);
-    above += total & 0xffff;
-    same += total >> 16;
+    above += all_sure;
+    same += all_ties;
   }
 }
 
-constexpr int kTakeThreads = 512;
+constexpr int kTakeThreads = 1024;
+
+// Shared memory of a CTA that takes the best of at most n: the histograms,
+// and the keys where they fit beside them (*held).
+inline size_t take_smem(long long n, bool* held) {
+  *held = kSelectBytes + rank_keys_bytes(n) <= 200 * 1024;
+  return kSelectBytes + (*held ? rank_keys_bytes(n) : 0);
+}
+inline int take_threads(long long n) { return n <= 1024 ? 256 : n <= 8192 ? 512 : kTakeThreads; }
 
 __global__ void __launch_bounds__(kTakeThreads)
     kv_choose_kernel(KvView kv, const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-                     const float* __restrict__ scores, int budget, int sinks, int recent, int32_t* __restrict__ pages,
-                     int32_t* __restrict__ counts, int* status) {
-  __shared__ int hist[256], red[kTakeThreads / 32];
+                     const float* __restrict__ scores, int budget, int sinks, int recent, int held,
+                     int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
+  extern __shared__ int hist[];
+  __shared__ int red[kTakeThreads / 32 + 2];
   chain_wait();
   const int row = blockIdx.x / kv.kv_heads;
   const int seq = seqs ? seqs[row] : row, len = lens[row];
@@ -140,10 +166,9 @@ __global__ void __launch_bounds__(kTakeThreads)
   if ((bad_seq || bad_len) && threadIdx.x == 0) kv_report(status, bad_seq ? ER_KV_BAD_SEQ : ER_KV_BAD_LENGTH);
   const int n = bad_seq || bad_len ? 0 : (len + kv.page_size - 1) / kv.page_size;
   const int take = min(n, budget);
-  const float* s = scores + (long long)blockIdx.x * kv.width;
   int32_t* out = pages + (long long)blockIdx.x * budget;
-  take_best([&](int i) { return rank_key(s[i]); }, n, budget, sinks, recent, hist, red,
-            [&](int slot, int i) { out[slot] = i; });
+  take_best(scores + (long long)blockIdx.x * kv.width, held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr, n, budget,
+            sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
   for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
   if (threadIdx.x == 0) counts[blockIdx.x] = take;
 }
@@ -157,8 +182,9 @@ struct MassView {
 
 __global__ void __launch_bounds__(kTakeThreads)
     kv_keep_kernel(KvView kv, MassView m, const int32_t* __restrict__ lens, int budget, int sinks, int recent,
-                   int32_t* __restrict__ kept, int32_t* __restrict__ lens_out, int* status) {
-  __shared__ int hist[256], red[kTakeThreads / 32];
+                   int held, int32_t* __restrict__ kept, int32_t* __restrict__ lens_out, int* status) {
+  extern __shared__ int hist[];
+  __shared__ int red[kTakeThreads / 32 + 2];
   chain_wait();
   const int seq = blockIdx.x / kv.kv_heads, h = blockIdx.x % kv.kv_heads;
   int n = lens[seq];
@@ -169,10 +195,11 @@ __global__ void __launch_bounds__(kTakeThreads)
   const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
   float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
   int32_t* out = kept + (long long)blockIdx.x * budget;
-  take_best([&](int i) { return rank_key(w[i]); }, n, budget, sinks, recent, hist, red, [&](int slot, int i) {
-    out[slot] = i;
-    to[slot] = w[i];
-  });
+  take_best(w, held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr, n, budget, sinks, recent, hist, red,
+            [&](int slot, int i) {
+              out[slot] = i;
+              to[slot] = w[i];
+            });
   const int take = min(n, budget);
   for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
   if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
@@ -253,8 +280,13 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
     rc = launch_chained(kv_score_kernel<float>, dim3(gx, units), dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
                         (const float*)q, q_stride, group, seqs, lens, codes, scales, (float*)workspace, status);
   if (rc) return rc;
-  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), 0, st, "kv_choose_kernel", kv, seqs, lens,
-                        (const float*)workspace, budget, sinks, recent, pages_out, counts_out, status);
+  bool held;
+  const size_t take = take_smem(kv.width, &held);
+  static std::atomic<unsigned long long> done;
+  if ((rc = allow_smem(kv_choose_kernel, 200 * 1024, done))) return rc;
+  return launch_chained(kv_choose_kernel, dim3(units), dim3(take_threads(kv.width)), take, st, "kv_choose_kernel", kv,
+                        seqs, lens, (const float*)workspace, budget, sinks, recent, (int)held, pages_out, counts_out,
+                        status);
 }
 
 extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
@@ -280,8 +312,13 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   const MassView m{mass,        to_mass,  mass_seq_stride, mass_head_stride, to_mass_seq_stride, to_mass_head_stride,
                    mass_len, to_mass_len};
   cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = launch_chained(kv_keep_kernel, dim3(a.seqs * a.kv_heads), dim3(kTakeThreads), 0, st, "kv_keep_kernel", a,
-                              m, lens, budget, sinks, recent, kept_out, lens_out, status))
+  bool held;
+  const size_t take = take_smem(mass_len, &held);
+  static std::atomic<unsigned long long> done;
+  if (int rc = allow_smem(kv_keep_kernel, 200 * 1024, done)) return rc;
+  if (int rc = launch_chained(kv_keep_kernel, dim3(a.seqs * a.kv_heads), dim3(take_threads(mass_len)), take, st,
+                              "kv_keep_kernel", a, m, lens, budget, sinks, recent, (int)held, kept_out, lens_out,
+                              status))
     return rc;
   const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4);
   const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;

@@ -25,8 +25,8 @@ workspace from torch's allocator on that stream unless given one.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -45,11 +45,35 @@ def _need(t, name: str, dtype, device: torch.device, shape=None, contiguous: boo
         raise ValueError(f"{name}: must be contiguous")
 
 
-def _guard(device: torch.device):
-    """The device's context where it is not the current one already."""
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _apart(shape, stride) -> bool:
+    """Whether no two elements of the strided tensor share a place (each stride passes all that smaller ones reach)."""
+    reach = 0
+    for step, n in sorted((s, n) for s, n in zip(stride, shape) if n > 1):
+        if step <= reach:
+            return False
+        reach += step * (n - 1)
+    return True
+
+
+def _weights(t, name: str, cache, rows: int, written: bool) -> None:
+    if not isinstance(t, torch.Tensor) or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name}: expected [{rows}, {cache.kv_heads}, n] with contiguous positions")
+    _need(t, name, torch.float32, cache.device, (rows, cache.kv_heads, t.shape[2]), contiguous=False)
+    if written and not _apart(t.shape, t.stride()):
+        raise ValueError(f"{name}: strides {t.stride()} make elements share memory")
+
+
+def _on_device(call):
+    """The call with its cache's device as the current one (kernels are launched and memory is allocated there)."""
+
+    @functools.wraps(call)
+    def on_device(cache, *args, **kwargs):
+        if torch.cuda.current_device() == cache._index:
+            return call(cache, *args, **kwargs)
+        with torch.cuda.device(cache._index):
+            return call(cache, *args, **kwargs)
+
+    return on_device
 
 
 class PagedKV:
@@ -66,7 +90,7 @@ class PagedKV:
         if k.dim() != 4 or k.dtype not in _DTYPES or not k.is_cuda:
             raise ValueError(f"k: expected a [pages, kv_heads, page_size, head_dim] float32 or bfloat16 CUDA tensor, "
                              f"got {tuple(k.shape)} {k.dtype} on {k.device}")
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.dtype, self._index = k.device, k.dtype, k.device.index
         _need(v, "v", k.dtype, k.device, k.shape, contiguous=False)
         if k.stride() != v.stride() or k.stride(3) != 1:
             raise ValueError(f"k, v: strides {k.stride()}, {v.stride()} (alike, the last dimension contiguous)")
@@ -77,15 +101,22 @@ class PagedKV:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.seqs, self.width = table.shape
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._status = self.status.data_ptr()
         self._c = _lib.KvCache(
             k=k.data_ptr(), v=v.data_ptr(), dtype=_DTYPES[k.dtype], num_pages=self.num_pages,
             page_size=self.page_size, kv_heads=self.kv_heads, head_dim=self.head_dim, page_stride=k.stride(0),
             head_stride=k.stride(1), slot_stride=k.stride(2), table=table.data_ptr(), seqs=self.seqs,
             table_width=self.width, table_stride=table.stride(0))
         self._ref = C.byref(self._c)
+        self._needs: dict[tuple, int] = {}  # workspace bytes by the sizes of a call
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # the handle of torch.cuda.current_stream(device), without building a Stream object for it
+        return torch._C._cuda_getCurrentRawStream(self._index)
+
+    def _writable(self) -> None:
+        if not _apart(self.k.shape, self.k.stride()):
+            raise ValueError(f"pools of strides {self.k.stride()} make slots share memory")
 
     def check(self) -> None:
         """Raises ValueError if a call since the last check met a bad page id,
@@ -110,6 +141,7 @@ class PageBounds:
         _need(codes, "codes", torch.int8, codes.device)
         _need(scales, "scales", torch.float32, codes.device, codes.shape[:2])
         self.codes, self.scales = codes, scales
+        self._codes, self._scales = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def new(cls, cache: PagedKV) -> PageBounds:
@@ -136,8 +168,8 @@ def _queries(cache: PagedKV, q: torch.Tensor):
     return rows, heads, q.stride(0) if rows > 1 else heads * d
 
 
-def _row_args(cache: PagedKV, rows: int, lens: torch.Tensor, seqs: torch.Tensor | None) -> None:
-    _need(lens, "lens", torch.int32, cache.device, (rows,))
+def _row_args(cache: PagedKV, rows: int, lens: torch.Tensor, seqs: torch.Tensor | None, name: str = "lens") -> None:
+    _need(lens, name, torch.int32, cache.device, (rows,))
     if seqs is not None:
         _need(seqs, "seqs", torch.int32, cache.device, (rows,))
     elif rows > cache.seqs:
@@ -155,6 +187,7 @@ def _scratch(need: int, workspace: torch.Tensor | None, device: torch.device) ->
     return workspace
 
 
+@_on_device
 def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: int, theta: float, *,
            seqs: torch.Tensor | None = None, q_dtype: torch.dtype | None = None) -> torch.Tensor:
     """New tokens into the cache: qkv [n, (heads + 2 kv_heads) head_dim]
@@ -167,20 +200,21 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
         raise ValueError(f"qkv: expected [n, {(heads + 2 * cache.kv_heads) * cache.head_dim}] float32 or bfloat16 on "
                          f"{cache.device}, got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
     n = qkv.shape[0]
-    _row_args(cache, n, positions, seqs)
+    _row_args(cache, n, positions, seqs, "positions")
+    cache._writable()
     dt = qkv.dtype if q_dtype is None else q_dtype
     if dt not in _DTYPES:
         raise ValueError(f"q_dtype: float32 or bfloat16, got {dt}")
-    with _guard(cache.device):
-        q = torch.empty((n, heads, cache.head_dim), dtype=dt, device=cache.device)
-        _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
-                                           qkv.stride(0) if n > 1 else qkv.shape[1],
-                                           None if seqs is None else seqs.data_ptr(), positions.data_ptr(), n,
-                                           int(heads), float(theta), q.data_ptr(), _DTYPES[dt],
-                                           cache.status.data_ptr(), cache._stream()), "er_kv_append")
+    q = torch.empty((n, heads, cache.head_dim), dtype=dt, device=cache.device)
+    _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
+                                       qkv.stride(0) if n > 1 else qkv.shape[1],
+                                       None if seqs is None else seqs.data_ptr(), positions.data_ptr(), n,
+                                       int(heads), float(theta), q.data_ptr(), _DTYPES[dt],
+                                       cache._status, cache._stream()), "er_kv_append")
     return q
 
 
+@_on_device
 def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.Tensor | None = None,
            scale: float | None = None, mass: torch.Tensor | None = None, pages: torch.Tensor | None = None,
            counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
@@ -204,7 +238,7 @@ def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.T
     io = _lib.KvAttendIO(
         q=q.data_ptr(), q_dtype=_DTYPES[q.dtype], q_stride=stride, out=out.data_ptr(), rows=rows, heads=heads,
         seqs=None if seqs is None else seqs.data_ptr(), lens=lens.data_ptr(),
-        scale=cache.head_dim ** -0.5 if scale is None else float(scale), status=cache.status.data_ptr())
+        scale=cache.head_dim ** -0.5 if scale is None else float(scale), status=cache._status)
     if (pages is None) != (counts is None):
         raise ValueError("pages and counts go together")
     if pages is not None:
@@ -216,33 +250,34 @@ def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.T
         _need(counts, "counts", torch.int32, cache.device, (rows, cache.kv_heads))
         io.pages, io.counts, io.max_pages = pages.data_ptr(), counts.data_ptr(), pages.shape[2]
     if mass is not None:
-        if mass.dim() != 3 or (mass.shape[2] > 1 and mass.stride(2) != 1):
-            raise ValueError("mass: expected [rows, kv_heads, n] with contiguous positions")
-        _need(mass, "mass", torch.float32, cache.device, (rows, cache.kv_heads, mass.shape[2]), contiguous=False)
+        _weights(mass, "mass", cache, rows, True)
         io.mass, io.mass_len = mass.data_ptr(), mass.shape[2]
         io.mass_row_stride, io.mass_head_stride = mass.stride(0), mass.stride(1)
     if rows == 0:
         return out
     lib, ref = _lib.lib(), C.byref(io)
-    with _guard(cache.device):
-        ws = _scratch(lib.er_kv_attend_workspace_bytes(cache._ref, ref), workspace, cache.device)
-        _lib.check(lib.er_kv_attend(cache._ref, ref, ws.data_ptr(), ws.numel() * ws.element_size(), cache._stream()),
-                   "er_kv_attend")
+    sizes = (rows, heads, q.dtype, io.max_pages, io.mass_len if mass is not None else -1)
+    need = cache._needs.get(sizes)
+    if need is None:
+        need = cache._needs[sizes] = lib.er_kv_attend_workspace_bytes(cache._ref, ref)
+    ws = _scratch(need, workspace, cache.device)
+    _lib.check(lib.er_kv_attend(cache._ref, ref, ws.data_ptr(), max(need, 16), cache._stream()), "er_kv_attend")
     return out
 
 
+@_on_device
 def page_bounds(cache: PagedKV, bounds: PageBounds, lens: torch.Tensor, start: torch.Tensor) -> None:
     """Renews the bounds of the pages that hold positions [start[s], lens[s])
     of every sequence s, from the page's keys up to lens[s]."""
     bounds._fit(cache)
     _need(lens, "lens", torch.int32, cache.device, (cache.seqs,))
     _need(start, "start", torch.int32, cache.device, (cache.seqs,))
-    with _guard(cache.device):
-        _lib.check(_lib.lib().er_kv_page_bounds(cache._ref, lens.data_ptr(), start.data_ptr(),
-                                                bounds.codes.data_ptr(), bounds.scales.data_ptr(),
-                                                cache.status.data_ptr(), cache._stream()), "er_kv_page_bounds")
+    _lib.check(_lib.lib().er_kv_page_bounds(cache._ref, lens.data_ptr(), start.data_ptr(),
+                                            bounds._codes, bounds._scales,
+                                            cache._status, cache._stream()), "er_kv_page_bounds")
 
 
+@_on_device
 def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torch.Tensor, budget: int, *,
                  sinks: int = 1, recent: int = 1, seqs: torch.Tensor | None = None,
                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -258,18 +293,19 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} with {sinks} first and {recent} last pages")
     lib = _lib.lib()
-    with _guard(cache.device):
-        pages = torch.empty((rows, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
-        counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
-        ws = _scratch(lib.er_kv_select_workspace_bytes(cache._ref, rows), workspace, cache.device)
-        _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
-                                    None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
-                                    bounds.codes.data_ptr(), bounds.scales.data_ptr(), int(budget), int(sinks),
-                                    int(recent), pages.data_ptr(), counts.data_ptr(), cache.status.data_ptr(),
-                                    ws.data_ptr(), ws.numel() * ws.element_size(), cache._stream()), "er_kv_select")
+    pages = torch.empty((rows, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
+    counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
+    need = lib.er_kv_select_workspace_bytes(cache._ref, rows)
+    ws = _scratch(need, workspace, cache.device)
+    _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
+                                None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
+                                bounds._codes, bounds._scales, int(budget), int(sinks),
+                                int(recent), pages.data_ptr(), counts.data_ptr(), cache._status,
+                                ws.data_ptr(), max(need, 16), cache._stream()), "er_kv_select")
     return pages, counts
 
 
+@_on_device
 def evict(cache: PagedKV, lens: torch.Tensor, mass: torch.Tensor, to: PagedKV, to_mass: torch.Tensor, budget: int, *,
           sinks: int = 4, recent: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
     """Keeps min(lens[s], budget) positions of every sequence and key head:
@@ -285,20 +321,18 @@ def evict(cache: PagedKV, lens: torch.Tensor, mass: torch.Tensor, to: PagedKV, t
     if to.table.data_ptr() == cache.table.data_ptr() and to.k.data_ptr() == cache.k.data_ptr():
         raise ValueError("to: the cache's own pages")
     _need(lens, "lens", torch.int32, cache.device, (cache.seqs,))
-    for t, name in ((mass, "mass"), (to_mass, "to_mass")):
-        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{name}: expected [seqs, kv_heads, n] with contiguous positions")
-        _need(t, name, torch.float32, cache.device, (cache.seqs, cache.kv_heads, t.shape[2]), contiguous=False)
+    _weights(mass, "mass", cache, cache.seqs, False)
+    _weights(to_mass, "to_mass", cache, cache.seqs, True)
+    to._writable()
     if to_mass.data_ptr() == mass.data_ptr() and mass.numel():
         raise ValueError("to_mass: must not be mass")
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} with {sinks} first and {recent} last positions")
-    with _guard(cache.device):
-        kept = torch.empty((cache.seqs, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
-        new = torch.empty(cache.seqs, dtype=torch.int32, device=cache.device)
-        _lib.check(_lib.lib().er_kv_evict(cache._ref, to._ref, lens.data_ptr(), mass.data_ptr(), mass.stride(0),
-                                          mass.stride(1), mass.shape[2], to_mass.data_ptr(), to_mass.stride(0),
-                                          to_mass.stride(1), to_mass.shape[2], int(budget), int(sinks), int(recent),
-                                          kept.data_ptr(), new.data_ptr(), cache.status.data_ptr(), cache._stream()),
-                   "er_kv_evict")
+    kept = torch.empty((cache.seqs, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
+    new = torch.empty(cache.seqs, dtype=torch.int32, device=cache.device)
+    _lib.check(_lib.lib().er_kv_evict(cache._ref, to._ref, lens.data_ptr(), mass.data_ptr(), mass.stride(0),
+                                      mass.stride(1), mass.shape[2], to_mass.data_ptr(), to_mass.stride(0),
+                                      to_mass.stride(1), to_mass.shape[2], int(budget), int(sinks), int(recent),
+                                      kept.data_ptr(), new.data_ptr(), cache._status, cache._stream()),
+               "er_kv_evict")
     return kept, new

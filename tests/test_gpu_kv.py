@@ -443,6 +443,10 @@ def test_refusals(cuda):
         (lambda: kv.attend(cache, q, lens, out=q[:1]), "out"),
         (lambda: kv.attend(cache, q, lens, pages=_i32([[[0], [0]]] * 2)), "together"),
         (lambda: kv.attend(cache, q, lens, mass=torch.zeros((2, 1, 64), device="cuda")), "mass"),
+        (lambda: kv.attend(cache, q, lens, mass=torch.zeros((1, 2, 64), device="cuda").expand(2, 2, 64)), "share memory"),
+        (lambda: kv.append(kv.PagedKV(cache.k[:1].expand(9, -1, -1, -1), cache.v[:1].expand(9, -1, -1, -1), cache.table),
+                           torch.zeros((2, 512), device="cuda"), lens, 4, 1e4), "share memory"),
+        (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens.long(), 4, 1e4), "positions"),
         (lambda: kv.attend(cache, q, lens, pages=_i32([[[0], [0]]] * 2), counts=_i32([[1, 1]] * 2),
                            mass=torch.zeros((2, 2, 64), device="cuda")), "not accumulated"),
         (lambda: kv.attend(cache, q, lens, workspace=torch.empty(16, dtype=torch.uint8, device="cuda")), "workspace"),
