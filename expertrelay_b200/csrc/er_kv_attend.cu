@@ -33,8 +33,9 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   using TC = float;
   constexpr int V = 16 / sizeof(TC);
   extern __shared__ __align__(16) char sm[];
-  __shared__ long long sums[129];
+  __shared__ long long sums[2 * 129], ends[3];
   __shared__ int where[3], spoiled;
+  __shared__ uint32_t live[4][kSimtStages];  // a stage's keys that exist, its bad ones in the upper half
   const int d = a.kv.d, warps = blockDim.x / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* qs = reinterpret_cast<float*>(sm);                // [GB][d]
   float* merge = qs + GB * d;                              // [warps][GB][d + 2]: m, l, o
@@ -45,57 +46,33 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   int wide = 2;  // lanes across a row; at most 16 rows at a time, so every lane group has as many
   while (wide < cols && wide < 32) wide *= 2;
   const int col = lane % wide, kg = lane / wide, kgs = 32 / wide;
-  const int cw = cols > 32 ? 2 : 1;  // columns a lane
 
   chain_wait();
   Place c;
-  const Run run = kv_run(a, sums, where, c);
-  long long left = run.left;
+  const Run run = kv_run(a, sums, where, ends, c);
+  long long left = run.left, begin = run.begin;
   if (left == 0) return;
 
-  uint32_t live[kSimtStages];  // keys of a stage that exist, bad ones in the upper half
   Place f = c;
   long long ahead = left;
-  auto fetch = [&](int st) {
-    uint32_t mask = 0;
-    if (ahead > 0) {
-      const int j0 = f.t * a.tile + warp * kKvChunk;
-      const int h = f.head(a);
-      const long long off = lane < kKvChunk ? kv_locate(a, f, h, j0 + lane) : -1;
-      mask = __ballot_sync(0xffffffffu, off >= 0) | (__ballot_sync(0xffffffffu, off == -2) << 16);
-      const uint32_t kd = smem_addr(ring + st * 2 * kKvChunk * pitch), vd = kd + kKvChunk * pitch;
-      for (int r = kg; r < kKvChunk; r += kgs) {
-        const long long o = __shfl_sync(0xffffffffu, off, r);
-        const int bytes = o >= 0 ? 16 : 0;
-        const long long at = o >= 0 ? o : 0;
-        for (int w = 0; w < cw; ++w) {
-          const int cc = col + 32 * w;
-          if (cc < cols) {
-            copy16(kd + r * pitch + cc * 16, a.kv.k + at + cc * 16, bytes);
-            copy16(vd + r * pitch + cc * 16, a.kv.v + at + cc * 16, bytes);
-          }
-        }
-      }
-      if (--ahead > 0) f.next(a);
-    }
-    copy_commit();
-    return mask;
-  };
-#pragma unroll
-  for (int s = 0; s < kSimtStages; ++s) live[s] = fetch(s);
-
   float m[GB], l[GB], o[GB][8];
-  bool fresh = true;
-  int st = 0, first_t = 0;
-  bool bad = false;
-  while (left > 0) {
-    const int h = c.head(a), blk = c.block(a), row = c.row(a);
-    const int g0 = blk * GB, live_g = min(GB, a.group - g0);
+  bool fresh = true, bad = false;
+  int st = 0, first_t = 0, filled = 0, row = 0, g0 = 0, live_g = 0;
+  // One loop fills the ring, then takes a stage and fills it again: each
+  // piece of code stands once, since a short launch waits for its
+  // instructions as it does for its data.
+#pragma unroll 1
+  for (;;) {
+    const bool work = filled == kSimtStages;
+    if (work) {
     if (fresh) {  // a new unit: its queries
       fresh = false;
       bad = false;
       first_t = c.t;
-      const TQ* q = (const TQ*)a.q + (long long)row * a.q_stride + (long long)(h * a.group + g0) * d;
+      row = c.row(a);
+      g0 = c.block(a) * GB;
+      live_g = min(GB, a.group - g0);
+      const TQ* q = (const TQ*)a.q + (long long)row * a.q_stride + (long long)(c.head * a.group + g0) * d;
       for (int i = threadIdx.x; i < GB * d; i += blockDim.x) qs[i] = i < live_g * d ? to_f32(q[i]) : 0.f;
       if (threadIdx.x == 0) spoiled = 0;
       __syncthreads();
@@ -109,10 +86,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     }
     copy_wait<kSimtStages - 1>();
     __syncwarp();
-    uint32_t mask = live[0];
-#pragma unroll
-    for (int s = 1; s < kSimtStages; ++s)
-      if (s == st) mask = live[s];
+    const uint32_t mask = live[warp][st];
     if (mask >> 16) bad = true;
     if (mask & 0xffff) {
       const char* kc = ring + st * 2 * kKvChunk * pitch;
@@ -142,7 +116,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
         if (!on) s[g] = -INFINITY;
       }
       if (a.scores && on && lane < 16) {
-        float* to = a.scores + (((long long)row * a.kv.kv_heads + h) * a.mass_len + c.t * a.tile + warp * kKvChunk + key) *
+        float* to = a.scores + (((long long)row * a.kv.kv_heads + c.head) * a.mass_len + c.t * a.tile + warp * kKvChunk + key) *
                                    a.group + g0;
 #pragma unroll
         for (int g = 0; g < GB; ++g)
@@ -185,13 +159,38 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       }
     }
     __syncwarp();
-    const uint32_t got = fetch(st);
+    }
+    if (ahead > 0) {  // the stage's next chunk
+      const long long off =
+          lane < kKvChunk ? kv_locate(a, f, f.t * a.tile + warp * kKvChunk + lane) : -1;
+      const uint32_t keys =
+          __ballot_sync(0xffffffffu, off >= 0) | (__ballot_sync(0xffffffffu, off == -2) << 16);
+      if (lane == 0) live[warp][st] = keys;
+      const uint32_t kd = smem_addr(ring + st * 2 * kKvChunk * pitch), vd = kd + kKvChunk * pitch;
+#pragma unroll 1
+      for (int r = kg; r < kKvChunk; r += kgs) {
+        const long long at = __shfl_sync(0xffffffffu, off, r);
+        const int bytes = at >= 0 ? 16 : 0;
+        const char *kp = a.kv.k + (at >= 0 ? at : 0), *vp = a.kv.v + (at >= 0 ? at : 0);
 #pragma unroll
-    for (int s = 0; s < kSimtStages; ++s)
-      if (s == st) live[s] = got;
+        for (int w = 0; w < 2; ++w) {
+          const int cc = col + 32 * w;
+          if (cc < cols) {
+            copy16(kd + r * pitch + cc * 16, kp + cc * 16, bytes);
+            copy16(vd + r * pitch + cc * 16, vp + cc * 16, bytes);
+          }
+        }
+      }
+      if (--ahead > 0) f.next(a);
+    }
+    copy_commit();
     st = st + 1 == kSimtStages ? 0 : st + 1;
+    if (!work) {
+      ++filled;
+      continue;
+    }
     --left;
-    const int t = c.t, tiles = c.tiles;
+    const int t = c.t, tiles = c.tiles, h = c.head;
     if (t + 1 < tiles && left > 0) {
       ++c.t;
       continue;
@@ -220,8 +219,8 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     if (bad && lane == 0) spoiled = 1;
     __syncthreads();
     const bool whole = first_t == 0 && t + 1 == tiles;
-    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind (the run's last tile is tile t)
-      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, run.begin + run.left - (t + 1), run.total};
+    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
+      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, begin, run.total};
     const bool nan = spoiled != 0;
     if (nan && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
     for (int i = threadIdx.x; i < GB * d; i += blockDim.x) {
@@ -251,8 +250,10 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       }
     }
     __syncthreads();
+    if (left == 0) return;
     fresh = true;
-    if (left > 0) c.next(a);
+    begin += kv_cost(tiles);
+    c.next(a);
   }
 }
 
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   const CutUnit c = a.cut[blockIdx.x];
   if (c.row < 0 || c.g0 + g >= a.group) return;
   const int shares = kv_shares(a, c.total), i0 = blockIdx.x;
-  const int n = kv_share_of(c.total, shares, c.begin + c.tiles - 1) - i0 + 1;  // pieces
+  const int n = kv_share_of(c.total, shares, c.begin + kUnitCost + c.tiles - 1) - i0 + 1;  // pieces
   auto piece = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * gb + g; };
   float top = -INFINITY, sum = 0.f;
   for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, a.part_ml[piece(k) * 2]);
@@ -478,7 +479,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     a.shift = -1;
     for (int b = 0; b < 31; ++b)
       if (cache->page_size == 1 << b) a.shift = b;
-    a.min_tiles = 2;
+    a.min_share = kUnitCost + 2;
     a.status = io->status;
     a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;
     a.units = io->pages ? L.blocks : cache->kv_heads * L.blocks;

@@ -23,7 +23,7 @@ constexpr int kKvChunk = 16;  // keys a warp takes at a time
 struct CutUnit {
   int row, head, g0;  // row -1: none begins here and ends behind
   int tiles;
-  long long begin, total;  // its first tile, and all tiles of the launch
+  long long begin, total;  // the unit's place in the line, and the line's length
 };
 
 struct AttendArgs {
@@ -41,7 +41,7 @@ struct AttendArgs {
   int max_pages;
   int tile;                    // keys a tile: warps a CTA * kKvChunk
   int shift;                   // log2 of page_size, -1 when it is no power of two
-  int min_tiles;               // fewest tiles worth a CTA
+  int min_share;               // the least share of the line worth a CTA
   int* status;
   // scan entries: rows, or (row, key head) pairs when each has its own page list
   int entries, units;          // units of one entry: the tiles repeat that often
@@ -62,7 +62,7 @@ struct Entry {
   int bad;  // ER_KV_BAD_* bits
 };
 
-__device__ __forceinline__ Entry kv_entry(const AttendArgs& a, int x) {
+static __device__ __noinline__ Entry kv_entry(const AttendArgs& a, int x) {
   const int row = a.pages ? x / a.kv.kv_heads : x;
   Entry e;
   e.seq = a.seqs ? a.seqs[row] : row;
@@ -86,121 +86,156 @@ __device__ __forceinline__ Entry kv_entry(const AttendArgs& a, int x) {
 
 __device__ __forceinline__ int kv_tiles(const AttendArgs& a, int n) { return (n + a.tile - 1) / a.tile; }
 
-// CTAs that share `total` tiles, the first tile of CTA i, and the CTA that has tile x.
+// The line that the CTAs share: a unit of c > 0 tiles takes kUnitCost + c of
+// it, for its queries, the joining of its warps and its result cost about
+// that many tiles beside the tiles themselves. (48 rows of 1 .. 4097 keys and
+// 16 heads, shares by tiles alone: the CTAs with the short rows ran on for 21 % of
+// the kernel after the others.)
+constexpr int kUnitCost = 3;
+__device__ __forceinline__ int kv_cost(int tiles) { return tiles ? tiles + kUnitCost : 0; }
+
+// 64-bit division as a call: inlined, each is a hundred instructions that
+// a short launch would fetch for the first time.
+static __device__ __noinline__ long long kv_div(long long a, long long b) { return a / b; }
 __device__ __forceinline__ int kv_shares(const AttendArgs& a, long long total) {
-  const long long s = (total + a.min_tiles - 1) / a.min_tiles;
-  return (int)(s < a.grid ? s : a.grid);
+  return total < (long long)a.grid * a.min_share ? ((int)total + a.min_share - 1) / a.min_share : a.grid;
 }
-__device__ __forceinline__ long long kv_share_start(long long total, int shares, int i) { return total * i / shares; }
+// where share i begins, and the share that place x lies in
+__device__ __forceinline__ long long kv_share_start(long long total, int shares, int i) {
+  return kv_div(total * i, shares);
+}
 __device__ __forceinline__ int kv_share_of(long long total, int shares, long long x) {
-  return (int)(((x + 1) * shares - 1) / total);
+  return (int)kv_div((x + 1) * shares - 1, total);
 }
 
-// A place in the line of tiles: entry x, unit u of it, tile t of that unit.
+// A tile: entry x, unit u of it, tile t of that unit's.
 struct Place {
-  int x, u, t, tiles;
+  int x, u, t, tiles, head;  // head: key head
   Entry e;
 
-  __device__ __forceinline__ void load(const AttendArgs& a, int entry) {
+  __device__ __forceinline__ void set(const AttendArgs& a, int entry, int unit, int tile) {
     x = entry;
+    u = unit;
+    t = tile;
     e = kv_entry(a, x);
     tiles = kv_tiles(a, e.n);
+    head = a.pages ? x % a.kv.kv_heads : u / a.blocks;
   }
   // The next tile; the caller knows that there is one.
   __device__ __forceinline__ void next(const AttendArgs& a) {
     if (++t < tiles) return;
-    t = 0;
-    if (++u < a.units) return;
-    u = 0;
-    do load(a, x + 1);
-    while (tiles == 0);
+    int y = x, v = u + 1;
+    if (v == a.units) {
+      v = 0;
+      do ++y;
+      while (kv_entry(a, y).n == 0);
+    }
+    set(a, y, v, 0);
   }
   __device__ __forceinline__ int row(const AttendArgs& a) const { return a.pages ? x / a.kv.kv_heads : x; }
-  __device__ __forceinline__ int head(const AttendArgs& a) const {  // key head
-    return a.pages ? x % a.kv.kv_heads : u / a.blocks;
-  }
   __device__ __forceinline__ int block(const AttendArgs& a) const { return u % a.blocks; }  // head block of the group
 };
 
-// The CTA's run of tiles: its first place and how many tiles it has. Every
-// CTA sums the entries' tiles itself (a few loads a thread). `sums`: blockDim.x + 1 long longs, shared.
+// What a CTA works through: `left` tiles from a place on; `begin` is where
+// the first tile's unit begins in the line of length `total`.
 struct Run {
-  long long begin, left, total;
+  long long left, begin, total;
 };
-__device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int* where, Place& p) {
-  if (threadIdx.x == 0) a.cut[blockIdx.x].row = -1;
-  const int per = (a.entries + blockDim.x - 1) / blockDim.x;
+
+// Every CTA sums the entries' costs itself (a few loads a thread) and finds
+// its share's ends. `sums`: 2 (blockDim.x + 1) long longs, `where`: 3 ints,
+// `ends`: 3 long longs, shared.
+__device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int* where, long long* ends, Place& p) {
+  const int threads = blockDim.x;
+  if (threadIdx.x == 0) {
+    a.cut[blockIdx.x].row = -1;
+    sums[0] = sums[threads + 1] = 0;
+  }
+  const int per = (a.entries + threads - 1) / threads;
   const int x0 = min(a.entries, (int)threadIdx.x * per), x1 = min(a.entries, x0 + per);
-  long long mine = 0;
+  long long cost = 0, tiles = 0;
+#pragma unroll 1
   for (int x = x0; x < x1; ++x) {
     const Entry e = kv_entry(a, x);
-    mine += kv_tiles(a, e.n);
+    const int c = kv_tiles(a, e.n);
+    tiles += c;
+    cost += kv_cost(c);
     if (blockIdx.x == 0 && e.bad) kv_report(a.status, e.bad);
   }
-  sums[threadIdx.x + 1] = mine;
-  if (threadIdx.x == 0) sums[0] = 0;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const int each = blockDim.x / 32, l = threadIdx.x;
-    long long s = 0;
-    for (int i = 0; i < each; ++i) s += sums[1 + l * each + i];
-    long long inc = s;
+  long long* tsum = sums + threads + 1;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (l >= o) inc += up;
-    }
-    long long run = inc - s;
-    for (int i = 0; i < each; ++i) {
-      run += sums[1 + l * each + i];
-      sums[1 + l * each + i] = run;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long uc = __shfl_up_sync(0xffffffffu, cost, o), ut = __shfl_up_sync(0xffffffffu, tiles, o);
+    if (lane >= o) {
+      cost += uc;
+      tiles += ut;
     }
   }
+  sums[threadIdx.x + 1] = cost;
+  tsum[threadIdx.x + 1] = tiles;
   __syncthreads();
-  const long long per_unit = sums[blockDim.x], total = per_unit * a.units;
+  long long c0 = 0, t0 = 0, all = 0, all_tiles = 0;  // before this warp, and in all
+#pragma unroll 1
+  for (int w = 1; w <= threads / 32; ++w) {
+    if (w == (int)threadIdx.x / 32 + 1) {
+      c0 = all;
+      t0 = all_tiles;
+    }
+    all += sums[w * 32];
+    all_tiles += tsum[w * 32];
+  }
+  const long long total = all * a.units;
   if (total == 0) return Run{0, 0, 0};
   const int shares = kv_shares(a, total);
   if ((int)blockIdx.x >= shares) return Run{0, 0, total};
-  const long long begin = kv_share_start(total, shares, blockIdx.x);
-  const long long end = kv_share_start(total, shares, blockIdx.x + 1);
-  // the entry whose units hold tile `begin`: all units of the entries before it are passed
-  const long long ex = sums[threadIdx.x] * a.units, in = sums[threadIdx.x + 1] * a.units;
-  if (ex <= begin && begin < in) {
-    long long rest = begin - ex;
+  // this thread's entries: the line from ex on, `tb` tiles before it
+  const long long ex = (c0 + (lane ? sums[threadIdx.x] : 0)) * a.units, in = (c0 + cost) * a.units;
+  const long long tb = (t0 + (lane ? tsum[threadIdx.x] : 0)) * a.units;
+#pragma unroll 1
+  for (int end = 0; end < 2; ++end) {
+    const long long at = kv_share_start(total, shares, blockIdx.x + end);
+    if (at == total && threadIdx.x == 0) ends[1] = all_tiles * a.units;
+    if (at < ex || at >= in) continue;
+    long long rest = at - ex, before = tb;
+#pragma unroll 1
     for (int x = x0; x < x1; ++x) {
-      const long long c = kv_tiles(a, kv_entry(a, x).n);
-      if (rest < c * a.units) {
-        where[0] = x;
-        where[1] = (int)(rest / c);
-        where[2] = (int)(rest % c);
+      const int c = kv_tiles(a, kv_entry(a, x).n), k = kv_cost(c);
+      if (rest < (long long)k * a.units) {
+        const int u = (int)kv_div(rest, k), in_unit = (int)(rest - (long long)u * k), t = max(0, in_unit - kUnitCost);
+        ends[end] = before + (long long)u * c + t;
+        if (end == 0) {
+          where[0] = x;
+          where[1] = u;
+          where[2] = t;
+          ends[2] = at - in_unit;
+        }
         break;
       }
-      rest -= c * a.units;
+      rest -= (long long)k * a.units;
+      before += (long long)c * a.units;
     }
   }
   __syncthreads();
-  p.load(a, where[0]);
-  p.u = where[1];
-  p.t = where[2];
-  return Run{begin, end - begin, total};
+  p.set(a, where[0], where[1], where[2]);
+  return Run{ends[1] - ends[0], ends[2], total};
 }
 
-// Where key j of a place lies: byte offset of its slot (key head included)
-// in the pools, or -1 when there is no such key (behind the length, a list's
-// page behind it) and -2 when its page id is bad.
-__device__ __forceinline__ long long kv_locate(const AttendArgs& a, const Place& p, int h, int j) {
+// Where key j of a place lies: byte offset of its slot in the pools, or -1
+// when there is no such key (behind the length, a list's page behind it) and
+// -2 when its page id is bad.
+__device__ __forceinline__ long long kv_locate(const AttendArgs& a, const Place& p, int j) {
   if (j >= p.e.n) return -1;
-  const int ps = a.kv.page_size;
-  int o = j / ps;
-  const int slot = j - o * ps;
+  int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
+  const int slot = j - o * a.kv.page_size;
   if (a.pages) {
     o = a.pages[(long long)p.x * a.max_pages + o];
     if (o < 0 || o >= a.kv.width) return -2;
-    if ((long long)o * ps + slot >= p.e.len) return -1;
+    if ((long long)o * a.kv.page_size + slot >= p.e.len) return -1;
   }
   const int page = a.kv.pages_of(p.e.seq)[o];
   if (page < 0 || page >= a.kv.num_pages) return -2;
-  return page * a.kv.page_stride + h * a.kv.head_stride + slot * a.kv.slot_stride;
+  return page * a.kv.page_stride + p.head * a.kv.head_stride + slot * a.kv.slot_stride;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -110,8 +110,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
   using Ring = MmaRing<DP, NT, QS>;
   constexpr int S = Ring::kStages, KS = DP / 16, PS = QS == 1 ? 2 : 3;
   extern __shared__ __align__(128) char sm[];
-  __shared__ long long sums[kMmaWarps * 32 + 1];
+  __shared__ long long sums[2 * (kMmaWarps * 32 + 1)], ends[3];
   __shared__ int where[3], spoiled;
+  __shared__ uint32_t live[kMmaWarps][S];  // a stage's keys that exist, its bad ones in the upper half
   const int d = a.kv.d, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   char* ring = sm + warp * S * 2 * Ring::kChunkBytes;
   uint2* qf = reinterpret_cast<uint2*>(sm + Ring::kBytes);               // [KS][QS][NT][32]
@@ -129,19 +130,17 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
   }
   chain_wait();
   Place c;
-  const Run run = kv_run(a, sums, where, c);
-  long long left = run.left;
+  const Run run = kv_run(a, sums, where, ends, c);
+  long long left = run.left, begin = run.begin;
   if (left == 0) return;
 
   Place f = c;
   long long ahead = left;
-  uint32_t live[S];
   // The page of the next chunk's key `lane` is loaded a step before it is
   // used: what (0: no key, 1: page id, 2: bad), page, slot.
   int what = 0, page = 0, slot = 0;
   auto peek = [&]() {
     what = 0;
-    if (ahead <= 0) return;
     const int j = f.t * a.tile + warp * kKvChunk + lane;
     if (lane >= kKvChunk || j >= f.e.n) return;
     int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
@@ -157,45 +156,27 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     what = 1;
     page = a.kv.pages_of(f.e.seq)[o];
   };
-  auto fetch = [&](int st) {
-    uint32_t mask = 0;
-    if (ahead > 0) {
-      const bool in = what == 1 && page >= 0 && page < a.kv.num_pages;
-      const long long off =
-          in ? page * a.kv.page_stride + f.head(a) * a.kv.head_stride + slot * a.kv.slot_stride : -1;
-      mask = __ballot_sync(0xffffffffu, in) | (__ballot_sync(0xffffffffu, what == 2 || (what == 1 && !in)) << 16);
-      const uint32_t kd = smem_addr(ring + st * 2 * Ring::kChunkBytes), vd = kd + Ring::kChunkBytes;
-#pragma unroll
-      for (int i = 0; i < kKvChunk / KG; ++i) {
-        const int r = i * KG + kg;
-        const long long o = __shfl_sync(0xffffffffu, off, r);
-        const int bytes = o >= 0 ? 16 : 0;
-        const long long at = (o >= 0 ? o : 0) + col * 16;
-        if (col < cols) {
-          copy16(kd + swz<DP>(r, col), a.kv.k + at, bytes);
-          copy16(vd + swz<DP>(r, col), a.kv.v + at, bytes);
-        }
-      }
-      if (--ahead > 0) f.next(a);
-      peek();
-    }
-    copy_commit();
-    return mask;
-  };
   peek();
-#pragma unroll
-  for (int s = 0; s < S; ++s) live[s] = fetch(s);
 
   float m[NT][2], l[NT][2], o[KS][NT][4];
   bool fresh = true, bad = false;
-  int st = 0, first_t = 0;
-  while (left > 0) {
-    const int h = c.head(a), row = c.row(a), g0 = c.block(a) * NT * 8, live_g = min(NT * 8, a.group - g0);
+  int st = 0, first_t = 0, row = 0, g0 = 0, live_g = 0, filled = 0;
+  // One loop fills the ring (S steps), then takes a stage and fills it again:
+  // each piece of code stands once, since a short launch waits for its
+  // instructions as it does for its data.
+#pragma unroll 1
+  for (;;) {
+    const bool work = filled == S;
+    if (work) {
     if (fresh) {  // a new unit: its queries in the matrix instructions' order
       fresh = false;
       bad = false;
       first_t = c.t;
-      const long long qat = (long long)row * a.q_stride + (long long)(h * a.group + g0) * d;
+      row = c.row(a);
+      g0 = c.block(a) * NT * 8;
+      live_g = min(NT * 8, a.group - g0);
+      const long long qat = (long long)row * a.q_stride + (long long)(c.head * a.group + g0) * d;
+#pragma unroll 1
       for (int i = threadIdx.x; i < KS * QS * NT * 32; i += kMmaWarps * 32) {
         const int ln = i % 32, nt = i / 32 % NT, part = i / (32 * NT) % QS, ks = i / (32 * NT * QS);
         const int g = nt * 8 + ln / 4, c0 = ks * 16 + ln % 4 * 2;
@@ -223,10 +204,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     }
     copy_wait<S - 1>();
     __syncwarp();
-    uint32_t mask = live[0];
-#pragma unroll
-    for (int s = 1; s < S; ++s)
-      if (s == st) mask = live[s];
+    const uint32_t mask = live[warp][st];
     if (mask >> 16) bad = true;
     if (mask & 0xffff) {
       const uint32_t kc = smem_addr(ring + st * 2 * Ring::kChunkBytes), vc = kc + Ring::kChunkBytes;
@@ -262,12 +240,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
           if (!(e < 2 ? on0 : on1)) s[e] = -INFINITY;
         }
         if (a.scores) {
-          const long long at = ((long long)row * a.kv.kv_heads + h) * a.mass_len + c.t * a.tile + warp * kKvChunk + lane / 4;
           const int g = nt * 8 + lane % 4 * 2;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if ((e < 2 ? on0 : on1) && g + (e & 1) < live_g)
-              a.scores[(at + (e >> 1) * 8) * a.group + g0 + g + (e & 1)] = s[e];
+          float* to = a.scores + (((long long)row * a.kv.kv_heads + c.head) * a.mass_len + c.t * a.tile + warp * kKvChunk +
+                                  lane / 4) * a.group + g0 + g;
+          if (on0 && g < live_g) to[0] = s[0];
+          if (on0 && g + 1 < live_g) to[1] = s[1];
+          to += 8 * a.group;
+          if (on1 && g < live_g) to[0] = s[2];
+          if (on1 && g + 1 < live_g) to[1] = s[3];
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -341,13 +321,38 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       }
     }
     __syncwarp();
-    const uint32_t got = fetch(st);
+    }
+    if (ahead > 0) {  // the stage's next chunk
+      const bool in = what == 1 && page >= 0 && page < a.kv.num_pages;
+      const long long off = in ? page * a.kv.page_stride + f.head * a.kv.head_stride + slot * a.kv.slot_stride : -1;
+      const uint32_t keys = __ballot_sync(0xffffffffu, in) |
+                            (__ballot_sync(0xffffffffu, what == 2 || (what == 1 && !in)) << 16);
+      if (lane == 0) live[warp][st] = keys;
+      const uint32_t kd = smem_addr(ring + st * 2 * Ring::kChunkBytes), vd = kd + Ring::kChunkBytes;
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-      if (s == st) live[s] = got;
+      for (int i = 0; i < kKvChunk / KG; ++i) {
+        const int r = i * KG + kg;
+        const long long o = __shfl_sync(0xffffffffu, off, r);
+        const int bytes = o >= 0 ? 16 : 0;
+        const long long at = (o >= 0 ? o : 0) + col * 16;
+        if (col < cols) {
+          copy16(kd + swz<DP>(r, col), a.kv.k + at, bytes);
+          copy16(vd + swz<DP>(r, col), a.kv.v + at, bytes);
+        }
+      }
+      if (--ahead > 0) {
+        f.next(a);
+        peek();
+      }
+    }
+    copy_commit();
     st = st + 1 == S ? 0 : st + 1;
+    if (!work) {
+      ++filled;
+      continue;
+    }
     --left;
-    const int t = c.t, tiles = c.tiles;
+    const int t = c.t, tiles = c.tiles, h = c.head;
     if (t + 1 < tiles && left > 0) {
       ++c.t;
       continue;
@@ -367,23 +372,23 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       }
     if (bad && lane == 0) spoiled = 1;
     const bool whole = first_t == 0 && t + 1 == tiles;
-    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind (the run's last tile is tile t)
-      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, run.begin + run.left - (t + 1), run.total};
-#pragma unroll
-    for (int q4 = 0; q4 < NT * 8 / kMergeHeads; ++q4) {
-      if (q4 * kMergeHeads >= live_g) break;
-      const int nt = q4 / 2;
+    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
+      a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, begin, run.total};
+#pragma unroll 1
+    for (int q4 = 0; q4 * kMergeHeads < live_g; ++q4) {
       if (lane % 4 / 2 == q4 % 2) {
         float* to = merge + (warp * kMergeHeads + lane % 2 * 2) * DP + lane / 4;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) to[(e & 1) * DP + k * 16 + (e >> 1) * 8] = o[k][nt][e];
+          for (int e = 0; e < 4; ++e)
+            to[(e & 1) * DP + k * 16 + (e >> 1) * 8] = NT > 1 && q4 >= 2 ? o[k][NT - 1][e] : o[k][0][e];
         }
       }
       __syncthreads();
       const bool nan = spoiled != 0;
       if (nan && q4 == 0 && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
+#pragma unroll 1
       for (int i = threadIdx.x; i < kMergeHeads * DP; i += kMmaWarps * 32) {
         const int g4 = i / DP, cc = i % DP, g = q4 * kMergeHeads + g4;
         if (g >= live_g || cc >= d) continue;
@@ -416,8 +421,10 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       }
       __syncthreads();
     }
+    if (left == 0) return;
     fresh = true;
-    if (left > 0) c.next(a);
+    begin += kv_cost(tiles);
+    c.next(a);
   }
 }
 
