@@ -28,14 +28,14 @@ inline KernelShape simt_shape(int d, int group) {
 // asynchronous copies. Scores: lane l holds key l % 16 and half of the
 // columns. Values: the lanes split a row's 16-byte columns, lane groups the
 // keys. GB queries of the group at a time share each key that is read.
-template <typename TQ, int GB>
+template <typename TQ, int GB, bool WHOLE>
 __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_constant__ AttendArgs a, int pitch) {
   using TC = float;
   constexpr int V = 16 / sizeof(TC);
   extern __shared__ __align__(16) char sm[];
-  __shared__ long long sums[2 * 129], ends[3];
-  __shared__ int where[3], spoiled;
-  __shared__ uint32_t live[4][kSimtStages];  // a stage's keys that exist, its bad ones in the upper half
+  __shared__ RunScratch scratch;
+  __shared__ int spoiled;
+  __shared__ StageInfo info[4][kSimtStages];
   const int d = a.kv.d, warps = blockDim.x / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* qs = reinterpret_cast<float*>(sm);                // [GB][d]
   float* merge = qs + GB * d;                              // [warps][GB][d + 2]: m, l, o
@@ -48,31 +48,29 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   const int col = lane % wide, kg = lane / wide, kgs = 32 / wide;
 
   chain_wait();
-  Place c;
-  const Run run = kv_run(a, sums, where, ends, c);
+  const Run run = kv_run(a, scratch);
+  if (run.left == 0) return;
   long long left = run.left, begin = run.begin;
-  if (left == 0) return;
+  Walk<WHOLE> walk(a, run);
 
-  Place f = c;
-  long long ahead = left;
   float m[GB], l[GB], o[GB][8];
   bool fresh = true, bad = false;
-  int st = 0, first_t = 0, filled = 0, row = 0, g0 = 0, live_g = 0;
+  int st = 0, first_t = 0, filled = 0, live_g = 0;
   // One loop fills the ring, then takes a stage and fills it again: each
   // piece of code stands once, since a short launch waits for its
   // instructions as it does for its data.
 #pragma unroll 1
   for (;;) {
     const bool work = filled == kSimtStages;
+    StageInfo now = {};
     if (work) {
+    now = info[warp][st];
     if (fresh) {  // a new unit: its queries
       fresh = false;
       bad = false;
-      first_t = c.t;
-      row = c.row(a);
-      g0 = c.block(a) * GB;
-      live_g = min(GB, a.group - g0);
-      const TQ* q = (const TQ*)a.q + (long long)row * a.q_stride + (long long)(c.head * a.group + g0) * d;
+      first_t = now.t;
+      live_g = min(GB, a.group - now.g0);
+      const TQ* q = (const TQ*)a.q + (long long)now.row * a.q_stride + (long long)(now.head * a.group + now.g0) * d;
       for (int i = threadIdx.x; i < GB * d; i += blockDim.x) qs[i] = i < live_g * d ? to_f32(q[i]) : 0.f;
       if (threadIdx.x == 0) spoiled = 0;
       __syncthreads();
@@ -86,7 +84,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     }
     copy_wait<kSimtStages - 1>();
     __syncwarp();
-    const uint32_t mask = live[warp][st];
+    const uint32_t mask = now.keys;
     if (mask >> 16) bad = true;
     if (mask & 0xffff) {
       const char* kc = ring + st * 2 * kKvChunk * pitch;
@@ -116,8 +114,8 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
         if (!on) s[g] = -INFINITY;
       }
       if (a.scores && on && lane < 16) {
-        float* to = a.scores + (((long long)row * a.kv.kv_heads + c.head) * a.mass_len + c.t * a.tile + warp * kKvChunk + key) *
-                                   a.group + g0;
+        float* to = a.scores + (((long long)now.row * a.kv.kv_heads + now.head) * a.mass_len + now.t * a.tile +
+                                warp * kKvChunk + key) * a.group + now.g0;
 #pragma unroll
         for (int g = 0; g < GB; ++g)
           if (g < live_g) to[g] = s[g];
@@ -127,10 +125,10 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
         float top = s[g];
 #pragma unroll
         for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float now = fmaxf(m[g], top);
-        const float base = now == -INFINITY ? 0.f : now;  // scores of -inf alone weigh nothing
+        const float high = fmaxf(m[g], top);
+        const float base = high == -INFINITY ? 0.f : high;  // scores of -inf alone weigh nothing
         const float keep = exp2f(m[g] - base);
-        m[g] = now;
+        m[g] = high;
         const float p = on ? exp2f(s[g] - base) : 0.f;
         l[g] = l[g] * keep + (lane < 16 ? p : 0.f);
         if (lane < 16) prob[key * GB + g] = p;
@@ -160,28 +158,27 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     }
     __syncwarp();
     }
-    if (ahead > 0) {  // the stage's next chunk
-      const long long off =
-          lane < kKvChunk ? kv_locate(a, f, f.t * a.tile + warp * kKvChunk + lane) : -1;
-      const uint32_t keys =
-          __ballot_sync(0xffffffffu, off >= 0) | (__ballot_sync(0xffffffffu, off == -2) << 16);
-      if (lane == 0) live[warp][st] = keys;
+    if (walk.ahead > 0) {  // the stage's next chunk
+      long long off = 0;
+      const uint32_t keys = walk.chunk(a, &off);
+      walk.note(a, keys, GB, &info[warp][st]);
       const uint32_t kd = smem_addr(ring + st * 2 * kKvChunk * pitch), vd = kd + kKvChunk * pitch;
-#pragma unroll 1
+#pragma unroll 4
       for (int r = kg; r < kKvChunk; r += kgs) {
-        const long long at = __shfl_sync(0xffffffffu, off, r);
-        const int bytes = at >= 0 ? 16 : 0;
-        const char *kp = a.kv.k + (at >= 0 ? at : 0), *vp = a.kv.v + (at >= 0 ? at : 0);
+        const long long at = WHOLE ? off + r * a.kv.slot_stride : __shfl_sync(0xffffffffu, off, r);
+        const int bytes = (keys >> r) & 1 ? 16 : 0;
+        // a key that is not there is not read: its address is the pool's first
+        const char *kp = a.kv.k + (bytes ? at : 0), *vp = a.kv.v + (bytes ? at : 0);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const int cc = col + 32 * w;
           if (cc < cols) {
-            copy16(kd + r * pitch + cc * 16, kp + cc * 16, bytes);
-            copy16(vd + r * pitch + cc * 16, vp + cc * 16, bytes);
+            copy16(kd + r * pitch + cc * 16, kp + (bytes ? cc * 16 : 0), bytes);
+            copy16(vd + r * pitch + cc * 16, vp + (bytes ? cc * 16 : 0), bytes);
           }
         }
       }
-      if (--ahead > 0) f.next(a);
+      walk.next(a);
     }
     copy_commit();
     st = st + 1 == kSimtStages ? 0 : st + 1;
@@ -190,18 +187,16 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       continue;
     }
     --left;
-    const int t = c.t, tiles = c.tiles, h = c.head;
-    if (t + 1 < tiles && left > 0) {
-      ++c.t;
-      continue;
-    }
+    const int t = now.t, tiles = now.tiles, h = now.head, row = now.row, g0 = now.g0;
+    if (t + 1 < tiles && left > 0) continue;
     // the unit ends here, or the CTA's part of it: the warps' pieces join
 #pragma unroll
     for (int g = 0; g < GB; ++g) {
       l[g] = warp_sum(l[g]);
+#pragma unroll 1
+      for (int x = wide; x < 32; x *= 2)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        for (int x = wide; x < 32; x *= 2) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], x);
+        for (int e = 0; e < 8; ++e) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], x);
       float* to = merge + (warp * GB + g) * (d + 2);
       if (lane == 0) {
         to[0] = m[g];
@@ -223,12 +218,15 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, begin, run.total};
     const bool nan = spoiled != 0;
     if (nan && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
+#pragma unroll 1
     for (int i = threadIdx.x; i < GB * d; i += blockDim.x) {
       const int g = i / d, cc = i % d;
       if (g >= live_g) continue;
       const float* from = merge + g * (d + 2);
       float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll 1
       for (int w = 0; w < warps; ++w) top = fmaxf(top, from[w * GB * (d + 2)]);
+#pragma unroll 1
       for (int w = 0; w < warps; ++w) {
         const float* p = from + w * GB * (d + 2);
         const float by = piece_weight(p[0], top);
@@ -253,7 +251,6 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     if (left == 0) return;
     fresh = true;
     begin += kv_cost(tiles);
-    c.next(a);
   }
 }
 
@@ -358,13 +355,18 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
 
 namespace {
 
-template <typename TQ, int GB>
-int simt_go(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
-  auto kernel = kv_attend_simt_kernel<TQ, GB>;
+template <typename TQ, int GB, bool WHOLE>
+int simt_launch(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
+  auto kernel = kv_attend_simt_kernel<TQ, GB, WHOLE>;
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, 224 * 1024, done)) return rc;
   return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a,
                         simt_pitch(a.kv.d));
+}
+
+template <typename TQ, int GB>
+int simt_go(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
+  return a.kv.page_size % kKvChunk ? simt_launch<TQ, GB, false>(a, s, st) : simt_launch<TQ, GB, true>(a, s, st);
 }
 
 template <typename TQ>
@@ -479,7 +481,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     a.shift = -1;
     for (int b = 0; b < 31; ++b)
       if (cache->page_size == 1 << b) a.shift = b;
-    a.min_share = kUnitCost + 2;
+    a.min_share = 2;
     a.status = io->status;
     a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;
     a.units = io->pages ? L.blocks : cache->kv_heads * L.blocks;

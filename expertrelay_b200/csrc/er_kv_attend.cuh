@@ -62,7 +62,7 @@ struct Entry {
   int bad;  // ER_KV_BAD_* bits
 };
 
-static __device__ __noinline__ Entry kv_entry(const AttendArgs& a, int x) {
+__device__ __forceinline__ Entry kv_entry(const AttendArgs& a, int x) {
   const int row = a.pages ? x / a.kv.kv_heads : x;
   Entry e;
   e.seq = a.seqs ? a.seqs[row] : row;
@@ -94,9 +94,12 @@ __device__ __forceinline__ int kv_tiles(const AttendArgs& a, int n) { return (n 
 constexpr int kUnitCost = 3;
 __device__ __forceinline__ int kv_cost(int tiles) { return tiles ? tiles + kUnitCost : 0; }
 
-// 64-bit division as a call: inlined, each is a hundred instructions that
-// a short launch would fetch for the first time.
-static __device__ __noinline__ long long kv_div(long long a, long long b) { return a / b; }
+// 64-bit division as a call (inlined, each is a hundred instructions that a
+// short launch would fetch for the first time), 32-bit where that is enough.
+static __device__ __noinline__ long long kv_div(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
 __device__ __forceinline__ int kv_shares(const AttendArgs& a, long long total) {
   return total < (long long)a.grid * a.min_share ? ((int)total + a.min_share - 1) / a.min_share : a.grid;
 }
@@ -108,62 +111,41 @@ __device__ __forceinline__ int kv_share_of(long long total, int shares, long lon
   return (int)kv_div((x + 1) * shares - 1, total);
 }
 
-// A tile: entry x, unit u of it, tile t of that unit's.
-struct Place {
-  int x, u, t, tiles, head;  // head: key head
-  Entry e;
-
-  __device__ __forceinline__ void set(const AttendArgs& a, int entry, int unit, int tile) {
-    x = entry;
-    u = unit;
-    t = tile;
-    e = kv_entry(a, x);
-    tiles = kv_tiles(a, e.n);
-    head = a.pages ? x % a.kv.kv_heads : u / a.blocks;
-  }
-  // The next tile; the caller knows that there is one.
-  __device__ __forceinline__ void next(const AttendArgs& a) {
-    if (++t < tiles) return;
-    int y = x, v = u + 1;
-    if (v == a.units) {
-      v = 0;
-      do ++y;
-      while (kv_entry(a, y).n == 0);
-    }
-    set(a, y, v, 0);
-  }
-  __device__ __forceinline__ int row(const AttendArgs& a) const { return a.pages ? x / a.kv.kv_heads : x; }
-  __device__ __forceinline__ int block(const AttendArgs& a) const { return u % a.blocks; }  // head block of the group
-};
-
-// What a CTA works through: `left` tiles from a place on; `begin` is where
-// the first tile's unit begins in the line of length `total`.
+// A CTA's run of tiles: the first one (entry x, unit u of it, tile t of the
+// `tiles` of that unit), how many, and where the first one's unit begins in
+// the line of length `total`.
 struct Run {
+  int x, u, t, tiles;
+  Entry e;
   long long left, begin, total;
+};
+struct RunScratch {  // shared memory of kv_run
+  long long cost[4], tiles[4];  // by warp
+  Run run;
+  long long before[2];  // tiles before the run, and before its end
 };
 
 // Every CTA sums the entries' costs itself (a few loads a thread) and finds
-// its share's ends. `sums`: 2 (blockDim.x + 1) long longs, `where`: 3 ints,
-// `ends`: 3 long longs, shared.
-__device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int* where, long long* ends, Place& p) {
-  const int threads = blockDim.x;
+// its share's two ends.
+__device__ __forceinline__ Run kv_run(const AttendArgs& a, RunScratch& s) {
+  const int threads = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     a.cut[blockIdx.x].row = -1;
-    sums[0] = sums[threads + 1] = 0;
+    s.before[0] = s.before[1] = 0;
   }
   const int per = (a.entries + threads - 1) / threads;
   const int x0 = min(a.entries, (int)threadIdx.x * per), x1 = min(a.entries, x0 + per);
   long long cost = 0, tiles = 0;
+  Entry e = {};
 #pragma unroll 1
   for (int x = x0; x < x1; ++x) {
-    const Entry e = kv_entry(a, x);
+    e = kv_entry(a, x);
     const int c = kv_tiles(a, e.n);
     tiles += c;
     cost += kv_cost(c);
     if (blockIdx.x == 0 && e.bad) kv_report(a.status, e.bad);
   }
-  long long* tsum = sums + threads + 1;
-  const int lane = threadIdx.x & 31;
+  const long long my_cost = cost, my_tiles = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long uc = __shfl_up_sync(0xffffffffu, cost, o), ut = __shfl_up_sync(0xffffffffu, tiles, o);
@@ -172,44 +154,42 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int*
       tiles += ut;
     }
   }
-  sums[threadIdx.x + 1] = cost;
-  tsum[threadIdx.x + 1] = tiles;
-  __syncthreads();
-  long long c0 = 0, t0 = 0, all = 0, all_tiles = 0;  // before this warp, and in all
-#pragma unroll 1
-  for (int w = 1; w <= threads / 32; ++w) {
-    if (w == (int)threadIdx.x / 32 + 1) {
-      c0 = all;
-      t0 = all_tiles;
-    }
-    all += sums[w * 32];
-    all_tiles += tsum[w * 32];
+  if (lane == 31) {
+    s.cost[warp] = cost;
+    s.tiles[warp] = tiles;
   }
-  const long long total = all * a.units;
-  if (total == 0) return Run{0, 0, 0};
-  const int shares = kv_shares(a, total);
-  if ((int)blockIdx.x >= shares) return Run{0, 0, total};
-  // this thread's entries: the line from ex on, `tb` tiles before it
-  const long long ex = (c0 + (lane ? sums[threadIdx.x] : 0)) * a.units, in = (c0 + cost) * a.units;
-  const long long tb = (t0 + (lane ? tsum[threadIdx.x] : 0)) * a.units;
+  __syncthreads();
+  long long all = 0, all_tiles = 0;
+#pragma unroll 1
+  for (int w = 0; w < threads / 32; ++w) {
+    if (w == warp) {
+      cost += all;
+      tiles += all_tiles;
+    }
+    all += s.cost[w];
+    all_tiles += s.tiles[w];
+  }
+  Run r = {};
+  r.total = all * a.units;
+  if (r.total == 0) return r;
+  const int shares = kv_shares(a, r.total);
+  if ((int)blockIdx.x >= shares) return r;
+  // this thread's entries hold the line from ex to in; `tb` tiles lie before them
+  const long long ex = (cost - my_cost) * a.units, in = cost * a.units, tb = (tiles - my_tiles) * a.units;
 #pragma unroll 1
   for (int end = 0; end < 2; ++end) {
-    const long long at = kv_share_start(total, shares, blockIdx.x + end);
-    if (at == total && threadIdx.x == 0) ends[1] = all_tiles * a.units;
+    const long long at = kv_share_start(r.total, shares, blockIdx.x + end);
+    if (at == r.total && threadIdx.x == 0) s.before[1] = all_tiles * a.units;
     if (at < ex || at >= in) continue;
     long long rest = at - ex, before = tb;
 #pragma unroll 1
     for (int x = x0; x < x1; ++x) {
-      const int c = kv_tiles(a, kv_entry(a, x).n), k = kv_cost(c);
+      if (per > 1) e = kv_entry(a, x);
+      const int c = kv_tiles(a, e.n), k = kv_cost(c);
       if (rest < (long long)k * a.units) {
         const int u = (int)kv_div(rest, k), in_unit = (int)(rest - (long long)u * k), t = max(0, in_unit - kUnitCost);
-        ends[end] = before + (long long)u * c + t;
-        if (end == 0) {
-          where[0] = x;
-          where[1] = u;
-          where[2] = t;
-          ends[2] = at - in_unit;
-        }
+        s.before[end] = before + (long long)u * c + t;
+        if (end == 0) s.run = Run{x, u, t, c, e, 0, at - in_unit, r.total};
         break;
       }
       rest -= (long long)k * a.units;
@@ -217,26 +197,107 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, long long* sums, int*
     }
   }
   __syncthreads();
-  p.set(a, where[0], where[1], where[2]);
-  return Run{ends[1] - ends[0], ends[2], total};
+  r = s.run;
+  r.left = s.before[1] - s.before[0];
+  return r;
 }
 
-// Where key j of a place lies: byte offset of its slot in the pools, or -1
-// when there is no such key (behind the length, a list's page behind it) and
-// -2 when its page id is bad.
-__device__ __forceinline__ long long kv_locate(const AttendArgs& a, const Place& p, int j) {
-  if (j >= p.e.n) return -1;
-  int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
-  const int slot = j - o * a.kv.page_size;
-  if (a.pages) {
-    o = a.pages[(long long)p.x * a.max_pages + o];
-    if (o < 0 || o >= a.kv.width) return -2;
-    if ((long long)o * a.kv.page_size + slot >= p.e.len) return -1;
+// What the arithmetic of a tile needs to know, left by the warp when it
+// issues the tile's copies.
+struct __align__(16) StageInfo {
+  uint32_t keys;  // the chunk's keys that exist, in the lower half; any of the upper: a bad page
+  int t, tiles;   // the tile, and its unit's tiles
+  int row, head, g0;
+  int pad[2];
+};
+
+// A warp's walk over its run, a chunk of 16 keys each tile, ahead of the
+// arithmetic. WHOLE: page_size is a multiple of 16, so a chunk lies in one
+// page: 32 lanes hold the pages of the next 32 tiles. Otherwise lanes 0 .. 15
+// hold the pages of the next chunk's keys, loaded a tile ahead of their use.
+template <bool WHOLE>
+struct Walk {
+  int x, u, t, tiles, head, lane, warp;
+  Entry e;
+  long long ahead;  // tiles not yet taken
+  int win;          // WHOLE: the tile lane 0 holds
+  int page;         // -1: no key, -2: a bad page
+  int more;         // WHOLE: keys of the chunk (0 .. 16); else the slot of the key in its page
+
+  __device__ __forceinline__ Walk(const AttendArgs& a, const Run& r)
+      : x(r.x), u(r.u), t(r.t), tiles(r.tiles), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), e(r.e), ahead(r.left) {
+    head = a.pages ? x % a.kv.kv_heads : u / a.blocks;
+    look(a);
   }
-  const int page = a.kv.pages_of(p.e.seq)[o];
-  if (page < 0 || page >= a.kv.num_pages) return -2;
-  return page * a.kv.page_stride + p.head * a.kv.head_stride + slot * a.kv.slot_stride;
-}
+
+  // loads the pages of the tiles (of the chunk's keys) from t on
+  __device__ __forceinline__ void look(const AttendArgs& a) {
+    win = t;
+    page = -1;
+    const int j = WHOLE ? (t + lane) * a.tile + warp * kKvChunk : t * a.tile + warp * kKvChunk + lane;
+    more = 0;
+    if (j >= e.n || j < 0 || (!WHOLE && lane >= kKvChunk)) return;
+    int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
+    const int slot = j - o * a.kv.page_size;
+    int live = e.n - j;  // keys from j on
+    if (a.pages) {
+      o = a.pages[(long long)x * a.max_pages + o];
+      if (o < 0 || o >= a.kv.width) {
+        page = -2;
+        return;
+      }
+      const long long left = e.len - ((long long)o * a.kv.page_size + slot);
+      live = left < live ? (int)left : live;
+      if (live <= 0) return;
+    }
+    more = WHOLE ? min(live, kKvChunk) : slot;
+    page = a.kv.pages_of(e.seq)[o];
+    if (page < 0 || page >= a.kv.num_pages) page = -2;
+  }
+
+  // The tile's chunk: which keys exist, and their first slot's offset in the
+  // pools (WHOLE), or each lane's (-1: none).
+  __device__ __forceinline__ uint32_t chunk(const AttendArgs& a, long long* off) const {
+    if (WHOLE) {
+      const int pg = __shfl_sync(0xffffffffu, page, t - win), n = __shfl_sync(0xffffffffu, more, t - win);
+      if (pg < 0) return pg == -2 ? 0x10000u : 0u;
+      const int j = t * a.tile + warp * kKvChunk;
+      const int slot = a.shift >= 0 ? j & (a.kv.page_size - 1) : j % a.kv.page_size;
+      *off = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.slot_stride;
+      return (1u << n) - 1;
+    }
+    *off = page >= 0 ? page * a.kv.page_stride + head * a.kv.head_stride + more * a.kv.slot_stride : -1;
+    return __ballot_sync(0xffffffffu, page >= 0) | (__ballot_sync(0xffffffffu, page == -2) << 16);
+  }
+
+  __device__ __forceinline__ void note(const AttendArgs& a, uint32_t keys, int block_heads, StageInfo* to) const {
+    if (lane) return;
+    to->keys = keys;
+    to->t = t;
+    to->tiles = tiles;
+    to->row = a.pages ? x / a.kv.kv_heads : x;
+    to->head = head;
+    to->g0 = u % a.blocks * block_heads;
+  }
+
+  // to the next tile, if there is one
+  __device__ __forceinline__ void next(const AttendArgs& a) {
+    if (--ahead <= 0) return;
+    if (++t == tiles) {
+      t = 0;
+      if (++u == a.units) {
+        u = 0;
+        win = 1;  // no page that is held belongs to the next entry
+        do e = kv_entry(a, ++x);
+        while (e.n == 0);
+        tiles = kv_tiles(a, e.n);
+      }
+      head = a.pages ? x % a.kv.kv_heads : u / a.blocks;
+    }
+    // another unit of the entry goes over the same pages again
+    if (!WHOLE || t < win || t - win >= 32) look(a);
+  }
+};
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

@@ -104,15 +104,16 @@ __device__ __forceinline__ int swz(int row, int col) {
 
 // DP: head_dim padded to 64, 128 or 256; NT: tiles of 8 queries; QS: bf16
 // parts of a query (1: bf16 queries and results, 3: fp32).
-template <int DP, int NT, int QS>
+// WHOLE: page_size is a multiple of 16.
+template <int DP, int NT, int QS, bool WHOLE>
 __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     kv_attend_mma_kernel(const __grid_constant__ AttendArgs a) {
   using Ring = MmaRing<DP, NT, QS>;
   constexpr int S = Ring::kStages, KS = DP / 16, PS = QS == 1 ? 2 : 3;
   extern __shared__ __align__(128) char sm[];
-  __shared__ long long sums[2 * (kMmaWarps * 32 + 1)], ends[3];
-  __shared__ int where[3], spoiled;
-  __shared__ uint32_t live[kMmaWarps][S];  // a stage's keys that exist, its bad ones in the upper half
+  __shared__ RunScratch scratch;
+  __shared__ int spoiled;
+  __shared__ StageInfo info[kMmaWarps][S];
   const int d = a.kv.d, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   char* ring = sm + warp * S * 2 * Ring::kChunkBytes;
   uint2* qf = reinterpret_cast<uint2*>(sm + Ring::kBytes);               // [KS][QS][NT][32]
@@ -129,53 +130,29 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     __syncwarp();
   }
   chain_wait();
-  Place c;
-  const Run run = kv_run(a, sums, where, ends, c);
+  const Run run = kv_run(a, scratch);
+  if (run.left == 0) return;
   long long left = run.left, begin = run.begin;
-  if (left == 0) return;
-
-  Place f = c;
-  long long ahead = left;
-  // The page of the next chunk's key `lane` is loaded a step before it is
-  // used: what (0: no key, 1: page id, 2: bad), page, slot.
-  int what = 0, page = 0, slot = 0;
-  auto peek = [&]() {
-    what = 0;
-    const int j = f.t * a.tile + warp * kKvChunk + lane;
-    if (lane >= kKvChunk || j >= f.e.n) return;
-    int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
-    slot = j - o * a.kv.page_size;
-    if (a.pages) {
-      o = a.pages[(long long)f.x * a.max_pages + o];
-      if (o < 0 || o >= a.kv.width) {
-        what = 2;
-        return;
-      }
-      if ((long long)o * a.kv.page_size + slot >= f.e.len) return;
-    }
-    what = 1;
-    page = a.kv.pages_of(f.e.seq)[o];
-  };
-  peek();
+  Walk<WHOLE> walk(a, run);
 
   float m[NT][2], l[NT][2], o[KS][NT][4];
   bool fresh = true, bad = false;
-  int st = 0, first_t = 0, row = 0, g0 = 0, live_g = 0, filled = 0;
+  int st = 0, first_t = 0, live_g = 0, filled = 0;
   // One loop fills the ring (S steps), then takes a stage and fills it again:
   // each piece of code stands once, since a short launch waits for its
   // instructions as it does for its data.
 #pragma unroll 1
   for (;;) {
     const bool work = filled == S;
+    StageInfo now = {};
     if (work) {
+    now = info[warp][st];
     if (fresh) {  // a new unit: its queries in the matrix instructions' order
       fresh = false;
       bad = false;
-      first_t = c.t;
-      row = c.row(a);
-      g0 = c.block(a) * NT * 8;
-      live_g = min(NT * 8, a.group - g0);
-      const long long qat = (long long)row * a.q_stride + (long long)(c.head * a.group + g0) * d;
+      first_t = now.t;
+      live_g = min(NT * 8, a.group - now.g0);
+      const long long qat = (long long)now.row * a.q_stride + (long long)(now.head * a.group + now.g0) * d;
 #pragma unroll 1
       for (int i = threadIdx.x; i < KS * QS * NT * 32; i += kMmaWarps * 32) {
         const int ln = i % 32, nt = i / 32 % NT, part = i / (32 * NT) % QS, ks = i / (32 * NT * QS);
@@ -204,7 +181,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     }
     copy_wait<S - 1>();
     __syncwarp();
-    const uint32_t mask = live[warp][st];
+    const uint32_t mask = now.keys;
     if (mask >> 16) bad = true;
     if (mask & 0xffff) {
       const uint32_t kc = smem_addr(ring + st * 2 * Ring::kChunkBytes), vc = kc + Ring::kChunkBytes;
@@ -229,7 +206,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
           }
       }
       const bool on0 = (mask >> (lane / 4)) & 1, on1 = (mask >> (lane / 4 + 8)) & 1;
-      float now[NT][2], p[NT][4];
+      float high[NT][2], p[NT][4];
       bool moved = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -241,8 +218,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         }
         if (a.scores) {
           const int g = nt * 8 + lane % 4 * 2;
-          float* to = a.scores + (((long long)row * a.kv.kv_heads + c.head) * a.mass_len + c.t * a.tile + warp * kKvChunk +
-                                  lane / 4) * a.group + g0 + g;
+          float* to = a.scores + (((long long)now.row * a.kv.kv_heads + now.head) * a.mass_len + now.t * a.tile +
+                                  warp * kKvChunk + lane / 4) * a.group + now.g0 + g;
           if (on0 && g < live_g) to[0] = s[0];
           if (on0 && g + 1 < live_g) to[1] = s[1];
           to += 8 * a.group;
@@ -254,8 +231,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
           float top = fmaxf(s[e], s[e + 2]);
 #pragma unroll
           for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          now[nt][e] = fmaxf(m[nt][e], top);
-          moved |= now[nt][e] != m[nt][e];
+          high[nt][e] = fmaxf(m[nt][e], top);
+          moved |= high[nt][e] != m[nt][e];
         }
       }
       if (__any_sync(0xffffffffu, moved)) {  // a new maximum: rescale what is there
@@ -263,8 +240,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float keep = exp2f(m[nt][e] - (now[nt][e] == -INFINITY ? 0.f : now[nt][e]));
-            m[nt][e] = now[nt][e];
+            const float keep = exp2f(m[nt][e] - (high[nt][e] == -INFINITY ? 0.f : high[nt][e]));
+            m[nt][e] = high[nt][e];
             l[nt][e] *= keep;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -322,28 +299,32 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     }
     __syncwarp();
     }
-    if (ahead > 0) {  // the stage's next chunk
-      const bool in = what == 1 && page >= 0 && page < a.kv.num_pages;
-      const long long off = in ? page * a.kv.page_stride + f.head * a.kv.head_stride + slot * a.kv.slot_stride : -1;
-      const uint32_t keys = __ballot_sync(0xffffffffu, in) |
-                            (__ballot_sync(0xffffffffu, what == 2 || (what == 1 && !in)) << 16);
-      if (lane == 0) live[warp][st] = keys;
+    if (walk.ahead > 0) {  // the stage's next chunk
+      long long off = 0;
+      const uint32_t keys = walk.chunk(a, &off);
+      walk.note(a, keys, NT * 8, &info[warp][st]);
       const uint32_t kd = smem_addr(ring + st * 2 * Ring::kChunkBytes), vd = kd + Ring::kChunkBytes;
+      if (col < cols || !WHOLE) {
+        const long long step = kg * a.kv.slot_stride + col * 16;
+        const char *kp = a.kv.k + off + step, *vp = a.kv.v + off + step;
 #pragma unroll
-      for (int i = 0; i < kKvChunk / KG; ++i) {
-        const int r = i * KG + kg;
-        const long long o = __shfl_sync(0xffffffffu, off, r);
-        const int bytes = o >= 0 ? 16 : 0;
-        const long long at = (o >= 0 ? o : 0) + col * 16;
-        if (col < cols) {
-          copy16(kd + swz<DP>(r, col), a.kv.k + at, bytes);
-          copy16(vd + swz<DP>(r, col), a.kv.v + at, bytes);
+        for (int i = 0; i < kKvChunk / KG; ++i) {
+          const int r = i * KG + kg, bytes = (keys >> r) & 1 ? 16 : 0;
+          if (!WHOLE) {
+            const long long at = __shfl_sync(0xffffffffu, off, r);
+            kp = a.kv.k + (at >= 0 ? at : 0) + col * 16;
+            vp = a.kv.v + (at >= 0 ? at : 0) + col * 16;
+          }
+          if (WHOLE || col < cols) {
+            // a key that is not there is not read: its address is the pool's first
+            copy16(kd + swz<DP>(r, col), bytes ? kp : a.kv.k, bytes);
+            copy16(vd + swz<DP>(r, col), bytes ? vp : a.kv.v, bytes);
+          }
+          kp += KG * a.kv.slot_stride;
+          vp += KG * a.kv.slot_stride;
         }
       }
-      if (--ahead > 0) {
-        f.next(a);
-        peek();
-      }
+      walk.next(a);
     }
     copy_commit();
     st = st + 1 == S ? 0 : st + 1;
@@ -352,11 +333,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       continue;
     }
     --left;
-    const int t = c.t, tiles = c.tiles, h = c.head;
-    if (t + 1 < tiles && left > 0) {
-      ++c.t;
-      continue;
-    }
+    const int t = now.t, tiles = now.tiles, h = now.head, row = now.row, g0 = now.g0;
+    if (t + 1 < tiles && left > 0) continue;
     // the unit ends here, or the CTA's part of it: the warps' pieces join
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -393,9 +371,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         const int g4 = i / DP, cc = i % DP, g = q4 * kMergeHeads + g4;
         if (g >= live_g || cc >= d) continue;
         float top = -INFINITY, sum = 0.f, acc = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, ml[(w * NT * 8 + g) * 2]);
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < kMmaWarps; ++w) {
           const float by = piece_weight(ml[(w * NT * 8 + g) * 2], top);
           sum = fmaf(ml[(w * NT * 8 + g) * 2 + 1], by, sum);
@@ -424,19 +402,23 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     if (left == 0) return;
     fresh = true;
     begin += kv_cost(tiles);
-    c.next(a);
   }
 }
 
 namespace {
 
-template <int DP, int NT, int QS>
-int mma_go(const AttendArgs& a, cudaStream_t st) {
-  auto kernel = kv_attend_mma_kernel<DP, NT, QS>;
+template <int DP, int NT, int QS, bool WHOLE>
+int mma_launch(const AttendArgs& a, cudaStream_t st) {
+  auto kernel = kv_attend_mma_kernel<DP, NT, QS, WHOLE>;
   constexpr int smem = mma_smem<DP, NT, QS>();
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, smem, done)) return rc;
   return launch_chained(kernel, dim3(a.grid), dim3(kMmaWarps * 32), smem, st, "kv_attend_mma_kernel", a);
+}
+
+template <int DP, int NT, int QS>
+int mma_go(const AttendArgs& a, cudaStream_t st) {
+  return a.kv.page_size % kKvChunk ? mma_launch<DP, NT, QS, false>(a, st) : mma_launch<DP, NT, QS, true>(a, st);
 }
 
 template <int NT, int QS>
