@@ -15,7 +15,7 @@ inline KernelShape simt_shape(int d, int group) {
   KernelShape s;
   s.heads = group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
   for (s.warps = 4; s.warps > 1; s.warps /= 2) {
-    s.smem = s.heads * d * 4 + s.warps * s.heads * (d + 2) * 4 + s.warps * s.heads * kKvChunk * 4 + 64 +
+    s.smem = s.heads * d * 4 + s.warps * s.heads * (d + 4) * 4 + s.warps * s.heads * kKvChunk * 4 + 64 +
              s.warps * kSimtStages * (2 * kKvChunk * simt_pitch(d));
     if (s.smem <= 220 * 1024) break;
   }
@@ -28,7 +28,7 @@ inline KernelShape simt_shape(int d, int group) {
 // asynchronous copies. Scores: lane l holds key l % 16 and half of the
 // columns. Values: the lanes split a row's 16-byte columns, lane groups the
 // keys. GB queries of the group at a time share each key that is read.
-template <typename TQ, int GB, bool WHOLE>
+template <typename TQ, int GB, bool WHOLE, bool CLUSTER>
 __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_constant__ AttendArgs a, int pitch) {
   using TC = float;
   constexpr int V = 16 / sizeof(TC);
@@ -38,9 +38,10 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   __shared__ StageInfo info[4][kSimtStages];
   const int d = a.kv.d, warps = blockDim.x / 32, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* qs = reinterpret_cast<float*>(sm);                // [GB][d]
-  float* merge = qs + GB * d;                              // [warps][GB][d + 2]: m, l, o
-  float* prob = merge + warps * GB * (d + 2) + warp * GB * kKvChunk;  // [16][GB]
-  char* ring0 = sm + ((GB * d + warps * GB * (d + 2) + warps * GB * kKvChunk) * 4 + 15) / 16 * 16;
+  const int pitch_m = d + 4;
+  float* merge = qs + GB * d;                              // [warps][GB][d + 4]: o, m, l
+  float* prob = merge + warps * GB * pitch_m + warp * GB * kKvChunk;  // [16][GB]
+  char* ring0 = sm + (GB * d + warps * GB * pitch_m + warps * GB * kKvChunk) * 4;
   char* ring = ring0 + warp * kSimtStages * 2 * kKvChunk * pitch;
   const int cols = d / V;
   int wide = 2;  // lanes across a row; at most 16 rows at a time, so every lane group has as many
@@ -48,8 +49,17 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   const int col = lane % wide, kg = lane / wide, kgs = 32 / wide;
 
   chain_wait();
-  const Run run = kv_run(a, scratch);
-  if (run.left == 0) return;
+  // a cluster's CTA leaves its piece where its ring was
+  float *piece_ml = reinterpret_cast<float*>(ring0), *piece_o = piece_ml + (GB * 2 + 3) / 4 * 4;
+  const Run run = CLUSTER ? kv_cluster_run(a) : kv_run(a, scratch);
+  if (run.left == 0) {
+    if (CLUSTER) {
+      for (int i = threadIdx.x; i < GB * 2; i += blockDim.x) piece_ml[i] = i & 1 ? 0.f : -INFINITY;
+      for (int i = threadIdx.x; i < GB * d; i += blockDim.x) piece_o[i] = 0.f;
+      kv_cluster_join<TQ>(a, run, GB, piece_ml, piece_o, d);
+    }
+    return;
+  }
   long long left = run.left, begin = run.begin;
   Walk<WHOLE> walk(a, run);
 
@@ -197,58 +207,61 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       for (int x = wide; x < 32; x *= 2)
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[g][e] += __shfl_xor_sync(0xffffffffu, o[g][e], x);
-      float* to = merge + (warp * GB + g) * (d + 2);
+      float* to = merge + (warp * GB + g) * pitch_m;
       if (lane == 0) {
-        to[0] = m[g];
-        to[1] = l[g];
+        to[d] = m[g];
+        to[d + 1] = l[g];
       }
       if (kg == 0) {
 #pragma unroll
         for (int w = 0; w < 8 / V; ++w)
           if (col + 32 * w < cols) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) to[2 + (col + 32 * w) * V + e] = o[g][w * V + e];
+            for (int e = 0; e < V; ++e) to[(col + 32 * w) * V + e] = o[g][w * V + e];
           }
       }
     }
     if (bad && lane == 0) spoiled = 1;
     __syncthreads();
-    const bool whole = first_t == 0 && t + 1 == tiles;
-    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
+    const bool whole = !CLUSTER && first_t == 0 && t + 1 == tiles;
+    if (!CLUSTER && first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
       a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, begin, run.total};
     const bool nan = spoiled != 0;
     if (nan && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
 #pragma unroll 1
-    for (int i = threadIdx.x; i < GB * d; i += blockDim.x) {
-      const int g = i / d, cc = i % d;
-      if (g >= live_g) continue;
-      const float* from = merge + g * (d + 2);
-      float top = -INFINITY, sum = 0.f, acc = 0.f;
-#pragma unroll 1
-      for (int w = 0; w < warps; ++w) top = fmaxf(top, from[w * GB * (d + 2)]);
-#pragma unroll 1
+    for (int i = threadIdx.x; i < live_g * cols; i += blockDim.x) {
+      const int g = i / cols, cc = (i - g * cols) * 4;
+      const float* from = merge + g * pitch_m;
+      float top = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int w = 0; w < warps; ++w) top = fmaxf(top, from[w * GB * pitch_m + d]);
+#pragma unroll 4
       for (int w = 0; w < warps; ++w) {
-        const float* p = from + w * GB * (d + 2);
-        const float by = piece_weight(p[0], top);
-        sum = fmaf(p[1], by, sum);
-        acc = fmaf(p[2 + cc], by, acc);
+        const float* p = from + w * GB * pitch_m;
+        const float by = piece_weight(p[d], top);
+        sum = fmaf(p[d + 1], by, sum);
+        fma4(acc, *reinterpret_cast<const float4*>(p + cc), by);
       }
-      if (nan) sum = acc = __int_as_float(0x7fc00000);
-      if (whole) {
+      if (nan) sum = __int_as_float(0x7fc00000);
+      if (CLUSTER) {
+        *reinterpret_cast<float4*>(piece_o + g * d + cc) = acc;
+        if (cc == 0) *reinterpret_cast<float2*>(piece_ml + g * 2) = make_float2(top, sum);
+      } else if (whole) {
         const long long at = (long long)row * a.heads + h * a.group + g0 + g;
-        ((TQ*)a.out)[at * d + cc] = kv_round<TQ>(sum == 0.f ? 0.f : acc / sum);
+        kv_store4((TQ*)a.out + at * d + cc, acc, sum);
         if (a.scores && cc == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
       } else {
-        const long long slot = (long long)blockIdx.x * 2 + (first_t != 0 ? 0 : 1);
-        a.part_o[(slot * GB + g) * d + cc] = acc;
-        if (cc == 0) {
-          a.part_ml[(slot * GB + g) * 2] = top;
-          a.part_ml[(slot * GB + g) * 2 + 1] = sum;
-        }
+        const long long piece = ((long long)blockIdx.x * 2 + (first_t != 0 ? 0 : 1)) * GB + g;
+        *reinterpret_cast<float4*>(a.part_o + piece * d + cc) = acc;
+        if (cc == 0) *reinterpret_cast<float2*>(a.part_ml + piece * 2) = make_float2(top, sum);
       }
     }
     __syncthreads();
-    if (left == 0) return;
+    if (left == 0) {
+      if (CLUSTER) kv_cluster_join<TQ>(a, run, GB, piece_ml, piece_o, d);
+      return;
+    }
     fresh = true;
     begin += kv_cost(tiles);
   }
@@ -311,10 +324,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
     for (int k = grp; k < n; k += groups) {
       const float4 x = *reinterpret_cast<const float4*>(a.part_o + piece(k) * d + col * 4);
       const float by = wt[k];
-      acc.x = fmaf(x.x, by, acc.x);
-      acc.y = fmaf(x.y, by, acc.y);
-      acc.z = fmaf(x.z, by, acc.z);
-      acc.w = fmaf(x.w, by, acc.w);
+      fma4(acc, x, by);
     }
   }
   float4* part = reinterpret_cast<float4*>(wt + (a.grid + 3) / 4 * 4);
@@ -329,11 +339,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
       acc.z += x.z;
       acc.w += x.w;
     }
-    TQ* out = (TQ*)a.out + at * d + col * 4;
-    out[0] = kv_round<TQ>(sum == 0.f ? 0.f : acc.x / sum);
-    out[1] = kv_round<TQ>(sum == 0.f ? 0.f : acc.y / sum);
-    out[2] = kv_round<TQ>(sum == 0.f ? 0.f : acc.z / sum);
-    out[3] = kv_round<TQ>(sum == 0.f ? 0.f : acc.w / sum);
+    kv_store4((TQ*)a.out + at * d + col * 4, acc, sum);
   }
   if (a.scores && threadIdx.x == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
@@ -355,18 +361,19 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
 
 namespace {
 
-template <typename TQ, int GB, bool WHOLE>
+template <typename TQ, int GB, bool WHOLE, bool CLUSTER>
 int simt_launch(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
-  auto kernel = kv_attend_simt_kernel<TQ, GB, WHOLE>;
+  auto kernel = kv_attend_simt_kernel<TQ, GB, WHOLE, CLUSTER>;
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, 224 * 1024, done)) return rc;
-  return launch_chained(kernel, dim3(a.grid), dim3(s.warps * 32), s.smem, st, "kv_attend_simt_kernel", a,
-                        simt_pitch(a.kv.d));
+  return attend_launch(kernel, a, s.warps * 32, s.smem, st, simt_pitch(a.kv.d));
 }
 
 template <typename TQ, int GB>
 int simt_go(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
-  return a.kv.page_size % kKvChunk ? simt_launch<TQ, GB, false>(a, s, st) : simt_launch<TQ, GB, true>(a, s, st);
+  if (a.kv.page_size % kKvChunk)
+    return a.cluster ? simt_launch<TQ, GB, false, true>(a, s, st) : simt_launch<TQ, GB, false, false>(a, s, st);
+  return a.cluster ? simt_launch<TQ, GB, true, true>(a, s, st) : simt_launch<TQ, GB, true, false>(a, s, st);
 }
 
 template <typename TQ>
@@ -384,6 +391,7 @@ constexpr int kMaxEntries = 4096;  // scan entries a launch takes; more rows go 
 struct Layout {
   KernelShape shape;
   int blocks, grid, rows;  // rows: of one launch
+  bool cluster;
   size_t cut, ml, o, lse, scores, bytes;
 };
 
@@ -396,6 +404,15 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
   if (L.rows < 1) L.rows = 1;
   if (L.rows > io.rows) L.rows = io.rows;
+  // A cluster per unit or equal shares of all tiles. Against the shares the
+  // clusters save about 7 tiles' time (no division of the line, no join), but
+  // a unit has 8 CTAs at most: taken while its longest row costs those CTAs
+  // less than 7 tiles more than a share would be, and all clusters run at once.
+  const long long units = (long long)L.rows * c.kv_heads * L.blocks, tile = L.shape.warps * kKvChunk;
+  const long long longest =
+      ((io.pages ? (long long)io.max_pages : (long long)c.table_width) * c.page_size + tile - 1) / tile;
+  L.cluster = L.rows == io.rows && units * kClusterCtas <= L.grid &&
+              longest * (L.grid - units * kClusterCtas) <= 7LL * kClusterCtas * L.grid;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -489,6 +506,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     a.part_ml = (float*)(ws + L.ml);
     a.part_o = (float*)(ws + L.o);
     a.grid = L.grid;
+    a.cluster = L.cluster;
     if (io->mass) {
       a.lse = (float*)(ws + L.lse);
       a.scores = (float*)(ws + L.scores);
@@ -508,6 +526,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
     const int gb = L.shape.heads;
     const dim3 grid(L.grid, gb < a.group ? gb : a.group);
     const size_t smem = (size_t)(L.grid + 3) / 4 * 16 + kJoinThreads * 16;
+    if (!L.cluster)
     rc = qb ? launch_chained(kv_join_kernel<bf>, grid, dim3(kJoinThreads), smem, st, "kv_join_kernel", a, gb)
             : launch_chained(kv_join_kernel<float>, grid, dim3(kJoinThreads), smem, st, "kv_join_kernel", a, gb);
     if (rc) return rc;

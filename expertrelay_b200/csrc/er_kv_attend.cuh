@@ -49,6 +49,7 @@ struct AttendArgs {
   float* part_ml;              // [2 grid][GB][2]: m, l of a CTA's first and last piece
   float* part_o;               // [2 grid][GB][d]
   int grid;                    // CTAs of the attention kernel
+  int cluster;                 // a cluster per unit instead of shares of the line
   float* scores;               // optional [rows][kv_heads][mass_len][group], log2 units
   float* lse;                  // with scores: [rows][heads], log2 units
   float* mass;
@@ -202,6 +203,119 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, RunScratch& s) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 2^(m_i - m) of a piece, 0 for a piece without keys or of -inf scores alone.
+__device__ __forceinline__ float piece_weight(float mi, float m) { return mi == -INFINITY ? 0.f : exp2f(mi - m); }
+
+// With few units, each is a cluster's: its CTAs take an eighth of the tiles
+// each and join their pieces through one another's shared memory, so there is
+// no line to divide, no workspace and no second launch.
+constexpr int kClusterCtas = 8;
+
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return (int)r;
+}
+// Every thread of every CTA of the cluster arrives and waits; what was written before is seen after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of `addr` (shared memory) in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+__device__ __forceinline__ Run kv_cluster_run(const AttendArgs& a) {
+  Run r = {};
+  const int unit = blockIdx.x / kClusterCtas, rank = cluster_rank();
+  r.x = unit / a.units;
+  r.u = unit % a.units;
+  r.e = kv_entry(a, r.x);
+  if (r.e.bad && r.u == 0 && rank == 0 && threadIdx.x == 0) kv_report(a.status, r.e.bad);
+  r.tiles = kv_tiles(a, r.e.n);
+  r.t = (int)((long long)r.tiles * rank / kClusterCtas);
+  r.left = (int)((long long)r.tiles * (rank + 1) / kClusterCtas) - r.t;
+  return r;
+}
+
+// Four results of query g of a unit, from their weighted sum and the weights' sum.
+template <typename TQ>
+__device__ __forceinline__ void kv_store4(TQ* to, float4 acc, float sum) {
+  const float inv = 1.f / sum;
+  const bool none = sum == 0.f;  // no key, or scores of -inf alone
+  float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = none ? 0.f : v[e];
+  if constexpr (sizeof(TQ) == 4) {
+    *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    uint2 raw = make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+    *reinterpret_cast<uint2*>(to) = raw;
+  }
+}
+__device__ __forceinline__ void fma4(float4& acc, float4 x, float by) {
+  acc.x = fmaf(x.x, by, acc.x);
+  acc.y = fmaf(x.y, by, acc.y);
+  acc.z = fmaf(x.z, by, acc.z);
+  acc.w = fmaf(x.w, by, acc.w);
+}
+
+// The cluster's pieces joined: in every CTA's shared memory, `ml` [heads][2]
+// and `o` [heads][pitch]. Each CTA writes an eighth of the unit's results.
+template <typename TQ>
+__device__ __forceinline__ void kv_cluster_join(const AttendArgs& a, const Run& r, int gb, const float* ml,
+                                                const float* o, int pitch) {
+  cluster_sync();
+  const int head = a.pages ? r.x % a.kv.kv_heads : r.u / a.blocks, row = a.pages ? r.x / a.kv.kv_heads : r.x;
+  const int d = a.kv.d, g0 = r.u % a.blocks * gb, live_g = min(gb, a.group - g0), cols = d / 4;
+  const uint32_t ml0 = smem_addr(ml), o0 = smem_addr(o);
+#pragma unroll 1
+  for (int i = threadIdx.x * kClusterCtas + cluster_rank(); i < live_g * cols; i += blockDim.x * kClusterCtas) {
+    const int g = i / cols, col = i - g * cols;
+    float2 p[kClusterCtas];
+    float4 x[kClusterCtas];
+#pragma unroll
+    for (int k = 0; k < kClusterCtas; ++k) {
+      p[k] = cluster_load2(cluster_addr(ml0 + g * 8, k));
+      x[k] = cluster_load4(cluster_addr(o0 + (g * pitch + col * 4) * 4, k));
+    }
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kClusterCtas; ++k) top = fmaxf(top, p[k].x);
+#pragma unroll
+    for (int k = 0; k < kClusterCtas; ++k) {
+      const float by = piece_weight(p[k].x, top);
+      sum = fmaf(p[k].y, by, sum);  // a spoiled piece's sum is NaN
+      fma4(acc, x[k], by);
+    }
+    if (r.e.bad) sum = __int_as_float(0x7fc00000);
+    const long long at = (long long)row * a.heads + head * a.group + g0 + g;
+    kv_store4((TQ*)a.out + at * d + col * 4, acc, sum);
+    if (a.scores && col == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
+  }
+  cluster_sync();  // no CTA's shared memory goes before all have read it
+}
+
 // What the arithmetic of a tile needs to know, left by the warp when it
 // issues the tile's copies.
 struct __align__(16) StageInfo {
@@ -299,8 +413,6 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
 // 16 bytes to shared memory, zeros when `bytes` is 0 (nothing is read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -318,9 +430,6 @@ __device__ __forceinline__ float kv_round<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 kv_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 2^(m_i - m) of a piece, 0 for a piece without keys or of -inf scores alone.
-__device__ __forceinline__ float piece_weight(float mi, float m) { return mi == -INFINITY ? 0.f : exp2f(mi - m); }
-
 
 // What a launch of an attention kernel takes: queries of a group together,
 // warps and shared memory of a CTA, CTAs an SM.
@@ -330,5 +439,24 @@ struct KernelShape {
 // the tensor-core kernel for bf16 caches (er_kv_attend_mma.cu)
 KernelShape mma_shape(int d, int group, int q_dtype);
 int attend_mma(const AttendArgs& a, int q_dtype, cudaStream_t st);
+
+// launch_chained, with clusters of kClusterCtas when a.cluster
+template <typename Kernel, typename... Args>
+int attend_launch(Kernel kernel, const AttendArgs& a, int threads, int smem, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.cluster ? a.entries * a.units * kClusterCtas : a.grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kClusterCtas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster ? 2 : 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a, args...), "kv_attend kernel");
+}
 
 }  // namespace er

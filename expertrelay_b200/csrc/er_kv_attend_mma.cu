@@ -20,6 +20,8 @@
 // under a quarter of the rounding of a bf16 result) for bf16 results and as
 // three (24 bits) for fp32 ones. Parts are cut, not rounded, so that they
 // share the sign of the whole and an infinite key or value stays infinite.
+#include <type_traits>
+
 #include "er_kv_attend.cuh"
 
 namespace er {
@@ -104,8 +106,8 @@ __device__ __forceinline__ int swz(int row, int col) {
 
 // DP: head_dim padded to 64, 128 or 256; NT: tiles of 8 queries; QS: bf16
 // parts of a query (1: bf16 queries and results, 3: fp32).
-// WHOLE: page_size is a multiple of 16.
-template <int DP, int NT, int QS, bool WHOLE>
+// WHOLE: page_size is a multiple of 16. CLUSTER: a cluster per unit.
+template <int DP, int NT, int QS, bool WHOLE, bool CLUSTER>
 __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     kv_attend_mma_kernel(const __grid_constant__ AttendArgs a) {
   using Ring = MmaRing<DP, NT, QS>;
@@ -130,8 +132,19 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     __syncwarp();
   }
   chain_wait();
-  const Run run = kv_run(a, scratch);
-  if (run.left == 0) return;
+  using TQ = std::conditional_t<QS == 1, __nv_bfloat16, float>;
+  // a cluster's CTA leaves its piece where its ring was
+  float *piece_ml = reinterpret_cast<float*>(sm), *piece_o = piece_ml + NT * 8 * 2;
+  const Run run = CLUSTER ? kv_cluster_run(a) : kv_run(a, scratch);
+  if (run.left == 0) {
+    if (CLUSTER) {
+      __syncthreads();  // the ring's zeros are written
+      for (int i = threadIdx.x; i < NT * 8 * (DP + 2); i += kMmaWarps * 32)
+        piece_ml[i] = i < NT * 16 && !(i & 1) ? -INFINITY : 0.f;
+      kv_cluster_join<TQ>(a, run, NT * 8, piece_ml, piece_o, DP);
+    }
+    return;
+  }
   long long left = run.left, begin = run.begin;
   Walk<WHOLE> walk(a, run);
 
@@ -153,21 +166,31 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       first_t = now.t;
       live_g = min(NT * 8, a.group - now.g0);
       const long long qat = (long long)now.row * a.q_stride + (long long)(now.head * a.group + now.g0) * d;
-#pragma unroll 1
-      for (int i = threadIdx.x; i < KS * QS * NT * 32; i += kMmaWarps * 32) {
-        const int ln = i % 32, nt = i / 32 % NT, part = i / (32 * NT) % QS, ks = i / (32 * NT * QS);
+#pragma unroll 2
+      for (int i = threadIdx.x; i < KS * NT * 32; i += kMmaWarps * 32) {
+        const int ln = i % 32, nt = i / 32 % NT, ks = i / (32 * NT);
         const int g = nt * 8 + ln / 4, c0 = ks * 16 + ln % 4 * 2;
-        uint32_t x[4];
+        if constexpr (QS == 1) {
+          uint32_t x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int cc = c0 + (e & 1) + (e >> 1) * 8;
-          const bool on = g < live_g && cc < d;
-          if (QS == 1)
-            x[e] = on ? (uint32_t)reinterpret_cast<const uint16_t*>(a.q)[qat + (long long)g * d + cc] : 0u;
-          else
-            x[e] = on ? query_part(reinterpret_cast<const float*>(a.q)[qat + (long long)g * d + cc], part) : 0u;
+          for (int e = 0; e < 4; ++e) {
+            const int cc = c0 + (e & 1) + (e >> 1) * 8;
+            x[e] = g < live_g && cc < d ? (uint32_t)reinterpret_cast<const uint16_t*>(a.q)[qat + (long long)g * d + cc] : 0u;
+          }
+          qf[i] = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+        } else {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int cc = c0 + (e & 1) + (e >> 1) * 8;
+            x[e] = g < live_g && cc < d ? reinterpret_cast<const float*>(a.q)[qat + (long long)g * d + cc] : 0.f;
+          }
+#pragma unroll 1
+          for (int part = 0; part < QS; ++part)
+            qf[((ks * QS + part) * NT + nt) * 32 + ln] =
+                make_uint2(query_part(x[0], part) | query_part(x[1], part) << 16,
+                           query_part(x[2], part) | query_part(x[3], part) << 16);
         }
-        qf[i] = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
       }
       if (threadIdx.x == 0) spoiled = 0;
       __syncthreads();
@@ -349,8 +372,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         }
       }
     if (bad && lane == 0) spoiled = 1;
-    const bool whole = first_t == 0 && t + 1 == tiles;
-    if (first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
+    const bool whole = !CLUSTER && first_t == 0 && t + 1 == tiles;
+    if (!CLUSTER && first_t == 0 && !whole && threadIdx.x == 0)  // begins here, ends behind
       a.cut[blockIdx.x] = CutUnit{row, h, g0, tiles, begin, run.total};
 #pragma unroll 1
     for (int q4 = 0; q4 * kMergeHeads < live_g; ++q4) {
@@ -367,39 +390,43 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       const bool nan = spoiled != 0;
       if (nan && q4 == 0 && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
 #pragma unroll 1
-      for (int i = threadIdx.x; i < kMergeHeads * DP; i += kMmaWarps * 32) {
-        const int g4 = i / DP, cc = i % DP, g = q4 * kMergeHeads + g4;
+      for (int i = threadIdx.x; i < kMergeHeads * DP / 4; i += kMmaWarps * 32) {
+        const int g4 = i / (DP / 4), cc = i % (DP / 4) * 4, g = q4 * kMergeHeads + g4;
         if (g >= live_g || cc >= d) continue;
-        float top = -INFINITY, sum = 0.f, acc = 0.f;
-#pragma unroll 1
-        for (int w = 0; w < kMmaWarps; ++w) top = fmaxf(top, ml[(w * NT * 8 + g) * 2]);
-#pragma unroll 1
+        float2 p[kMmaWarps];
+        float top = -INFINITY, sum = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
         for (int w = 0; w < kMmaWarps; ++w) {
-          const float by = piece_weight(ml[(w * NT * 8 + g) * 2], top);
-          sum = fmaf(ml[(w * NT * 8 + g) * 2 + 1], by, sum);
-          acc = fmaf(merge[(w * kMergeHeads + g4) * DP + cc], by, acc);
+          p[w] = *reinterpret_cast<const float2*>(ml + (w * NT * 8 + g) * 2);
+          top = fmaxf(top, p[w].x);
         }
-        if (nan) sum = acc = __int_as_float(0x7fc00000);
-        if (whole) {
+#pragma unroll
+        for (int w = 0; w < kMmaWarps; ++w) {
+          const float by = piece_weight(p[w].x, top);
+          sum = fmaf(p[w].y, by, sum);
+          fma4(acc, *reinterpret_cast<const float4*>(merge + (w * kMergeHeads + g4) * DP + cc), by);
+        }
+        if (nan) sum = __int_as_float(0x7fc00000);
+        if (CLUSTER) {
+          *reinterpret_cast<float4*>(piece_o + g * DP + cc) = acc;
+          if (cc == 0) *reinterpret_cast<float2*>(piece_ml + g * 2) = make_float2(top, sum);
+        } else if (whole) {
           const long long at = (long long)row * a.heads + h * a.group + g0 + g;
-          const float v = sum == 0.f ? 0.f : acc / sum;
-          if (QS == 1)
-            ((__nv_bfloat16*)a.out)[at * d + cc] = __float2bfloat16_rn(v);
-          else
-            ((float*)a.out)[at * d + cc] = v;
+          kv_store4((TQ*)a.out + at * d + cc, acc, sum);
           if (a.scores && cc == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
         } else {
           const long long piece = ((long long)blockIdx.x * 2 + (first_t != 0 ? 0 : 1)) * (NT * 8) + g;
-          a.part_o[piece * d + cc] = acc;
-          if (cc == 0) {
-            a.part_ml[piece * 2] = top;
-            a.part_ml[piece * 2 + 1] = sum;
-          }
+          *reinterpret_cast<float4*>(a.part_o + piece * d + cc) = acc;
+          if (cc == 0) *reinterpret_cast<float2*>(a.part_ml + piece * 2) = make_float2(top, sum);
         }
       }
       __syncthreads();
     }
-    if (left == 0) return;
+    if (left == 0) {
+      if (CLUSTER) kv_cluster_join<TQ>(a, run, NT * 8, piece_ml, piece_o, DP);
+      return;
+    }
     fresh = true;
     begin += kv_cost(tiles);
   }
@@ -407,18 +434,21 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
 
 namespace {
 
-template <int DP, int NT, int QS, bool WHOLE>
+template <int DP, int NT, int QS, bool WHOLE, bool CLUSTER>
 int mma_launch(const AttendArgs& a, cudaStream_t st) {
-  auto kernel = kv_attend_mma_kernel<DP, NT, QS, WHOLE>;
+  auto kernel = kv_attend_mma_kernel<DP, NT, QS, WHOLE, CLUSTER>;
   constexpr int smem = mma_smem<DP, NT, QS>();
+  static_assert(NT * 8 * (DP + 2) * 4 <= MmaRing<DP, NT, QS>::kBytes, "a piece fits the ring");
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, smem, done)) return rc;
-  return launch_chained(kernel, dim3(a.grid), dim3(kMmaWarps * 32), smem, st, "kv_attend_mma_kernel", a);
+  return attend_launch(kernel, a, kMmaWarps * 32, smem, st);
 }
 
 template <int DP, int NT, int QS>
 int mma_go(const AttendArgs& a, cudaStream_t st) {
-  return a.kv.page_size % kKvChunk ? mma_launch<DP, NT, QS, false>(a, st) : mma_launch<DP, NT, QS, true>(a, st);
+  if (a.kv.page_size % kKvChunk)
+    return a.cluster ? mma_launch<DP, NT, QS, false, true>(a, st) : mma_launch<DP, NT, QS, false, false>(a, st);
+  return a.cluster ? mma_launch<DP, NT, QS, true, true>(a, st) : mma_launch<DP, NT, QS, true, false>(a, st);
 }
 
 template <int NT, int QS>

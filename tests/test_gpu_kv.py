@@ -73,6 +73,31 @@ def test_attend_one_row(cuda, dtype, length):
     assert torch.equal(out, kv.attend(cache, q, _i32([length])))  # bit for bit again
 
 
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize(("rows", "kv_heads", "group", "d", "ps"), [(1, 16, 1, 128, 16), (3, 2, 5, 80, 7), (2, 1, 12, 256, 32)])
+def test_attend_few_units(cuda, cache_dtype, q_dtype, rows, kv_heads, group, d, ps):
+    """Few (row, key head) units, a cluster each, and the same with a table too wide for that."""
+    for lens in ([577, 0, 1][:rows], [1, 130, 64][:rows], [0, 0, 0][:rows]):
+        cache, q = _case(sum(lens), lens, kv_heads, group, d, ps, cache_dtype, q_dtype)
+        mass = torch.rand((rows, kv_heads, 600), device="cuda")
+        mass0 = mass.clone()
+        out = kv.attend(cache, q, _i32(lens), mass=mass)
+        _check_attend(cache, q, lens, out, mass=mass, mass0=mass0)
+        wide = torch.full((rows, 40000), -1, dtype=torch.int32, device="cuda")
+        wide[:, :cache.width] = cache.table
+        _check_attend(cache, q, lens, kv.attend(kv.PagedKV(cache.k, cache.v, wide), q, _i32(lens)))
+        cache.check()
+    table = cache.table.clone()
+    if rows > 1:
+        lens = [5, 6, 7][:rows]
+        cache, q = _case(3, lens, kv_heads, group, d, ps, cache_dtype, q_dtype)
+        table = cache.table.clone()
+        table[1, 0] = -9
+        out = kv.attend(kv.PagedKV(cache.k, cache.v, table), q, _i32(lens))
+        assert torch.isnan(out[1]).all() and not torch.isnan(out[0]).any()
+        assert torch.isnan(kv.attend(cache, q, _i32([5, -1, 7][:rows]))[1]).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("layout", ["nhd", "wide"])
 def test_attend_strides(cuda, dtype, layout):
