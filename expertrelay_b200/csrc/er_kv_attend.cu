@@ -11,13 +11,14 @@ constexpr int kSimtStages = 3;
 // then per warp a ring of kSimtStages chunks of keys and values, their rows
 // an odd number of 16-byte columns apart (no bank conflicts across keys).
 inline int simt_pitch(int d) { return d * 4 + ((d / 4) % 2 ? 0 : 16); }
-inline KernelShape simt_shape(int d, int group) {
+// `most`: 220 KB for one CTA an SM, half of it for two.
+inline KernelShape simt_shape(int d, int group, int most) {
   KernelShape s;
   s.heads = group <= 1 ? 1 : group <= 2 ? 2 : group <= 4 ? 4 : 8;
   for (s.warps = 4; s.warps > 1; s.warps /= 2) {
     s.smem = s.heads * d * 4 + s.warps * s.heads * (d + 4) * 4 + s.warps * s.heads * kKvChunk * 4 + 64 +
              s.warps * kSimtStages * (2 * kKvChunk * simt_pitch(d));
-    if (s.smem <= 220 * 1024) break;
+    if (s.smem <= most) break;
   }
   s.per_sm = 227 * 1024 / (s.smem + 3072);
   if (s.per_sm > 4) s.per_sm = 4;
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
       float s[GB];
 #pragma unroll
       for (int g = 0; g < GB; ++g) s[g] = 0.f;
+#pragma unroll 4
       for (int cc = lane >> 4; cc < cols; cc += 2) {
         const uint4 raw = *reinterpret_cast<const uint4*>(kc + key * pitch + cc * 16);
         const TC* kx = reinterpret_cast<const TC*>(&raw);
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
         for (int e = 0; e < 8; ++e) o[g][e] *= keep;
       }
       __syncwarp();
+#pragma unroll 4
       for (int r = kg; r < kKvChunk; r += kgs) {
         float p[GB];
 #pragma unroll
@@ -398,7 +401,8 @@ struct Layout {
 Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   Layout L;
   const int group = io.heads / c.kv_heads;
-  L.shape = c.dtype == ER_DTYPE_BF16 ? mma_shape(c.head_dim, group, io.q_dtype) : simt_shape(c.head_dim, group);
+  const bool mma = c.dtype == ER_DTYPE_BF16;
+  L.shape = mma ? mma_shape(c.head_dim, group, io.q_dtype) : simt_shape(c.head_dim, group, 220 * 1024);
   L.blocks = (group + L.shape.heads - 1) / L.shape.heads;
   L.grid = sms * L.shape.per_sm;
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
@@ -407,12 +411,17 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   // A cluster per unit or equal shares of all tiles. Against the shares the
   // clusters save about 7 tiles' time (no division of the line, no join), but
   // a unit has 8 CTAs at most: taken while its longest row costs those CTAs
-  // less than 7 tiles more than a share would be, and all clusters run at once.
-  const long long units = (long long)L.rows * c.kv_heads * L.blocks, tile = L.shape.warps * kKvChunk;
+  // less than 7 tiles more than a share would be, and all clusters run at
+  // once. That takes two CTAs an SM: with one, 16 clusters of 8 did not all
+  // find room in the processor clusters of 148 SMs, and 16 units of 640
+  // fp32 keys took 20 us, a wave after the other (14 by shares).
+  const KernelShape half = mma ? L.shape : simt_shape(c.head_dim, group, 108 * 1024);
+  const long long units = (long long)L.rows * c.kv_heads * L.blocks, tile = half.warps * kKvChunk, ctas = sms * 2;
   const long long longest =
       ((io.pages ? (long long)io.max_pages : (long long)c.table_width) * c.page_size + tile - 1) / tile;
-  L.cluster = L.rows == io.rows && units * kClusterCtas <= L.grid &&
-              longest * (L.grid - units * kClusterCtas) <= 7LL * kClusterCtas * L.grid;
+  L.cluster = L.rows == io.rows && half.per_sm >= 2 && units * kClusterCtas <= ctas &&
+              longest * (ctas - units * kClusterCtas) <= 7LL * kClusterCtas * ctas;
+  if (L.cluster) L.shape = half;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
