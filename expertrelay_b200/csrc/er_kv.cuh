@@ -86,6 +86,49 @@ __device__ __forceinline__ uint32_t rank_key(float f) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+constexpr int kClusterCtas = 8;  // of the kernels that run a cluster for each of few units
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return (int)r;
+}
+// Every thread of every CTA of the cluster arrives and waits; what was written before is seen after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of `addr` (shared memory) in the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+// Launch with programmatic stream serialization, in clusters of kClusterCtas when `cluster`.
+template <typename... KArgs, typename... Args>
+inline int kv_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, bool cluster, cudaStream_t st,
+                     const char* what, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kClusterCtas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...), what);
+}
+
+constexpr uint32_t kZeroKey = 0x80000000u;  // rank_key(0)
+
 // Exclusive prefix of `v` over the block's threads in thread order, and the
 // block's sum in *total. `red`: one int per warp plus one, shared.
 __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
@@ -120,10 +163,10 @@ struct RankKeys {
 };
 inline size_t rank_keys_bytes(long long n) { return (size_t)(n + n / 32 + 1) * 4; }
 
-// Bins of one pass of the select: 11, 11, then 10 bits. Four copies of the
-// histogram, by lane, where there are many keys: scores crowd into few bins
-// (a sum that is still zero, one binade) and shared-memory atomics on one
-// address run one by one.
+// Bins of one pass of the select: 11, 11, then 10 bits. Shared-memory atomics
+// on one address run one by one, and scores crowd into few bins: those of
+// exactly zero (sums that nothing was added to yet) are counted a warp at a
+// time, and many keys go to four copies of the histogram, by lane.
 constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
 constexpr size_t kSelectBytes = (size_t)kSelectBins * kSelectCopies * 4;
 
@@ -141,10 +184,16 @@ __device__ __forceinline__ uint32_t block_select(const RankKeys& key, int lo, in
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
     for (int b = threadIdx.x; b < copies * kSelectBins; b += blockDim.x) hist[b] = 0;
     __syncthreads();
-    for (int i = lo + (int)threadIdx.x; i < hi; i += blockDim.x) {
-      const uint32_t k = key(i);
-      if ((k & mask) == prefix) atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
+    int zeros = 0;  // of this warp
+#pragma unroll 2
+    for (int i0 = lo; i0 < hi; i0 += blockDim.x) {
+      const int i = i0 + (int)threadIdx.x;
+      const uint32_t k = i < hi ? key(i) : ~prefix;
+      const bool in = i < hi && (k & mask) == prefix, zero = in && k == kZeroKey;
+      zeros += __popc(__ballot_sync(0xffffffffu, zero));
+      if (in && !zero) atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
     }
+    if (zeros && (threadIdx.x & 31) == 0) atomicAdd(&mine[(kZeroKey >> shift) & (bins - 1)], zeros);
     __syncthreads();
     // thread t: `per` bins from the top
     const int per = (bins + blockDim.x - 1) / blockDim.x, top = bins - 1 - (int)threadIdx.x * per;

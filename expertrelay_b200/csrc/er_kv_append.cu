@@ -21,22 +21,25 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// VEC values as fp32, by 16-byte loads and stores where VEC is 8.
+// VEC values (16-byte loads where VEC is 8), and as fp32.
 template <int VEC, typename T>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[VEC]) {
-  if constexpr (VEC == 1) {
-    x[0] = to_f32(*p);
-  } else {
-    constexpr int N = 16 / sizeof(T);
+struct Vec {
+  static constexpr int N = VEC == 1 ? 1 : VEC * (int)sizeof(T) / 16;
+  uint4 raw[N];
+
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC == 1) {
+      *reinterpret_cast<T*>(raw) = *p;
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; i += N) {
-      const uint4 raw = ld_stream_u4(p + i);
-      const T* v = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[i + e] = to_f32(v[e]);
+      for (int i = 0; i < N; ++i) raw[i] = ld_stream_u4(p + i * (16 / sizeof(T)));
     }
   }
-}
+  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[e] = to_f32(reinterpret_cast<const T*>(raw)[e]);
+  }
+};
 template <int VEC, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
   if constexpr (VEC == 1) {
@@ -58,10 +61,10 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
 // copies two VECs of a v head. The products and sums of the rotation are
 // rounded one by one (no fused multiply-add), so a key's bits do not depend
 // on which half of the pair it is, and the pages' codes follow from the
-// formula alone. Memory-bound; the angles' sines (64 bits, half a row of
-// threads) run while the other CTAs of the SM have their rows in flight.
+// formula alone. Memory-bound: every thread has its values in flight before
+// the angles' sines (64 bits) are computed.
 template <typename TX, typename TQ, typename TC, int VEC>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
+__global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
                                                         const int32_t* __restrict__ seqs,
                                                         const int32_t* __restrict__ positions, int heads,
                                                         const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
@@ -69,13 +72,15 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __r
   __shared__ __align__(16) float cs[256];  // [d/2] cos, then [d/2] sin
   chain_wait();
   const int t = blockIdx.x, d = kv.d, half = d / 2, kvh = kv.kv_heads;
-  const int pos = positions[t], seq = seqs ? seqs[t] : t;
-  for (int j = threadIdx.x; j < half; j += blockDim.x) {
-    double s, c;
-    sincos((double)pos * inv.f[j], &s, &c);
-    cs[j] = (float)c;
-    cs[half + j] = (float)s;
+  const TX* row = qkv + (long long)t * ld;
+  const int per = half / VEC, tasks = (heads + 2 * kvh) * per;
+  Vec<VEC, TX> va, vb;
+  int i = threadIdx.x, head = i / per, j = i % per * VEC;
+  if (i < tasks) {
+    va.load(row + (long long)head * d + j);
+    vb.load(row + (long long)head * d + j + half);
   }
+  const int pos = positions[t], seq = seqs ? seqs[t] : t;
   char *kp = nullptr, *vp = nullptr;
   int bad = 0;
   if (seq < 0 || seq >= kv.seqs) {
@@ -93,14 +98,17 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __r
     }
   }
   if (bad && threadIdx.x == 0) kv_report(status, bad);
+  for (int f = threadIdx.x; f < half; f += blockDim.x) {
+    double s, c;
+    sincos((double)pos * inv.f[f], &s, &c);
+    cs[f] = (float)c;
+    cs[half + f] = (float)s;
+  }
   __syncthreads();
-  const TX* row = qkv + (long long)t * ld;
-  const int per = half / VEC;
-  for (int i = threadIdx.x; i < (heads + 2 * kvh) * per; i += blockDim.x) {
-    const int head = i / per, j = i % per * VEC;
+  while (i < tasks) {
     float a[VEC], b[VEC];
-    load_vec<VEC>(row + (long long)head * d + j, a);
-    load_vec<VEC>(row + (long long)head * d + j + half, b);
+    va.get(a);
+    vb.get(b);
     if (head < heads + kvh) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
@@ -120,6 +128,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView kv, const TX* __r
       store_vec<VEC>(o, a);
       store_vec<VEC>(o + half, b);
     }
+    i += blockDim.x;
+    if (i >= tasks) break;
+    head = i / per;
+    j = i % per * VEC;
+    va.load(row + (long long)head * d + j);
+    vb.load(row + (long long)head * d + j + half);
   }
 }
 
@@ -230,8 +244,10 @@ int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* se
               int heads, double theta, void* q_out, int* status, cudaStream_t st) {
   // 16-byte accesses need half a head in whole VECs and aligned rows
   const bool vec = kv.d % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)(ld * sizeof(TX))) & 15);
-  return launch_chained(vec ? kv_append_kernel<TX, TQ, TC, 8> : kv_append_kernel<TX, TQ, TC, 1>, dim3(n), dim3(256), 0,
-                        st, "kv_append_kernel", kv, (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d),
+  const int tasks = (heads + 2 * kv.kv_heads) * (kv.d / 2) / (vec ? 8 : 1);  // of a token
+  const int threads = tasks >= 512 ? 512 : (tasks + 31) / 32 * 32;
+  return launch_chained(vec ? kv_append_kernel<TX, TQ, TC, 8> : kv_append_kernel<TX, TQ, TC, 1>, dim3(n), dim3(threads),
+                        0, st, "kv_append_kernel", kv, (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d),
                         (TQ*)q_out, status);
 }
 

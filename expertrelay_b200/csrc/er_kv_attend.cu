@@ -369,7 +369,8 @@ int simt_launch(const AttendArgs& a, const KernelShape& s, cudaStream_t st) {
   auto kernel = kv_attend_simt_kernel<TQ, GB, WHOLE, CLUSTER>;
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, 224 * 1024, done)) return rc;
-  return attend_launch(kernel, a, s.warps * 32, s.smem, st, simt_pitch(a.kv.d));
+  return kv_launch(kernel, dim3(CLUSTER ? a.entries * a.units * kClusterCtas : a.grid), s.warps * 32, s.smem, CLUSTER, st,
+                   "kv_attend_simt_kernel", a, simt_pitch(a.kv.d));
 }
 
 template <typename TQ, int GB>
@@ -428,9 +429,10 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
     at += align_up(bytes, 256);
     return here;
   };
-  L.cut = take((size_t)L.grid * sizeof(CutUnit));
-  L.ml = take((size_t)L.grid * 2 * L.shape.heads * 2 * 4);
-  L.o = take((size_t)L.grid * 2 * L.shape.heads * c.head_dim * 4);
+  const size_t pieces = L.cluster ? 0 : (size_t)L.grid * 2 * L.shape.heads;  // two a CTA
+  L.cut = take(L.cluster ? 0 : (size_t)L.grid * sizeof(CutUnit));
+  L.ml = take(pieces * 2 * 4);
+  L.o = take(pieces * c.head_dim * 4);
   L.lse = take(io.mass ? (size_t)L.rows * io.heads * 4 : 0);
   L.scores = take(io.mass ? (size_t)L.rows * io.heads * io.mass_len * 4 : 0);
   L.bytes = at;
@@ -475,7 +477,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   const Layout L = attend_layout(*cache, *io, sms);
-  if (!workspace || workspace_bytes < L.bytes)
+  if (L.bytes && (!workspace || workspace_bytes < L.bytes))
     return fail(ER_ENOSPACE, "er_kv_attend: workspace %zu bytes, need %zu", workspace_bytes, L.bytes);
   if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_kv_attend: workspace must be 256-byte aligned");
   cudaStream_t st = (cudaStream_t)stream;

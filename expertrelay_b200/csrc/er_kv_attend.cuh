@@ -203,32 +203,12 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, RunScratch& s) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
 // 2^(m_i - m) of a piece, 0 for a piece without keys or of -inf scores alone.
 __device__ __forceinline__ float piece_weight(float mi, float m) { return mi == -INFINITY ? 0.f : exp2f(mi - m); }
 
 // With few units, each is a cluster's: its CTAs take an eighth of the tiles
 // each and join their pieces through one another's shared memory, so there is
 // no line to divide, no workspace and no second launch.
-constexpr int kClusterCtas = 8;
-
-__device__ __forceinline__ int cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return (int)r;
-}
-// Every thread of every CTA of the cluster arrives and waits; what was written before is seen after.
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// the address of `addr` (shared memory) in the cluster's CTA `rank`
-__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
 __device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
@@ -439,24 +419,5 @@ struct KernelShape {
 // the tensor-core kernel for bf16 caches (er_kv_attend_mma.cu)
 KernelShape mma_shape(int d, int group, int q_dtype);
 int attend_mma(const AttendArgs& a, int q_dtype, cudaStream_t st);
-
-// launch_chained, with clusters of kClusterCtas when a.cluster
-template <typename Kernel, typename... Args>
-int attend_launch(Kernel kernel, const AttendArgs& a, int threads, int smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.cluster ? a.entries * a.units * kClusterCtas : a.grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = kClusterCtas;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.cluster ? 2 : 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, a, args...), "kv_attend kernel");
-}
 
 }  // namespace er

@@ -441,7 +441,8 @@ int mma_launch(const AttendArgs& a, cudaStream_t st) {
   static_assert(NT * 8 * (DP + 2) * 4 <= MmaRing<DP, NT, QS>::kBytes, "a piece fits the ring");
   static std::atomic<unsigned long long> done;
   if (int rc = allow_smem(kernel, smem, done)) return rc;
-  return attend_launch(kernel, a, kMmaWarps * 32, smem, st);
+  return kv_launch(kernel, dim3(CLUSTER ? a.entries * a.units * kClusterCtas : a.grid), kMmaWarps * 32, smem, CLUSTER, st,
+                   "kv_attend_mma_kernel", a);
 }
 
 template <int DP, int NT, int QS>

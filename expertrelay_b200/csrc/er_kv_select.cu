@@ -9,28 +9,23 @@
 
 namespace er {
 
-constexpr int kScoreThreads = 256;
-
 // Page scores of one (row, key head): the group's queries as int8 codes
-// against the pages' int8 bounds. 8 codes of each bound per lane, `wide`
-// lanes a page. The dot products are exact integers (|I| <= 256 * 127^2 <
-// 2^24, so float(I) is exact too) and the two roundings after them are in a
-// fixed order: the scores, and so the choice, are the same on any grid.
+// against the pages' int8 bounds. The dot products are exact integers
+// (|I| <= 256 * 127^2 < 2^24, so float(I) is exact too) and the two roundings
+// after them are in a fixed order: the scores, and so the choice, are the
+// same on any grid.
+
+constexpr int kScoreThreads = 512;
+
+inline size_t codes_bytes(int group, int d) { return align_up((size_t)group * (2 * d + 4), 16); }
+
+// The group's queries as codes, by the whole block: qc [group][2][d], the
+// negative ones, then the positive ones; qt [group], the steps.
 template <typename TQ>
-__global__ void __launch_bounds__(kScoreThreads)
-    kv_score_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
-                    const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
-                    const float* __restrict__ scales, float* __restrict__ scores, int* status) {
-  extern __shared__ __align__(16) int8_t qc[];  // [group][2][d]: negative codes, positive codes; then [group] floats t
-  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
-  chain_wait();
-  const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads, d = kv.d;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int seq = seqs ? seqs[row] : row, len = lens[row];
-  if (seq < 0 || seq >= kv.seqs || len < 0 || len > kv.capacity()) return;  // reported by the selection
-  const int np = (len + kv.page_size - 1) / kv.page_size;
-  for (int g = warp; g < group; g += kScoreThreads / 32) {
-    const TQ* qr = q + (long long)row * q_stride + (long long)(h * group + g) * d;
+__device__ __forceinline__ void code_queries(const TQ* q, int group, int d, int8_t* qc, float* qt) {
+  const int lane = threadIdx.x & 31;
+  for (int g = threadIdx.x >> 5; g < group; g += blockDim.x >> 5) {
+    const TQ* qr = q + (long long)g * d;
     float top = 0.f;
     bool nan = false;
     for (int c = lane; c < d; c += 32) {
@@ -51,16 +46,25 @@ __global__ void __launch_bounds__(kScoreThreads)
     if (lane == 0) qt[g] = t;
   }
   __syncthreads();
-  const int cols = d / 8;  // 1 .. 32
+}
+
+// Scores of the pages [first, last) of a sequence; emit(o, score) by one lane
+// each. 8 codes of each bound a lane, `wide` lanes a page.
+template <typename Emit>
+__device__ __forceinline__ void score_pages(const KvView& kv, int seq, int h, int first, int last, int group,
+                                            const int8_t* qc, const float* qt, const int8_t* codes,
+                                            const float* scales, int* status, Emit emit) {
+  const int d = kv.d, cols = d / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // 1 .. 32 columns
   int wide = 1;
   while (wide < cols) wide *= 2;
-  const int col = lane % wide, per = 32 / wide;
-  float* out = scores + (long long)blockIdx.y * kv.width;
-  for (int o0 = (blockIdx.x * (kScoreThreads / 32) + warp) * per; o0 < np; o0 += gridDim.x * (kScoreThreads / 32) * per) {
+  const int col = lane % wide, per = 32 / wide, step = (blockDim.x >> 5) * per;
+  const int32_t* table = kv.pages_of(seq);
+#pragma unroll 2
+  for (int o0 = first + warp * per; o0 < last; o0 += step) {
     const int o = o0 + lane / wide;
-    const int page = o < np ? kv.pages_of(seq)[o] : -1;
+    const int page = o < last ? table[o] : -1;
     const bool ok = page >= 0 && page < kv.num_pages;
-    if (o < np && !ok && col == 0) kv_report(status, ER_KV_BAD_PAGE);
+    if (o < last && !ok && col == 0) kv_report(status, ER_KV_BAD_PAGE);
     uint2 lo = make_uint2(0, 0), hi = lo;
     float scale = 0.f;
     if (ok) {
@@ -88,32 +92,71 @@ __global__ void __launch_bounds__(kScoreThreads)
       nan |= v != v;
       best = fmaxf(best, v);
     }
-    if (o < np && col == 0) out[o] = nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale);
+    if (o < last && col == 0) emit(o, nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale));
   }
 }
 
+// What a row asks for: its sequence and how many pages that has, 0 when something is wrong with it.
+__device__ __forceinline__ int row_pages(const KvView& kv, const int32_t* seqs, const int32_t* lens, int row, int* seq,
+                                         int* bad) {
+  *seq = seqs ? seqs[row] : row;
+  const int len = lens[row];
+  *bad = *seq < 0 || *seq >= kv.seqs ? ER_KV_BAD_SEQ : len < 0 || len > kv.capacity() ? ER_KV_BAD_LENGTH : 0;
+  return *bad ? 0 : (int)(((long long)len + kv.page_size - 1) / kv.page_size);
+}
+
+// Scores alone, for tables too wide for shared memory.
+template <typename TQ>
+__global__ void __launch_bounds__(kScoreThreads)
+    kv_score_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
+                    const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
+                    const float* __restrict__ scales, float* __restrict__ scores, int* status) {
+  extern __shared__ __align__(16) int8_t qc[];
+  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
+  chain_wait();
+  const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads;
+  int seq, bad;
+  const int np = row_pages(kv, seqs, lens, row, &seq, &bad);  // what is wrong is reported by the choice
+  if (np == 0) return;
+  code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
+  float* out = scores + (long long)blockIdx.y * kv.width;
+  const int each = (np + gridDim.x - 1) / gridDim.x, first = min(np, (int)blockIdx.x * each);
+  score_pages(kv, seq, h, first, min(np, first + each), group, qc, qt, codes, scales, status,
+              [&](int o, float v) { out[o] = v; });
+}
+
+// The rank keys of n scores into shared memory, four scores a load from the first 16-byte boundary on.
+__device__ __forceinline__ void hold_keys(const float* scores, int n, uint32_t* held) {
+  const int skip = min(n, (int)((16 - ((uintptr_t)scores & 15)) & 15) / 4), quads = (n - skip) / 4;
+  for (int i = threadIdx.x; i < skip; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
+#pragma unroll 4
+  for (int q = threadIdx.x; q < quads; q += blockDim.x) {
+    const float4 x = *reinterpret_cast<const float4*>(scores + skip + q * 4);
+    const int i = skip + q * 4;
+    held[RankKeys::at(i)] = rank_key(x.x);
+    held[RankKeys::at(i + 1)] = rank_key(x.y);
+    held[RankKeys::at(i + 2)] = rank_key(x.z);
+    held[RankKeys::at(i + 3)] = rank_key(x.w);
+  }
+  for (int i = skip + quads * 4 + threadIdx.x; i < n; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
+  __syncthreads();
+}
+
 // Writes, ascending, the `take` of n positions that are forced (the first
-// `sinks`, the last `recent`) or rank best; emit(slot, i) for each. `held`:
-// room for the n keys in shared memory, or NULL.
+// `sinks`, the last `recent`) or rank best; emit(slot, i) for each.
 template <typename Emit>
-__device__ __forceinline__ void take_best(const float* scores, uint32_t* held, int n, int take, int sinks, int recent,
-                                          int* hist, int* red, Emit emit) {
+__device__ __forceinline__ void take_best(const RankKeys& key, int n, int take, int sinks, int recent, int* hist, int* red,
+                                          Emit emit) {
   if (n <= take) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) emit(i, i);
     return;
   }
   const int lo = sinks, hi = n - recent, want = take - sinks - recent;
-  if (held) {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < n; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
-    __syncthreads();
-  }
-  const RankKeys key{held, scores};
   uint32_t least = 0xffffffffu;
   int equal = 0;
   if (want > 0) least = block_select(key, lo, hi, want, hist, red, &equal);
   // in rounds of a run of positions a thread: one run takes them all when they are held
-  const int run = held ? (n + blockDim.x - 1) / blockDim.x : 8;
+  const int run = key.held ? (n + blockDim.x - 1) / blockDim.x : 8;
   int above = 0, same = 0;  // taken outright, and equal to the threshold, so far
   for (int i0 = 0; i0 < n; i0 += run * blockDim.x) {
     const int b = min(n, i0 + (int)threadIdx.x * run), e = min(n, b + run);
@@ -153,24 +196,72 @@ inline size_t take_smem(long long n, bool* held) {
 }
 inline int take_threads(long long n) { return n <= 1024 ? 256 : n <= 8192 ? 512 : kTakeThreads; }
 
+template <int THREADS>
+__device__ __forceinline__ void write_choice(const RankKeys& key, int n, int budget, int sinks, int recent, int* hist,
+                                             int* red, int32_t* out, int32_t* count) {
+  take_best(key, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
+  const int take = min(n, budget);
+  for (int i = take + threadIdx.x; i < budget; i += THREADS) out[i] = -1;
+  if (threadIdx.x == 0) *count = take;
+}
+
+// Scores and choice of one (row, key head) in one launch: a CTA, or with few
+// units a cluster whose CTAs score an eighth of the pages each, straight into
+// the shared memory of the first, which chooses.
+template <typename TQ, bool CLUSTER>
+__global__ void __launch_bounds__(kScoreThreads)
+    kv_pick_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
+                   const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
+                   const float* __restrict__ scales, int budget, int sinks, int recent, int32_t* __restrict__ pages,
+                   int32_t* __restrict__ counts, int* status) {
+  extern __shared__ __align__(16) char sm[];
+  __shared__ int red[kScoreThreads / 32 + 2];
+  int* hist = reinterpret_cast<int*>(sm);
+  int8_t* qc = reinterpret_cast<int8_t*>(sm + kSelectBytes);
+  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
+  uint32_t* held = reinterpret_cast<uint32_t*>(sm + kSelectBytes + (group * (2 * kv.d + 4) + 15) / 16 * 16);
+  chain_wait();
+  const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
+  const int row = unit / kv.kv_heads, h = unit % kv.kv_heads;
+  int seq, bad;
+  const int np = row_pages(kv, seqs, lens, row, &seq, &bad);
+  if (bad && rank == 0 && threadIdx.x == 0) kv_report(status, bad);
+  if (np > budget) {  // else all are taken, whatever they score
+    code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
+    if (CLUSTER) cluster_sync();  // the first CTA runs: its shared memory can be written
+    const int first = CLUSTER ? (int)((long long)np * rank / kClusterCtas) : 0;
+    const int last = CLUSTER ? (int)((long long)np * (rank + 1) / kClusterCtas) : np;
+    const uint32_t to = CLUSTER ? cluster_addr(smem_addr(held), 0) : smem_addr(held);
+    score_pages(kv, seq, h, first, last, group, qc, qt, codes, scales, status, [&](int o, float v) {
+      const uint32_t at = to + RankKeys::at(o) * 4, k = rank_key(v);
+      if (CLUSTER)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
+      else
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
+    });
+    if (CLUSTER)
+      cluster_sync();
+    else
+      __syncthreads();
+  }
+  if (rank == 0)
+    write_choice<kScoreThreads>(RankKeys{held, nullptr}, np, budget, sinks, recent, hist, red,
+                                pages + (long long)unit * budget, counts + unit);
+}
+
+// The choice alone, from scores in memory.
 __global__ void __launch_bounds__(kTakeThreads)
     kv_choose_kernel(KvView kv, const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-                     const float* __restrict__ scores, int budget, int sinks, int recent, int held,
+                     const float* __restrict__ scores, int budget, int sinks, int recent,
                      int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
   extern __shared__ int hist[];
   __shared__ int red[kTakeThreads / 32 + 2];
   chain_wait();
-  const int row = blockIdx.x / kv.kv_heads;
-  const int seq = seqs ? seqs[row] : row, len = lens[row];
-  const bool bad_seq = seq < 0 || seq >= kv.seqs, bad_len = len < 0 || len > kv.capacity();
-  if ((bad_seq || bad_len) && threadIdx.x == 0) kv_report(status, bad_seq ? ER_KV_BAD_SEQ : ER_KV_BAD_LENGTH);
-  const int n = bad_seq || bad_len ? 0 : (len + kv.page_size - 1) / kv.page_size;
-  const int take = min(n, budget);
-  int32_t* out = pages + (long long)blockIdx.x * budget;
-  take_best(scores + (long long)blockIdx.x * kv.width, held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr, n, budget,
-            sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
-  for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
-  if (threadIdx.x == 0) counts[blockIdx.x] = take;
+  int seq, bad;
+  const int n = row_pages(kv, seqs, lens, blockIdx.x / kv.kv_heads, &seq, &bad);
+  if (bad && threadIdx.x == 0) kv_report(status, bad);
+  write_choice<kTakeThreads>(RankKeys{nullptr, scores + (long long)blockIdx.x * kv.width}, n, budget, sinks, recent,
+                             hist, red, pages + (long long)blockIdx.x * budget, counts + blockIdx.x);
 }
 
 struct MassView {
@@ -193,21 +284,21 @@ __global__ void __launch_bounds__(kTakeThreads)
     n = 0;
   }
   const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
-  float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
   int32_t* out = kept + (long long)blockIdx.x * budget;
-  take_best(w, held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr, n, budget, sinks, recent, hist, red,
-            [&](int slot, int i) {
-              out[slot] = i;
-              to[slot] = w[i];
-            });
+  uint32_t* keys = held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr;
+  if (keys && n > budget) hold_keys(w, n, keys);
+  take_best(RankKeys{keys, w}, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
   const int take = min(n, budget);
   for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
   if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
 }
 
-// Rows of the kept positions, 16 bytes a lane, into the destination's pages.
-__global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, const int32_t* __restrict__ kept,
-                                                      int budget, int row_bytes, int* status) {
+// Rows of the kept positions, 16 bytes a lane, into the destination's pages,
+// and their weights. At 16 sequences of 8 key heads cut to 4096 positions of
+// 256 + 256 bytes it moves 6.3 TB/s.
+__global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, MassView m,
+                                                      const int32_t* __restrict__ kept, int budget, int row_bytes,
+                                                      int* status) {
   chain_wait();
   const int seq = blockIdx.y, h = blockIdx.z;
   const int cols = row_bytes / 16;
@@ -216,6 +307,8 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, co
     const int slot = (int)(i / cols), c = (int)(i % cols);
     const int src = list[slot];
     if (src < 0) continue;
+    if (c == 0)
+      m.to_mass[seq * m.to_seq_stride + h * m.to_head_stride + slot] = m.mass[seq * m.seq_stride + h * m.head_stride + src];
     const int a = from.pages_of(seq)[src / from.page_size], b = to.pages_of(seq)[slot / to.page_size];
     if (a < 0 || a >= from.num_pages || b < 0 || b >= to.num_pages) {
       if (c == 0) kv_report(status, ER_KV_BAD_PAGE);
@@ -234,8 +327,31 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, co
 
 using namespace er;
 
-extern "C" size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows) {
-  if (!cache || rows <= 0 || cache->kv_heads <= 0 || cache->table_width <= 0) return 0;
+namespace {
+
+// Shared memory of kv_pick_kernel; more than kPickSmem means that the scores go through the workspace.
+constexpr size_t kPickSmem = 200 * 1024;
+size_t pick_smem(int width, int group, int d) { return kSelectBytes + codes_bytes(group, d) + rank_keys_bytes(width); }
+
+template <typename TQ>
+int pick_go(const KvView& kv, const void* q, long long q_stride, int units, int group, const int32_t* seqs,
+            const int32_t* lens, const int8_t* codes, const float* scales, int budget, int sinks, int recent,
+            int32_t* pages, int32_t* counts, int* status, cudaStream_t st) {
+  const size_t smem = pick_smem(kv.width, group, kv.d);
+  const bool cluster = units * kClusterCtas <= 148 * 2;  // all at once
+  auto kernel = cluster ? kv_pick_kernel<TQ, true> : kv_pick_kernel<TQ, false>;
+  static std::atomic<unsigned long long> done[2];
+  if (int rc = allow_smem(kernel, kPickSmem, done[cluster])) return rc;
+  return kv_launch(kernel, dim3(cluster ? units * kClusterCtas : units), kScoreThreads, smem, cluster, st,
+                   "kv_pick_kernel", kv, (const TQ*)q, q_stride, group, seqs, lens, codes, scales, budget, sinks,
+                   recent, pages, counts, status);
+}
+
+}  // namespace
+
+extern "C" size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows, int heads) {
+  if (!cache || rows <= 0 || cache->kv_heads <= 0 || heads <= 0 || cache->table_width <= 0) return 0;
+  if (pick_smem(cache->table_width, heads / cache->kv_heads, cache->head_dim) <= kPickSmem) return 0;
   return align_up((size_t)rows * cache->kv_heads * cache->table_width * sizeof(float), 256);
 }
 
@@ -256,37 +372,31 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
   if (!q || !lens || !codes || !scales || !pages_out || !counts_out) return fail(ER_EINVAL, "er_kv_select: null pointer");
   if (((uintptr_t)codes & 7)) return fail(ER_EINVAL, "er_kv_select: codes must be 8-byte aligned");
   const int group = heads / cache->kv_heads;
-  const size_t smem = (size_t)group * (2 * cache->head_dim + 4);
-  if (smem > 48 * 1024) return fail(ER_EINVAL, "er_kv_select: %d queries a key head", group);
+  const size_t smem = codes_bytes(group, cache->head_dim);
+  if (smem > 40 * 1024) return fail(ER_EINVAL, "er_kv_select: %d queries a key head", group);
   if ((long long)rows * cache->kv_heads > 65535)
     return fail(ER_EINVAL, "er_kv_select: %d rows of %d key heads (at most 65535 in all)", rows, cache->kv_heads);
-  const size_t need = er_kv_select_workspace_bytes(cache, rows);
+  const size_t need = er_kv_select_workspace_bytes(cache, rows, heads);
   if (need && (!workspace || workspace_bytes < need))
     return fail(ER_ENOSPACE, "er_kv_select: workspace %zu bytes, need %zu", workspace_bytes, need);
   const KvView kv = kv_view(*cache);
   cudaStream_t st = (cudaStream_t)stream;
   const int units = rows * kv.kv_heads;
-  int wide = 1;
-  while (wide < kv.d / 8) wide *= 2;
-  const int per = kScoreThreads / wide;  // pages a CTA scores at a time
-  const long long most = (kv.width + per - 1) / per, want = 148 * 8 / units + 1;
-  const unsigned gx = (unsigned)(most < 1 ? 1 : most < want ? most : want);
-  int rc;
-  if (q_dtype == ER_DTYPE_BF16)
-    rc = launch_chained(kv_score_kernel<__nv_bfloat16>, dim3(gx, units), dim3(kScoreThreads), smem, st,
-                        "kv_score_kernel", kv, (const __nv_bfloat16*)q, q_stride, group, seqs, lens, codes, scales,
-                        (float*)workspace, status);
-  else
-    rc = launch_chained(kv_score_kernel<float>, dim3(gx, units), dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
-                        (const float*)q, q_stride, group, seqs, lens, codes, scales, (float*)workspace, status);
+  const bool qb = q_dtype == ER_DTYPE_BF16;
+  if (!need)
+    return qb ? pick_go<__nv_bfloat16>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent,
+                                       pages_out, counts_out, status, st)
+              : pick_go<float>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent,
+                               pages_out, counts_out, status, st);
+  const dim3 grid((unsigned)(148 * 4 / units + 1), units);
+  float* scores = (float*)workspace;
+  int rc = qb ? launch_chained(kv_score_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), smem, st, "kv_score_kernel",
+                               kv, (const __nv_bfloat16*)q, q_stride, group, seqs, lens, codes, scales, scores, status)
+              : launch_chained(kv_score_kernel<float>, grid, dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
+                               (const float*)q, q_stride, group, seqs, lens, codes, scales, scores, status);
   if (rc) return rc;
-  bool held;
-  const size_t take = take_smem(kv.width, &held);
-  static std::atomic<unsigned long long> done;
-  if ((rc = allow_smem(kv_choose_kernel, 200 * 1024, done))) return rc;
-  return launch_chained(kv_choose_kernel, dim3(units), dim3(take_threads(kv.width)), take, st, "kv_choose_kernel", kv,
-                        seqs, lens, (const float*)workspace, budget, sinks, recent, (int)held, pages_out, counts_out,
-                        status);
+  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), kSelectBytes, st, "kv_choose_kernel", kv,
+                        seqs, lens, (const float*)scores, budget, sinks, recent, pages_out, counts_out, status);
 }
 
 extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
@@ -324,6 +434,6 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;
   const long long most = ((long long)budget * (row_bytes / 16) + 255) / 256;
   const dim3 grid((unsigned)(most < want ? most : want), a.seqs, a.kv_heads);
-  return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, (const int32_t*)kept_out,
-                        budget, row_bytes, status);
+  return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, m,
+                        (const int32_t*)kept_out, budget, row_bytes, status);
 }

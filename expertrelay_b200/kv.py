@@ -59,7 +59,7 @@ def _weights(t, name: str, cache, rows: int, written: bool) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"{name}: expected [{rows}, {cache.kv_heads}, n] with contiguous positions")
     _need(t, name, torch.float32, cache.device, (rows, cache.kv_heads, t.shape[2]), contiguous=False)
-    if written and not _apart(t.shape, t.stride()):
+    if written and not t.is_contiguous() and not _apart(t.shape, t.stride()):
         raise ValueError(f"{name}: strides {t.stride()} make elements share memory")
 
 
@@ -100,6 +100,7 @@ class PagedKV:
         self.k, self.v, self.table = k, v, table
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.seqs, self.width = table.shape
+        self._apart = _apart(k.shape, k.stride())
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._status = self.status.data_ptr()
         self._c = _lib.KvCache(
@@ -115,7 +116,7 @@ class PagedKV:
         return torch._C._cuda_getCurrentRawStream(self._index)
 
     def _writable(self) -> None:
-        if not _apart(self.k.shape, self.k.stride()):
+        if not self._apart:
             raise ValueError(f"pools of strides {self.k.stride()} make slots share memory")
 
     def check(self) -> None:
@@ -178,7 +179,7 @@ def _row_args(cache: PagedKV, rows: int, lens: torch.Tensor, seqs: torch.Tensor 
 
 def _scratch(need: int, workspace: torch.Tensor | None, device: torch.device) -> torch.Tensor:
     if workspace is None:
-        return torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+        return torch.empty(need, dtype=torch.uint8, device=device)
     if workspace.device != device or not workspace.is_contiguous() or \
             workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace: {need} contiguous bytes on {device} needed")
@@ -232,7 +233,7 @@ def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.T
     rows, heads, stride = _queries(cache, q)
     _row_args(cache, rows, lens, seqs)
     if out is None:
-        out = torch.empty((rows, heads, cache.head_dim), dtype=q.dtype, device=cache.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     else:
         _need(out, "out", q.dtype, cache.device, (rows, heads, cache.head_dim))
     io = _lib.KvAttendIO(
@@ -260,8 +261,9 @@ def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.T
     need = cache._needs.get(sizes)
     if need is None:
         need = cache._needs[sizes] = lib.er_kv_attend_workspace_bytes(cache._ref, ref)
-    ws = _scratch(need, workspace, cache.device)
-    _lib.check(lib.er_kv_attend(cache._ref, ref, ws.data_ptr(), max(need, 16), cache._stream()), "er_kv_attend")
+    ws = _scratch(need, workspace, cache.device) if need else None
+    _lib.check(lib.er_kv_attend(cache._ref, ref, ws.data_ptr() if need else None, need, cache._stream()),
+               "er_kv_attend")
     return out
 
 
@@ -295,13 +297,13 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
     lib = _lib.lib()
     pages = torch.empty((rows, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
     counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
-    need = lib.er_kv_select_workspace_bytes(cache._ref, rows)
-    ws = _scratch(need, workspace, cache.device)
+    need = lib.er_kv_select_workspace_bytes(cache._ref, rows, heads)
+    ws = _scratch(need, workspace, cache.device) if need else None
     _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
                                 None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
                                 bounds._codes, bounds._scales, int(budget), int(sinks),
                                 int(recent), pages.data_ptr(), counts.data_ptr(), cache._status,
-                                ws.data_ptr(), max(need, 16), cache._stream()), "er_kv_select")
+                                ws.data_ptr() if need else None, need, cache._stream()), "er_kv_select")
     return pages, counts
 
 

@@ -370,6 +370,33 @@ def test_select_pages(cuda, dtype, group, d, ps, budget, sinks, recent):
     _check_attend(cache, q, lens, out, picks=picks)
 
 
+def test_select_from_a_table_too_wide_for_shared_memory(cuda):
+    lens = [1500, 0, 60000]
+    cache, q, bounds = _select_case(3, lens, 1, 2, 32, 1, F32)
+    pages, counts = kv.select_pages(cache, bounds, q, _i32(lens), 70, sinks=2, recent=3)
+    for r, (ids,) in enumerate(_want_pages(cache, bounds, q, lens, 70, 2, 3)):
+        assert pages[r, 0].tolist() == ids + [-1] * (70 - len(ids)) and counts[r, 0].item() == len(ids)
+    lens = [1000, 1500, 7]  # many units: one CTA each
+    cache, q, bounds = _select_case(4, lens, 16, 2, 64, 4, BF16)
+    pages, counts = kv.select_pages(cache, bounds, q, _i32(lens), 40, sinks=1, recent=1)
+    for r, row in enumerate(_want_pages(cache, bounds, q, lens, 40, 1, 1)):
+        for h, ids in enumerate(row):
+            assert pages[r, h].tolist() == ids + [-1] * (40 - len(ids)) and counts[r, h].item() == len(ids)
+
+
+def test_evict_more_than_shared_memory_holds(cuda):
+    gen = torch.Generator().manual_seed(9)
+    n, budget = 70000, 50
+    k = torch.randn((n // 100, 1, 100, 8), generator=gen).cuda()
+    cache = kv.PagedKV(k, k.clone(), torch.arange(n // 100, dtype=torch.int32, device="cuda")[None])
+    to = kv.PagedKV(torch.zeros((1, 1, 50, 8), device="cuda"), torch.zeros((1, 1, 50, 8), device="cuda"), _i32([[0]]))
+    mass = torch.randint(0, 20, (1, 1, n), generator=gen).float()
+    kept, new = kv.evict(cache, _i32([n]), mass.cuda(), to, torch.zeros((1, 1, 50), device="cuda"), budget, sinks=3, recent=7)
+    ids = choose(mass[0, 0].numpy(), n, budget, 3, 7)
+    assert kept[0, 0].tolist() == ids and new.tolist() == [budget]
+    assert torch.equal(to.k[0, 0], k.reshape(-1, 8)[ids])
+
+
 def test_select_ties_zeros_and_bad_rows(cuda):
     lens = [640, 640, 640, 640]
     cache, q, bounds = _select_case(4, lens, 1, 2, 64, 16, F32)
@@ -474,7 +501,8 @@ def test_refusals(cuda):
         (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens.long(), 4, 1e4), "positions"),
         (lambda: kv.attend(cache, q, lens, pages=_i32([[[0], [0]]] * 2), counts=_i32([[1, 1]] * 2),
                            mass=torch.zeros((2, 2, 64), device="cuda")), "not accumulated"),
-        (lambda: kv.attend(cache, q, lens, workspace=torch.empty(16, dtype=torch.uint8, device="cuda")), "workspace"),
+        (lambda: kv.attend(cache, q, lens, mass=torch.zeros((2, 2, 64), device="cuda"),
+                           workspace=torch.empty(16, dtype=torch.uint8, device="cuda")), "workspace"),
         (lambda: kv.append(cache, torch.zeros((2, 64), device="cuda"), lens, 4, 1e4), "qkv"),
         (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens, 4, 0.0), "theta"),
         (lambda: kv.append(cache, torch.zeros((2, 512), device="cuda"), lens, 4, 1e4, q_dtype=torch.half), "q_dtype"),

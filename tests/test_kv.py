@@ -69,8 +69,11 @@ def test_select_refusals():
                              (5, 5, "heads 5"), (7, None, "null"), (8, P + 4, "8-byte"), (10, 0, "budget 0"),
                              (11, 4, "budget 4"), (12, -1, "budget 4"), (4, 4, "4 rows, 3 sequences")]:
         _fails(L.er_kv_select(*[value if i == at else x for i, x in enumerate(args)]), words)
+    assert L.er_kv_select_workspace_bytes(C.byref(c), 3, 4) == 0
+    wide = _cache(table_width=60000)
+    args[0] = C.byref(wide)
     assert L.er_kv_select(*args) == _lib.ER_ENOSPACE and "workspace 0 bytes" in _lib.last_error()
-    assert L.er_kv_select_workspace_bytes(C.byref(c), 3) >= 3 * 2 * 4 * 4
+    assert L.er_kv_select_workspace_bytes(C.byref(wide), 3, 4) >= 3 * 2 * 60000 * 4
 
 
 def test_evict_refusals():
