@@ -86,6 +86,14 @@ __device__ __forceinline__ uint32_t rank_key(float f) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// First thing in every kernel: the next one of the chain may launch and run
+// up to here beside this one, and nothing of this one reads or writes memory
+// before all that was queued earlier is done.
+__device__ __forceinline__ void kv_enter() {
+  chain_trigger();
+  chain_wait();
+}
+
 constexpr int kClusterCtas = 8;  // of the kernels that run a cluster for each of few units
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -151,17 +159,28 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   return before + inc - v;
 }
 
-// Positions ranked by a score: their rank keys in shared memory where they
-// fit (a key behind every 32 is left out, so that runs of any length start in
-// different banks), else read from the scores each time.
-struct RankKeys {
-  uint32_t* held;
-  const float* scores;
-
-  __device__ __forceinline__ static int at(int i) { return i + (i >> 5); }
-  __device__ __forceinline__ uint32_t operator()(int i) const { return held ? held[at(i)] : rank_key(scores[i]); }
+// Positions ranked by a score, four at a time: their rank keys in shared
+// memory where they fit, else made from the scores each time. In shared
+// memory four places behind every 32 stay empty, so that threads which read
+// runs of 32 do so from different banks.
+struct HeldKeys {
+  const uint32_t* held;
+  __device__ __forceinline__ static int at(int i) { return i + ((i >> 5) << 2); }
+  // keys i .. i + 3, i a multiple of 4 (those behind the last are anything)
+  __device__ __forceinline__ uint4 four(int i, int) const { return *reinterpret_cast<const uint4*>(held + at(i)); }
 };
-inline size_t rank_keys_bytes(long long n) { return (size_t)(n + n / 32 + 1) * 4; }
+inline size_t held_bytes(long long n) { return (size_t)(n + n / 32 * 4 + 40) * 4; }
+struct ScoreKeys {
+  const float* scores;
+  __device__ __forceinline__ uint4 four(int i, int n) const {
+    uint4 k = make_uint4(0, 0, 0, 0);
+    k.x = rank_key(scores[i]);
+    if (i + 1 < n) k.y = rank_key(scores[i + 1]);
+    if (i + 2 < n) k.z = rank_key(scores[i + 2]);
+    if (i + 3 < n) k.w = rank_key(scores[i + 3]);
+    return k;
+  }
+};
 
 // Bins of one pass of the select: 11, 11, then 10 bits. Shared-memory atomics
 // on one address run one by one, and scores crowd into few bins: those of
@@ -170,12 +189,13 @@ inline size_t rank_keys_bytes(long long n) { return (size_t)(n + n / 32 + 1) * 4
 constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
 constexpr size_t kSelectBytes = (size_t)kSelectBins * kSelectCopies * 4;
 
-// The `want`-th largest of key(i), i in [lo, hi), by the whole block.
+// The `want`-th largest of the keys [lo, hi) of n, by the whole block.
 // Returns the threshold; *equal is how many of the keys equal to it belong to
 // the `want` largest (the lowest i first). 1 <= want <= hi - lo. `hist`:
 // kSelectBytes, `red`: one int per warp and two more, shared.
-__device__ __forceinline__ uint32_t block_select(const RankKeys& key, int lo, int hi, int want, int* hist, int* red,
-                                                 int* equal) {
+template <typename Keys>
+__device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo, int hi, int want, int* hist,
+                                                 int* red, int* equal) {
   const int copies = hi - lo >= kSelectMany ? kSelectCopies : 1, warps = blockDim.x >> 5;
   int* mine = hist + (copies > 1 ? (threadIdx.x & (kSelectCopies - 1)) * kSelectBins : 0);
   uint32_t prefix = 0, mask = 0;
@@ -184,15 +204,23 @@ __device__ __forceinline__ uint32_t block_select(const RankKeys& key, int lo, in
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
     for (int b = threadIdx.x; b < copies * kSelectBins; b += blockDim.x) hist[b] = 0;
     __syncthreads();
-    int zeros = 0;  // of this warp
+    int zeros = 0;  // of this thread
+    auto count = [&](uint32_t k, int i) {
+      if ((k & mask) != prefix || i < lo || i >= hi) return;
+      if (k == kZeroKey)
+        ++zeros;
+      else
+        atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
+    };
 #pragma unroll 2
-    for (int i0 = lo; i0 < hi; i0 += blockDim.x) {
-      const int i = i0 + (int)threadIdx.x;
-      const uint32_t k = i < hi ? key(i) : ~prefix;
-      const bool in = i < hi && (k & mask) == prefix, zero = in && k == kZeroKey;
-      zeros += __popc(__ballot_sync(0xffffffffu, zero));
-      if (in && !zero) atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
+    for (int i = lo / 4 * 4 + (int)threadIdx.x * 4; i < hi; i += blockDim.x * 4) {
+      const uint4 k = keys.four(i, n);
+      count(k.x, i);
+      count(k.y, i + 1);
+      count(k.z, i + 2);
+      count(k.w, i + 3);
     }
+    zeros = __reduce_add_sync(0xffffffffu, zeros);
     if (zeros && (threadIdx.x & 31) == 0) atomicAdd(&mine[(kZeroKey >> shift) & (bins - 1)], zeros);
     __syncthreads();
     // thread t: `per` bins from the top

@@ -57,94 +57,112 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
   }
 }
 
-// One CTA per token; a thread turns VEC pairs (j, j + d/2) of a head, or
-// copies two VECs of a v head. The products and sums of the rotation are
-// rounded one by one (no fused multiply-add), so a key's bits do not depend
-// on which half of the pair it is, and the pages' codes follow from the
-// formula alone. Memory-bound: every thread has its values in flight before
-// the angles' sines (64 bits) are computed.
-template <typename TX, typename TQ, typename TC, int VEC>
+// TOK tokens a CTA; a thread turns VEC pairs (j, j + d/2) of a head, or copies
+// two VECs of a v head, for each of them. The products and sums of the
+// rotation are rounded one by one (no fused multiply-add), so a key's bits do
+// not depend on which half of the pair it is, and the pages' codes follow
+// from the formula alone. Memory-bound, if enough is in flight: every thread
+// has its values of all TOK tokens under way before the angles' sines (64
+// bits) are computed, by TOK d/2 threads at once. One token a CTA while that
+// leaves SMs without work (a decode step), 4 for prompts (16384 tokens of
+// 16 + 16 + 16 heads: 98 us with one).
+template <typename TX, typename TQ, typename TC, int VEC, int TOK>
 __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
                                                         const int32_t* __restrict__ seqs,
-                                                        const int32_t* __restrict__ positions, int heads,
+                                                        const int32_t* __restrict__ positions, int n, int heads,
                                                         const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
                                                         int* status) {
-  __shared__ __align__(16) float cs[256];  // [d/2] cos, then [d/2] sin
-  chain_wait();
-  const int t = blockIdx.x, d = kv.d, half = d / 2, kvh = kv.kv_heads;
-  const TX* row = qkv + (long long)t * ld;
+  __shared__ __align__(16) float cs[TOK][256];  // [d/2] cos, then [d/2] sin
+  __shared__ long long slot[TOK];               // byte offset of the token's slot in the pools, -1: not written
+  kv_enter();
+  const int t0 = blockIdx.x * TOK, live = TOK == 1 ? 1 : min(TOK, n - t0);
+  const int d = kv.d, half = d / 2, kvh = kv.kv_heads;
+  const TX* row = qkv + (long long)t0 * ld;
   const int per = half / VEC, tasks = (heads + 2 * kvh) * per;
-  Vec<VEC, TX> va, vb;
+  Vec<VEC, TX> va[TOK], vb[TOK];
+  auto fetch = [&](int head, int j) {
+#pragma unroll
+    for (int k = 0; k < TOK; ++k)
+      if (k < live) {
+        va[k].load(row + k * ld + (long long)head * d + j);
+        vb[k].load(row + k * ld + (long long)head * d + j + half);
+      }
+  };
   int i = threadIdx.x, head = i / per, j = i % per * VEC;
-  if (i < tasks) {
-    va.load(row + (long long)head * d + j);
-    vb.load(row + (long long)head * d + j + half);
-  }
-  const int pos = positions[t], seq = seqs ? seqs[t] : t;
-  char *kp = nullptr, *vp = nullptr;
-  int bad = 0;
-  if (seq < 0 || seq >= kv.seqs) {
-    bad = ER_KV_BAD_SEQ;
-  } else if (pos < 0 || pos >= kv.capacity()) {
-    bad = ER_KV_BAD_LENGTH;
-  } else {
-    const int page = kv.pages_of(seq)[pos / kv.page_size];
-    if (page < 0 || page >= kv.num_pages) {
-      bad = ER_KV_BAD_PAGE;
+  if (i < tasks) fetch(head, j);
+  if ((int)threadIdx.x < live) {
+    const int t = t0 + threadIdx.x, pos = positions[t], seq = seqs ? seqs[t] : t;
+    long long off = -1;
+    int bad = 0;
+    if (seq < 0 || seq >= kv.seqs) {
+      bad = ER_KV_BAD_SEQ;
+    } else if (pos < 0 || pos >= kv.capacity()) {
+      bad = ER_KV_BAD_LENGTH;
     } else {
-      const long long off = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride;
-      kp = kv.k + off;
-      vp = kv.v + off;
+      const int page = kv.pages_of(seq)[pos / kv.page_size];
+      if (page < 0 || page >= kv.num_pages)
+        bad = ER_KV_BAD_PAGE;
+      else
+        off = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride;
     }
+    slot[threadIdx.x] = off;
+    if (bad) kv_report(status, bad);
   }
-  if (bad && threadIdx.x == 0) kv_report(status, bad);
-  for (int f = threadIdx.x; f < half; f += blockDim.x) {
+#pragma unroll 1
+  for (int f = threadIdx.x; f < live * half; f += blockDim.x) {
+    const int k = f / half, c0 = f - k * half;
     double s, c;
-    sincos((double)pos * inv.f[f], &s, &c);
-    cs[f] = (float)c;
-    cs[half + f] = (float)s;
+    sincos((double)positions[t0 + k] * inv.f[c0], &s, &c);
+    cs[k][c0] = (float)c;
+    cs[k][half + c0] = (float)s;
   }
   __syncthreads();
+#pragma unroll 1
   while (i < tasks) {
-    float a[VEC], b[VEC];
-    va.get(a);
-    vb.get(b);
-    if (head < heads + kvh) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float c = cs[j + e], s = cs[half + j + e], x = a[e], y = b[e];
-        a[e] = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
-        b[e] = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+    for (int k = 0; k < TOK; ++k) {
+      if (k >= live) break;
+      float a[VEC], b[VEC];
+      va[k].get(a);
+      vb[k].get(b);
+      if (head < heads + kvh) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float c = cs[k][j + e], s = cs[k][half + j + e], x = a[e], y = b[e];
+          a[e] = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
+          b[e] = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
+        }
       }
-    }
-    if (head < heads) {
-      TQ* o = q_out + ((long long)t * heads + head) * d + j;
-      store_vec<VEC>(o, a);
-      store_vec<VEC>(o + half, b);
-    } else if (!bad) {
-      const bool key = head < heads + kvh;
-      TC* o = reinterpret_cast<TC*>((key ? kp + (head - heads) * kv.head_stride
-                                         : vp + (head - heads - kvh) * kv.head_stride)) + j;
-      store_vec<VEC>(o, a);
-      store_vec<VEC>(o + half, b);
+      if (head < heads) {
+        TQ* o = q_out + ((long long)(t0 + k) * heads + head) * d + j;
+        store_vec<VEC>(o, a);
+        store_vec<VEC>(o + half, b);
+      } else if (slot[k] >= 0) {
+        const bool key = head < heads + kvh;
+        char* pool = key ? kv.k : kv.v;
+        const long long h = key ? head - heads : head - heads - kvh;
+        TC* o = reinterpret_cast<TC*>(pool + slot[k] + h * kv.head_stride) + j;
+        store_vec<VEC>(o, a);
+        store_vec<VEC>(o + half, b);
+      }
     }
     i += blockDim.x;
     if (i >= tasks) break;
     head = i / per;
     j = i % per * VEC;
-    va.load(row + (long long)head * d + j);
-    vb.load(row + (long long)head * d + j + half);
+    fetch(head, j);
   }
 }
 
 // Least and greatest key of every channel of a page, a warp per (page, key
 // head): the lanes split a slot's 16-byte columns, lane groups the slots.
-template <typename TC>
+// COLS: columns a lane (2 for fp32 rows over 512 bytes).
+template <typename TC, int COLS>
 __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t* __restrict__ lens,
                                                         const int32_t* __restrict__ start, int8_t* __restrict__ codes,
                                                         float* __restrict__ scales, int* status) {
   constexpr int V = 16 / sizeof(TC);
-  chain_wait();
+  kv_enter();
   const int seq = blockIdx.y, h = blockIdx.z, lane = threadIdx.x & 31;
   const int len = lens[seq], from = start[seq], ps = kv.page_size, d = kv.d;
   if (len < 0 || len > kv.capacity() || from < 0) {
@@ -157,6 +175,7 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
   while (wide < cols && wide < 32) wide *= 2;
   const int col = lane % wide, group = lane / wide, groups = 32 / wide;
   const int last = (len - 1) / ps;
+#pragma unroll 1
   for (int o = from / ps + blockIdx.x * 4 + (threadIdx.x >> 5); o <= last; o += gridDim.x * 4) {
     const int page = kv.pages_of(seq)[o];
     if (page < 0 || page >= kv.num_pages) {
@@ -165,13 +184,11 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
     }
     const int slots = min(ps, len - o * ps);
     const char* base = kv.k + page * kv.page_stride + h * kv.head_stride;
-    float lo[2][V], hi[2][V];
+    float lo[COLS][V], hi[COLS][V], top = 0.f;
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+    for (int w = 0; w < COLS; ++w) {
 #pragma unroll
       for (int e = 0; e < V; ++e) lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
       const int c = col + 32 * w;
       if (c < cols) {
 #pragma unroll 4
@@ -186,39 +203,43 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
           }
         }
       }
-    }
-    float top = 0.f;
+#pragma unroll 1
+      for (int x = wide; x < 32; x *= 2) {
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        for (int x = wide; x < 32; x *= 2) {
+        for (int e = 0; e < V; ++e) {
           lo[w][e] = fminf(lo[w][e], __shfl_xor_sync(0xffffffffu, lo[w][e], x));
           hi[w][e] = fmaxf(hi[w][e], __shfl_xor_sync(0xffffffffu, hi[w][e], x));
         }
-        if (col + 32 * w < cols && lo[w][e] <= hi[w][e]) top = fmaxf(top, fmaxf(fabsf(lo[w][e]), fabsf(hi[w][e])));
       }
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (c < cols && lo[w][e] <= hi[w][e]) top = fmaxf(top, fmaxf(fabsf(lo[w][e]), fabsf(hi[w][e])));
+    }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     const float scale = top * kCodeStep;
     const long long at = ((long long)page * kv.kv_heads + h) * 2 * d;
     if (lane == 0) scales[(long long)page * kv.kv_heads + h] = scale;
-    if (group == 0) {
+    if (group != 0) continue;
+    auto code = [&](float x) {  // 0 where there is no number; a division each, as the codes are defined
+      const float r = rintf(x / scale);
+      return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
+    };
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int c = col + 32 * w;
-        if (c < cols) {
+    for (int w = 0; w < COLS; ++w) {
+      const int c = col + 32 * w;
+      if (c >= cols) break;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float a = 0.f, b = 0.f;
-            if (scale > 0.f && lo[w][e] <= hi[w][e]) {
-              a = rintf(lo[w][e] / scale);
-              b = rintf(hi[w][e] / scale);
-            }
-            codes[at + c * V + e] = (int8_t)(a == a ? (int)fminf(fmaxf(a, -127.f), 127.f) : 0);
-            codes[at + d + c * V + e] = (int8_t)(b == b ? (int)fminf(fmaxf(b, -127.f), 127.f) : 0);
-          }
+      for (int e = 0; e < V; e += 4) {
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const bool some = scale > 0.f && lo[w][e + f] <= hi[w][e + f];
+          a |= (uint32_t)(uint8_t)(some ? code(lo[w][e + f]) : 0) << (8 * f);
+          b |= (uint32_t)(uint8_t)(some ? code(hi[w][e + f]) : 0) << (8 * f);
         }
+        *reinterpret_cast<uint32_t*>(codes + at + c * V + e) = a;
+        *reinterpret_cast<uint32_t*>(codes + at + d + c * V + e) = b;
       }
     }
   }
@@ -246,9 +267,12 @@ int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* se
   const bool vec = kv.d % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)(ld * sizeof(TX))) & 15);
   const int tasks = (heads + 2 * kv.kv_heads) * (kv.d / 2) / (vec ? 8 : 1);  // of a token
   const int threads = tasks >= 512 ? 512 : (tasks + 31) / 32 * 32;
-  return launch_chained(vec ? kv_append_kernel<TX, TQ, TC, 8> : kv_append_kernel<TX, TQ, TC, 1>, dim3(n), dim3(threads),
-                        0, st, "kv_append_kernel", kv, (const TX*)qkv, ld, seqs, positions, heads, inv_freq(theta, kv.d),
-                        (TQ*)q_out, status);
+  const bool many = vec && n >= 148 * 8;
+  return launch_chained(!vec   ? kv_append_kernel<TX, TQ, TC, 1, 1>
+                        : many ? kv_append_kernel<TX, TQ, TC, 8, 4>
+                               : kv_append_kernel<TX, TQ, TC, 8, 1>,
+                        dim3(many ? (n + 3) / 4 : n), dim3(threads), 0, st, "kv_append_kernel", kv, (const TX*)qkv, ld,
+                        seqs, positions, n, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
 }
 
 }  // namespace
@@ -290,6 +314,7 @@ extern "C" int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, 
   if (int rc = kv_check("er_kv_page_bounds", cache)) return rc;
   if (cache->seqs == 0 || cache->table_width == 0) return ER_OK;
   if (!lens || !start || !codes || !scales) return fail(ER_EINVAL, "er_kv_page_bounds: null pointer");
+  if ((uintptr_t)codes & 7) return fail(ER_EINVAL, "er_kv_page_bounds: codes must be 8-byte aligned");
   if (cache->seqs > 65535 || cache->kv_heads > 65535)
     return fail(ER_EINVAL, "er_kv_page_bounds: %d sequences, %d key heads", cache->seqs, cache->kv_heads);
   const KvView kv = kv_view(*cache);
@@ -298,9 +323,9 @@ extern "C" int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, 
   const long long want = 148 * 16 / ((long long)kv.seqs * kv.kv_heads), most = (kv.width + 3) / 4;
   const unsigned gx = (unsigned)(want < 1 ? 1 : want > most ? most : want);
   const dim3 grid(gx, kv.seqs, kv.kv_heads);
-  if (cache->dtype == ER_DTYPE_BF16)
-    return launch_chained(kv_bounds_kernel<__nv_bfloat16>, grid, dim3(128), 0, (cudaStream_t)stream,
-                          "kv_bounds_kernel", kv, lens, start, codes, scales, status);
-  return launch_chained(kv_bounds_kernel<float>, grid, dim3(128), 0, (cudaStream_t)stream, "kv_bounds_kernel", kv,
-                        lens, start, codes, scales, status);
+  return launch_chained(cache->dtype == ER_DTYPE_BF16 ? kv_bounds_kernel<__nv_bfloat16, 1>
+                        : kv.d > 128                  ? kv_bounds_kernel<float, 2>
+                                                      : kv_bounds_kernel<float, 1>,
+                        grid, dim3(128), 0, (cudaStream_t)stream, "kv_bounds_kernel", kv, lens, start, codes, scales,
+                        status);
 }

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   while (wide < cols && wide < 32) wide *= 2;
   const int col = lane % wide, kg = lane / wide, kgs = 32 / wide;
 
-  chain_wait();
+  kv_enter();
   // a cluster's CTA leaves its piece where its ring was
   float *piece_ml = reinterpret_cast<float*>(ring0), *piece_o = piece_ml + (GB * 2 + 3) / 4 * 4;
   const Run run = CLUSTER ? kv_cluster_run(a) : kv_run(a, scratch);
@@ -282,7 +282,7 @@ template <typename TQ>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttendArgs a, int gb) {
   extern __shared__ float wt[];  // [grid] weights, then [kJoinThreads][4] partial sums
   __shared__ float red[2][kJoinThreads / 32];
-  chain_wait();
+  kv_enter();
   const int g = blockIdx.y, d = a.kv.d;
   if (g == 0) {
     for (int x = blockIdx.x; x < a.entries; x += a.grid) {
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 
 // mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position.
 __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ AttendArgs a) {
-  chain_wait();
+  kv_enter();
   const int unit = blockIdx.y, row = unit / a.kv.kv_heads, h = unit % a.kv.kv_heads;
   const Entry e = kv_entry(a, row);
   float* to = a.mass + row * a.mass_row_stride + h * a.mass_head_stride;

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
       *reinterpret_cast<uint4*>(ring + i * 16) = make_uint4(0, 0, 0, 0);
     __syncwarp();
   }
-  chain_wait();
+  kv_enter();
   using TQ = std::conditional_t<QS == 1, __nv_bfloat16, float>;
   // a cluster's CTA leaves its piece where its ring was
   float *piece_ml = reinterpret_cast<float*>(sm), *piece_o = piece_ml + NT * 8 * 2;

@@ -48,51 +48,56 @@ __device__ __forceinline__ void code_queries(const TQ* q, int group, int d, int8
   __syncthreads();
 }
 
-// Scores of the pages [first, last) of a sequence; emit(o, score) by one lane
-// each. 8 codes of each bound a lane, `wide` lanes a page.
+// Scores of the pages [first, last) of a sequence; emit(o, score). A lane a
+// page: its row of codes comes in 8-byte loads whose sectors the next loads
+// find in L1, the queries' codes are broadcast from shared memory, and no
+// lane has to add up another's. kGroup queries at a time go over the row.
+constexpr int kGroup = 8;
 template <typename Emit>
 __device__ __forceinline__ void score_pages(const KvView& kv, int seq, int h, int first, int last, int group,
                                             const int8_t* qc, const float* qt, const int8_t* codes,
                                             const float* scales, int* status, Emit emit) {
-  const int d = kv.d, cols = d / 8, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // 1 .. 32 columns
-  int wide = 1;
-  while (wide < cols) wide *= 2;
-  const int col = lane % wide, per = 32 / wide, step = (blockDim.x >> 5) * per;
+  const int d = kv.d;
   const int32_t* table = kv.pages_of(seq);
-#pragma unroll 2
-  for (int o0 = first + warp * per; o0 < last; o0 += step) {
-    const int o = o0 + lane / wide;
-    const int page = o < last ? table[o] : -1;
-    const bool ok = page >= 0 && page < kv.num_pages;
-    if (o < last && !ok && col == 0) kv_report(status, ER_KV_BAD_PAGE);
-    uint2 lo = make_uint2(0, 0), hi = lo;
-    float scale = 0.f;
-    if (ok) {
-      const long long at = (long long)page * kv.kv_heads + h;
-      scale = scales[at];
-      if (col < cols) {
-        lo = *reinterpret_cast<const uint2*>(codes + at * 2 * d + col * 8);
-        hi = *reinterpret_cast<const uint2*>(codes + at * 2 * d + d + col * 8);
-      }
+  for (int o = first + (int)threadIdx.x; o < last; o += blockDim.x) {
+    const int page = table[o];
+    if (page < 0 || page >= kv.num_pages) {
+      kv_report(status, ER_KV_BAD_PAGE);
+      emit(o, __int_as_float(0x7fc00000));
+      continue;
     }
+    const long long at = (long long)page * kv.kv_heads + h;
+    const float scale = scales[at];
+    const uint2* row = reinterpret_cast<const uint2*>(codes + at * 2 * d);
     float best = -INFINITY;
-    bool nan = !ok;
-    for (int g = 0; g < group; ++g) {
-      int sum = 0;
-      if (col < cols) {
-        const uint2 neg = *reinterpret_cast<const uint2*>(qc + (g * 2 + 0) * d + col * 8);
-        const uint2 pos = *reinterpret_cast<const uint2*>(qc + (g * 2 + 1) * d + col * 8);
-        sum = __dp4a((int)neg.x, (int)lo.x, sum);
-        sum = __dp4a((int)neg.y, (int)lo.y, sum);
-        sum = __dp4a((int)pos.x, (int)hi.x, sum);
-        sum = __dp4a((int)pos.y, (int)hi.y, sum);
+    bool nan = false;
+    for (int g0 = 0; g0 < group; g0 += kGroup) {
+      int sum[kGroup];
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) sum[g] = 0;
+      const uint2* qr = reinterpret_cast<const uint2*>(qc + g0 * 2 * d);
+#pragma unroll 4
+      for (int c = 0; c < d / 8; ++c) {
+        const uint2 lo = row[c], hi = row[d / 8 + c];
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g) {
+          if (g0 + g >= group) break;
+          const uint2 neg = qr[(g * 2 + 0) * (d / 8) + c], pos = qr[(g * 2 + 1) * (d / 8) + c];
+          sum[g] = __dp4a((int)neg.x, (int)lo.x, sum[g]);
+          sum[g] = __dp4a((int)neg.y, (int)lo.y, sum[g]);
+          sum[g] = __dp4a((int)pos.x, (int)hi.x, sum[g]);
+          sum[g] = __dp4a((int)pos.y, (int)hi.y, sum[g]);
+        }
       }
-      for (int x = wide / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      const float v = __fmul_rn((float)sum, qt[g]);
-      nan |= v != v;
-      best = fmaxf(best, v);
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) {
+        if (g0 + g >= group) break;
+        const float v = __fmul_rn((float)sum[g], qt[g0 + g]);
+        nan |= v != v;
+        best = fmaxf(best, v);
+      }
     }
-    if (o < last && col == 0) emit(o, nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale));
+    emit(o, nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale));
   }
 }
 
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(kScoreThreads)
                     const float* __restrict__ scales, float* __restrict__ scores, int* status) {
   extern __shared__ __align__(16) int8_t qc[];
   float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
-  chain_wait();
+  kv_enter();
   const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads;
   int seq, bad;
   const int np = row_pages(kv, seqs, lens, row, &seq, &bad);  // what is wrong is reported by the choice
@@ -128,24 +133,30 @@ __global__ void __launch_bounds__(kScoreThreads)
 // The rank keys of n scores into shared memory, four scores a load from the first 16-byte boundary on.
 __device__ __forceinline__ void hold_keys(const float* scores, int n, uint32_t* held) {
   const int skip = min(n, (int)((16 - ((uintptr_t)scores & 15)) & 15) / 4), quads = (n - skip) / 4;
-  for (int i = threadIdx.x; i < skip; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
+  if ((int)threadIdx.x < skip) held[HeldKeys::at(threadIdx.x)] = rank_key(scores[threadIdx.x]);
 #pragma unroll 4
   for (int q = threadIdx.x; q < quads; q += blockDim.x) {
     const float4 x = *reinterpret_cast<const float4*>(scores + skip + q * 4);
     const int i = skip + q * 4;
-    held[RankKeys::at(i)] = rank_key(x.x);
-    held[RankKeys::at(i + 1)] = rank_key(x.y);
-    held[RankKeys::at(i + 2)] = rank_key(x.z);
-    held[RankKeys::at(i + 3)] = rank_key(x.w);
+    const uint4 k = make_uint4(rank_key(x.x), rank_key(x.y), rank_key(x.z), rank_key(x.w));
+    if (skip == 0) {
+      *reinterpret_cast<uint4*>(held + HeldKeys::at(i)) = k;
+    } else {
+      held[HeldKeys::at(i)] = k.x;
+      held[HeldKeys::at(i + 1)] = k.y;
+      held[HeldKeys::at(i + 2)] = k.z;
+      held[HeldKeys::at(i + 3)] = k.w;
+    }
   }
-  for (int i = skip + quads * 4 + threadIdx.x; i < n; i += blockDim.x) held[RankKeys::at(i)] = rank_key(scores[i]);
+  const int i = skip + quads * 4 + threadIdx.x;
+  if (i < n) held[HeldKeys::at(i)] = rank_key(scores[i]);
   __syncthreads();
 }
 
 // Writes, ascending, the `take` of n positions that are forced (the first
 // `sinks`, the last `recent`) or rank best; emit(slot, i) for each.
-template <typename Emit>
-__device__ __forceinline__ void take_best(const RankKeys& key, int n, int take, int sinks, int recent, int* hist, int* red,
+template <typename Keys, typename Emit>
+__device__ __forceinline__ void take_best(const Keys& keys, int n, int take, int sinks, int recent, int* hist, int* red,
                                           Emit emit) {
   if (n <= take) {
     for (int i = threadIdx.x; i < n; i += blockDim.x) emit(i, i);
@@ -154,35 +165,43 @@ __device__ __forceinline__ void take_best(const RankKeys& key, int n, int take, 
   const int lo = sinks, hi = n - recent, want = take - sinks - recent;
   uint32_t least = 0xffffffffu;
   int equal = 0;
-  if (want > 0) least = block_select(key, lo, hi, want, hist, red, &equal);
-  // in rounds of a run of positions a thread: one run takes them all when they are held
-  const int run = key.held ? (n + blockDim.x - 1) / blockDim.x : 8;
+  if (want > 0) least = block_select(keys, n, lo, hi, want, hist, red, &equal);
+  // in rounds of a run of 4, 8, .. 32 positions a thread
+  int run = 4;
+  while (run < 32 && run * (int)blockDim.x < n) run *= 2;
   int above = 0, same = 0;  // taken outright, and equal to the threshold, so far
   for (int i0 = 0; i0 < n; i0 += run * blockDim.x) {
-    const int b = min(n, i0 + (int)threadIdx.x * run), e = min(n, b + run);
-    int sure = 0, ties = 0;
-    for (int i = b; i < e; ++i) {
-      const bool forced = i < lo || i >= hi;
-      const uint32_t k = key(i);
-      sure += forced || (want > 0 && k > least);
-      ties += !forced && want > 0 && k == least;
+    const int b = i0 + (int)threadIdx.x * run;
+    uint32_t sure = 0, tied = 0;  // of the run's positions
+    for (int j = 0; j < run && b + j < n; j += 4) {
+      const uint4 k4 = keys.four(b + j, n);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = b + j + e;
+        const bool forced = i < lo || i >= hi;
+        if (i < n) {
+          sure |= (uint32_t)(forced || (want > 0 && k[e] > least)) << (j + e);
+          tied |= (uint32_t)(!forced && want > 0 && k[e] == least) << (j + e);
+        }
+      }
     }
-    int all_sure, all_ties;
-    int at = above + block_scan(sure, red, &all_sure);
-    int tie = same + block_scan(ties, red, &all_ties);
-    for (int i = b; i < e; ++i) {
-      const bool forced = i < lo || i >= hi;
-      const uint32_t k = key(i);
-      if (forced || (want > 0 && k > least)) {
-        emit(at + min(tie, equal), i);
+    // 16 bits each: a round has at most 32 * 1024 positions
+    int all;
+    const int before = block_scan(__popc(sure) | __popc(tied) << 16, red, &all);
+    int at = above + (before & 0xffff), tie = same + (before >> 16);
+    for (uint32_t left = sure | tied; left; left &= left - 1) {
+      const int j = __ffs(left) - 1;
+      if ((sure >> j) & 1) {
+        emit(at + min(tie, equal), b + j);
         ++at;
-      } else if (want > 0 && k == least) {
-        if (tie < equal) emit(at + tie, i);
+      } else {
+        if (tie < equal) emit(at + tie, b + j);
         ++tie;
       }
     }
-    above += all_sure;
-    same += all_ties;
+    above += all & 0xffff;
+    same += all >> 16;
   }
 }
 
@@ -191,15 +210,15 @@ constexpr int kTakeThreads = 1024;
 // Shared memory of a CTA that takes the best of at most n: the histograms,
 // and the keys where they fit beside them (*held).
 inline size_t take_smem(long long n, bool* held) {
-  *held = kSelectBytes + rank_keys_bytes(n) <= 200 * 1024;
-  return kSelectBytes + (*held ? rank_keys_bytes(n) : 0);
+  *held = kSelectBytes + held_bytes(n) <= 200 * 1024;
+  return kSelectBytes + (*held ? held_bytes(n) : 0);
 }
 inline int take_threads(long long n) { return n <= 1024 ? 256 : n <= 8192 ? 512 : kTakeThreads; }
 
-template <int THREADS>
-__device__ __forceinline__ void write_choice(const RankKeys& key, int n, int budget, int sinks, int recent, int* hist,
+template <int THREADS, typename Keys>
+__device__ __forceinline__ void write_choice(const Keys& keys, int n, int budget, int sinks, int recent, int* hist,
                                              int* red, int32_t* out, int32_t* count) {
-  take_best(key, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
+  take_best(keys, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
   const int take = min(n, budget);
   for (int i = take + threadIdx.x; i < budget; i += THREADS) out[i] = -1;
   if (threadIdx.x == 0) *count = take;
@@ -220,7 +239,7 @@ __global__ void __launch_bounds__(kScoreThreads)
   int8_t* qc = reinterpret_cast<int8_t*>(sm + kSelectBytes);
   float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
   uint32_t* held = reinterpret_cast<uint32_t*>(sm + kSelectBytes + (group * (2 * kv.d + 4) + 15) / 16 * 16);
-  chain_wait();
+  kv_enter();
   const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
   const int row = unit / kv.kv_heads, h = unit % kv.kv_heads;
   int seq, bad;
@@ -233,7 +252,7 @@ __global__ void __launch_bounds__(kScoreThreads)
     const int last = CLUSTER ? (int)((long long)np * (rank + 1) / kClusterCtas) : np;
     const uint32_t to = CLUSTER ? cluster_addr(smem_addr(held), 0) : smem_addr(held);
     score_pages(kv, seq, h, first, last, group, qc, qt, codes, scales, status, [&](int o, float v) {
-      const uint32_t at = to + RankKeys::at(o) * 4, k = rank_key(v);
+      const uint32_t at = to + HeldKeys::at(o) * 4, k = rank_key(v);
       if (CLUSTER)
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
       else
@@ -245,7 +264,7 @@ __global__ void __launch_bounds__(kScoreThreads)
       __syncthreads();
   }
   if (rank == 0)
-    write_choice<kScoreThreads>(RankKeys{held, nullptr}, np, budget, sinks, recent, hist, red,
+    write_choice<kScoreThreads>(HeldKeys{held}, np, budget, sinks, recent, hist, red,
                                 pages + (long long)unit * budget, counts + unit);
 }
 
@@ -256,12 +275,12 @@ __global__ void __launch_bounds__(kTakeThreads)
                      int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
   extern __shared__ int hist[];
   __shared__ int red[kTakeThreads / 32 + 2];
-  chain_wait();
+  kv_enter();
   int seq, bad;
   const int n = row_pages(kv, seqs, lens, blockIdx.x / kv.kv_heads, &seq, &bad);
   if (bad && threadIdx.x == 0) kv_report(status, bad);
-  write_choice<kTakeThreads>(RankKeys{nullptr, scores + (long long)blockIdx.x * kv.width}, n, budget, sinks, recent,
-                             hist, red, pages + (long long)blockIdx.x * budget, counts + blockIdx.x);
+  write_choice<kTakeThreads>(ScoreKeys{scores + (long long)blockIdx.x * kv.width}, n, budget, sinks, recent, hist, red,
+                             pages + (long long)blockIdx.x * budget, counts + blockIdx.x);
 }
 
 struct MassView {
@@ -276,7 +295,7 @@ __global__ void __launch_bounds__(kTakeThreads)
                    int held, int32_t* __restrict__ kept, int32_t* __restrict__ lens_out, int* status) {
   extern __shared__ int hist[];
   __shared__ int red[kTakeThreads / 32 + 2];
-  chain_wait();
+  kv_enter();
   const int seq = blockIdx.x / kv.kv_heads, h = blockIdx.x % kv.kv_heads;
   int n = lens[seq];
   if (n < 0 || n > kv.capacity() || n > m.len) {
@@ -285,21 +304,28 @@ __global__ void __launch_bounds__(kTakeThreads)
   }
   const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
   int32_t* out = kept + (long long)blockIdx.x * budget;
-  uint32_t* keys = held ? (uint32_t*)(hist + kSelectBytes / 4) : nullptr;
-  if (keys && n > budget) hold_keys(w, n, keys);
-  take_best(RankKeys{keys, w}, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
+  auto emit = [&](int slot, int i) { out[slot] = i; };
+  if (held) {
+    uint32_t* keys = (uint32_t*)(hist + kSelectBytes / 4);
+    if (n > budget) hold_keys(w, n, keys);
+    take_best(HeldKeys{keys}, n, budget, sinks, recent, hist, red, emit);
+  } else {
+    take_best(ScoreKeys{w}, n, budget, sinks, recent, hist, red, emit);
+  }
   const int take = min(n, budget);
   for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
   if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
+  __syncthreads();  // the list is written
+  float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < take; i += blockDim.x) to[i] = w[out[i]];
 }
 
-// Rows of the kept positions, 16 bytes a lane, into the destination's pages,
-// and their weights. At 16 sequences of 8 key heads cut to 4096 positions of
+// Rows of the kept positions, 16 bytes a lane, into the destination's pages. At 16 sequences of 8 key heads cut to 4096 positions of
 // 256 + 256 bytes it moves 6.3 TB/s.
-__global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, MassView m,
-                                                      const int32_t* __restrict__ kept, int budget, int row_bytes,
-                                                      int* status) {
-  chain_wait();
+__global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, const int32_t* __restrict__ kept,
+                                                      int budget, int row_bytes, int* status) {
+  kv_enter();
   const int seq = blockIdx.y, h = blockIdx.z;
   const int cols = row_bytes / 16;
   const int32_t* list = kept + ((long long)seq * from.kv_heads + h) * budget;
@@ -307,8 +333,6 @@ __global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, Ma
     const int slot = (int)(i / cols), c = (int)(i % cols);
     const int src = list[slot];
     if (src < 0) continue;
-    if (c == 0)
-      m.to_mass[seq * m.to_seq_stride + h * m.to_head_stride + slot] = m.mass[seq * m.seq_stride + h * m.head_stride + src];
     const int a = from.pages_of(seq)[src / from.page_size], b = to.pages_of(seq)[slot / to.page_size];
     if (a < 0 || a >= from.num_pages || b < 0 || b >= to.num_pages) {
       if (c == 0) kv_report(status, ER_KV_BAD_PAGE);
@@ -331,7 +355,7 @@ namespace {
 
 // Shared memory of kv_pick_kernel; more than kPickSmem means that the scores go through the workspace.
 constexpr size_t kPickSmem = 200 * 1024;
-size_t pick_smem(int width, int group, int d) { return kSelectBytes + codes_bytes(group, d) + rank_keys_bytes(width); }
+size_t pick_smem(int width, int group, int d) { return kSelectBytes + codes_bytes(group, d) + held_bytes(width); }
 
 template <typename TQ>
 int pick_go(const KvView& kv, const void* q, long long q_stride, int units, int group, const int32_t* seqs,
@@ -434,6 +458,6 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;
   const long long most = ((long long)budget * (row_bytes / 16) + 255) / 256;
   const dim3 grid((unsigned)(most < want ? most : want), a.seqs, a.kv_heads);
-  return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, m,
-                        (const int32_t*)kept_out, budget, row_bytes, status);
+  return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, (const int32_t*)kept_out,
+                        budget, row_bytes, status);
 }
