@@ -187,12 +187,14 @@ struct ScoreKeys {
 // exactly zero (sums that nothing was added to yet) are counted a warp at a
 // time, and many keys go to four copies of the histogram, by lane.
 constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
-constexpr size_t kSelectBytes = (size_t)kSelectBins * kSelectCopies * 4;
+inline __host__ __device__ size_t select_bytes(long long most) {  // of the histograms, for at most `most` keys
+  return (size_t)kSelectBins * (most >= kSelectMany ? kSelectCopies : 1) * 4;
+}
 
 // The `want`-th largest of the keys [lo, hi) of n, by the whole block.
 // Returns the threshold; *equal is how many of the keys equal to it belong to
 // the `want` largest (the lowest i first). 1 <= want <= hi - lo. `hist`:
-// kSelectBytes, `red`: one int per warp and two more, shared.
+// select_bytes(), `red`: one int per warp and two more, shared.
 template <typename Keys>
 __device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo, int hi, int want, int* hist,
                                                  int* red, int* equal) {

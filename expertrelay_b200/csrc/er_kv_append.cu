@@ -154,16 +154,21 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __r
   }
 }
 
-// Least and greatest key of every channel of a page, a warp per (page, key
-// head): the lanes split a slot's 16-byte columns, lane groups the slots.
-// COLS: columns a lane (2 for fp32 rows over 512 bytes).
+// Least and greatest key of every channel of a page, a CTA per (page, key
+// head): a warp's lanes split a slot's 16-byte columns, lane groups and warps
+// the slots, so that a page's loads are all under way at once (after a decode
+// step only one page of a sequence changes). The warps' results meet in
+// shared memory. COLS: columns a lane (2 for fp32 rows over 512 bytes).
+constexpr int kBoundsWarps = 4;
+
 template <typename TC, int COLS>
-__global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t* __restrict__ lens,
-                                                        const int32_t* __restrict__ start, int8_t* __restrict__ codes,
-                                                        float* __restrict__ scales, int* status) {
+__global__ void __launch_bounds__(kBoundsWarps * 32)
+    kv_bounds_kernel(KvView kv, const int32_t* __restrict__ lens, const int32_t* __restrict__ start,
+                     int8_t* __restrict__ codes, float* __restrict__ scales, int* status) {
   constexpr int V = 16 / sizeof(TC);
+  __shared__ __align__(16) float low[kBoundsWarps][COLS * 32 * V], high[kBoundsWarps][COLS * 32 * V];
   kv_enter();
-  const int seq = blockIdx.y, h = blockIdx.z, lane = threadIdx.x & 31;
+  const int seq = blockIdx.y, h = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int len = lens[seq], from = start[seq], ps = kv.page_size, d = kv.d;
   if (len < 0 || len > kv.capacity() || from < 0) {
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) kv_report(status, ER_KV_BAD_LENGTH);
@@ -173,13 +178,13 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
   const int cols = d / V;  // 1 .. 64
   int wide = 1;            // lanes across a slot
   while (wide < cols && wide < 32) wide *= 2;
-  const int col = lane % wide, group = lane / wide, groups = 32 / wide;
+  const int col = lane % wide, group = warp * (32 / wide) + lane / wide, groups = kBoundsWarps * (32 / wide);
   const int last = (len - 1) / ps;
 #pragma unroll 1
-  for (int o = from / ps + blockIdx.x * 4 + (threadIdx.x >> 5); o <= last; o += gridDim.x * 4) {
+  for (int o = from / ps + blockIdx.x; o <= last; o += gridDim.x) {
     const int page = kv.pages_of(seq)[o];
     if (page < 0 || page >= kv.num_pages) {
-      if (lane == 0) kv_report(status, ER_KV_BAD_PAGE);
+      if (threadIdx.x == 0) kv_report(status, ER_KV_BAD_PAGE);
       continue;
     }
     const int slots = min(ps, len - o * ps);
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
       for (int e = 0; e < V; ++e) lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
       const int c = col + 32 * w;
       if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
         for (int s = group; s < slots; s += groups) {
           const uint4 raw = *reinterpret_cast<const uint4*>(base + s * kv.slot_stride + c * 16);
           const TC* x = reinterpret_cast<const TC*>(&raw);
@@ -211,26 +216,49 @@ __global__ void __launch_bounds__(128) kv_bounds_kernel(KvView kv, const int32_t
           hi[w][e] = fmaxf(hi[w][e], __shfl_xor_sync(0xffffffffu, hi[w][e], x));
         }
       }
+      if (lane < wide && c < cols) {
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (c < cols && lo[w][e] <= hi[w][e]) top = fmaxf(top, fmaxf(fabsf(lo[w][e]), fabsf(hi[w][e])));
+        for (int e = 0; e < V; ++e) {
+          low[warp][c * V + e] = lo[w][e];
+          high[warp][c * V + e] = hi[w][e];
+        }
+      }
     }
+    __syncthreads();
+    // every warp joins all channels (for the scale); lane l has columns l and l + 32
+#pragma unroll
+    for (int w = 0; w < COLS; ++w) {
+      const int c = lane + 32 * w;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
+        if (c < cols) {
+#pragma unroll
+          for (int k = 0; k < kBoundsWarps; ++k) {
+            lo[w][e] = fminf(lo[w][e], low[k][c * V + e]);
+            hi[w][e] = fmaxf(hi[w][e], high[k][c * V + e]);
+          }
+          if (lo[w][e] <= hi[w][e]) top = fmaxf(top, fmaxf(fabsf(lo[w][e]), fabsf(hi[w][e])));
+        }
+      }
+    }
+    __syncthreads();  // the page after this one may be written
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     const float scale = top * kCodeStep;
     const long long at = ((long long)page * kv.kv_heads + h) * 2 * d;
-    if (lane == 0) scales[(long long)page * kv.kv_heads + h] = scale;
-    if (group != 0) continue;
+    if (threadIdx.x == 0) scales[(long long)page * kv.kv_heads + h] = scale;
     auto code = [&](float x) {  // 0 where there is no number; a division each, as the codes are defined
       const float r = rintf(x / scale);
       return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
     };
 #pragma unroll
     for (int w = 0; w < COLS; ++w) {
-      const int c = col + 32 * w;
+      const int c = lane + 32 * w;
       if (c >= cols) break;
 #pragma unroll
       for (int e = 0; e < V; e += 4) {
+        if (V == 8 ? e / 4 != warp % 2 || warp > 1 : warp > 0) continue;  // four channels a lane and warp
         uint32_t a = 0, b = 0;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {
@@ -320,7 +348,7 @@ extern "C" int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, 
   const KvView kv = kv_view(*cache);
   // a step touches one page a sequence, a prompt all of them: the CTAs of a
   // (sequence, key head) walk its pages, about 16 CTAs an SM in all
-  const long long want = 148 * 16 / ((long long)kv.seqs * kv.kv_heads), most = (kv.width + 3) / 4;
+  const long long want = 148 * 16 / ((long long)kv.seqs * kv.kv_heads), most = kv.width;
   const unsigned gx = (unsigned)(want < 1 ? 1 : want > most ? most : want);
   const dim3 grid(gx, kv.seqs, kv.kv_heads);
   return launch_chained(cache->dtype == ER_DTYPE_BF16 ? kv_bounds_kernel<__nv_bfloat16, 1>

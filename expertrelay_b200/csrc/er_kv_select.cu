@@ -10,94 +10,138 @@
 namespace er {
 
 // Page scores of one (row, key head): the group's queries as int8 codes
-// against the pages' int8 bounds. The dot products are exact integers
-// (|I| <= 256 * 127^2 < 2^24, so float(I) is exact too) and the two roundings
-// after them are in a fixed order: the scores, and so the choice, are the
-// same on any grid.
-
+// against the pages' int8 bounds, on the tensor cores. The dot products are
+// exact integers (|I| <= 256 * 127^2 < 2^24, so float(I) is exact too) and the
+// two roundings after them are in a fixed order: the scores, and so the
+// choice, are the same on any grid.
+//
+// A warp takes 16 pages against 8 queries (m16n8k32): in each 64 channels a
+// lane loads 16 consecutive codes of two pages, coalesced with its
+// neighbours, and they serve as its share of two products' channels; the
+// queries' codes lie in shared memory in the same order. (A lane a page, by
+// dp4a, touches 32 lines a load: 35 us for 256 (row, key head) pairs of 512
+// pages, and a page by 16 lanes with shuffles 47 us.)
 constexpr int kScoreThreads = 512;
 
-inline size_t codes_bytes(int group, int d) { return align_up((size_t)group * (2 * d + 4), 16); }
+inline __host__ __device__ int codes_pitch(int d) { return (d + 63) / 64 * 64 + 16; }  // of a query's codes of one sign
+inline __host__ __device__ int codes_bytes(int group, int d) {
+  const int heads = (group + 7) / 8 * 8;
+  return heads * 2 * codes_pitch(d) + heads * 4;
+}
 
-// The group's queries as codes, by the whole block: qc [group][2][d], the
-// negative ones, then the positive ones; qt [group], the steps.
+// The group's queries as codes, by the whole block: qc [heads][2][pitch], the
+// negative ones, then the positive ones, zeros behind head_dim and the group;
+// qt [heads], the steps. Returns whether a query is no number (no page ranks then).
 template <typename TQ>
-__device__ __forceinline__ void code_queries(const TQ* q, int group, int d, int8_t* qc, float* qt) {
-  const int lane = threadIdx.x & 31;
-  for (int g = threadIdx.x >> 5; g < group; g += blockDim.x >> 5) {
-    const TQ* qr = q + (long long)g * d;
-    float top = 0.f;
+__device__ __forceinline__ bool code_queries(const TQ* q, int group, int d, int8_t* qc, float* qt) {
+  const int lane = threadIdx.x & 31, heads = (group + 7) / 8 * 8, pitch = codes_pitch(d);
+  bool none = false;
+  for (int g = threadIdx.x >> 5; g < heads; g += blockDim.x >> 5) {
+    float x[8], top = 0.f;  // head_dim is 256 at the most
     bool nan = false;
-    for (int c = lane; c < d; c += 32) {
-      const float x = to_f32(qr[c]);
-      nan |= x != x;
-      top = fmaxf(top, fabsf(x));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = lane + 32 * i;
+      x[i] = g < group && c < d ? to_f32(q[(long long)g * d + c]) : 0.f;
+      nan |= x[i] != x[i];
+      top = fmaxf(top, fabsf(x[i]));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float t = top * kCodeStep;
-    if (__any_sync(0xffffffffu, nan)) t = __int_as_float(0x7fc00000);
-    for (int c = lane; c < d; c += 32) {
-      float r = t == 0.f ? 0.f : rintf(to_f32(qr[c]) / t);
+    const float t = top * kCodeStep;
+    none |= __any_sync(0xffffffffu, nan) || !(t < INFINITY);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = lane + 32 * i;
+      float r = t == 0.f ? 0.f : rintf(x[i] / t);
       r = r == r ? fminf(fmaxf(r, -127.f), 127.f) : 0.f;
-      qc[(g * 2 + 0) * d + c] = (int8_t)fminf(r, 0.f);
-      qc[(g * 2 + 1) * d + c] = (int8_t)fmaxf(r, 0.f);
+      if (c < pitch) {
+        qc[(g * 2 + 0) * pitch + c] = (int8_t)fminf(r, 0.f);
+        qc[(g * 2 + 1) * pitch + c] = (int8_t)fmaxf(r, 0.f);
+      }
     }
     if (lane == 0) qt[g] = t;
   }
-  __syncthreads();
+  return __syncthreads_or(none);
 }
 
-// Scores of the pages [first, last) of a sequence; emit(o, score). A lane a
-// page: its row of codes comes in 8-byte loads whose sectors the next loads
-// find in L1, the queries' codes are broadcast from shared memory, and no
-// lane has to add up another's. kGroup queries at a time go over the row.
-constexpr int kGroup = 8;
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 codes from channel c on, zeros behind head_dim (8-byte boundaries are all that is sure)
+__device__ __forceinline__ uint4 load_codes(const int8_t* row, int c, int d) {
+  uint4 x = make_uint4(0, 0, 0, 0);
+  if (row && c < d) {
+    if ((d & 15) == 0) {
+      x = *reinterpret_cast<const uint4*>(row + c);
+    } else {
+      const uint2 lo = *reinterpret_cast<const uint2*>(row + c);
+      x.x = lo.x;
+      x.y = lo.y;
+      if (c + 8 < d) {
+        const uint2 hi = *reinterpret_cast<const uint2*>(row + c + 8);
+        x.z = hi.x;
+        x.w = hi.y;
+      }
+    }
+  }
+  return x;
+}
+
+// Scores of the pages [first, last) of a sequence; emit(o, score) by one lane each.
 template <typename Emit>
 __device__ __forceinline__ void score_pages(const KvView& kv, int seq, int h, int first, int last, int group,
-                                            const int8_t* qc, const float* qt, const int8_t* codes,
+                                            const int8_t* qc, const float* qt, bool none, const int8_t* codes,
                                             const float* scales, int* status, Emit emit) {
-  const int d = kv.d;
+  const int d = kv.d, lane = threadIdx.x & 31, r = lane / 4, q = lane % 4, pitch = codes_pitch(d);
   const int32_t* table = kv.pages_of(seq);
-  for (int o = first + (int)threadIdx.x; o < last; o += blockDim.x) {
-    const int page = table[o];
-    if (page < 0 || page >= kv.num_pages) {
-      kv_report(status, ER_KV_BAD_PAGE);
-      emit(o, __int_as_float(0x7fc00000));
-      continue;
+  for (int o0 = first + (int)(threadIdx.x >> 5) * 16; o0 < last; o0 += (int)(blockDim.x >> 5) * 16) {
+    const int8_t* row[2];
+    float scale[2], best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int o = o0 + r + 8 * i, page = o < last ? table[o] : -1;
+      const bool ok = page >= 0 && page < kv.num_pages;
+      if (o < last && !ok && q == 0) kv_report(status, ER_KV_BAD_PAGE);
+      const long long at = ok ? (long long)page * kv.kv_heads + h : 0;
+      row[i] = ok ? codes + at * 2 * d : nullptr;
+      scale[i] = ok ? scales[at] : __int_as_float(0x7fc00000);
     }
-    const long long at = (long long)page * kv.kv_heads + h;
-    const float scale = scales[at];
-    const uint2* row = reinterpret_cast<const uint2*>(codes + at * 2 * d);
-    float best = -INFINITY;
-    bool nan = false;
-    for (int g0 = 0; g0 < group; g0 += kGroup) {
-      int sum[kGroup];
+#pragma unroll 1
+    for (int g0 = 0; g0 < group; g0 += 8) {
+      int sum[4] = {0, 0, 0, 0};
+#pragma unroll 2
+      for (int c0 = 0; c0 < d; c0 += 64) {
+        const int c = c0 + q * 16;
+        uint4 x[2][2];  // [least, greatest][page]
 #pragma unroll
-      for (int g = 0; g < kGroup; ++g) sum[g] = 0;
-      const uint2* qr = reinterpret_cast<const uint2*>(qc + g0 * 2 * d);
-#pragma unroll 4
-      for (int c = 0; c < d / 8; ++c) {
-        const uint2 lo = row[c], hi = row[d / 8 + c];
+        for (int i = 0; i < 2; ++i) {
+          x[0][i] = load_codes(row[i], c, d);
+          x[1][i] = load_codes(row[i] ? row[i] + d : nullptr, c, d);
+        }
 #pragma unroll
-        for (int g = 0; g < kGroup; ++g) {
-          if (g0 + g >= group) break;
-          const uint2 neg = qr[(g * 2 + 0) * (d / 8) + c], pos = qr[(g * 2 + 1) * (d / 8) + c];
-          sum[g] = __dp4a((int)neg.x, (int)lo.x, sum[g]);
-          sum[g] = __dp4a((int)neg.y, (int)lo.y, sum[g]);
-          sum[g] = __dp4a((int)pos.x, (int)hi.x, sum[g]);
-          sum[g] = __dp4a((int)pos.y, (int)hi.y, sum[g]);
+        for (int s = 0; s < 2; ++s) {
+          const uint4 b = *reinterpret_cast<const uint4*>(qc + ((g0 + r) * 2 + s) * pitch + c);
+          mma_s8(sum, x[s][0].x, x[s][1].x, x[s][0].y, x[s][1].y, b.x, b.y);
+          mma_s8(sum, x[s][0].z, x[s][1].z, x[s][0].w, x[s][1].w, b.z, b.w);
         }
       }
 #pragma unroll
-      for (int g = 0; g < kGroup; ++g) {
-        if (g0 + g >= group) break;
-        const float v = __fmul_rn((float)sum[g], qt[g0 + g]);
-        nan |= v != v;
-        best = fmaxf(best, v);
+      for (int e = 0; e < 4; ++e) {  // page r + 8 (e / 2), query 2 q + e % 2
+        const int g = g0 + q * 2 + (e & 1);
+        if (g < group) best[e >> 1] = fmaxf(best[e >> 1], __fmul_rn((float)sum[e], qt[g]));
       }
     }
-    emit(o, nan ? __int_as_float(0x7fc00000) : __fmul_rn(best, scale));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 1));
+      best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], 2));
+      const int o = o0 + r + 8 * i;
+      if (q == 0 && o < last) emit(o, none ? __int_as_float(0x7fc00000) : __fmul_rn(best[i], scale[i]));
+    }
   }
 }
 
@@ -117,16 +161,16 @@ __global__ void __launch_bounds__(kScoreThreads)
                     const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
                     const float* __restrict__ scales, float* __restrict__ scores, int* status) {
   extern __shared__ __align__(16) int8_t qc[];
-  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
+  float* qt = reinterpret_cast<float*>(qc + (group + 7) / 8 * 16 * codes_pitch(kv.d));
   kv_enter();
   const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads;
   int seq, bad;
   const int np = row_pages(kv, seqs, lens, row, &seq, &bad);  // what is wrong is reported by the choice
   if (np == 0) return;
-  code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
+  const bool none = code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
   float* out = scores + (long long)blockIdx.y * kv.width;
   const int each = (np + gridDim.x - 1) / gridDim.x, first = min(np, (int)blockIdx.x * each);
-  score_pages(kv, seq, h, first, min(np, first + each), group, qc, qt, codes, scales, status,
+  score_pages(kv, seq, h, first, min(np, first + each), group, qc, qt, none, codes, scales, status,
               [&](int o, float v) { out[o] = v; });
 }
 
@@ -210,8 +254,8 @@ constexpr int kTakeThreads = 1024;
 // Shared memory of a CTA that takes the best of at most n: the histograms,
 // and the keys where they fit beside them (*held).
 inline size_t take_smem(long long n, bool* held) {
-  *held = kSelectBytes + held_bytes(n) <= 200 * 1024;
-  return kSelectBytes + (*held ? held_bytes(n) : 0);
+  *held = select_bytes(n) + held_bytes(n) <= 200 * 1024;
+  return select_bytes(n) + (*held ? held_bytes(n) : 0);
 }
 inline int take_threads(long long n) { return n <= 1024 ? 256 : n <= 8192 ? 512 : kTakeThreads; }
 
@@ -236,9 +280,9 @@ __global__ void __launch_bounds__(kScoreThreads)
   extern __shared__ __align__(16) char sm[];
   __shared__ int red[kScoreThreads / 32 + 2];
   int* hist = reinterpret_cast<int*>(sm);
-  int8_t* qc = reinterpret_cast<int8_t*>(sm + kSelectBytes);
-  float* qt = reinterpret_cast<float*>(qc + group * 2 * kv.d);
-  uint32_t* held = reinterpret_cast<uint32_t*>(sm + kSelectBytes + (group * (2 * kv.d + 4) + 15) / 16 * 16);
+  int8_t* qc = reinterpret_cast<int8_t*>(sm + select_bytes(kv.width));
+  float* qt = reinterpret_cast<float*>(qc + (group + 7) / 8 * 16 * codes_pitch(kv.d));
+  uint32_t* held = reinterpret_cast<uint32_t*>(qc + codes_bytes(group, kv.d));
   kv_enter();
   const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
   const int row = unit / kv.kv_heads, h = unit % kv.kv_heads;
@@ -246,12 +290,13 @@ __global__ void __launch_bounds__(kScoreThreads)
   const int np = row_pages(kv, seqs, lens, row, &seq, &bad);
   if (bad && rank == 0 && threadIdx.x == 0) kv_report(status, bad);
   if (np > budget) {  // else all are taken, whatever they score
-    code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
+    const bool none =
+        code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
     if (CLUSTER) cluster_sync();  // the first CTA runs: its shared memory can be written
     const int first = CLUSTER ? (int)((long long)np * rank / kClusterCtas) : 0;
     const int last = CLUSTER ? (int)((long long)np * (rank + 1) / kClusterCtas) : np;
     const uint32_t to = CLUSTER ? cluster_addr(smem_addr(held), 0) : smem_addr(held);
-    score_pages(kv, seq, h, first, last, group, qc, qt, codes, scales, status, [&](int o, float v) {
+    score_pages(kv, seq, h, first, last, group, qc, qt, none, codes, scales, status, [&](int o, float v) {
       const uint32_t at = to + HeldKeys::at(o) * 4, k = rank_key(v);
       if (CLUSTER)
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
@@ -306,7 +351,7 @@ __global__ void __launch_bounds__(kTakeThreads)
   int32_t* out = kept + (long long)blockIdx.x * budget;
   auto emit = [&](int slot, int i) { out[slot] = i; };
   if (held) {
-    uint32_t* keys = (uint32_t*)(hist + kSelectBytes / 4);
+    uint32_t* keys = (uint32_t*)(hist + select_bytes(m.len) / 4);
     if (n > budget) hold_keys(w, n, keys);
     take_best(HeldKeys{keys}, n, budget, sinks, recent, hist, red, emit);
   } else {
@@ -355,7 +400,7 @@ namespace {
 
 // Shared memory of kv_pick_kernel; more than kPickSmem means that the scores go through the workspace.
 constexpr size_t kPickSmem = 200 * 1024;
-size_t pick_smem(int width, int group, int d) { return kSelectBytes + codes_bytes(group, d) + held_bytes(width); }
+size_t pick_smem(int width, int group, int d) { return select_bytes(width) + codes_bytes(group, d) + held_bytes(width); }
 
 template <typename TQ>
 int pick_go(const KvView& kv, const void* q, long long q_stride, int units, int group, const int32_t* seqs,
@@ -394,7 +439,7 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
   if (!seqs && rows > cache->seqs) return fail(ER_EINVAL, "er_kv_select: %d rows, %d sequences", rows, cache->seqs);
   if (rows == 0) return ER_OK;
   if (!q || !lens || !codes || !scales || !pages_out || !counts_out) return fail(ER_EINVAL, "er_kv_select: null pointer");
-  if (((uintptr_t)codes & 7)) return fail(ER_EINVAL, "er_kv_select: codes must be 8-byte aligned");
+  if (((uintptr_t)codes & 15)) return fail(ER_EINVAL, "er_kv_select: codes must be 16-byte aligned");
   const int group = heads / cache->kv_heads;
   const size_t smem = codes_bytes(group, cache->head_dim);
   if (smem > 40 * 1024) return fail(ER_EINVAL, "er_kv_select: %d queries a key head", group);
@@ -419,7 +464,7 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
               : launch_chained(kv_score_kernel<float>, grid, dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
                                (const float*)q, q_stride, group, seqs, lens, codes, scales, scores, status);
   if (rc) return rc;
-  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), kSelectBytes, st, "kv_choose_kernel", kv,
+  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), select_bytes(kv.width), st, "kv_choose_kernel", kv,
                         seqs, lens, (const float*)scores, budget, sinks, recent, pages_out, counts_out, status);
 }
 

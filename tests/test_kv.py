@@ -66,7 +66,7 @@ def test_select_refusals():
     L, c = _lib.lib(), _cache()
     args = [C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 1, 1, P, P, None, None, 0, None]
     for at, value, words in [(1, None, "null"), (2, 3, "q dtype"), (3, 8, "row stride"), (4, -2, "rows -2"),
-                             (5, 5, "heads 5"), (7, None, "null"), (8, P + 4, "8-byte"), (10, 0, "budget 0"),
+                             (5, 5, "heads 5"), (7, None, "null"), (8, P + 8, "16-byte"), (10, 0, "budget 0"),
                              (11, 4, "budget 4"), (12, -1, "budget 4"), (4, 4, "4 rows, 3 sequences")]:
         _fails(L.er_kv_select(*[value if i == at else x for i, x in enumerate(args)]), words)
     assert L.er_kv_select_workspace_bytes(C.byref(c), 3, 4) == 0
