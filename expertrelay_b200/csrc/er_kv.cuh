@@ -15,17 +15,24 @@ struct KvView {
   const int32_t* table;
   long long table_stride;
   int num_pages, page_size, kv_heads, d, seqs, width;
+  int shift;  // log2 of page_size, -1 when it is no power of two
 
   __device__ __forceinline__ const int32_t* pages_of(int seq) const { return table + (long long)seq * table_stride; }
+  // the ordinal of the page that holds a position, and the position's slot in it
+  __device__ __forceinline__ int ordinal(int pos) const { return shift >= 0 ? pos >> shift : pos / page_size; }
+  __device__ __forceinline__ int slot(int pos) const { return shift >= 0 ? pos & (page_size - 1) : pos % page_size; }
   // positions the table has room for (64 bits: width * page_size may pass 2^31)
   __device__ __forceinline__ long long capacity() const { return (long long)width * page_size; }
 };
 
 inline KvView kv_view(const er_kv_cache& c) {
   const long long es = c.dtype == ER_DTYPE_BF16 ? 2 : 4;
+  int shift = -1;
+  for (int b = 0; b < 31; ++b)
+    if (c.page_size == 1 << b) shift = b;
   return KvView{(char*)c.k,     (char*)c.v,  c.page_stride * es, c.head_stride * es, c.slot_stride * es, c.table,
                 c.table_stride, c.num_pages, c.page_size,        c.kv_heads,         c.head_dim,         c.seqs,
-                c.table_width};
+                c.table_width,  shift};
 }
 
 inline int kv_check(const char* who, const er_kv_cache* c) {

@@ -99,11 +99,11 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __r
     } else if (pos < 0 || pos >= kv.capacity()) {
       bad = ER_KV_BAD_LENGTH;
     } else {
-      const int page = kv.pages_of(seq)[pos / kv.page_size];
+      const int page = kv.pages_of(seq)[kv.ordinal(pos)];
       if (page < 0 || page >= kv.num_pages)
         bad = ER_KV_BAD_PAGE;
       else
-        off = page * kv.page_stride + (pos % kv.page_size) * kv.slot_stride;
+        off = page * kv.page_stride + kv.slot(pos) * kv.slot_stride;
     }
     slot[threadIdx.x] = off;
     if (bad) kv_report(status, bad);
@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __r
 // head): a warp's lanes split a slot's 16-byte columns, lane groups and warps
 // the slots, so that a page's loads are all under way at once (after a decode
 // step only one page of a sequence changes). The warps' results meet in
-// shared memory. COLS: columns a lane (2 for fp32 rows over 512 bytes).
+// shared memory. Where a CTA has several pages to do, each warp does its own
+// (4096 pages of 64 slots: 20 us, 35 with a CTA a page). COLS: columns a lane (2 for fp32 rows over 512 bytes).
 constexpr int kBoundsWarps = 4;
 
 template <typename TC, int COLS>
@@ -178,13 +179,16 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
   const int cols = d / V;  // 1 .. 64
   int wide = 1;            // lanes across a slot
   while (wide < cols && wide < 32) wide *= 2;
-  const int col = lane % wide, group = warp * (32 / wide) + lane / wide, groups = kBoundsWarps * (32 / wide);
-  const int last = (len - 1) / ps;
+  const int first = from / ps, last = (len - 1) / ps;
+  const bool solo = last - first >= 2 * (int)gridDim.x;  // the same for the whole CTA
+  const int each = solo ? kBoundsWarps : 1, mine = solo ? 0 : warp;
+  const int col = lane % wide, group = mine * (32 / wide) + lane / wide;
+  const int groups = (solo ? 1 : kBoundsWarps) * (32 / wide);
 #pragma unroll 1
-  for (int o = from / ps + blockIdx.x; o <= last; o += gridDim.x) {
+  for (int o = first + blockIdx.x * each + (solo ? warp : 0); o <= last; o += gridDim.x * each) {
     const int page = kv.pages_of(seq)[o];
     if (page < 0 || page >= kv.num_pages) {
-      if (threadIdx.x == 0) kv_report(status, ER_KV_BAD_PAGE);
+      if (lane == 0) kv_report(status, ER_KV_BAD_PAGE);
       continue;
     }
     const int slots = min(ps, len - o * ps);
@@ -216,7 +220,7 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
           hi[w][e] = fmaxf(hi[w][e], __shfl_xor_sync(0xffffffffu, hi[w][e], x));
         }
       }
-      if (lane < wide && c < cols) {
+      if (!solo && lane < wide && c < cols) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           low[warp][c * V + e] = lo[w][e];
@@ -224,17 +228,17 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
         }
       }
     }
-    __syncthreads();
+    if (!solo) __syncthreads();
     // every warp joins all channels (for the scale); lane l has columns l and l + 32
 #pragma unroll
     for (int w = 0; w < COLS; ++w) {
       const int c = lane + 32 * w;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
+        if (!solo) lo[w][e] = INFINITY, hi[w][e] = -INFINITY;
         if (c < cols) {
 #pragma unroll
-          for (int k = 0; k < kBoundsWarps; ++k) {
+          for (int k = 0; k < (solo ? 0 : kBoundsWarps); ++k) {
             lo[w][e] = fminf(lo[w][e], low[k][c * V + e]);
             hi[w][e] = fmaxf(hi[w][e], high[k][c * V + e]);
           }
@@ -242,12 +246,12 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
         }
       }
     }
-    __syncthreads();  // the page after this one may be written
+    if (!solo) __syncthreads();  // the page after this one may be written
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
     const float scale = top * kCodeStep;
     const long long at = ((long long)page * kv.kv_heads + h) * 2 * d;
-    if (threadIdx.x == 0) scales[(long long)page * kv.kv_heads + h] = scale;
+    if (lane == 0 && mine == 0) scales[(long long)page * kv.kv_heads + h] = scale;
     auto code = [&](float x) {  // 0 where there is no number; a division each, as the codes are defined
       const float r = rintf(x / scale);
       return r == r ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0;
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
       if (c >= cols) break;
 #pragma unroll
       for (int e = 0; e < V; e += 4) {
-        if (V == 8 ? e / 4 != warp % 2 || warp > 1 : warp > 0) continue;  // four channels a lane and warp
+        if (!solo && (V == 8 ? e / 4 != warp : warp > 0)) continue;  // four channels a lane and warp
         uint32_t a = 0, b = 0;
 #pragma unroll
         for (int f = 0; f < 4; ++f) {

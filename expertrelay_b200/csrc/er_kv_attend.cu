@@ -74,9 +74,11 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
   for (;;) {
     const bool work = filled == kSimtStages;
     StageInfo now = {};
-    if (work) {
-    now = info[warp][st];
-    if (fresh) {  // a new unit: its queries
+    if (work) now = info[warp][st];
+    // a new unit: its queries (the first unit's before the ring is filled,
+    // while its pages are looked up)
+    if (fresh && (work || filled == 0)) {
+      if (!work) now = walk.info(a, 0, GB);
       fresh = false;
       bad = false;
       first_t = now.t;
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
         for (int e = 0; e < 8; ++e) o[g][e] = 0.f;
       }
     }
+    if (work) {
     copy_wait<kSimtStages - 1>();
     __syncwarp();
     const uint32_t mask = now.keys;
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
     if (walk.ahead > 0) {  // the stage's next chunk
       long long off = 0;
       const uint32_t keys = walk.chunk(a, &off);
-      walk.note(a, keys, GB, &info[warp][st]);
+      if (lane == 0) info[warp][st] = walk.info(a, keys, GB);
       const uint32_t kd = smem_addr(ring + st * 2 * kKvChunk * pitch), vd = kd + kKvChunk * pitch;
 #pragma unroll 4
       for (int r = kg; r < kKvChunk; r += kgs) {
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(128) kv_attend_simt_kernel(const __grid_consta
 // found once, then threads split the pieces and the channels (four each).
 // The CTAs of g = 0 also write the rows without keys (zeros) and the bad
 // ones (NaN), which no attention CTA meets.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinPieces = 3;  // 768 pieces
 
 template <typename TQ>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_constant__ AttendArgs a, int gb) {
@@ -299,19 +302,28 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   const int shares = kv_shares(a, c.total), i0 = blockIdx.x;
   const int n = kv_share_of(c.total, shares, c.begin + kUnitCost + c.tiles - 1) - i0 + 1;  // pieces
   auto piece = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * gb + g; };
+  // a thread has pieces tid, tid + 256 and tid + 512 (CTAs, so pieces, are 4 an SM at the most)
+  float2 ml[kJoinPieces];
   float top = -INFINITY, sum = 0.f;
-  for (int k = threadIdx.x; k < n; k += kJoinThreads) top = fmaxf(top, a.part_ml[piece(k) * 2]);
+#pragma unroll
+  for (int j = 0; j < kJoinPieces; ++j) {
+    const int k = threadIdx.x + j * kJoinThreads;
+    ml[j] = k < n ? *reinterpret_cast<const float2*>(a.part_ml + piece(k) * 2) : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[j].x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (threadIdx.x % 32 == 0) red[0][threadIdx.x / 32] = top;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, red[0][w]);
-  for (int k = threadIdx.x; k < n; k += kJoinThreads) {
-    const float li = a.part_ml[piece(k) * 2 + 1];
-    const float by = li != li ? 1.f : piece_weight(a.part_ml[piece(k) * 2], top);  // a spoiled piece spoils the row
-    wt[k] = by;
-    sum = fmaf(li, by, sum);
+#pragma unroll
+  for (int j = 0; j < kJoinPieces; ++j) {
+    const int k = threadIdx.x + j * kJoinThreads;
+    if (k < n) {
+      wt[k] = piece_weight(ml[j].x, top);
+      sum = fmaf(ml[j].y, wt[k], sum);  // a spoiled piece's sum is NaN
+    }
   }
   sum = warp_sum(sum);
   if (threadIdx.x % 32 == 0) red[1][threadIdx.x / 32] = sum;
@@ -323,7 +335,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   const int col = threadIdx.x % cols, grp = threadIdx.x / cols;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < groups) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = grp; k < n; k += groups) {
       const float4 x = *reinterpret_cast<const float4*>(a.part_o + piece(k) * d + col * 4);
       const float by = wt[k];
@@ -406,6 +418,7 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   L.shape = mma ? mma_shape(c.head_dim, group, io.q_dtype) : simt_shape(c.head_dim, group, 220 * 1024);
   L.blocks = (group + L.shape.heads - 1) / L.shape.heads;
   L.grid = sms * L.shape.per_sm;
+  if (L.grid > kJoinThreads * kJoinPieces) L.grid = kJoinThreads * kJoinPieces;
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
   if (L.rows < 1) L.rows = 1;
   if (L.rows > io.rows) L.rows = io.rows;
@@ -506,9 +519,6 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
       a.counts = io->counts + (size_t)r0 * cache->kv_heads;
     }
     a.tile = L.shape.warps * kKvChunk;
-    a.shift = -1;
-    for (int b = 0; b < 31; ++b)
-      if (cache->page_size == 1 << b) a.shift = b;
     a.min_share = 2;
     a.status = io->status;
     a.entries = io->pages ? a.rows * cache->kv_heads : a.rows;

@@ -40,7 +40,6 @@ struct AttendArgs {
   const int32_t* counts;
   int max_pages;
   int tile;                    // keys a tile: warps a CTA * kKvChunk
-  int shift;                   // log2 of page_size, -1 when it is no power of two
   int min_share;               // the least share of the line worth a CTA
   int* status;
   // scan entries: rows, or (row, key head) pairs when each has its own page list
@@ -331,7 +330,7 @@ struct Walk {
     const int j = WHOLE ? (t + lane) * a.tile + warp * kKvChunk : t * a.tile + warp * kKvChunk + lane;
     more = 0;
     if (j >= e.n || j < 0 || (!WHOLE && lane >= kKvChunk)) return;
-    int o = a.shift >= 0 ? j >> a.shift : j / a.kv.page_size;
+    int o = a.kv.ordinal(j);
     const int slot = j - o * a.kv.page_size;
     int live = e.n - j;  // keys from j on
     if (a.pages) {
@@ -356,7 +355,7 @@ struct Walk {
       const int pg = __shfl_sync(0xffffffffu, page, t - win), n = __shfl_sync(0xffffffffu, more, t - win);
       if (pg < 0) return pg == -2 ? 0x10000u : 0u;
       const int j = t * a.tile + warp * kKvChunk;
-      const int slot = a.shift >= 0 ? j & (a.kv.page_size - 1) : j % a.kv.page_size;
+      const int slot = a.kv.slot(j);
       *off = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.slot_stride;
       return (1u << n) - 1;
     }
@@ -364,14 +363,8 @@ struct Walk {
     return __ballot_sync(0xffffffffu, page >= 0) | (__ballot_sync(0xffffffffu, page == -2) << 16);
   }
 
-  __device__ __forceinline__ void note(const AttendArgs& a, uint32_t keys, int block_heads, StageInfo* to) const {
-    if (lane) return;
-    to->keys = keys;
-    to->t = t;
-    to->tiles = tiles;
-    to->row = a.pages ? x / a.kv.kv_heads : x;
-    to->head = head;
-    to->g0 = u % a.blocks * block_heads;
+  __device__ __forceinline__ StageInfo info(const AttendArgs& a, uint32_t keys, int block_heads) const {
+    return StageInfo{keys, t, tiles, a.pages ? x / a.kv.kv_heads : x, head, u % a.blocks * block_heads, {0, 0}};
   }
 
   // to the next tile, if there is one

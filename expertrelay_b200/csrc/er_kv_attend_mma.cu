@@ -60,19 +60,21 @@ __device__ __forceinline__ uint32_t cut2(float& x, float& y) {
   return __byte_perm(a, b, 0x7632);
 }
 
-// Part `i` of three of a query, as bf16 bits. A part that is zero where the
-// query is not takes the least value of its sign (2^-133): times an infinite
-// key it has to stay infinite, and beside a finite one it vanishes.
-__device__ __forceinline__ uint32_t query_part(float x, int i) {
-  if (!(fabsf(x) < INFINITY)) return i == 0 ? (x != x ? 0x7fc0u : __float_as_uint(x) >> 16) : (__float_as_uint(x) >> 31 << 15 | 1u);
-  float rest = x;
-  uint32_t bits = 0;
-  for (int p = 0; p <= i; ++p) {
-    bits = __float_as_uint(rest) >> 16;
-    rest -= __uint_as_float(bits << 16);
-  }
-  if ((bits & 0x7fff) == 0 && x != 0.f) bits = __float_as_uint(x) >> 31 << 15 | 1u;
-  return bits;
+// A query as three bf16 parts (bits) whose sum it is exactly. A part that is
+// zero where the query is not takes the least value of its sign (2^-133):
+// times an infinite key it has to stay infinite, and beside a finite one it
+// vanishes.
+__device__ __forceinline__ void query_parts(float x, uint32_t (&p)[3]) {
+  const uint32_t tiny = __float_as_uint(x) >> 31 << 15 | 1u;
+  const bool finite = fabsf(x) < INFINITY;
+  p[0] = x != x ? 0x7fc0u : __float_as_uint(x) >> 16;
+  float rest = finite ? x - __uint_as_float(p[0] << 16) : 0.f;
+  p[1] = __float_as_uint(rest) >> 16;
+  rest -= __uint_as_float(p[1] << 16);
+  p[2] = __float_as_uint(rest) >> 16;
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if ((p[i] & 0x7fff) == 0 && x != 0.f) p[i] = tiny;
 }
 
 constexpr int kMmaWarps = 4;
@@ -158,9 +160,11 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
   for (;;) {
     const bool work = filled == S;
     StageInfo now = {};
-    if (work) {
-    now = info[warp][st];
-    if (fresh) {  // a new unit: its queries in the matrix instructions' order
+    if (work) now = info[warp][st];
+    // a new unit: its queries in the matrix instructions' order (the first
+    // unit's before the ring is filled, while its pages are looked up)
+    if (fresh && (work || filled == 0)) {
+      if (!work) now = walk.info(a, 0, NT * 8);
       fresh = false;
       bad = false;
       first_t = now.t;
@@ -185,11 +189,13 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
             const int cc = c0 + (e & 1) + (e >> 1) * 8;
             x[e] = g < live_g && cc < d ? reinterpret_cast<const float*>(a.q)[qat + (long long)g * d + cc] : 0.f;
           }
-#pragma unroll 1
+          uint32_t p[4][QS];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) query_parts(x[e], p[e]);
+#pragma unroll
           for (int part = 0; part < QS; ++part)
             qf[((ks * QS + part) * NT + nt) * 32 + ln] =
-                make_uint2(query_part(x[0], part) | query_part(x[1], part) << 16,
-                           query_part(x[2], part) | query_part(x[3], part) << 16);
+                make_uint2(p[0][part] | p[1][part] << 16, p[2][part] | p[3][part] << 16);
         }
       }
       if (threadIdx.x == 0) spoiled = 0;
@@ -202,6 +208,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
         for (int k = 0; k < KS; ++k) o[k][nt][0] = o[k][nt][1] = o[k][nt][2] = o[k][nt][3] = 0.f;
       }
     }
+    if (work) {
     copy_wait<S - 1>();
     __syncwarp();
     const uint32_t mask = now.keys;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, DP <= 128 && NT == 1 ? 2 : 1)
     if (walk.ahead > 0) {  // the stage's next chunk
       long long off = 0;
       const uint32_t keys = walk.chunk(a, &off);
-      walk.note(a, keys, NT * 8, &info[warp][st]);
+      if (lane == 0) info[warp][st] = walk.info(a, keys, NT * 8);
       const uint32_t kd = smem_addr(ring + st * 2 * Ring::kChunkBytes), vd = kd + Ring::kChunkBytes;
       if (col < cols || !WHOLE) {
         const long long step = kg * a.kv.slot_stride + col * 16;

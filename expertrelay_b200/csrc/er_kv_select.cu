@@ -335,61 +335,109 @@ struct MassView {
   int len, to_len;
 };
 
+// Copies a (sequence, key head)'s kept rows into the destination's pages, by
+// warps `warp`, warp + warps, .. : the lanes split a row's 16-byte columns,
+// lane groups the rows, four rows of a lane under way at once (list, pages
+// and values are three waits, one after the other).
+__device__ __forceinline__ void move_rows(const KvView& from, const KvView& to, int seq, int h, const int32_t* list,
+                                          int n, int row_bytes, int warp, int warps, int* status) {
+  constexpr int N = 4;
+  const int cols = row_bytes / 16, lane = threadIdx.x & 31;  // 1 .. 64 columns
+  int wide = 1;
+  while (wide < cols && wide < 32) wide *= 2;
+  const int per = 32 / wide, col = lane % wide;
+  const int32_t *ft = from.pages_of(seq), *tt = to.pages_of(seq);
+#pragma unroll 1
+  for (int s0 = warp * per * N + lane / wide; s0 < n; s0 += warps * per * N) {
+    int src[N], pa[N], pb[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) src[j] = s0 + j * per < n ? list[s0 + j * per] : -1;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      pa[j] = src[j] >= 0 ? ft[from.ordinal(src[j])] : 0;
+      pb[j] = src[j] >= 0 ? tt[to.ordinal(s0 + j * per)] : 0;
+    }
+#pragma unroll 1
+    for (int c = col; c < cols; c += 32) {
+      uint4 x[N], y[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (src[j] < 0) continue;
+        if (pa[j] < 0 || pa[j] >= from.num_pages || pb[j] < 0 || pb[j] >= to.num_pages) {
+          if (c == 0) kv_report(status, ER_KV_BAD_PAGE);
+          src[j] = -1;
+          continue;
+        }
+        const long long so =
+            pa[j] * from.page_stride + h * from.head_stride + from.slot(src[j]) * from.slot_stride + c * 16;
+        x[j] = ld_stream_u4(from.k + so);
+        y[j] = ld_stream_u4(from.v + so);
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (src[j] < 0) continue;
+        const long long de =
+            pb[j] * to.page_stride + h * to.head_stride + to.slot(s0 + j * per) * to.slot_stride + c * 16;
+        *reinterpret_cast<uint4*>(to.k + de) = x[j];
+        *reinterpret_cast<uint4*>(to.v + de) = y[j];
+      }
+    }
+  }
+}
+
+// The kept positions of a (sequence, key head) and their weights, by a CTA.
+// CLUSTER (few units): by the first CTA of a cluster, whose CTAs then move the
+// rows together; otherwise kv_move_kernel moves them.
+template <bool CLUSTER>
 __global__ void __launch_bounds__(kTakeThreads)
-    kv_keep_kernel(KvView kv, MassView m, const int32_t* __restrict__ lens, int budget, int sinks, int recent,
-                   int held, int32_t* __restrict__ kept, int32_t* __restrict__ lens_out, int* status) {
+    kv_keep_kernel(KvView kv, KvView dst, MassView m, const int32_t* __restrict__ lens, int budget, int sinks,
+                   int recent, int held, int row_bytes, int32_t* kept, int32_t* __restrict__ lens_out, int* status) {
   extern __shared__ int hist[];
   __shared__ int red[kTakeThreads / 32 + 2];
   kv_enter();
-  const int seq = blockIdx.x / kv.kv_heads, h = blockIdx.x % kv.kv_heads;
+  const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
+  const int seq = unit / kv.kv_heads, h = unit % kv.kv_heads;
   int n = lens[seq];
   if (n < 0 || n > kv.capacity() || n > m.len) {
-    if (threadIdx.x == 0 && h == 0) kv_report(status, ER_KV_BAD_LENGTH);
+    if (threadIdx.x == 0 && h == 0 && rank == 0) kv_report(status, ER_KV_BAD_LENGTH);
     n = 0;
   }
   const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
-  int32_t* out = kept + (long long)blockIdx.x * budget;
-  auto emit = [&](int slot, int i) { out[slot] = i; };
-  if (held) {
-    uint32_t* keys = (uint32_t*)(hist + select_bytes(m.len) / 4);
-    if (n > budget) hold_keys(w, n, keys);
-    take_best(HeldKeys{keys}, n, budget, sinks, recent, hist, red, emit);
-  } else {
-    take_best(ScoreKeys{w}, n, budget, sinks, recent, hist, red, emit);
-  }
+  int32_t* out = kept + (long long)unit * budget;
   const int take = min(n, budget);
-  for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
-  if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
-  __syncthreads();  // the list is written
-  float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
+  if (rank == 0) {
+    auto emit = [&](int slot, int i) { out[slot] = i; };
+    if (held) {
+      uint32_t* keys = (uint32_t*)(hist + select_bytes(m.len) / 4);
+      if (n > budget) hold_keys(w, n, keys);
+      take_best(HeldKeys{keys}, n, budget, sinks, recent, hist, red, emit);
+    } else {
+      take_best(ScoreKeys{w}, n, budget, sinks, recent, hist, red, emit);
+    }
+    for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
+    if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
+  }
+  if (CLUSTER)
+    cluster_sync();  // the list is written
+  else
+    __syncthreads();
+  if (rank == 0) {
+    float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < take; i += blockDim.x) to[i] = w[out[i]];
+    for (int i = threadIdx.x; i < take; i += blockDim.x) to[i] = w[out[i]];
+  }
+  if (CLUSTER)
+    move_rows(kv, dst, seq, h, out, take, row_bytes, rank * (blockDim.x >> 5) + (threadIdx.x >> 5),
+              kClusterCtas * (blockDim.x >> 5), status);
 }
 
-// Rows of the kept positions, 16 bytes a lane, into the destination's pages. At 16 sequences of 8 key heads cut to 4096 positions of
-// 256 + 256 bytes it moves 6.3 TB/s.
+// The rows of the kept positions. At 16 sequences of 8 key heads cut to 4096
+// positions of 256 + 256 bytes it moves 6.3 TB/s.
 __global__ void __launch_bounds__(256) kv_move_kernel(KvView from, KvView to, const int32_t* __restrict__ kept,
                                                       int budget, int row_bytes, int* status) {
   kv_enter();
-  const int seq = blockIdx.y, h = blockIdx.z;
-  const int cols = row_bytes / 16;
-  const int32_t* list = kept + ((long long)seq * from.kv_heads + h) * budget;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < (long long)budget * cols; i += gridDim.x * 256LL) {
-    const int slot = (int)(i / cols), c = (int)(i % cols);
-    const int src = list[slot];
-    if (src < 0) continue;
-    const int a = from.pages_of(seq)[src / from.page_size], b = to.pages_of(seq)[slot / to.page_size];
-    if (a < 0 || a >= from.num_pages || b < 0 || b >= to.num_pages) {
-      if (c == 0) kv_report(status, ER_KV_BAD_PAGE);
-      continue;
-    }
-    const long long so = a * from.page_stride + h * from.head_stride + (src % from.page_size) * from.slot_stride;
-    const long long de = b * to.page_stride + h * to.head_stride + (slot % to.page_size) * to.slot_stride;
-    const uint4 x = *reinterpret_cast<const uint4*>(from.k + so + c * 16);
-    const uint4 y = *reinterpret_cast<const uint4*>(from.v + so + c * 16);
-    *reinterpret_cast<uint4*>(to.k + de + c * 16) = x;
-    *reinterpret_cast<uint4*>(to.v + de + c * 16) = y;
-  }
+  move_rows(from, to, blockIdx.y, blockIdx.z, kept + ((long long)blockIdx.y * from.kv_heads + blockIdx.z) * budget,
+            budget, row_bytes, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8, status);
 }
 
 }  // namespace er
@@ -493,15 +541,22 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   cudaStream_t st = (cudaStream_t)stream;
   bool held;
   const size_t take = take_smem(mass_len, &held);
-  static std::atomic<unsigned long long> done;
-  if (int rc = allow_smem(kv_keep_kernel, 200 * 1024, done)) return rc;
-  if (int rc = launch_chained(kv_keep_kernel, dim3(a.seqs * a.kv_heads), dim3(take_threads(mass_len)), take, st,
-                              "kv_keep_kernel", a, m, lens, budget, sinks, recent, (int)held, kept_out, lens_out,
-                              status))
+  const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4), units = a.seqs * a.kv_heads;
+  // clusters all at once, each with little to move beside the choice (the
+  // second launch costs about what 64 MB take to move)
+  const bool cluster = units * kClusterCtas <= 148 * 2 && 2LL * units * budget * row_bytes <= 64ll << 20;
+  static std::atomic<unsigned long long> done[2];
+  if (int rc = cluster ? allow_smem(kv_keep_kernel<true>, 200 * 1024, done[1])
+                       : allow_smem(kv_keep_kernel<false>, 200 * 1024, done[0]))
     return rc;
-  const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4);
+  if (int rc = kv_launch(cluster ? kv_keep_kernel<true> : kv_keep_kernel<false>,
+                         dim3(cluster ? units * kClusterCtas : units), take_threads(mass_len), take, cluster, st,
+                         "kv_keep_kernel", a, b, m, lens, budget, sinks, recent, (int)held, row_bytes, kept_out,
+                         lens_out, status))
+    return rc;
+  if (cluster) return ER_OK;
   const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;
-  const long long most = ((long long)budget * (row_bytes / 16) + 255) / 256;
+  const long long most = (budget + 31) / 32;  // rows of a warp's first round, times 8
   const dim3 grid((unsigned)(most < want ? most : want), a.seqs, a.kv_heads);
   return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, (const int32_t*)kept_out,
                         budget, row_bytes, status);
