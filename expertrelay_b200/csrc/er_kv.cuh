@@ -157,13 +157,15 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   __syncthreads();  // `red` is free
   if (lane == 31) red[warp] = inc;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w < warp) before += red[w];
-    all += red[w];
+  const int mine = lane < warps ? red[lane] : 0;  // at most 32 warps
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += up;
   }
-  *total = all;
-  return before + inc - v;
+  *total = __shfl_sync(0xffffffffu, before, 31);
+  return __shfl_sync(0xffffffffu, before - mine, warp) + inc - v;
 }
 
 // Positions ranked by a score, four at a time: their rank keys in shared
@@ -193,7 +195,8 @@ struct ScoreKeys {
 // on one address run one by one, and scores crowd into few bins: those of
 // exactly zero (sums that nothing was added to yet) are counted a warp at a
 // time, and many keys go to four copies of the histogram, by lane.
-constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
+// Once a bin of few keys is found they are listed and ranked against one another instead.
+constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096, kSelectFew = 512;
 inline __host__ __device__ size_t select_bytes(long long most) {  // of the histograms, for at most `most` keys
   return (size_t)kSelectBins * (most >= kSelectMany ? kSelectCopies : 1) * 4;
 }
@@ -201,7 +204,7 @@ inline __host__ __device__ size_t select_bytes(long long most) {  // of the hist
 // The `want`-th largest of the keys [lo, hi) of n, by the whole block.
 // Returns the threshold; *equal is how many of the keys equal to it belong to
 // the `want` largest (the lowest i first). 1 <= want <= hi - lo. `hist`:
-// select_bytes(), `red`: one int per warp and two more, shared.
+// select_bytes(), `red`: one int per warp and four more, shared.
 template <typename Keys>
 __device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo, int hi, int want, int* hist,
                                                  int* red, int* equal) {
@@ -247,6 +250,8 @@ __device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo
         if (above < want && want <= above + n) {
           red[warps] = top - j;
           red[warps + 1] = want - above;
+          red[warps + 2] = n;
+          red[warps + 3] = 0;
         }
         above += n;
       }
@@ -255,6 +260,37 @@ __device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo
     prefix |= (uint32_t)red[warps] << shift;
     mask |= (uint32_t)(bins - 1) << shift;
     want = red[warps + 1];
+    const int few = red[warps + 2];
+    if (pass == 2 || few > kSelectFew) continue;
+    uint32_t* list = reinterpret_cast<uint32_t*>(hist);
+#pragma unroll 2
+    for (int i = lo / 4 * 4 + (int)threadIdx.x * 4; i < hi; i += blockDim.x * 4) {
+      const uint4 k4 = keys.four(i, n);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((k[e] & mask) == prefix && i + e >= lo && i + e < hi) list[atomicAdd(&red[warps + 3], 1)] = k[e];
+    }
+    __syncthreads();
+    for (int i = few + threadIdx.x; i < (few + 3) / 4 * 4; i += blockDim.x) list[i] = 0;  // below all that counts
+    __syncthreads();
+    for (int i = threadIdx.x; i < few; i += blockDim.x) {
+      const uint32_t k = list[i];
+      int more = 0, same = 0;
+#pragma unroll 4
+      for (int j = 0; j < few; j += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(list + j);
+        more += (x.x > k) + (x.y > k) + (x.z > k) + (x.w > k);
+        same += (x.x == k) + (x.y == k) + (x.z == k) + (x.w == k);
+      }
+      if (more < want && want <= more + same) {  // the threshold; its equals write the same
+        red[warps] = (int)k;
+        red[warps + 1] = want - more;
+      }
+    }
+    __syncthreads();
+    *equal = red[warps + 1];
+    return (uint32_t)red[warps];
   }
   *equal = want;
   return prefix;

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kBoundsWarps * 32)
   int wide = 1;            // lanes across a slot
   while (wide < cols && wide < 32) wide *= 2;
   const int first = from / ps, last = (len - 1) / ps;
-  const bool solo = last - first >= 2 * (int)gridDim.x;  // the same for the whole CTA
+  const bool solo = last - first >= (int)gridDim.x;  // the same for the whole CTA
   const int each = solo ? kBoundsWarps : 1, mine = solo ? 0 : warp;
   const int col = lane % wide, group = mine * (32 / wide) + lane / wide;
   const int groups = (solo ? 1 : kBoundsWarps) * (32 / wide);

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kScoreThreads)
 __device__ __forceinline__ void hold_keys(const float* scores, int n, uint32_t* held) {
   const int skip = min(n, (int)((16 - ((uintptr_t)scores & 15)) & 15) / 4), quads = (n - skip) / 4;
   if ((int)threadIdx.x < skip) held[HeldKeys::at(threadIdx.x)] = rank_key(scores[threadIdx.x]);
-#pragma unroll 4
+#pragma unroll 8
   for (int q = threadIdx.x; q < quads; q += blockDim.x) {
     const float4 x = *reinterpret_cast<const float4*>(scores + skip + q * 4);
     const int i = skip + q * 4;
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kScoreThreads)
                    const float* __restrict__ scales, int budget, int sinks, int recent, int32_t* __restrict__ pages,
                    int32_t* __restrict__ counts, int* status) {
   extern __shared__ __align__(16) char sm[];
-  __shared__ int red[kScoreThreads / 32 + 2];
+  __shared__ int red[kScoreThreads / 32 + 4];
   int* hist = reinterpret_cast<int*>(sm);
   int8_t* qc = reinterpret_cast<int8_t*>(sm + select_bytes(kv.width));
   float* qt = reinterpret_cast<float*>(qc + (group + 7) / 8 * 16 * codes_pitch(kv.d));
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kTakeThreads)
                      const float* __restrict__ scores, int budget, int sinks, int recent,
                      int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
   extern __shared__ int hist[];
-  __shared__ int red[kTakeThreads / 32 + 2];
+  __shared__ int red[kTakeThreads / 32 + 4];
   kv_enter();
   int seq, bad;
   const int n = row_pages(kv, seqs, lens, blockIdx.x / kv.kv_heads, &seq, &bad);
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kTakeThreads)
     kv_keep_kernel(KvView kv, KvView dst, MassView m, const int32_t* __restrict__ lens, int budget, int sinks,
                    int recent, int held, int row_bytes, int32_t* kept, int32_t* __restrict__ lens_out, int* status) {
   extern __shared__ int hist[];
-  __shared__ int red[kTakeThreads / 32 + 2];
+  __shared__ int red[kTakeThreads / 32 + 4];
   kv_enter();
   const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
   const int seq = unit / kv.kv_heads, h = unit % kv.kv_heads;
