@@ -41,6 +41,7 @@ inline int kv_check(const char* who, const er_kv_cache* c) {
   if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->seqs < 0 || c->table_width < 0)
     return fail(ER_EINVAL, "%s: %d pages of %d positions, %d key heads, table of %d x %d", who, c->num_pages,
                 c->page_size, c->kv_heads, c->seqs, c->table_width);
+  if (c->kv_heads > 1024) return fail(ER_EINVAL, "%s: %d key heads (at most 1024)", who, c->kv_heads);
   if (c->head_dim <= 0 || c->head_dim % 8 || c->head_dim > 256)
     return fail(ER_EINVAL, "%s: head_dim %d (a multiple of 8, at most 256)", who, c->head_dim);
   if (!c->k || !c->v || (c->seqs > 0 && c->table_width > 0 && !c->table)) return fail(ER_EINVAL, "%s: null pointer", who);

@@ -17,7 +17,7 @@
 namespace er {
 
 constexpr int kKvMaxLen = 0x7fff0000;  // positions stay ints with a tile's keys added
-constexpr int kKvChunk = 16;  // keys a warp takes at a time
+constexpr int kKvSegment = 8;           // keys that are looked up together where pages allow
 
 // A unit whose tiles several CTAs share: the first of them writes it, the join reads it.
 struct CutUnit {
@@ -39,7 +39,7 @@ struct AttendArgs {
   const int32_t* pages;        // optional page lists [rows, kv_heads, max_pages]
   const int32_t* counts;
   int max_pages;
-  int tile;                    // keys a tile: warps a CTA * kKvChunk
+  int tile;                    // keys a tile: warps a CTA * keys of a warp's chunk
   int min_share;               // the least share of the line worth a CTA
   int* status;
   // scan entries: rows, or (row, key head) pairs when each has its own page list
@@ -120,7 +120,7 @@ struct Run {
   long long left, begin, total;
 };
 struct RunScratch {  // shared memory of kv_run
-  long long cost[4], tiles[4];  // by warp
+  long long cost[8], tiles[8];  // by warp
   Run run;
   long long before[2];  // tiles before the run, and before its end
 };
@@ -298,24 +298,27 @@ __device__ __forceinline__ void kv_cluster_join(const AttendArgs& a, const Run& 
 // What the arithmetic of a tile needs to know, left by the warp when it
 // issues the tile's copies.
 struct __align__(16) StageInfo {
-  uint32_t keys;  // the chunk's keys that exist, in the lower half; any of the upper: a bad page
+  uint32_t keys;  // the chunk's keys that exist
+  int bad;        // whether one has a bad page
   int t, tiles;   // the tile, and its unit's tiles
   int row, head, g0;
-  int pad[2];
+  int pad;
 };
 
-// A warp's walk over its run, a chunk of 16 keys each tile, ahead of the
-// arithmetic. WHOLE: page_size is a multiple of 16, so a chunk lies in one
-// page: 32 lanes hold the pages of the next 32 tiles. Otherwise lanes 0 .. 15
-// hold the pages of the next chunk's keys, loaded a tile ahead of their use.
-template <bool WHOLE>
+// A warp's walk over its run, a chunk of KEYS keys each tile, ahead of the
+// arithmetic. WHOLE: page_size is a multiple of 8, so each 8 keys lie in one
+// page: the lanes hold the pages of the next tiles' eights. Otherwise lane i
+// holds the page of the next chunk's key i, loaded a tile ahead of its use.
+template <bool WHOLE, int KEYS>
 struct Walk {
+  static constexpr int kSegs = KEYS / kKvSegment, kWindow = 32 / kSegs;  // eights of a chunk, tiles that are held
   int x, u, t, tiles, head, lane, warp;
   Entry e;
   long long ahead;  // tiles not yet taken
-  int win;          // WHOLE: the tile lane 0 holds
+  int win;          // WHOLE: the first tile that is held
   int page;         // -1: no key, -2: a bad page
-  int more;         // WHOLE: keys of the chunk (0 .. 16); else the slot of the key in its page
+  int slot;         // of the (first) key in its page
+  int live;         // WHOLE: keys of the eight
 
   __device__ __forceinline__ Walk(const AttendArgs& a, const Run& r)
       : x(r.x), u(r.u), t(r.t), tiles(r.tiles), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), e(r.e), ahead(r.left) {
@@ -323,16 +326,16 @@ struct Walk {
     look(a);
   }
 
-  // loads the pages of the tiles (of the chunk's keys) from t on
+  // loads the pages of the tiles' eights (of the chunk's keys) from tile t on
   __device__ __forceinline__ void look(const AttendArgs& a) {
     win = t;
     page = -1;
-    const int j = WHOLE ? (t + lane) * a.tile + warp * kKvChunk : t * a.tile + warp * kKvChunk + lane;
-    more = 0;
-    if (j >= e.n || j < 0 || (!WHOLE && lane >= kKvChunk)) return;
+    slot = live = 0;
+    const int j = warp * KEYS + (WHOLE ? (t + lane / kSegs) * a.tile + lane % kSegs * kKvSegment : t * a.tile + lane);
+    if (j >= e.n || j < 0 || (!WHOLE && lane >= KEYS)) return;
     int o = a.kv.ordinal(j);
-    const int slot = j - o * a.kv.page_size;
-    int live = e.n - j;  // keys from j on
+    slot = j - o * a.kv.page_size;
+    live = min(e.n - j, kKvSegment);
     if (a.pages) {
       o = a.pages[(long long)x * a.max_pages + o];
       if (o < 0 || o >= a.kv.width) {
@@ -341,30 +344,44 @@ struct Walk {
       }
       const long long left = e.len - ((long long)o * a.kv.page_size + slot);
       live = left < live ? (int)left : live;
-      if (live <= 0) return;
+      if (live <= 0) {
+        live = 0;
+        return;
+      }
     }
-    more = WHOLE ? min(live, kKvChunk) : slot;
     page = a.kv.pages_of(e.seq)[o];
     if (page < 0 || page >= a.kv.num_pages) page = -2;
   }
 
-  // The tile's chunk: which keys exist, and their first slot's offset in the
-  // pools (WHOLE), or each lane's (-1: none).
-  __device__ __forceinline__ uint32_t chunk(const AttendArgs& a, long long* off) const {
-    if (WHOLE) {
-      const int pg = __shfl_sync(0xffffffffu, page, t - win), n = __shfl_sync(0xffffffffu, more, t - win);
-      if (pg < 0) return pg == -2 ? 0x10000u : 0u;
-      const int j = t * a.tile + warp * kKvChunk;
-      const int slot = a.kv.slot(j);
-      *off = pg * a.kv.page_stride + head * a.kv.head_stride + slot * a.kv.slot_stride;
-      return (1u << n) - 1;
+  // The tile's chunk: which keys exist, whether one has a bad page, and the
+  // offsets in the pools: of each eight's first key (WHOLE; the same in all
+  // lanes), or of the lane's key in off[0].
+  __device__ __forceinline__ uint32_t chunk(const AttendArgs& a, long long (&off)[kSegs], int* bad) const {
+    const long long base = head * a.kv.head_stride;
+    if (!WHOLE) {
+      off[0] = page >= 0 ? page * a.kv.page_stride + base + slot * a.kv.slot_stride : 0;
+      *bad = __any_sync(0xffffffffu, page == -2);
+      return __ballot_sync(0xffffffffu, page >= 0);
     }
-    *off = page >= 0 ? page * a.kv.page_stride + head * a.kv.head_stride + more * a.kv.slot_stride : -1;
-    return __ballot_sync(0xffffffffu, page >= 0) | (__ballot_sync(0xffffffffu, page == -2) << 16);
+    uint32_t keys = 0;
+    *bad = 0;
+#pragma unroll
+    for (int i = 0; i < kSegs; ++i) {
+      const int from = (t - win) * kSegs + i;
+      const int pg = __shfl_sync(0xffffffffu, page, from), n = __shfl_sync(0xffffffffu, live, from);
+      const int first = __shfl_sync(0xffffffffu, slot, from);
+      off[i] = 0;
+      if (pg >= 0) {
+        off[i] = pg * a.kv.page_stride + base + first * a.kv.slot_stride;
+        keys |= ((1u << n) - 1) << (i * kKvSegment);
+      }
+      *bad |= pg == -2;
+    }
+    return keys;
   }
 
-  __device__ __forceinline__ StageInfo info(const AttendArgs& a, uint32_t keys, int block_heads) const {
-    return StageInfo{keys, t, tiles, a.pages ? x / a.kv.kv_heads : x, head, u % a.blocks * block_heads, {0, 0}};
+  __device__ __forceinline__ StageInfo info(const AttendArgs& a, uint32_t keys, int bad, int block_heads) const {
+    return StageInfo{keys, bad, t, tiles, a.pages ? x / a.kv.kv_heads : x, head, u % a.blocks * block_heads, 0};
   }
 
   // to the next tile, if there is one
@@ -382,7 +399,7 @@ struct Walk {
       head = a.pages ? x % a.kv.kv_heads : u / a.blocks;
     }
     // another unit of the entry goes over the same pages again
-    if (!WHOLE || t < win || t - win >= 32) look(a);
+    if (!WHOLE || t < win || t - win >= kWindow) look(a);
   }
 };
 
@@ -404,13 +421,15 @@ template <>
 __device__ __forceinline__ __nv_bfloat16 kv_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 
-// What a launch of an attention kernel takes: queries of a group together,
-// warps and shared memory of a CTA, CTAs an SM.
+// What a launch of the attention kernel takes: queries of a group together,
+// keys a tile, shared memory of a CTA, CTAs an SM.
 struct KernelShape {
-  int heads, warps, smem, per_sm;
+  int heads, tile, smem, per_sm;
 };
-// the tensor-core kernel for bf16 caches (er_kv_attend_mma.cu)
-KernelShape mma_shape(int d, int group, int q_dtype);
-int attend_mma(const AttendArgs& a, int q_dtype, cudaStream_t st);
+// er_kv_attend_bf16.cu and er_kv_attend_f32.cu: for caches of either type
+KernelShape attend_shape_bf16(int d, int group, int q_dtype);
+KernelShape attend_shape_f32(int d, int group, int q_dtype);
+int attend_bf16(const AttendArgs& a, int q_dtype, cudaStream_t st);
+int attend_f32(const AttendArgs& a, int q_dtype, cudaStream_t st);
 
 }  // namespace er
