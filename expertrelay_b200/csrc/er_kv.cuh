@@ -264,13 +264,26 @@ __device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo
     const int few = red[warps + 2];
     if (pass == 2 || few > kSelectFew) continue;
     uint32_t* list = reinterpret_cast<uint32_t*>(hist);
-#pragma unroll 2
-    for (int i = lo / 4 * 4 + (int)threadIdx.x * 4; i < hi; i += blockDim.x * 4) {
-      const uint4 k4 = keys.four(i, n);
+    for (int i0 = lo / 4 * 4; i0 < hi; i0 += blockDim.x * 4) {  // a warp's keys get their places together
+      const int i = i0 + (int)threadIdx.x * 4;
+      const uint4 k4 = i < hi ? keys.four(i, n) : make_uint4(0, 0, 0, 0);
       const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+      int in = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in |= ((k[e] & mask) == prefix && i + e >= lo && i + e < hi) << e;
+      if (!__any_sync(0xffffffffu, in)) continue;
+      int at = __popc(in);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, at, o);
+        if ((int)(threadIdx.x & 31) >= o) at += up;
+      }
+      int first = 0;
+      if ((threadIdx.x & 31) == 31) first = atomicAdd(&red[warps + 3], at);
+      at += __shfl_sync(0xffffffffu, first, 31) - __popc(in);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if ((k[e] & mask) == prefix && i + e >= lo && i + e < hi) list[atomicAdd(&red[warps + 3], 1)] = k[e];
+        if ((in >> e) & 1) list[at++] = k[e];
     }
     __syncthreads();
     for (int i = few + threadIdx.x; i < (few + 3) / 4 * 4; i += blockDim.x) list[i] = 0;  // below all that counts

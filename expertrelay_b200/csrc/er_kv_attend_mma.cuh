@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
         for (int i = 0; i < KB * CH * NT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s2[i / (CH * NT)][i / NT % CH][i % NT][e] = 0.f;
-#pragma unroll(DP <= 128 ? KS : 8)
+#pragma unroll(KS <= 16 ? KS : 8)
         for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
