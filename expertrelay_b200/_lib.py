@@ -197,9 +197,8 @@ SIGNATURES: dict[str, tuple] = {
     "er_kv_attend_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvAttendIO)]),
     "er_kv_attend": (_i, [C.POINTER(KvCache), C.POINTER(KvAttendIO), _vp, C.c_size_t, _vp]),
     "er_kv_page_bounds": (_i, [C.POINTER(KvCache), _vp, _vp, _vp, _vp, _vp, _vp]),
-    "er_kv_select_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), _i, _i]),
     "er_kv_select": (_i, [C.POINTER(KvCache), _vp, _i, C.c_longlong, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp,
-                          _vp, _vp, C.c_size_t, _vp]),
+                          _vp, _vp]),
     "er_kv_evict": (_i, [C.POINTER(KvCache), C.POINTER(KvCache), _vp, _vp, C.c_longlong, C.c_longlong, _i, _vp,
                          C.c_longlong, C.c_longlong, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "er_trace_record_bytes": (C.c_size_t, [_i, _i]),

@@ -123,6 +123,12 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
   return r;
 }
 
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 // Launch with programmatic stream serialization, in clusters of kClusterCtas when `cluster`.
 template <typename... KArgs, typename... Args>
 inline int kv_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, bool cluster, cudaStream_t st,
@@ -169,145 +175,202 @@ __device__ __forceinline__ int block_scan(int v, int* red, int* total) {
   return __shfl_sync(0xffffffffu, before - mine, warp) + inc - v;
 }
 
-// Positions ranked by a score, four at a time: their rank keys in shared
-// memory where they fit, else made from the scores each time. In shared
-// memory four places behind every 32 stay empty, so that threads which read
-// runs of 32 do so from different banks.
+// Positions ranked by a score: rank keys in shared memory, four at a time.
+// Four places behind every 32 stay empty, so that threads which read runs of
+// 32 do so from different banks.
 struct HeldKeys {
   const uint32_t* held;
-  __device__ __forceinline__ static int at(int i) { return i + ((i >> 5) << 2); }
+  __host__ __device__ static constexpr int at(int i) { return i + ((i >> 5) << 2); }
   // keys i .. i + 3, i a multiple of 4 (those behind the last are anything)
-  __device__ __forceinline__ uint4 four(int i, int) const { return *reinterpret_cast<const uint4*>(held + at(i)); }
+  __device__ __forceinline__ uint4 four(int i) const { return *reinterpret_cast<const uint4*>(held + at(i)); }
 };
 inline size_t held_bytes(long long n) { return (size_t)(n + n / 32 * 4 + 40) * 4; }
-struct ScoreKeys {
-  const float* scores;
-  __device__ __forceinline__ uint4 four(int i, int n) const {
-    uint4 k = make_uint4(0, 0, 0, 0);
-    k.x = rank_key(scores[i]);
-    if (i + 1 < n) k.y = rank_key(scores[i + 1]);
-    if (i + 2 < n) k.z = rank_key(scores[i + 2]);
-    if (i + 3 < n) k.w = rank_key(scores[i + 3]);
-    return k;
-  }
-};
 
 // Bins of one pass of the select: 11, 11, then 10 bits. Shared-memory atomics
 // on one address run one by one, and scores crowd into few bins: those of
-// exactly zero (sums that nothing was added to yet) are counted a warp at a
+// exactly zero (sums that nothing was added to yet) are counted a thread at a
 // time, and many keys go to four copies of the histogram, by lane.
-// Once a bin of few keys is found they are listed and ranked against one another instead.
-constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096, kSelectFew = 512;
-inline __host__ __device__ size_t select_bytes(long long most) {  // of the histograms, for at most `most` keys
+constexpr int kSelectBins = 2048, kSelectCopies = 4, kSelectMany = 4096;
+inline __host__ __device__ size_t select_bytes(long long most) {  // of the histograms, for at most `most` keys a CTA
   return (size_t)kSelectBins * (most >= kSelectMany ? kSelectCopies : 1) * 4;
 }
 
-// The `want`-th largest of the keys [lo, hi) of n, by the whole block.
-// Returns the threshold; *equal is how many of the keys equal to it belong to
-// the `want` largest (the lowest i first). 1 <= want <= hi - lo. `hist`:
-// select_bytes(), `red`: one int per warp and four more, shared.
-template <typename Keys>
-__device__ __forceinline__ uint32_t block_select(const Keys& keys, int n, int lo, int hi, int want, int* hist,
-                                                 int* red, int* equal) {
-  const int copies = hi - lo >= kSelectMany ? kSelectCopies : 1, warps = blockDim.x >> 5;
+// What the CTAs that choose together (a cluster of C, or one alone) share.
+struct SelectScratch {
+  int red[34];    // block_scan; the bin and the rank in it that a pass finds
+  int counts[2];  // this CTA's keys above the threshold, and equal to it
+};
+
+// Chooses `take` of n ranked positions, n > take: the first `sinks` and the
+// last `recent`, then those of the greatest keys, equal ones from the lowest
+// position on; emit(slot, i) for each chosen position i, slots in position
+// order. By the C CTAs of a cluster together (rank r holds the keys of the nl
+// positions from b0 on, in rank order) or by one (C = 1). A radix select from
+// the top bits down finds the least key that is taken: every CTA counts its
+// own keys, then sums all CTAs' histograms; last, the CTAs' counts place each
+// one's positions. sinks + recent <= take. `hist`: select_bytes(), shared.
+template <int C, typename Emit>
+__device__ __forceinline__ void take_best(const HeldKeys& keys, int b0, int nl, int n, int take, int sinks, int recent,
+                                          int* hist, SelectScratch& sc, Emit emit) {
+  const int lo = sinks, hi = n - recent;
+  int want = take - sinks - recent;
+  const int copies = nl >= kSelectMany ? kSelectCopies : 1;
+  const int rank = C > 1 ? cluster_rank() : 0;
+  auto meet = [&]() {
+    if (C > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+  };
+  const uint32_t hist0 = smem_addr(hist);
   int* mine = hist + (copies > 1 ? (threadIdx.x & (kSelectCopies - 1)) * kSelectBins : 0);
   uint32_t prefix = 0, mask = 0;
+  if (want > 0) {
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int b = threadIdx.x; b < copies * kSelectBins; b += blockDim.x) hist[b] = 0;
-    __syncthreads();
-    int zeros = 0;  // of this thread
-    auto count = [&](uint32_t k, int i) {
-      if ((k & mask) != prefix || i < lo || i >= hi) return;
-      if (k == kZeroKey)
-        ++zeros;
-      else
-        atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
-    };
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+      for (int b = threadIdx.x * 4; b < copies * kSelectBins; b += blockDim.x * 4)
+        *reinterpret_cast<int4*>(hist + b) = make_int4(0, 0, 0, 0);
+      __syncthreads();
+      int zeros = 0;  // of this thread
+      auto count = [&](uint32_t k, int i) {
+        if ((k & mask) != prefix || i < lo || i >= hi) return;
+        if (k == kZeroKey)
+          ++zeros;
+        else
+          atomicAdd(&mine[(k >> shift) & (bins - 1)], 1);
+      };
 #pragma unroll 2
-    for (int i = lo / 4 * 4 + (int)threadIdx.x * 4; i < hi; i += blockDim.x * 4) {
-      const uint4 k = keys.four(i, n);
-      count(k.x, i);
-      count(k.y, i + 1);
-      count(k.z, i + 2);
-      count(k.w, i + 3);
-    }
-    zeros = __reduce_add_sync(0xffffffffu, zeros);
-    if (zeros && (threadIdx.x & 31) == 0) atomicAdd(&mine[(kZeroKey >> shift) & (bins - 1)], zeros);
-    __syncthreads();
-    // thread t: `per` bins from the top
-    const int per = (bins + blockDim.x - 1) / blockDim.x, top = bins - 1 - (int)threadIdx.x * per;
-    int sum = 0;
-    for (int j = 0; j < per; ++j)
-      if (top - j >= 0)
-        for (int c = 0; c < copies; ++c) sum += hist[c * kSelectBins + top - j];
-    int total;
-    int above = block_scan(sum, red, &total);
-    if (above < want && want <= above + sum) {
-      for (int j = 0; j < per; ++j) {
-        int n = 0;
-        for (int c = 0; c < copies; ++c) n += hist[c * kSelectBins + top - j];
-        if (above < want && want <= above + n) {
-          red[warps] = top - j;
-          red[warps + 1] = want - above;
-          red[warps + 2] = n;
-          red[warps + 3] = 0;
+      for (int i = threadIdx.x * 4; i < nl; i += blockDim.x * 4) {
+        const uint4 k = keys.four(i);
+        count(k.x, b0 + i);
+        if (i + 1 < nl) count(k.y, b0 + i + 1);
+        if (i + 2 < nl) count(k.z, b0 + i + 2);
+        if (i + 3 < nl) count(k.w, b0 + i + 3);
+      }
+      zeros = __reduce_add_sync(0xffffffffu, zeros);
+      if (zeros && (threadIdx.x & 31) == 0) atomicAdd(&mine[(kZeroKey >> shift) & (bins - 1)], zeros);
+      if (copies > 1) {
+        __syncthreads();
+        for (int b = threadIdx.x; b < bins; b += blockDim.x) {
+          int c = hist[b];
+          for (int j = 1; j < kSelectCopies; ++j) c += hist[j * kSelectBins + b];
+          hist[b] = c;
         }
-        above += n;
       }
-    }
-    __syncthreads();
-    prefix |= (uint32_t)red[warps] << shift;
-    mask |= (uint32_t)(bins - 1) << shift;
-    want = red[warps + 1];
-    const int few = red[warps + 2];
-    if (pass == 2 || few > kSelectFew) continue;
-    uint32_t* list = reinterpret_cast<uint32_t*>(hist);
-    for (int i0 = lo / 4 * 4; i0 < hi; i0 += blockDim.x * 4) {  // a warp's keys get their places together
-      const int i = i0 + (int)threadIdx.x * 4;
-      const uint4 k4 = i < hi ? keys.four(i, n) : make_uint4(0, 0, 0, 0);
-      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-      int in = 0;
+      meet();
+      // four bins a thread, from the top (a block has at least 256 threads, so two rounds at the most)
+      int above = 0;
+#pragma unroll 1
+      for (int top = bins - 4 - (int)threadIdx.x * 4, round = 0; round * (int)blockDim.x * 4 < bins;
+           ++round, top -= blockDim.x * 4) {
+        int4 c = make_int4(0, 0, 0, 0);
+        if (top >= 0) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) in |= ((k[e] & mask) == prefix && i + e >= lo && i + e < hi) << e;
-      if (!__any_sync(0xffffffffu, in)) continue;
-      int at = __popc(in);
+          for (int r = 0; r < C; ++r) {
+            int4 x;
+            if (C > 1)
+              asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
+                           : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                           : "r"(cluster_addr(hist0, r) + top * 4)
+                           : "memory");
+            else
+              x = *reinterpret_cast<const int4*>(hist + top);
+            c.x += x.x;
+            c.y += x.y;
+            c.z += x.z;
+            c.w += x.w;
+          }
+        }
+        const int sum = c.x + c.y + c.z + c.w;
+        int total;
+        int at = above + block_scan(sum, sc.red, &total);
+        above += total;
+        if (at < want && want <= at + sum) {
+          const int n4[4] = {c.w, c.z, c.y, c.x};
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, at, o);
-        if ((int)(threadIdx.x & 31) >= o) at += up;
+          for (int j = 0; j < 4; ++j) {
+            if (at < want && want <= at + n4[j]) {
+              sc.red[32] = top + 3 - j;
+              sc.red[33] = want - at;
+            }
+            at += n4[j];
+          }
+        }
       }
-      int first = 0;
-      if ((threadIdx.x & 31) == 31) first = atomicAdd(&red[warps + 3], at);
-      at += __shfl_sync(0xffffffffu, first, 31) - __popc(in);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if ((in >> e) & 1) list[at++] = k[e];
+      meet();  // the bin is found, and the histograms may be written again
+      prefix |= (uint32_t)sc.red[32] << shift;
+      mask |= (uint32_t)(bins - 1) << shift;
+      want = sc.red[33];
     }
-    __syncthreads();
-    for (int i = few + threadIdx.x; i < (few + 3) / 4 * 4; i += blockDim.x) list[i] = 0;  // below all that counts
-    __syncthreads();
-    for (int i = threadIdx.x; i < few; i += blockDim.x) {
-      const uint32_t k = list[i];
-      int more = 0, same = 0;
-#pragma unroll 4
-      for (int j = 0; j < few; j += 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(list + j);
-        more += (x.x > k) + (x.y > k) + (x.z > k) + (x.w > k);
-        same += (x.x == k) + (x.y == k) + (x.z == k) + (x.w == k);
-      }
-      if (more < want && want <= more + same) {  // the threshold; its equals write the same
-        red[warps] = (int)k;
-        red[warps + 1] = want - more;
-      }
-    }
-    __syncthreads();
-    *equal = red[warps + 1];
-    return (uint32_t)red[warps];
+  } else {
+    want = 0;
   }
-  *equal = want;
-  return prefix;
+  const uint32_t least = prefix;  // `want` of the keys equal to it are taken; without any, none is above or equal
+  const bool none = mask == 0;
+  // a run of 4, 8, .. 32 positions a thread, in rounds; first how many there are, then where they go
+  int run = 4;
+  while (run < 32 && run * (int)blockDim.x < nl) run *= 2;
+  auto look = [&](int b, uint32_t* sure, uint32_t* tied) {
+    *sure = *tied = 0;
+    for (int j = 0; j < run && b + j < nl; j += 4) {
+      const uint4 k4 = keys.four(b + j);
+      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = b0 + b + j + e;
+        const bool forced = i < lo || i >= hi, there = b + j + e < nl;
+        *sure |= (uint32_t)(there && (forced || (!none && k[e] > least))) << (j + e);
+        *tied |= (uint32_t)(there && !forced && !none && k[e] == least) << (j + e);
+      }
+    }
+  };
+  int above = 0, same = 0;  // taken outright, and equal to the threshold, before this CTA's positions
+  if (C > 1) {
+    int s = 0, q = 0;
+    for (int r0 = 0; r0 < nl; r0 += run * blockDim.x) {
+      uint32_t sure, tied;
+      look(r0 + (int)threadIdx.x * run, &sure, &tied);
+      s += __popc(sure);
+      q += __popc(tied);
+    }
+    int all_s, all_q;
+    block_scan(s, sc.red, &all_s);
+    block_scan(q, sc.red, &all_q);
+    if (threadIdx.x == 0) {
+      sc.counts[0] = all_s;
+      sc.counts[1] = all_q;
+    }
+    cluster_sync();
+    const uint32_t at = smem_addr(sc.counts);
+    for (int r = 0; r < rank; ++r) {
+      const float2 c = cluster_load2(cluster_addr(at, r));
+      above += __float_as_int(c.x);
+      same += __float_as_int(c.y);
+    }
+  }
+  for (int r0 = 0; r0 < nl; r0 += run * blockDim.x) {
+    const int b = r0 + (int)threadIdx.x * run;
+    uint32_t sure, tied;
+    look(b, &sure, &tied);
+    // 16 bits each: a round has at most 32 * 1024 positions
+    int all;
+    const int before = block_scan(__popc(sure) | __popc(tied) << 16, sc.red, &all);
+    int at = above + (before & 0xffff), tie = same + (before >> 16);
+    for (uint32_t left = sure | tied; left; left &= left - 1) {
+      const int j = __ffs(left) - 1;
+      if ((sure >> j) & 1) {
+        emit(at + min(tie, want), b0 + b + j);
+        ++at;
+      } else {
+        if (tie < want) emit(at + tie, b0 + b + j);
+        ++tie;
+      }
+    }
+    above += all & 0xffff;
+    same += all >> 16;
+  }
+  meet();  // no CTA leaves while its counts may be read
 }
 
 }  // namespace er

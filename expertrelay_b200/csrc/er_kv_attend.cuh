@@ -208,11 +208,6 @@ __device__ __forceinline__ float piece_weight(float mi, float m) { return mi == 
 // With few units, each is a cluster's: its CTAs take an eighth of the tiles
 // each and join their pieces through one another's shared memory, so there is
 // no line to divide, no workspace and no second launch.
-__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"

@@ -1,10 +1,8 @@
 // er_kv_select.cu -- the pages worth reading for each query, and the
 // positions worth keeping in a cache that grows too long.
 //
-// Both rank by a score and take the best: a radix select by the whole CTA
-// (er_kv.cuh) finds the score of the last one taken, a second pass in
-// position order writes the taken ones ascending, equal scores to the lower
-// position.
+// Both rank by a score and take the best (take_best in er_kv.cuh): equal
+// scores to the lower position, the taken ones in position order.
 #include "er_kv.cuh"
 
 namespace er {
@@ -154,26 +152,6 @@ __device__ __forceinline__ int row_pages(const KvView& kv, const int32_t* seqs, 
   return *bad ? 0 : (int)(((long long)len + kv.page_size - 1) / kv.page_size);
 }
 
-// Scores alone, for tables too wide for shared memory.
-template <typename TQ>
-__global__ void __launch_bounds__(kScoreThreads)
-    kv_score_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
-                    const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
-                    const float* __restrict__ scales, float* __restrict__ scores, int* status) {
-  extern __shared__ __align__(16) int8_t qc[];
-  float* qt = reinterpret_cast<float*>(qc + (group + 7) / 8 * 16 * codes_pitch(kv.d));
-  kv_enter();
-  const int row = blockIdx.y / kv.kv_heads, h = blockIdx.y % kv.kv_heads;
-  int seq, bad;
-  const int np = row_pages(kv, seqs, lens, row, &seq, &bad);  // what is wrong is reported by the choice
-  if (np == 0) return;
-  const bool none = code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
-  float* out = scores + (long long)blockIdx.y * kv.width;
-  const int each = (np + gridDim.x - 1) / gridDim.x, first = min(np, (int)blockIdx.x * each);
-  score_pages(kv, seq, h, first, min(np, first + each), group, qc, qt, none, codes, scales, status,
-              [&](int o, float v) { out[o] = v; });
-}
-
 // The rank keys of n scores into shared memory, four scores a load from the first 16-byte boundary on.
 __device__ __forceinline__ void hold_keys(const float* scores, int n, uint32_t* held) {
   const int skip = min(n, (int)((16 - ((uintptr_t)scores & 15)) & 15) / 4), quads = (n - skip) / 4;
@@ -197,90 +175,38 @@ __device__ __forceinline__ void hold_keys(const float* scores, int n, uint32_t* 
   __syncthreads();
 }
 
-// Writes, ascending, the `take` of n positions that are forced (the first
-// `sinks`, the last `recent`) or rank best; emit(slot, i) for each.
-template <typename Keys, typename Emit>
-__device__ __forceinline__ void take_best(const Keys& keys, int n, int take, int sinks, int recent, int* hist, int* red,
-                                          Emit emit) {
-  if (n <= take) {
-    for (int i = threadIdx.x; i < n; i += blockDim.x) emit(i, i);
-    return;
-  }
-  const int lo = sinks, hi = n - recent, want = take - sinks - recent;
-  uint32_t least = 0xffffffffu;
-  int equal = 0;
-  if (want > 0) least = block_select(keys, n, lo, hi, want, hist, red, &equal);
-  // in rounds of a run of 4, 8, .. 32 positions a thread
-  int run = 4;
-  while (run < 32 && run * (int)blockDim.x < n) run *= 2;
-  int above = 0, same = 0;  // taken outright, and equal to the threshold, so far
-  for (int i0 = 0; i0 < n; i0 += run * blockDim.x) {
-    const int b = i0 + (int)threadIdx.x * run;
-    uint32_t sure = 0, tied = 0;  // of the run's positions
-    for (int j = 0; j < run && b + j < n; j += 4) {
-      const uint4 k4 = keys.four(b + j, n);
-      const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = b + j + e;
-        const bool forced = i < lo || i >= hi;
-        if (i < n) {
-          sure |= (uint32_t)(forced || (want > 0 && k[e] > least)) << (j + e);
-          tied |= (uint32_t)(!forced && want > 0 && k[e] == least) << (j + e);
-        }
-      }
-    }
-    // 16 bits each: a round has at most 32 * 1024 positions
-    int all;
-    const int before = block_scan(__popc(sure) | __popc(tied) << 16, red, &all);
-    int at = above + (before & 0xffff), tie = same + (before >> 16);
-    for (uint32_t left = sure | tied; left; left &= left - 1) {
-      const int j = __ffs(left) - 1;
-      if ((sure >> j) & 1) {
-        emit(at + min(tie, equal), b + j);
-        ++at;
-      } else {
-        if (tie < equal) emit(at + tie, b + j);
-        ++tie;
-      }
-    }
-    above += all & 0xffff;
-    same += all >> 16;
-  }
+constexpr size_t kSelectSmem = 220 * 1024;  // of a CTA that chooses: histograms, codes, keys
+
+// Positions that rank r of a cluster holds: `each` of them, a multiple of 4.
+__host__ __device__ inline int cluster_each(int n) { return (n + 4 * kClusterCtas - 1) / (4 * kClusterCtas) * 4; }
+
+// How a (sequence, key head)'s positions are chosen from: by a CTA alone; or
+// by a cluster, whose first CTA chooses, or whose CTAs choose together.
+enum ChooseMode { kAlone, kFirst, kTogether };
+// Few units run as clusters, all at once, and those choose together where
+// there is much to choose from (8 units of 38855 positions: 81 us by a CTA
+// each, 43 together; but 16 of 2501 20 against 28, for every pass of the
+// choice then reads the histograms of 8 CTAs). Otherwise a CTA a unit, unless
+// its shared memory cannot hold the keys beside `beside` bytes.
+inline int choose_mode(long long units, int n, size_t beside) {
+  if (select_bytes(n) + held_bytes(n) + beside > kSelectSmem) return kTogether;
+  return units * kClusterCtas > 148 * 2 ? kAlone : n > 8192 ? kTogether : kFirst;
 }
+inline int choose_held(int mode, int n) { return mode == kTogether ? cluster_each(n) : n; }  // keys a CTA holds
 
-constexpr int kTakeThreads = 1024;
-
-// Shared memory of a CTA that takes the best of at most n: the histograms,
-// and the keys where they fit beside them (*held).
-inline size_t take_smem(long long n, bool* held) {
-  *held = select_bytes(n) + held_bytes(n) <= 200 * 1024;
-  return select_bytes(n) + (*held ? held_bytes(n) : 0);
-}
-inline int take_threads(long long n) { return n <= 1024 ? 256 : n <= 8192 ? 512 : kTakeThreads; }
-
-template <int THREADS, typename Keys>
-__device__ __forceinline__ void write_choice(const Keys& keys, int n, int budget, int sinks, int recent, int* hist,
-                                             int* red, int32_t* out, int32_t* count) {
-  take_best(keys, n, budget, sinks, recent, hist, red, [&](int slot, int i) { out[slot] = i; });
-  const int take = min(n, budget);
-  for (int i = take + threadIdx.x; i < budget; i += THREADS) out[i] = -1;
-  if (threadIdx.x == 0) *count = take;
-}
-
-// Scores and choice of one (row, key head) in one launch: a CTA, or with few
-// units a cluster whose CTAs score an eighth of the pages each, straight into
-// the shared memory of the first, which chooses.
-template <typename TQ, bool CLUSTER>
+// Scores and choice of one (row, key head); in a cluster each CTA scores an
+// eighth of the pages.
+template <typename TQ, int MODE>
 __global__ void __launch_bounds__(kScoreThreads)
     kv_pick_kernel(KvView kv, const TQ* __restrict__ q, long long q_stride, int group, const int32_t* __restrict__ seqs,
                    const int32_t* __restrict__ lens, const int8_t* __restrict__ codes,
-                   const float* __restrict__ scales, int budget, int sinks, int recent, int32_t* __restrict__ pages,
-                   int32_t* __restrict__ counts, int* status) {
+                   const float* __restrict__ scales, int most, int budget, int sinks, int recent,
+                   int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
+  constexpr bool CLUSTER = MODE != kAlone;
   extern __shared__ __align__(16) char sm[];
-  __shared__ int red[kScoreThreads / 32 + 4];
+  __shared__ SelectScratch sc;
   int* hist = reinterpret_cast<int*>(sm);
-  int8_t* qc = reinterpret_cast<int8_t*>(sm + select_bytes(kv.width));
+  int8_t* qc = reinterpret_cast<int8_t*>(sm + select_bytes(most));
   float* qt = reinterpret_cast<float*>(qc + (group + 7) / 8 * 16 * codes_pitch(kv.d));
   uint32_t* held = reinterpret_cast<uint32_t*>(qc + codes_bytes(group, kv.d));
   kv_enter();
@@ -289,43 +215,33 @@ __global__ void __launch_bounds__(kScoreThreads)
   int seq, bad;
   const int np = row_pages(kv, seqs, lens, row, &seq, &bad);
   if (bad && rank == 0 && threadIdx.x == 0) kv_report(status, bad);
-  if (np > budget) {  // else all are taken, whatever they score
+  int32_t* out = pages + (long long)unit * budget;
+  const int take = min(np, budget);
+  if (np > budget) {
     const bool none =
         code_queries(q + (long long)row * q_stride + (long long)h * group * kv.d, group, kv.d, qc, qt);
-    if (CLUSTER) cluster_sync();  // the first CTA runs: its shared memory can be written
-    const int first = CLUSTER ? (int)((long long)np * rank / kClusterCtas) : 0;
-    const int last = CLUSTER ? (int)((long long)np * (rank + 1) / kClusterCtas) : np;
-    const uint32_t to = CLUSTER ? cluster_addr(smem_addr(held), 0) : smem_addr(held);
+    if (MODE == kFirst) cluster_sync();  // the first CTA runs: its shared memory can be written
+    const int each = CLUSTER ? cluster_each(np) : np;
+    const int first = min(np, rank * each), last = min(np, first + each);
+    const uint32_t to = MODE == kFirst ? cluster_addr(smem_addr(held), 0) : 0;
     score_pages(kv, seq, h, first, last, group, qc, qt, none, codes, scales, status, [&](int o, float v) {
-      const uint32_t at = to + HeldKeys::at(o) * 4, k = rank_key(v);
-      if (CLUSTER)
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
+      if (MODE == kFirst)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + HeldKeys::at(o) * 4), "r"(rank_key(v)) : "memory");
       else
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(k) : "memory");
+        held[HeldKeys::at(o - first)] = rank_key(v);
     });
-    if (CLUSTER)
+    if (MODE == kFirst)
       cluster_sync();
     else
       __syncthreads();
+    const int b0 = MODE == kTogether ? first : 0, nl = MODE == kTogether ? last - first : np;
+    if (MODE == kTogether || rank == 0)
+      take_best<MODE == kTogether ? kClusterCtas : 1>(HeldKeys{held}, b0, nl, np, budget, sinks, recent, hist, sc,
+                                                      [&](int slot, int i) { out[slot] = i; });
+  } else if (rank == 0) {  // all are taken, whatever they score
+    for (int i = threadIdx.x; i < budget; i += kScoreThreads) out[i] = i < np ? i : -1;
   }
-  if (rank == 0)
-    write_choice<kScoreThreads>(HeldKeys{held}, np, budget, sinks, recent, hist, red,
-                                pages + (long long)unit * budget, counts + unit);
-}
-
-// The choice alone, from scores in memory.
-__global__ void __launch_bounds__(kTakeThreads)
-    kv_choose_kernel(KvView kv, const int32_t* __restrict__ seqs, const int32_t* __restrict__ lens,
-                     const float* __restrict__ scores, int budget, int sinks, int recent,
-                     int32_t* __restrict__ pages, int32_t* __restrict__ counts, int* status) {
-  extern __shared__ int hist[];
-  __shared__ int red[kTakeThreads / 32 + 4];
-  kv_enter();
-  int seq, bad;
-  const int n = row_pages(kv, seqs, lens, blockIdx.x / kv.kv_heads, &seq, &bad);
-  if (bad && threadIdx.x == 0) kv_report(status, bad);
-  write_choice<kTakeThreads>(ScoreKeys{scores + (long long)blockIdx.x * kv.width}, n, budget, sinks, recent, hist, red,
-                             pages + (long long)blockIdx.x * budget, counts + blockIdx.x);
+  if (rank == 0 && threadIdx.x == 0) counts[unit] = take;
 }
 
 struct MassView {
@@ -385,15 +301,17 @@ __device__ __forceinline__ void move_rows(const KvView& from, const KvView& to, 
   }
 }
 
-// The kept positions of a (sequence, key head) and their weights, by a CTA.
-// CLUSTER (few units): by the first CTA of a cluster, whose CTAs then move the
-// rows together; otherwise kv_move_kernel moves them.
-template <bool CLUSTER>
-__global__ void __launch_bounds__(kTakeThreads)
-    kv_keep_kernel(KvView kv, KvView dst, MassView m, const int32_t* __restrict__ lens, int budget, int sinks,
-                   int recent, int held, int row_bytes, int32_t* kept, int32_t* __restrict__ lens_out, int* status) {
-  extern __shared__ int hist[];
-  __shared__ int red[kTakeThreads / 32 + 4];
+// The kept positions of a (sequence, key head) and their weights. A cluster
+// moves the rows, too; for CTAs alone kv_move_kernel does.
+template <int MODE>
+__global__ void __launch_bounds__(1024)
+    kv_keep_kernel(KvView kv, KvView dst, MassView m, const int32_t* __restrict__ lens, int most, int budget, int sinks,
+                   int recent, int row_bytes, int32_t* kept, int32_t* __restrict__ lens_out, int* status) {
+  constexpr bool CLUSTER = MODE != kAlone;
+  extern __shared__ __align__(16) char sm[];
+  __shared__ SelectScratch sc;
+  int* hist = reinterpret_cast<int*>(sm);
+  uint32_t* held = reinterpret_cast<uint32_t*>(sm + select_bytes(most));
   kv_enter();
   const int unit = CLUSTER ? blockIdx.x / kClusterCtas : blockIdx.x, rank = CLUSTER ? cluster_rank() : 0;
   const int seq = unit / kv.kv_heads, h = unit % kv.kv_heads;
@@ -404,28 +322,26 @@ __global__ void __launch_bounds__(kTakeThreads)
   }
   const float* w = m.mass + seq * m.seq_stride + h * m.head_stride;
   int32_t* out = kept + (long long)unit * budget;
-  const int take = min(n, budget);
-  if (rank == 0) {
-    auto emit = [&](int slot, int i) { out[slot] = i; };
-    if (held) {
-      uint32_t* keys = (uint32_t*)(hist + select_bytes(m.len) / 4);
-      if (n > budget) hold_keys(w, n, keys);
-      take_best(HeldKeys{keys}, n, budget, sinks, recent, hist, red, emit);
-    } else {
-      take_best(ScoreKeys{w}, n, budget, sinks, recent, hist, red, emit);
+  const int take = min(n, budget), ctas = CLUSTER ? kClusterCtas : 1;
+  const int t0 = rank * blockDim.x + threadIdx.x, threads = ctas * blockDim.x;
+  if (n > budget) {
+    if (MODE == kTogether || rank == 0) {
+      const int each = MODE == kTogether ? cluster_each(n) : n, first = min(n, rank * each), last = min(n, first + each);
+      hold_keys(w + first, last - first, held);
+      take_best<MODE == kTogether ? kClusterCtas : 1>(HeldKeys{held}, first, last - first, n, budget, sinks, recent, hist,
+                                                      sc, [&](int slot, int i) { out[slot] = i; });
     }
-    for (int i = take + threadIdx.x; i < budget; i += blockDim.x) out[i] = -1;
-    if (threadIdx.x == 0 && h == 0) lens_out[seq] = take;
+  } else {
+    for (int i = t0; i < budget; i += threads) out[i] = i < n ? i : -1;
   }
   if (CLUSTER)
-    cluster_sync();  // the list is written
+    cluster_sync();
   else
-    __syncthreads();
-  if (rank == 0) {
-    float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
+    __syncthreads();  // the list is written
+  if (t0 == 0 && h == 0) lens_out[seq] = take;
+  float* to = m.to_mass + seq * m.to_seq_stride + h * m.to_head_stride;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < take; i += blockDim.x) to[i] = w[out[i]];
-  }
+  for (int i = t0; i < take; i += threads) to[i] = w[out[i]];
   if (CLUSTER)
     move_rows(kv, dst, seq, h, out, take, row_bytes, rank * (blockDim.x >> 5) + (threadIdx.x >> 5),
               kClusterCtas * (blockDim.x >> 5), status);
@@ -446,36 +362,30 @@ using namespace er;
 
 namespace {
 
-// Shared memory of kv_pick_kernel; more than kPickSmem means that the scores go through the workspace.
-constexpr size_t kPickSmem = 200 * 1024;
-size_t pick_smem(int width, int group, int d) { return select_bytes(width) + codes_bytes(group, d) + held_bytes(width); }
+size_t pick_smem(int most, int group, int d) { return select_bytes(most) + codes_bytes(group, d) + held_bytes(most); }
 
 template <typename TQ>
 int pick_go(const KvView& kv, const void* q, long long q_stride, int units, int group, const int32_t* seqs,
             const int32_t* lens, const int8_t* codes, const float* scales, int budget, int sinks, int recent,
             int32_t* pages, int32_t* counts, int* status, cudaStream_t st) {
-  const size_t smem = pick_smem(kv.width, group, kv.d);
-  const bool cluster = units * kClusterCtas <= 148 * 2;  // all at once
-  auto kernel = cluster ? kv_pick_kernel<TQ, true> : kv_pick_kernel<TQ, false>;
-  static std::atomic<unsigned long long> done[2];
-  if (int rc = allow_smem(kernel, kPickSmem, done[cluster])) return rc;
-  return kv_launch(kernel, dim3(cluster ? units * kClusterCtas : units), kScoreThreads, smem, cluster, st,
-                   "kv_pick_kernel", kv, (const TQ*)q, q_stride, group, seqs, lens, codes, scales, budget, sinks,
-                   recent, pages, counts, status);
+  const int mode = choose_mode(units, kv.width, codes_bytes(group, kv.d)), most = choose_held(mode, kv.width);
+  auto kernel = mode == kTogether ? kv_pick_kernel<TQ, kTogether>
+                : mode == kFirst  ? kv_pick_kernel<TQ, kFirst>
+                                  : kv_pick_kernel<TQ, kAlone>;
+  static std::atomic<unsigned long long> done[3];
+  if (int rc = allow_smem(kernel, kSelectSmem, done[mode])) return rc;
+  const bool cluster = mode != kAlone;
+  return kv_launch(kernel, dim3(cluster ? units * kClusterCtas : units), kScoreThreads, pick_smem(most, group, kv.d),
+                   cluster, st, "kv_pick_kernel", kv, (const TQ*)q, q_stride, group, seqs, lens, codes, scales, most,
+                   budget, sinks, recent, pages, counts, status);
 }
 
 }  // namespace
 
-extern "C" size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows, int heads) {
-  if (!cache || rows <= 0 || cache->kv_heads <= 0 || heads <= 0 || cache->table_width <= 0) return 0;
-  if (pick_smem(cache->table_width, heads / cache->kv_heads, cache->head_dim) <= kPickSmem) return 0;
-  return align_up((size_t)rows * cache->kv_heads * cache->table_width * sizeof(float), 256);
-}
-
 extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, long long q_stride, int rows,
                             int heads, const int32_t* seqs, const int32_t* lens, const int8_t* codes,
                             const float* scales, int budget, int sinks, int recent, int32_t* pages_out,
-                            int32_t* counts_out, int* status, void* workspace, size_t workspace_bytes, void* stream) {
+                            int32_t* counts_out, int* status, void* stream) {
   if (int rc = kv_check("er_kv_select", cache)) return rc;
   if (rows < 0 || heads <= 0 || heads % cache->kv_heads)
     return fail(ER_EINVAL, "er_kv_select: rows %d, heads %d / %d", rows, heads, cache->kv_heads);
@@ -489,31 +399,18 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
   if (!q || !lens || !codes || !scales || !pages_out || !counts_out) return fail(ER_EINVAL, "er_kv_select: null pointer");
   if (((uintptr_t)codes & 15)) return fail(ER_EINVAL, "er_kv_select: codes must be 16-byte aligned");
   const int group = heads / cache->kv_heads;
-  const size_t smem = codes_bytes(group, cache->head_dim);
-  if (smem > 40 * 1024) return fail(ER_EINVAL, "er_kv_select: %d queries a key head", group);
-  if ((long long)rows * cache->kv_heads > 65535)
-    return fail(ER_EINVAL, "er_kv_select: %d rows of %d key heads (at most 65535 in all)", rows, cache->kv_heads);
-  const size_t need = er_kv_select_workspace_bytes(cache, rows, heads);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(ER_ENOSPACE, "er_kv_select: workspace %zu bytes, need %zu", workspace_bytes, need);
+  if (group > 64) return fail(ER_EINVAL, "er_kv_select: %d queries a key head (at most 64)", group);
+  if ((long long)rows * cache->kv_heads > 0x7fffffff / kClusterCtas)
+    return fail(ER_EINVAL, "er_kv_select: %d rows of %d key heads", rows, cache->kv_heads);
+  if (pick_smem(cluster_each(cache->table_width), group, cache->head_dim) > kSelectSmem)
+    return fail(ER_EINVAL, "er_kv_select: a table of %d pages (about 300000 fit)", cache->table_width);
   const KvView kv = kv_view(*cache);
-  cudaStream_t st = (cudaStream_t)stream;
   const int units = rows * kv.kv_heads;
-  const bool qb = q_dtype == ER_DTYPE_BF16;
-  if (!need)
-    return qb ? pick_go<__nv_bfloat16>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent,
-                                       pages_out, counts_out, status, st)
-              : pick_go<float>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent,
-                               pages_out, counts_out, status, st);
-  const dim3 grid((unsigned)(148 * 4 / units + 1), units);
-  float* scores = (float*)workspace;
-  int rc = qb ? launch_chained(kv_score_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), smem, st, "kv_score_kernel",
-                               kv, (const __nv_bfloat16*)q, q_stride, group, seqs, lens, codes, scales, scores, status)
-              : launch_chained(kv_score_kernel<float>, grid, dim3(kScoreThreads), smem, st, "kv_score_kernel", kv,
-                               (const float*)q, q_stride, group, seqs, lens, codes, scales, scores, status);
-  if (rc) return rc;
-  return launch_chained(kv_choose_kernel, dim3(units), dim3(kTakeThreads), select_bytes(kv.width), st, "kv_choose_kernel", kv,
-                        seqs, lens, (const float*)scores, budget, sinks, recent, pages_out, counts_out, status);
+  return q_dtype == ER_DTYPE_BF16
+             ? pick_go<__nv_bfloat16>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent,
+                                      pages_out, counts_out, status, (cudaStream_t)stream)
+             : pick_go<float>(kv, q, q_stride, units, group, seqs, lens, codes, scales, budget, sinks, recent, pages_out,
+                              counts_out, status, (cudaStream_t)stream);
 }
 
 extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
@@ -539,25 +436,27 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   const MassView m{mass,        to_mass,  mass_seq_stride, mass_head_stride, to_mass_seq_stride, to_mass_head_stride,
                    mass_len, to_mass_len};
   cudaStream_t st = (cudaStream_t)stream;
-  bool held;
-  const size_t take = take_smem(mass_len, &held);
   const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4), units = a.seqs * a.kv_heads;
-  // clusters all at once, each with little to move beside the choice (the
-  // second launch costs about what 64 MB take to move)
-  const bool cluster = units * kClusterCtas <= 148 * 2 && 2LL * units * budget * row_bytes <= 64ll << 20;
-  static std::atomic<unsigned long long> done[2];
-  if (int rc = cluster ? allow_smem(kv_keep_kernel<true>, 200 * 1024, done[1])
-                       : allow_smem(kv_keep_kernel<false>, 200 * 1024, done[0]))
-    return rc;
-  if (int rc = kv_launch(cluster ? kv_keep_kernel<true> : kv_keep_kernel<false>,
-                         dim3(cluster ? units * kClusterCtas : units), take_threads(mass_len), take, cluster, st,
-                         "kv_keep_kernel", a, b, m, lens, budget, sinks, recent, (int)held, row_bytes, kept_out,
-                         lens_out, status))
+  if (select_bytes(cluster_each(mass_len)) + held_bytes(cluster_each(mass_len)) > kSelectSmem)
+    return fail(ER_EINVAL, "er_kv_evict: %d weights a key head (about 370000 fit)", mass_len);
+  if ((long long)a.seqs * a.kv_heads > 0x7fffffff / kClusterCtas)
+    return fail(ER_EINVAL, "er_kv_evict: %d sequences, %d key heads", a.seqs, a.kv_heads);
+  const int mode = choose_mode(units, mass_len, 0), most = choose_held(mode, mass_len);
+  auto keep = mode == kTogether ? kv_keep_kernel<kTogether>
+              : mode == kFirst ? kv_keep_kernel<kFirst>
+                                   : kv_keep_kernel<kAlone>;
+  static std::atomic<unsigned long long> done[3];
+  if (int rc = allow_smem(keep, kSelectSmem, done[mode])) return rc;
+  const bool cluster = mode != kAlone;
+  if (int rc = kv_launch(keep, dim3(cluster ? units * kClusterCtas : units),
+                         most <= 1024 ? 256 : most <= 8192 ? 512 : 1024, select_bytes(most) + held_bytes(most), cluster,
+                         st, "kv_keep_kernel", a, b, m, lens, most, budget, sinks, recent, row_bytes, kept_out, lens_out,
+                         status))
     return rc;
   if (cluster) return ER_OK;
   const long long want = 148 * 32 / ((long long)a.seqs * a.kv_heads) + 1;
-  const long long most = (budget + 31) / 32;  // rows of a warp's first round, times 8
-  const dim3 grid((unsigned)(most < want ? most : want), a.seqs, a.kv_heads);
+  const long long first_rows = (budget + 31) / 32;  // rows of a warp's first round, times 8
+  const dim3 grid((unsigned)(first_rows < want ? first_rows : want), a.seqs, a.kv_heads);
   return launch_chained(kv_move_kernel, grid, dim3(256), 0, st, "kv_move_kernel", a, b, (const int32_t*)kept_out,
                         budget, row_bytes, status);
 }

@@ -281,8 +281,8 @@ def page_bounds(cache: PagedKV, bounds: PageBounds, lens: torch.Tensor, start: t
 
 @_on_device
 def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torch.Tensor, budget: int, *,
-                 sinks: int = 1, recent: int = 1, seqs: torch.Tensor | None = None,
-                 workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                 sinks: int = 1, recent: int = 1,
+                 seqs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """For each row and key head up to `budget` pages: the first `sinks`, the
     last `recent`, then those whose bounds allow the greatest product with
     one of the key head's queries (both as int8 codes, so the choice is exact
@@ -297,13 +297,10 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
     lib = _lib.lib()
     pages = torch.empty((rows, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
     counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
-    need = lib.er_kv_select_workspace_bytes(cache._ref, rows, heads)
-    ws = _scratch(need, workspace, cache.device) if need else None
     _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
                                 None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
                                 bounds._codes, bounds._scales, int(budget), int(sinks),
-                                int(recent), pages.data_ptr(), counts.data_ptr(), cache._status,
-                                ws.data_ptr() if need else None, need, cache._stream()), "er_kv_select")
+                                int(recent), pages.data_ptr(), counts.data_ptr(), cache._status, cache._stream()), "er_kv_select")
     return pages, counts
 
 

@@ -465,11 +465,9 @@ ER_API int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, cons
  * (I exact, the products rounded in this order; ties to the lower page, NaN
  * last). pages_out [rows, kv_heads, budget]: ordinals ascending, -1 behind
  * them; counts_out [rows, kv_heads]. lens, seqs as for er_kv_attend. */
-ER_API size_t er_kv_select_workspace_bytes(const er_kv_cache* cache, int rows, int heads);
 ER_API int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, long long q_stride, int rows, int heads,
                         const int32_t* seqs, const int32_t* lens, const int8_t* codes, const float* scales, int budget,
-                        int sinks, int recent, int32_t* pages_out, int32_t* counts_out, int* status, void* workspace,
-                        size_t workspace_bytes, void* stream);
+                        int sinks, int recent, int32_t* pages_out, int32_t* counts_out, int* status, void* stream);
 
 /* Eviction by accumulated attention weight: each key head of each sequence
  * keeps min(lens[s], budget) positions: the first `sinks`, the last `recent`,

@@ -39,7 +39,7 @@ def test_cache_refusals(change, words):
     _fails(L.er_kv_attend(C.byref(c), C.byref(_io()), None, 0, None), words)
     _fails(L.er_kv_append(C.byref(c), P, 1, 8 * 64, None, P, 1, 4, 1e4, P, 1, None, None), words)
     _fails(L.er_kv_page_bounds(C.byref(c), P, P, P, P, None, None), words)
-    _fails(L.er_kv_select(C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 0, 0, P, P, None, None, 0, None), words)
+    _fails(L.er_kv_select(C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 0, 0, P, P, None, None), words)
     _fails(L.er_kv_evict(C.byref(c), C.byref(_cache()), P, P, 1, 1, 64, P, 1, 1, 64, 8, 0, 0, P, P, None, None), words)
 
 
@@ -64,16 +64,15 @@ def test_append_refusals():
 
 def test_select_refusals():
     L, c = _lib.lib(), _cache()
-    args = [C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 1, 1, P, P, None, None, 0, None]
+    args = [C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 1, 1, P, P, None, None]
     for at, value, words in [(1, None, "null"), (2, 3, "q dtype"), (3, 8, "row stride"), (4, -2, "rows -2"),
                              (5, 5, "heads 5"), (7, None, "null"), (8, P + 8, "16-byte"), (10, 0, "budget 0"),
                              (11, 4, "budget 4"), (12, -1, "budget 4"), (4, 4, "4 rows, 3 sequences")]:
         _fails(L.er_kv_select(*[value if i == at else x for i, x in enumerate(args)]), words)
-    assert L.er_kv_select_workspace_bytes(C.byref(c), 3, 4) == 0
-    wide = _cache(table_width=60000)
-    args[0] = C.byref(wide)
-    assert L.er_kv_select(*args) == _lib.ER_ENOSPACE and "workspace 0 bytes" in _lib.last_error()
-    assert L.er_kv_select_workspace_bytes(C.byref(wide), 3, 4) >= 3 * 2 * 60000 * 4
+    args[0] = C.byref(_cache(table_width=600000))
+    _fails(L.er_kv_select(*args), "table of 600000 pages")
+    args[0], args[3], args[5] = C.byref(c), 130 * 64, 130
+    _fails(L.er_kv_select(*args), "65 queries a key head")
 
 
 def test_evict_refusals():
@@ -91,6 +90,7 @@ def test_evict_refusals():
     _fails(call(budget=65), "destination holds 64")
     _fails(call(to_mass_len=7), "7 weights")
     _fails(call(out=P), "lens_out is lens")
+    _fails(call(mass_len=500000), "500000 weights")
     for name in ("lens", "mass", "to_mass", "kept", "out"):
         _fails(call(**{name: None}), "null")
 
