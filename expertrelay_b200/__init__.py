@@ -2,6 +2,8 @@
 
   expertrelay_b200.moe.MoeBlock         one MoE layer in HBM, run by er_moe_block
   expertrelay_b200.backend.B200Backend  the reference's compute-backend protocol
+  expertrelay_b200.kv                   paged key-value cache: append, attention, page selection, eviction
+  expertrelay_b200.kv_cache             PagedKVCache: a model's keys and values of many sequences
   expertrelay_b200.store                expert record layouts (store/layout.py, store/int4.py)
   expertrelay_b200.quant                store weight encodings (int8, int4, GPTQ v1)
   expertrelay_b200.synth                seeded synthetic blocks and activations

@@ -193,7 +193,7 @@ SIGNATURES: dict[str, tuple] = {
     "er_cache_resize": (_i, [_vp, _i, _vp, C.POINTER(_i)]),
     "er_cache_lookup": (_i, [_vp, _i, _i, C.POINTER(_i), C.POINTER(_i)]),
     "er_cache_stats_get": (_i, [_vp, C.POINTER(CacheStats)]),
-    "er_kv_append": (_i, [C.POINTER(KvCache), _vp, _i, C.c_longlong, _vp, _vp, _i, _i, C.c_double, _vp, _i, _vp, _vp]),
+    "er_kv_append": (_i, [C.POINTER(KvCache), _vp, _i, C.c_longlong, _vp, _vp, _vp, _i, _i, C.c_double, _vp, _i, _vp, _vp]),
     "er_kv_attend_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvAttendIO)]),
     "er_kv_attend": (_i, [C.POINTER(KvCache), C.POINTER(KvAttendIO), _vp, C.c_size_t, _vp]),
     "er_kv_page_bounds": (_i, [C.POINTER(KvCache), _vp, _vp, _vp, _vp, _vp, _vp]),

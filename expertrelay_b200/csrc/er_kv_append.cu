@@ -69,7 +69,8 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
 template <typename TX, typename TQ, typename TC, int VEC, int TOK>
 __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
                                                         const int32_t* __restrict__ seqs,
-                                                        const int32_t* __restrict__ positions, int n, int heads,
+                                                        const int32_t* __restrict__ positions,
+                                                        const int32_t* __restrict__ slots, int n, int heads,
                                                         const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
                                                         int* status) {
   __shared__ __align__(16) float cs[TOK][256];  // [d/2] cos, then [d/2] sin
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __r
   int i = threadIdx.x, head = i / per, j = i % per * VEC;
   if (i < tasks) fetch(head, j);
   if ((int)threadIdx.x < live) {
-    const int t = t0 + threadIdx.x, pos = positions[t], seq = seqs ? seqs[t] : t;
+    const int t = t0 + threadIdx.x, pos = slots ? slots[t] : positions[t], seq = seqs ? seqs[t] : t;
     long long off = -1;
     int bad = 0;
     if (seq < 0 || seq >= kv.seqs) {
@@ -293,8 +294,8 @@ const InvFreq& inv_freq(double theta, int d) {
 }
 
 template <typename TX, typename TQ, typename TC>
-int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* seqs, const int32_t* positions, int n,
-              int heads, double theta, void* q_out, int* status, cudaStream_t st) {
+int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* seqs, const int32_t* positions,
+              const int32_t* slots, int n, int heads, double theta, void* q_out, int* status, cudaStream_t st) {
   // 16-byte accesses need half a head in whole VECs and aligned rows
   const bool vec = kv.d % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)(ld * sizeof(TX))) & 15);
   const int tasks = (heads + 2 * kv.kv_heads) * (kv.d / 2) / (vec ? 8 : 1);  // of a token
@@ -304,7 +305,7 @@ int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* se
                         : many ? kv_append_kernel<TX, TQ, TC, 8, 4>
                                : kv_append_kernel<TX, TQ, TC, 8, 1>,
                         dim3(many ? (n + 3) / 4 : n), dim3(threads), 0, st, "kv_append_kernel", kv, (const TX*)qkv, ld,
-                        seqs, positions, n, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
+                        seqs, positions, slots, n, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
 }
 
 }  // namespace
@@ -313,8 +314,8 @@ int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* se
 using namespace er;
 
 extern "C" int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype, long long ld,
-                            const int32_t* seqs, const int32_t* positions, int n, int heads, double theta, void* q_out,
-                            int q_dtype, int* status, void* stream) {
+                            const int32_t* seqs, const int32_t* positions, const int32_t* slots, int n, int heads,
+                            double theta, void* q_out, int q_dtype, int* status, void* stream) {
   if (int rc = kv_check("er_kv_append", cache)) return rc;
   if (n < 0 || heads <= 0 || !(theta > 0))
     return fail(ER_EINVAL, "er_kv_append: n %d, heads %d, theta %g", n, heads, theta);
@@ -330,14 +331,14 @@ extern "C" int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_d
   const int sel = (qkv_dtype == ER_DTYPE_BF16) * 4 + (q_dtype == ER_DTYPE_BF16) * 2 + (cache->dtype == ER_DTYPE_BF16);
   using bf = __nv_bfloat16;
   switch (sel) {
-    case 0: return append_go<float, float, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 1: return append_go<float, float, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 2: return append_go<float, bf, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 3: return append_go<float, bf, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 4: return append_go<bf, float, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 5: return append_go<bf, float, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    case 6: return append_go<bf, bf, float>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
-    default: return append_go<bf, bf, bf>(kv, qkv, ld, seqs, positions, n, heads, theta, q_out, status, st);
+    case 0: return append_go<float, float, float>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 1: return append_go<float, float, bf>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 2: return append_go<float, bf, float>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 3: return append_go<float, bf, bf>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 4: return append_go<bf, float, float>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 5: return append_go<bf, float, bf>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    case 6: return append_go<bf, bf, float>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
+    default: return append_go<bf, bf, bf>(kv, qkv, ld, seqs, positions, slots, n, heads, theta, q_out, status, st);
   }
 }
 

@@ -36,10 +36,10 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 def _need(t, name: str, dtype, device: torch.device, shape=None, contiguous: bool = True) -> None:
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device:
         got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise ValueError(f"{name}: expected a {dtype} tensor on {device}, got {got}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
@@ -84,9 +84,10 @@ class PagedKV:
     table [seqs, width] int32, rows contiguous: the page of each run of
     page_size positions. head_dim: a multiple of 8, at most 256.
 
-    `status` collects what the device found wrong (check())."""
+    `status` ([1] int32; a new one unless given) collects what the device
+    found wrong (check())."""
 
-    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor):
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, status: torch.Tensor | None = None):
         if k.dim() != 4 or k.dtype not in _DTYPES or not k.is_cuda:
             raise ValueError(f"k: expected a [pages, kv_heads, page_size, head_dim] float32 or bfloat16 CUDA tensor, "
                              f"got {tuple(k.shape)} {k.dtype} on {k.device}")
@@ -101,7 +102,9 @@ class PagedKV:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.seqs, self.width = table.shape
         self._apart = _apart(k.shape, k.stride())
-        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        if status is not None:
+            _need(status, "status", torch.int32, k.device, (1,))
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device) if status is None else status
         self._status = self.status.data_ptr()
         self._c = _lib.KvCache(
             k=k.data_ptr(), v=v.data_ptr(), dtype=_DTYPES[k.dtype], num_pages=self.num_pages,
@@ -190,18 +193,23 @@ def _scratch(need: int, workspace: torch.Tensor | None, device: torch.device) ->
 
 @_on_device
 def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: int, theta: float, *,
-           seqs: torch.Tensor | None = None, q_dtype: torch.dtype | None = None) -> torch.Tensor:
-    """New tokens into the cache: qkv [n, (heads + 2 kv_heads) head_dim]
-    (float32 or bfloat16, rows may be strided), one row at positions[i] of
-    sequence seqs[i] (default: i). Returns the rotated queries
-    [n, heads, head_dim] in q_dtype (default: qkv's); k (rotated) and v go to
-    the pages. A (sequence, position) pair may occur once in a call."""
+           seqs: torch.Tensor | None = None, slots: torch.Tensor | None = None,
+           q_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """New tokens into the cache: row i of qkv [n, (heads + 2 kv_heads) head_dim]
+    (float32 or bfloat16, rows may be strided) is token positions[i] of
+    sequence seqs[i] (default: i) and goes to place slots[i] of it in the
+    cache (default: positions[i]; they differ once positions were evicted).
+    Returns the queries, rotated, [n, heads, head_dim] in q_dtype (default:
+    qkv's); k (rotated) and v go to the pages. A (sequence, place) pair may
+    occur once in a call."""
     if qkv.dim() != 2 or qkv.dtype not in _DTYPES or qkv.device != cache.device or \
             qkv.shape[1] != (heads + 2 * cache.kv_heads) * cache.head_dim or qkv.stride(1) != 1:
         raise ValueError(f"qkv: expected [n, {(heads + 2 * cache.kv_heads) * cache.head_dim}] float32 or bfloat16 on "
                          f"{cache.device}, got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
     n = qkv.shape[0]
     _row_args(cache, n, positions, seqs, "positions")
+    if slots is not None:
+        _need(slots, "slots", torch.int32, cache.device, (n,))
     cache._writable()
     dt = qkv.dtype if q_dtype is None else q_dtype
     if dt not in _DTYPES:
@@ -209,8 +217,8 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
     q = torch.empty((n, heads, cache.head_dim), dtype=dt, device=cache.device)
     _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
                                        qkv.stride(0) if n > 1 else qkv.shape[1],
-                                       None if seqs is None else seqs.data_ptr(), positions.data_ptr(), n,
-                                       int(heads), float(theta), q.data_ptr(), _DTYPES[dt],
+                                       None if seqs is None else seqs.data_ptr(), positions.data_ptr(),
+                                       None if slots is None else slots.data_ptr(), n, int(heads), float(theta), q.data_ptr(), _DTYPES[dt],
                                        cache._status, cache._stream()), "er_kv_append")
     return q
 

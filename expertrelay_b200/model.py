@@ -15,6 +15,10 @@ pinned host records on the cache's copy stream), the Fate prefetch of the
 next layer's guesses when a policy is given, and the block on the cached
 records. Only the expert ids cross to the host each layer, to drive the
 cache, as in the reference.
+
+With a PagedKVCache in place of a KVCache, the keys and values of many
+sequences lie in pages (fp32 or bf16): one call may carry tokens of several
+sequences, and attention runs over the pages (expertrelay_b200.kv).
 """
 
 from __future__ import annotations
@@ -27,6 +31,7 @@ import torch
 
 from . import _lib
 from .cache import HbmExpertCache, HostRecords
+from .kv_cache import PagedKVCache
 from .paged import PagedMoeStack
 from .prefetch import PrefetchPolicy
 from .trace import PHASE_DECODE, PHASE_PREFILL
@@ -136,6 +141,10 @@ class QwenMoeModel:
     def new_cache(self, max_seq: int) -> KVCache:
         return KVCache(self.c, max_seq, self.device)
 
+    def new_paged_cache(self, seqs: int, max_seq: int, **options) -> PagedKVCache:
+        """A cache for `seqs` sequences of up to max_seq places each (PagedKVCache's options)."""
+        return PagedKVCache(self.c, seqs, max_seq, device=self.device, **options)
+
     def _stream(self) -> int:
         return torch.cuda.current_stream(self.device).cuda_stream
 
@@ -157,10 +166,14 @@ class QwenMoeModel:
                    "er_rms_norm")
         return h
 
-    def _attention(self, layer: int, h: torch.Tensor, kv: KVCache, allowed: torch.Tensor) -> torch.Tensor:
+    def _attention(self, layer: int, h: torch.Tensor, kv, allowed) -> torch.Tensor:
+        """allowed: the causal mask of a KVCache, or the Step of a PagedKVCache."""
         c, w = self.c, self.layers[layer]
         n, d = h.shape[0], c.head_dim
         qkv = self._linear(h, w["qkv"], w["qkv_bias"])
+        if isinstance(kv, PagedKVCache):
+            out = kv.attend(layer, allowed, qkv, c.num_heads, c.rope_theta)
+            return self._linear(out.view(n, c.num_heads * d), w["o_proj"])
         q = torch.empty((n, c.num_heads * d), dtype=torch.float32, device=self.device)
         start, end = kv.length, kv.length + n
         _lib.check(_lib.lib().er_rope_kv(qkv.data_ptr(), qkv.shape[1], q.data_ptr(), n, c.num_heads, c.num_kv_heads,
@@ -176,25 +189,40 @@ class QwenMoeModel:
                                            self._stream()), "er_attention")
         return self._linear(out, w["o_proj"])
 
-    def forward(self, token_ids, kv: KVCache, *, all_logits: bool = False, expert_trace=None) -> torch.Tensor:
+    def forward(self, token_ids, kv: KVCache | PagedKVCache, *, all_logits: bool = False, expert_trace=None,
+                seqs=None) -> torch.Tensor:
         """Run `token_ids` after what `kv` holds; logits [vocab] of the last
-        position (or [n, vocab] with all_logits), on the device."""
+        position (or [n, vocab] with all_logits), on the device. With a
+        PagedKVCache, `seqs` names the sequence of every token (default: all
+        of sequence 0)."""
         c = self.c
         ids = torch.as_tensor(np.asarray(token_ids, dtype=np.int64)).to(self.device)
         n = ids.shape[0]
-        if kv.length + n > kv.max_seq:
+        paged = isinstance(kv, PagedKVCache)
+        if paged:
+            seqs = np.zeros(n, dtype=np.int64) if seqs is None else np.asarray(seqs, dtype=np.int64)
+            if seqs.shape != (n,):
+                raise ValueError(f"seqs: one sequence for each of {n} tokens, got {seqs.shape}")
+            if expert_trace is not None and len(np.unique(seqs)) > 1:
+                raise ValueError("a trace follows one sequence")
+            allowed = kv.step(seqs)
+        elif seqs is not None:
+            raise ValueError("seqs: only with a PagedKVCache")
+        elif kv.length + n > kv.max_seq:
             raise ValueError(f"sequence length {kv.length + n} exceeds the KV cache ({kv.max_seq})")
         x = torch.empty((n, c.hidden_size), dtype=torch.float32, device=self.device)
         _lib.check(_lib.lib().er_embed_int8(self.embed_q.data_ptr(), self.embed_s.data_ptr(), c.vocab_size,
                                             c.hidden_size, ids.data_ptr(), n, x.data_ptr(), self._bad.data_ptr(),
                                             self._stream()), "er_embed_int8")
+        start = kv.length if not paged else int(kv.pages.position[seqs[0]]) - n
         if expert_trace is not None:
-            positions = kv.length + np.arange(n)
-            expert_trace.begin(positions, np.asarray(token_ids), PHASE_PREFILL if kv.length == 0 else PHASE_DECODE)
-        # causal: query start + i sees keys 0 .. start + i (the same for every layer)
-        start, end = kv.length, kv.length + n
-        allowed = (torch.arange(end, device=self.device)[None, :]
-                   <= (start + torch.arange(n, device=self.device))[:, None]).to(torch.uint8)
+            positions = start + np.arange(n)
+            expert_trace.begin(positions, np.asarray(token_ids), PHASE_PREFILL if start == 0 else PHASE_DECODE)
+        if not paged:
+            # causal: query start + i sees keys 0 .. start + i (the same for every layer)
+            end = start + n
+            allowed = (torch.arange(end, device=self.device)[None, :]
+                       <= (start + torch.arange(n, device=self.device))[:, None]).to(torch.uint8)
         h = self._norm(x, self.layers[0]["in_norm"])
         for layer in range(c.num_layers):
             a = self._attention(layer, h, kv, allowed)
@@ -202,7 +230,8 @@ class QwenMoeModel:
             y = self.stack.moe(layer, h, self.path, trace=expert_trace)
             if layer + 1 < c.num_layers:
                 h = self._norm(x, self.layers[layer + 1]["in_norm"], add=y)
-        kv.length += n
+        if not paged:
+            kv.length += n
         if expert_trace is not None:
             expert_trace.end()
         rows = slice(None) if all_logits else slice(n - 1, n)
@@ -214,12 +243,14 @@ class QwenMoeModel:
             raise ValueError(f"token ids outside [0, {c.vocab_size})")
         return logits if all_logits else logits[0]
 
-    def generate(self, prompt, new_tokens: int, *, max_seq: int | None = None, expert_trace=None):
+    def generate(self, prompt, new_tokens: int, *, max_seq: int | None = None, expert_trace=None, kv=None):
         """Greedy decoding (runtime/generate.py): the prompt in one call, then
         one token per call. Returns (generated ids, seconds of the prompt call,
-        seconds per decode call)."""
+        seconds per decode call). kv: a cache of one's own (a PagedKVCache's
+        sequence 0); otherwise a new KVCache of max_seq positions."""
         prompt = [int(t) for t in prompt]
-        kv = self.new_cache(max_seq or len(prompt) + new_tokens)
+        if kv is None:
+            kv = self.new_cache(max_seq or len(prompt) + new_tokens)
         torch.cuda.synchronize(self.device)
         t0 = time.perf_counter()
         logits = self.forward(prompt, kv, expert_trace=expert_trace)

@@ -406,14 +406,15 @@ typedef struct er_kv_cache {
 
 /* RoPE and the write of new tokens' rows into the pages: row i of qkv
  * [n, (heads + 2 kv_heads) head_dim] (q | k | v, dtype qkv_dtype, row stride
- * ld) belongs to position positions[i] of sequence seqs[i] (seqs NULL: i).
- * Its q heads are rotated into q_out [n, heads, head_dim] (q_dtype), its k
- * heads rotated into the page, its v heads copied there. Angles are
- * position * theta^(-2j/head_dim) in 64 bits, rotate-half. A (sequence,
- * position) pair may occur once per call. */
+ * ld) is token positions[i] of sequence seqs[i] (seqs NULL: i) and goes to
+ * place slots[i] of it in the cache (slots NULL: positions[i]; the two differ
+ * once positions were evicted). Its q heads are rotated into q_out
+ * [n, heads, head_dim] (q_dtype, not over qkv), its k heads rotated into the
+ * page, its v heads copied there. Angles are position * theta^(-2j/head_dim)
+ * in 64 bits, rotate-half. A (sequence, place) pair may occur once per call. */
 ER_API int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype, long long ld, const int32_t* seqs,
-                        const int32_t* positions, int n, int heads, double theta, void* q_out, int q_dtype,
-                        int* status, void* stream);
+                        const int32_t* positions, const int32_t* slots, int n, int heads, double theta, void* q_out,
+                        int q_dtype, int* status, void* stream);
 
 /* Attention of rows of queries over the pages: row r has `heads` queries
  * (heads / kv_heads of them per key head) that see the first lens[r]

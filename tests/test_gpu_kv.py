@@ -564,3 +564,69 @@ def test_streams_and_graph_replay(cuda):
         out = kv.attend(cache, q, ns)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, outs[0])
+
+
+def test_append_into_other_places(cuda):
+    """slots apart from positions: the angle goes by one, the place by the other."""
+    k = torch.zeros((4, 1, 16, 64), device="cuda")
+    cache = kv.PagedKV(k, k.clone(), _i32([[2, 0]]))
+    x = torch.randn((2, 3 * 64), device="cuda")
+    kv.append(cache, x, _i32([900, 901]), 1, 1e4, seqs=_i32([0, 0]), slots=_i32([3, 17]))
+    other = kv.PagedKV(torch.zeros((64, 1, 16, 64), device="cuda"), torch.zeros((64, 1, 16, 64), device="cuda"),
+                       torch.arange(64, dtype=torch.int32, device="cuda")[None])
+    kv.append(other, x, _i32([900, 901]), 1, 1e4, seqs=_i32([0, 0]))
+    assert torch.equal(k[2, 0, 3], other.k[900 // 16, 0, 900 % 16]) and torch.equal(k[0, 0, 1], other.k[901 // 16, 0, 901 % 16])
+    assert int((k != 0).any(-1).sum()) == 2
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_run_of_them_together(cuda, dtype):
+    """Prompts appended and attended with their weights, sequences cut by
+    them, then new tokens: against attention over the kept keys in 64 bits."""
+    gen = torch.Generator().manual_seed(11)
+    S, KH, H, d, ps, theta = 3, 2, 6, 64, 16, 1e4
+    lens, budget, sinks, recent = [200, 90, 37], 64, 4, 16
+    pages = 60
+    k, v = (torch.full((pages, KH, ps, d), float("nan"), dtype=dtype, device="cuda") for _ in range(2))
+    ids = torch.randperm(pages, generator=gen).to(torch.int32)
+    table, to_table = ids[:3 * 14].view(3, 14).cuda(), ids[42:54].view(3, 4).cuda()
+    cache, to = kv.PagedKV(k, v, table), kv.PagedKV(k, v, to_table)
+    seqs = [s for s, n in enumerate(lens) for _ in range(n)]
+    pos = [p for n in lens for p in range(n)]
+    qkv = torch.randn((len(seqs), (H + 2 * KH) * d), generator=gen).to(dtype).cuda()
+    q = kv.append(cache, qkv, _i32(pos), H, theta, seqs=_i32(seqs))
+    rows = torch.zeros((len(seqs), KH, 224), device="cuda")
+    seen = [p + 1 for p in pos]
+    out = kv.attend(cache, q, _i32(seen), seqs=_i32(seqs), mass=rows)
+    pick = [0, 7, 199, 200, 289, 290, 326]
+    _check_attend(cache, q[pick], [seen[i] for i in pick], out[pick], seqs=[seqs[i] for i in pick])
+    mass = torch.stack([rows[[i for i, s in enumerate(seqs) if s == r]].sum(0) for r in range(S)])
+    to_mass = torch.zeros((S, KH, 64), device="cuda")
+    kept, new = kv.evict(cache, _i32(lens), mass, to, to_mass, budget, sinks=sinks, recent=recent)
+    assert new.tolist() == [64, 64, 37]
+    host = mass.cpu().numpy()
+    old = {s: (tokens(k, table, s, lens[s]), tokens(v, table, s, lens[s])) for s in range(S)}
+    for s in range(S):
+        for h in range(KH):
+            assert kept[s, h, :new[s]].tolist() == choose(host[s, h], lens[s], budget, sinks, recent)
+    # 60 places more of every table: new tokens go behind the kept ones, at their own positions
+    table2 = torch.cat([to_table, ids[54:60].view(3, 2).cuda()], 1)
+    cache2 = kv.PagedKV(k, v, table2)
+    step = torch.randn((S, (H + 2 * KH) * d), generator=gen).to(dtype).cuda()
+    q2 = kv.append(cache2, step, _i32(lens), H, theta, slots=new)
+    mass2 = torch.zeros((S, KH, 96), device="cuda")
+    mass2[:, :, :64] = to_mass
+    mass0 = mass2.clone()
+    out2 = kv.attend(cache2, q2, new + 1, mass=mass2)
+    _check_attend(cache2, q2, (new + 1).tolist(), out2, mass=mass2, mass0=mass0)
+    for s in range(S):
+        got_k, got_v = tokens(k, table2, s, int(new[s])), tokens(v, table2, s, int(new[s]))
+        for h in range(KH):
+            at = kept[s, h, :new[s]].cpu().numpy()
+            assert np.array_equal(got_k[h], old[s][0][h][at]) and np.array_equal(got_v[h], old[s][1][h][at])
+    # and sparsely, with room for every page: the same keys
+    bounds = kv.PageBounds.new(cache2)
+    kv.page_bounds(cache2, bounds, new + 1, _i32([0, 0, 0]))
+    sel, counts = kv.select_pages(cache2, bounds, q2, new + 1, 6)
+    _check_attend(cache2, q2, (new + 1).tolist(), kv.attend(cache2, q2, new + 1, pages=sel, counts=counts))
+    cache.check(), cache2.check()

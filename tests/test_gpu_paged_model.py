@@ -1,0 +1,132 @@
+"""GPU: the decoder over a paged key-value cache (PagedKVCache): the
+reference's logits and greedy tokens as with the contiguous cache, several
+sequences in one call as each alone, page selection and eviction that leave
+everything in as the full cache, and what a generation does under both."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from conftest import golden
+from golden.make_golden import MODEL_CASES, MODEL_NEW, MODEL_PROMPT
+
+from expertrelay_b200 import _lib, synth
+from expertrelay_b200.model import QwenMoeModel
+from oracle.moe_oracle import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+TOL = 1e-4  # the contiguous cache's, on the exact-fp32 expert path
+
+
+def _model(case, cuda, path=_lib.PATH_GEMM):
+    cfg, seed = MODEL_CASES[case]
+    return QwenMoeModel(synth.make_model(cfg, seed=seed), device=cuda, path=path)
+
+
+@pytest.mark.parametrize("case", range(len(MODEL_CASES)))
+@pytest.mark.parametrize("options", [{}, {"page_size": 5}, {"mass": True, "page_size": 8}, {"select": (64, 1, 1), "page_size": 4}])
+def test_paged_model_matches_reference(case, options, cuda):
+    g = golden("model")
+    model = _model(case, cuda)
+    kv = model.new_paged_cache(1, MODEL_PROMPT + MODEL_NEW, **options)
+    logits = model.forward(g[f"prompt{case}"], kv, all_logits=True).cpu().numpy()
+    assert rel_l2(logits, g[f"prompt_logits{case}"]) < TOL
+    tok = int(np.argmax(logits[-1]))
+    for step in range(MODEL_NEW):
+        assert tok == g[f"tokens{case}"][step]
+        lg = model.forward([tok], kv).cpu().numpy()
+        assert rel_l2(lg, g[f"step_logits{case}"][step]) < TOL
+        tok = int(np.argmax(lg))
+    if kv.mass is not None:
+        # every row's weights sum to one for each query: length x queries a key head in all
+        n, group = MODEL_PROMPT + MODEL_NEW, model.c.num_heads // model.c.num_kv_heads
+        total = kv.mass.sum(-1).cpu().numpy()
+        np.testing.assert_allclose(total, n * group, rtol=1e-4)
+        assert torch.all(kv.mass[..., n:] == 0)
+    kv.check()
+    model.close()
+
+
+def test_bf16_cache_is_near(cuda):
+    """Keys and values rounded to 16 bits (2^-8 at most each) move the logits by about as much."""
+    g = golden("model")
+    model = _model(0, cuda)
+    kv = model.new_paged_cache(1, MODEL_PROMPT, dtype=torch.bfloat16)
+    logits = model.forward(g["prompt0"], kv, all_logits=True).cpu().numpy()
+    assert rel_l2(logits, g["prompt_logits0"]) < 2.0 ** -5
+    model.close()
+
+
+def test_sequences_in_one_call_are_as_alone(cuda):
+    model = _model(1, cuda)
+    rng = np.random.default_rng(4)
+    prompts = [rng.integers(0, model.c.vocab_size, n) for n in (9, 1, 14)]
+    alone = []
+    for p in prompts:
+        kv = model.new_cache(len(p) + 3)
+        steps = [model.forward(p, kv).cpu().numpy()]
+        for t in (5, 6, 7):
+            steps.append(model.forward([t], kv).cpu().numpy())
+        alone.append(steps)
+    kv = model.new_paged_cache(4, 32, page_size=8)
+    seqs = np.concatenate([np.full(len(p), s) for s, p in zip((0, 1, 3), prompts)])
+    order = np.argsort(np.concatenate([np.arange(len(p)) for p in prompts]), kind="stable")  # interleaved
+    logits = model.forward(np.concatenate(prompts)[order], kv, all_logits=True, seqs=seqs[order]).cpu().numpy()
+    last = [int(np.flatnonzero(seqs[order] == s)[-1]) for s in (0, 1, 3)]
+    for i in range(3):
+        assert rel_l2(logits[last[i]], alone[i][0]) < TOL
+    for j, t in enumerate((5, 6, 7)):
+        lg = model.forward([t, t, t], kv, all_logits=True, seqs=[3, 0, 1]).cpu().numpy()
+        for row, i in ((0, 2), (1, 0), (2, 1)):
+            assert rel_l2(lg[row], alone[i][j + 1]) < TOL
+    assert [kv.length(s) for s in range(4)] == [12, 4, 0, 17]
+    kv.release(0)
+    assert kv.length(0) == 0
+    assert rel_l2(model.forward(prompts[0], kv).cpu().numpy(), alone[0][0]) < TOL
+    kv.check()
+    model.close()
+
+
+def test_generation_with_eviction(cuda):
+    model = _model(0, cuda)
+    g = golden("model")
+    kv = model.new_paged_cache(2, 64, page_size=4, mass=True)
+    for s in (0, 1):
+        model.forward(g["prompt0"], kv, seqs=[s] * MODEL_PROMPT)
+    free = len(kv.pages.free)
+    kv.evict(64, recent=8)  # nothing is that long
+    assert len(kv.pages.free) == free and kv.length(0) == MODEL_PROMPT
+    budget = MODEL_PROMPT - 3
+    kv.evict(budget, sinks=1, recent=2)
+    assert kv.length(0) == kv.length(1) == budget and int(kv.pages.position[0]) == MODEL_PROMPT
+    assert len(kv.pages.free) >= free
+    assert sorted(kv.pages.free + [int(p) for p in kv.pages.table.ravel() if p >= 0]) == list(range(32))
+    tok = int(g["tokens0"][0])
+    both = model.forward([tok, tok], kv, all_logits=True, seqs=[0, 1])
+    assert torch.equal(both[0], both[1]) and torch.isfinite(both).all()
+    assert kv.length(0) == budget + 1
+    kv.check()
+    model.close()
+
+
+def test_paged_refusals(cuda):
+    model = _model(0, cuda)
+    kv = model.new_paged_cache(1, 8, page_size=4)
+    with pytest.raises(ValueError, match="sequence length 9 exceeds the KV cache"):
+        model.forward([1] * 9, kv)
+    assert kv.length() == 0
+    with pytest.raises(ValueError, match="outside"):
+        model.forward([1], kv, seqs=[1])
+    with pytest.raises(ValueError, match="one sequence for each"):
+        model.forward([1, 2], kv, seqs=[0])
+    with pytest.raises(ValueError, match="only with a PagedKVCache"):
+        model.forward([1], model.new_cache(4), seqs=[0])
+    with pytest.raises(ValueError, match="mass=True"):
+        kv.evict(4)
+    with pytest.raises(ValueError, match="mass and select"):
+        model.new_paged_cache(1, 8, mass=True, select=(4, 1, 1))
+    with pytest.raises(ValueError, match="select"):
+        model.new_paged_cache(1, 8, select=(1, 1, 1))
+    model.close()

@@ -7,6 +7,7 @@ import ctypes as C
 import pytest
 
 from expertrelay_b200 import _lib
+from expertrelay_b200.kv_cache import PageTable
 
 P = 0x1000  # an address that is never followed
 
@@ -37,7 +38,7 @@ def _fails(rc, words):
 def test_cache_refusals(change, words):
     L, c = _lib.lib(), _cache(**change)
     _fails(L.er_kv_attend(C.byref(c), C.byref(_io()), None, 0, None), words)
-    _fails(L.er_kv_append(C.byref(c), P, 1, 8 * 64, None, P, 1, 4, 1e4, P, 1, None, None), words)
+    _fails(L.er_kv_append(C.byref(c), P, 1, 8 * 64, None, P, None, 1, 4, 1e4, P, 1, None, None), words)
     _fails(L.er_kv_page_bounds(C.byref(c), P, P, P, P, None, None), words)
     _fails(L.er_kv_select(C.byref(c), P, 1, 256, 1, 4, None, P, P, P, 4, 0, 0, P, P, None, None), words)
     _fails(L.er_kv_evict(C.byref(c), C.byref(_cache()), P, P, 1, 1, 64, P, 1, 1, 64, 8, 0, 0, P, P, None, None), words)
@@ -55,10 +56,10 @@ def test_attend_refusals(change, words):
 
 def test_append_refusals():
     L, c = _lib.lib(), _cache()
-    args = [C.byref(c), P, 1, 8 * 64, None, P, 1, 4, 1e4, P, 1, None, None]
+    args = [C.byref(c), P, 1, 8 * 64, None, P, None, 1, 4, 1e4, P, 1, None, None]
     for at, value, words in [(1, None, "null"), (2, 5, "dtypes 5"), (3, 8 * 64 - 1, "row stride"), (5, None, "null"),
-                             (6, -1, "n -1"), (7, 0, "heads 0"), (8, 0.0, "theta 0"), (8, float("nan"), "theta"),
-                             (9, None, "null"), (10, 9, "9")]:
+                             (7, -1, "n -1"), (8, 0, "heads 0"), (9, 0.0, "theta 0"), (9, float("nan"), "theta"),
+                             (10, None, "null"), (11, 9, "9")]:
         _fails(L.er_kv_append(*[value if i == at else x for i, x in enumerate(args)]), words)
 
 
@@ -98,5 +99,39 @@ def test_evict_refusals():
 def test_nothing_to_do_is_fine():
     L = _lib.lib()
     assert L.er_kv_attend(C.byref(_cache()), C.byref(_io(rows=0)), None, 0, None) == _lib.ER_OK
-    assert L.er_kv_append(C.byref(_cache()), P, 1, 512, None, P, 0, 4, 1e4, P, 1, None, None) == _lib.ER_OK
+    assert L.er_kv_append(C.byref(_cache()), P, 1, 512, None, P, None, 0, 4, 1e4, P, 1, None, None) == _lib.ER_OK
     assert L.er_kv_page_bounds(C.byref(_cache(seqs=0)), P, P, P, P, None, None) == _lib.ER_OK
+
+
+def test_page_table_gives_and_takes_pages():
+    t = PageTable(3, 4, 7, 16)
+    pos, slots = t.extend([0] * 17 + [2])
+    assert pos.tolist() == slots.tolist() == [*range(17), 0]
+    assert t.length.tolist() == t.position.tolist() == [17, 0, 1] and len(t.free) == 4
+    pages = [p for p in t.table.ravel() if p >= 0]
+    assert len(pages) == len(set(pages)) == 3
+    pos, slots = t.extend([2, 0, 2])  # interleaved
+    assert pos.tolist() == [1, 17, 2] and slots.tolist() == [1, 17, 2]
+    # evicted to 5 places: positions go on, places start over
+    t.replace(0, t.take(1), 5)
+    pos, slots = t.extend([0])
+    assert pos.tolist() == [18] and slots.tolist() == [5]
+    t.release(0)
+    assert t.length.tolist() == [0, 0, 3] and t.position.tolist() == [0, 0, 3] and len(t.free) == 6
+    assert sorted(t.free + [int(p) for p in t.table.ravel() if p >= 0]) == list(range(7))
+
+
+def test_page_table_refusals_change_nothing():
+    t = PageTable(2, 4, 5, 16)
+    t.extend([0] * 48)
+    before = (t.table.copy(), t.length.copy(), t.position.copy(), list(t.free))
+    for seqs, words in [([0] * 17, "sequence length 65 exceeds"), ([1] * 33, "out of pages"), ([2], "outside"), ([-1], "outside")]:
+        with pytest.raises(ValueError, match=words):
+            t.extend(seqs)
+    with pytest.raises(ValueError, match="out of pages"):
+        t.take(3)
+    assert (t.table == before[0]).all() and (t.length == before[1]).all() and (t.position == before[2]).all()
+    assert t.free == before[3]
+    assert [len(x) for x in t.extend([])] == [0, 0]
+    with pytest.raises(ValueError, match="at least one"):
+        PageTable(1, 0, 1, 16)
