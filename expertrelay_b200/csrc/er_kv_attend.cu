@@ -67,11 +67,16 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   const int col = threadIdx.x % cols, grp = threadIdx.x / cols;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < groups) {
-#pragma unroll 8
-    for (int k = grp; k < n; k += groups) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + piece(k) * d + col * 4);
-      const float by = wt[k];
-      fma4(acc, x, by);
+    constexpr int N = 12;  // pieces a thread has under way
+#pragma unroll 1
+    for (int k0 = grp; k0 < n; k0 += groups * N) {
+      float4 x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k0 + j * groups < n) x[j] = *reinterpret_cast<const float4*>(a.part_o + piece(k0 + j * groups) * d + col * 4);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k0 + j * groups < n) fma4(acc, x[j], wt[k0 + j * groups]);
     }
   }
   float4* part = reinterpret_cast<float4*>(wt + (a.grid + 3) / 4 * 4);

@@ -133,6 +133,24 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, RunScratch& s) {
     a.cut[blockIdx.x].row = -1;
     s.before[0] = s.before[1] = 0;
   }
+  if (a.entries == 1) {  // nothing to sum
+    Run r = {};
+    r.e = kv_entry(a, 0);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && r.e.bad) kv_report(a.status, r.e.bad);
+    r.tiles = kv_tiles(a, r.e.n);
+    const int k = kv_cost(r.tiles);
+    r.total = (long long)k * a.units;
+    if (k == 0) return r;
+    const int shares = kv_shares(a, r.total);
+    if ((int)blockIdx.x >= shares) return r;
+    const long long at = kv_share_start(r.total, shares, blockIdx.x), to = kv_share_start(r.total, shares, blockIdx.x + 1);
+    r.u = (int)kv_div(at, k);
+    r.begin = (long long)r.u * k;
+    r.t = max(0, (int)(at - r.begin) - kUnitCost);
+    const int v = (int)kv_div(to, k);
+    r.left = (long long)v * r.tiles + max(0, (int)(to - (long long)v * k) - kUnitCost) - ((long long)r.u * r.tiles + r.t);
+    return r;
+  }
   const int per = (a.entries + threads - 1) / threads;
   const int x0 = min(a.entries, (int)threadIdx.x * per), x1 = min(a.entries, x0 + per);
   long long cost = 0, tiles = 0;

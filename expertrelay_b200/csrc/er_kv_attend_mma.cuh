@@ -104,8 +104,10 @@ __device__ __forceinline__ float cut_tf32(float& x) {
 constexpr int kMergeHeads = 4;  // queries whose pieces the warps exchange at a time
 
 // A CTA's shape for a cache of TC, queries and results of TQ, head_dim padded
-// to DP, NT tiles of 8 queries. The rings hold about 96 KB (two CTAs an SM)
-// where a warp's stage is 8 KB, one CTA's worth beyond.
+// to DP, NT tiles of 8 queries. Two CTAs an SM where a warp's stage is 8 KB:
+// two stages of 8 warps are 128 KB under way on an SM, twice what latency
+// times bandwidth asks for (three stages gained nothing, and 12 warps of two
+// stages lost 40 % at head_dim 128, their registers cut to 168).
 template <typename TC, typename TQ, int DP, int NT>
 struct Mma {
   static constexpr bool kBf16 = sizeof(TC) == 2;
@@ -115,7 +117,7 @@ struct Mma {
   static constexpr int kKeys = kRow == 128 ? 32 : 16;  // keys a warp takes at a time
   static constexpr int kChunkBytes = kKeys * kRow;
   static constexpr int kWarps = kRow <= 256 ? 4 : kBf16 ? 4 : kRow == 512 ? (NT == 1 ? 3 : 6) : 3;
-  static constexpr int kStages = kRow <= 256 ? 3 : kBf16 ? (NT * QS == 6 ? 2 : 3) : 2;
+  static constexpr int kStages = kBf16 && kRow == 512 && NT * QS < 6 ? 3 : 2;
   static constexpr int kRing = kWarps * kStages * 2 * kChunkBytes;
   static constexpr int kKSteps = kBf16 ? DP / 16 : DP / 8;  // matrix products along the channels of the scores
   static constexpr int kQuery = kKSteps * QS * NT * 32 * 8;
