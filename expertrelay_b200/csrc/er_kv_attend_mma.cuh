@@ -21,8 +21,8 @@
 // bf16 results and as three for fp32 ones. Parts are cut, not rounded, so
 // that they share the sign of the whole and an infinite key or value stays
 // infinite. fp32 caches (m16n8k8, tf32 with 11 bits): every operand is its
-// leading 11 bits and the rest, and of the products all but rest times rest
-// (2^-22 of the whole) are taken; where a key or value that is seen is
+// leading 11 bits and the rest (11 more), and of the products all but rest
+// times rest (2^-22 of the whole) are taken; where a key or value that is seen is
 // infinite, the result is infinite or NaN. The tensor cores cut their sums
 // (they do not round), so fp32 results add each chunk's products up there and
 // the running sum in rounded fp32.
@@ -94,6 +94,8 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const float (&a)[4], flo
       : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
         "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
 }
+// x, such that its leading 11 bits (all that the tensor cores look at) are x rounded
+__device__ __forceinline__ float round_tf32(float x) { return __uint_as_float(__float_as_uint(x) + 0x1000u); }
 // the leading 11 bits of x; x becomes the rest
 __device__ __forceinline__ float cut_tf32(float& x) {
   const float hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
@@ -226,8 +228,16 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
           for (int e = 0; e < 2; ++e) {
             const int cc = c0 + e * 4;
             x[e] = g < live_g && cc < d ? to_f32(qr[g * d + cc]) : 0.f;
-            hi[e] = cut_tf32(x[e]);
-            if (!(fabsf(hi[e]) < INFINITY)) x[e] = 0.f;
+            // leading bits rounded, so that the rest has either sign and what the
+            // products leave out (rest times rest) has no mean; cut where that overflows
+            const float near = __uint_as_float(__float_as_uint(round_tf32(x[e])) & 0xffffe000u);
+            if (fabsf(near) < INFINITY && fabsf(x[e]) < INFINITY) {
+              hi[e] = near;
+              x[e] = round_tf32(x[e] - near);
+            } else {
+              hi[e] = cut_tf32(x[e]);
+              if (!(fabsf(hi[e]) < INFINITY)) x[e] = 0.f;
+            }
           }
           to[0] = make_uint2(__float_as_uint(hi[0]), __float_as_uint(hi[1]));
           to[NT * 32] = make_uint2(__float_as_uint(x[0]), __float_as_uint(x[1]));
@@ -250,10 +260,10 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
       if (now.keys) {
         const uint32_t kc = smem_addr(ring + st * 2 * C::kChunkBytes), vc = kc + C::kChunkBytes;
         const int mi = lane / 8, mr = lane % 8;  // the 8x8 matrix and its row that this lane addresses
-        // Two chains of products: their latencies overlap, and each is summed
-        // over half as many steps (the parts below the leading ones in the
-        // second). With 32 keys the key blocks are chains of their own.
-        constexpr int CH = KB == 1 || QS > 1 ? 2 : 1;
+        // Two or three chains of products: their latencies overlap, and each is
+        // summed over fewer steps (the parts below the leading ones in the
+        // last). With 32 keys the key blocks are chains of their own.
+        constexpr int CH = !BF ? 3 : KB == 1 || QS > 1 ? 2 : 1;
         float s2[KB][CH][NT][4];
 #pragma unroll
         for (int i = 0; i < KB * CH * NT; ++i)
@@ -279,13 +289,14 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
               for (int e = 0; e < 4; ++e) {
                 lo[e] = __uint_as_float(kf[e]);
                 hi[e] = cut_tf32(lo[e]);
+                lo[e] = round_tf32(lo[e]);  // cut, it would lower every score by about 2^-23 of it
               }
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 const uint2 bh = qf[(ks * QS * NT + nt) * 32 + lane], bl = qf[((ks * QS + 1) * NT + nt) * 32 + lane];
-                mma_tf32(s2[kb][1][nt], lo, __uint_as_float(bh.x), __uint_as_float(bh.y));
-                mma_tf32(s2[kb][1][nt], hi, __uint_as_float(bl.x), __uint_as_float(bl.y));
-                mma_tf32(s2[kb][0][nt], hi, __uint_as_float(bh.x), __uint_as_float(bh.y));
+                mma_tf32(s2[kb][CH - 1][nt], lo, __uint_as_float(bh.x), __uint_as_float(bh.y));
+                mma_tf32(s2[kb][CH - 1][nt], hi, __uint_as_float(bl.x), __uint_as_float(bl.y));
+                mma_tf32(s2[kb][ks & (CH / 2)][nt], hi, __uint_as_float(bh.x), __uint_as_float(bh.y));
               }
             }
           }
@@ -300,7 +311,9 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const bool on = (now.keys >> (kb * 16 + lane / 4 + (e >> 1) * 8)) & 1;
-              const float s = s2[kb][0][nt][e] + (CH == 2 ? s2[kb][CH - 1][nt][e] : 0.f);
+              float s = s2[kb][0][nt][e];
+#pragma unroll
+              for (int c = 1; c < CH; ++c) s += s2[kb][c][nt][e];
               p[kb][nt][e] = on ? s * a.scale : -INFINITY;
             }
             if (a.scores) {
@@ -409,8 +422,12 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
               const uint32_t low = transpose8(__byte_perm(x, y, 0x5410)), up = transpose8(__byte_perm(x, y, 0x7632));
               bl[half][nt][0] = __uint_as_float(__byte_perm(low, up, 0x5410));
               bl[half][nt][1] = __uint_as_float(__byte_perm(low, up, 0x7632));
-              bh[half][nt][0] = cut_tf32(bl[half][nt][0]);
-              bh[half][nt][1] = cut_tf32(bl[half][nt][1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {  // rounded, as the queries; a weight is 1 at the most
+                float& w = bl[half][nt][e];
+                bh[half][nt][e] = __uint_as_float(__float_as_uint(round_tf32(w)) & 0xffffe000u);
+                w = w == w ? round_tf32(w - bh[half][nt][e]) : w;
+              }
             }
 #pragma unroll
           for (int k = 0; k < MT; ++k) {
