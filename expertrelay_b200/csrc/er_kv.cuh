@@ -353,10 +353,10 @@ __device__ __forceinline__ void take_best(const HeldKeys& keys, int b0, int nl, 
     const int b = r0 + (int)threadIdx.x * run;
     uint32_t sure, tied;
     look(b, &sure, &tied);
-    // 16 bits each: a round has at most 32 * 1024 positions
+    // 16 bits each, without sign: a round has at most 32 * 1024 positions
     int all;
     const int before = block_scan(__popc(sure) | __popc(tied) << 16, sc.red, &all);
-    int at = above + (before & 0xffff), tie = same + (before >> 16);
+    int at = above + (before & 0xffff), tie = same + (int)((uint32_t)before >> 16);
     for (uint32_t left = sure | tied; left; left &= left - 1) {
       const int j = __ffs(left) - 1;
       if ((sure >> j) & 1) {
@@ -368,7 +368,7 @@ __device__ __forceinline__ void take_best(const HeldKeys& keys, int b0, int nl, 
       }
     }
     above += all & 0xffff;
-    same += all >> 16;
+    same += (int)((uint32_t)all >> 16);
   }
   meet();  // no CTA leaves while its counts may be read
 }

@@ -397,6 +397,23 @@ def test_evict_more_than_shared_memory_holds(cuda):
     assert torch.equal(to.k[0, 0], k.reshape(-1, 8)[ids])
 
 
+@pytest.mark.parametrize(("seqs", "n", "budget"), [(38, 32768 + 100, 50), (38, 32768 + 100, 32800), (1, 8 * 32768 + 800, 270)])
+def test_evict_equal_weights_fill_a_round(cuda, seqs, n, budget):
+    # a round of a CTA's scan is 32768 positions, here all of them ties: by a CTA alone, and by a cluster together
+    k = torch.randn((n // 4 + 1, 1, 4, 8), generator=torch.Generator().manual_seed(3)).cuda()
+    table = torch.arange(n // 4 + 1, dtype=torch.int32, device="cuda").expand(seqs, -1)  # all read the same pages
+    cache = kv.PagedKV(k, k, table)
+    tk = torch.zeros((seqs, 1, budget, 8), device="cuda")
+    to = kv.PagedKV(tk, tk.clone(), torch.arange(seqs, dtype=torch.int32, device="cuda")[:, None])
+    mass = torch.full((seqs, 1, n), 0.25, device="cuda")
+    mass[:, :, n - 10] = 1.0
+    kept, new = kv.evict(cache, _i32([n] * seqs), mass, to, torch.zeros((seqs, 1, budget), device="cuda"), budget, sinks=0, recent=0)
+    want = torch.tensor([*range(budget - 1), n - 10], dtype=torch.int32, device="cuda")
+    assert torch.all(kept == want) and torch.all(new == budget)
+    assert torch.equal(to.k, k.view(-1, 8)[want.long()].expand(seqs, 1, -1, -1))
+    cache.check()
+
+
 def test_select_ties_zeros_and_bad_rows(cuda):
     lens = [640, 640, 640, 640]
     cache, q, bounds = _select_case(4, lens, 1, 2, 64, 16, F32)
