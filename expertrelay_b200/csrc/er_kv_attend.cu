@@ -104,9 +104,9 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
   float* to = a.mass + row * a.mass_row_stride + h * a.mass_head_stride;
   const float* s = a.scores + (long long)unit * a.mass_len * a.group;
   const float* lse = a.lse + (long long)row * a.heads + h * a.group;
-  for (int j = blockIdx.x * 256 + threadIdx.x; j < e.n; j += gridDim.x * 256) {
+  for (long long j = blockIdx.x * 256 + threadIdx.x; j < e.n; j += gridDim.x * 256) {  // a step may pass 2^31
     float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) sum += exp2f(s[(long long)j * a.group + g] - lse[g]);
+    for (int g = 0; g < a.group; ++g) sum += exp2f(s[j * a.group + g] - lse[g]);
     to[j] += sum;
   }
 }
@@ -200,6 +200,7 @@ extern "C" int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io,
   if (int rc = attend_check(cache, io)) return rc;
   if (io->rows == 0) return ER_OK;
   if (!io->q || !io->out || !io->lens) return fail(ER_EINVAL, "er_kv_attend: null pointer");
+  if ((uintptr_t)io->out & 15) return fail(ER_EINVAL, "er_kv_attend: out must be 16-byte aligned");
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   const Layout L = attend_layout(*cache, *io, sms);

@@ -19,8 +19,13 @@ waits on the host. Lengths, positions, tables and lists are read on the
 device, so a call captured in a CUDA graph serves whatever they hold at
 replay. What is wrong with them (a page id outside the pool, a length
 outside the table) is found there too: the rows concerned come back as NaN
-or stay unwritten, and PagedKV.check() raises. Each call allocates its
-workspace from torch's allocator on that stream unless given one.
+(their mass with them) or stay unwritten, and PagedKV.check() raises. attend
+allocates its workspace from torch's allocator on that stream unless given one.
+
+Infinities: an infinite or NaN key or value behind a row's length changes
+nothing. One that is seen makes the row's results what the formula gives,
+infinite or NaN; over an fp32 cache they may be NaN where the formula gives an
+infinity. Scores of -inf weigh nothing.
 """
 
 from __future__ import annotations
@@ -55,6 +60,20 @@ def _apart(shape, stride) -> bool:
     return True
 
 
+def _share(a, b) -> bool:
+    """Whether two [seqs, heads, n] tensors may share an element: their extents meet, and they are no two
+    layers of one array."""
+    (a, b) = sorted((a, b), key=lambda t: t.data_ptr())
+    size = a.element_size()
+    if not a.numel() or not b.numel():
+        return False
+    apart = (b.data_ptr() - a.data_ptr()) // size
+    if apart > sum((n - 1) * s for n, s in zip(a.shape, a.stride())):
+        return False
+    shape = [max(m, n) for m, n in zip(a.shape, b.shape)]
+    return a.stride() != b.stride() or not _apart((2, *shape), (apart, *a.stride()))
+
+
 def _weights(t, name: str, cache, rows: int, written: bool) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"{name}: expected [{rows}, {cache.kv_heads}, n] with contiguous positions")
@@ -82,7 +101,8 @@ class PagedKV:
     the last dimension contiguous and every slot on 16 bytes (so
     [pages, page_size, kv_heads, head_dim] pools are passed transposed);
     table [seqs, width] int32, rows contiguous: the page of each run of
-    page_size positions. head_dim: a multiple of 8, at most 256.
+    page_size positions. head_dim: a multiple of 8, at most 256; kv_heads: at
+    most 1024. Sequences may share pages as long as no call writes to them.
 
     `status` ([1] int32; a new one unless given) collects what the device
     found wrong (check())."""
@@ -218,8 +238,8 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
     _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
                                        qkv.stride(0) if n > 1 else qkv.shape[1],
                                        None if seqs is None else seqs.data_ptr(), positions.data_ptr(),
-                                       None if slots is None else slots.data_ptr(), n, int(heads), float(theta), q.data_ptr(), _DTYPES[dt],
-                                       cache._status, cache._stream()), "er_kv_append")
+                                       None if slots is None else slots.data_ptr(), n, int(heads), float(theta),
+                                       q.data_ptr(), _DTYPES[dt], cache._status, cache._stream()), "er_kv_append")
     return q
 
 
@@ -307,8 +327,8 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
     counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
     _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
                                 None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
-                                bounds._codes, bounds._scales, int(budget), int(sinks),
-                                int(recent), pages.data_ptr(), counts.data_ptr(), cache._status, cache._stream()), "er_kv_select")
+                                bounds._codes, bounds._scales, int(budget), int(sinks), int(recent),
+                                pages.data_ptr(), counts.data_ptr(), cache._status, cache._stream()), "er_kv_select")
     return pages, counts
 
 
@@ -331,8 +351,8 @@ def evict(cache: PagedKV, lens: torch.Tensor, mass: torch.Tensor, to: PagedKV, t
     _weights(mass, "mass", cache, cache.seqs, False)
     _weights(to_mass, "to_mass", cache, cache.seqs, True)
     to._writable()
-    if to_mass.data_ptr() == mass.data_ptr() and mass.numel():
-        raise ValueError("to_mass: must not be mass")
+    if _share(mass, to_mass):
+        raise ValueError("to_mass: must not share memory with mass")
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} with {sinks} first and {recent} last positions")
     kept = torch.empty((cache.seqs, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)

@@ -392,7 +392,8 @@ typedef struct er_kv_cache {
   void* k;                     /* [num_pages, kv_heads, page_size, head_dim] by the strides below */
   void* v;
   int dtype;                   /* ER_DTYPE_F32 / ER_DTYPE_BF16 */
-  int num_pages, page_size, kv_heads;
+  int num_pages, page_size;
+  int kv_heads;                /* <= 1024 */
   int head_dim;                /* a multiple of 8, <= 256 */
   long long page_stride, head_stride, slot_stride;
   const int32_t* table;        /* device [seqs, table_width], row stride table_stride */
@@ -427,12 +428,13 @@ ER_API int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype
  * (distinct; positions behind lens[r] are left out).
  * With mass, mass[r * mass_row_stride + h * mass_head_stride + j] grows by
  * key head h's attention weight on position j, summed over its queries
- * (not together with pages). */
+ * (not together with pages; NaN where the row is spoiled). The workspace is
+ * 256-byte aligned; some calls need none (0 bytes). */
 typedef struct er_kv_attend_io {
   const void* q;               /* [rows, heads, head_dim], row stride q_stride elements */
   int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */
   long long q_stride;
-  void* out;                   /* [rows, heads, head_dim] contiguous */
+  void* out;                   /* [rows, heads, head_dim] contiguous, 16-byte aligned */
   int rows, heads;
   const int32_t* seqs;         /* optional [rows] */
   const int32_t* lens;         /* [rows] */
@@ -455,7 +457,7 @@ ER_API int er_kv_attend(const er_kv_cache* cache, const er_kv_attend_io* io, voi
  * codes[(page * kv_heads + h) * 2 * head_dim + {0, head_dim} + c] =
  * rint(x / scale) with scale[page * kv_heads + h] = max |x| * (1/127), the
  * factor rounded to 32 bits (code 0 where that is no number; NaN keys are
- * passed over). */
+ * passed over). At most 65535 sequences; codes 8-byte aligned. */
 ER_API int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, const int32_t* start, int8_t* codes,
                              float* scales, int* status, void* stream);
 
@@ -465,7 +467,9 @@ ER_API int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, cons
  *   I = sum_c (c_c > 0 ? c_c * greatest_c : c_c * least_c), c_c = rint(q_c / t), t = max |q| * (1/127)
  * (I exact, the products rounded in this order; ties to the lower page, NaN
  * last). pages_out [rows, kv_heads, budget]: ordinals ascending, -1 behind
- * them; counts_out [rows, kv_heads]. lens, seqs as for er_kv_attend. */
+ * them; counts_out [rows, kv_heads]. lens, seqs as for er_kv_attend. At most
+ * 64 queries a key head and tables of about 300000 pages (a cluster's shared
+ * memory holds the scores); codes 16-byte aligned. */
 ER_API int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, long long q_stride, int rows, int heads,
                         const int32_t* seqs, const int32_t* lens, const int8_t* codes, const float* scales, int budget,
                         int sinks, int recent, int32_t* pages_out, int32_t* counts_out, int* status, void* stream);
@@ -479,7 +483,9 @@ ER_API int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype, lo
  * one that `from` reads), their mass to to_mass (same kind of strides).
  * kept_out [seqs, kv_heads, budget]: the positions, -1 behind them;
  * lens_out [seqs]. What lies behind the kept positions in `to` and to_mass
- * stays as it was. A sequence with a bad length keeps nothing. */
+ * stays as it was. A sequence with a bad length keeps nothing. mass_len at
+ * most about 370000 (a cluster's shared memory holds the weights), at most
+ * 65535 sequences; neither to_mass over mass nor lens_out over lens. */
 ER_API int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int32_t* lens, const float* mass,
                        long long mass_seq_stride, long long mass_head_stride, int mass_len, float* to_mass,
                        long long to_mass_seq_stride, long long to_mass_head_stride, int to_mass_len, int budget,

@@ -536,6 +536,10 @@ def test_refusals(cuda):
     to = kv.PagedKV(torch.zeros_like(cache.k), torch.zeros_like(cache.v), cache.table.clone())
     with pytest.raises(ValueError, match="to_mass"):
         kv.evict(cache, lens, mass, to, mass, 8, recent=2)
+    with pytest.raises(ValueError, match="share memory with mass"):
+        kv.evict(cache, lens, mass[:, :, :32], to, mass[:, :, 16:], 8, recent=2)
+    with pytest.raises(ValueError, match="out must be 16-byte"):
+        kv.attend(cache, q, lens, out=torch.zeros(q.numel() + 1, device="cuda")[1:].view(q.shape))
     with pytest.raises(ValueError, match="destination holds"):
         kv.evict(cache, lens, mass, to, torch.zeros((2, 2, 65), device="cuda"), 65, recent=2)
     unaligned = torch.zeros(cache.k.numel() + 2, device="cuda")[2:].view(cache.k.shape)

@@ -5,8 +5,9 @@ from __future__ import annotations
 import ctypes as C
 
 import pytest
+import torch
 
-from expertrelay_b200 import _lib
+from expertrelay_b200 import _lib, kv
 from expertrelay_b200.kv_cache import PageTable
 
 P = 0x1000  # an address that is never followed
@@ -48,7 +49,7 @@ def test_cache_refusals(change, words):
     ({"rows": -1}, "rows -1"), ({"heads": 3}, "heads 3 / 2"), ({"heads": 0}, "heads 0"), ({"q_dtype": 7}, "q dtype 7"),
     ({"q_stride": 255}, "row stride 255"), ({"pages": P}, "page lists"), ({"pages": P, "max_pages": 4}, "page lists"),
     ({"pages": P, "counts": P, "max_pages": 4, "mass": P}, "page lists"), ({"mass": P, "mass_len": -1}, "mass_len"),
-    ({"rows": 4}, "4 rows, 3 sequences"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lens": None}, "null"),
+    ({"rows": 4}, "4 rows, 3 sequences"), ({"out": P + 8}, "16-byte"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lens": None}, "null"),
 ])
 def test_attend_refusals(change, words):
     _fails(_lib.lib().er_kv_attend(C.byref(_cache()), C.byref(_io(**change)), None, 0, None), words)
@@ -101,6 +102,17 @@ def test_nothing_to_do_is_fine():
     assert L.er_kv_attend(C.byref(_cache()), C.byref(_io(rows=0)), None, 0, None) == _lib.ER_OK
     assert L.er_kv_append(C.byref(_cache()), P, 1, 512, None, P, None, 0, 4, 1e4, P, 1, None, None) == _lib.ER_OK
     assert L.er_kv_page_bounds(C.byref(_cache(seqs=0)), P, P, P, P, None, None) == _lib.ER_OK
+
+
+def test_weights_that_share_memory():
+    a = torch.zeros(4 * 2 * 3 * 10)
+    share = kv._share
+    two = a.view(4, 2, 3, 10)
+    assert not share(two[0], two[1]) and not share(two[3], two[0])       # one behind the other
+    assert not share(two.transpose(0, 1)[0][:, :, :4], two.transpose(0, 1)[1])  # layers of one array
+    assert share(two[0], two[0]) and share(two[0], two[0][:, :, :4]) and share(two[0][:, :, 1:], two[0])
+    assert share(a[:60].view(2, 3, 10), a[5:65].view(2, 3, 10)) and share(a[:60].view(2, 3, 10), a[40:58].view(2, 3, 3))
+    assert not share(two[0], torch.zeros(2, 3, 10)) and not share(two[:, :0, 0], two[:, :, 0])
 
 
 def test_page_table_gives_and_takes_pages():
