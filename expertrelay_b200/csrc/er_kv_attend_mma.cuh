@@ -27,8 +27,12 @@
 // (they do not round), so fp32 results add each chunk's products up there and
 // the running sum in rounded fp32.
 //
-// Measured (16 rows of 16000 positions, 8 key heads, head_dim 128, pages of
-// 16): @@MEASURED@@
+// Measured (16 rows of 16000 positions, 8 key heads, head_dim 128, pages of 16;
+// at the rate of a copy bf16 pages take 161 us, fp32 pages 322): bf16 pages and
+// queries, 4 queries a key head 165 us, 16 queries 211; fp32 queries 183 and
+// 261; fp32 pages 344 and 478. With 4 queries memory bounds it; with 16 the
+// chain of a tile's steps in a warp does, and the rescaling and exponentials of
+// twice as many columns.
 #pragma once
 
 #include <type_traits>
@@ -106,20 +110,32 @@ __device__ __forceinline__ float cut_tf32(float& x) {
 constexpr int kMergeHeads = 4;  // queries whose pieces the warps exchange at a time
 
 // A CTA's shape for a cache of TC, queries and results of TQ, head_dim padded
-// to DP, NT tiles of 8 queries. Two CTAs an SM where a warp's stage is 8 KB:
-// two stages of 8 warps are 128 KB under way on an SM, twice what latency
-// times bandwidth asks for (three stages gained nothing, and 12 warps of two
-// stages lost 40 % at head_dim 128, their registers cut to 168).
+// to DP, NT tiles of 8 queries. What bounds a warp is the chain of a tile (wait,
+// scores, maximum, exponentials, products), so what carries it are warps
+// enough, as many on each of the SM's four schedulers, and registers enough for
+// each (8 warps of 255, 12 of 168); 96 to 192 KB under way on an SM come with
+// that. Times of 16 rows, 8 key heads, 4 queries each, over 1.05 GB of keys and
+// values (rows of 512 bytes and more: 2.1 GB):
+//   bf16 rows of 128 bytes: 12 warps of 32 keys, two stages (8 warps: 194 us, 167)
+//     256 bytes: 8 warps of 16 keys, two stages (165 us; one stage of 32 keys 172);
+//       of 32 keys and one stage where the queries have parts or two tiles
+//       (16 queries a key head: 225 us with 16 keys and two stages, 211)
+//     512 bytes: 8 warps of one stage (4 of three: 350 us, 314; 7 of one: 323)
+//   fp32 rows of 256 bytes: 12 warps of one stage, 8 of two for two tiles (206 us, 193)
+//     512 bytes: 8 warps of one stage (6 of two: 404 us, 345; 10 of one, registers short: 396)
+//     1024 bytes: 5 warps of one stage, all that fits (3 of two: 723 us, 443)
 template <typename TC, typename TQ, int DP, int NT>
 struct Mma {
   static constexpr bool kBf16 = sizeof(TC) == 2;
   // parts of a query and of a weight (fp32 caches: leading bits and rest)
   static constexpr int QS = !kBf16 ? 2 : sizeof(TQ) == 2 ? 1 : 3, PS = !kBf16 ? 2 : sizeof(TQ) == 2 ? 2 : 3;
   static constexpr int kRow = DP * (int)sizeof(TC);  // bytes of a key in shared memory
-  static constexpr int kKeys = kRow == 128 ? 32 : 16;  // keys a warp takes at a time
+  static constexpr bool kParts = NT * QS > 1;
+  static constexpr int kKeys = kBf16 && (kRow == 128 || (kRow == 256 && kParts)) ? 32 : 16;  // keys a warp takes at a time
   static constexpr int kChunkBytes = kKeys * kRow;
-  static constexpr int kWarps = kRow <= 256 ? 4 : kBf16 ? 4 : kRow == 512 ? (NT == 1 ? 3 : 6) : 3;
-  static constexpr int kStages = kBf16 && kRow == 512 && NT * QS < 6 ? 3 : 2;
+  static constexpr int kWarps = kBf16 ? (kRow == 128 ? 6 : kRow == 256 ? 4 : 8)
+                                      : kRow == 256 ? (NT == 1 ? 6 : 4) : kRow == 512 ? (NT == 1 ? 4 : 8) : 5;
+  static constexpr int kStages = kBf16 ? (kRow == 128 || (kRow == 256 && !kParts) ? 2 : 1) : kRow == 256 && NT == 2 ? 2 : 1;
   static constexpr int kRing = kWarps * kStages * 2 * kChunkBytes;
   static constexpr int kKSteps = kBf16 ? DP / 16 : DP / 8;  // matrix products along the channels of the scores
   static constexpr int kQuery = kKSteps * QS * NT * 32 * 8;
@@ -147,6 +163,10 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
   using C = Mma<TC, TQ, DP, NT>;
   constexpr int S = C::kStages, KEYS = C::kKeys, KB = KEYS / 16, KS = C::kKSteps, QS = C::QS, PS = C::PS, W = C::kWarps;
   constexpr int MT = DP / 16;  // tiles of 16 channels
+  // Over 1024-byte rows the products of the last quarter stand behind a branch
+  // of their own (256 channels: 550 -> 443 us, the code then keeps to its
+  // registers; 192: 551 -> 380). Elsewhere that branch cost 1 .. 20 %.
+  constexpr int DP1 = !C::kBf16 && DP == 256 ? 192 : DP, KS1 = KS * DP1 / DP, MT1 = MT * DP1 / DP;
   constexpr bool BF = C::kBf16, EXACT = sizeof(TQ) == 4;  // EXACT: running sums in rounded fp32
   extern __shared__ __align__(128) char sm[];
   __shared__ RunScratch scratch;
@@ -269,8 +289,7 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
         for (int i = 0; i < KB * CH * NT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s2[i / (CH * NT)][i / NT % CH][i % NT][e] = 0.f;
-#pragma unroll(KS <= 16 ? KS : 8)
-        for (int ks = 0; ks < KS; ++ks) {
+        auto score = [&](int ks) {
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
             uint32_t kf[4];
@@ -300,6 +319,12 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
               }
             }
           }
+        };
+#pragma unroll(KS1 <= 16 ? KS1 : 8)
+        for (int ks = 0; ks < KS1; ++ks) score(ks);
+        if (KS1 < KS && d > DP1) {
+#pragma unroll
+          for (int ks = KS1; ks < KS; ++ks) score(ks);
         }
         // p: [kb][nt][e]: key kb 16 + lane / 4 + 8 (e / 2), query 2 (lane % 4) + e % 2
         float high[NT][2], p[KB][NT][4];
@@ -429,8 +454,7 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
                 w = w == w ? round_tf32(w - bh[half][nt][e]) : w;
               }
             }
-#pragma unroll
-          for (int k = 0; k < MT; ++k) {
+          auto weigh = [&](int k) {
             float x[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
@@ -458,6 +482,12 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[k][nt][e] += x[nt][e];
+          };
+#pragma unroll
+          for (int k = 0; k < MT1; ++k) weigh(k);
+          if (MT1 < MT && d > DP1) {
+#pragma unroll
+            for (int k = MT1; k < MT; ++k) weigh(k);
           }
         }
       }
