@@ -65,21 +65,17 @@ struct Entry {
 __device__ __forceinline__ Entry kv_entry(const AttendArgs& a, int x) {
   const int row = a.pages ? x / a.kv.kv_heads : x;
   Entry e;
-  e.seq = a.seqs ? a.seqs[row] : row;
+  e.seq = a.seqs ? a.seqs[row] : row;  // three loads, none waiting for another
   e.len = a.lens[row];
-  e.n = e.len;
+  const int c = a.pages ? a.counts[x] : 0;
+  e.n = a.pages ? (int)((uint32_t)c * a.kv.page_size) : e.len;  // of a page list, positions behind len are left out key by key
   e.bad = 0;
-  if (e.seq < 0 || e.seq >= a.kv.seqs) {
+  if (e.seq < 0 || e.seq >= a.kv.seqs)
     e.bad = ER_KV_BAD_SEQ;
-  } else if (e.len < 0 || e.len > kKvMaxLen || e.len > a.kv.capacity() || (a.scores && e.len > a.mass_len)) {
+  else if (e.len < 0 || e.len > kKvMaxLen || e.len > a.kv.capacity() || (a.scores && e.len > a.mass_len))
     e.bad = ER_KV_BAD_LENGTH;
-  } else if (a.pages) {
-    const int c = a.counts[x];
-    if (c < 0 || c > a.max_pages || (long long)c * a.kv.page_size > kKvMaxLen)
-      e.bad = ER_KV_BAD_LENGTH;
-    else
-      e.n = c * a.kv.page_size;  // positions behind len are left out key by key
-  }
+  else if (a.pages && (c < 0 || c > a.max_pages || (long long)c * a.kv.page_size > kKvMaxLen))
+    e.bad = ER_KV_BAD_LENGTH;
   if (e.bad) e.n = 0;
   return e;
 }
@@ -155,7 +151,7 @@ __device__ __forceinline__ Run kv_run(const AttendArgs& a, RunScratch& s) {
   const int x0 = min(a.entries, (int)threadIdx.x * per), x1 = min(a.entries, x0 + per);
   long long cost = 0, tiles = 0;
   Entry e = {};
-#pragma unroll 1
+#pragma unroll 2
   for (int x = x0; x < x1; ++x) {
     e = kv_entry(a, x);
     const int c = kv_tiles(a, e.n);

@@ -234,7 +234,7 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
     dt = qkv.dtype if q_dtype is None else q_dtype
     if dt not in _DTYPES:
         raise ValueError(f"q_dtype: float32 or bfloat16, got {dt}")
-    q = torch.empty((n, heads, cache.head_dim), dtype=dt, device=cache.device)
+    q = qkv.new_empty((n, heads, cache.head_dim), dtype=dt)
     _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
                                        qkv.stride(0) if n > 1 else qkv.shape[1],
                                        None if seqs is None else seqs.data_ptr(), positions.data_ptr(),
@@ -323,8 +323,7 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} with {sinks} first and {recent} last pages")
     lib = _lib.lib()
-    pages = torch.empty((rows, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
-    counts = torch.empty((rows, cache.kv_heads), dtype=torch.int32, device=cache.device)
+    pages, counts = lens.new_empty((rows, cache.kv_heads, budget)), lens.new_empty((rows, cache.kv_heads))
     _lib.check(lib.er_kv_select(cache._ref, q.data_ptr(), _DTYPES[q.dtype], stride, rows, heads,
                                 None if seqs is None else seqs.data_ptr(), lens.data_ptr(),
                                 bounds._codes, bounds._scales, int(budget), int(sinks), int(recent),
@@ -355,8 +354,7 @@ def evict(cache: PagedKV, lens: torch.Tensor, mass: torch.Tensor, to: PagedKV, t
         raise ValueError("to_mass: must not share memory with mass")
     if budget <= 0 or sinks < 0 or recent < 0 or sinks + recent > budget:
         raise ValueError(f"budget {budget} with {sinks} first and {recent} last positions")
-    kept = torch.empty((cache.seqs, cache.kv_heads, budget), dtype=torch.int32, device=cache.device)
-    new = torch.empty(cache.seqs, dtype=torch.int32, device=cache.device)
+    kept, new = lens.new_empty((cache.seqs, cache.kv_heads, budget)), lens.new_empty(cache.seqs)
     _lib.check(_lib.lib().er_kv_evict(cache._ref, to._ref, lens.data_ptr(), mass.data_ptr(), mass.stride(0),
                                       mass.stride(1), mass.shape[2], to_mass.data_ptr(), to_mass.stride(0),
                                       to_mass.stride(1), to_mass.shape[2], int(budget), int(sinks), int(recent),
