@@ -6,6 +6,8 @@
 // token's page. The angle position * theta^(-2j/d) and its sine and cosine
 // are taken in 64 bits and rounded once: in 32 bits the product alone loses
 // 2^-24 of the angle, 0.004 rad at position 65536 of the fastest channel.
+#include <type_traits>
+
 #include "er_kv.cuh"
 
 namespace er {
@@ -21,38 +23,39 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// VEC values (16-byte loads where VEC is 8), and as fp32.
+// VEC values, 16 bytes of them or a single one, and as fp32.
 template <int VEC, typename T>
 struct Vec {
-  static constexpr int N = VEC == 1 ? 1 : VEC * (int)sizeof(T) / 16;
-  uint4 raw[N];
+  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "one load");
+  uint4 raw;
 
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (VEC == 1) {
-      *reinterpret_cast<T*>(raw) = *p;
+      *reinterpret_cast<T*>(&raw) = *p;
     } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) raw[i] = ld_stream_u4(p + i * (16 / sizeof(T)));
+      raw = ld_stream_u4(p);
     }
   }
   __device__ __forceinline__ void get(float (&x)[VEC]) const {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) x[e] = to_f32(reinterpret_cast<const T*>(raw)[e]);
+    for (int e = 0; e < VEC; ++e) x[e] = to_f32(reinterpret_cast<const T*>(&raw)[e]);
   }
 };
+// VEC values to memory, 16 bytes a store (8 where fewer bytes are all).
 template <int VEC, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
   if constexpr (VEC == 1) {
     *p = from_f32<T>(x[0]);
   } else {
-    constexpr int N = 16 / sizeof(T);
+    using S = std::conditional_t<VEC * sizeof(T) == 8, uint2, uint4>;
+    constexpr int N = sizeof(S) / sizeof(T);
 #pragma unroll
     for (int i = 0; i < VEC; i += N) {
-      uint4 raw;
+      S raw;
       T* v = reinterpret_cast<T*>(&raw);
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] = from_f32<T>(x[i + e]);
-      *reinterpret_cast<uint4*>(p + i) = raw;
+      *reinterpret_cast<S*>(p + i) = raw;
     }
   }
 }
@@ -62,17 +65,20 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[VEC]) {
 // rotation are rounded one by one (no fused multiply-add), so a key's bits do
 // not depend on which half of the pair it is, and the pages' codes follow
 // from the formula alone. Memory-bound, if enough is in flight: every thread
-// has its values of all TOK tokens under way before the angles' sines (64
-// bits) are computed, by TOK d/2 threads at once. One token a CTA while that
-// leaves SMs without work (a decode step), 4 for prompts (16384 tokens of
-// 16 + 16 + 16 heads: 98 us with one).
+// has its values of all TOK tokens under way, 16 bytes a load, before the
+// angles' sines (64 bits) are computed, by TOK d/2 threads at once. One token a
+// CTA while that leaves SMs without work (a decode step), 4 for prompts
+// (16384 tokens of 16 + 16 + 16 heads of 128, bf16: 98 us with one, 70). Up to
+// 448 threads, so that two CTAs of 72 registers a thread share an SM, in rounds
+// of equal size (6745 tokens of 64 + 8 + 8 heads of 96, fp32: 81 us with up to
+// 512 threads, 69, where a copy takes 64; loads of 32 bytes a thread: 105).
+constexpr int kAppendThreads = 448;
+
 template <typename TX, typename TQ, typename TC, int VEC, int TOK>
-__global__ void __launch_bounds__(512) kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld,
-                                                        const int32_t* __restrict__ seqs,
-                                                        const int32_t* __restrict__ positions,
-                                                        const int32_t* __restrict__ slots, int n, int heads,
-                                                        const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out,
-                                                        int* status) {
+__global__ void __launch_bounds__(kAppendThreads, 2)
+    kv_append_kernel(KvView kv, const TX* __restrict__ qkv, long long ld, const int32_t* __restrict__ seqs,
+                     const int32_t* __restrict__ positions, const int32_t* __restrict__ slots, int n, int heads,
+                     const __grid_constant__ InvFreq inv, TQ* __restrict__ q_out, int* status) {
   __shared__ __align__(16) float cs[TOK][256];  // [d/2] cos, then [d/2] sin
   __shared__ long long slot[TOK];               // byte offset of the token's slot in the pools, -1: not written
   kv_enter();
@@ -296,14 +302,15 @@ const InvFreq& inv_freq(double theta, int d) {
 template <typename TX, typename TQ, typename TC>
 int append_go(const KvView& kv, const void* qkv, long long ld, const int32_t* seqs, const int32_t* positions,
               const int32_t* slots, int n, int heads, double theta, void* q_out, int* status, cudaStream_t st) {
-  // 16-byte accesses need half a head in whole VECs and aligned rows
+  // wide accesses need half a head in whole VECs and aligned rows
+  constexpr int V = 16 / sizeof(TX);
   const bool vec = kv.d % 16 == 0 && !(((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)(ld * sizeof(TX))) & 15);
-  const int tasks = (heads + 2 * kv.kv_heads) * (kv.d / 2) / (vec ? 8 : 1);  // of a token
-  const int threads = tasks >= 512 ? 512 : (tasks + 31) / 32 * 32;
+  const int tasks = (heads + 2 * kv.kv_heads) * (kv.d / 2) / (vec ? V : 1);  // of a token
+  const int rounds = (tasks + kAppendThreads - 1) / kAppendThreads, threads = (tasks + 32 * rounds - 1) / (32 * rounds) * 32;
   const bool many = vec && n >= 148 * 8;
   return launch_chained(!vec   ? kv_append_kernel<TX, TQ, TC, 1, 1>
-                        : many ? kv_append_kernel<TX, TQ, TC, 8, 4>
-                               : kv_append_kernel<TX, TQ, TC, 8, 1>,
+                        : many ? kv_append_kernel<TX, TQ, TC, V, 4>
+                               : kv_append_kernel<TX, TQ, TC, V, 1>,
                         dim3(many ? (n + 3) / 4 : n), dim3(threads), 0, st, "kv_append_kernel", kv, (const TX*)qkv, ld,
                         seqs, positions, slots, n, heads, inv_freq(theta, kv.d), (TQ*)q_out, status);
 }

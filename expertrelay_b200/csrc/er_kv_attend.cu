@@ -96,7 +96,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
   if (a.scores && threadIdx.x == 0) a.lse[at] = sum == 0.f ? INFINITY : top + log2f(sum);
 }
 
-// mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position.
+// mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position. The scores
+// have just been written and lie in L2; what bounds it is latency (7 us beside
+// the 61 of the rest at 8 rows of up to 16000 positions, 8 key heads of 4
+// queries; four positions of a thread under way at once, or more CTAs, changed
+// nothing). A score a load cost 12 us more with 16 queries (54 rows of up to
+// 6689 positions, 2 key heads: 90 us, 78).
 __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ AttendArgs a) {
   kv_enter();
   const int unit = blockIdx.y, row = unit / a.kv.kv_heads, h = unit % a.kv.kv_heads;
@@ -106,7 +111,16 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
   const float* lse = a.lse + (long long)row * a.heads + h * a.group;
   for (long long j = blockIdx.x * 256 + threadIdx.x; j < e.n; j += gridDim.x * 256) {  // a step may pass 2^31
     float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) sum += exp2f(s[j * a.group + g] - lse[g]);
+    if (a.group % 4 == 0) {
+#pragma unroll 4
+      for (int g = 0; g < a.group; g += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(s + j * a.group + g);
+        sum += exp2f(x.x - lse[g]) + exp2f(x.y - lse[g + 1]) + exp2f(x.z - lse[g + 2]) + exp2f(x.w - lse[g + 3]);
+      }
+    } else {
+#pragma unroll 4
+      for (int g = 0; g < a.group; ++g) sum += exp2f(s[j * a.group + g] - lse[g]);
+    }
     to[j] += sum;
   }
 }
