@@ -212,7 +212,10 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
   for (;;) {
     const bool work = filled == S;
     StageInfo now = {};
-    if (work) now = info[warp][st];
+    if (work) {
+      if (S == 1) __syncwarp();  // lane 0 has just written it; of more stages, before the last tile's __syncwarp
+      now = info[warp][st];
+    }
     // a new unit: its queries in the matrix instructions' order (the first
     // unit's before the ring is filled, while its pages are looked up)
     if (fresh && (work || filled == 0)) {
@@ -525,6 +528,7 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
     st = st + 1 == S ? 0 : st + 1;
     if (!work) {
       ++filled;
+      __syncwarp();
       continue;
     }
     --left;
