@@ -7,6 +7,8 @@
 
 namespace er {
 
+constexpr int kMaxHeads = 65536;  // of queries: their products with head_dim stay ints
+
 // er_kv_cache with strides in bytes (the pools' element type is a template
 // parameter of the kernels that touch values).
 struct KvView {

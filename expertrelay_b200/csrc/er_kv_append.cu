@@ -324,7 +324,7 @@ extern "C" int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_d
                             const int32_t* seqs, const int32_t* positions, const int32_t* slots, int n, int heads,
                             double theta, void* q_out, int q_dtype, int* status, void* stream) {
   if (int rc = kv_check("er_kv_append", cache)) return rc;
-  if (n < 0 || heads <= 0 || !(theta > 0))
+  if (n < 0 || heads <= 0 || heads > kMaxHeads || !(theta > 0))
     return fail(ER_EINVAL, "er_kv_append: n %d, heads %d, theta %g", n, heads, theta);
   if ((qkv_dtype != ER_DTYPE_F32 && qkv_dtype != ER_DTYPE_BF16) || (q_dtype != ER_DTYPE_F32 && q_dtype != ER_DTYPE_BF16))
     return fail(ER_EINVAL, "er_kv_append: dtypes %d, %d", qkv_dtype, q_dtype);

@@ -182,7 +182,7 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
 int attend_check(const er_kv_cache* c, const er_kv_attend_io* io) {
   if (int rc = kv_check("er_kv_attend", c)) return rc;
   if (!io) return fail(ER_EINVAL, "er_kv_attend: null io");
-  if (io->rows < 0 || io->heads <= 0 || io->heads % c->kv_heads)
+  if (io->rows < 0 || io->heads <= 0 || io->heads > kMaxHeads || io->heads % c->kv_heads)
     return fail(ER_EINVAL, "er_kv_attend: rows %d, heads %d / %d", io->rows, io->heads, c->kv_heads);
   if (io->q_dtype != ER_DTYPE_F32 && io->q_dtype != ER_DTYPE_BF16)
     return fail(ER_EINVAL, "er_kv_attend: q dtype %d", io->q_dtype);

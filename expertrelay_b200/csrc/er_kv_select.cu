@@ -387,7 +387,7 @@ extern "C" int er_kv_select(const er_kv_cache* cache, const void* q, int q_dtype
                             const float* scales, int budget, int sinks, int recent, int32_t* pages_out,
                             int32_t* counts_out, int* status, void* stream) {
   if (int rc = kv_check("er_kv_select", cache)) return rc;
-  if (rows < 0 || heads <= 0 || heads % cache->kv_heads)
+  if (rows < 0 || heads <= 0 || heads > kMaxHeads || heads % cache->kv_heads)
     return fail(ER_EINVAL, "er_kv_select: rows %d, heads %d / %d", rows, heads, cache->kv_heads);
   if (q_dtype != ER_DTYPE_F32 && q_dtype != ER_DTYPE_BF16) return fail(ER_EINVAL, "er_kv_select: q dtype %d", q_dtype);
   if (budget <= 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)

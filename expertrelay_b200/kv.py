@@ -257,7 +257,9 @@ def attend(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, *, seqs: torch.T
     mass [rows, kv_heads, n] float32 (the last dimension contiguous): grows
     by each position's attention weight, summed over its key head's queries.
     pages [rows, kv_heads, m], counts [rows, kv_heads] int32 (select_pages):
-    only those pages are read."""
+    only those pages are read, each of them listed once. workspace: scratch of
+    one's own instead of a new one (ValueError names the bytes needed); it
+    serves one call at a time, captured ones included."""
     rows, heads, stride = _queries(cache, q)
     _row_args(cache, rows, lens, seqs)
     if out is None:

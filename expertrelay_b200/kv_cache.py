@@ -201,11 +201,18 @@ class PagedKVCache:
         to_table = self._ints(np.asarray(pages).reshape(len(long), each))
         at = torch.tensor(long, device=self.device)
         table, lens = self.table[at], self._ints(self.pages.length[long])
-        for layer in range(len(self.layers)):
-            old = kv.PagedKV(self.k[layer], self.v[layer], table, self.status)
-            new = kv.PagedKV(self.k[layer], self.v[layer], to_table, self.status)
-            mass = torch.zeros((len(long), *self.mass.shape[2:]), device=self.device)
-            kv.evict(old, lens, self.mass[layer][at], new, mass, budget, sinks=sinks, recent=recent)
+        masses = []
+        try:
+            for layer in range(len(self.layers)):
+                old = kv.PagedKV(self.k[layer], self.v[layer], table, self.status)
+                new = kv.PagedKV(self.k[layer], self.v[layer], to_table, self.status)
+                mass = torch.zeros((len(long), *self.mass.shape[2:]), device=self.device)
+                kv.evict(old, lens, self.mass[layer][at], new, mass, budget, sinks=sinks, recent=recent)
+                masses.append(mass)
+        except Exception:  # nothing has changed but pages that nothing names
+            self.pages.free += pages
+            raise
+        for layer, mass in enumerate(masses):
             self.mass[layer][at] = mass
         for i, s in enumerate(long):
             self.pages.replace(s, pages[i * each:(i + 1) * each], budget)

@@ -411,7 +411,7 @@ typedef struct er_kv_cache {
  * place slots[i] of it in the cache (slots NULL: positions[i]; the two differ
  * once positions were evicted). Its q heads are rotated into q_out
  * [n, heads, head_dim] (q_dtype, not over qkv), its k heads rotated into the
- * page, its v heads copied there. Angles are position * theta^(-2j/head_dim)
+ * page, its v heads copied there. At most 65536 query heads. Angles are position * theta^(-2j/head_dim)
  * in 64 bits, rotate-half. A (sequence, place) pair may occur once per call. */
 ER_API int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype, long long ld, const int32_t* seqs,
                         const int32_t* positions, const int32_t* slots, int n, int heads, double theta, void* q_out,
@@ -435,7 +435,7 @@ typedef struct er_kv_attend_io {
   int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */
   long long q_stride;
   void* out;                   /* [rows, heads, head_dim] contiguous, 16-byte aligned */
-  int rows, heads;
+  int rows, heads;             /* heads <= 65536 */
   const int32_t* seqs;         /* optional [rows] */
   const int32_t* lens;         /* [rows] */
   float scale;

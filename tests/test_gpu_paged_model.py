@@ -5,6 +5,8 @@ everything in as the full cache, and what a generation does under both."""
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -12,6 +14,7 @@ from conftest import golden
 from golden.make_golden import MODEL_CASES, MODEL_NEW, MODEL_PROMPT
 
 from expertrelay_b200 import _lib, synth
+from expertrelay_b200.kv_cache import PagedKVCache
 from expertrelay_b200.model import QwenMoeModel
 from oracle.moe_oracle import rel_l2
 
@@ -130,3 +133,13 @@ def test_paged_refusals(cuda):
     with pytest.raises(ValueError, match="select"):
         model.new_paged_cache(1, 8, select=(1, 1, 1))
     model.close()
+
+
+def test_an_eviction_that_is_refused_changes_nothing(cuda):
+    shape = SimpleNamespace(num_layers=1, num_kv_heads=1, head_dim=8)
+    cache = PagedKVCache(shape, 1, 400000, page_size=100, pages=8, mass=True, device=cuda)  # more weights than are ranked
+    cache.step([0] * 300)
+    before = (cache.pages.table.copy(), sorted(cache.pages.free))
+    with pytest.raises(ValueError, match="400000 weights"):
+        cache.evict(200, recent=10)
+    assert cache.length() == 300 and sorted(cache.pages.free) == before[1] and (cache.pages.table == before[0]).all()

@@ -46,7 +46,8 @@ def test_cache_refusals(change, words):
 
 
 @pytest.mark.parametrize(("change", "words"), [
-    ({"rows": -1}, "rows -1"), ({"heads": 3}, "heads 3 / 2"), ({"heads": 0}, "heads 0"), ({"q_dtype": 7}, "q dtype 7"),
+    ({"rows": -1}, "rows -1"), ({"heads": 3}, "heads 3 / 2"), ({"heads": 0}, "heads 0"),
+    ({"heads": 2**31 - 2, "q_stride": 2**40}, "heads 2147483646"), ({"q_dtype": 7}, "q dtype 7"),
     ({"q_stride": 255}, "row stride 255"), ({"pages": P}, "page lists"), ({"pages": P, "max_pages": 4}, "page lists"),
     ({"pages": P, "counts": P, "max_pages": 4, "mass": P}, "page lists"), ({"mass": P, "mass_len": -1}, "mass_len"),
     ({"rows": 4}, "4 rows, 3 sequences"), ({"out": P + 8}, "16-byte"), ({"q": None}, "null"), ({"out": None}, "null"), ({"lens": None}, "null"),
@@ -59,7 +60,7 @@ def test_append_refusals():
     L, c = _lib.lib(), _cache()
     args = [C.byref(c), P, 1, 8 * 64, None, P, None, 1, 4, 1e4, P, 1, None, None]
     for at, value, words in [(1, None, "null"), (2, 5, "dtypes 5"), (3, 8 * 64 - 1, "row stride"), (5, None, "null"),
-                             (7, -1, "n -1"), (8, 0, "heads 0"), (9, 0.0, "theta 0"), (9, float("nan"), "theta"),
+                             (7, -1, "n -1"), (8, 0, "heads 0"), (8, 2**31 - 1, "heads"), (9, 0.0, "theta 0"), (9, float("nan"), "theta"),
                              (10, None, "null"), (11, 9, "9")]:
         _fails(L.er_kv_append(*[value if i == at else x for i, x in enumerate(args)]), words)
 
