@@ -651,3 +651,70 @@ def test_a_run_of_them_together(cuda, dtype):
     sel, counts = kv.select_pages(cache2, bounds, q2, new + 1, 6)
     _check_attend(cache2, q2, (new + 1).tolist(), kv.attend(cache2, q2, new + 1, pages=sel, counts=counts))
     cache.check(), cache2.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), [(F32, F32), (BF16, F32), (BF16, BF16), (F32, BF16)])
+@pytest.mark.parametrize(("heads", "kv_heads", "d", "ps"), [(4, 2, 64, 16), (40, 8, 96, 24), (3, 1, 24, 8)])
+def test_append_of_a_prompt_is_that_of_its_parts(cuda, cache_dtype, q_dtype, heads, kv_heads, d, ps):
+    """Long calls take several tokens a block, and heads in rounds: bit for bit what short calls leave."""
+    gen = torch.Generator().manual_seed(heads)
+    n, width = 1187, -(-1200 // ps)  # no multiple of the tokens a block takes
+    shape = (width + 1, kv_heads, ps, d)
+    table = torch.randperm(width + 1, generator=gen)[:width].to(torch.int32)[None].cuda()
+    qkv = torch.randn((n, (heads + 2 * kv_heads) * d), generator=gen).to(q_dtype).cuda()
+    pos = torch.randperm(1200, generator=gen)[:n].to(torch.int32).cuda()
+    pos[7], pos[n - 1] = width * ps, -1  # outside the table: left out, the tokens beside them written
+    got = []
+    for cuts in ([0, n], [0, 400, 800, n]):
+        k, v = (torch.full(shape, 9.0, dtype=cache_dtype, device="cuda") for _ in range(2))
+        cache = kv.PagedKV(k, v, table)
+        q = [kv.append(cache, qkv[a:b], pos[a:b], heads, 1e4, seqs=_i32([0] * (b - a))) for a, b in zip(cuts, cuts[1:])]
+        got.append((torch.cat(q), k, v))
+        with pytest.raises(ValueError, match="a length, position"):
+            cache.check()
+    for one, parts in zip(*got):
+        assert torch.equal(one, parts)
+    assert int((got[0][2] != 9).any(-1).sum()) == (n - 2) * kv_heads
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize(("d", "ps"), [(32, 24), (64, 16), (128, 7), (192, 64), (256, 8)])
+def test_attend_wide_groups_over_many_tiles(cuda, cache_dtype, q_dtype, d, ps):
+    """Two tiles of queries, units that end within a block's run and units that several blocks share."""
+    lens = [3000, 1, 700, 0, 2049]
+    cache, q = _case(d, lens, 2, 11, d, ps, cache_dtype, q_dtype)
+    out = kv.attend(cache, q, _i32(lens))
+    _check_attend(cache, q, lens, out)
+    wide = torch.full((5, 40000), -1, dtype=torch.int32, device="cuda")  # a longest row that rules clusters out
+    wide[:, :cache.width] = cache.table
+    _check_attend(cache, q, lens, kv.attend(kv.PagedKV(cache.k, cache.v, wide), q, _i32(lens)))
+    cache.check()
+
+
+def test_calls_of_one_cache_on_two_streams(cuda):
+    """Nothing is shared by two calls under way at once, captured or not."""
+    lens = [5000, 333, 40, 2100]
+    cache, q = _case(8, lens, 2, 4, 128, 16, BF16, BF16)
+    ns, bounds = _i32(lens), kv.PageBounds.new(cache)
+    kv.page_bounds(cache, bounds, ns, _i32([0] * 4))
+    want = kv.attend(cache, q, ns)
+    want_pages, _ = kv.select_pages(cache, bounds, q, ns, 9)
+    streams, outs, graphs = [torch.cuda.Stream() for _ in range(2)], [], []
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append((kv.attend(cache, q, ns), kv.select_pages(cache, bounds, q, ns, 9)[0]))
+    torch.cuda.synchronize()
+    for _ in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(5):
+                outs.append((kv.attend(cache, q, ns), kv.select_pages(cache, bounds, q, ns, 9)[0]))
+        graphs.append(g)
+    for s, g in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    for out, pages in outs:
+        assert torch.equal(out, want) and torch.equal(pages, want_pages)
