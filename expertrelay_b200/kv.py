@@ -41,6 +41,9 @@ _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
 def _need(t, name: str, dtype, device: torch.device, shape=None, contiguous: bool = True) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and \
+            (shape is None or t.shape == shape) and (not contiguous or t.is_contiguous()):
+        return
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device:
         got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
         raise ValueError(f"{name}: expected a {dtype} tensor on {device}, got {got}")
@@ -87,7 +90,7 @@ def _on_device(call):
 
     @functools.wraps(call)
     def on_device(cache, *args, **kwargs):
-        if torch.cuda.current_device() == cache._index:
+        if torch._C._cuda_getDevice() == cache._index:
             return call(cache, *args, **kwargs)
         with torch.cuda.device(cache._index):
             return call(cache, *args, **kwargs)
@@ -181,15 +184,17 @@ class PageBounds:
 
 def _queries(cache: PagedKV, q: torch.Tensor):
     """(rows, heads, row stride) of q [rows, heads, head_dim]."""
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.dtype not in _DTYPES or q.device != cache.device:
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or q.dtype not in _DTYPES or q.device != cache.device:
         raise ValueError(f"q: expected [rows, heads, {cache.head_dim}] float32 or bfloat16 on {cache.device}, "
-                         f"got {tuple(q.shape)} {q.dtype} on {q.device}")
-    rows, heads, d = q.shape
+                         f"got {tuple(shape)} {q.dtype} on {q.device}")
+    rows, heads, d = shape
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"q: {heads} heads over {cache.kv_heads} key heads")
-    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != d) or (rows > 1 and q.stride(0) < heads * d):
-        raise ValueError(f"q: strides {q.stride()} (heads contiguous, rows apart)")
-    return rows, heads, q.stride(0) if rows > 1 else heads * d
+    by = q.stride()
+    if by[2] != 1 or (heads > 1 and by[1] != d) or (rows > 1 and by[0] < heads * d):
+        raise ValueError(f"q: strides {by} (heads contiguous, rows apart)")
+    return rows, heads, by[0] if rows > 1 else heads * d
 
 
 def _row_args(cache: PagedKV, rows: int, lens: torch.Tensor, seqs: torch.Tensor | None, name: str = "lens") -> None:
@@ -222,10 +227,11 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
     Returns the queries, rotated, [n, heads, head_dim] in q_dtype (default:
     qkv's); k (rotated) and v go to the pages. A (sequence, place) pair may
     occur once in a call."""
-    if qkv.dim() != 2 or qkv.dtype not in _DTYPES or qkv.device != cache.device or \
-            qkv.shape[1] != (heads + 2 * cache.kv_heads) * cache.head_dim or qkv.stride(1) != 1:
-        raise ValueError(f"qkv: expected [n, {(heads + 2 * cache.kv_heads) * cache.head_dim}] float32 or bfloat16 on "
-                         f"{cache.device}, got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
+    row = (heads + 2 * cache.kv_heads) * cache.head_dim
+    if len(qkv.shape) != 2 or qkv.dtype not in _DTYPES or qkv.device != cache.device or qkv.shape[1] != row or \
+            qkv.stride(1) != 1:
+        raise ValueError(f"qkv: expected [n, {row}] float32 or bfloat16 on {cache.device}, "
+                         f"got {tuple(qkv.shape)} {qkv.dtype} on {qkv.device}")
     n = qkv.shape[0]
     _row_args(cache, n, positions, seqs, "positions")
     if slots is not None:
@@ -236,7 +242,7 @@ def append(cache: PagedKV, qkv: torch.Tensor, positions: torch.Tensor, heads: in
         raise ValueError(f"q_dtype: float32 or bfloat16, got {dt}")
     q = qkv.new_empty((n, heads, cache.head_dim), dtype=dt)
     _lib.check(_lib.lib().er_kv_append(cache._ref, qkv.data_ptr(), _DTYPES[qkv.dtype],
-                                       qkv.stride(0) if n > 1 else qkv.shape[1],
+                                       qkv.stride(0) if n > 1 else row,
                                        None if seqs is None else seqs.data_ptr(), positions.data_ptr(),
                                        None if slots is None else slots.data_ptr(), n, int(heads), float(theta),
                                        q.data_ptr(), _DTYPES[dt], cache._status, cache._stream()), "er_kv_append")
