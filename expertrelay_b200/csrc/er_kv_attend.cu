@@ -151,18 +151,20 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
     const long long most = (256ll << 20) / (4ll * io.heads * (io.mass_len > 0 ? io.mass_len : 1));
     if (L.rows > most) L.rows = most < 1 ? 1 : (int)most;
   }
-  // A cluster per unit or equal shares of all tiles. Against the shares the
-  // clusters save about 7 tiles' time (no division of the line, no join), but
-  // a unit has 8 CTAs at most: taken while its longest row costs those CTAs
-  // less than 7 tiles more than a share would be, and all clusters run at
-  // once. That takes two CTAs an SM: with one, 16 clusters of 8 did not all
-  // find room in the processor clusters of 148 SMs, and 16 units of 640
-  // fp32 keys took 20 us, a wave after the other (14 by shares).
-  const long long units = (long long)L.rows * c.kv_heads * L.blocks, tile = L.shape.tile, ctas = L.grid;
-  const long long longest =
-      ((io.pages ? (long long)io.max_pages : (long long)c.table_width) * c.page_size + tile - 1) / tile;
+  // A cluster per unit or equal shares of all tiles. The clusters save the
+  // division of the line and the join, 4 to 5 us, but a unit has 8 CTAs at most:
+  // taken while its longest row gives each of those at most 120 KB of keys and
+  // values more than a share would be (they take in 25 GB/s each), and all
+  // clusters run at once. (One row of 2000 positions, by clusters and by shares:
+  // 8 key heads of 64, bf16 8.5 and 11.7 us; of 128 10.3 and 11.5; 16 of 128, fp32
+  // 18.5 and 16.3. Of 5000: 11.9 and 12.6; 18.1 and 13.3; 35.9 and 28.1.) It
+  // takes two CTAs an SM: with one, 16 clusters of 8 did not all find room in the
+  // processor clusters of 148 SMs, and went in two waves.
+  const long long units = (long long)L.rows * c.kv_heads * L.blocks, ctas = L.grid, most = kKvMaxLen;
+  const long long room = (io.pages ? (long long)io.max_pages : (long long)c.table_width) * c.page_size;
+  const long long bytes = (room < most ? room : most) * 2 * c.head_dim * (c.dtype == ER_DTYPE_BF16 ? 2 : 4);
   L.cluster = L.rows == io.rows && L.shape.per_sm >= 2 && units * kClusterCtas <= ctas &&
-              longest * (ctas - units * kClusterCtas) <= 7LL * kClusterCtas * ctas;
+              bytes / kClusterCtas * (ctas - units * kClusterCtas) <= (120ll << 10) * ctas;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
