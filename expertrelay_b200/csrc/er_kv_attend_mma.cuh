@@ -16,21 +16,24 @@
 // and the scores' accumulator turns into P^T by 8x8 transposes (movmatrix).
 //
 // Numbers. bf16 caches (m16n8k16, V by ldmatrix.trans): bf16 has 8 bits, fp32
-// 24; fp32 queries enter as the exact sum of three bf16 parts, the weights as
-// two parts (16 bits, under a quarter of the rounding of a bf16 result) for
-// bf16 results and as three for fp32 ones. Parts are cut, not rounded, so
-// that they share the sign of the whole and an infinite key or value stays
-// infinite. fp32 caches (m16n8k8, tf32 with 11 bits): every operand is its
-// leading 11 bits and the rest (11 more), and of the products all but rest
-// times rest (2^-22 of the whole) are taken; where a key or value that is seen is
-// infinite, the result is infinite or NaN. The tensor cores cut their sums
-// (they do not round), so fp32 results add each chunk's products up there and
-// the running sum in rounded fp32.
+// 24; fp32 queries enter as the exact sum of three bf16 parts, and so do the
+// weights. Parts are cut, not rounded, so that they share the sign of the whole
+// and an infinite key or value stays infinite. fp32 caches (m16n8k8, tf32 with
+// 11 bits): every operand is its leading 11 bits and the rest (11 more), and of
+// the products all but rest times rest (2^-21 of the whole at the most, of
+// either sign) are taken: with that product too, 344 us became 363 and 482
+// became 540 below. Where a key or value that is seen is infinite, the result is
+// infinite or NaN. The tensor cores cut their sums (they do not round), so a
+// chunk's products are added up there and the running sum over the chunks in
+// rounded fp32, whatever the result's type. (With weights of two parts and the
+// sums left in the tensor cores, bf16 results took 166 us in place of 170 below
+// and were 3 to 4.5 10^-6 off before their rounding, now 1 to 5 10^-7: of 400000
+// outputs 0.35 % were rounded to the wrong side, 0.02 % are.)
 //
 // Measured (16 rows of 16000 positions, 8 key heads, head_dim 128, pages of 16;
 // at the rate of a copy bf16 pages take 161 us, fp32 pages 322): bf16 pages and
-// queries, 4 queries a key head 165 us, 16 queries 211; fp32 queries 183 and
-// 261; fp32 pages 344 and 478. With 4 queries memory bounds it; with 16 the
+// queries, 4 queries a key head 170 us, 16 queries 236; fp32 queries 183 and
+// 262; fp32 pages 344 and 482. With 4 queries memory bounds it; with 16 the
 // chain of a tile's steps in a warp does, and the rescaling and exponentials of
 // twice as many columns.
 #pragma once
@@ -117,10 +120,12 @@ constexpr int kMergeHeads = 4;  // queries whose pieces the warps exchange at a 
 // that. Times of 16 rows, 8 key heads, 4 queries each, over 1.05 GB of keys and
 // values (rows of 512 bytes and more: 2.1 GB):
 //   bf16 rows of 128 bytes: 12 warps of 32 keys, two stages (8 warps: 194 us, 167)
-//     256 bytes: 8 warps of 16 keys, two stages (165 us; one stage of 32 keys 172);
+//     256 bytes: 8 warps of 16 keys, two stages (170 us; one stage of 32 keys 176);
 //       of 32 keys and one stage where the queries have parts or two tiles
 //       (16 queries a key head: 225 us with 16 keys and two stages, 211)
 //     512 bytes: 8 warps of one stage (4 of three: 350 us, 314; 7 of one: 323)
+//   (pairs with 167, 211 and 314 are of weights in two parts; in three, the ones
+//   taken are at 179, 236 and 321)
 //   fp32 rows of 256 bytes: 12 warps of one stage, 8 of two for two tiles (206 us, 193)
 //     512 bytes: 8 warps of one stage (6 of two: 404 us, 345; 10 of one, registers short: 396)
 //     1024 bytes: 5 warps of one stage, all that fits (3 of two: 723 us, 443)
@@ -128,7 +133,7 @@ template <typename TC, typename TQ, int DP, int NT>
 struct Mma {
   static constexpr bool kBf16 = sizeof(TC) == 2;
   // parts of a query and of a weight (fp32 caches: leading bits and rest)
-  static constexpr int QS = !kBf16 ? 2 : sizeof(TQ) == 2 ? 1 : 3, PS = !kBf16 ? 2 : sizeof(TQ) == 2 ? 2 : 3;
+  static constexpr int QS = !kBf16 ? 2 : sizeof(TQ) == 2 ? 1 : 3, PS = kBf16 ? 3 : 2;
   static constexpr int kRow = DP * (int)sizeof(TC);  // bytes of a key in shared memory
   static constexpr bool kParts = NT * QS > 1;
   static constexpr int kKeys = kBf16 && (kRow == 128 || (kRow == 256 && kParts)) ? 32 : 16;  // keys a warp takes at a time
@@ -167,7 +172,7 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
   // of their own (256 channels: 550 -> 443 us, the code then keeps to its
   // registers; 192: 551 -> 380). Elsewhere that branch cost 1 .. 20 %.
   constexpr int DP1 = !C::kBf16 && DP == 256 ? 192 : DP, KS1 = KS * DP1 / DP, MT1 = MT * DP1 / DP;
-  constexpr bool BF = C::kBf16, EXACT = sizeof(TQ) == 4;  // EXACT: running sums in rounded fp32
+  constexpr bool BF = C::kBf16;
   extern __shared__ __align__(128) char sm[];
   __shared__ RunScratch scratch;
   __shared__ int spoiled;
@@ -418,10 +423,8 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
 #pragma unroll
           for (int k = 0; k < MT; ++k) {
             float x[NT][4];
-            if (EXACT) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-            }
+            for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
               uint32_t vf[4];
@@ -429,14 +432,12 @@ __global__ void __launch_bounds__(Mma<TC, TQ, DP, NT>::kWarps * 32, Mma<TC, TQ, 
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = PS - 1; i >= 0; --i) mma(EXACT ? x[nt] : o[k][nt], vf, b[kb][i][nt][0], b[kb][i][nt][1]);
+                for (int i = PS - 1; i >= 0; --i) mma(x[nt], vf, b[kb][i][nt][0], b[kb][i][nt][1]);
             }
-            if (EXACT) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[k][nt][e] += x[nt][e];
-            }
+              for (int e = 0; e < 4; ++e) o[k][nt][e] += x[nt][e];
           }
         } else {
           // weights of keys (2 t, 2 t + 1), t = lane % 4, of query lane / 4: two 16-bit

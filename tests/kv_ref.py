@@ -112,3 +112,42 @@ def page_scores(q, codes_lo, codes_hi, scales):
         c = np.nan_to_num(c, nan=0.0).astype(np.int64)
         whole = np.maximum(c, 0) @ codes_hi.T.astype(np.int64) + np.minimum(c, 0) @ codes_lo.T.astype(np.int64)
         return ((whole.astype(np.float32) * t[:, None]).max(0) * scales).astype(np.float32)
+
+
+def result_bound(d, n, size=1.0):
+    """The most an attention result may be off before its own rounding, as a
+    share (2-norm) of the result, with 32-bit sums and 24-bit operands over
+    normal inputs. size: the spread of the scores (1 where scale is d^-0.5).
+
+    A score is at most d / 8 matrix products added up one after another, each
+    cutting the sum by up to U of what it is so far. The sum grows as the square
+    root, so the cuts come to no more than half of U (d / 8) of the score, and
+    change its weight by that times the score: (d / 16) size U. The operands'
+    last bits, the product of their rests where that is left out (2^-21 at the
+    most, 2^-23.6 on average), exponentials, weights and the two sums over a
+    chunk of keys: 4 U together. Running sums over n / 16 chunks are rounded:
+    half of U each at the most, a third of that on average, of a sum that
+    grows as the square root too: sqrt(n / 16) U / 4 covers it."""
+    return (d / 16 * size + 4 + (n / 16) ** 0.5 / 4) * U
+
+
+def result_error(out, want, dtype):
+    """How far `out` (tensor of dtype, one row's results or many of one size)
+    is from the 64-bit `want` before its rounding, as a share of the 2-norm.
+    In 32 bits that is what is seen. A bf16 result shows an error only where
+    it crosses the border between two bf16 values: with chance |error| / step,
+    and then by a step. So the squares of (out - rounded want) add up to the sum of
+    |error| step, and |error| is 0.8 of its root mean square for normal ones."""
+    out, want = out.double().flatten(), want.double().flatten()
+    rms = want.pow(2).mean().sqrt()
+    if dtype == torch.float32:
+        return float((out - want).pow(2).mean().sqrt() / rms)
+    right = want.to(dtype).double()
+    step = torch.exp2(torch.floor(torch.log2(right.abs().clamp(min=1e-30))) - 7)
+    return float((out - right).pow(2).sum() / (0.8 * rms * step.sum()))
+
+
+def attend_exact(q, k, v, scale):
+    """q [rows, kv_heads, group, d], k, v [rows, kv_heads, n, d] -> results, in 64 bits."""
+    p = torch.softmax(torch.einsum("rhgd,rhnd->rhgn", q.double(), k.double()) * scale, -1)
+    return torch.einsum("rhgn,rhnd->rhgd", p, v.double())
