@@ -71,6 +71,16 @@ class PageTable:
         self.position[ids] += counts
         return positions, slots
 
+    def shrink(self, seqs) -> None:
+        """Takes the last extend(seqs) back: places, positions and pages as before it."""
+        ids, counts = np.unique(np.asarray(seqs, dtype=np.int64), return_counts=True)
+        for s, c in zip(ids[::-1], counts[::-1]):
+            self.length[s] -= c
+            self.position[s] -= c
+            for o in range(self._pages(self.length[s] + c) - 1, self._pages(self.length[s]) - 1, -1):
+                self.free.append(int(self.table[s, o]))
+                self.table[s, o] = -1
+
     def take(self, n: int) -> list[int]:
         """n free pages, out of the pool."""
         if n > len(self.free):
@@ -101,6 +111,9 @@ class Step:
     every: bool                   # one row for each sequence, in order
     lengths: torch.Tensor         # of all sequences, after the call
     start: torch.Tensor           # and before it
+    number: int                   # which of the cache's steps
+    longest: int                  # places of the longest sequence in the step
+    mass: dict[int, torch.Tensor] # the sequences' weights before the call, of the layers that have attended
 
 
 class PagedKVCache:
@@ -119,7 +132,8 @@ class PagedKVCache:
         self.pages = PageTable(seqs, width, seqs * width if pages is None else pages, page_size)
         self.seqs, self.max_seq, self.page_size, self.device = seqs, width * page_size, page_size, torch.device(device)
         shape = (config.num_layers, len(self.pages.free), config.num_kv_heads, page_size, config.head_dim)
-        # never read before they are written: places behind a sequence's length are masked out
+        # never read before they are written: places behind a sequence's length are masked out, and a call
+        # that fails before every layer has written its places gives them back (undo)
         self.k = torch.empty(shape, dtype=dtype, device=self.device)
         self.v = torch.empty(shape, dtype=dtype, device=self.device)
         self.table = torch.full((seqs, width), -1, dtype=torch.int32, device=self.device)
@@ -130,6 +144,7 @@ class PagedKVCache:
             self.mass = torch.zeros((config.num_layers, seqs, config.num_kv_heads, self.max_seq), device=self.device)
         self.select = select
         self.bounds = [kv.PageBounds.new(c) for c in self.layers] if select is not None else None
+        self._number = 0  # steps, evictions and releases so far
 
     @property
     def nbytes(self) -> int:
@@ -143,15 +158,39 @@ class PagedKVCache:
         return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(self.device)
 
     def step(self, seqs) -> Step:
-        """Places for one more token of every sequence in `seqs`, row by row; the tables follow."""
+        """Places for one more token of every sequence in `seqs`, row by row; the tables follow. Every layer
+        has to attend with the step; where one cannot, undo(step) takes it back."""
         seqs = np.asarray(seqs, dtype=np.int64)
         before = self.pages.length.copy()
         positions, slots = self.pages.extend(seqs)
+        self._number += 1
+        try:
+            self.table.copy_(torch.from_numpy(self.pages.table))
+            rows = self._ints(np.stack([seqs, positions, slots, slots + 1]))
+            both = self._ints(np.stack([self.pages.length, before]))
+            spans = {int(s): np.flatnonzero(seqs == s) for s in np.unique(seqs)}
+            return Step(rows[0], rows[1], rows[2], rows[3], spans,
+                        len(seqs) == self.seqs and bool(np.all(seqs == np.arange(self.seqs))), both[0], both[1],
+                        self._number, int(slots.max()) + 1 if len(slots) else 0, {})
+        except BaseException:
+            self._give_back(seqs)
+            raise
+
+    def undo(self, step: Step) -> None:
+        """Takes a step back of which not every layer has attended (an error between layers): lengths,
+        positions, pages and accumulated weights are what they were. Only the cache's last step, before
+        any eviction or release after it."""
+        if step.number != self._number:
+            raise ValueError("undo: not the cache's last step")
+        self._give_back([s for s, rows in step.spans.items() for _ in rows])
+        for layer, before in step.mass.items():
+            for i, s in enumerate(step.spans):
+                self.mass[layer, s, :, :step.longest] = before[i]
+
+    def _give_back(self, seqs) -> None:
+        self._number += 1
+        self.pages.shrink(seqs)
         self.table.copy_(torch.from_numpy(self.pages.table))
-        rows = self._ints(np.stack([seqs, positions, slots, slots + 1]))
-        both = self._ints(np.stack([self.pages.length, before]))
-        return Step(rows[0], rows[1], rows[2], rows[3], {int(s): np.flatnonzero(seqs == s) for s in np.unique(seqs)},
-                    len(seqs) == self.seqs and bool(np.all(seqs == np.arange(self.seqs))), both[0], both[1])
 
     def attend(self, layer: int, step: Step, qkv: torch.Tensor, heads: int, theta: float) -> torch.Tensor:
         """One layer's attention for a step: qkv [n, (heads + 2 kv_heads) head_dim]
@@ -168,6 +207,10 @@ class PagedKVCache:
         if self.mass is None:
             return kv.attend(cache, q, step.lens, seqs=step.seqs)
         mass = self.mass[layer]
+        # kept for undo: 4 bytes a place and key head, beside the keys and values of a place
+        seen = mass[:, :, :step.longest]
+        if layer not in step.mass:
+            step.mass[layer] = seen.clone() if step.every else torch.stack([seen[s] for s in step.spans])
         if step.every:
             return kv.attend(cache, q, step.lens, mass=mass)
         # rows of their own, some at a time (256 MB), then summed by sequence in row order: the same sum every time
@@ -214,12 +257,14 @@ class PagedKVCache:
             raise
         for layer, mass in enumerate(masses):
             self.mass[layer][at] = mass
+        self._number += 1
         for i, s in enumerate(long):
             self.pages.replace(s, pages[i * each:(i + 1) * each], budget)
         self.table.copy_(torch.from_numpy(self.pages.table))
 
     def release(self, seq: int) -> None:
         """Forgets a sequence; its pages are free."""
+        self._number += 1
         self.pages.release(seq)
         self.table.copy_(torch.from_numpy(self.pages.table))
         if self.mass is not None:

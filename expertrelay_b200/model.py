@@ -194,35 +194,43 @@ class QwenMoeModel:
         """Run `token_ids` after what `kv` holds; logits [vocab] of the last
         position (or [n, vocab] with all_logits), on the device. With a
         PagedKVCache, `seqs` names the sequence of every token (default: all
-        of sequence 0)."""
+        of sequence 0), and a call that raises leaves it as it was."""
         c = self.c
         ids = torch.as_tensor(np.asarray(token_ids, dtype=np.int64)).to(self.device)
         n = ids.shape[0]
-        paged = isinstance(kv, PagedKVCache)
-        if paged:
+        if isinstance(kv, PagedKVCache):
             seqs = np.zeros(n, dtype=np.int64) if seqs is None else np.asarray(seqs, dtype=np.int64)
             if seqs.shape != (n,):
                 raise ValueError(f"seqs: one sequence for each of {n} tokens, got {seqs.shape}")
             if expert_trace is not None and len(np.unique(seqs)) > 1:
                 raise ValueError("a trace follows one sequence")
-            allowed = kv.step(seqs)
-        elif seqs is not None:
+            step = kv.step(seqs)
+            try:
+                return self._forward(token_ids, ids, kv, step, int(kv.pages.position[seqs[0]]) - n, all_logits,
+                                     expert_trace)
+            except BaseException:  # the places of a call that fails hold nothing, or not in every layer
+                kv.undo(step)
+                raise
+        if seqs is not None:
             raise ValueError("seqs: only with a PagedKVCache")
-        elif kv.length + n > kv.max_seq:
+        if kv.length + n > kv.max_seq:
             raise ValueError(f"sequence length {kv.length + n} exceeds the KV cache ({kv.max_seq})")
+        # causal: query start + i sees keys 0 .. start + i (the same for every layer)
+        start, end = kv.length, kv.length + n
+        allowed = (torch.arange(end, device=self.device)[None, :]
+                   <= (start + torch.arange(n, device=self.device))[:, None]).to(torch.uint8)
+        return self._forward(token_ids, ids, kv, allowed, start, all_logits, expert_trace)
+
+    def _forward(self, token_ids, ids, kv, allowed, start: int, all_logits: bool, expert_trace) -> torch.Tensor:
+        """forward() from position `start` on; allowed as for _attention."""
+        c, n = self.c, ids.shape[0]
         x = torch.empty((n, c.hidden_size), dtype=torch.float32, device=self.device)
         _lib.check(_lib.lib().er_embed_int8(self.embed_q.data_ptr(), self.embed_s.data_ptr(), c.vocab_size,
                                             c.hidden_size, ids.data_ptr(), n, x.data_ptr(), self._bad.data_ptr(),
                                             self._stream()), "er_embed_int8")
-        start = kv.length if not paged else int(kv.pages.position[seqs[0]]) - n
         if expert_trace is not None:
             positions = start + np.arange(n)
             expert_trace.begin(positions, np.asarray(token_ids), PHASE_PREFILL if start == 0 else PHASE_DECODE)
-        if not paged:
-            # causal: query start + i sees keys 0 .. start + i (the same for every layer)
-            end = start + n
-            allowed = (torch.arange(end, device=self.device)[None, :]
-                       <= (start + torch.arange(n, device=self.device))[:, None]).to(torch.uint8)
         h = self._norm(x, self.layers[0]["in_norm"])
         for layer in range(c.num_layers):
             a = self._attention(layer, h, kv, allowed)
@@ -230,7 +238,7 @@ class QwenMoeModel:
             y = self.stack.moe(layer, h, self.path, trace=expert_trace)
             if layer + 1 < c.num_layers:
                 h = self._norm(x, self.layers[layer + 1]["in_norm"], add=y)
-        if not paged:
+        if not isinstance(kv, PagedKVCache):
             kv.length += n
         if expert_trace is not None:
             expert_trace.end()

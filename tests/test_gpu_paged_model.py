@@ -143,3 +143,65 @@ def test_an_eviction_that_is_refused_changes_nothing(cuda):
     with pytest.raises(ValueError, match="400000 weights"):
         cache.evict(200, recent=10)
     assert cache.length() == 300 and sorted(cache.pages.free) == before[1] and (cache.pages.table == before[0]).all()
+
+
+class _Fails:
+    """A model's MoE stack whose layer `at` raises on its next call."""
+
+    def __init__(self, stack, at, error):
+        self.stack, self.at, self.error = stack, at, error
+
+    def moe(self, layer, *args, **kwargs):
+        if layer == self.at and self.error is not None:
+            error, self.error = self.error, None
+            raise error
+        return self.stack.moe(layer, *args, **kwargs)
+
+
+@pytest.mark.parametrize("error", [RuntimeError("no room"), KeyboardInterrupt()])
+@pytest.mark.parametrize("options", [{}, {"mass": True}, {"select": (2, 1, 1)}])
+@pytest.mark.parametrize("at", [0, 1])
+def test_a_call_that_raises_can_be_made_again(cuda, options, error, at):
+    """Nothing of a call that fails between layers stays: lengths, positions, pages, weights; the same call again
+    gives what it would have, prompts, steps of some sequences and steps of all."""
+    g = golden("model")
+    model = _model(0, cuda)
+    kv, fresh = (model.new_paged_cache(3, 64, page_size=4, **options) for _ in range(2))
+    prompt = [int(t) for t in g["prompt0"]]
+    calls = [(prompt, [1] * len(prompt)), (prompt[:5] + prompt[:3], [2] * 5 + [0] * 3), ([7, 8], [1, 2]), ([3, 4, 5], [0, 1, 2]),
+             ([9] * 6, [0, 1, 2] * 2)]
+    stack = model.stack
+    for tokens, seqs in calls:
+        before = (kv.pages.table.copy(), kv.pages.length.copy(), kv.pages.position.copy(), list(kv.pages.free),
+                  None if kv.mass is None else kv.mass.clone())
+        model.stack = _Fails(stack, at, error)
+        with pytest.raises(type(error)):
+            model.forward(tokens, kv, seqs=seqs)
+        model.stack = stack
+        assert (kv.pages.table == before[0]).all() and (kv.table.cpu().numpy() == before[0]).all()
+        assert (kv.pages.length == before[1]).all() and (kv.pages.position == before[2]).all()
+        assert kv.pages.free == before[3] and (kv.mass is None or torch.equal(kv.mass, before[4]))
+        got, want = (model.forward(tokens, c, all_logits=True, seqs=seqs) for c in (kv, fresh))
+        assert torch.equal(got, want)
+    assert kv.mass is None or torch.equal(kv.mass, fresh.mass)
+    with pytest.raises(ValueError, match="token ids"):
+        model.forward([model.c.vocab_size], kv, seqs=[1])
+    assert torch.equal(model.forward([2], kv, seqs=[1]), model.forward([2], fresh, seqs=[1]))
+    kv.check()
+    model.close()
+
+
+def test_only_the_last_step_is_taken_back(cuda):
+    shape = SimpleNamespace(num_layers=1, num_kv_heads=1, head_dim=8)
+    cache = PagedKVCache(shape, 2, 16, page_size=4, device=cuda)
+    first, second = cache.step([0] * 5), cache.step([1])
+    with pytest.raises(ValueError, match="last step"):
+        cache.undo(first)
+    cache.undo(second)
+    with pytest.raises(ValueError, match="last step"):
+        cache.undo(second)
+    third = cache.step([1, 1])
+    cache.release(1)
+    with pytest.raises(ValueError, match="last step"):
+        cache.undo(third)
+    assert cache.length(0) == 5 and cache.length(1) == 0 and len(cache.pages.free) == 6

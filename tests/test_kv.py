@@ -148,3 +148,17 @@ def test_page_table_refusals_change_nothing():
     assert [len(x) for x in t.extend([])] == [0, 0]
     with pytest.raises(ValueError, match="at least one"):
         PageTable(1, 0, 1, 16)
+
+
+def test_page_table_takes_an_extension_back():
+    t = PageTable(4, 8, 20, 4)
+    t.extend([0] * 5 + [2] * 4)
+    t.release(0)
+    t.extend([3] * 3 + [2])
+    t.replace(2, t.take(1), 3)  # evicted: positions and places differ
+    before = (t.table.copy(), t.length.copy(), t.position.copy(), list(t.free))
+    for seqs in ([2], [2, 3, 2, 0, 3, 3, 3, 0], [1] * 9, [], [0] * 32, [3, 2, 1, 0]):
+        t.extend(seqs)
+        t.shrink(seqs)
+        assert (t.table == before[0]).all() and (t.length == before[1]).all() and (t.position == before[2]).all()
+        assert t.free == before[3]  # in order, so that a retry gets the same pages
