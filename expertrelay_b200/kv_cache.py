@@ -88,8 +88,9 @@ class PageTable:
         return [self.free.pop() for _ in range(n)]
 
     def replace(self, seq: int, pages: list[int], length: int) -> None:
-        """The sequence's places are now `length`, in `pages`; its old pages are free."""
-        self.free += [int(p) for p in self.table[seq] if p >= 0]
+        """The sequence's places are now `length`, in `pages`; its old pages that are none of them are free."""
+        kept = set(pages)
+        self.free += [int(p) for p in self.table[seq] if p >= 0 and int(p) not in kept]
         self.table[seq] = -1
         self.table[seq, :len(pages)] = pages
         self.length[seq] = length
@@ -119,7 +120,9 @@ class Step:
 class PagedKVCache:
     """`seqs` sequences of up to max_seq places each in `pages` pages of
     page_size places (default: as many as all of them can need). config: a
-    ModelConfig (layers, key heads, head_dim); dtype: float32 or bfloat16."""
+    ModelConfig (layers, key heads, head_dim); dtype: float32 or bfloat16.
+    Caches that are to be cut (mass=True, evict) have at most about 370000 places
+    a sequence."""
 
     def __init__(self, config, seqs: int, max_seq: int, *, page_size: int = 64, pages: int | None = None,
                  dtype: torch.dtype = torch.float32, device="cuda", mass: bool = False,
@@ -230,35 +233,57 @@ class PagedKVCache:
         """Cuts every sequence of more than `budget` places to `budget`: each
         layer and key head keeps the first `sinks`, the last `recent` and the
         places of the greatest accumulated weight (kv.evict). Later tokens keep
-        their positions. The kept places are copied to free pages, and the old
-        pages are free afterwards; ValueError if there are not enough."""
+        their positions. As many sequences at a time as there are free pages
+        for are copied to those, and their old pages are free afterwards; where
+        there are none for a single one, it goes by way of new memory back into
+        its own first pages. Caches of more than about 370000 places are
+        refused (kv.evict), which changes nothing; an error that only a later
+        sequence meets leaves the ones before it cut and the rest as they were."""
         if self.mass is None:
             raise ValueError("evict needs a cache made with mass=True")
         if not 1 <= budget <= self.max_seq or sinks < 0 or recent < 0 or sinks + recent > budget:
             raise ValueError(f"budget {budget} of {self.max_seq} places, with {sinks} first and {recent} last")
         long = [s for s in range(self.seqs) if self.pages.length[s] > budget]
-        if not long:
-            return
         each = -(-budget // self.page_size)
-        pages = self.pages.take(each * len(long))
-        to_table = self._ints(np.asarray(pages).reshape(len(long), each))
-        at = torch.tensor(long, device=self.device)
-        table, lens = self.table[at], self._ints(self.pages.length[long])
+        while long:
+            n = min(len(long), len(self.pages.free) // each)
+            if n:
+                pages = self.pages.take(n * each)
+                try:
+                    self._cut(long[:n], pages, self.k, self.v, pages, budget, sinks, recent)
+                except BaseException:  # nothing has changed but pages that nothing names
+                    self.pages.free += pages[::-1]
+                    raise
+            else:
+                n, pages = 1, [int(p) for p in self.pages.table[long[0], :each]]
+                shape = (self.k.shape[0], each, *self.k.shape[2:])
+                k, v = (torch.empty(shape, dtype=self.k.dtype, device=self.device) for _ in range(2))
+                self._cut(long[:1], range(each), k, v, pages, budget, sinks, recent)
+            long = long[n:]
+
+    def _cut(self, seqs: list[int], to: list[int], k: torch.Tensor, v: torch.Tensor, pages: list[int], budget: int,
+             sinks: int, recent: int) -> None:
+        """Evicts from `seqs` into the pages `to` of the pools k, v (all layers'), which become the cache's `pages`."""
+        each = len(pages) // len(seqs)
+        to_table = self._ints(np.asarray(to).reshape(len(seqs), each))
+        at = torch.tensor(seqs, device=self.device)
+        table, lens = self.table[at], self._ints(self.pages.length[seqs])
+        own = None if k is self.k else torch.tensor(pages, device=self.device)
         masses = []
-        try:
-            for layer in range(len(self.layers)):
-                old = kv.PagedKV(self.k[layer], self.v[layer], table, self.status)
-                new = kv.PagedKV(self.k[layer], self.v[layer], to_table, self.status)
-                mass = torch.zeros((len(long), *self.mass.shape[2:]), device=self.device)
-                kv.evict(old, lens, self.mass[layer][at], new, mass, budget, sinks=sinks, recent=recent)
-                masses.append(mass)
-        except Exception:  # nothing has changed but pages that nothing names
-            self.pages.free += pages
-            raise
-        for layer, mass in enumerate(masses):
-            self.mass[layer][at] = mass
+        for layer in range(len(self.layers)):
+            old = kv.PagedKV(self.k[layer], self.v[layer], table, self.status)
+            new = kv.PagedKV(k[layer], v[layer], to_table, self.status)
+            mass = torch.zeros((len(seqs), *self.mass.shape[2:]), device=self.device)
+            kv.evict(old, lens, self.mass[layer][at], new, mass, budget, sinks=sinks, recent=recent)
+            masses.append(mass)
+        # every layer has been chosen from: nothing is refused from here on
         self._number += 1
-        for i, s in enumerate(long):
+        for layer, mass in enumerate(masses):
+            self.mass[layer].index_copy_(0, at, mass)
+            if own is not None:
+                self.k[layer].index_copy_(0, own, k[layer])
+                self.v[layer].index_copy_(0, own, v[layer])
+        for i, s in enumerate(seqs):
             self.pages.replace(s, pages[i * each:(i + 1) * each], budget)
         self.table.copy_(torch.from_numpy(self.pages.table))
 

@@ -12,6 +12,7 @@ import pytest
 import torch
 from conftest import golden
 from golden.make_golden import MODEL_CASES, MODEL_NEW, MODEL_PROMPT
+from kv_ref import choose, tokens
 
 from expertrelay_b200 import _lib, synth
 from expertrelay_b200.kv_cache import PagedKVCache
@@ -205,3 +206,77 @@ def test_only_the_last_step_is_taken_back(cuda):
     with pytest.raises(ValueError, match="last step"):
         cache.undo(third)
     assert cache.length(0) == 5 and cache.length(1) == 0 and len(cache.pages.free) == 6
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize(("budget", "sinks", "recent"), [(32, 4, 8), (13, 0, 1), (61, 2, 5), (63, 0, 0)])
+@pytest.mark.parametrize("pages", [None, 34, 40, 64])
+def test_eviction_whatever_pages_are_free(cuda, dtype, budget, sinks, recent, pages):
+    """Pools without a free page, with one sequence's worth, with all: the same places stay, in pages of the pool, and
+    later calls go on from them."""
+    shape = SimpleNamespace(num_layers=2, num_kv_heads=2, head_dim=16)
+    lens = [64, 64, 5, 64, 50]
+    cache = PagedKVCache(shape, 5, 64, page_size=8, pages=pages or 32, dtype=dtype, mass=True, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(budget)
+    seqs = [s for s, n in enumerate(lens) for _ in range(n)]
+    step = cache.step(seqs)
+    for layer in range(2):
+        cache.attend(layer, step, torch.randn((len(seqs), 6 * 16), generator=gen, device=cuda), 2, 1e4)
+    if pages is None:
+        assert not cache.pages.free
+    table = torch.from_numpy(cache.pages.table.copy())
+    old = {(i, s): (tokens(cache.k[i], table, s, n), tokens(cache.v[i], table, s, n)) for i in range(2) for s, n in enumerate(lens)}
+    mass = cache.mass.cpu().numpy()
+    cache.evict(budget, sinks=sinks, recent=recent)
+    cache.check()
+    total = pages or 32
+    used = [int(p) for p in cache.pages.table.ravel() if p >= 0]
+    assert sorted(used + cache.pages.free) == list(range(total)) and len(set(used)) == len(used)
+    assert (cache.table.cpu().numpy() == cache.pages.table).all()
+    assert cache.pages.position.tolist() == lens
+    table = torch.from_numpy(cache.pages.table.copy())
+    for s, n in enumerate(lens):
+        m = min(n, budget)
+        assert cache.length(s) == m
+        for i in range(2):
+            k, v = tokens(cache.k[i], table, s, m), tokens(cache.v[i], table, s, m)
+            for h in range(2):
+                ids = choose(mass[i, s, h], n, budget, sinks, recent)
+                assert np.array_equal(k[h], old[i, s][0][h][ids]) and np.array_equal(v[h], old[i, s][1][h][ids])
+                assert np.array_equal(cache.mass[i, s, h].cpu().numpy(), np.pad(mass[i, s, h][ids], (0, 64 - m)))
+    step = cache.step([0, 1, 2, 3, 4])
+    for layer in range(2):
+        assert torch.isfinite(cache.attend(layer, step, torch.randn((5, 96), generator=gen, device=cuda), 2, 1e4)).all()
+    cache.check()
+
+
+def test_an_eviction_that_fails_between_layers_changes_nothing(cuda, monkeypatch):
+    from expertrelay_b200 import kv as operators
+
+    shape = SimpleNamespace(num_layers=2, num_kv_heads=1, head_dim=8)
+    for pages in (8, 16):  # without free pages, and with some
+        cache = PagedKVCache(shape, 2, 32, page_size=8, pages=pages, mass=True, device=cuda)
+        step = cache.step([0] * 32 + [1] * 32)
+        for layer in range(2):
+            cache.attend(layer, step, torch.randn((64, 3 * 8), device=cuda), 1, 1e4)
+        before = [x.clone() for x in (cache.k, cache.v, cache.mass, cache.table)]
+        host = (cache.pages.table.copy(), cache.pages.length.copy(), list(cache.pages.free))
+        real, calls = operators.evict, []
+
+        def failing(*args, **kwargs):
+            calls.append(0)
+            if len(calls) == 2:
+                raise RuntimeError("no room")
+            return real(*args, **kwargs)
+
+        monkeypatch.setattr(operators, "evict", failing)
+        with pytest.raises(RuntimeError, match="no room"):
+            cache.evict(20, recent=4)
+        monkeypatch.setattr(operators, "evict", real)
+        assert (cache.pages.table == host[0]).all() and (cache.pages.length == host[1]).all() and cache.pages.free == host[2]
+        assert torch.equal(cache.mass, before[2]) and torch.equal(cache.table, before[3])
+        table = torch.from_numpy(host[0])
+        for s in (0, 1):
+            for i in range(2):
+                assert np.array_equal(tokens(cache.k[i], table, s, 32), tokens(before[0][i], table, s, 32))
+                assert np.array_equal(tokens(cache.v[i], table, s, 32), tokens(before[1][i], table, s, 32))

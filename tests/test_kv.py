@@ -162,3 +162,13 @@ def test_page_table_takes_an_extension_back():
         t.shrink(seqs)
         assert (t.table == before[0]).all() and (t.length == before[1]).all() and (t.position == before[2]).all()
         assert t.free == before[3]  # in order, so that a retry gets the same pages
+
+
+def test_a_sequence_keeps_some_of_its_own_pages():
+    t = PageTable(2, 4, 8, 16)
+    t.extend([0] * 64 + [1] * 64)
+    own = [int(p) for p in t.table[0, :2]]
+    rest = [int(p) for p in t.table[0, 2:]]
+    t.replace(0, own, 20)
+    assert t.table[0].tolist() == [*own, -1, -1] and sorted(t.free) == sorted(rest)
+    assert t.length.tolist() == [20, 64] and t.position.tolist() == [64, 64]
