@@ -107,6 +107,10 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
   const int unit = blockIdx.y, row = unit / a.kv.kv_heads, h = unit % a.kv.kv_heads;
   const Entry e = kv_entry(a, row);
   float* to = a.mass + row * a.mass_row_stride + h * a.mass_head_stride;
+  if (e.bad) {  // which positions it meant is not known: all are spoilt
+    for (long long j = blockIdx.x * 256 + threadIdx.x; j < a.mass_len; j += gridDim.x * 256) to[j] = __int_as_float(0x7fc00000);
+    return;
+  }
   const float* s = a.scores + (long long)unit * a.mass_len * a.group;
   const float* lse = a.lse + (long long)row * a.heads + h * a.group;
   for (long long j = blockIdx.x * 256 + threadIdx.x; j < e.n; j += gridDim.x * 256) {  // a step may pass 2^31

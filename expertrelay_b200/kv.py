@@ -19,8 +19,9 @@ waits on the host. Lengths, positions, tables and lists are read on the
 device, so a call captured in a CUDA graph serves whatever they hold at
 replay. What is wrong with them (a page id outside the pool, a length
 outside the table) is found there too: the rows concerned come back as NaN
-(their mass with them) or stay unwritten, and PagedKV.check() raises. attend
-allocates its workspace from torch's allocator on that stream unless given one.
+(their mass with them, all of it where a length or sequence is bad) or stay
+unwritten, and PagedKV.check() raises. attend allocates its workspace from
+torch's allocator on that stream unless given one.
 
 Infinities: an infinite or NaN key or value behind a row's length changes
 nothing. One that is seen makes the row's results what the formula gives,

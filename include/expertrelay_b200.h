@@ -428,8 +428,9 @@ ER_API int er_kv_append(const er_kv_cache* cache, const void* qkv, int qkv_dtype
  * (distinct; positions behind lens[r] are left out).
  * With mass, mass[r * mass_row_stride + h * mass_head_stride + j] grows by
  * key head h's attention weight on position j, summed over its queries
- * (not together with pages; NaN where the row is spoiled). The workspace is
- * 256-byte aligned; some calls need none (0 bytes). */
+ * (not together with pages). A bad page makes it NaN over the row's positions, a
+ * bad length (one beyond mass_len too) or sequence over all mass_len of them.
+ * The workspace is 256-byte aligned; some calls need none (0 bytes). */
 typedef struct er_kv_attend_io {
   const void* q;               /* [rows, heads, head_dim], row stride q_stride elements */
   int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */

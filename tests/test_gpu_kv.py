@@ -718,3 +718,34 @@ def test_calls_of_one_cache_on_two_streams(cuda):
     torch.cuda.synchronize()
     for out, pages in outs:
         assert torch.equal(out, want) and torch.equal(pages, want_pages)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("wide", [False, True])
+def test_mass_of_spoilt_rows(cuda, dtype, wide):
+    """A bad page spoils a row's mass up to its length, a bad length or sequence, or one beyond the mass, all of it;
+    the rows beside them grow as ever. By a cluster a unit and (a table too wide for that) by equal shares."""
+    cache, q = _case(13, [100] * 7, 1, 3, 64, 16, dtype, dtype)
+    table = torch.full((7, 40000 if wide else cache.width), -1, dtype=torch.int32, device="cuda")
+    table[:, :cache.width] = cache.table
+    table[1, 6] = cache.num_pages
+    cache = kv.PagedKV(cache.k, cache.v, table)
+    given = [100, 100, -1, 113 if not wide else 640001, 100, 90, 0]
+    mass = torch.rand((7, 1, 112), device="cuda")
+    mass0 = mass.clone()
+    out = kv.attend(cache, q, _i32(given), seqs=_i32([0, 1, 2, 3, 7, 5, 6]), mass=mass)
+    for r in (1, 2, 3, 4):
+        assert torch.isnan(out[r]).all() and torch.isnan(mass[r, 0, :100]).all(), r
+    assert torch.equal(mass[1, :, 100:], mass0[1, :, 100:])
+    for r in (2, 3, 4):
+        assert torch.isnan(mass[r]).all(), r
+    for r in (0, 5, 6):
+        _check_attend(cache, q[r:r + 1], [given[r]], out[r:r + 1], seqs=[r], mass=mass[r:r + 1], mass0=mass0[r:r + 1])
+    with pytest.raises(ValueError, match="page id outside the pool, a length.*, a sequence"):
+        cache.check()
+    short = mass0[:, :, :99].clone()  # a row longer than the mass has room for
+    out = kv.attend(cache, q, _i32([100, 10, 0, 99, 5, 90, 0]), mass=short)
+    assert torch.isnan(out[0]).all() and torch.isnan(short[0]).all()
+    assert not torch.isnan(out[1:]).any() and not torch.isnan(short[1:]).any()
+    with pytest.raises(ValueError, match="a length"):
+        cache.check()
