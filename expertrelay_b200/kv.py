@@ -65,8 +65,8 @@ def _apart(shape, stride) -> bool:
 
 
 def _share(a, b) -> bool:
-    """Whether two [seqs, heads, n] tensors may share an element: their extents meet, and they are no two
-    layers of one array."""
+    """Whether two tensors of as many dimensions may share an element: their extents meet, and they are no
+    two layers of one array."""
     (a, b) = sorted((a, b), key=lambda t: t.data_ptr())
     size = a.element_size()
     if not a.numel() or not b.numel():
@@ -106,7 +106,8 @@ class PagedKV:
     [pages, page_size, kv_heads, head_dim] pools are passed transposed);
     table [seqs, width] int32, rows contiguous: the page of each run of
     page_size positions. head_dim: a multiple of 8, at most 256; kv_heads: at
-    most 1024. Sequences may share pages as long as no call writes to them.
+    most 1024. Sequences may share pages, and k and v memory, as long as no call
+    writes to them.
 
     `status` ([1] int32; a new one unless given) collects what the device
     found wrong (check())."""
@@ -126,6 +127,7 @@ class PagedKV:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.seqs, self.width = table.shape
         self._apart = _apart(k.shape, k.stride())
+        self._two = not _share(k, v)
         if status is not None:
             _need(status, "status", torch.int32, k.device, (1,))
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device) if status is None else status
@@ -145,6 +147,8 @@ class PagedKV:
     def _writable(self) -> None:
         if not self._apart:
             raise ValueError(f"pools of strides {self.k.stride()} make slots share memory")
+        if not self._two:
+            raise ValueError("k and v share memory")
 
     def check(self) -> None:
         """Raises ValueError if a call since the last check met a bad page id,

@@ -749,3 +749,26 @@ def test_mass_of_spoilt_rows(cuda, dtype, wide):
     assert not torch.isnan(out[1:]).any() and not torch.isnan(short[1:]).any()
     with pytest.raises(ValueError, match="a length"):
         cache.check()
+
+
+def test_pools_of_shared_memory_are_not_written(cuda):
+    """k and v in one place are read as they are, and refused where a call would write both there."""
+    cache, q = _case(14, [40, 9], 2, 2, 64, 16, F32, F32)
+    lens = _i32([40, 9])
+    table = cache.table.clone()
+    one = kv.PagedKV(cache.k, cache.k, table)
+    _check_attend(one, q, [40, 9], kv.attend(one, q, lens))
+    shifted = kv.PagedKV(cache.k[:-1], cache.k[1:], table)
+    to_mass = torch.zeros((2, 2, 8), device="cuda")
+    for pools in (one, shifted):
+        with pytest.raises(ValueError, match="k and v share memory"):
+            kv.append(pools, torch.zeros((2, 8 * 64), device="cuda"), _i32([0, 0]), 4, 1e4)
+        with pytest.raises(ValueError, match="k and v share memory"):
+            kv.evict(cache, lens, torch.zeros((2, 2, 64), device="cuda"), pools, to_mass, 8, recent=2)
+    pool = torch.zeros((4, 2, 2, 16, 64), device="cuda")  # a page's keys and values side by side
+    both = kv.PagedKV(pool[:, 0], pool[:, 1], _i32([[1, 3], [2, 0]]))
+    x = torch.randn((2, 8 * 64), device="cuda")
+    kv.append(both, x, _i32([17, 2]), 4, 1e4)
+    assert torch.equal(pool[3, 1, :, 1], x[0].view(8, 64)[6:]) and torch.equal(pool[2, 1, :, 2], x[1].view(8, 64)[6:])
+    assert int((pool != 0).any(-1).sum()) == 8
+    both.check()

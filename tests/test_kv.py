@@ -172,3 +172,15 @@ def test_a_sequence_keeps_some_of_its_own_pages():
     t.replace(0, own, 20)
     assert t.table[0].tolist() == [*own, -1, -1] and sorted(t.free) == sorted(rest)
     assert t.length.tolist() == [20, 64] and t.position.tolist() == [64, 64]
+
+
+def test_pools_that_share_memory():
+    share = kv._share
+    a = torch.zeros(6 * 2 * 3 * 4 * 8)
+    both = a.view(6, 2, 3, 4, 8)  # keys and values of a page side by side
+    assert not share(both[:, 0], both[:, 1]) and not share(both[:, 1], both[:, 0])
+    wide = a.view(6, 3, 4, 16)  # or of a slot
+    assert not share(wide[..., :8], wide[..., 8:])
+    assert not share(both[:3, 0], both[3:, 0])
+    k = a.view(12, 3, 4, 8)
+    assert share(k, k) and share(k[:8], k[4:]) and share(wide[..., :8], wide[..., 4:12])
