@@ -43,13 +43,20 @@ class PageTable:
     def _pages(self, n: int) -> int:
         return -(-int(n) // self.page_size)
 
+    def known(self, seqs) -> None:
+        """ValueError for a sequence that is none of the table's (a negative one would count from the end)."""
+        seqs = np.asarray(seqs)
+        if seqs.size and (seqs.min() < 0 or seqs.max() >= len(self.length)):
+            raise ValueError(f"sequences outside [0, {len(self.length)})")
+
     def extend(self, seqs) -> tuple[np.ndarray, np.ndarray]:
         """A place for one more token of each sequence in `seqs` (in order; a
         sequence may occur more than once): (positions, slots). Raises
         ValueError, changing nothing, if a table or the pool is full."""
         seqs = np.asarray(seqs, dtype=np.int64)
-        if seqs.ndim != 1 or (len(seqs) and (seqs.min() < 0 or seqs.max() >= len(self.length))):
-            raise ValueError(f"sequences outside [0, {len(self.length)})")
+        if seqs.ndim != 1:
+            raise ValueError(f"sequences: one for each row, got {seqs.shape}")
+        self.known(seqs)
         ids, counts = np.unique(seqs, return_counts=True)
         new = []
         for s, c in zip(ids, counts):
@@ -96,6 +103,7 @@ class PageTable:
         self.length[seq] = length
 
     def release(self, seq: int) -> None:
+        self.known(seq)
         self.replace(seq, [], 0)
         self.position[seq] = 0
 
@@ -155,6 +163,7 @@ class PagedKVCache:
 
     def length(self, seq: int = 0) -> int:
         """The places sequence `seq` uses."""
+        self.pages.known(seq)
         return int(self.pages.length[seq])
 
     def _ints(self, a) -> torch.Tensor:
@@ -289,8 +298,8 @@ class PagedKVCache:
 
     def release(self, seq: int) -> None:
         """Forgets a sequence; its pages are free."""
-        self._number += 1
         self.pages.release(seq)
+        self._number += 1
         self.table.copy_(torch.from_numpy(self.pages.table))
         if self.mass is not None:
             self.mass[:, seq].zero_()

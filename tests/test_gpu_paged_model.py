@@ -280,3 +280,13 @@ def test_an_eviction_that_fails_between_layers_changes_nothing(cuda, monkeypatch
             for i in range(2):
                 assert np.array_equal(tokens(cache.k[i], table, s, 32), tokens(before[0][i], table, s, 32))
                 assert np.array_equal(tokens(cache.v[i], table, s, 32), tokens(before[1][i], table, s, 32))
+
+
+def test_a_sequence_outside_the_cache_is_not_another_one(cuda):
+    cache = PagedKVCache(SimpleNamespace(num_layers=1, num_kv_heads=1, head_dim=8), 2, 16, page_size=4, mass=True, device=cuda)
+    cache.step([1] * 5)
+    cache.mass[:, 1] = 1
+    for call in (lambda: cache.release(-1), lambda: cache.release(2), lambda: cache.length(-1), lambda: cache.length(2)):
+        with pytest.raises(ValueError, match="outside"):
+            call()
+    assert cache.length(1) == 5 and (cache.mass[:, 1] == 1).all()

@@ -184,3 +184,14 @@ def test_pools_that_share_memory():
     assert not share(both[:3, 0], both[3:, 0])
     k = a.view(12, 3, 4, 8)
     assert share(k, k) and share(k[:8], k[4:]) and share(wide[..., :8], wide[..., 4:12])
+
+
+def test_a_sequence_outside_the_table_is_not_another_one():
+    t = PageTable(3, 4, 7, 16)
+    t.extend([2] * 20)
+    for seq in (-1, 3):
+        with pytest.raises(ValueError, match="outside"):
+            t.release(seq)
+    assert t.length.tolist() == [0, 0, 20] and len(t.free) == 5
+    with pytest.raises(ValueError, match="one for each row"):
+        t.extend([[0, 1]])
