@@ -139,7 +139,7 @@ class PagedKVCache:
             raise ValueError("mass and select: attention over selected pages does not accumulate weights")
         if select is not None and (min(select) < 0 or select[0] < 1 or select[1] + select[2] > select[0]):
             raise ValueError(f"select: (budget, sinks, recent), got {select}")
-        width = -(-max_seq // page_size)
+        width = -(-max_seq // page_size) if page_size > 0 else 0  # PageTable refuses 0
         self.pages = PageTable(seqs, width, seqs * width if pages is None else pages, page_size)
         self.seqs, self.max_seq, self.page_size, self.device = seqs, width * page_size, page_size, torch.device(device)
         shape = (config.num_layers, len(self.pages.free), config.num_kv_heads, page_size, config.head_dim)

@@ -3,12 +3,13 @@
 from __future__ import annotations
 
 import ctypes as C
+from types import SimpleNamespace
 
 import pytest
 import torch
 
 from expertrelay_b200 import _lib, kv
-from expertrelay_b200.kv_cache import PageTable
+from expertrelay_b200.kv_cache import PagedKVCache, PageTable
 
 P = 0x1000  # an address that is never followed
 
@@ -195,3 +196,11 @@ def test_a_sequence_outside_the_table_is_not_another_one():
     assert t.length.tolist() == [0, 0, 20] and len(t.free) == 5
     with pytest.raises(ValueError, match="one for each row"):
         t.extend([[0, 1]])
+
+
+@pytest.mark.parametrize("change", [{"page_size": 0}, {"page_size": -4}, {"max_seq": 0}, {"seqs": 0}, {"pages": 0}])
+def test_a_cache_of_nothing_is_refused(change):
+    shape = SimpleNamespace(num_layers=1, num_kv_heads=1, head_dim=8)
+    args = {"seqs": 1, "max_seq": 8, "page_size": 4, "device": "cpu", **change}
+    with pytest.raises(ValueError, match="at least one"):
+        PagedKVCache(shape, **args)
