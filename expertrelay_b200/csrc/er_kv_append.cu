@@ -355,8 +355,7 @@ extern "C" int er_kv_page_bounds(const er_kv_cache* cache, const int32_t* lens, 
   if (cache->seqs == 0 || cache->table_width == 0) return ER_OK;
   if (!lens || !start || !codes || !scales) return fail(ER_EINVAL, "er_kv_page_bounds: null pointer");
   if ((uintptr_t)codes & 7) return fail(ER_EINVAL, "er_kv_page_bounds: codes must be 8-byte aligned");
-  if (cache->seqs > 65535 || cache->kv_heads > 65535)
-    return fail(ER_EINVAL, "er_kv_page_bounds: %d sequences, %d key heads", cache->seqs, cache->kv_heads);
+  if (cache->seqs > 65535) return fail(ER_EINVAL, "er_kv_page_bounds: %d sequences (at most 65535)", cache->seqs);
   const KvView kv = kv_view(*cache);
   // a step touches one page a sequence, a prompt all of them: the CTAs of a
   // (sequence, key head) walk its pages, about 16 CTAs an SM in all

@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(const __grid_constant__ At
 
 namespace {
 
-constexpr int kMaxEntries = 4096;  // scan entries a launch takes; more rows go in several launches
+// scan entries a launch takes (at least four rows: key heads are 1024 at the most); more rows go in several launches
+constexpr int kMaxEntries = 4096;
 
 struct Layout {
   KernelShape shape;
@@ -149,7 +150,6 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   L.grid = sms * L.shape.per_sm;
   if (L.grid > kJoinThreads * kJoinPieces) L.grid = kJoinThreads * kJoinPieces;
   L.rows = io.pages ? kMaxEntries / c.kv_heads : kMaxEntries;
-  if (L.rows < 1) L.rows = 1;
   if (L.rows > io.rows) L.rows = io.rows;
   if (io.mass) {  // the scores of a launch stay within 256 MB, or one row's
     const long long most = (256ll << 20) / (4ll * io.heads * (io.mass_len > 0 ? io.mass_len : 1));
@@ -200,7 +200,6 @@ int attend_check(const er_kv_cache* c, const er_kv_attend_io* io) {
   if (io->mass && io->mass_len < 0) return fail(ER_EINVAL, "er_kv_attend: mass_len %d", io->mass_len);
   if (!io->seqs && io->rows > c->seqs)
     return fail(ER_EINVAL, "er_kv_attend: %d rows, %d sequences", io->rows, c->seqs);
-  if (io->pages && c->kv_heads > kMaxEntries) return fail(ER_EINVAL, "er_kv_attend: %d key heads", c->kv_heads);
   return ER_OK;
 }
 

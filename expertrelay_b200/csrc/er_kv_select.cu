@@ -430,8 +430,7 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   if (from->seqs == 0) return ER_OK;
   if (!lens || !mass || !to_mass || !kept_out || !lens_out) return fail(ER_EINVAL, "er_kv_evict: null pointer");
   if (lens == lens_out) return fail(ER_EINVAL, "er_kv_evict: lens_out is lens");
-  if (from->seqs > 65535 || from->kv_heads > 65535)
-    return fail(ER_EINVAL, "er_kv_evict: %d sequences, %d key heads", from->seqs, from->kv_heads);
+  if (from->seqs > 65535) return fail(ER_EINVAL, "er_kv_evict: %d sequences (at most 65535)", from->seqs);
   const KvView a = kv_view(*from), b = kv_view(*to);
   const MassView m{mass,        to_mass,  mass_seq_stride, mass_head_stride, to_mass_seq_stride, to_mass_head_stride,
                    mass_len, to_mass_len};
@@ -439,8 +438,6 @@ extern "C" int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const
   const int row_bytes = a.d * (from->dtype == ER_DTYPE_BF16 ? 2 : 4), units = a.seqs * a.kv_heads;
   if (select_bytes(cluster_each(mass_len)) + held_bytes(cluster_each(mass_len)) > kSelectSmem)
     return fail(ER_EINVAL, "er_kv_evict: %d weights a key head (about 370000 fit)", mass_len);
-  if ((long long)a.seqs * a.kv_heads > 0x7fffffff / kClusterCtas)
-    return fail(ER_EINVAL, "er_kv_evict: %d sequences, %d key heads", a.seqs, a.kv_heads);
   const int mode = choose_mode(units, mass_len, 0), most = choose_held(mode, mass_len);
   auto keep = mode == kTogether ? kv_keep_kernel<kTogether>
               : mode == kFirst ? kv_keep_kernel<kFirst>

@@ -99,6 +99,15 @@ def test_evict_refusals():
         _fails(call(**{name: None}), "null")
 
 
+def test_limits_of_sequences_and_key_heads():
+    L, c = _lib.lib(), _cache(seqs=65536)
+    _fails(L.er_kv_page_bounds(C.byref(c), P, P, P, P, None, None), "65536 sequences")
+    _fails(L.er_kv_evict(C.byref(c), C.byref(c), P, P, 1, 1, 64, P, 1, 1, 64, 8, 0, 0, P, P + 64, None, None), "65536 sequences")
+    c = _cache(kv_heads=1025)
+    _fails(L.er_kv_attend(C.byref(c), C.byref(_io(heads=1025, q_stride=2**30)), None, 0, None), "1025 key heads")
+    _fails(L.er_kv_page_bounds(C.byref(c), P, P, P, P, None, None), "1025 key heads")
+
+
 def test_nothing_to_do_is_fine():
     L = _lib.lib()
     assert L.er_kv_attend(C.byref(_cache()), C.byref(_io(rows=0)), None, 0, None) == _lib.ER_OK
