@@ -163,7 +163,8 @@ class PagedKV:
 
 
 class PageBounds:
-    """Per page and key head, the least and greatest key of every channel:
+    """Per page and key head, the least and greatest key of every channel,
+    rounded to the nearest code (a key may pass them by half a step):
     codes [pages, kv_heads, 2, head_dim] int8 and scales [pages, kv_heads]
     float32, contiguous, on the cache's device."""
 
@@ -326,8 +327,10 @@ def select_pages(cache: PagedKV, bounds: PageBounds, q: torch.Tensor, lens: torc
                  seqs: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """For each row and key head up to `budget` pages: the first `sinks`, the
     last `recent`, then those whose bounds allow the greatest product with
-    one of the key head's queries (both as int8 codes, so the choice is exact
-    and the same everywhere; ties to the lower page). Returns pages
+    one of the key head's queries. Both enter as int8 codes, rounded to the
+    nearest: the choice is exact in them and the same everywhere (ties to the
+    lower page), and goes by the keys' true bounds up to half a step of either
+    code, a step being a 127th of the greatest value. Returns pages
     [rows, kv_heads, budget] int32, page ordinals ascending with -1 behind
     them, and counts [rows, kv_heads] int32."""
     bounds._fit(cache)

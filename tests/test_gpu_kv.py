@@ -772,3 +772,40 @@ def test_pools_of_shared_memory_are_not_written(cuda):
     assert torch.equal(pool[3, 1, :, 1], x[0].view(8, 64)[6:]) and torch.equal(pool[2, 1, :, 2], x[1].view(8, 64)[6:])
     assert int((pool != 0).any(-1).sum()) == 8
     both.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize(("group", "d", "ps"), [(1, 128, 16), (4, 64, 32), (8, 80, 8)])
+def test_select_follows_the_unquantised_bounds(cuda, dtype, group, d, ps):
+    """A page that is left out allows no greater product than one that is taken, but for the codes' rounding: half a
+    step of a key's code times the query's size, half a step of the query's times the key's, a quarter of both."""
+    lens = [2000, 1111, 640]
+    gen = torch.Generator().manual_seed(d + group)
+    k, v, table = make_cache(gen, lens, 2, d, ps, dtype)
+    strong = 1.0 + 4.0 * (torch.rand(d, generator=gen) < 0.05)  # a few strong channels, as trained keys have
+    k *= strong.to(dtype).cuda()
+    cache = kv.PagedKV(k, v, table)
+    q = torch.randn((3, 2 * group, d), generator=gen).to(dtype).cuda()
+    bounds = kv.PageBounds.new(cache)
+    kv.page_bounds(cache, bounds, _i32(lens), _i32([0] * 3))
+    budget = 12
+    pages, counts = kv.select_pages(cache, bounds, q, _i32(lens), budget, sinks=1, recent=1)
+    for r, n in enumerate(lens):
+        total = -(-n // ps)
+        keys = tokens(k, table, r, n)
+        for h in range(2):
+            qs = q[r, h * group:(h + 1) * group].double().cpu().numpy()
+            lo = np.stack([keys[h, i * ps:(i + 1) * ps].min(0) for i in range(total)])
+            hi = np.stack([keys[h, i * ps:(i + 1) * ps].max(0) for i in range(total)])
+            allow = np.maximum(qs[:, None] * lo, qs[:, None] * hi).sum(-1).max(0)  # greatest product a key in them can have
+            step = np.maximum(np.abs(lo), np.abs(hi)).max(-1) / 127
+            t = np.abs(qs).max(-1) / 127
+            size = np.maximum(np.abs(lo), np.abs(hi)).sum(-1)
+            off = (0.5 * step * np.abs(qs).sum(-1)[:, None] + 0.5 * t[:, None] * size + 0.25 * d * t[:, None] * step).max(0)
+            off = off * (1 + 2.0 ** -20)  # the steps and the score's two products are rounded to 32 bits
+            taken = [p for p in pages[r, h].tolist() if 0 < p < total - 1]
+            left = [p for p in range(1, total - 1) if p not in taken]
+            assert len(taken) == budget - 2 and counts[r, h].item() == budget
+            assert min(allow[p] + off[p] for p in taken) >= max(allow[p] - off[p] for p in left)
+            assert (allow[taken].mean() - allow[left].mean()) > allow[left].std()  # and they are the better ones
+    cache.check()
