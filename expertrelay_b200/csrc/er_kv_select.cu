@@ -184,9 +184,13 @@ __host__ __device__ inline int cluster_each(int n) { return (n + 4 * kClusterCta
 // by a cluster, whose first CTA chooses, or whose CTAs choose together.
 enum ChooseMode { kAlone, kFirst, kTogether };
 // Few units run as clusters, all at once, and those choose together where
-// there is much to choose from (8 units of 38855 positions: 81 us by a CTA
-// each, 43 together; but 16 of 2501 20 against 28, for every pass of the
-// choice then reads the histograms of 8 CTAs). Otherwise a CTA a unit, unless
+// there is much to choose from: every pass of the choice then reads the
+// histograms of 8 CTAs, which small ones do not repay. (Eviction to 512 of
+// 16 units, by the first CTA and together: of 2048 positions 13.8 and 29.6 us,
+// 4096 16.7 and 29.9, 8192 21.7 and 31.1, 12288 36.5 and 28.3, 16384 41.3 and
+// 29.1, 32768 61.6 and 32.5; 64 pages of one position each, 4 queries a key head:
+// 8192 23.2 and 31.9, 16384 36.3 and 39.7, 32768 71.6 and 56.4. With 4 and 32
+// units eviction crosses at the same place.) Otherwise a CTA a unit, unless
 // its shared memory cannot hold the keys beside `beside` bytes.
 inline int choose_mode(long long units, int n, size_t beside) {
   if (select_bytes(n) + held_bytes(n) + beside > kSelectSmem) return kTogether;
