@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const __grid_cons
 
 // mass[row, h, j] += sum_g 2^(s_gj - lse_g), a thread per position. The scores
 // have just been written and lie in L2; what bounds it is latency (7 us beside
-// the 61 of the rest at 8 rows of up to 16000 positions, 8 key heads of 4
+// the 62 of the rest at 8 rows of up to 16000 positions, 8 key heads of 4
 // queries; four positions of a thread under way at once, or more CTAs, changed
 // nothing). A score a load cost 12 us more with 16 queries (54 rows of up to
 // 6689 positions, 2 key heads: 90 us, 78).
@@ -160,10 +160,11 @@ Layout attend_layout(const er_kv_cache& c, const er_kv_attend_io& io, int sms) {
   // taken while its longest row gives each of those at most 120 KB of keys and
   // values more than a share would be (they take in 25 GB/s each), and all
   // clusters run at once. (One row of 2000 positions, by clusters and by shares:
-  // 8 key heads of 64, bf16 8.5 and 11.7 us; of 128 10.3 and 11.5; 16 of 128, fp32
-  // 18.5 and 16.3. Of 5000: 11.9 and 12.6; 18.1 and 13.3; 35.9 and 28.1.) It
-  // takes two CTAs an SM: with one, 16 clusters of 8 did not all find room in the
-  // processor clusters of 148 SMs, and went in two waves.
+  // 8 key heads of 64, bf16 8.8 and 11.7 us; of 128 10.5 and 11.5; 16 of 128, fp32
+  // 18.5 and 16.3. Of 5000, before bf16 results had weights of three parts: 11.9
+  // and 12.6; 18.1 and 13.3; 35.9 and 28.1.) It takes two CTAs an SM: with one,
+  // 16 clusters of 8 did not all find room in the processor clusters of 148 SMs,
+  // and went in two waves.
   const long long units = (long long)L.rows * c.kv_heads * L.blocks, ctas = L.grid, most = kKvMaxLen;
   const long long room = (io.pages ? (long long)io.max_pages : (long long)c.table_width) * c.page_size;
   const long long bytes = (room < most ? room : most) * 2 * c.head_dim * (c.dtype == ER_DTYPE_BF16 ? 2 : 4);
