@@ -65,8 +65,8 @@ def _apart(shape, stride) -> bool:
 
 
 def _share(a, b) -> bool:
-    """Whether two tensors of as many dimensions may share an element: their extents meet, and they are no
-    two layers of one array."""
+    """Whether two [seqs, heads, n] tensors may share an element: their extents meet, and they are no two
+    layers of one array."""
     (a, b) = sorted((a, b), key=lambda t: t.data_ptr())
     size = a.element_size()
     if not a.numel() or not b.numel():
@@ -76,6 +76,20 @@ def _share(a, b) -> bool:
         return False
     shape = [max(m, n) for m, n in zip(a.shape, b.shape)]
     return a.stride() != b.stride() or not _apart((2, *shape), (apart, *a.stride()))
+
+
+def _meet(apart: int, shape, stride) -> bool:
+    """Whether two tensors of this shape and these strides (_apart), the second `apart` elements on, share a
+    place: whether the distance is a sum of steps, fewer of each dimension than it has elements."""
+    dims = sorted(((s, n) for s, n in zip(stride, shape) if n > 1), reverse=True)
+
+    def steps(left, i):
+        if i == len(dims):
+            return left == 0
+        s, n = dims[i]
+        return any(abs(m) < n and steps(left - m * s, i + 1) for m in {left // s, -(-left // s)})
+
+    return steps(apart, 0)
 
 
 def _weights(t, name: str, cache, rows: int, written: bool) -> None:
@@ -127,7 +141,7 @@ class PagedKV:
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.seqs, self.width = table.shape
         self._apart = _apart(k.shape, k.stride())
-        self._two = not _share(k, v)
+        self._two = self._apart and not _meet((v.data_ptr() - k.data_ptr()) // k.element_size(), k.shape, k.stride())
         if status is not None:
             _need(status, "status", torch.int32, k.device, (1,))
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device) if status is None else status

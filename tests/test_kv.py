@@ -185,7 +185,14 @@ def test_a_sequence_keeps_some_of_its_own_pages():
 
 
 def test_pools_that_share_memory():
-    share = kv._share
+    def share(k, v):
+        assert k.stride() == v.stride() and kv._apart(k.shape, k.stride())
+        got = kv._meet((v.data_ptr() - k.data_ptr()) // k.element_size(), k.shape, k.stride())
+        at = torch.arange(a.numel()).view(a.shape)  # and as counted place by place
+        both = [set(torch.as_strided(at, x.shape, x.stride(), x.storage_offset()).flatten().tolist()) for x in (k, v)]
+        assert got == bool(both[0] & both[1])
+        return got
+
     a = torch.zeros(6 * 2 * 3 * 4 * 8)
     both = a.view(6, 2, 3, 4, 8)  # keys and values of a page side by side
     assert not share(both[:, 0], both[:, 1]) and not share(both[:, 1], both[:, 0])
@@ -194,6 +201,9 @@ def test_pools_that_share_memory():
     assert not share(both[:3, 0], both[3:, 0])
     k = a.view(12, 3, 4, 8)
     assert share(k, k) and share(k[:8], k[4:]) and share(wide[..., :8], wide[..., 4:12])
+    assert not share(k[0:6:2], k[3:9:2]) and share(k[0:6:2], k[4:10:2])  # every other page, from an odd or an even one on
+    assert not share(k[0:9:3], k[1:10:3]) and share(k[3:12:3], k[0:9:3]) and not share(k[:, 2:], k[:, 1:2])
+    assert not share(k[..., 2:3, :], k[..., 0:1, :]) and share(k[..., 1:3, :], k[..., 0:2, :])
 
 
 def test_a_sequence_outside_the_table_is_not_another_one():
