@@ -123,7 +123,27 @@ class KvAttendIO(C.Structure):
     ]
 
 
-KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_SEQ = 1, 2, 4
+class KvTreeIO(C.Structure):
+    """struct er_kv_tree_io."""
+
+    _fields_ = [
+        ("q", _vp),
+        ("q_dtype", _i),
+        ("q_stride", C.c_longlong),
+        ("out", _vp),
+        ("rows", _i),
+        ("heads", _i),
+        ("trees", _i),
+        ("starts", _vp),
+        ("parents", _vp),
+        ("seqs", _vp),
+        ("lens", _vp),
+        ("scale", C.c_float),
+        ("status", _vp),
+    ]
+
+
+KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_SEQ, KV_BAD_TREE = 1, 2, 4, 8
 
 MOE_STAGES = ("router", "plan", "gate_up", "down", "combine")
 
@@ -201,6 +221,12 @@ SIGNATURES: dict[str, tuple] = {
                           _vp, _vp]),
     "er_kv_evict": (_i, [C.POINTER(KvCache), C.POINTER(KvCache), _vp, _vp, C.c_longlong, C.c_longlong, _i, _vp,
                          C.c_longlong, C.c_longlong, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "er_kv_tree_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvTreeIO)]),
+    "er_kv_tree": (_i, [C.POINTER(KvCache), C.POINTER(KvTreeIO), _vp, C.c_size_t, _vp]),
+    "er_kv_copy_pages": (_i, [C.POINTER(KvCache), _i, C.c_longlong, _vp, _vp, _vp, _i, _vp, _vp]),
+    "er_kv_compact": (_i, [C.POINTER(KvCache), _i, C.c_longlong, _vp, _vp, _vp, C.c_longlong, _i, _vp, _i, _vp, _vp, _vp]),
+    "er_beam_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i]),
+    "er_beam_select": (_i, [_vp, _i, C.c_longlong, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "er_trace_record_bytes": (C.c_size_t, [_i, _i]),
     "er_rms_norm": (_i, [_vp, _vp, _vp, C.c_float, _i, _i, _vp, _vp, _vp]),
     "er_rope_kv": (_i, [_vp, C.c_longlong, _vp, _i, _i, _i, _i, _i, C.c_float, _vp, _vp, _i, _vp]),

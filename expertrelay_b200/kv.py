@@ -13,6 +13,10 @@ keys and values of many sequences lie in pages of a pool, in 16 or 32 bits:
                  score best against a query; attend(pages=, counts=) reads
                  only those
   evict          keeps the positions of greatest accumulated weight
+  attend_tree    attention of trees of drafted tokens, each tree's context read
+                 once for all its nodes
+  PagedLayers    all layers' pools; copy_pages (forks of sequences) and compact
+                 (an accepted draft's places moved together), all layers in one launch
 
 All work is queued on the current stream of the cache's device; nothing
 waits on the host. Lengths, positions, tables and lists are read on the
@@ -152,6 +156,7 @@ class PagedKV:
             head_stride=k.stride(1), slot_stride=k.stride(2), table=table.data_ptr(), seqs=self.seqs,
             table_width=self.width, table_stride=table.stride(0))
         self._ref = C.byref(self._c)
+        self._layers, self._layer_stride = 1, 0
         self._needs: dict[tuple, int] = {}  # workspace bytes by the sizes of a call
 
     def _stream(self) -> int:
@@ -172,8 +177,34 @@ class PagedKV:
             self.status.zero_()
             what = [t for b, t in ((_lib.KV_BAD_PAGE, "a page id outside the pool"),
                                    (_lib.KV_BAD_LENGTH, "a length, position or count outside its table"),
-                                   (_lib.KV_BAD_SEQ, "a sequence outside the table")) if bits & b]
+                                   (_lib.KV_BAD_SEQ, "a sequence outside the table"),
+                                   (_lib.KV_BAD_TREE, "a tree's rows or parents out of order")) if bits & b]
             raise ValueError("paged cache: " + ", ".join(what))
+
+
+class PagedLayers:
+    """All layers' caches: k, v [layers, pages, kv_heads, page_size, head_dim],
+    one table for all of them; `layers` has each one's PagedKV. Strides, table
+    and status as for PagedKV."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, status: torch.Tensor | None = None):
+        if k.dim() != 5 or k.shape[0] == 0 or v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError(f"k, v: expected [layers, pages, kv_heads, page_size, head_dim] with strides alike, "
+                             f"got {tuple(k.shape)} by {k.stride()}, {tuple(v.shape)} by {v.stride()}")
+        first = PagedKV(k[0], v[0], table, status)
+        self.layers = [first] + [PagedKV(k[i], v[i], table, first.status) for i in range(1, k.shape[0])]
+        self.k, self.v, self.table, self.status = k, v, table, first.status
+        self.device, self.dtype, self.seqs, self.page_size = first.device, first.dtype, first.seqs, first.page_size
+        self._index, self._ref, self._status = first._index, first._ref, first._status
+        self._layers, self._layer_stride = k.shape[0], k.stride(0)
+        self._apart = _apart(k.shape, k.stride())
+        self._two = self._apart and not _meet((v.data_ptr() - k.data_ptr()) // k.element_size(), k.shape, k.stride())
+
+    _stream, _writable = PagedKV._stream, PagedKV._writable
+
+    def check(self) -> None:
+        """PagedKV.check() of all layers."""
+        self.layers[0].check()
 
 
 class PageBounds:
@@ -391,3 +422,92 @@ def evict(cache: PagedKV, lens: torch.Tensor, mass: torch.Tensor, to: PagedKV, t
                                       kept.data_ptr(), new.data_ptr(), cache._status, cache._stream()),
                "er_kv_evict")
     return kept, new
+
+
+@_on_device
+def attend_tree(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, parents: torch.Tensor, *,
+                seqs: torch.Tensor | None = None, scale: float | None = None, out: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens: tree t's nodes are the rows
+    starts[t] .. starts[t + 1] - 1 of q [rows, heads, head_dim] (as for attend),
+    starts [trees + 1] int32. Node i's key and value lie at place lens[t] + i of
+    sequence seqs[t] (default: t; append with slots= puts them there), and
+    parents [rows] int32 names its parent within the tree, a lower one, or -1
+    for the sequence's last token. It sees the sequence's first lens[t] places,
+    its ancestors and itself: softmax(scale q k^T) v, as attend computes it, but
+    the context's keys and values are read once for all nodes of a tree. At most
+    4096 trees of at most 256 nodes; a chain (each node the next one's parent) is
+    a piece of a text.
+
+    Rows of no tree are left as they were in `out`. scale, workspace: as for attend."""
+    rows, heads, stride = _queries(cache, q)
+    if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] == 0:
+        raise ValueError("starts: expected [trees + 1] int32")
+    trees = starts.shape[0] - 1
+    _need(starts, "starts", torch.int32, cache.device)
+    _need(parents, "parents", torch.int32, cache.device, (rows,))
+    _row_args(cache, trees, lens, seqs)
+    if out is None:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    else:
+        _need(out, "out", q.dtype, cache.device, (rows, heads, cache.head_dim))
+    io = _lib.KvTreeIO(
+        q=q.data_ptr(), q_dtype=_DTYPES[q.dtype], q_stride=stride, out=out.data_ptr(), rows=rows, heads=heads,
+        trees=trees, starts=starts.data_ptr(), parents=parents.data_ptr(),
+        seqs=None if seqs is None else seqs.data_ptr(), lens=lens.data_ptr(),
+        scale=cache.head_dim ** -0.5 if scale is None else float(scale), status=cache._status)
+    if rows == 0 or trees == 0:
+        return out
+    lib, ref = _lib.lib(), C.byref(io)
+    sizes = ("tree", rows, heads, q.dtype, trees)
+    need = cache._needs.get(sizes)
+    if need is None:
+        need = cache._needs[sizes] = lib.er_kv_tree_workspace_bytes(cache._ref, ref)
+    ws = _scratch(need, workspace, cache.device) if need else None
+    _lib.check(lib.er_kv_tree(cache._ref, ref, ws.data_ptr() if need else None, need, cache._stream()), "er_kv_tree")
+    return out
+
+
+@_on_device
+def copy_pages(cache: PagedLayers | PagedKV, src: torch.Tensor, dst: torch.Tensor, *,
+               used: torch.Tensor | None = None) -> None:
+    """The first used[i] slots (default: all) of page src[i] to page dst[i],
+    keys and values of every layer; all [n] int32. A page may be a destination
+    once in a call, and none that is a source. Pairs whose source is negative
+    are passed over, so that a captured call may take fewer than its list's."""
+    if not isinstance(src, torch.Tensor) or src.dim() != 1:
+        raise ValueError("src: expected [n] int32")
+    _need(src, "src", torch.int32, cache.device)
+    _need(dst, "dst", torch.int32, cache.device, src.shape)
+    if used is not None:
+        _need(used, "used", torch.int32, cache.device, src.shape)
+    cache._writable()
+    _lib.check(_lib.lib().er_kv_copy_pages(cache._ref, cache._layers, cache._layer_stride, src.data_ptr(),
+                                           dst.data_ptr(), None if used is None else used.data_ptr(), src.shape[0],
+                                           cache._status, cache._stream()), "er_kv_copy_pages")
+
+
+@_on_device
+def compact(cache: PagedLayers | PagedKV, start: torch.Tensor, keep: torch.Tensor, counts: torch.Tensor, *,
+            seqs: torch.Tensor | None = None) -> torch.Tensor:
+    """Moves places of sequences together in every layer: place start[r] +
+    keep[r, j] of sequence seqs[r] (default: r) goes to place start[r] + j, for
+    j < counts[r]; keep [rows, m] int32 with contiguous rows, each ascending.
+    What lies behind stays as it was. Returns the lengths [rows] int32, start +
+    counts; -1 for a row whose list, length, sequence or pages are bad, which
+    stays unwritten. A sequence may occur once in a call, and its places from
+    start on must lie in pages that no other sequence of it has."""
+    if not isinstance(keep, torch.Tensor) or keep.dim() != 2 or (keep.shape[1] > 1 and keep.stride(1) != 1) or \
+            (keep.shape[0] > 1 and keep.stride(0) < keep.shape[1]):
+        raise ValueError("keep: expected [rows, m] int32 with contiguous rows, apart")
+    _need(keep, "keep", torch.int32, cache.device, contiguous=False)
+    rows, most = keep.shape
+    _row_args(cache, rows, start, seqs, "start")
+    _need(counts, "counts", torch.int32, cache.device, (rows,))
+    cache._writable()
+    lens = start.new_empty(rows)
+    _lib.check(_lib.lib().er_kv_compact(cache._ref, cache._layers, cache._layer_stride,
+                                        None if seqs is None else seqs.data_ptr(), start.data_ptr(), keep.data_ptr(),
+                                        keep.stride(0) if rows > 1 else most, most, counts.data_ptr(), rows,
+                                        lens.data_ptr(), cache._status, cache._stream()), "er_kv_compact")
+    return lens

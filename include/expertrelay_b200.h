@@ -404,6 +404,7 @@ typedef struct er_kv_cache {
 #define ER_KV_BAD_PAGE 1       /* status bits: a page id outside the pool */
 #define ER_KV_BAD_LENGTH 2     /* a length, position or count outside its table */
 #define ER_KV_BAD_SEQ 4        /* a sequence index outside [0, seqs) */
+#define ER_KV_BAD_TREE 8       /* a tree's rows or parents */
 
 /* RoPE and the write of new tokens' rows into the pages: row i of qkv
  * [n, (heads + 2 kv_heads) head_dim] (q | k | v, dtype qkv_dtype, row stride
@@ -491,6 +492,68 @@ ER_API int er_kv_evict(const er_kv_cache* from, const er_kv_cache* to, const int
                        long long mass_seq_stride, long long mass_head_stride, int mass_len, float* to_mass,
                        long long to_mass_seq_stride, long long to_mass_head_stride, int to_mass_len, int budget,
                        int sinks, int recent, int32_t* kept_out, int32_t* lens_out, int* status, void* stream);
+
+/* Attention of trees of drafted tokens: tree t's nodes are the query rows
+ * starts[t] .. starts[t + 1] - 1, node i's key and value lie at place lens[t] + i
+ * of sequence seqs[t] (seqs NULL: t), parents[row] is the node's parent within
+ * its tree (less than the node; -1: the sequence's last token). A node sees the
+ * first lens[t] places, its ancestors and itself:
+ *   out = softmax(scale q k^T) v, in fp32 sums; zeros where every score is -inf.
+ * At most 4096 trees of at most 256 nodes. Rows of no tree stay as they were.
+ * A bad length, sequence, page or parent (ER_KV_BAD_TREE, more than 256 nodes
+ * too) makes the tree's rows NaN; a tree whose rows are not within [0, rows) in
+ * ascending order has none. The workspace is 256-byte aligned. */
+typedef struct er_kv_tree_io {
+  const void* q;               /* [rows, heads, head_dim], row stride q_stride elements */
+  int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */
+  long long q_stride;
+  void* out;                   /* [rows, heads, head_dim] contiguous, 16-byte aligned */
+  int rows, heads;             /* heads <= 65536 */
+  int trees;
+  const int32_t* starts;       /* [trees + 1] */
+  const int32_t* parents;      /* [rows] */
+  const int32_t* seqs;         /* optional [trees] */
+  const int32_t* lens;         /* [trees] */
+  float scale;
+  int* status;                 /* optional */
+} er_kv_tree_io;
+ER_API size_t er_kv_tree_workspace_bytes(const er_kv_cache* cache, const er_kv_tree_io* io);
+ER_API int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* Copies of pages in `layers` pools at once (layer l's pages begin
+ * l * layer_stride elements behind cache->k and cache->v): the first used[i]
+ * slots (used NULL: all) of page src[i] to page dst[i], keys and values. A
+ * page may be dst once in a call, and none that is src; a pair of negative
+ * src is passed over, one with a page outside the pool or used outside
+ * [0, page_size] reported and passed over. */
+ER_API int er_kv_copy_pages(const er_kv_cache* cache, int layers, long long layer_stride, const int32_t* src,
+                            const int32_t* dst, const int32_t* used, int n, int* status, void* stream);
+
+/* Places of sequences moved together in `layers` pools at once: place
+ * start[r] + keep[r * keep_stride + j] of sequence seqs[r] (seqs NULL: r) goes
+ * to place start[r] + j, j < counts[r] <= most; keep ascends, from 0 at the
+ * least. lens_out[r] (optional) = start[r] + counts[r], or -1 where something is
+ * wrong with the row, which then stays as it was. A sequence may occur once in
+ * a call, and the pages that it writes belong to it alone. */
+ER_API int er_kv_compact(const er_kv_cache* cache, int layers, long long layer_stride, const int32_t* seqs,
+                         const int32_t* start, const int32_t* keep, long long keep_stride, int most,
+                         const int32_t* counts, int rows, int32_t* lens_out, int* status, void* stream);
+
+/* ---- beam search ----
+ * Of each batch's beams x vocab candidates, value = scores[batch, beam] +
+ * logits[batch * beams + beam, token] - log(sum over tokens of exp(logits)), the
+ * best `count` in descending order: scores_out, beams_out, tokens_out [batch,
+ * count]. Values are compared in 64 bits (within a beam by the logit), ties go to
+ * the lower beam, then the lower token. Candidates of a beam whose score is NaN
+ * or infinite or whose log-sum is none (a NaN or +inf logit, nothing but -inf),
+ * and logits of -inf, have value -inf. logits ER_DTYPE_F32 / ER_DTYPE_BF16, rows
+ * row_stride elements apart on any element boundary. At most 1024 beams, 65535
+ * rows, count at most 128. The workspace is 256-byte aligned. */
+ER_API size_t er_beam_workspace_bytes(int batch, int beams, int vocab, int count);
+ER_API int er_beam_select(const void* logits, int dtype, long long row_stride, const float* scores, int batch,
+                          int beams, int vocab, int count, float* scores_out, int32_t* beams_out, int32_t* tokens_out,
+                          void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- expert store reads (store/unbuffered_io.py, store/expert_reader.py) ----
  * experts.bin opened for reads that bypass the page cache (O_DIRECT; with

@@ -1,0 +1,226 @@
+"""GPU: attention of trees of drafted tokens against its definition in 64 bits
+(tests/tree_ref.py), at the shapes, lengths, pages and masks where it can go wrong."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+from kv_ref import make_cache
+from tree_ref import check_trees
+
+from expertrelay_b200 import kv
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+TYPES = [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)]
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _tree(rng, n, kind="tree"):
+    if kind == "chain":
+        return list(range(-1, n - 1))
+    if kind == "flat":
+        return [-1] * n
+    return [int(rng.integers(-1, i)) if i else -1 for i in range(n)]
+
+
+def _case(seed, lens, trees, kv_heads, group, d, ps, cache_dtype, q_dtype, layout="hnd"):
+    gen = torch.Generator().manual_seed(seed)
+    k, v, table = make_cache(gen, [n + len(t) for n, t in zip(lens, trees)], kv_heads, d, ps, cache_dtype, layout=layout)
+    rows = sum(len(t) for t in trees)
+    q = torch.randn((rows, kv_heads * group, d), generator=gen).to(q_dtype).cuda()
+    starts = np.concatenate([[0], np.cumsum([len(t) for t in trees])])
+    parents = [p for t in trees for p in t]
+    return kv.PagedKV(k, v, table), q, _i32(lens), _i32(starts.tolist()), _i32(parents)
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("kv_heads", "group", "d", "ps"), [
+    (16, 1, 128, 16), (4, 8, 128, 64), (2, 3, 64, 24), (3, 2, 80, 7), (1, 16, 96, 1), (2, 5, 256, 32), (1, 4, 8, 5),
+    (2, 1, 192, 128), (1, 2, 136, 16), (1, 33, 64, 16),
+])
+def test_trees_match_the_definition(cuda, cache_dtype, q_dtype, kv_heads, group, d, ps):
+    rng = np.random.default_rng(d + group)
+    # empty and short contexts, ends around a tile of 32, 64 and 128 keys, drafts across a tile's and a page's end
+    lens = [0, 0, 1, 31, 33, 60, 64, 100, 127, 128, 333, 1501]
+    sizes = [1, 9, 3, 2, 17, 12, 1, 40, 5, 64, 8, 33]
+    trees = [_tree(rng, n, kind) for n, kind in zip(sizes, ["tree", "chain", "tree", "flat"] * 3)]
+    cache, q, ln, starts, parents = _case(d + group, lens, trees, kv_heads, group, d, ps, cache_dtype, q_dtype)
+    out = kv.attend_tree(cache, q, ln, starts, parents)
+    assert out.dtype == q_dtype and tuple(out.shape) == tuple(q.shape)
+    check_trees(cache, q, lens, trees, out)
+    cache.check()
+    assert torch.equal(out, kv.attend_tree(cache, q, ln, starts, parents))  # bit for bit again
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("length", "nodes", "kv_heads", "group", "d"), [
+    (0, 256, 1, 1, 64), (5000, 1, 2, 4, 128), (640, 8, 16, 1, 128), (20001, 16, 2, 6, 64), (3000, 130, 1, 2, 128),
+    (700, 256, 2, 3, 32), (1200, 70, 1, 4, 256),
+])
+def test_one_tree(cuda, cache_dtype, q_dtype, length, nodes, kv_heads, group, d):
+    tree = _tree(np.random.default_rng(nodes), nodes)
+    cache, q, ln, starts, parents = _case(length, [length], [tree], kv_heads, group, d, 16, cache_dtype, q_dtype)
+    check_trees(cache, q, [length], [tree], kv.attend_tree(cache, q, ln, starts, parents))
+    cache.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_many_uneven_trees(cuda, cache_dtype, q_dtype):
+    rng = np.random.default_rng(3)
+    lens = [int(n) for n in np.exp(rng.uniform(0, 7.5, 70))]
+    trees = [_tree(rng, int(n)) for n in np.exp(rng.uniform(0, 3.5, 70))]
+    cache, q, ln, starts, parents = _case(9, lens, trees, 2, 2, 64, 32, cache_dtype, q_dtype)
+    check_trees(cache, q, lens, trees, kv.attend_tree(cache, q, ln, starts, parents))
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize("layout", ["nhd", "wide"])
+def test_strides_scales_and_rows_of_no_tree(cuda, cache_dtype, q_dtype, layout):
+    rng = np.random.default_rng(5)
+    lens, trees = [200, 0, 77], [_tree(rng, 11), _tree(rng, 4), _tree(rng, 30)]
+    cache, q, _, _, parents = _case(5, lens, trees, 3, 2, 64, 16, cache_dtype, q_dtype, layout=layout)
+    order = [2, 0, 1]
+    rows = q.shape[0]
+    wide = torch.randn((rows + 7, 6 * 64 + 40), device="cuda").to(q_dtype)
+    wide[3:3 + rows, 8:8 + 6 * 64] = q.reshape(rows, -1)
+    qs = wide[:, 8:8 + 6 * 64].view(rows + 7, 6, 64)
+    out = torch.full((rows + 7, 6, 64), 7.0, dtype=q_dtype, device="cuda")
+    # the trees begin behind three rows of no tree, four follow; sequences in another order
+    starts = _i32([3, 14, 18, 48])
+    tables = torch.full((3, cache.width + 3), -7, dtype=torch.int32, device="cuda")
+    tables[order, :cache.width] = cache.table
+    other = kv.PagedKV(cache.k, cache.v, tables[:, :cache.width])
+    more = torch.cat([_i32([-9, -9, 500]), parents, _i32([3, 3, 3, 3])])
+    assert kv.attend_tree(other, qs, _i32(lens), starts, more, seqs=_i32(order), scale=0.3, out=out) is out
+    check_trees(other, qs, lens, trees, out, first=3, seqs=order, scale=0.3)
+    assert torch.all(out[:3] == 7.0) and torch.all(out[3 + rows:] == 7.0)
+    other.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_masked_places_change_nothing(cuda, cache_dtype, q_dtype):
+    """NaN and infinite keys and values of nodes that a node does not see; scores of -inf."""
+    lens, tree = [150], [-1, 0, 0, 1, 2, -1, 5]
+    cache, q, ln, starts, parents = _case(7, lens, [tree], 2, 3, 64, 16, cache_dtype, q_dtype)
+    want = kv.attend_tree(cache, q, ln, starts, parents)
+    for node, key, value in ((5, float("nan"), float("nan")), (2, float("inf"), float("-inf")), (1, 1.0, float("inf"))):
+        place = lens[0] + node
+        page = int(cache.table[0, place // 16])
+        was = cache.k[page, :, place % 16].clone(), cache.v[page, :, place % 16].clone()
+        cache.k[page, :, place % 16], cache.v[page, :, place % 16] = key, value
+        got = kv.attend_tree(cache, q, ln, starts, parents)
+        blind = [i for i, p in enumerate(tree) if i != node and p != node and (p < 0 or tree[p] != node)]
+        assert torch.equal(got[blind], want[blind])
+        assert not torch.isfinite(got[node]).any()
+        cache.k[page, :, place % 16], cache.v[page, :, place % 16] = was
+    # no context, and a node whose own key scores -inf: nothing is left of the row
+    cache, q, ln, starts, parents = _case(8, [0], [[-1]], 1, 1, 64, 16, cache_dtype, q_dtype)
+    q.fill_(1.0)
+    cache.k[int(cache.table[0, 0]), :, 0] = float("-inf")
+    out = kv.attend_tree(cache, q, ln, starts, parents)
+    assert torch.all(out == 0) or (cache_dtype == F32 and torch.isnan(out).all())
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_bad_trees_spoil_their_own_rows(cuda, cache_dtype, q_dtype):
+    rng = np.random.default_rng(1)
+    lens, trees = [300, 40, 77, 20], [_tree(rng, 6), _tree(rng, 5), _tree(rng, 7), _tree(rng, 4)]
+    cache, q, ln, starts, parents = _case(11, lens, trees, 2, 2, 64, 16, cache_dtype, q_dtype)
+    want = kv.attend_tree(cache, q, ln, starts, parents)
+    rows = slice(6, 11)
+    others = [i for i in range(22) if not 6 <= i < 11]
+
+    def spoilt(words, cache=cache, ln=ln, parents=parents, starts=starts, seqs=None):
+        got = kv.attend_tree(cache, q, ln, starts, parents, seqs=seqs)
+        assert torch.isnan(got[rows]).all() and torch.equal(got[others], want[others])
+        with pytest.raises(ValueError, match=words):
+            cache.check()
+        cache.check()
+
+    for bad in (4, 7, -2, 2**31 - 1, -2**31):
+        p = parents.clone()
+        p[6 + 4] = bad
+        spoilt("tree", parents=p)
+    for bad in (-1, cache.width * 16, 2**31 - 1):
+        n = ln.clone()
+        n[1] = bad
+        spoilt("length", ln=n)
+    for bad in (-1, 4, 2**31 - 1):
+        spoilt("sequence", seqs=_i32([0, bad, 2, 3]))
+    for bad, page in ((-1, 0), (cache.num_pages, 2), (2**31 - 1, 2)):
+        table = cache.table.clone()
+        table[1, page] = bad
+        spoilt("page", cache=kv.PagedKV(cache.k, cache.v, table))
+    # rows outside the queries or descending: the tree has none, its rows are left
+    for bad in ([0, 6, 5, 18, 22], [0, 6, 30, 18, 22], [0, -6, 11, 18, 22]):
+        out = torch.full_like(q, 3.0)
+        kv.attend_tree(cache, q, ln, _i32(bad), parents, out=out)
+        assert torch.equal(out[18:], want[18:])
+        with pytest.raises(ValueError, match="tree"):
+            cache.check()
+
+
+def test_too_many_nodes(cuda):
+    tree = list(range(-1, 256))  # 257
+    cache, q, ln, starts, parents = _case(2, [10], [tree], 1, 1, 64, 16, BF16, BF16)
+    assert torch.isnan(kv.attend_tree(cache, q, ln, starts, parents)).all()
+    with pytest.raises(ValueError, match="tree"):
+        cache.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_captured_calls_follow_their_tensors(cuda, cache_dtype, q_dtype):
+    """One graph, replayed over other lengths, trees and tables; two graphs of one cache; another stream."""
+    rng = np.random.default_rng(2)
+    lens, trees = [300, 5, 700], [_tree(rng, 8) for _ in range(3)]
+    cache, q, ln, starts, parents = _case(4, lens, trees, 2, 4, 128, 16, cache_dtype, q_dtype)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kv.attend_tree(cache, q, ln, starts, parents)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(kv.attend_tree(cache, q, ln, starts, parents))
+        graphs.append(g)
+    for lens, sizes in (([10, 705, 0], [1, 20, 3]), ([300, 5, 700], [8, 8, 8]), ([0, 0, 3], [2, 2, 2])):
+        trees = [_tree(rng, n) for n in sizes]
+        lens = [min(n, 13 * 16 - m if t == 1 else n) for t, (n, m) in enumerate(zip(lens, sizes))]
+        lens = [min(n, (int((cache.table[t] >= 0).sum()) * 16) - m) for t, (n, m) in enumerate(zip(lens, sizes))]
+        trees = [t if n >= 0 else [-1] for t, n in zip(trees, lens)]
+        lens = [max(n, 0) for n in lens]
+        ln.copy_(_i32(lens))
+        starts.copy_(_i32(np.concatenate([[0], np.cumsum([len(t) for t in trees])]).tolist()))
+        flat = [p for t in trees for p in t]
+        parents[:len(flat)] = _i32(flat)
+        # every slot that these lengths reach holds something
+        cache.k.nan_to_num_(nan=0.25)
+        cache.v.nan_to_num_(nan=0.5)
+        for g, out in zip(graphs, outs):
+            out.zero_()
+            g.replay()
+            check_trees(cache, q, lens, trees, out)
+    cache.check()
+
+
+def test_refusals(cuda):
+    cache, q, ln, starts, parents = _case(2, [10], [[-1, 0]], 2, 2, 64, 16, BF16, BF16)
+    for change, words in (({"lens": ln.long()}, "lens"), ({"lens": _i32([1, 2])}, "lens"), ({"starts": starts[:0]}, "starts"),
+                          ({"starts": starts.float()}, "starts"), ({"starts": None}, "starts"), ({"parents": parents[:1]}, "parents"),
+                          ({"q": q.half()}, "q:"), ({"q": q[:, :3]}, "heads"), ({"seqs": starts}, "seqs"),
+                          ({"out": q[:1].clone()}, "out")):
+        args = {"q": q, "lens": ln, "starts": starts, "parents": parents, **change}
+        with pytest.raises(ValueError, match=words):
+            kv.attend_tree(cache, args.pop("q"), args.pop("lens"), args.pop("starts"), args.pop("parents"), **args)
+    with pytest.raises(ValueError, match="seqs"):
+        kv.attend_tree(cache, q, _i32([1, 1]), _i32([0, 1, 2]), parents)
+    assert kv.attend_tree(cache, q, ln[:0], starts[:1], parents).shape == q.shape
+    assert kv.attend_tree(cache, q[:0], _i32([0]), _i32([0, 0]), parents[:0]).shape == (0, 4, 64)
