@@ -143,7 +143,7 @@ class KvTreeIO(C.Structure):
     ]
 
 
-KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_SEQ, KV_BAD_TREE = 1, 2, 4, 8
+KV_BAD_PAGE, KV_BAD_LENGTH, KV_BAD_SEQ, KV_BAD_TREE, KV_GAVE_UP = 1, 2, 4, 8, 16
 
 MOE_STAGES = ("router", "plan", "gate_up", "down", "combine")
 

@@ -1,91 +1,62 @@
 // er_kv_tree.cu -- attention of a tree of drafted tokens over a paged cache.
-#include "er_kv_attend.cuh"
 #include "er_kv_tree.cuh"
+#include "er_ptx.cuh"
 
 namespace er {
 
 namespace {
 
-// A CTA a (node, head): its warps take every fourth key.
-template <typename TC, typename TQ>
-__global__ void __launch_bounds__(128) kv_tree_simple_kernel(const __grid_constant__ TreeArgs a) {
+// Joins the units that several CTAs share: a warp a query row, the rows of the
+// unit that begins in CTA blockIdx.x's run. Also writes the rows of trees that
+// something is wrong with, which no attention CTA meets.
+constexpr int kJoinWarps = 8;
+
+template <typename TQ>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv_tree_join_kernel(const __grid_constant__ TreeArgs a) {
   kv_enter();
-  __shared__ float part[4][2 + 256];
-  __shared__ int find[2], bad_page;
-  const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
-  if (threadIdx.x == 0) find[0] = -1, bad_page = 0;
-  __syncthreads();
-  for (int t = threadIdx.x; t < a.trees; t += 128) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
+  for (int t = blockIdx.y * a.grid + blockIdx.x; t < a.trees; t += a.grid * gridDim.y) {
     const Tree e = kv_tree(a, t);
-    if (e.bad && blockIdx.x == 0 && blockIdx.y == 0) kv_report(a.status, e.bad);
-    if (row >= e.first && row < e.first + e.nodes) find[0] = t;
+    if (!e.bad) continue;
+    TQ* out = (TQ*)a.out + (long long)e.first * a.heads * d;
+    for (long long i = threadIdx.x; i < (long long)e.nodes * a.heads * d; i += kJoinWarps * 32)
+      out[i] = kv_round<TQ>(__int_as_float(0x7fc00000));
   }
-  __syncthreads();
-  if (find[0] < 0) return;
-  const Tree e = kv_tree(a, find[0]);
-  int bad = e.bad;
-  if (!bad) {
-    for (int i = threadIdx.x; i < e.nodes; i += 128) {
-      const int p = a.parents[e.first + i];
-      if (p < -1 || p >= i) bad = ER_KV_BAD_TREE;
+  const TreeCut c = a.cut[blockIdx.x];
+  if (c.live == 0) return;
+  const int shares = tree_shares(a, c.total), i0 = blockIdx.x;
+  const int n = kv_share_of(c.total, shares, c.begin + kTreeCost + c.tiles - 1) - i0 + 1;  // pieces
+  for (int r = blockIdx.y * kJoinWarps + warp; r < c.live; r += gridDim.y * kJoinWarps) {
+    auto at = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * a.piece_rows + r; };
+    float top = -INFINITY;
+    for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[at(k) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int width = min(a.channels, d - c.ch0);
+    const bool mine = lane * 4 < width;
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (k0 + j >= n) continue;
+        ml[j] = *reinterpret_cast<const float2*>(a.part_ml + at(k0 + j) * 2);
+        if (mine) x[j] = *reinterpret_cast<const float4*>(a.part_o + at(k0 + j) * a.channels + lane * 4);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (k0 + j >= n) continue;
+        const float by = piece_weight(ml[j].x, top);
+        sum = fmaf(ml[j].y, by, sum);  // a spoilt piece's sum is NaN
+        if (mine) fma4(acc, x[j], by);
+      }
     }
-  }
-  if (bad) kv_report(a.status, bad);
-  bad = __syncthreads_or(bad);
-  TQ* out = (TQ*)a.out + ((long long)row * a.heads + head) * d;
-  if (bad) {
-    for (int c = threadIdx.x; c < d; c += 128) out[c] = kv_round<TQ>(__int_as_float(0x7fc00000));
-    return;
-  }
-  const TQ* q = (const TQ*)a.q + (long long)row * a.q_stride + (long long)head * d;
-  const int h = head / a.group, node = row - e.first;
-  float x[8], o[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    x[j] = lane + 32 * j < d ? to_f32(q[lane + 32 * j]) * a.scale : 0.f;
-    o[j] = 0.f;
-  }
-  const int32_t* pages = a.kv.pages_of(e.seq);
-  for (int j = warp; j < e.len + e.nodes; j += 4) {
-    const int pg = pages[a.kv.ordinal(j)];
-    if (pg < 0 || pg >= a.kv.num_pages) {
-      bad_page = 1;
-      continue;
-    }
-    if (j >= e.len) {
-      int at = node;
-      while (at > j - e.len) at = a.parents[e.first + at];
-      if (at != j - e.len) continue;
-    }
-    const long long off = pg * a.kv.page_stride + h * a.kv.head_stride + a.kv.slot(j) * a.kv.slot_stride;
-    const TC *k = (const TC*)(a.kv.k + off), *v = (const TC*)(a.kv.v + off);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < d) s = fmaf(x[i], to_f32(k[lane + 32 * i]), s);
-    s = warp_sum(s);
-    if (s == -INFINITY) continue;
-    const float top = fmaxf(m, s), by = piece_weight(m, top), p = exp2f(s - top);
-    m = top;
-    l = l * by + p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < d) o[i] = o[i] * by + p * to_f32(v[lane + 32 * i]);
-  }
-  if (lane == 0) part[warp][0] = m, part[warp][1] = l;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < d) part[warp][2 + lane + 32 * i] = o[i];
-  __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][0]);
-  for (int w = 0; w < 4; ++w) sum += part[w][1] * piece_weight(part[w][0], top);
-  if (bad_page && threadIdx.x == 0) kv_report(a.status, ER_KV_BAD_PAGE);
-  for (int c = threadIdx.x; c < d; c += 128) {
-    float v = 0.f;
-    for (int w = 0; w < 4; ++w) v += part[w][2 + c] * piece_weight(part[w][0], top);
-    v = sum == 0.f ? 0.f : v / sum;
-    out[c] = kv_round<TQ>(bad_page ? __int_as_float(0x7fc00000) : v);
+    const int q = c.q0 + r, node = q / a.group, g = q - node * a.group;
+    if (mine)
+      kv_store4((TQ*)a.out + ((long long)(c.first + node) * a.heads + c.head * a.group + g) * d + c.ch0 + lane * 4, acc, sum);
   }
 }
 
@@ -109,29 +80,106 @@ int tree_check(const er_kv_cache* c, const er_kv_tree_io* io) {
 
 using namespace er;
 
+namespace {
+
+struct TreeLayout {
+  TreeLaunch shape;
+  int piece_rows;
+  size_t cut, ml, o, bytes;
+};
+
+TreeLayout tree_layout(const er_kv_cache& c, const er_kv_tree_io& io, int sms) {
+  TreeLayout L;
+  const int group = io.heads / c.kv_heads;
+  L.shape = c.dtype == ER_DTYPE_BF16 ? tree_shape_bf16(c.head_dim, io.q_dtype) : tree_shape_f32(c.head_dim);
+  const long long rows = (long long)(io.rows < kMaxNodes ? io.rows : kMaxNodes) * group;
+  L.piece_rows = rows < L.shape.rows ? (int)rows : L.shape.rows;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align_up(bytes, 256);
+    return here;
+  };
+  const size_t n = (size_t)sms * 2 * L.piece_rows;
+  L.cut = take(sms * sizeof(TreeCut));
+  L.ml = take(n * 8);
+  L.o = take(n * L.shape.channels * 4);
+  L.bytes = at;
+  return L;
+}
+
+// Pages of a bf16 pool as copies see them: channels, positions, key heads, pages; boxes of 64 channels.
+int tree_map(CUtensorMap* m, const er_kv_cache& c, void* pool, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(ER_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads, (cuuint64_t)c.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+  for (int i = 0; i < 3; ++i)
+    if (dims[i + 1] == 1) strides[i] = (cuuint64_t)c.head_dim * 2;  // never used
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, each[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims, strides, box, each,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(ER_EINVAL, "er_kv_tree: pools of strides %lld, %lld, %lld cannot be copied by tiles (%d)", c.page_stride,
+                c.head_stride, c.slot_stride, (int)r);
+  return ER_OK;
+}
+
+}  // namespace
+
 extern "C" size_t er_kv_tree_workspace_bytes(const er_kv_cache* cache, const er_kv_tree_io* io) {
-  if (tree_check(cache, io)) return 0;
-  return 0;
+  int sms = 0;
+  if (tree_check(cache, io) || io->rows == 0 || io->trees == 0 || device_sms(&sms)) return 0;
+  return tree_layout(*cache, *io, sms).bytes;
 }
 
 extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, void* workspace, size_t workspace_bytes,
                           void* stream) {
-  (void)workspace, (void)workspace_bytes;
   if (int rc = tree_check(cache, io)) return rc;
   if (io->rows == 0 || io->trees == 0) return ER_OK;
   if (!io->q || !io->out || !io->lens || !io->starts || !io->parents)
     return fail(ER_EINVAL, "er_kv_tree: null pointer");
   if ((uintptr_t)io->out & 15) return fail(ER_EINVAL, "er_kv_tree: out must be 16-byte aligned");
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  const TreeLayout L = tree_layout(*cache, *io, sms);
+  if (!workspace || workspace_bytes < L.bytes)
+    return fail(ER_ENOSPACE, "er_kv_tree: workspace %zu bytes, need %zu", workspace_bytes, L.bytes);
+  if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_kv_tree: workspace must be 256-byte aligned");
+  cudaStream_t st = (cudaStream_t)stream;
+  char* ws = (char*)workspace;
   TreeArgs a = {};
   a.kv = kv_view(*cache);
   a.q = io->q, a.q_stride = io->q_stride, a.out = io->out;
   a.rows = io->rows, a.heads = io->heads, a.group = io->heads / cache->kv_heads, a.trees = io->trees;
   a.starts = io->starts, a.parents = io->parents, a.seqs = io->seqs, a.lens = io->lens;
-  a.scale = io->scale * 1.4426950408889634f;
+  // positive in the kernel, so that the greatest product has the greatest score
+  a.q_flip = io->scale < 0.f, a.q_zero = io->scale == 0.f;
+  a.scale = (a.q_zero ? 1.f : a.q_flip ? -io->scale : io->scale) * 1.4426950408889634f;
   a.status = io->status;
   using bf = __nv_bfloat16;
   const bool qb = io->q_dtype == ER_DTYPE_BF16, cb = cache->dtype == ER_DTYPE_BF16;
-  auto kernel = cb ? (qb ? kv_tree_simple_kernel<bf, bf> : kv_tree_simple_kernel<bf, float>)
-                   : (qb ? kv_tree_simple_kernel<float, bf> : kv_tree_simple_kernel<float, float>);
-  return kv_launch(kernel, dim3(io->rows, io->heads), 128, 0, false, (cudaStream_t)stream, "kv_tree_kernel", a);
+  const long long qs = qb ? 2 : 4;
+  a.q_wide = (((uintptr_t)io->q | (uintptr_t)(io->q_stride * qs)) & 15) == 0;
+  a.grid = sms;
+  a.piece_rows = L.piece_rows;
+  a.cut = (TreeCut*)(ws + L.cut);
+  a.part_ml = (float*)(ws + L.ml);
+  a.part_o = (float*)(ws + L.o);
+  a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
+  int box = kTreeTile;
+  while (cache->page_size % box) box >>= 1;
+  a.box_rows = box;
+  if (cb) {
+    CUtensorMap maps[2];
+    if (int rc = tree_map(&maps[0], *cache, cache->k, box)) return rc;
+    if (int rc = tree_map(&maps[1], *cache, cache->v, box)) return rc;
+    if (int rc = tree_bf16(a, io->q_dtype, maps, st)) return rc;
+  } else if (int rc = tree_f32(a, io->q_dtype, st)) {
+    return rc;
+  }
+  const dim3 grid(sms, (L.piece_rows + kJoinWarps - 1) / kJoinWarps);
+  return qb ? kv_launch(kv_tree_join_kernel<bf>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a)
+            : kv_launch(kv_tree_join_kernel<float>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a);
 }

@@ -1,0 +1,31 @@
+// er_kv_tree_bf16.cu -- tree attention over bf16 caches.
+#include "er_kv_tree_mma.cuh"
+
+namespace er {
+
+namespace {
+using bf = __nv_bfloat16;
+using B64 = TreeShape<1, 1, 2, 64, 128, 6>;
+using B128 = TreeShape<1, 1, 2, 128, 128, 4>;
+using B256 = TreeShape<1, 1, 2, 256, 128, 2>;
+using F64 = TreeShape<1, 3, 3, 64, 128, 6>;
+using F128 = TreeShape<1, 3, 3, 128, 128, 3>;
+using F256 = TreeShape<1, 3, 3, 256, 64, 2>;
+}  // namespace
+
+TreeLaunch tree_shape_bf16(int d, int q_dtype) {
+  return TreeLaunch{d > 128 && q_dtype == ER_DTYPE_F32 ? F256::ROWS : kTreeRows, d <= 64 ? 64 : kTreeChannels, d > 128 ? 2 : 1};
+}
+
+int tree_bf16(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st) {
+  const int d = a.kv.d;
+  if (q_dtype == ER_DTYPE_BF16)
+    return d <= 64    ? tree_launch<B64, bf, bf>(a, maps, st)
+           : d <= 128 ? tree_launch<B128, bf, bf>(a, maps, st)
+                      : tree_launch<B256, bf, bf>(a, maps, st);
+  return d <= 64    ? tree_launch<F64, bf, float>(a, maps, st)
+         : d <= 128 ? tree_launch<F128, bf, float>(a, maps, st)
+                    : tree_launch<F256, bf, float>(a, maps, st);
+}
+
+}  // namespace er

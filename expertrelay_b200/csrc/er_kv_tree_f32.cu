@@ -1,0 +1,29 @@
+// er_kv_tree_f32.cu -- tree attention over fp32 caches.
+#include "er_kv_tree_mma.cuh"
+
+namespace er {
+
+namespace {
+using S64 = TreeShape<3, 3, 3, 64, 128, 2>;
+using S128 = TreeShape<3, 3, 3, 128, 128, 1>;
+using S256 = TreeShape<3, 3, 3, 256, 32, 1>;
+
+template <typename TQ>
+int launch(const TreeArgs& a, cudaStream_t st) {
+  const CUtensorMap none[2] = {};
+  const int d = a.kv.d;
+  return d <= 64    ? tree_launch<S64, float, TQ>(a, none, st)
+         : d <= 128 ? tree_launch<S128, float, TQ>(a, none, st)
+                    : tree_launch<S256, float, TQ>(a, none, st);
+}
+}  // namespace
+
+TreeLaunch tree_shape_f32(int d) {
+  return TreeLaunch{d > 128 ? S256::ROWS : kTreeRows, d <= 64 ? 64 : kTreeChannels, d > 128 ? 2 : 1};
+}
+
+int tree_f32(const TreeArgs& a, int q_dtype, cudaStream_t st) {
+  return q_dtype == ER_DTYPE_BF16 ? launch<__nv_bfloat16>(a, st) : launch<float>(a, st);
+}
+
+}  // namespace er

@@ -1,0 +1,799 @@
+// er_kv_tree_mma.cuh -- tree attention on the tensor cores (tcgen05).
+#pragma once
+
+#include <type_traits>
+
+#include "er_kv_tree.cuh"
+#include "er_ptx.cuh"
+
+namespace er {
+
+namespace {
+
+constexpr int kSoftmaxWarps = 4, kSumWarps = 8, kIssueWarp = kSoftmaxWarps + kSumWarps;
+constexpr int kStagePitch = 36;  // floats of a row of the epilogue's exchange: 2 x 16 channels and 4 of padding
+
+// KP: bf16 parts of a key or value in shared memory (1: as they come from a bf16 cache, 3: of fp32), QP of a query,
+// PP of a weight. DP: head_dim padded. ROWS: rows of queries in shared memory (of 128 of a product; the others are
+// whatever lies there). PAIRS: stages, each a tile of keys and one of VD channels of values.
+template <int KP_, int QP_, int PP_, int DP_, int ROWS_, int PAIRS_>
+struct TreeShape {
+  static constexpr int KP = KP_, QP = QP_, PP = PP_, DP = DP_, ROWS = ROWS_, SLOTS = 2 * PAIRS_;
+  static constexpr int VD = DP < kTreeChannels ? DP : kTreeChannels;
+  static constexpr int kKPart = kTreeTile * DP * 2, kVPart = kTreeTile * VD * 2;  // bytes of one part of a tile
+  static constexpr int kPair = (kKPart + kVPart) * KP;
+  static constexpr int kQPart = ROWS * DP * 2, kQ = kQPart * QP;
+  static constexpr int kSP = PP * 32 > 64 ? PP * 32 : 64;  // columns of a tile's scores, then of its weights
+  static constexpr int kSmem = kQ + PAIRS_ * kPair + ROWS * kStagePitch * 4;
+  // warps that fill shared memory: of a bf16 cache one that issues copies and two that look after the drafted
+  // values, of an fp32 cache all of them by way of registers
+  static constexpr int kLoadWarps = KP == 1 ? 3 : 7, kFixWarps = KP == 1 ? 2 : 7;
+  static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
+  static __device__ __forceinline__ uint32_t slot(uint32_t base, int i) {
+    return base + (i >> 1) * kPair + (i & 1) * kKPart * KP;
+  }
+};
+
+template <typename S>
+struct TreeShared {
+  uint64_t full[S::SLOTS], empty[S::SLOTS], raw[S::SLOTS];
+  uint64_t qfirst, qfull, qfree, sfull[2], pfull[2], ofull[2], ofree[2], staged, masked, drain;
+  uint32_t tmem;
+  volatile int abort;
+  TreeRun run;
+  TreeScratch scratch;
+  int bad_tree[2], parents[2][kMaxNodes];  // of units in turn: a warp may be one ahead of another
+  int bad_unit[16];                 // units (numbers + 1) of a bad page, in turn
+  uint32_t sees[S::ROWS][9];        // each row's ancestors and itself, a bit a node
+  uint32_t vbad[S::SLOTS][S::kFixWarps][2];  // keys of a slot whose value was no number (drafted ones)
+  float by[4][S::ROWS];             // what a tile's sums so far are multiplied by
+  float2 ml[4][S::ROWS];            // maximum and sum of a unit's last tile
+};
+
+// Descriptors of operands in shared memory, 128-byte swizzle, eight-row groups 1024 bytes apart: the upper word is
+// the same for all, the lower one (address, and for operands whose N is contiguous the distance `lbo` of the next 64
+// elements) is put together where the product is issued.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return (addr & 0x3FFFFu) >> 4 | (lbo >> 4) << 16; }
+
+// d (+)= A B, A and B in shared memory, or A in tensor memory
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
+      : "memory");
+}
+// bf16 operands, fp32 sums, M = 128; b_mn: B's rows (N) are contiguous, not its K
+__device__ __forceinline__ uint32_t idesc_bf16(int n, int b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void async_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// two floats rounded to bf16, packed, the first one low; x, y become what is left
+__device__ __forceinline__ uint32_t split2(float& x, float& y) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  x -= __uint_as_float(r << 16);
+  y -= __uint_as_float(r & 0xffff0000u);
+  return r;
+}
+// Eight floats as three bf16 parts, cut, whose sum they are exactly. A part that is zero where the value is not
+// takes the least value of its sign: times an infinite key it stays infinite, beside a finite one it vanishes.
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[3]) {
+  uint32_t p[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = __float_as_uint(x[j]), tiny = b >> 31 << 15 | 1u;
+    const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+    p[0][j] = x[j] != x[j] ? 0x7fc0u : b >> 16;
+    float rest = finite ? x[j] - __uint_as_float(b & 0xffff0000u) : 0.f;
+    p[1][j] = __float_as_uint(rest) >> 16;
+    rest -= __uint_as_float(p[1][j] << 16);
+    p[2][j] = __float_as_uint(rest) >> 16;
+    if (x[j] != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if ((p[i][j] & 0x7fffu) == 0) p[i][j] = tiny;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    out[i] = make_uint4(p[i][0] | p[i][1] << 16, p[i][2] | p[i][3] << 16, p[i][4] | p[i][5] << 16, p[i][6] | p[i][7] << 16);
+}
+
+// Bits of nodes node0 .. node0 + 31 that a row sees; below 0 lies the context, all of which it sees.
+__device__ __forceinline__ uint32_t seen_from(const uint32_t* sees, int node0) {
+  if (node0 <= -32) return 0xffffffffu;
+  if (node0 < 0) return sees[0] << -node0 | ((1u << -node0) - 1);
+  const int w = node0 >> 5;
+  return __funnelshift_r(w < 8 ? sees[w] : 0u, w < 7 ? sees[w + 1] : 0u, node0 & 31);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int slot, int head,
+                                        int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(slot), "r"(head), "r"(page)
+      : "memory");
+}
+
+// Where 16-byte vector c (8 channels) of row r lies in a tile of `rows` rows: 64 channels to a 128-byte line, the
+// lines' vectors exchanged by the row (the 128-byte swizzle)
+__device__ __forceinline__ uint32_t swizzled(int c, int r, int rows) {
+  return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// Eight elements at src as 32-bit floats; `wide`: src lies on a 16-byte boundary.
+__device__ __forceinline__ void load8(const float* src, bool wide, float (&x)[8]) {
+  if (wide) {
+    const float4 u = load4(src), v = load4(src + 4);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = src[j];
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* src, bool wide, float (&x)[8]) {
+  if (wide) {
+    const uint4 u = *reinterpret_cast<const uint4*>(src);
+    const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[2 * j] = __uint_as_float(h[j] << 16), x[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = to_f32(src[j]);
+  }
+}
+
+// A unit's queries into shared memory, by `warps` warps of which this is one: eight lanes take 64 channels of a
+// query, which is row qi of every replica.
+template <typename S, typename TQ>
+__device__ __forceinline__ void load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps) {
+  const int lane = threadIdx.x & 31, d = a.kv.d, chunks = (d + 63) / 64, R = w.replicas(), per = S::ROWS / R;
+  const int items = (w.live + 3) / 4 * chunks;  // of four queries
+#pragma unroll 2
+  for (int i = warp; i < items; i += warps) {
+    const int g = i / chunks, qi = g * 4 + lane / 8, c = (i - g * chunks) * 8 + (lane & 7);
+    if (qi >= w.live || c * 8 >= (d + 15) / 16 * 16) continue;
+    const int q = w.q0 + qi, node = q / a.group;
+    float x[8] = {};
+    if (c * 8 < d && !a.q_zero)
+      load8((const TQ*)a.q + (long long)(w.e.first + node) * a.q_stride + (long long)(w.head * a.group + q - node * a.group) * d +
+                c * 8,
+            a.q_wide, x);
+    if (a.q_flip) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = -x[j];
+    }
+    uint4 parts[3];
+    if constexpr (S::QP == 1) {  // bf16 as they are
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = __byte_perm(__float_as_uint(x[2 * j]), __float_as_uint(x[2 * j + 1]), 0x7632);
+      parts[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+      split8(x, parts);
+    }
+    for (int r = 0; r < R; ++r) {
+      const uint32_t to = q0 + swizzled(c, r * per + qi, S::ROWS);
+#pragma unroll
+      for (int p = 0; p < S::QP; ++p) sts16(to + p * S::kQPart, parts[p]);
+    }
+  }
+  __syncwarp();
+  async_fence();
+  __syncwarp();
+}
+
+template <typename S, typename TC, typename TQ>
+__global__ void __launch_bounds__(S::kThreads, 1)
+    kv_tree_kernel(const __grid_constant__ TreeArgs a, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ unsigned char raw[];
+  __shared__ TreeShared<S> s;
+  constexpr int TK = kTreeTile, SLOTS = S::SLOTS;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.kv.d;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;  // swizzled tiles repeat every 1024 bytes
+  // the queries first: products read 128 rows from there, whatever lies behind S::ROWS
+  const uint32_t q0 = base, slots0 = base + S::kQ;
+  float* stage = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kQ + SLOTS / 2 * S::kPair);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&s.full[i], S::kFixWarps);
+      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.raw[i], 1);
+    }
+    mbar_init(&s.qfirst, kIssueWarp);
+    mbar_init(&s.qfull, S::kFixWarps);
+    mbar_init(&s.qfree, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.sfull[i], 1);
+      mbar_init(&s.pfull[i], kSoftmaxWarps);
+      mbar_init(&s.ofull[i], 1);
+      mbar_init(&s.ofree[i], kSumWarps);
+    }
+    mbar_init(&s.staged, kSumWarps);
+    mbar_init(&s.masked, kSoftmaxWarps);
+    mbar_init(&s.drain, 1);
+    s.abort = 0;
+    s.bad_tree[0] = s.bad_tree[1] = 0;
+    for (int i = 0; i < 16; ++i) s.bad_unit[i] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kIssueWarp) tmem_alloc<1>(&s.tmem, 512);
+  kv_enter();
+  tree_run(a, s.run, s.scratch);  // all threads; ends with a barrier
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  const unsigned long long limit = kDefaultWaitNs;
+  auto wait = [&](uint64_t* bar, int parity) { return warp_wait(bar, (uint32_t)parity & 1, &s.abort, lane, limit); };
+  TreeWalk w(a, s.run, S::ROWS / 32);
+  if (warp < kIssueWarp && w.begin()) {  // the first unit's queries by the warps that have nothing to do yet
+    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp);
+    if (lane == 0) mbar_arrive(&s.qfirst);
+  }
+
+  if (warp < kSoftmaxWarps) {
+    // ---- weights: a thread a row, of one replica's share of the tile's keys
+    int it = 0, masks = 0, unit = 0;
+#pragma unroll 1
+    for (bool go = w.begin(); go && !s.abort; go = w.next(), ++unit) {
+      const int R = w.replicas(), per = S::ROWS / R, row = threadIdx.x;
+      const int qi = row % per, slice = row < S::ROWS ? row / per : 0;
+      const bool mine = row < S::ROWS && qi < w.live, live = __any_sync(0xffffffffu, mine);
+      uint32_t* sees = s.sees[row < S::ROWS ? row : 0];
+      // the rows' masks, where this CTA meets drafted keys
+      const bool drafted = w.hi * TK > w.e.len;
+      if (drafted) {
+        for (int i = threadIdx.x; i < w.e.nodes; i += kSoftmaxWarps * 32) {
+          int p = a.parents[w.e.first + i];
+          if (p < -1 || p >= i) {
+            kv_report(a.status, ER_KV_BAD_TREE);
+            s.bad_tree[masks & 1] = masks + 1;  // of this unit
+            p = -1;
+          }
+          s.parents[masks & 1][i] = p;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.masked);
+        if (!wait(&s.masked, masks)) break;
+        if (row < S::ROWS)
+          for (int i = 0; i < 9; ++i) sees[i] = 0;
+        if (mine)
+          for (int p = (w.q0 + qi) / a.group; p >= 0; p = s.parents[masks & 1][p]) sees[p >> 5] |= 1u << (p & 31);
+        ++masks;
+        __syncwarp();
+      }
+      float m = -INFINITY, l = 0.f;
+      if (drafted && s.bad_tree[(masks - 1) & 1] == masks) l = __int_as_float(0x7fc00000);
+      auto tile = [&](auto replicas, int t) {
+        constexpr int RR = decltype(replicas)::value, KPT = TK / RR;
+        const int b = it & 1, key0 = t * TK + slice * KPT;
+        const uint32_t sp = tmem + ((uint32_t)(warp * 32) << 16) + b * S::kSP;
+        uint32_t x[KPT];
+        if constexpr (KPT == 64) {
+          tmem_ld32(sp, x);
+          tmem_ld32(sp + 32, x + 32);
+        } else if constexpr (KPT == 32) {
+          tmem_ld32(sp + slice * 32, x);
+        } else {
+          tmem_ld16(sp + slice * 16, x);
+        }
+        tmem_wait_ld();
+        if (key0 + KPT > w.e.len) {  // drafted keys, or none: what the row sees of them
+          const int slot = (2 * it + 1) % SLOTS;
+          uint32_t spoils = 0;
+#pragma unroll
+          for (int c = 0; c < KPT; c += 32) {
+            const uint32_t see = seen_from(sees, key0 + c - w.e.len);
+#pragma unroll
+            for (int j = c; j < KPT && j < c + 32; ++j)
+              if (!(see >> (j - c) & 1)) x[j] = 0xff800000u;
+            uint32_t vb = 0;
+            const int first = slice * KPT + c;  // of the tile's keys
+            for (int i = 0; i < S::kFixWarps; ++i) vb |= s.vbad[slot][i][first >> 5] >> (first & 31);
+            spoils |= vb & see & (KPT < 32 ? (1u << (KPT & 31)) - 1 : 0xffffffffu);
+          }
+          if (spoils) l = __int_as_float(0x7fc00000);
+        }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+        const float ref = top == -INFINITY ? 0.f : top, shift = -ref * a.scale, by = ex2(fmaf(m, a.scale, shift));
+        m = top;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          const float p = ex2(fmaf(__uint_as_float(x[j]), a.scale, shift));
+          x[j] = __float_as_uint(p);
+          sum += p;
+        }
+        l = l * by + sum;
+        if (row < S::ROWS) s.by[it & 3][row] = by;
+        __syncwarp();
+#pragma unroll
+        for (int part = 0; part < S::PP; ++part) {
+#pragma unroll
+          for (int c = 0; c < KPT / 2; c += 8) {
+            uint32_t y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              float u = __uint_as_float(x[2 * (c + j)]), v = __uint_as_float(x[2 * (c + j) + 1]);
+              y[j] = split2(u, v);
+              x[2 * (c + j)] = __float_as_uint(u);
+              x[2 * (c + j) + 1] = __float_as_uint(v);
+            }
+            tmem_st8(sp + part * 32 + slice * (KPT / 2) + c, y);
+          }
+          const uint32_t zero[8] = {};  // the other keys are other replicas'
+#pragma unroll
+          for (int c = KPT / 2; c < 32; c += 8) tmem_st8(sp + part * 32 + ((slice * (KPT / 2) + c) & 31), zero);
+        }
+      };
+      bool ok = true;
+#pragma unroll 1
+      for (int t = w.lo; t < w.hi; ++t, ++it) {
+        if (!(ok = wait(&s.sfull[it & 1], it >> 1))) break;
+        if ((t + 1) * TK > w.e.len && !(ok = wait(&s.full[(2 * it + 1) % SLOTS], (2 * it + 1) / SLOTS))) break;
+        tc_fence_after();
+        if (live) {
+          if (R == 1)
+            tile(std::integral_constant<int, 1>{}, t);
+          else if (R == 2)
+            tile(std::integral_constant<int, 2>{}, t);
+          else
+            tile(std::integral_constant<int, 4>{}, t);
+          tmem_wait_st();
+        }
+        if (t + 1 == w.hi && row < S::ROWS) {
+          if (s.bad_unit[unit & 15] == unit + 1) l = __int_as_float(0x7fc00000);
+          s.ml[it & 3][row] = make_float2(m == -INFINITY ? m : m * a.scale, l);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.pfull[it & 1]);
+      }
+      if (!ok) break;
+    }
+  } else if (warp < kIssueWarp) {
+    // ---- sums: a thread a row, of half of the channels
+    constexpr int CH = S::VD / 2;
+    const int row = (warp & 3) * 32 + lane, half = (warp - kSoftmaxWarps) >> 2, id = threadIdx.x - kSoftmaxWarps * 32;
+    int it = 0, stages = 0;
+    if (id == 0) a.cut[blockIdx.x].live = 0;
+#pragma unroll 1
+    for (bool go = w.begin(); go && !s.abort; go = w.next()) {
+      float o[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) o[c] = 0.f;
+      const int R = w.replicas(), per = S::ROWS / R, vd = min(S::VD, d - w.ch0);
+      const bool there = row < S::ROWS, live = __any_sync(0xffffffffu, there && row % per < w.live);
+      bool ok = true;
+      float2 ml = make_float2(0.f, 0.f);
+#pragma unroll 1
+      for (int t = w.lo; t < w.hi; ++t, ++it) {
+        const int ob = it & 1;
+        if (!(ok = wait(&s.ofull[ob], it >> 1))) break;  // after the tile's weights, so `by` and `ml` are there
+        tc_fence_after();
+        if (live) {
+          const float by = there ? s.by[it & 3][row] : 0.f;
+          const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 2 * S::kSP + ob * S::VD + half * CH;
+          constexpr int N = S::kThreads > 512 ? 16 : 32;  // registers
+#pragma unroll
+          for (int c = 0; c < CH; c += N) {
+            uint32_t x[N];
+            if constexpr (N == 32)
+              tmem_ld32(at + c, x);
+            else
+              tmem_ld16(at + c, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < N; ++j) o[c + j] = fmaf(o[c + j], by, __uint_as_float(x[j]));
+          }
+        }
+        if (t + 1 == w.hi && there) ml = s.ml[it & 3][row];
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.ofree[ob]);
+      }
+      if (!ok) break;
+      // the replicas' rows joined: 16 channels of each half at a time by way of shared memory
+      const bool whole = w.lo == 0 && w.hi == w.tiles, begins = w.lo == 0;
+      if (!whole && begins && id == 0)
+        a.cut[blockIdx.x] = TreeCut{w.e.first, w.head, w.q0, w.live, w.tiles, w.ch0, w.pos, s.run.total};
+      const long long piece = (long long)blockIdx.x * 2 + begins;
+#pragma unroll
+      for (int c0 = 0; c0 < CH; c0 += 16) {
+        if (there) {
+          float* mine = stage + row * kStagePitch + half * 16;
+#pragma unroll
+          for (int j = 0; j < 16; j += 4)
+            *reinterpret_cast<float4*>(mine + j) = make_float4(o[c0 + j], o[c0 + j + 1], o[c0 + j + 2], o[c0 + j + 3]);
+          if (c0 == 0 && half == 0) *reinterpret_cast<float2*>(stage + row * kStagePitch + 32) = ml;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.staged);
+        if (!(ok = wait(&s.staged, stages))) break;
+        ++stages;
+        for (int i = id; i < w.live * 8; i += kSumWarps * 32) {
+          const int qi = i >> 3, hh = i >> 2 & 1, v = i & 3, ch = hh * CH + c0 + v * 4;
+          if (ch >= vd) continue;
+          float2 p[4];
+          float4 x[4];
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[r] = make_float2(-INFINITY, 0.f);
+            x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < R) {
+              const float* at = stage + (r * per + qi) * kStagePitch;
+              p[r] = *reinterpret_cast<const float2*>(at + 32);
+              x[r] = *reinterpret_cast<const float4*>(at + hh * 16 + v * 4);
+            }
+            top = fmaxf(top, p[r].x);
+          }
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float by = piece_weight(p[r].x, top);
+            sum = fmaf(p[r].y, by, sum);  // a spoilt row's sum is NaN
+            fma4(acc, x[r], by);
+          }
+          if (whole) {
+            const int q = w.q0 + qi, node = q / a.group, g = q - node * a.group;
+            const long long at = (long long)(w.e.first + node) * a.heads + w.head * a.group + g;
+            kv_store4((TQ*)a.out + at * d + w.ch0 + ch, acc, sum);
+          } else {
+            *reinterpret_cast<float4*>(a.part_o + (piece * a.piece_rows + qi) * S::VD + ch) = acc;
+            if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + (piece * a.piece_rows + qi) * 2) = make_float2(top, sum);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.staged);
+        if (!(ok = wait(&s.staged, stages))) break;
+        ++stages;
+      }
+      if (!ok) break;
+    }
+  } else if (warp == kIssueWarp) {
+    // ---- products
+    const int ksteps = (d + 15) / 16;
+    const uint32_t is = idesc_bf16(TK, 0);
+    int it = 0, unit = 0;
+    uint32_t io = 0;
+    auto values = [&](int i) {  // out += P V of tile i
+      const int item = 2 * i + 1, slot = item % SLOTS, b = i & 1;
+      if (!wait(&s.pfull[b], i >> 1)) return false;
+      if (!wait(&s.full[slot], item / SLOTS)) return false;
+      if (i >= 2 && !wait(&s.ofree[b], (i >> 1) - 1)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        uint32_t at = S::slot(slots0, slot);
+        asm volatile("" : "+r"(at));  // put together here, not held over the waits
+        const uint32_t v = desc_low(at, TK * 128);
+        uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + b * S::kSP, id = io;
+        asm volatile("" : "+r"(to), "+r"(p), "+r"(id));
+        // the small products first
+#pragma unroll
+        for (int pp = S::PP - 1; pp >= 0; --pp)
+#pragma unroll
+          for (int kp = S::KP - 1; kp >= 0; --kp) {
+            if (S::KP > 1 && pp + kp > 2) continue;  // under 2^-24 of the whole
+            constexpr int kFirst = S::KP > 1 ? 1 : 0;
+#pragma unroll
+            for (int k = 0; k < TK / 16; ++k)
+              mma_f16_ts(to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
+                         !(pp == S::PP - 1 && kp == (kFirst ? 2 - pp : 0) && k == 0));
+          }
+        umma_commit<1>(&s.ofull[b]);
+        umma_commit<1>(&s.empty[slot]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+#pragma unroll 1
+    for (bool go = w.begin(); go && ok; go = w.next(), ++unit) {
+      if (it > 0 && !(ok = values(it - 1))) break;
+      io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
+      if (!(ok = unit ? wait(&s.qfull, unit - 1) : wait(&s.qfirst, 0))) break;
+#pragma unroll 1
+      for (int t = w.lo; t < w.hi; ++t, ++it) {
+        const int item = 2 * it, slot = item % SLOTS, b = it & 1;
+        if (!(ok = wait(&s.full[slot], item / SLOTS))) break;
+        tc_fence_after();
+        if (lane == 0) {
+          uint32_t at = S::slot(slots0, slot), qat = q0;
+          asm volatile("" : "+r"(at), "+r"(qat));
+          const uint32_t kd = desc_low(at, 16), qd = desc_low(qat, 16);
+          uint32_t to = tmem + b * S::kSP, id = is;
+          asm volatile("" : "+r"(to), "+r"(id));
+#pragma unroll
+          for (int qp = S::QP - 1; qp >= 0; --qp)
+#pragma unroll
+            for (int kp = S::KP - 1; kp >= 0; --kp) {
+              if (S::KP > 1 && qp + kp > 2) continue;
+              constexpr int kFirst = S::KP > 1 ? 1 : 0;
+#pragma unroll
+              for (int k = 0; k < S::DP / 16; ++k)
+                if (k < ksteps)
+                  mma_f16_ss(to, qd + ((qp * S::kQPart + (k >> 2) * (S::ROWS * 128) + (k & 3) * 32) >> 4),
+                             kd + ((kp * S::kKPart + (k >> 2) * (TK * 128) + (k & 3) * 32) >> 4), id,
+                             !(qp == S::QP - 1 && kp == (kFirst ? 2 - qp : 0) && k == 0));
+            }
+          umma_commit<1>(&s.sfull[b]);
+          umma_commit<1>(&s.empty[slot]);
+          if (t + 1 == w.hi) umma_commit<1>(&s.qfree);
+        }
+        __syncwarp();
+        if (t > w.lo && !(ok = values(it - 1))) break;
+      }
+      if (!ok) break;
+    }
+    if (ok && it > 0) ok = values(it - 1) && wait(&s.empty[(2 * it - 1) % SLOTS], (2 * it - 1) / SLOTS);
+    if (!ok && lane == 0) {  // the products under way end before their memory goes
+      umma_commit<1>(&s.drain);
+      mbar_drain(&s.drain, 0, limit);
+    }
+    __syncwarp();
+  } else if (S::KP == 1 && warp == kIssueWarp + 1) {
+    // ---- copies of keys and values: boxes of as many positions as lie in one page
+    const int rows = a.box_rows, boxes = TK / rows, kc = (d + 63) / 64;
+    int item = 0, unit = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
+      const int32_t* pages = a.kv.pages_of(w.e.seq);
+      const int keys = w.e.len + w.e.nodes, vc = (min(S::VD, d - w.ch0) + 63) / 64;
+      auto page_of = [&](int t, int i) {  // of box i; behind the last key none
+        const int key = t * TK + i * rows;
+        return i < boxes && key < keys ? pages[a.kv.ordinal(key)] : a.kv.num_pages;
+      };
+      int next[2] = {page_of(w.lo, lane), page_of(w.lo, lane + 32)};
+#pragma unroll 1
+      for (int t = w.lo; t < w.hi && ok; ++t) {
+        int page[2];
+        bool bad = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          page[j] = next[j];
+          const int i = lane + 32 * j;
+          if (i < boxes && (page[j] < 0 || page[j] >= a.kv.num_pages)) {
+            bad |= t * TK + i * rows < keys;
+            page[j] = a.kv.num_pages;  // outside the pool: zeros
+          }
+          if (t + 1 < w.hi) next[j] = page_of(t + 1, i);
+        }
+        if (__any_sync(0xffffffffu, bad) && lane == 0) {
+          kv_report(a.status, ER_KV_BAD_PAGE);
+          s.bad_unit[unit & 15] = unit + 1;
+        }
+#pragma unroll 1
+        for (int kind = 0; kind < 2; ++kind, ++item) {  // keys, values
+          const int slot = item % SLOTS, chunks = kind ? vc : kc, x0 = kind ? w.ch0 : 0;
+          if (item >= SLOTS && !(ok = wait(&s.empty[slot], item / SLOTS - 1))) break;
+          // values of a tile with drafted keys are looked at before they count
+          const bool look = kind && (t + 1) * TK > w.e.len;
+          uint64_t* bar = look ? &s.raw[slot] : &s.full[slot];
+          if (lane == 0) {
+            mbar_expect_tx(bar, chunks * TK * 128);
+            if (!look)
+              for (int i = 1; i < S::kFixWarps; ++i) mbar_arrive(bar);
+          }
+          __syncwarp();
+          const uint32_t to = S::slot(slots0, slot);
+          // one lane issues all copies: their operands are the warp's, not a lane's
+          for (int i = 0; i < boxes; ++i) {
+            const int pg = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31);
+            if (lane == 0) {
+              const int at = a.kv.slot(t * TK + i * rows);
+              for (int c = 0; c < chunks; ++c) {
+                if (kind)
+                  tma_box(to + c * (TK * 128) + i * rows * 128, &vmap, bar, x0 + c * 64, at, w.head, pg);
+                else
+                  tma_box(to + c * (TK * 128) + i * rows * 128, &kmap, bar, c * 64, at, w.head, pg);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    // nothing of its copies is under way when the CTA's memory goes
+    if (!ok || s.abort)
+      for (int i = 0; i < SLOTS; ++i) {
+        const int last = item - 1 - (item - 1 - i + SLOTS * 4) % SLOTS;  // the last item of slot i
+        if (item > 0 && last >= 0 && last < item) {
+          mbar_drain(&s.full[i], (last / SLOTS) & 1, limit / 8);
+        }
+      }
+  } else {
+    // ---- queries, and drafted values (bf16 caches) or all keys and values (fp32 caches)
+    const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kFixWarps);
+    const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
+    int item = 0, unit = 0, looks = 0;
+    bool ok = true;
+    auto signal = [&](uint64_t* bar) {
+      async_fence();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+#pragma unroll 1
+    for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
+      if (unit > 0) {
+        if (!(ok = wait(&s.qfree, unit - 1))) break;
+        load_queries<S, TQ>(a, w, q0, loader, S::kFixWarps);
+        signal(&s.qfull);
+      }
+      const int keys = w.e.len + w.e.nodes;
+      if constexpr (S::KP == 1) {
+        item += 2 * (w.hi - w.lo);
+        const int first = max(w.lo, w.e.len / TK);
+        for (int t = first; t < w.hi; ++t) {  // tiles with drafted keys, or none
+          const int it = item / 2 - (w.hi - t), n = 2 * it + 1, slot = n % SLOTS;
+          if (!(ok = wait(&s.raw[slot], looks >> slot))) break;
+          looks ^= 1 << slot;
+          const uint32_t to = S::slot(slots0, slot);
+          uint32_t marks[2] = {0, 0};
+          const int vv = (min(S::VD, d - w.ch0) + 15) / 16 * 2, r0 = max(0, w.e.len - t * TK);
+          for (int i = loader * 32 + lane; i < (TK - r0) * vv; i += S::kFixWarps * 32) {
+            const int r = r0 + i / vv, c = i % vv;
+            const uint32_t at = to + swizzled(c, r, TK);
+            const uint4 v = lds16(at);
+            const uint32_t h[4] = {v.x, v.y, v.z, v.w};
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bad |= (h[j] & 0x7f80u) == 0x7f80u || (h[j] & 0x7f800000u) == 0x7f800000u;
+            // no numbers: zero, for the rows that do not see them, and marked for those that do
+            if (bad || t * TK + r >= keys) sts16(at, make_uint4(0, 0, 0, 0));
+            if (bad) marks[r >> 5] |= 1u << (r & 31);
+          }
+          __syncwarp();
+          for (int i = 0; i < 2; ++i) {
+            marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
+            if (lane == 0) s.vbad[slot][loader][i] = marks[i];
+          }
+          signal(&s.full[slot]);
+        }
+      } else {
+        constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;  // of four rows, eight lanes a row
+        // the place in the pools of row i of this warp's in a tile (-1: none, or a bad page)
+        const int32_t* pages = a.kv.pages_of(w.e.seq);
+        auto row_of = [&](int i) { return (loader + i * S::kFixWarps) * 4; };
+        const int own = row_of(lane >> 2) + (lane & 3);  // the row that this lane looks up
+        auto page_of = [&](int t) {
+          const int key = t * TK + own;
+          return lane < GROUPS * 4 && own < TK && key < keys ? pages[a.kv.ordinal(key)] : -1;
+        };
+        int page = page_of(w.lo);
+#pragma unroll 1
+        for (int t = w.lo; t < w.hi && ok; ++t) {
+          long long off = -1;
+          const int key = t * TK + own;
+          if (lane < GROUPS * 4 && own < TK && key < keys) {
+            if (page < 0 || page >= a.kv.num_pages) {
+              kv_report(a.status, ER_KV_BAD_PAGE);
+              s.bad_unit[unit & 15] = unit + 1;
+            } else {
+              off = page * a.kv.page_stride + w.head * a.kv.head_stride + a.kv.slot(key) * a.kv.slot_stride;
+            }
+          }
+          if (t + 1 < w.hi) page = page_of(t + 1);
+          __syncwarp();
+#pragma unroll 1
+          for (int kind = 0; kind < 2; ++kind, ++item) {  // keys, values
+            const int slot = item % SLOTS;
+            if (item >= SLOTS && !(ok = wait(&s.empty[slot], item / SLOTS - 1))) break;
+            const uint32_t to = S::slot(slots0, slot);
+            const char* pool = kind ? a.kv.v + w.ch0 * 4 : a.kv.k;
+            const bool look = kind && (t + 1) * TK > w.e.len;
+            const int width = kind ? min(S::VD, d - w.ch0) : d, n = kind ? (width + 15) / 16 * 2 : vecs;
+            uint32_t marks[2] = {0, 0};
+            for (int c0 = 0; c0 < n; c0 += 8) {  // the same for all lanes: they exchange the rows' places
+              const int c = c0 + (lane & 7);
+              float4 x[GROUPS][2];
+#pragma unroll
+              for (int i = 0; i < GROUPS; ++i) {
+                const long long o = __shfl_sync(0xffffffffu, off, i * 4 + lane / 8);
+                x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (o >= 0 && c * 8 < width) {
+                  x[i][0] = load4((const float*)(pool + o) + c * 8);
+                  x[i][1] = load4((const float*)(pool + o) + c * 8 + 4);
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < GROUPS; ++i) {
+                const int r = row_of(i) + lane / 8;
+                if (r >= TK || c >= n) continue;
+                float y[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
+                if (look && t * TK + r >= w.e.len) {
+                  bool bad = false;
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) bad |= !(fabsf(y[j]) < INFINITY);
+                  if (bad) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = 0.f;
+                    marks[r >> 5] |= 1u << (r & 31);
+                  }
+                }
+                uint4 parts[3];
+                split8(y, parts);
+                const uint32_t dst = to + swizzled(c, r, TK);
+#pragma unroll
+                for (int j = 0; j < 3; ++j) sts16(dst + j * (kind ? S::kVPart : S::kKPart), parts[j]);
+              }
+            }
+            __syncwarp();
+            if (look) {
+              for (int i = 0; i < 2; ++i) {
+                marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
+                if (lane == 0) s.vbad[slot][loader][i] = marks[i];
+              }
+            }
+            signal(&s.full[slot]);
+          }
+        }
+      }
+    }
+  }
+  if (s.abort && threadIdx.x == 0) kv_report(a.status, ER_KV_GAVE_UP);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssueWarp) tmem_dealloc<1>(tmem, 512);
+}
+
+template <typename S, typename TC, typename TQ>
+int tree_launch(const TreeArgs& a, const CUtensorMap* maps, cudaStream_t st) {
+  static std::atomic<unsigned long long> allowed;
+  const int smem = S::kSmem + 1024;
+  if (int rc = allow_smem(kv_tree_kernel<S, TC, TQ>, smem, allowed)) return rc;
+  return kv_launch(kv_tree_kernel<S, TC, TQ>, dim3(a.grid), S::kThreads, smem, false, st, "kv_tree_kernel", a, maps[0],
+                   maps[1]);
+}
+
+}  // namespace
+}  // namespace er

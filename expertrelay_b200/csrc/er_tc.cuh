@@ -381,22 +381,6 @@ inline uint32_t maps_used_bits(const TcMaps& maps) {
 // host side: tensor maps
 // ---------------------------------------------------------------------------
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  }
-  return fn;
-}
-
 // uint8 tensor map, K innermost (contiguous), box box_k x box_rows [x 1]:
 // 128-byte swizzle for MMA operand tiles (box_k = 128), none for staged tiles.
 inline int make_map(CUtensorMap* m, const void* base, int rank, uint64_t k, uint64_t rows, uint64_t slots,

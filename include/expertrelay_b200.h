@@ -405,6 +405,7 @@ typedef struct er_kv_cache {
 #define ER_KV_BAD_LENGTH 2     /* a length, position or count outside its table */
 #define ER_KV_BAD_SEQ 4        /* a sequence index outside [0, seqs) */
 #define ER_KV_BAD_TREE 8       /* a tree's rows or parents */
+#define ER_KV_GAVE_UP 16       /* a wait of the kernel ran out (2 s): its results are not to be used */
 
 /* RoPE and the write of new tokens' rows into the pages: row i of qkv
  * [n, (heads + 2 kv_heads) head_dim] (q | k | v, dtype qkv_dtype, row stride
