@@ -25,9 +25,9 @@ struct TreeShape {
   static constexpr int kQPart = ROWS * DP * 2, kQ = kQPart * QP;
   static constexpr int kSP = PP * 32 > 64 ? PP * 32 : 64;  // columns of a tile's scores, then of its weights
   static constexpr int kSmem = kQ + PAIRS_ * kPair + ROWS * kStagePitch * 4;
-  // warps that fill shared memory: of a bf16 cache one that issues copies and two that look after the drafted
-  // values, of an fp32 cache all of them by way of registers
-  static constexpr int kLoadWarps = KP == 1 ? 3 : 7, kFixWarps = KP == 1 ? 2 : 7;
+  // warps that fill shared memory: of a bf16 cache one that issues the keys' copies, one the values' and one that
+  // looks after the drafted values, of an fp32 cache all of them by way of registers
+  static constexpr int kLoadWarps = KP == 1 ? 3 : 7, kFixWarps = KP == 1 ? 1 : 7;
   static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
   static __device__ __forceinline__ uint32_t slot(uint32_t base, int i) {
     return base + (i >> 1) * kPair + (i & 1) * kKPart * KP;
@@ -56,23 +56,73 @@ struct TreeShared {
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return (addr & 0x3FFFFu) >> 4 | (lbo >> 4) << 16; }
 
-// d (+)= A B, A and B in shared memory, or A in tensor memory
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+// d (+)= A B, A and B in shared memory, or A in tensor memory; issued by the lane whose `go` is not zero. All lanes
+// come here, so the operands may be the warp's.
+__device__ __forceinline__ void mma_f16_ss(uint32_t go, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, g;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %6, 0;\n\t"
       "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh), "r"(go)
       : "memory");
 }
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t go, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, g;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 g, %6, 0;\n\t"
       "mov.b64 y, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
+      "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh), "r"(go)
       : "memory");
 }
+// arrives on the barrier once the products issued so far are done
+__device__ __forceinline__ void commit_on(uint32_t go, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %1, 0;\n\t"
+      "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(go)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+// a barrier by its address in shared memory
+__device__ __forceinline__ bool bar_done(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const unsigned long long t0 = globaltimer();
+  bool ok = true;
+  while (!bar_done(bar, parity)) {
+    if (*abort_flag || globaltimer() - t0 > kDefaultWaitNs) {
+      *abort_flag = 1;
+      ok = false;
+      break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// A place in a ring of N and how often, modulo 2, it has been gone round.
+template <int N>
+struct Ring {
+  int at = 0;
+  uint32_t turn = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) at = 0, turn ^= 1;
+  }
+};
+
 // bf16 operands, fp32 sums, M = 128; b_mn: B's rows (N) are contiguous, not its K
 __device__ __forceinline__ uint32_t idesc_bf16(int n, int b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -150,12 +200,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int slot, int head,
-                                        int page) {
+// (issued by the lane whose `go` is not zero)
+__device__ __forceinline__ void tma_box(uint32_t go, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int slot,
+                                        int head, int page) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
-      "[%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(slot), "r"(head), "r"(page)
+      "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %7, 0;\n\t"
+      "@g cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], "
+      "[%2];\n\t}" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(go)
       : "memory");
 }
 
@@ -247,7 +299,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       mbar_init(&s.raw[i], 1);
     }
     mbar_init(&s.qfirst, kIssueWarp);
-    mbar_init(&s.qfull, S::kFixWarps);
+    mbar_init(&s.qfull, kSoftmaxWarps);
     mbar_init(&s.qfree, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.sfull[i], 1);
@@ -268,19 +320,34 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   tree_run(a, s.run, s.scratch);  // all threads; ends with a barrier
   tc_fence_after();
   const uint32_t tmem = s.tmem;
-  const unsigned long long limit = kDefaultWaitNs;
-  auto wait = [&](uint64_t* bar, int parity) { return warp_wait(bar, (uint32_t)parity & 1, &s.abort, lane, limit); };
+  // the whole warp waits, with a limit; false once any wait of the CTA has given up
+  auto wait = [&](const uint64_t& b, uint32_t parity) {
+    const uint32_t bar = smem_u32(&b);
+    if (__all_sync(0xffffffffu, bar_done(bar, parity))) return true;
+    return bar_wait_slow(bar, parity, &s.abort);
+  };
+  auto arrive = [&](const uint64_t& b) {  // the warp's one arrival, after all its lanes
+    __syncwarp();
+    if (lane == 0) bar_arrive(smem_u32(&b));
+  };
   TreeWalk w(a, s.run, S::ROWS / 32);
   if (warp < kIssueWarp && w.begin()) {  // the first unit's queries by the warps that have nothing to do yet
     load_queries<S, TQ>(a, w, q0, warp, kIssueWarp);
-    if (lane == 0) mbar_arrive(&s.qfirst);
+    arrive(s.qfirst);
   }
 
   if (warp < kSoftmaxWarps) {
     // ---- weights: a thread a row, of one replica's share of the tile's keys
     int it = 0, masks = 0, unit = 0;
+    Ring<2> sp_ring;
+    Ring<SLOTS / 2> pair;
 #pragma unroll 1
     for (bool go = w.begin(); go && !s.abort; go = w.next(), ++unit) {
+      if (unit > 0) {  // the first one's are on their way
+        if (!wait(s.qfree, (unit - 1) & 1)) break;
+        load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps);
+        arrive(s.qfull);
+      }
       const int R = w.replicas(), per = S::ROWS / R, row = threadIdx.x;
       const int qi = row % per, slice = row < S::ROWS ? row / per : 0;
       const bool mine = row < S::ROWS && qi < w.live, live = __any_sync(0xffffffffu, mine);
@@ -297,9 +364,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           }
           s.parents[masks & 1][i] = p;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.masked);
-        if (!wait(&s.masked, masks)) break;
+        arrive(s.masked);
+        if (!wait(s.masked, masks & 1)) break;
         if (row < S::ROWS)
           for (int i = 0; i < 9; ++i) sees[i] = 0;
         if (mine)
@@ -311,8 +377,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       if (drafted && s.bad_tree[(masks - 1) & 1] == masks) l = __int_as_float(0x7fc00000);
       auto tile = [&](auto replicas, int t) {
         constexpr int RR = decltype(replicas)::value, KPT = TK / RR;
-        const int b = it & 1, key0 = t * TK + slice * KPT;
-        const uint32_t sp = tmem + ((uint32_t)(warp * 32) << 16) + b * S::kSP;
+        const int key0 = t * TK + slice * KPT;
+        const uint32_t sp = tmem + ((uint32_t)(warp * 32) << 16) + sp_ring.at * S::kSP;
         uint32_t x[KPT];
         if constexpr (KPT == 64) {
           tmem_ld32(sp, x);
@@ -324,7 +390,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         }
         tmem_wait_ld();
         if (key0 + KPT > w.e.len) {  // drafted keys, or none: what the row sees of them
-          const int slot = (2 * it + 1) % SLOTS;
+          const int slot = 2 * pair.at + 1;
           uint32_t spoils = 0;
 #pragma unroll
           for (int c = 0; c < KPT; c += 32) {
@@ -375,9 +441,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       };
       bool ok = true;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it) {
-        if (!(ok = wait(&s.sfull[it & 1], it >> 1))) break;
-        if ((t + 1) * TK > w.e.len && !(ok = wait(&s.full[(2 * it + 1) % SLOTS], (2 * it + 1) / SLOTS))) break;
+      for (int t = w.lo; t < w.hi; ++t, ++it, sp_ring.next(), pair.next()) {
+        if (!(ok = wait(s.sfull[sp_ring.at], sp_ring.turn))) break;
+        if ((t + 1) * TK > w.e.len && !(ok = wait(s.full[2 * pair.at + 1], pair.turn))) break;
         tc_fence_after();
         if (live) {
           if (R == 1)
@@ -393,8 +459,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           s.ml[it & 3][row] = make_float2(m == -INFINITY ? m : m * a.scale, l);
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.pfull[it & 1]);
+        arrive(s.pfull[sp_ring.at]);
       }
       if (!ok) break;
     }
@@ -402,7 +467,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     // ---- sums: a thread a row, of half of the channels
     constexpr int CH = S::VD / 2;
     const int row = (warp & 3) * 32 + lane, half = (warp - kSoftmaxWarps) >> 2, id = threadIdx.x - kSoftmaxWarps * 32;
-    int it = 0, stages = 0;
+    int it = 0;
+    Ring<2> o_ring;
+    uint32_t stages = 0;
     if (id == 0) a.cut[blockIdx.x].live = 0;
 #pragma unroll 1
     for (bool go = w.begin(); go && !s.abort; go = w.next()) {
@@ -414,9 +481,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       bool ok = true;
       float2 ml = make_float2(0.f, 0.f);
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it) {
-        const int ob = it & 1;
-        if (!(ok = wait(&s.ofull[ob], it >> 1))) break;  // after the tile's weights, so `by` and `ml` are there
+      for (int t = w.lo; t < w.hi; ++t, ++it, o_ring.next()) {
+        const int ob = o_ring.at;
+        if (!(ok = wait(s.ofull[ob], o_ring.turn))) break;  // after the tile's weights, so `by` and `ml` are there
         tc_fence_after();
         if (live) {
           const float by = there ? s.by[it & 3][row] : 0.f;
@@ -436,8 +503,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         }
         if (t + 1 == w.hi && there) ml = s.ml[it & 3][row];
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.ofree[ob]);
+        arrive(s.ofree[ob]);
       }
       if (!ok) break;
       // the replicas' rows joined: 16 channels of each half at a time by way of shared memory
@@ -454,10 +520,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             *reinterpret_cast<float4*>(mine + j) = make_float4(o[c0 + j], o[c0 + j + 1], o[c0 + j + 2], o[c0 + j + 3]);
           if (c0 == 0 && half == 0) *reinterpret_cast<float2*>(stage + row * kStagePitch + 32) = ml;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.staged);
-        if (!(ok = wait(&s.staged, stages))) break;
-        ++stages;
+        arrive(s.staged);
+        if (!(ok = wait(s.staged, stages))) break;
+        stages ^= 1;
         for (int i = id; i < w.live * 8; i += kSumWarps * 32) {
           const int qi = i >> 3, hh = i >> 2 & 1, v = i & 3, ch = hh * CH + c0 + v * 4;
           if (ch >= vd) continue;
@@ -491,110 +556,112 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + (piece * a.piece_rows + qi) * 2) = make_float2(top, sum);
           }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.staged);
-        if (!(ok = wait(&s.staged, stages))) break;
-        ++stages;
+        arrive(s.staged);
+        if (!(ok = wait(s.staged, stages))) break;
+        stages ^= 1;
       }
       if (!ok) break;
     }
   } else if (warp == kIssueWarp) {
     // ---- products
     const int ksteps = (d + 15) / 16;
-    const uint32_t is = idesc_bf16(TK, 0);
-    int it = 0, unit = 0;
+    const uint32_t is = idesc_bf16(TK, 0), one = elected();
+    int unit = 0, scored = 0, summed = 0;  // tiles
     uint32_t io = 0;
-    auto values = [&](int i) {  // out += P V of tile i
-      const int item = 2 * i + 1, slot = item % SLOTS, b = i & 1;
-      if (!wait(&s.pfull[b], i >> 1)) return false;
-      if (!wait(&s.full[slot], item / SLOTS)) return false;
-      if (i >= 2 && !wait(&s.ofree[b], (i >> 1) - 1)) return false;
+    constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
+    Ring<2> sp_ring, p_ring;            // of the tile whose scores, whose values are next
+    Ring<SLOTS / 2> k_ring, v_ring;
+    auto values = [&]() {  // out += P V of the tile before
+      const int b = p_ring.at;
+      if (!wait(s.pfull[b], p_ring.turn) || !wait(s.full[2 * v_ring.at + 1], v_ring.turn)) return false;
+      if (summed >= 2 && !wait(s.ofree[b], p_ring.turn ^ 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        uint32_t at = S::slot(slots0, slot);
-        asm volatile("" : "+r"(at));  // put together here, not held over the waits
-        const uint32_t v = desc_low(at, TK * 128);
-        uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + b * S::kSP, id = io;
-        asm volatile("" : "+r"(to), "+r"(p), "+r"(id));
-        // the small products first
+      uint32_t v = desc_low(S::slot(slots0, 2 * v_ring.at + 1), TK * 128);
+      uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + b * S::kSP, id = io;
+      // put together here: descriptors that the compiler kept from before the waits' calls came out wrong
+      asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
+      // the small products first
 #pragma unroll
-        for (int pp = S::PP - 1; pp >= 0; --pp)
+      for (int pp = S::PP - 1; pp >= 0; --pp)
 #pragma unroll
-          for (int kp = S::KP - 1; kp >= 0; --kp) {
-            if (S::KP > 1 && pp + kp > 2) continue;  // under 2^-24 of the whole
-            constexpr int kFirst = S::KP > 1 ? 1 : 0;
+        for (int kp = S::KP - 1; kp >= 0; --kp) {
+          if (kThree && pp + kp > 2) continue;
 #pragma unroll
-            for (int k = 0; k < TK / 16; ++k)
-              mma_f16_ts(to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
-                         !(pp == S::PP - 1 && kp == (kFirst ? 2 - pp : 0) && k == 0));
-          }
-        umma_commit<1>(&s.ofull[b]);
-        umma_commit<1>(&s.empty[slot]);
-      }
-      __syncwarp();
+          for (int k = 0; k < TK / 16; ++k)
+            mma_f16_ts(one, to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
+                       !(pp == S::PP - 1 && kp == (kThree ? 2 - pp : 0) && k == 0));
+        }
+      commit_on(one, smem_u32(&s.ofull[b]));
+      commit_on(one, smem_u32(&s.empty[2 * v_ring.at + 1]));
+      p_ring.next();
+      v_ring.next();
+      ++summed;
       return true;
     };
     bool ok = true;
 #pragma unroll 1
     for (bool go = w.begin(); go && ok; go = w.next(), ++unit) {
-      if (it > 0 && !(ok = values(it - 1))) break;
+      if (scored > summed && !(ok = values())) break;
       io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
-      if (!(ok = unit ? wait(&s.qfull, unit - 1) : wait(&s.qfirst, 0))) break;
+      if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it) {
-        const int item = 2 * it, slot = item % SLOTS, b = it & 1;
-        if (!(ok = wait(&s.full[slot], item / SLOTS))) break;
+      for (int t = w.lo; t < w.hi; ++t) {
+        if (!(ok = wait(s.full[2 * k_ring.at], k_ring.turn))) break;
         tc_fence_after();
-        if (lane == 0) {
-          uint32_t at = S::slot(slots0, slot), qat = q0;
-          asm volatile("" : "+r"(at), "+r"(qat));
-          const uint32_t kd = desc_low(at, 16), qd = desc_low(qat, 16);
-          uint32_t to = tmem + b * S::kSP, id = is;
-          asm volatile("" : "+r"(to), "+r"(id));
+        uint32_t kd = desc_low(S::slot(slots0, 2 * k_ring.at), 16), qd = desc_low(q0, 16);
+        uint32_t to = tmem + sp_ring.at * S::kSP, id = is;
+        asm volatile("" : "+r"(kd), "+r"(qd), "+r"(to), "+r"(id));
 #pragma unroll
-          for (int qp = S::QP - 1; qp >= 0; --qp)
+        for (int qp = S::QP - 1; qp >= 0; --qp)
 #pragma unroll
-            for (int kp = S::KP - 1; kp >= 0; --kp) {
-              if (S::KP > 1 && qp + kp > 2) continue;
-              constexpr int kFirst = S::KP > 1 ? 1 : 0;
+          for (int kp = S::KP - 1; kp >= 0; --kp) {
+            if (kThree && qp + kp > 2) continue;
 #pragma unroll
-              for (int k = 0; k < S::DP / 16; ++k)
-                if (k < ksteps)
-                  mma_f16_ss(to, qd + ((qp * S::kQPart + (k >> 2) * (S::ROWS * 128) + (k & 3) * 32) >> 4),
-                             kd + ((kp * S::kKPart + (k >> 2) * (TK * 128) + (k & 3) * 32) >> 4), id,
-                             !(qp == S::QP - 1 && kp == (kFirst ? 2 - qp : 0) && k == 0));
-            }
-          umma_commit<1>(&s.sfull[b]);
-          umma_commit<1>(&s.empty[slot]);
-          if (t + 1 == w.hi) umma_commit<1>(&s.qfree);
-        }
-        __syncwarp();
-        if (t > w.lo && !(ok = values(it - 1))) break;
+            for (int k = 0; k < S::DP / 16; ++k)
+              mma_f16_ss(k < ksteps ? one : 0u, to, qd + ((qp * S::kQPart + (k >> 2) * (S::ROWS * 128) + (k & 3) * 32) >> 4),
+                         kd + ((kp * S::kKPart + (k >> 2) * (TK * 128) + (k & 3) * 32) >> 4), id,
+                         !(qp == S::QP - 1 && kp == (kThree ? 2 - qp : 0) && k == 0));
+          }
+        commit_on(one, smem_u32(&s.sfull[sp_ring.at]));
+        commit_on(one, smem_u32(&s.empty[2 * k_ring.at]));
+        if (t + 1 == w.hi) commit_on(one, smem_u32(&s.qfree));
+        sp_ring.next();
+        k_ring.next();
+        ++scored;
+        if (t > w.lo && !(ok = values())) break;
       }
       if (!ok) break;
     }
-    if (ok && it > 0) ok = values(it - 1) && wait(&s.empty[(2 * it - 1) % SLOTS], (2 * it - 1) / SLOTS);
-    if (!ok && lane == 0) {  // the products under way end before their memory goes
-      umma_commit<1>(&s.drain);
-      mbar_drain(&s.drain, 0, limit);
+    if (ok && scored > summed) {
+      const Ring<SLOTS / 2> last = v_ring;
+      ok = values() && wait(s.empty[2 * last.at + 1], last.turn);
+    }
+    if (!ok) {  // the products under way end before their memory goes
+      commit_on(one, smem_u32(&s.drain));
+      mbar_drain(&s.drain, 0, kDefaultWaitNs);
     }
     __syncwarp();
-  } else if (S::KP == 1 && warp == kIssueWarp + 1) {
-    // ---- copies of keys and values: boxes of as many positions as lie in one page
-    const int rows = a.box_rows, boxes = TK / rows, kc = (d + 63) / 64;
-    int item = 0, unit = 0;
+  } else if (S::KP == 1 && warp <= kIssueWarp + 2) {
+    // ---- copies of keys, or of values: boxes of as many positions as lie in one page
+    const bool values = warp == kIssueWarp + 2;
+    const int rows = a.box_rows, boxes = TK / rows;
+    const CUtensorMap* map = values ? &vmap : &kmap;
+    const uint32_t one = elected();
+    Ring<SLOTS / 2> pair;
+    int unit = 0, it = 0;
     bool ok = true;
 #pragma unroll 1
     for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
       const int32_t* pages = a.kv.pages_of(w.e.seq);
-      const int keys = w.e.len + w.e.nodes, vc = (min(S::VD, d - w.ch0) + 63) / 64;
+      const int keys = w.e.len + w.e.nodes, x0 = values ? w.ch0 : 0;
+      const int chunks = ((values ? min(S::VD, d - w.ch0) : d) + 63) / 64;
       auto page_of = [&](int t, int i) {  // of box i; behind the last key none
         const int key = t * TK + i * rows;
         return i < boxes && key < keys ? pages[a.kv.ordinal(key)] : a.kv.num_pages;
       };
       int next[2] = {page_of(w.lo, lane), page_of(w.lo, lane + 32)};
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi && ok; ++t) {
+      for (int t = w.lo; t < w.hi; ++t, ++it, pair.next()) {
         int page[2];
         bool bad = false;
 #pragma unroll
@@ -611,70 +678,51 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           kv_report(a.status, ER_KV_BAD_PAGE);
           s.bad_unit[unit & 15] = unit + 1;
         }
+        const int slot = 2 * pair.at + values;
+        if (it >= SLOTS / 2 && !(ok = wait(s.empty[slot], pair.turn ^ 1))) break;
+        // values of a tile with drafted keys are looked at before they count
+        const uint32_t bar = smem_u32(values && (t + 1) * TK > w.e.len ? &s.raw[slot] : &s.full[slot]);
+        asm volatile(
+            "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
+            "@g mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+            "r"(chunks * TK * 128), "r"(one)
+            : "memory");
+        uint32_t to = S::slot(slots0, slot);
+        int at = a.kv.slot(t * TK);
 #pragma unroll 1
-        for (int kind = 0; kind < 2; ++kind, ++item) {  // keys, values
-          const int slot = item % SLOTS, chunks = kind ? vc : kc, x0 = kind ? w.ch0 : 0;
-          if (item >= SLOTS && !(ok = wait(&s.empty[slot], item / SLOTS - 1))) break;
-          // values of a tile with drafted keys are looked at before they count
-          const bool look = kind && (t + 1) * TK > w.e.len;
-          uint64_t* bar = look ? &s.raw[slot] : &s.full[slot];
-          if (lane == 0) {
-            mbar_expect_tx(bar, chunks * TK * 128);
-            if (!look)
-              for (int i = 1; i < S::kFixWarps; ++i) mbar_arrive(bar);
-          }
-          __syncwarp();
-          const uint32_t to = S::slot(slots0, slot);
-          // one lane issues all copies: their operands are the warp's, not a lane's
-          for (int i = 0; i < boxes; ++i) {
-            const int pg = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31);
-            if (lane == 0) {
-              const int at = a.kv.slot(t * TK + i * rows);
-              for (int c = 0; c < chunks; ++c) {
-                if (kind)
-                  tma_box(to + c * (TK * 128) + i * rows * 128, &vmap, bar, x0 + c * 64, at, w.head, pg);
-                else
-                  tma_box(to + c * (TK * 128) + i * rows * 128, &kmap, bar, c * 64, at, w.head, pg);
-              }
-            }
-          }
-          __syncwarp();
+        for (int i = 0; i < boxes; ++i, to += rows * 128, at += rows) {
+          if (at == a.kv.page_size) at = 0;
+          const int pg = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31);
+#pragma unroll
+          for (int c = 0; c < S::DP / 64; ++c)
+            if (c < chunks) tma_box(one, to + c * (TK * 128), map, bar, x0 + c * 64, at, w.head, pg);
         }
       }
     }
-    // nothing of its copies is under way when the CTA's memory goes
-    if (!ok || s.abort)
-      for (int i = 0; i < SLOTS; ++i) {
-        const int last = item - 1 - (item - 1 - i + SLOTS * 4) % SLOTS;  // the last item of slot i
-        if (item > 0 && last >= 0 && last < item) {
-          mbar_drain(&s.full[i], (last / SLOTS) & 1, limit / 8);
-        }
+    if (!ok || s.abort) {  // no copy is under way when the CTA's memory goes: they take microseconds
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
       }
+    }
   } else {
     // ---- queries, and drafted values (bf16 caches) or all keys and values (fp32 caches)
     const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kFixWarps);
     const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
-    int item = 0, unit = 0, looks = 0;
+    int unit = 0, it = 0, looks = 0;
+    Ring<SLOTS / 2> pair;
     bool ok = true;
-    auto signal = [&](uint64_t* bar) {
+    auto signal = [&](const uint64_t& b) {
       async_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
+      arrive(b);
     };
 #pragma unroll 1
     for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
-      if (unit > 0) {
-        if (!(ok = wait(&s.qfree, unit - 1))) break;
-        load_queries<S, TQ>(a, w, q0, loader, S::kFixWarps);
-        signal(&s.qfull);
-      }
       const int keys = w.e.len + w.e.nodes;
       if constexpr (S::KP == 1) {
-        item += 2 * (w.hi - w.lo);
-        const int first = max(w.lo, w.e.len / TK);
-        for (int t = first; t < w.hi; ++t) {  // tiles with drafted keys, or none
-          const int it = item / 2 - (w.hi - t), n = 2 * it + 1, slot = n % SLOTS;
-          if (!(ok = wait(&s.raw[slot], looks >> slot))) break;
+        for (int t = w.lo; t < w.hi; ++t, pair.next()) {
+          if ((t + 1) * TK <= w.e.len) continue;  // neither drafted keys nor places behind the last
+          const int slot = 2 * pair.at + 1;
+          if (!(ok = wait(s.raw[slot], looks >> slot & 1))) break;
           looks ^= 1 << slot;
           const uint32_t to = S::slot(slots0, slot);
           uint32_t marks[2] = {0, 0};
@@ -696,7 +744,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
             if (lane == 0) s.vbad[slot][loader][i] = marks[i];
           }
-          signal(&s.full[slot]);
+          signal(s.full[slot]);
         }
       } else {
         constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;  // of four rows, eight lanes a row
@@ -710,7 +758,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         };
         int page = page_of(w.lo);
 #pragma unroll 1
-        for (int t = w.lo; t < w.hi && ok; ++t) {
+        for (int t = w.lo; t < w.hi && ok; ++t, ++it, pair.next()) {
           long long off = -1;
           const int key = t * TK + own;
           if (lane < GROUPS * 4 && own < TK && key < keys) {
@@ -724,9 +772,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           if (t + 1 < w.hi) page = page_of(t + 1);
           __syncwarp();
 #pragma unroll 1
-          for (int kind = 0; kind < 2; ++kind, ++item) {  // keys, values
-            const int slot = item % SLOTS;
-            if (item >= SLOTS && !(ok = wait(&s.empty[slot], item / SLOTS - 1))) break;
+          for (int kind = 0; kind < 2; ++kind) {  // keys, values
+            const int slot = 2 * pair.at + kind;
+            if (it >= SLOTS / 2 && !(ok = wait(s.empty[slot], pair.turn ^ 1))) break;
             const uint32_t to = S::slot(slots0, slot);
             const char* pool = kind ? a.kv.v + w.ch0 * 4 : a.kv.k;
             const bool look = kind && (t + 1) * TK > w.e.len;
@@ -773,7 +821,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                 if (lane == 0) s.vbad[slot][loader][i] = marks[i];
               }
             }
-            signal(&s.full[slot]);
+            signal(s.full[slot]);
           }
         }
       }
