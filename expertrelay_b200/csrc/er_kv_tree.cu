@@ -167,8 +167,8 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   a.cut = (TreeCut*)(ws + L.cut);
   a.part_ml = (float*)(ws + L.ml);
   a.part_o = (float*)(ws + L.o);
-  a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
-  int box = kTreeTile;
+  a.tile = L.shape.tile, a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
+  int box = L.shape.tile;
   while (cache->page_size % box) box >>= 1;
   a.box_rows = box;
   if (cb) {

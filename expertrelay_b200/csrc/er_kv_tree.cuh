@@ -13,7 +13,7 @@
 namespace er {
 
 constexpr int kMaxTrees = 4096, kMaxNodes = 256;
-constexpr int kTreeTile = 64, kTreeRows = 128;  // keys of a tile, rows of a matrix product
+constexpr int kTreeRows = 128;  // of a matrix product
 constexpr int kTreeChannels = 128;  // of the values, at most, that a unit has
 
 // A unit whose tiles several CTAs share: the first of them writes it, the join reads it.
@@ -35,6 +35,7 @@ struct TreeArgs {
   int* status;
   int q_wide;              // rows of q on 16-byte boundaries
   int q_flip, q_zero;      // the scale was negative, or zero: queries change their sign, or are zero
+  int tile;                // keys of a tile
   int block_rows;          // query rows of a unit at most
   int channels, halves;    // of the values: those of a unit, units beside each other for all of them
   int box_rows;            // positions that a copy takes: they lie in one page wherever it begins
@@ -91,7 +92,7 @@ __device__ __forceinline__ TreeUnits tree_units(const TreeArgs& a, const Tree& e
   u.blocks = (u.rows + a.block_rows - 1) / a.block_rows;
   u.per = (u.rows + u.blocks - 1) / u.blocks;
   u.units = u.blocks * a.halves * a.kv.kv_heads;
-  u.tiles = (e.len + e.nodes + kTreeTile - 1) / kTreeTile;
+  u.tiles = (e.len + e.nodes + a.tile - 1) / a.tile;
   return u;
 }
 
@@ -216,14 +217,18 @@ struct TreeWalk {
   }
 };
 
-// What a launch of the attention kernel takes: query rows of a unit, its
-// channels and how many units have the others.
+// What a launch of the attention kernel takes: keys of a tile, query rows of a
+// unit, its channels and how many units have the others.
 struct TreeLaunch {
-  int rows, channels, halves;
+  int tile, rows, channels, halves;
 };
 // er_kv_tree_bf16.cu and er_kv_tree_f32.cu: for caches of either type
 TreeLaunch tree_shape_bf16(int d, int q_dtype);
 TreeLaunch tree_shape_f32(int d);
+template <typename S>
+constexpr TreeLaunch tree_shape() {
+  return TreeLaunch{S::TK, S::ROWS, S::VD, S::DP / S::VD};
+}
 int tree_bf16(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st);
 int tree_f32(const TreeArgs& a, int q_dtype, cudaStream_t st);
 

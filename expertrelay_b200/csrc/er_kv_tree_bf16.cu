@@ -5,16 +5,17 @@ namespace er {
 
 namespace {
 using bf = __nv_bfloat16;
-using B64 = TreeShape<1, 1, 2, 64, 128, 6>;
-using B128 = TreeShape<1, 1, 2, 128, 128, 4>;
-using B256 = TreeShape<1, 1, 2, 256, 128, 2>;
-using F64 = TreeShape<1, 3, 3, 64, 128, 6>;
-using F128 = TreeShape<1, 3, 3, 128, 128, 3>;
-using F256 = TreeShape<1, 3, 3, 256, 64, 2>;
+using B64 = TreeShape<1, 1, 2, 64, 128, 64, 6, 6>;
+using B128 = TreeShape<1, 1, 2, 128, 128, 64, 4, 4>;
+using B256 = TreeShape<1, 1, 2, 256, 128, 64, 2, 2>;
+using F64 = TreeShape<1, 3, 3, 64, 128, 64, 6, 6>;
+using F128 = TreeShape<1, 3, 3, 128, 128, 64, 3, 3>;
+using F256 = TreeShape<1, 3, 3, 256, 64, 64, 2, 2>;
 }  // namespace
 
 TreeLaunch tree_shape_bf16(int d, int q_dtype) {
-  return TreeLaunch{d > 128 && q_dtype == ER_DTYPE_F32 ? F256::ROWS : kTreeRows, d <= 64 ? 64 : kTreeChannels, d > 128 ? 2 : 1};
+  if (q_dtype == ER_DTYPE_BF16) return d <= 64 ? tree_shape<B64>() : d <= 128 ? tree_shape<B128>() : tree_shape<B256>();
+  return d <= 64 ? tree_shape<F64>() : d <= 128 ? tree_shape<F128>() : tree_shape<F256>();
 }
 
 int tree_bf16(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st) {

@@ -4,9 +4,9 @@
 namespace er {
 
 namespace {
-using S64 = TreeShape<3, 3, 3, 64, 128, 2>;
-using S128 = TreeShape<3, 3, 3, 128, 128, 1>;
-using S256 = TreeShape<3, 3, 3, 256, 32, 1>;
+using S64 = TreeShape<3, 3, 3, 64, 128, 64, 2, 2>;
+using S128 = TreeShape<3, 3, 3, 128, 128, 64, 1, 1>;
+using S256 = TreeShape<3, 3, 3, 256, 32, 64, 1, 1>;
 
 template <typename TQ>
 int launch(const TreeArgs& a, cudaStream_t st) {
@@ -19,7 +19,7 @@ int launch(const TreeArgs& a, cudaStream_t st) {
 }  // namespace
 
 TreeLaunch tree_shape_f32(int d) {
-  return TreeLaunch{d > 128 ? S256::ROWS : kTreeRows, d <= 64 ? 64 : kTreeChannels, d > 128 ? 2 : 1};
+  return d <= 64 ? tree_shape<S64>() : d <= 128 ? tree_shape<S128>() : tree_shape<S256>();
 }
 
 int tree_f32(const TreeArgs& a, int q_dtype, cudaStream_t st) {

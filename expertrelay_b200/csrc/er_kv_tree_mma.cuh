@@ -15,28 +15,29 @@ constexpr int kStagePitch = 36;  // floats of a row of the epilogue's exchange: 
 
 // KP: bf16 parts of a key or value in shared memory (1: as they come from a bf16 cache, 3: of fp32), QP of a query,
 // PP of a weight. DP: head_dim padded. ROWS: rows of queries in shared memory (of 128 of a product; the others are
-// whatever lies there). PAIRS: stages, each a tile of keys and one of VD channels of values.
-template <int KP_, int QP_, int PP_, int DP_, int ROWS_, int PAIRS_>
+// whatever lies there). TK: keys of a tile. KS, VS: tiles of keys and of values (VD channels of them) in shared memory.
+template <int KP_, int QP_, int PP_, int DP_, int ROWS_, int TK_, int KS_, int VS_>
 struct TreeShape {
-  static constexpr int KP = KP_, QP = QP_, PP = PP_, DP = DP_, ROWS = ROWS_, SLOTS = 2 * PAIRS_;
+  static constexpr int KP = KP_, QP = QP_, PP = PP_, DP = DP_, ROWS = ROWS_, TK = TK_, KS = KS_, VS = VS_;
   static constexpr int VD = DP < kTreeChannels ? DP : kTreeChannels;
-  static constexpr int kKPart = kTreeTile * DP * 2, kVPart = kTreeTile * VD * 2;  // bytes of one part of a tile
-  static constexpr int kPair = (kKPart + kVPart) * KP;
+  static constexpr int kKPart = TK * DP * 2, kVPart = TK * VD * 2;  // bytes of one part of a tile
+  static constexpr int kKSlot = kKPart * KP, kVSlot = kVPart * KP;
   static constexpr int kQPart = ROWS * DP * 2, kQ = kQPart * QP;
-  static constexpr int kSP = PP * 32 > 64 ? PP * 32 : 64;  // columns of a tile's scores, then of its weights
-  static constexpr int kSmem = kQ + PAIRS_ * kPair + ROWS * kStagePitch * 4;
+  // columns of a tile's scores, then of its weights: by 64 keys, two parts over the scores, a third one behind them
+  static constexpr int kSP = PP > 2 ? TK * 3 / 2 : TK;
+  static constexpr int OB = 2 * kSP + 2 * VD <= 512 ? 2 : 1;  // results of a tile, kept while they are read
+  static constexpr int kSmem = kQ + KS * kKSlot + VS * kVSlot + ROWS * kStagePitch * 4;
   // warps that fill shared memory: of a bf16 cache one that issues the keys' copies, one the values' and one that
   // looks after the drafted values, of an fp32 cache all of them by way of registers
   static constexpr int kLoadWarps = KP == 1 ? 3 : 7, kFixWarps = KP == 1 ? 1 : 7;
   static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
-  static __device__ __forceinline__ uint32_t slot(uint32_t base, int i) {
-    return base + (i >> 1) * kPair + (i & 1) * kKPart * KP;
-  }
+  // the column of a tile's weights: part p of the 64 keys from 64 h on
+  static __device__ __forceinline__ constexpr int column(int h, int p) { return p < 2 ? h * 64 + p * 32 : TK + h * 32; }
 };
 
 template <typename S>
 struct TreeShared {
-  uint64_t full[S::SLOTS], empty[S::SLOTS], raw[S::SLOTS];
+  uint64_t kfull[S::KS], kempty[S::KS], vfull[S::VS], vempty[S::VS], raw[S::VS];
   uint64_t qfirst, qfull, qfree, sfull[2], pfull[2], ofull[2], ofree[2], staged, masked, drain;
   uint32_t tmem;
   volatile int abort;
@@ -45,7 +46,7 @@ struct TreeShared {
   int bad_tree[2], parents[2][kMaxNodes];  // of units in turn: a warp may be one ahead of another
   int bad_unit[16];                 // units (numbers + 1) of a bad page, in turn
   uint32_t sees[S::ROWS][9];        // each row's ancestors and itself, a bit a node
-  uint32_t vbad[S::SLOTS][S::kFixWarps][2];  // keys of a slot whose value was no number (drafted ones)
+  uint32_t vbad[S::VS][S::kFixWarps][S::TK / 32];  // keys of a tile whose value was no number (drafted ones)
   float by[4][S::ROWS];             // what a tile's sums so far are multiplied by
   float2 ml[4][S::ROWS];            // maximum and sum of a unit's last tile
 };
@@ -155,14 +156,36 @@ __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// two floats rounded to bf16, packed, the first one low; x, y become what is left
-__device__ __forceinline__ uint32_t split2(float& x, float& y) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-  x -= __uint_as_float(r << 16);
-  y -= __uint_as_float(r & 0xffff0000u);
+// Two floats at a time: the arithmetic of the weights is bound by instructions.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
   return r;
 }
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// two floats rounded to bf16, packed, the first one low
+__device__ __forceinline__ uint32_t round2(uint64_t v) {
+  float x, y;
+  unpack2(v, x, y);
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+  return r;
+}
+// what rounding to `h` has left of v
+__device__ __forceinline__ uint64_t rest2(uint64_t v, uint32_t h) {
+  return fma2(pack2(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u)), pack2(-1.f, -1.f), v);
+}
+
 // Eight floats as three bf16 parts, cut, whose sum they are exactly. A part that is zero where the value is not
 // takes the least value of its sign: times an infinite key it stays infinite, beside a finite one it vanishes.
 __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[3]) {
@@ -285,19 +308,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                    const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char raw[];
   __shared__ TreeShared<S> s;
-  constexpr int TK = kTreeTile, SLOTS = S::SLOTS;
+  constexpr int TK = S::TK, KS = S::KS, VS = S::VS, OB = S::OB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.kv.d;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;  // swizzled tiles repeat every 1024 bytes
   // the queries first: products read 128 rows from there, whatever lies behind S::ROWS
-  const uint32_t q0 = base, slots0 = base + S::kQ;
-  float* stage = reinterpret_cast<float*>(raw + (base - smem_u32(raw)) + S::kQ + SLOTS / 2 * S::kPair);
+  const uint32_t q0 = base, k0 = q0 + S::kQ, v0 = k0 + KS * S::kKSlot;
+  float* stage = reinterpret_cast<float*>(raw + (v0 + VS * S::kVSlot - smem_u32(raw)));
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SLOTS; ++i) {
-      mbar_init(&s.full[i], S::kFixWarps);
-      mbar_init(&s.empty[i], 1);
-      mbar_init(&s.raw[i], 1);
-    }
+    for (int i = 0; i < KS; ++i) mbar_init(&s.kfull[i], S::kFixWarps), mbar_init(&s.kempty[i], 1);
+    for (int i = 0; i < VS; ++i)
+      mbar_init(&s.vfull[i], S::kFixWarps), mbar_init(&s.vempty[i], 1), mbar_init(&s.raw[i], 1);
     mbar_init(&s.qfirst, kIssueWarp);
     mbar_init(&s.qfull, kSoftmaxWarps);
     mbar_init(&s.qfree, 1);
@@ -340,7 +361,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     // ---- weights: a thread a row, of one replica's share of the tile's keys
     int it = 0, masks = 0, unit = 0;
     Ring<2> sp_ring;
-    Ring<SLOTS / 2> pair;
+    Ring<VS> v_ring;
 #pragma unroll 1
     for (bool go = w.begin(); go && !s.abort; go = w.next(), ++unit) {
       if (unit > 0) {  // the first one's are on their way
@@ -375,75 +396,111 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
       float m = -INFINITY, l = 0.f;
       if (drafted && s.bad_tree[(masks - 1) & 1] == masks) l = __int_as_float(0x7fc00000);
-      auto tile = [&](auto replicas, int t) {
-        constexpr int RR = decltype(replicas)::value, KPT = TK / RR;
-        const int key0 = t * TK + slice * KPT;
-        const uint32_t sp = tmem + ((uint32_t)(warp * 32) << 16) + sp_ring.at * S::kSP;
-        uint32_t x[KPT];
-        if constexpr (KPT == 64) {
-          tmem_ld32(sp, x);
-          tmem_ld32(sp + 32, x + 32);
-        } else if constexpr (KPT == 32) {
-          tmem_ld32(sp + slice * 32, x);
+      const uint32_t sp0 = tmem + ((uint32_t)(warp * 32) << 16);
+      // N scores of this row into x: those of the keys from key on of tile t, -inf where the row does not see them
+      auto scores = [&](auto& x, int t, int key) {
+        constexpr int N = sizeof(x) / 4;
+        const uint32_t sp = sp0 + sp_ring.at * S::kSP + key;
+        if constexpr (N == 16) {
+          tmem_ld16(sp, x);
         } else {
-          tmem_ld16(sp + slice * 16, x);
+          tmem_ld32(sp, x);
+          if constexpr (N == 64) tmem_ld32(sp + 32, x + 32);
         }
         tmem_wait_ld();
-        if (key0 + KPT > w.e.len) {  // drafted keys, or none: what the row sees of them
-          const int slot = 2 * pair.at + 1;
+        const int node0 = t * TK + key - w.e.len;
+        if (node0 + N > 0) {  // drafted keys, or none
           uint32_t spoils = 0;
 #pragma unroll
-          for (int c = 0; c < KPT; c += 32) {
-            const uint32_t see = seen_from(sees, key0 + c - w.e.len);
+          for (int c = 0; c < N; c += 32) {
+            const uint32_t see = seen_from(sees, node0 + c);
 #pragma unroll
-            for (int j = c; j < KPT && j < c + 32; ++j)
+            for (int j = c; j < N && j < c + 32; ++j)
               if (!(see >> (j - c) & 1)) x[j] = 0xff800000u;
             uint32_t vb = 0;
-            const int first = slice * KPT + c;  // of the tile's keys
-            for (int i = 0; i < S::kFixWarps; ++i) vb |= s.vbad[slot][i][first >> 5] >> (first & 31);
-            spoils |= vb & see & (KPT < 32 ? (1u << (KPT & 31)) - 1 : 0xffffffffu);
+            for (int i = 0; i < S::kFixWarps; ++i) vb |= s.vbad[v_ring.at][i][(key + c) >> 5] >> ((key + c) & 31);
+            spoils |= vb & see & (N < 32 ? (1u << (N & 31)) - 1 : 0xffffffffu);
           }
           if (spoils) l = __int_as_float(0x7fc00000);
         }
-        float top = m;
+      };
+      // the weights of N scores, as they are multiplied: in parts, into column c of the 64 keys from 64 h on; their sum
+      auto weights = [&](auto& x, float shift, int h, int c) {
+        constexpr int N = sizeof(x) / 4;
+        const uint32_t sp = sp0 + sp_ring.at * S::kSP + c;
+        const uint64_t scale = pack2(a.scale, a.scale), by = pack2(shift, shift);
+        uint64_t sum = 0;  // of even and of odd keys
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) top = fmaxf(top, __uint_as_float(x[j]));
-        const float ref = top == -INFINITY ? 0.f : top, shift = -ref * a.scale, by = ex2(fmaf(m, a.scale, shift));
-        m = top;
-        float sum = 0.f;
+        for (int i = 0; i < N / 2; i += 8) {
+          uint64_t p[8];
+          uint32_t y[8];
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-          const float p = ex2(fmaf(__uint_as_float(x[j]), a.scale, shift));
-          x[j] = __float_as_uint(p);
-          sum += p;
-        }
-        l = l * by + sum;
-        if (row < S::ROWS) s.by[it & 3][row] = by;
-        __syncwarp();
+          for (int j = 0; j < 8; ++j) {
+            float u, v;
+            unpack2(fma2(pack2(__uint_as_float(x[2 * (i + j)]), __uint_as_float(x[2 * (i + j) + 1])), scale, by), u, v);
+            p[j] = pack2(ex2(u), ex2(v));
+            sum = add2(sum, p[j]);
+          }
 #pragma unroll
-        for (int part = 0; part < S::PP; ++part) {
-#pragma unroll
-          for (int c = 0; c < KPT / 2; c += 8) {
-            uint32_t y[8];
+          for (int part = 0; part < S::PP; ++part) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              float u = __uint_as_float(x[2 * (c + j)]), v = __uint_as_float(x[2 * (c + j) + 1]);
-              y[j] = split2(u, v);
-              x[2 * (c + j)] = __float_as_uint(u);
-              x[2 * (c + j) + 1] = __float_as_uint(v);
+              y[j] = round2(p[j]);
+              if (part + 1 < S::PP) p[j] = rest2(p[j], y[j]);
             }
-            tmem_st8(sp + part * 32 + slice * (KPT / 2) + c, y);
+            tmem_st8(sp + S::column(h, part) + i, y);
           }
-          const uint32_t zero[8] = {};  // the other keys are other replicas'
+        }
+        float even, odd;
+        unpack2(sum, even, odd);
+        return even + odd;
+      };
+      // what the sums so far are multiplied by, once the greatest score is `top`, and the exponents' shift
+      auto rise = [&](float top, float* shift) {
+        const float ref = top == -INFINITY ? 0.f : top;
+        *shift = -ref * a.scale;
+        const float by = ex2(fmaf(m, a.scale, *shift));
+        m = top;
+        if (row < S::ROWS) s.by[it & 3][row] = by;
+        __syncwarp();
+        return by;
+      };
+      auto tile = [&](auto replicas, int t) {
+        constexpr int RR = decltype(replicas)::value, KPT = TK / RR, N = KPT < 64 ? KPT : 64;
+        uint32_t x[N];
+        float top = m, shift;
+        const int key = slice * KPT;
+        scores(x, t, key);
 #pragma unroll
-          for (int c = KPT / 2; c < 32; c += 8) tmem_st8(sp + part * 32 + ((slice * (KPT / 2) + c) & 31), zero);
+        for (int j = 0; j < N; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+        if constexpr (KPT == 128) {  // the other half; then the first one's scores once more
+          scores(x, t, 64);
+#pragma unroll
+          for (int j = 0; j < N; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+          const float by = rise(top, &shift);
+          float sum = weights(x, shift, 1, 0);
+          scores(x, t, 0);
+          sum += weights(x, shift, 0, 0);
+          l = l * by + sum;
+        } else {
+          const float by = rise(top, &shift);
+          l = l * by + weights(x, shift, key >> 6, (key & 63) / 2);
+        }
+        // the other keys are other replicas'
+        const uint32_t zero[8] = {};
+        const uint32_t sp = sp0 + sp_ring.at * S::kSP;
+#pragma unroll
+        for (int c = KPT / 2; c < TK / 2; c += 8) {
+          const int at = (key / 2 + c) & (TK / 2 - 1);
+#pragma unroll
+          for (int part = 0; part < S::PP; ++part) tmem_st8(sp + S::column(at >> 5, part) + (at & 31), zero);
         }
       };
       bool ok = true;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it, sp_ring.next(), pair.next()) {
+      for (int t = w.lo; t < w.hi; ++t, ++it, sp_ring.next(), v_ring.next()) {
         if (!(ok = wait(s.sfull[sp_ring.at], sp_ring.turn))) break;
-        if ((t + 1) * TK > w.e.len && !(ok = wait(s.full[2 * pair.at + 1], pair.turn))) break;
+        if ((t + 1) * TK > w.e.len && !(ok = wait(s.vfull[v_ring.at], v_ring.turn))) break;
         tc_fence_after();
         if (live) {
           if (R == 1)
@@ -468,14 +525,14 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     constexpr int CH = S::VD / 2;
     const int row = (warp & 3) * 32 + lane, half = (warp - kSoftmaxWarps) >> 2, id = threadIdx.x - kSoftmaxWarps * 32;
     int it = 0;
-    Ring<2> o_ring;
+    Ring<OB> o_ring;
     uint32_t stages = 0;
     if (id == 0) a.cut[blockIdx.x].live = 0;
 #pragma unroll 1
     for (bool go = w.begin(); go && !s.abort; go = w.next()) {
-      float o[CH];
+      uint64_t o[CH / 2];  // two channels each
 #pragma unroll
-      for (int c = 0; c < CH; ++c) o[c] = 0.f;
+      for (int c = 0; c < CH / 2; ++c) o[c] = 0;
       const int R = w.replicas(), per = S::ROWS / R, vd = min(S::VD, d - w.ch0);
       const bool there = row < S::ROWS, live = __any_sync(0xffffffffu, there && row % per < w.live);
       bool ok = true;
@@ -486,7 +543,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         if (!(ok = wait(s.ofull[ob], o_ring.turn))) break;  // after the tile's weights, so `by` and `ml` are there
         tc_fence_after();
         if (live) {
-          const float by = there ? s.by[it & 3][row] : 0.f;
+          const float by1 = there ? s.by[it & 3][row] : 0.f;
+          const uint64_t by = pack2(by1, by1);
           const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 2 * S::kSP + ob * S::VD + half * CH;
           constexpr int N = S::kThreads > 512 ? 16 : 32;  // registers
 #pragma unroll
@@ -498,7 +556,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
               tmem_ld16(at + c, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int j = 0; j < N; ++j) o[c + j] = fmaf(o[c + j], by, __uint_as_float(x[j]));
+            for (int j = 0; j < N; j += 2)
+              o[(c + j) / 2] = fma2(o[(c + j) / 2], by, pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
           }
         }
         if (t + 1 == w.hi && there) ml = s.ml[it & 3][row];
@@ -517,7 +576,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           float* mine = stage + row * kStagePitch + half * 16;
 #pragma unroll
           for (int j = 0; j < 16; j += 4)
-            *reinterpret_cast<float4*>(mine + j) = make_float4(o[c0 + j], o[c0 + j + 1], o[c0 + j + 2], o[c0 + j + 3]);
+            *reinterpret_cast<ulonglong2*>(mine + j) = make_ulonglong2(o[(c0 + j) / 2], o[(c0 + j) / 2 + 1]);
           if (c0 == 0 && half == 0) *reinterpret_cast<float2*>(stage + row * kStagePitch + 32) = ml;
         }
         arrive(s.staged);
@@ -570,14 +629,16 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     uint32_t io = 0;
     constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
     Ring<2> sp_ring, p_ring;            // of the tile whose scores, whose values are next
-    Ring<SLOTS / 2> k_ring, v_ring;
+    Ring<OB> o_ring;
+    Ring<KS> k_ring;
+    Ring<VS> v_ring;
     auto values = [&]() {  // out += P V of the tile before
-      const int b = p_ring.at;
-      if (!wait(s.pfull[b], p_ring.turn) || !wait(s.full[2 * v_ring.at + 1], v_ring.turn)) return false;
-      if (summed >= 2 && !wait(s.ofree[b], p_ring.turn ^ 1)) return false;
+      const int b = o_ring.at;
+      if (!wait(s.pfull[p_ring.at], p_ring.turn) || !wait(s.vfull[v_ring.at], v_ring.turn)) return false;
+      if (summed >= OB && !wait(s.ofree[b], o_ring.turn ^ 1)) return false;
       tc_fence_after();
-      uint32_t v = desc_low(S::slot(slots0, 2 * v_ring.at + 1), TK * 128);
-      uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + b * S::kSP, id = io;
+      uint32_t v = desc_low(v0 + v_ring.at * S::kVSlot, TK * 128);
+      uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = io;
       // put together here: descriptors that the compiler kept from before the waits' calls came out wrong
       asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
       // the small products first
@@ -588,12 +649,13 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           if (kThree && pp + kp > 2) continue;
 #pragma unroll
           for (int k = 0; k < TK / 16; ++k)
-            mma_f16_ts(one, to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
+            mma_f16_ts(one, to, p + S::column(k >> 2, pp) + (k & 3) * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
                        !(pp == S::PP - 1 && kp == (kThree ? 2 - pp : 0) && k == 0));
         }
       commit_on(one, smem_u32(&s.ofull[b]));
-      commit_on(one, smem_u32(&s.empty[2 * v_ring.at + 1]));
+      commit_on(one, smem_u32(&s.vempty[v_ring.at]));
       p_ring.next();
+      o_ring.next();
       v_ring.next();
       ++summed;
       return true;
@@ -606,9 +668,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
 #pragma unroll 1
       for (int t = w.lo; t < w.hi; ++t) {
-        if (!(ok = wait(s.full[2 * k_ring.at], k_ring.turn))) break;
+        if (!(ok = wait(s.kfull[k_ring.at], k_ring.turn))) break;
         tc_fence_after();
-        uint32_t kd = desc_low(S::slot(slots0, 2 * k_ring.at), 16), qd = desc_low(q0, 16);
+        uint32_t kd = desc_low(k0 + k_ring.at * S::kKSlot, 16), qd = desc_low(q0, 16);
         uint32_t to = tmem + sp_ring.at * S::kSP, id = is;
         asm volatile("" : "+r"(kd), "+r"(qd), "+r"(to), "+r"(id));
 #pragma unroll
@@ -623,7 +685,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                          !(qp == S::QP - 1 && kp == (kThree ? 2 - qp : 0) && k == 0));
           }
         commit_on(one, smem_u32(&s.sfull[sp_ring.at]));
-        commit_on(one, smem_u32(&s.empty[2 * k_ring.at]));
+        commit_on(one, smem_u32(&s.kempty[k_ring.at]));
         if (t + 1 == w.hi) commit_on(one, smem_u32(&s.qfree));
         sp_ring.next();
         k_ring.next();
@@ -633,8 +695,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       if (!ok) break;
     }
     if (ok && scored > summed) {
-      const Ring<SLOTS / 2> last = v_ring;
-      ok = values() && wait(s.empty[2 * last.at + 1], last.turn);
+      const Ring<VS> last = v_ring;
+      ok = values() && wait(s.vempty[last.at], last.turn);
     }
     if (!ok) {  // the products under way end before their memory goes
       commit_on(one, smem_u32(&s.drain));
@@ -644,11 +706,11 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   } else if (S::KP == 1 && warp <= kIssueWarp + 2) {
     // ---- copies of keys, or of values: boxes of as many positions as lie in one page
     const bool values = warp == kIssueWarp + 2;
-    const int rows = a.box_rows, boxes = TK / rows;
+    const int rows = a.box_rows, boxes = TK / rows, ring = values ? VS : KS;
     const CUtensorMap* map = values ? &vmap : &kmap;
-    const uint32_t one = elected();
-    Ring<SLOTS / 2> pair;
-    int unit = 0, it = 0;
+    const uint32_t one = elected(), slots0 = values ? v0 : k0, slot_bytes = values ? S::kVSlot : S::kKSlot;
+    int unit = 0, it = 0, at_slot = 0;
+    uint32_t turn = 0;
     bool ok = true;
 #pragma unroll 1
     for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
@@ -659,13 +721,16 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         const int key = t * TK + i * rows;
         return i < boxes && key < keys ? pages[a.kv.ordinal(key)] : a.kv.num_pages;
       };
-      int next[2] = {page_of(w.lo, lane), page_of(w.lo, lane + 32)};
+      constexpr int B = TK / 32;  // boxes of a lane at most
+      int next[B];
+#pragma unroll
+      for (int j = 0; j < B; ++j) next[j] = page_of(w.lo, lane + 32 * j);
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it, pair.next()) {
-        int page[2];
+      for (int t = w.lo; t < w.hi; ++t, ++it) {
+        int page[B];
         bool bad = false;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < B; ++j) {
           page[j] = next[j];
           const int i = lane + 32 * j;
           if (i < boxes && (page[j] < 0 || page[j] >= a.kv.num_pages)) {
@@ -678,25 +743,29 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           kv_report(a.status, ER_KV_BAD_PAGE);
           s.bad_unit[unit & 15] = unit + 1;
         }
-        const int slot = 2 * pair.at + values;
-        if (it >= SLOTS / 2 && !(ok = wait(s.empty[slot], pair.turn ^ 1))) break;
+        if (it >= ring && !(ok = wait(values ? s.vempty[at_slot] : s.kempty[at_slot], turn ^ 1))) break;
         // values of a tile with drafted keys are looked at before they count
-        const uint32_t bar = smem_u32(values && (t + 1) * TK > w.e.len ? &s.raw[slot] : &s.full[slot]);
+        const uint32_t bar = smem_u32(!values ? &s.kfull[at_slot] : (t + 1) * TK > w.e.len ? &s.raw[at_slot] : &s.vfull[at_slot]);
         asm volatile(
             "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
             "@g mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
             "r"(chunks * TK * 128), "r"(one)
             : "memory");
-        uint32_t to = S::slot(slots0, slot);
+        uint32_t to = slots0 + at_slot * slot_bytes;
         int at = a.kv.slot(t * TK);
 #pragma unroll 1
         for (int i = 0; i < boxes; ++i, to += rows * 128, at += rows) {
           if (at == a.kv.page_size) at = 0;
-          const int pg = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31);
+          int mine = page[0];
+#pragma unroll
+          for (int j = 1; j < B; ++j)
+            if (i >> 5 == j) mine = page[j];
+          const int pg = __shfl_sync(0xffffffffu, mine, i & 31);
 #pragma unroll
           for (int c = 0; c < S::DP / 64; ++c)
             if (c < chunks) tma_box(one, to + c * (TK * 128), map, bar, x0 + c * 64, at, w.head, pg);
         }
+        if (++at_slot == ring) at_slot = 0, turn ^= 1;
       }
     }
     if (!ok || s.abort) {  // no copy is under way when the CTA's memory goes: they take microseconds
@@ -709,7 +778,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kFixWarps);
     const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
     int unit = 0, it = 0, looks = 0;
-    Ring<SLOTS / 2> pair;
+    Ring<KS> k_ring;
+    Ring<VS> v_ring;
     bool ok = true;
     auto signal = [&](const uint64_t& b) {
       async_fence();
@@ -719,32 +789,42 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
       const int keys = w.e.len + w.e.nodes;
       if constexpr (S::KP == 1) {
-        for (int t = w.lo; t < w.hi; ++t, pair.next()) {
+        for (int t = w.lo; t < w.hi; ++t, v_ring.next()) {
           if ((t + 1) * TK <= w.e.len) continue;  // neither drafted keys nor places behind the last
-          const int slot = 2 * pair.at + 1;
+          const int slot = v_ring.at;
           if (!(ok = wait(s.raw[slot], looks >> slot & 1))) break;
           looks ^= 1 << slot;
-          const uint32_t to = S::slot(slots0, slot);
-          uint32_t marks[2] = {0, 0};
+          const uint32_t to = v0 + slot * S::kVSlot;
+          uint32_t marks[TK / 32] = {};
           const int vv = (min(S::VD, d - w.ch0) + 15) / 16 * 2, r0 = max(0, w.e.len - t * TK);
-          for (int i = loader * 32 + lane; i < (TK - r0) * vv; i += S::kFixWarps * 32) {
-            const int r = r0 + i / vv, c = i % vv;
-            const uint32_t at = to + swizzled(c, r, TK);
-            const uint4 v = lds16(at);
-            const uint32_t h[4] = {v.x, v.y, v.z, v.w};
-            bool bad = false;
+          // eight lanes a row; 32 rows of one 64 channels at a time
+          for (int c = lane & 7; c - (lane & 7) < vv; c += 8)
+#pragma unroll 1
+            for (int r1 = r0 & ~31; r1 < TK; r1 += 32) {
+              uint4 v[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bad |= (h[j] & 0x7f80u) == 0x7f80u || (h[j] & 0x7f800000u) == 0x7f800000u;
-            // no numbers: zero, for the rows that do not see them, and marked for those that do
-            if (bad || t * TK + r >= keys) sts16(at, make_uint4(0, 0, 0, 0));
-            if (bad) marks[r >> 5] |= 1u << (r & 31);
-          }
+              for (int j = 0; j < 8; ++j) v[j] = lds16(to + swizzled(c, r1 + j * 4 + lane / 8, TK));
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int r = r1 + j * 4 + lane / 8;
+                const uint32_t h[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                uint32_t bad = 0;  // whether an exponent is all ones
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= ((h[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                // no numbers: zero, for the rows that do not see them, and marked for those that do
+                if (r >= r0 && c < vv && (bad || t * TK + r >= keys)) sts16(to + swizzled(c, r, TK), make_uint4(0, 0, 0, 0));
+#pragma unroll
+                for (int e = 0; e < TK / 32; ++e)
+                  if (bad && r >= r0 && c < vv && r >> 5 == e) marks[e] |= 1u << (r & 31);
+              }
+            }
           __syncwarp();
-          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int i = 0; i < TK / 32; ++i) {
             marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
             if (lane == 0) s.vbad[slot][loader][i] = marks[i];
           }
-          signal(s.full[slot]);
+          signal(s.vfull[slot]);
         }
       } else {
         constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;  // of four rows, eight lanes a row
@@ -758,7 +838,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         };
         int page = page_of(w.lo);
 #pragma unroll 1
-        for (int t = w.lo; t < w.hi && ok; ++t, ++it, pair.next()) {
+        for (int t = w.lo; t < w.hi && ok; ++t, ++it, k_ring.next(), v_ring.next()) {
           long long off = -1;
           const int key = t * TK + own;
           if (lane < GROUPS * 4 && own < TK && key < keys) {
@@ -773,13 +853,15 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           __syncwarp();
 #pragma unroll 1
           for (int kind = 0; kind < 2; ++kind) {  // keys, values
-            const int slot = 2 * pair.at + kind;
-            if (it >= SLOTS / 2 && !(ok = wait(s.empty[slot], pair.turn ^ 1))) break;
-            const uint32_t to = S::slot(slots0, slot);
+            const int slot = kind ? v_ring.at : k_ring.at;
+            if (kind ? it >= VS && !(ok = wait(s.vempty[slot], v_ring.turn ^ 1))
+                     : it >= KS && !(ok = wait(s.kempty[slot], k_ring.turn ^ 1)))
+              break;
+            const uint32_t to = kind ? v0 + slot * S::kVSlot : k0 + slot * S::kKSlot;
             const char* pool = kind ? a.kv.v + w.ch0 * 4 : a.kv.k;
             const bool look = kind && (t + 1) * TK > w.e.len;
             const int width = kind ? min(S::VD, d - w.ch0) : d, n = kind ? (width + 15) / 16 * 2 : vecs;
-            uint32_t marks[2] = {0, 0};
+            uint32_t marks[TK / 32] = {};
             for (int c0 = 0; c0 < n; c0 += 8) {  // the same for all lanes: they exchange the rows' places
               const int c = c0 + (lane & 7);
               float4 x[GROUPS][2];
@@ -804,7 +886,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                   if (bad) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) y[j] = 0.f;
-                    marks[r >> 5] |= 1u << (r & 31);
+#pragma unroll
+                    for (int j = 0; j < TK / 32; ++j)
+                      if (r >> 5 == j) marks[j] |= 1u << (r & 31);
                   }
                 }
                 uint4 parts[3];
@@ -816,12 +900,13 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             }
             __syncwarp();
             if (look) {
-              for (int i = 0; i < 2; ++i) {
+#pragma unroll
+              for (int i = 0; i < TK / 32; ++i) {
                 marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
                 if (lane == 0) s.vbad[slot][loader][i] = marks[i];
               }
             }
-            signal(s.full[slot]);
+            signal(kind ? s.vfull[slot] : s.kfull[slot]);
           }
         }
       }
