@@ -12,7 +12,7 @@ namespace {
 constexpr int kJoinWarps = 8;
 
 template <typename TQ>
-__global__ void __launch_bounds__(kJoinWarps * 32) kv_tree_join_kernel(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) kv_tree_join_kernel(const __grid_constant__ TreeArgs a) {
   kv_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
   for (int t = blockIdx.y * a.grid + blockIdx.x; t < a.trees; t += a.grid * gridDim.y) {
@@ -26,6 +26,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_tree_join_kernel(const __g
   if (c.live == 0) return;
   const int shares = tree_shares(a, c.total), i0 = blockIdx.x;
   const int n = kv_share_of(c.total, shares, c.begin + kTreeCost + c.tiles - 1) - i0 + 1;  // pieces
+  const int width = min(a.channels, d - c.ch0);
+  const bool mine = lane * 4 < width;
   for (int r = blockIdx.y * kJoinWarps + warp; r < c.live; r += gridDim.y * kJoinWarps) {
     auto at = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * a.piece_rows + r; };
     float top = -INFINITY;
@@ -34,24 +36,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv_tree_join_kernel(const __g
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int width = min(a.channels, d - c.ch0);
-    const bool mine = lane * 4 < width;
+    constexpr int N = 8;  // pieces under way
 #pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float2 ml[8];
-      float4 x[8];
+    for (int k0 = 0; k0 < n; k0 += N) {
+      float2 ml[N];
+      float4 x[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < N; ++j) {
         if (k0 + j >= n) continue;
         ml[j] = *reinterpret_cast<const float2*>(a.part_ml + at(k0 + j) * 2);
         if (mine) x[j] = *reinterpret_cast<const float4*>(a.part_o + at(k0 + j) * a.channels + lane * 4);
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < N; ++j) {
         if (k0 + j >= n) continue;
-        const float by = piece_weight(ml[j].x, top);
-        sum = fmaf(ml[j].y, by, sum);  // a spoilt piece's sum is NaN
-        if (mine) fma4(acc, x[j], by);
+        const float weight = piece_weight(ml[j].x, top);
+        sum = fmaf(ml[j].y, weight, sum);  // a spoilt piece's sum is NaN
+        if (mine) fma4(acc, x[j], weight);
       }
     }
     const int q = c.q0 + r, node = q / a.group, g = q - node * a.group;
@@ -108,18 +109,22 @@ TreeLayout tree_layout(const er_kv_cache& c, const er_kv_tree_io& io, int sms) {
   return L;
 }
 
-// Pages of a bf16 pool as copies see them: channels, positions, key heads, pages; boxes of 64 channels.
-int tree_map(CUtensorMap* m, const er_kv_cache& c, void* pool, int box_rows) {
+// Pages of a pool as copies see them: channels, positions, key heads, pages. bf16: boxes of 64 channels, as the
+// products want them (128-byte swizzle), fp32: rows as they are.
+int tree_map(CUtensorMap* m, const er_kv_cache& c, void* pool, int box_rows, int box_channels) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(ER_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const bool half = c.dtype == ER_DTYPE_BF16;
+  const cuuint64_t es = half ? 2 : 4;
   const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads, (cuuint64_t)c.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+  cuuint64_t strides[3] = {(cuuint64_t)c.slot_stride * es, (cuuint64_t)c.head_stride * es, (cuuint64_t)c.page_stride * es};
   for (int i = 0; i < 3; ++i)
-    if (dims[i + 1] == 1) strides[i] = (cuuint64_t)c.head_dim * 2;  // never used
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, each[4] = {1, 1, 1, 1};
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, pool, dims, strides, box, each,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (dims[i + 1] == 1) strides[i] = (cuuint64_t)c.head_dim * es;  // never used
+  const cuuint32_t box[4] = {(cuuint32_t)box_channels, (cuuint32_t)box_rows, 1, 1}, each[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, half ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, pool, dims, strides,
+                        box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        half ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(ER_EINVAL, "er_kv_tree: pools of strides %lld, %lld, %lld cannot be copied by tiles (%d)", c.page_stride,
                 c.head_stride, c.slot_stride, (int)r);
@@ -167,19 +172,22 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   a.cut = (TreeCut*)(ws + L.cut);
   a.part_ml = (float*)(ws + L.ml);
   a.part_o = (float*)(ws + L.o);
-  a.tile = L.shape.tile, a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
-  int box = L.shape.tile;
-  while (cache->page_size % box) box >>= 1;
-  a.box_rows = box;
-  if (cb) {
-    CUtensorMap maps[2];
-    if (int rc = tree_map(&maps[0], *cache, cache->k, box)) return rc;
-    if (int rc = tree_map(&maps[1], *cache, cache->v, box)) return rc;
-    if (int rc = tree_bf16(a, io->q_dtype, maps, st)) return rc;
-  } else if (int rc = tree_f32(a, io->q_dtype, st)) {
-    return rc;
+  while (1 << a.tile_shift < L.shape.tile) ++a.tile_shift;
+  while (1 << a.block_shift < L.shape.rows) ++a.block_shift;
+  a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
+  CUtensorMap maps[2] = {};
+  if (L.shape.box_rows) {
+    a.box_rows = L.shape.box_rows;
+    while (cache->page_size % a.box_rows) a.box_rows >>= 1;
+    if (int rc = tree_map(&maps[0], *cache, cache->k, a.box_rows, L.shape.box_channels)) return rc;
+    if (int rc = tree_map(&maps[1], *cache, cache->v, a.box_rows, L.shape.box_channels)) return rc;
   }
-  const dim3 grid(sms, (L.piece_rows + kJoinWarps - 1) / kJoinWarps);
+  if (int rc = cb ? tree_bf16(a, io->q_dtype, maps, st) : tree_f32(a, io->q_dtype, maps, st)) return rc;
+  // as many units as CTAs: each is cut in two or three pieces, and few CTAs do for its rows
+  int parts = (L.piece_rows + kJoinWarps - 1) / kJoinWarps;
+  const int most = (long long)io->trees * cache->kv_heads >= sms ? 4 : 16;
+  if (parts > most) parts = most;
+  const dim3 grid(sms, parts);
   return qb ? kv_launch(kv_tree_join_kernel<bf>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a)
             : kv_launch(kv_tree_join_kernel<float>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a);
 }

@@ -35,8 +35,8 @@ struct TreeArgs {
   int* status;
   int q_wide;              // rows of q on 16-byte boundaries
   int q_flip, q_zero;      // the scale was negative, or zero: queries change their sign, or are zero
-  int tile;                // keys of a tile
-  int block_rows;          // query rows of a unit at most
+  int tile_shift;          // log2 of a tile's keys
+  int block_rows, block_shift;  // query rows of a unit at most (a power of two), and its log2
   int channels, halves;    // of the values: those of a unit, units beside each other for all of them
   int box_rows;            // positions that a copy takes: they lie in one page wherever it begins
   int grid;                // CTAs of the attention kernel
@@ -88,11 +88,11 @@ struct TreeUnits {
 __device__ __forceinline__ TreeUnits tree_units(const TreeArgs& a, const Tree& e) {
   TreeUnits u = {};
   if (e.bad || e.nodes == 0) return u;
-  u.rows = e.nodes * a.group;
-  u.blocks = (u.rows + a.block_rows - 1) / a.block_rows;
-  u.per = (u.rows + u.blocks - 1) / u.blocks;
+  u.rows = e.nodes * a.group;  // divisions are left out where they can be: every warp comes here at its start
+  u.blocks = (u.rows + a.block_rows - 1) >> a.block_shift;
+  u.per = u.blocks == 1 ? u.rows : (u.rows + u.blocks - 1) / u.blocks;
   u.units = u.blocks * a.halves * a.kv.kv_heads;
-  u.tiles = (e.len + e.nodes + a.tile - 1) / a.tile;
+  u.tiles = (e.len + e.nodes + (1 << a.tile_shift) - 1) >> a.tile_shift;
   return u;
 }
 
@@ -155,81 +155,82 @@ __device__ __forceinline__ void tree_run(const TreeArgs& a, TreeRun& run, TreeSc
   __syncthreads();
 }
 
-// The units of a run that have tiles in it, one after another: tiles lo .. hi - 1 of `tiles`.
+// The units of a run that have tiles in it, one after another. Every warp goes
+// its own way through them, in shared memory and by one copy of the code: each
+// copy would be fetched for the first time in every launch.
 struct TreeWalk {
-  const TreeArgs& a;
-  const TreeRun& run;
   int t, unit;
   Tree e;
   TreeUnits u;
-  long long pos;  // where the unit begins in the line
-  int lo, hi, tiles, head, q0, live, ch0;
-  int most;  // replicas
+  long long pos;    // where the unit begins in the line
+  int lo, hi;       // its tiles in the run, of u.tiles
+  int head, q0, live, ch0;
+  int replicas;
+};
 
-  __device__ __forceinline__ TreeWalk(const TreeArgs& args, const TreeRun& r, int most_replicas)
-      : a(args), run(r), most(most_replicas) {}
-
-  __device__ __forceinline__ bool look() {  // from unit `unit` of tree t at pos on: the next one with tiles in the run
-    for (;;) {
-      if (pos >= run.to) return false;
-      if (unit >= u.units) {
-        do {
-          if (++t >= a.trees) return false;
-          e = kv_tree(a, t);
-          u = tree_units(a, e);
-        } while (u.units == 0);
-        unit = 0;
-      }
-      const long long first = pos + kTreeCost;
-      lo = run.from > first ? (int)(run.from - first < u.tiles ? run.from - first : u.tiles) : 0;
-      hi = run.to < first + u.tiles ? (int)(run.to > first ? run.to - first : 0) : u.tiles;
-      if (hi > lo) break;
-      pos += u.tiles + kTreeCost;
-      ++unit;
+// The warp's next unit (its first one where `first`); false where there is none. `most`: replicas.
+static __device__ __noinline__ bool tree_next(const TreeArgs& a, const TreeRun& run, TreeWalk* walk, bool first, int most) {
+  if (run.total == 0 || run.from == run.to) return false;
+  TreeWalk w;
+  if (first) {
+    w.t = run.t;
+    w.e = kv_tree(a, w.t);
+    w.u = tree_units(a, w.e);
+    const int c = w.u.tiles + kTreeCost;
+    w.unit = (int)kv_div(run.from - run.at, c);
+    w.pos = run.at + (long long)w.unit * c;
+  } else {
+    w = *walk;
+    w.pos += w.u.tiles + kTreeCost;
+    ++w.unit;
+  }
+  for (;;) {
+    if (w.pos >= run.to) return false;
+    if (w.unit >= w.u.units) {
+      do {
+        if (++w.t >= a.trees) return false;
+        w.e = kv_tree(a, w.t);
+        w.u = tree_units(a, w.e);
+      } while (w.u.units == 0);
+      w.unit = 0;
     }
-    tiles = u.tiles;
-    const int beside = u.blocks * a.halves, rest = unit % beside;
-    head = unit / beside;
-    q0 = rest / a.halves * u.per;
-    ch0 = rest % a.halves * kTreeChannels;
-    live = min(u.per, u.rows - q0);
-    return true;
+    const long long tile0 = w.pos + kTreeCost;
+    w.lo = run.from > tile0 ? (int)(run.from - tile0 < w.u.tiles ? run.from - tile0 : w.u.tiles) : 0;
+    w.hi = run.to < tile0 + w.u.tiles ? (int)(run.to > tile0 ? run.to - tile0 : 0) : w.u.tiles;
+    if (w.hi > w.lo) break;
+    w.pos += w.u.tiles + kTreeCost;
+    ++w.unit;
   }
-  __device__ __forceinline__ bool begin() {
-    if (run.total == 0 || run.from == run.to) return false;
-    t = run.t;
-    e = kv_tree(a, t);
-    u = tree_units(a, e);
-    const int c = u.tiles + kTreeCost;
-    unit = (int)kv_div(run.from - run.at, c);
-    pos = run.at + (long long)unit * c;
-    return look();
-  }
-  __device__ __forceinline__ bool next() {
-    pos += u.tiles + kTreeCost;
-    ++unit;
-    return look();
-  }
+  const int beside = w.u.blocks * a.halves;
+  w.head = beside == 1 ? w.unit : w.unit / beside;
+  const int rest = w.unit - w.head * beside;
+  w.q0 = (a.halves == 2 ? rest >> 1 : rest) * w.u.per;
+  w.ch0 = a.halves == 2 ? (rest & 1) * kTreeChannels : 0;
+  w.live = min(w.u.per, w.u.rows - w.q0);
   // Few rows are taken several times, each for its share of a tile's keys, so that all of the lanes of the
   // scores' memory have work.
-  __device__ __forceinline__ int replicas() const {
-    return most >= 4 && live <= 32 ? 4 : most >= 2 && live <= 16 * most ? 2 : 1;
-  }
-};
+  w.replicas = most >= 4 && w.live <= 32 ? 4 : most >= 2 && w.live <= 16 * most ? 2 : 1;
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) *walk = w;
+  __syncwarp();
+  return true;
+}
 
 // What a launch of the attention kernel takes: keys of a tile, query rows of a
 // unit, its channels and how many units have the others.
 struct TreeLaunch {
   int tile, rows, channels, halves;
+  int box_rows, box_channels;  // of a copy, at most (0: none are issued)
 };
 // er_kv_tree_bf16.cu and er_kv_tree_f32.cu: for caches of either type
 TreeLaunch tree_shape_bf16(int d, int q_dtype);
 TreeLaunch tree_shape_f32(int d);
 template <typename S>
 constexpr TreeLaunch tree_shape() {
-  return TreeLaunch{S::TK, S::ROWS, S::VD, S::DP / S::VD};
+  return TreeLaunch{S::TK, S::ROWS, S::VD, S::DP / S::VD, S::KP == 1 ? S::TK : S::kRaw ? S::kRawRows : 0,
+                    S::KP == 1 ? 64 : S::DP};
 }
 int tree_bf16(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st);
-int tree_f32(const TreeArgs& a, int q_dtype, cudaStream_t st);
+int tree_f32(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st);
 
 }  // namespace er

@@ -9,7 +9,7 @@ using B64 = TreeShape<1, 1, 2, 64, 128, 64, 6, 6>;
 using B128 = TreeShape<1, 1, 2, 128, 128, 64, 4, 4>;
 using B256 = TreeShape<1, 1, 2, 256, 128, 64, 2, 2>;
 using F64 = TreeShape<1, 3, 3, 64, 128, 64, 6, 6>;
-using F128 = TreeShape<1, 3, 3, 128, 128, 64, 3, 3>;
+using F128 = TreeShape<1, 3, 3, 128, 128, 64, 3, 2>;
 using F256 = TreeShape<1, 3, 3, 256, 64, 64, 2, 2>;
 }  // namespace
 

@@ -5,16 +5,15 @@ namespace er {
 
 namespace {
 using S64 = TreeShape<3, 3, 3, 64, 128, 64, 2, 2>;
-using S128 = TreeShape<3, 3, 3, 128, 128, 64, 1, 1>;
+using S128 = TreeShape<3, 3, 3, 128, 64, 64, 1, 1>;
 using S256 = TreeShape<3, 3, 3, 256, 32, 64, 1, 1>;
 
 template <typename TQ>
-int launch(const TreeArgs& a, cudaStream_t st) {
-  const CUtensorMap none[2] = {};
+int launch(const TreeArgs& a, const CUtensorMap* maps, cudaStream_t st) {
   const int d = a.kv.d;
-  return d <= 64    ? tree_launch<S64, float, TQ>(a, none, st)
-         : d <= 128 ? tree_launch<S128, float, TQ>(a, none, st)
-                    : tree_launch<S256, float, TQ>(a, none, st);
+  return d <= 64    ? tree_launch<S64, float, TQ>(a, maps, st)
+         : d <= 128 ? tree_launch<S128, float, TQ>(a, maps, st)
+                    : tree_launch<S256, float, TQ>(a, maps, st);
 }
 }  // namespace
 
@@ -22,8 +21,8 @@ TreeLaunch tree_shape_f32(int d) {
   return d <= 64 ? tree_shape<S64>() : d <= 128 ? tree_shape<S128>() : tree_shape<S256>();
 }
 
-int tree_f32(const TreeArgs& a, int q_dtype, cudaStream_t st) {
-  return q_dtype == ER_DTYPE_BF16 ? launch<__nv_bfloat16>(a, st) : launch<float>(a, st);
+int tree_f32(const TreeArgs& a, int q_dtype, const CUtensorMap* maps, cudaStream_t st) {
+  return q_dtype == ER_DTYPE_BF16 ? launch<__nv_bfloat16>(a, maps, st) : launch<float>(a, maps, st);
 }
 
 }  // namespace er

@@ -25,11 +25,15 @@ struct TreeShape {
   static constexpr int kQPart = ROWS * DP * 2, kQ = kQPart * QP;
   // columns of a tile's scores, then of its weights: by 64 keys, two parts over the scores, a third one behind them
   static constexpr int kSP = PP > 2 ? TK * 3 / 2 : TK;
-  static constexpr int OB = 2 * kSP + 2 * VD <= 512 ? 2 : 1;  // results of a tile, kept while they are read
-  static constexpr int kSmem = kQ + KS * kKSlot + VS * kVSlot + ROWS * kStagePitch * 4;
-  // warps that fill shared memory: of a bf16 cache one that issues the keys' copies, one the values' and one that
-  // looks after the drafted values, of an fp32 cache all of them by way of registers
-  static constexpr int kLoadWarps = KP == 1 ? 3 : 7, kFixWarps = KP == 1 ? 1 : 7;
+  // tiles of scores (the products' warp issues them ahead), and results of a tile, kept while they are read
+  static constexpr int SB = 3 * kSP + 2 * VD <= 512 ? 3 : 2, OB = SB * kSP + 2 * VD <= 512 ? 2 : 1;
+  // fp32 caches, up to 128 channels: RS half tiles as they come, to be split into parts from there
+  static constexpr bool kRaw = KP > 1 && DP <= 128;
+  static constexpr int RS = kRaw ? 3 : 0, kRawRows = TK / 2, kRawSlot = kRawRows * DP * 4;
+  static constexpr int kSmem = kQ + KS * kKSlot + VS * kVSlot + RS * kRawSlot + ROWS * kStagePitch * 4;
+  // warps that fill shared memory. bf16 caches: one that issues the keys' copies, one the values' and one that looks
+  // after the drafted values. fp32: one that issues copies and four that split, or seven that split from registers.
+  static constexpr int kLoadWarps = KP == 1 ? 3 : kRaw ? 5 : 7, kFixWarps = KP == 1 ? 1 : kRaw ? 4 : 7;
   static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
   // the column of a tile's weights: part p of the 64 keys from 64 h on
   static __device__ __forceinline__ constexpr int column(int h, int p) { return p < 2 ? h * 64 + p * 32 : TK + h * 32; }
@@ -37,18 +41,21 @@ struct TreeShape {
 
 template <typename S>
 struct TreeShared {
-  uint64_t kfull[S::KS], kempty[S::KS], vfull[S::VS], vempty[S::VS], raw[S::VS];
-  uint64_t qfirst, qfull, qfree, sfull[2], pfull[2], ofull[2], ofree[2], staged, masked, drain;
+  uint64_t kfull[S::KS], kempty[S::KS], vfull[S::VS], vempty[S::VS], raw[S::VS], looked[S::VS], rfull[S::RS + 1], rempty[S::RS + 1];
+  uint64_t qfirst, qfull, qfree, sfull[S::SB], pfull[S::SB], ofull[2], ofree[2], staged, masked, drain;
   uint32_t tmem;
   volatile int abort;
   TreeRun run;
   TreeScratch scratch;
-  int bad_tree[2], parents[2][kMaxNodes];  // of units in turn: a warp may be one ahead of another
+  TreeWalk walk[S::kThreads / 32];
+  int bad_tree[2];
+  int16_t parents[2][kMaxNodes];  // of units in turn: a warp may be one ahead of another
   int bad_unit[16];                 // units (numbers + 1) of a bad page, in turn
   uint32_t sees[S::ROWS][9];        // each row's ancestors and itself, a bit a node
   uint32_t vbad[S::VS][S::kFixWarps][S::TK / 32];  // keys of a tile whose value was no number (drafted ones)
-  float by[4][S::ROWS];             // what a tile's sums so far are multiplied by
-  float2 ml[4][S::ROWS];            // maximum and sum of a unit's last tile
+  // of tiles in turn: five may be between the weights' warps and the sums'
+  float by[8][S::ROWS];             // what a tile's sums so far are multiplied by
+  float2 ml[8][S::ROWS];            // maximum and sum of a unit's last tile
 };
 
 // Descriptors of operands in shared memory, 128-byte swizzle, eight-row groups 1024 bytes apart: the upper word is
@@ -210,6 +217,26 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&out)[3]) {
     out[i] = make_uint4(p[i][0] | p[i][1] << 16, p[i][2] | p[i][3] << 16, p[i][4] | p[i][5] << 16, p[i][6] | p[i][7] << 16);
 }
 
+// Eight finite floats as three bf16 parts, cut, whose sum they are exactly (one that is not finite: parts without a
+// number among them).
+__device__ __forceinline__ void cut8(const float (&x)[8], uint4 (&out)[3]) {
+  uint32_t p[3][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float u = x[2 * j], v = x[2 * j + 1];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      p[i][j] = __byte_perm(__float_as_uint(u), __float_as_uint(v), 0x7632);
+      if (i < 2) {
+        u -= __uint_as_float(__float_as_uint(u) & 0xffff0000u);
+        v -= __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) out[i] = make_uint4(p[i][0], p[i][1], p[i][2], p[i][3]);
+}
+
 // Bits of nodes node0 .. node0 + 31 that a row sees; below 0 lies the context, all of which it sees.
 __device__ __forceinline__ uint32_t seen_from(const uint32_t* sees, int node0) {
   if (node0 <= -32) return 0xffffffffu;
@@ -266,7 +293,7 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* src, bool wide, float
 // query, which is row qi of every replica.
 template <typename S, typename TQ>
 __device__ __forceinline__ void load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps) {
-  const int lane = threadIdx.x & 31, d = a.kv.d, chunks = (d + 63) / 64, R = w.replicas(), per = S::ROWS / R;
+  const int lane = threadIdx.x & 31, d = a.kv.d, chunks = (d + 63) / 64, R = w.replicas, per = S::ROWS / R;
   const int items = (w.live + 3) / 4 * chunks;  // of four queries
 #pragma unroll 2
   for (int i = warp; i < items; i += warps) {
@@ -308,23 +335,23 @@ __global__ void __launch_bounds__(S::kThreads, 1)
                    const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ unsigned char raw[];
   __shared__ TreeShared<S> s;
-  constexpr int TK = S::TK, KS = S::KS, VS = S::VS, OB = S::OB;
+  constexpr int TK = S::TK, KS = S::KS, VS = S::VS, SB = S::SB, OB = S::OB;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.kv.d;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;  // swizzled tiles repeat every 1024 bytes
   // the queries first: products read 128 rows from there, whatever lies behind S::ROWS
-  const uint32_t q0 = base, k0 = q0 + S::kQ, v0 = k0 + KS * S::kKSlot;
-  float* stage = reinterpret_cast<float*>(raw + (v0 + VS * S::kVSlot - smem_u32(raw)));
+  const uint32_t q0 = base, k0 = q0 + S::kQ, v0 = k0 + KS * S::kKSlot, raw0 = v0 + VS * S::kVSlot;
+  float* stage = reinterpret_cast<float*>(raw + (raw0 + S::RS * S::kRawSlot - smem_u32(raw)));
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < KS; ++i) mbar_init(&s.kfull[i], S::kFixWarps), mbar_init(&s.kempty[i], 1);
     for (int i = 0; i < VS; ++i)
-      mbar_init(&s.vfull[i], S::kFixWarps), mbar_init(&s.vempty[i], 1), mbar_init(&s.raw[i], 1);
+      mbar_init(&s.vfull[i], S::kFixWarps), mbar_init(&s.vempty[i], 1), mbar_init(&s.raw[i], 1), mbar_init(&s.looked[i], S::kFixWarps);
+    for (int i = 0; i < S::RS; ++i) mbar_init(&s.rfull[i], 1), mbar_init(&s.rempty[i], S::kFixWarps);
     mbar_init(&s.qfirst, kIssueWarp);
     mbar_init(&s.qfull, kSoftmaxWarps);
     mbar_init(&s.qfree, 1);
+    for (int i = 0; i < SB; ++i) mbar_init(&s.sfull[i], 1), mbar_init(&s.pfull[i], kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.sfull[i], 1);
-      mbar_init(&s.pfull[i], kSoftmaxWarps);
       mbar_init(&s.ofull[i], 1);
       mbar_init(&s.ofree[i], kSumWarps);
     }
@@ -351,30 +378,31 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     __syncwarp();
     if (lane == 0) bar_arrive(smem_u32(&b));
   };
-  TreeWalk w(a, s.run, S::ROWS / 32);
-  if (warp < kIssueWarp && w.begin()) {  // the first unit's queries by the warps that have nothing to do yet
+  const TreeWalk& w = s.walk[warp];
+  auto next = [&](bool first) { return tree_next(a, s.run, &s.walk[warp], first, S::ROWS / 32); };
+  if (warp < kIssueWarp && next(true)) {  // the first unit's queries by the warps that have nothing to do yet
     load_queries<S, TQ>(a, w, q0, warp, kIssueWarp);
     arrive(s.qfirst);
   }
 
   if (warp < kSoftmaxWarps) {
     // ---- weights: a thread a row, of one replica's share of the tile's keys
-    int it = 0, masks = 0, unit = 0;
-    Ring<2> sp_ring;
+    int it = 0, masks = 0, unit = 0, looks = 0;
+    Ring<SB> sp_ring;
     Ring<VS> v_ring;
 #pragma unroll 1
-    for (bool go = w.begin(); go && !s.abort; go = w.next(), ++unit) {
+    for (bool go = next(true); go && !s.abort; go = next(false), ++unit) {
       if (unit > 0) {  // the first one's are on their way
         if (!wait(s.qfree, (unit - 1) & 1)) break;
         load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps);
         arrive(s.qfull);
       }
-      const int R = w.replicas(), per = S::ROWS / R, row = threadIdx.x;
+      const int R = w.replicas, per = S::ROWS / R, row = threadIdx.x, len = w.e.len, lo = w.lo, hi = w.hi;
       const int qi = row % per, slice = row < S::ROWS ? row / per : 0;
       const bool mine = row < S::ROWS && qi < w.live, live = __any_sync(0xffffffffu, mine);
       uint32_t* sees = s.sees[row < S::ROWS ? row : 0];
       // the rows' masks, where this CTA meets drafted keys
-      const bool drafted = w.hi * TK > w.e.len;
+      const bool drafted = hi * TK > len;
       if (drafted) {
         for (int i = threadIdx.x; i < w.e.nodes; i += kSoftmaxWarps * 32) {
           int p = a.parents[w.e.first + i];
@@ -383,7 +411,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             s.bad_tree[masks & 1] = masks + 1;  // of this unit
             p = -1;
           }
-          s.parents[masks & 1][i] = p;
+          s.parents[masks & 1][i] = (int16_t)p;
         }
         arrive(s.masked);
         if (!wait(s.masked, masks & 1)) break;
@@ -408,7 +436,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           if constexpr (N == 64) tmem_ld32(sp + 32, x + 32);
         }
         tmem_wait_ld();
-        const int node0 = t * TK + key - w.e.len;
+        const int node0 = t * TK + key - len;
         if (node0 + N > 0) {  // drafted keys, or none
           uint32_t spoils = 0;
 #pragma unroll
@@ -461,7 +489,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         *shift = -ref * a.scale;
         const float by = ex2(fmaf(m, a.scale, *shift));
         m = top;
-        if (row < S::ROWS) s.by[it & 3][row] = by;
+        if (row < S::ROWS) s.by[it & 7][row] = by;
         __syncwarp();
         return by;
       };
@@ -498,9 +526,12 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       };
       bool ok = true;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it, sp_ring.next(), v_ring.next()) {
+      for (int t = lo; t < hi; ++t, ++it, sp_ring.next(), v_ring.next()) {
         if (!(ok = wait(s.sfull[sp_ring.at], sp_ring.turn))) break;
-        if ((t + 1) * TK > w.e.len && !(ok = wait(s.vfull[v_ring.at], v_ring.turn))) break;
+        if ((t + 1) * TK > len) {  // its values have been looked at
+          if (!(ok = wait(s.looked[v_ring.at], looks >> v_ring.at & 1))) break;
+          looks ^= 1 << v_ring.at;
+        }
         tc_fence_after();
         if (live) {
           if (R == 1)
@@ -511,9 +542,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             tile(std::integral_constant<int, 4>{}, t);
           tmem_wait_st();
         }
-        if (t + 1 == w.hi && row < S::ROWS) {
+        if (t + 1 == hi && row < S::ROWS) {
           if (s.bad_unit[unit & 15] == unit + 1) l = __int_as_float(0x7fc00000);
-          s.ml[it & 3][row] = make_float2(m == -INFINITY ? m : m * a.scale, l);
+          s.ml[it & 7][row] = make_float2(m == -INFINITY ? m : m * a.scale, l);
         }
         tc_fence_before();
         arrive(s.pfull[sp_ring.at]);
@@ -529,23 +560,24 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     uint32_t stages = 0;
     if (id == 0) a.cut[blockIdx.x].live = 0;
 #pragma unroll 1
-    for (bool go = w.begin(); go && !s.abort; go = w.next()) {
+    for (bool go = next(true); go && !s.abort; go = next(false)) {
       uint64_t o[CH / 2];  // two channels each
 #pragma unroll
       for (int c = 0; c < CH / 2; ++c) o[c] = 0;
-      const int R = w.replicas(), per = S::ROWS / R, vd = min(S::VD, d - w.ch0);
+      const int R = w.replicas, per = S::ROWS / R, vd = min(S::VD, d - w.ch0);
       const bool there = row < S::ROWS, live = __any_sync(0xffffffffu, there && row % per < w.live);
       bool ok = true;
       float2 ml = make_float2(0.f, 0.f);
+      const int hi = w.hi;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it, o_ring.next()) {
+      for (int t = w.lo; t < hi; ++t, ++it, o_ring.next()) {
         const int ob = o_ring.at;
         if (!(ok = wait(s.ofull[ob], o_ring.turn))) break;  // after the tile's weights, so `by` and `ml` are there
         tc_fence_after();
         if (live) {
-          const float by1 = there ? s.by[it & 3][row] : 0.f;
+          const float by1 = there ? s.by[it & 7][row] : 0.f;
           const uint64_t by = pack2(by1, by1);
-          const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 2 * S::kSP + ob * S::VD + half * CH;
+          const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SB * S::kSP + ob * S::VD + half * CH;
           constexpr int N = S::kThreads > 512 ? 16 : 32;  // registers
 #pragma unroll
           for (int c = 0; c < CH; c += N) {
@@ -560,15 +592,15 @@ __global__ void __launch_bounds__(S::kThreads, 1)
               o[(c + j) / 2] = fma2(o[(c + j) / 2], by, pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])));
           }
         }
-        if (t + 1 == w.hi && there) ml = s.ml[it & 3][row];
+        if (t + 1 == hi && there) ml = s.ml[it & 7][row];
         tc_fence_before();
         arrive(s.ofree[ob]);
       }
       if (!ok) break;
       // the replicas' rows joined: 16 channels of each half at a time by way of shared memory
-      const bool whole = w.lo == 0 && w.hi == w.tiles, begins = w.lo == 0;
+      const bool whole = w.lo == 0 && w.hi == w.u.tiles, begins = w.lo == 0;
       if (!whole && begins && id == 0)
-        a.cut[blockIdx.x] = TreeCut{w.e.first, w.head, w.q0, w.live, w.tiles, w.ch0, w.pos, s.run.total};
+        a.cut[blockIdx.x] = TreeCut{w.e.first, w.head, w.q0, w.live, w.u.tiles, w.ch0, w.pos, s.run.total};
       const long long piece = (long long)blockIdx.x * 2 + begins;
 #pragma unroll
       for (int c0 = 0; c0 < CH; c0 += 16) {
@@ -628,17 +660,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     int unit = 0, scored = 0, summed = 0;  // tiles
     uint32_t io = 0;
     constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
-    Ring<2> sp_ring, p_ring;            // of the tile whose scores, whose values are next
+    Ring<SB> sp_ring, p_ring;           // of the tile whose scores, whose values are next
     Ring<OB> o_ring;
     Ring<KS> k_ring;
     Ring<VS> v_ring;
-    auto values = [&]() {  // out += P V of the tile before
+    auto values = [&]() {  // out += P V of the first tile that has not been
       const int b = o_ring.at;
       if (!wait(s.pfull[p_ring.at], p_ring.turn) || !wait(s.vfull[v_ring.at], v_ring.turn)) return false;
       if (summed >= OB && !wait(s.ofree[b], o_ring.turn ^ 1)) return false;
       tc_fence_after();
       uint32_t v = desc_low(v0 + v_ring.at * S::kVSlot, TK * 128);
-      uint32_t to = tmem + 2 * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = io;
+      uint32_t to = tmem + SB * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = io;
       // put together here: descriptors that the compiler kept from before the waits' calls came out wrong
       asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
       // the small products first
@@ -662,12 +694,15 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     };
     bool ok = true;
 #pragma unroll 1
-    for (bool go = w.begin(); go && ok; go = w.next(), ++unit) {
-      if (scored > summed && !(ok = values())) break;
+    for (bool go = next(true); go && ok; go = next(false), ++unit) {
+      while (scored > summed && (ok = values())) {
+      }
+      if (!ok) break;
       io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
       if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
+      const int hi = w.hi;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t) {
+      for (int t = w.lo; t < hi; ++t) {
         if (!(ok = wait(s.kfull[k_ring.at], k_ring.turn))) break;
         tc_fence_after();
         uint32_t kd = desc_low(k0 + k_ring.at * S::kKSlot, 16), qd = desc_low(q0, 16);
@@ -686,23 +721,86 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           }
         commit_on(one, smem_u32(&s.sfull[sp_ring.at]));
         commit_on(one, smem_u32(&s.kempty[k_ring.at]));
-        if (t + 1 == w.hi) commit_on(one, smem_u32(&s.qfree));
+        if (t + 1 == hi) commit_on(one, smem_u32(&s.qfree));
         sp_ring.next();
         k_ring.next();
         ++scored;
-        if (t > w.lo && !(ok = values())) break;
+        if (scored - summed == SB && !(ok = values())) break;
       }
       if (!ok) break;
     }
-    if (ok && scored > summed) {
-      const Ring<VS> last = v_ring;
-      ok = values() && wait(s.vempty[last.at], last.turn);
-    }
+    Ring<VS> last = v_ring;
+    while (ok && scored > summed) last = v_ring, ok = values();
+    if (ok && summed > 0) ok = wait(s.vempty[last.at], last.turn);
     if (!ok) {  // the products under way end before their memory goes
       commit_on(one, smem_u32(&s.drain));
       mbar_drain(&s.drain, 0, kDefaultWaitNs);
     }
     __syncwarp();
+  } else if (S::kRaw && warp == kIssueWarp + 1) {
+    // ---- copies of fp32 keys and values, half a tile each, in the order in which they are split: the next tile's
+    // keys before a tile's values
+    const int rows = a.box_rows, each = S::kRawRows / rows;
+    const uint32_t one = elected();
+    Ring<S::kRaw ? S::RS : 1> ring;
+    int unit = 0, item = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
+      const int32_t* pages = a.kv.pages_of(w.e.seq);
+      const int keys = w.e.len + w.e.nodes, hi = w.hi, head = w.head;
+      auto page_of = [&](int t, int i) {  // of box i; behind the last key none
+        const int key = t * TK + i * rows;
+        return t < hi && i < 2 * each && key < keys ? pages[a.kv.ordinal(key)] : a.kv.num_pages;
+      };
+      auto checked = [&](int page, int t, int i) {
+        if (page >= 0 && page < a.kv.num_pages) return page;
+        if (t < hi && i < 2 * each && t * TK + i * rows < keys) {
+          kv_report(a.status, ER_KV_BAD_PAGE);
+          s.bad_unit[unit & 15] = unit + 1;
+        }
+        return a.kv.num_pages;  // outside the pool: zeros
+      };
+      auto copy = [&](int t, const int (&page)[2], const CUtensorMap* map) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h, ++item, ring.next()) {
+          if (item >= S::RS && !(ok = wait(s.rempty[ring.at], ring.turn ^ 1))) return;
+          const uint32_t bar = smem_u32(&s.rfull[ring.at]);
+          asm volatile(
+              "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
+              "@g mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+              "r"(S::kRawSlot), "r"(one)
+              : "memory");
+          uint32_t to = raw0 + ring.at * S::kRawSlot;
+          int at = a.kv.slot(t * TK + h * S::kRawRows);
+#pragma unroll 1
+          for (int b = 0; b < each; ++b, to += rows * S::DP * 4) {
+            const int i = h * each + b, pg = __shfl_sync(0xffffffffu, i < 32 ? page[0] : page[1], i & 31);
+            tma_box(one, to, map, bar, 0, at, head, pg);
+            at = at + rows == a.kv.page_size ? 0 : at + rows;
+          }
+        }
+      };
+      int now[2], then[2] = {page_of(w.lo, lane), page_of(w.lo, lane + 32)};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) now[j] = checked(then[j], w.lo, lane + 32 * j), then[j] = page_of(w.lo + 1, lane + 32 * j);
+      copy(w.lo, now, &kmap);
+#pragma unroll 1
+      for (int t = w.lo; t < hi && ok; ++t) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) then[j] = checked(then[j], t + 1, lane + 32 * j);
+        __syncwarp();
+        if (t + 1 < hi) copy(t + 1, then, &kmap);
+        if (ok) copy(t, now, &vmap);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) now[j] = then[j], then[j] = page_of(t + 2, lane + 32 * j);
+      }
+    }
+    if (!ok || s.abort) {  // no copy is under way when the CTA's memory goes: they take microseconds
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) {
+      }
+    }
   } else if (S::KP == 1 && warp <= kIssueWarp + 2) {
     // ---- copies of keys, or of values: boxes of as many positions as lie in one page
     const bool values = warp == kIssueWarp + 2;
@@ -713,7 +811,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     uint32_t turn = 0;
     bool ok = true;
 #pragma unroll 1
-    for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
+    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
       const int32_t* pages = a.kv.pages_of(w.e.seq);
       const int keys = w.e.len + w.e.nodes, x0 = values ? w.ch0 : 0;
       const int chunks = ((values ? min(S::VD, d - w.ch0) : d) + 63) / 64;
@@ -753,17 +851,29 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             : "memory");
         uint32_t to = slots0 + at_slot * slot_bytes;
         int at = a.kv.slot(t * TK);
-#pragma unroll 1
-        for (int i = 0; i < boxes; ++i, to += rows * 128, at += rows) {
-          if (at == a.kv.page_size) at = 0;
-          int mine = page[0];
-#pragma unroll
-          for (int j = 1; j < B; ++j)
-            if (i >> 5 == j) mine = page[j];
-          const int pg = __shfl_sync(0xffffffffu, mine, i & 31);
+        auto box = [&](int pg) {
 #pragma unroll
           for (int c = 0; c < S::DP / 64; ++c)
             if (c < chunks) tma_box(one, to + c * (TK * 128), map, bar, x0 + c * 64, at, w.head, pg);
+          to += rows * 128;
+          at = at + rows == a.kv.page_size ? 0 : at + rows;
+        };
+        if (boxes <= 4) {  // their pages first: each exchange would be waited for
+          int pg[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, page[0], i);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i < boxes) box(pg[i]);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < boxes; ++i) {
+            int mine = page[0];
+#pragma unroll
+            for (int j = 1; j < B; ++j)
+              if (i >> 5 == j) mine = page[j];
+            box(__shfl_sync(0xffffffffu, mine, i & 31));
+          }
         }
         if (++at_slot == ring) at_slot = 0, turn ^= 1;
       }
@@ -777,16 +887,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     // ---- queries, and drafted values (bf16 caches) or all keys and values (fp32 caches)
     const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kFixWarps);
     const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
-    int unit = 0, it = 0, looks = 0;
+    int unit = 0, it = 0, looks = 0, k_item = 0;
     Ring<KS> k_ring;
     Ring<VS> v_ring;
+    Ring<S::kRaw ? S::RS : 1> r_ring;
     bool ok = true;
     auto signal = [&](const uint64_t& b) {
       async_fence();
       arrive(b);
     };
 #pragma unroll 1
-    for (bool go = w.begin(); go && ok && !s.abort; go = w.next(), ++unit) {
+    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
       const int keys = w.e.len + w.e.nodes;
       if constexpr (S::KP == 1) {
         for (int t = w.lo; t < w.hi; ++t, v_ring.next()) {
@@ -825,77 +936,172 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             if (lane == 0) s.vbad[slot][loader][i] = marks[i];
           }
           signal(s.vfull[slot]);
+          arrive(s.looked[slot]);
         }
-      } else {
-        constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;  // of four rows, eight lanes a row
-        // the place in the pools of row i of this warp's in a tile (-1: none, or a bad page)
-        const int32_t* pages = a.kv.pages_of(w.e.seq);
-        auto row_of = [&](int i) { return (loader + i * S::kFixWarps) * 4; };
-        const int own = row_of(lane >> 2) + (lane & 3);  // the row that this lane looks up
-        auto page_of = [&](int t) {
-          const int key = t * TK + own;
-          return lane < GROUPS * 4 && own < TK && key < keys ? pages[a.kv.ordinal(key)] : -1;
-        };
-        int page = page_of(w.lo);
+      } else if constexpr (S::kRaw) {
+        const int len = w.e.len, hi = w.hi;
+        constexpr int ITEMS = (S::kRawRows / 4 * (S::DP / 64) + S::kFixWarps - 1) / S::kFixWarps;  // four rows, 64 channels
+        auto split = [&](int t, const uint64_t& full, uint32_t to, int part, bool look, int slot) {
+          uint32_t marks[TK / 32] = {};
 #pragma unroll 1
-        for (int t = w.lo; t < w.hi && ok; ++t, ++it, k_ring.next(), v_ring.next()) {
-          long long off = -1;
-          const int key = t * TK + own;
-          if (lane < GROUPS * 4 && own < TK && key < keys) {
-            if (page < 0 || page >= a.kv.num_pages) {
-              kv_report(a.status, ER_KV_BAD_PAGE);
-              s.bad_unit[unit & 15] = unit + 1;
-            } else {
-              off = page * a.kv.page_stride + w.head * a.kv.head_stride + a.kv.slot(key) * a.kv.slot_stride;
+          for (int h = 0; h < 2; ++h, r_ring.next()) {
+            if (!(ok = wait(s.rfull[r_ring.at], r_ring.turn))) return;
+            const uint32_t from = raw0 + r_ring.at * S::kRawSlot;
+            uint4 u[ITEMS], v[ITEMS];
+            // eight lanes read 256 bytes of a row: four of them their second 16 bytes first, for the banks
+            const uint32_t swap = (lane & 4) * 4;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+              const int n = loader + i * S::kFixWarps, r = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
+              if (r >= S::kRawRows) continue;
+              u[i] = lds16(from + r * (S::DP * 4) + c * 32 + swap);
+              v[i] = lds16(from + r * (S::DP * 4) + c * 32 + (swap ^ 16));
+            }
+            arrive(s.rempty[r_ring.at]);
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+              const int n = loader + i * S::kFixWarps, r0 = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
+              const int r = h * S::kRawRows + r0;
+              if (r0 >= S::kRawRows) continue;
+              const uint4 x = swap ? v[i] : u[i], z = swap ? u[i] : v[i];
+              float y[8] = {__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w),
+                            __uint_as_float(z.x), __uint_as_float(z.y), __uint_as_float(z.z), __uint_as_float(z.w)};
+              if (look && t * TK + r >= len) {  // values of drafted tokens, and what lies behind the last one
+                bool bad = false;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) bad |= !(fabsf(y[j]) < INFINITY);
+                if (bad || t * TK + r >= keys) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) y[j] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < TK / 32; ++j)
+                  if (bad && r >> 5 == j) marks[j] |= 1u << (r & 31);
+              }
+              uint4 parts[3];
+              cut8(y, parts);
+              const uint32_t dst = to + swizzled(c, r, TK);
+#pragma unroll
+              for (int j = 0; j < 3; ++j) sts16(dst + j * part, parts[j]);
             }
           }
-          if (t + 1 < w.hi) page = page_of(t + 1);
           __syncwarp();
+          if (look) {
+#pragma unroll
+            for (int i = 0; i < TK / 32; ++i) {
+              marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
+              if (lane == 0) s.vbad[slot][loader][i] = marks[i];
+            }
+          }
+          signal(full);
+          if (look) arrive(s.looked[slot]);
+        };
+        auto keys_of = [&](int t) {
+          if (k_item >= KS && !(ok = wait(s.kempty[k_ring.at], k_ring.turn ^ 1))) return;
+          split(t, s.kfull[k_ring.at], k0 + k_ring.at * S::kKSlot, S::kKPart, false, 0);
+          k_ring.next();
+          ++k_item;
+        };
+        keys_of(w.lo);
+#pragma unroll 1
+        for (int t = w.lo; t < hi && ok; ++t, ++it, v_ring.next()) {
+          if (t + 1 < hi) keys_of(t + 1);
+          if (!ok || (it >= VS && !(ok = wait(s.vempty[v_ring.at], v_ring.turn ^ 1)))) break;
+          split(t, s.vfull[v_ring.at], v0 + v_ring.at * S::kVSlot, S::kVPart, (t + 1) * TK > len, v_ring.at);
+        }
+      } else {
+        // a step: up to 128 channels of the rows in groups of four, eight lanes a row and 64 channels
+        constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;
+        const int32_t* pages = a.kv.pages_of(w.e.seq);
+        const int hi = w.hi, len = w.e.len;
+        auto row_of = [&](int i) { return (loader + i * S::kFixWarps) * 4; };
+        const int own = row_of(lane >> 2) + (lane & 3);  // the row that this lane looks up
+        const bool looks_up = lane < GROUPS * 4 && own < TK;
+        auto page_of = [&](int t) {
+          const int key = t * TK + own;
+          return t < hi && looks_up && key < keys ? pages[a.kv.ordinal(key)] : -1;
+        };
+        auto place_of = [&](int t, int page) -> long long {  // in the pools; -1: none, or a bad page
+          const int key = t * TK + own;
+          if (!looks_up || key >= keys) return -1;
+          if (page < 0 || page >= a.kv.num_pages) {
+            kv_report(a.status, ER_KV_BAD_PAGE);
+            s.bad_unit[unit & 15] = unit + 1;
+            return -1;
+          }
+          return page * a.kv.page_stride + w.head * a.kv.head_stride + a.kv.slot(key) * a.kv.slot_stride;
+        };
+        float4 x[2][GROUPS][2];
+        long long off = place_of(w.lo, page_of(w.lo));
+        int page = page_of(w.lo + 1);
+        const int widths[2] = {d, min(S::VD, d - w.ch0)}, ch0 = w.ch0;
+        auto fetch = [&](int kind, int c0) {
+          __syncwarp();
+          const char* pool = kind ? a.kv.v + ch0 * 4 : a.kv.k;
+          const int width = kind ? widths[1] : widths[0];
+#pragma unroll
+          for (int i = 0; i < GROUPS; ++i) {
+            const long long o = __shfl_sync(0xffffffffu, off, i * 4 + lane / 8);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = c0 + h * 8 + (lane & 7);
+              x[h][i][0] = x[h][i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (o >= 0 && c * 8 < width) {
+                x[h][i][0] = load4((const float*)(pool + o) + c * 8);
+                x[h][i][1] = load4((const float*)(pool + o) + c * 8 + 4);
+              }
+            }
+          }
+        };
+        fetch(0, 0);
+#pragma unroll 1
+        for (int t = w.lo; t < hi && ok; ++t, ++it, k_ring.next(), v_ring.next()) {
 #pragma unroll 1
           for (int kind = 0; kind < 2; ++kind) {  // keys, values
-            const int slot = kind ? v_ring.at : k_ring.at;
+            const int slot = kind ? v_ring.at : k_ring.at, n = ((kind ? widths[1] : widths[0]) + 15) / 16 * 2;
             if (kind ? it >= VS && !(ok = wait(s.vempty[slot], v_ring.turn ^ 1))
                      : it >= KS && !(ok = wait(s.kempty[slot], k_ring.turn ^ 1)))
               break;
             const uint32_t to = kind ? v0 + slot * S::kVSlot : k0 + slot * S::kKSlot;
-            const char* pool = kind ? a.kv.v + w.ch0 * 4 : a.kv.k;
-            const bool look = kind && (t + 1) * TK > w.e.len;
-            const int width = kind ? min(S::VD, d - w.ch0) : d, n = kind ? (width + 15) / 16 * 2 : vecs;
+            const bool look = kind && (t + 1) * TK > len;
             uint32_t marks[TK / 32] = {};
-            for (int c0 = 0; c0 < n; c0 += 8) {  // the same for all lanes: they exchange the rows' places
-              const int c = c0 + (lane & 7);
-              float4 x[GROUPS][2];
+#pragma unroll 1
+            for (int c0 = 0; c0 < n; c0 += 16) {  // the same for all lanes: they exchange the rows' places
 #pragma unroll
-              for (int i = 0; i < GROUPS; ++i) {
-                const long long o = __shfl_sync(0xffffffffu, off, i * 4 + lane / 8);
-                x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (o >= 0 && c * 8 < width) {
-                  x[i][0] = load4((const float*)(pool + o) + c * 8);
-                  x[i][1] = load4((const float*)(pool + o) + c * 8 + 4);
-                }
-              }
+              for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int i = 0; i < GROUPS; ++i) {
-                const int r = row_of(i) + lane / 8;
-                if (r >= TK || c >= n) continue;
-                float y[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
-                if (look && t * TK + r >= w.e.len) {
-                  bool bad = false;
+                for (int i = 0; i < GROUPS; ++i) {
+                  const int r = row_of(i) + lane / 8, c = c0 + h * 8 + (lane & 7);
+                  if (r >= TK || c >= n) continue;
+                  float y[8] = {x[h][i][0].x, x[h][i][0].y, x[h][i][0].z, x[h][i][0].w,
+                                x[h][i][1].x, x[h][i][1].y, x[h][i][1].z, x[h][i][1].w};
+                  if (look && t * TK + r >= len) {
+                    bool bad = false;
 #pragma unroll
-                  for (int j = 0; j < 8; ++j) bad |= !(fabsf(y[j]) < INFINITY);
-                  if (bad) {
+                    for (int j = 0; j < 8; ++j) bad |= !(fabsf(y[j]) < INFINITY);
+                    if (bad) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = 0.f;
+                      for (int j = 0; j < 8; ++j) y[j] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < TK / 32; ++j)
-                      if (r >> 5 == j) marks[j] |= 1u << (r & 31);
+                      for (int j = 0; j < TK / 32; ++j)
+                        if (r >> 5 == j) marks[j] |= 1u << (r & 31);
+                    }
                   }
-                }
-                uint4 parts[3];
-                split8(y, parts);
-                const uint32_t dst = to + swizzled(c, r, TK);
+                  uint4 parts[3];
+                  cut8(y, parts);
+                  const uint32_t dst = to + swizzled(c, r, TK);
 #pragma unroll
-                for (int j = 0; j < 3; ++j) sts16(dst + j * (kind ? S::kVPart : S::kKPart), parts[j]);
+                  for (int j = 0; j < 3; ++j) sts16(dst + j * (kind ? S::kVPart : S::kKPart), parts[j]);
+                }
+              // the next step's are on their way while this one is waited for
+              if (c0 + 16 < n) {
+                fetch(kind, c0 + 16);
+              } else if (kind == 0) {
+                fetch(1, 0);
+              } else if (t + 1 < hi) {
+                off = place_of(t + 1, page);
+                page = page_of(t + 2);
+                fetch(0, 0);
               }
             }
             __syncwarp();
@@ -907,6 +1113,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
               }
             }
             signal(kind ? s.vfull[slot] : s.kfull[slot]);
+            if (look) arrive(s.looked[slot]);
           }
         }
       }
