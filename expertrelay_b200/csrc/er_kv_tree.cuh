@@ -82,6 +82,9 @@ __device__ __forceinline__ Tree kv_tree(const TreeArgs& a, int t) {
 // line, for its queries, masks and result.
 constexpr int kTreeCost = 4, kTreeMinShare = 2;
 
+// the node that a key head's query row belongs to
+__device__ __forceinline__ int tree_node(const TreeArgs& a, int q) { return a.group == 1 ? q : q / a.group; }
+
 struct TreeUnits {
   int rows, blocks, per, units, tiles;  // query rows of a key head, blocks of them, rows of a block
 };

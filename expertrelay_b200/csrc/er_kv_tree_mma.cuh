@@ -11,7 +11,6 @@ namespace er {
 namespace {
 
 constexpr int kSoftmaxWarps = 4, kSumWarps = 8, kIssueWarp = kSoftmaxWarps + kSumWarps;
-constexpr int kStagePitch = 36;  // floats of a row of the epilogue's exchange: 2 x 16 channels and 4 of padding
 
 // KP: bf16 parts of a key or value in shared memory (1: as they come from a bf16 cache, 3: of fp32), QP of a query,
 // PP of a weight. DP: head_dim padded. ROWS: rows of queries in shared memory (of 128 of a product; the others are
@@ -27,13 +26,21 @@ struct TreeShape {
   static constexpr int kSP = PP > 2 ? TK * 3 / 2 : TK;
   // tiles of scores (the products' warp issues them ahead), and results of a tile, kept while they are read
   static constexpr int SB = 3 * kSP + 2 * VD <= 512 ? 3 : 2, OB = SB * kSP + 2 * VD <= 512 ? 2 : 1;
+  // the products' warp goes SB - 1 tiles ahead, over a unit's end too, and the last tile's values are looked at before
+  // its weights
+  static_assert(VS >= SB - 1, "a unit's last values would wait for products behind the next one's queries");
+  // the epilogue's exchange: EC channels of each half at a time, and 4 floats of padding a row
+  static constexpr int EC = KP == 1 && QP > 1 && DP == 128 ? 16 : 32, kStagePitch = 2 * EC + 4;
   // fp32 caches, up to 128 channels: RS half tiles as they come, to be split into parts from there
   static constexpr bool kRaw = KP > 1 && DP <= 128;
   static constexpr int RS = kRaw ? 3 : 0, kRawRows = TK / 2, kRawSlot = kRawRows * DP * 4;
   static constexpr int kSmem = kQ + KS * kKSlot + VS * kVSlot + RS * kRawSlot + ROWS * kStagePitch * 4;
-  // warps that fill shared memory. bf16 caches: one that issues the keys' copies, one the values' and one that looks
-  // after the drafted values. fp32: one that issues copies and four that split, or seven that split from registers.
-  static constexpr int kLoadWarps = KP == 1 ? 3 : kRaw ? 5 : 7, kFixWarps = KP == 1 ? 1 : kRaw ? 4 : 7;
+  // warps that fill shared memory. bf16 caches: one that issues the keys' copies, one the values' and one for the next
+  // unit's queries. fp32: one that issues copies and four that split, or seven that split from registers.
+  static constexpr int kLoadWarps = KP == 1 ? 3 : kRaw ? 5 : 7, kSplitWarps = KP == 1 ? 0 : kRaw ? 4 : 7;
+  static constexpr int kQueryWarps = KP == 1 ? 1 : kSoftmaxWarps;  // of all units but a CTA's first
+  // the warps that look at values of drafted keys
+  static constexpr int kLookWarps = KP == 1 ? kSoftmaxWarps : kSplitWarps;
   static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
   // the column of a tile's weights: part p of the 64 keys from 64 h on
   static __device__ __forceinline__ constexpr int column(int h, int p) { return p < 2 ? h * 64 + p * 32 : TK + h * 32; }
@@ -52,10 +59,11 @@ struct TreeShared {
   int16_t parents[2][kMaxNodes];  // of units in turn: a warp may be one ahead of another
   int bad_unit[16];                 // units (numbers + 1) of a bad page, in turn
   uint32_t sees[S::ROWS][9];        // each row's ancestors and itself, a bit a node
-  uint32_t vbad[S::VS][S::kFixWarps][S::TK / 32];  // keys of a tile whose value was no number (drafted ones)
+  uint32_t vbad[S::VS][S::kLookWarps][S::TK / 32];  // keys of a tile whose value was no number (drafted ones)
   // of tiles in turn: five may be between the weights' warps and the sums'
   float by[8][S::ROWS];             // what a tile's sums so far are multiplied by
   float2 ml[8][S::ROWS];            // maximum and sum of a unit's last tile
+  uint32_t io[S::SB];               // what kind of product a tile's values take
 };
 
 // Descriptors of operands in shared memory, 128-byte swizzle, eight-row groups 1024 bytes apart: the upper word is
@@ -105,13 +113,34 @@ __device__ __forceinline__ bool bar_done(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// a look that does not wait
+__device__ __forceinline__ bool bar_is_done(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// the same, asleep until it is done or for 20 us: a warp that waits leaves the issue slots to those that work
+__device__ __forceinline__ bool bar_done_asleep(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(20000)
+      : "memory");
+  return ok != 0;
+}
 static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, bar_done_asleep(bar, parity))) return true;
   const unsigned long long t0 = globaltimer();
   bool ok = true;
-  while (!bar_done(bar, parity)) {
+  while (!bar_done_asleep(bar, parity)) {
     if (*abort_flag || globaltimer() - t0 > kDefaultWaitNs) {
       *abort_flag = 1;
       ok = false;
@@ -267,66 +296,87 @@ __device__ __forceinline__ uint32_t swizzled(int c, int r, int rows) {
   return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Eight elements at src as 32-bit floats; `wide`: src lies on a 16-byte boundary.
-__device__ __forceinline__ void load8(const float* src, bool wide, float (&x)[8]) {
-  if (wide) {
-    const float4 u = load4(src), v = load4(src + 4);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = src[j];
-  }
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* src, bool wide, float (&x)[8]) {
-  if (wide) {
-    const uint4 u = *reinterpret_cast<const uint4*>(src);
-    const uint32_t h[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[2 * j] = __uint_as_float(h[j] << 16), x[2 * j + 1] = __uint_as_float(h[j] & 0xffff0000u);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = to_f32(src[j]);
-  }
-}
-
 // A unit's queries into shared memory, by `warps` warps of which this is one: eight lanes take 64 channels of a
-// query, which is row qi of every replica.
-template <typename S, typename TQ>
-__device__ __forceinline__ void load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps) {
-  const int lane = threadIdx.x & 31, d = a.kv.d, chunks = (d + 63) / 64, R = w.replicas, per = S::ROWS / R;
-  const int items = (w.live + 3) / 4 * chunks;  // of four queries
-#pragma unroll 2
-  for (int i = warp; i < items; i += warps) {
-    const int g = i / chunks, qi = g * 4 + lane / 8, c = (i - g * chunks) * 8 + (lane & 7);
-    if (qi >= w.live || c * 8 >= (d + 15) / 16 * 16) continue;
-    const int q = w.q0 + qi, node = q / a.group;
-    float x[8] = {};
-    if (c * 8 < d && !a.q_zero)
-      load8((const TQ*)a.q + (long long)(w.e.first + node) * a.q_stride + (long long)(w.head * a.group + q - node * a.group) * d +
-                c * 8,
-            a.q_wide, x);
-    if (a.q_flip) {
+// query, which is row qi of every replica. Several loads are under way at once, the first ones before ready() says
+// that the queries there are used no more.
+template <typename S, typename TQ, typename Ready>
+__device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps, Ready ready) {
+  const int lane = threadIdx.x & 31, d = a.kv.d, R = w.replicas, per = S::ROWS / R, live = w.live;
+  constexpr int chunks = S::DP / 64;
+  const int items = (live + 3) / 4 * chunks;  // of four queries
+  constexpr int U = S::QP == 1 ? 8 : 4, W = sizeof(TQ) / 2;  // W: 16-byte words of eight elements
+  auto place = [&](int i, int* qi, int* c) {
+    const int g = i / chunks;
+    *qi = g * 4 + lane / 8;
+    *c = (i - g * chunks) * 8 + (lane & 7);
+    return i < items && *qi < live && *c * 8 < (d + 15) / 16 * 16;
+  };
+#pragma unroll 1
+  for (int i0 = warp; i0 < items; i0 += warps * U) {
+    uint4 x[U][W];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = -x[j];
+    for (int u = 0; u < U; ++u) {
+      int qi, c;
+#pragma unroll
+      for (int j = 0; j < W; ++j) x[u][j] = make_uint4(0, 0, 0, 0);
+      if (!place(i0 + u * warps, &qi, &c) || c * 8 >= d || a.q_zero) continue;
+      const int q = w.q0 + qi, node = tree_node(a, q);
+      const TQ* src = (const TQ*)a.q + (long long)(w.e.first + node) * a.q_stride +
+                      (long long)(w.head * a.group + q - node * a.group) * d + c * 8;
+      if (a.q_wide) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[u][j] = reinterpret_cast<const uint4*>(src)[j];
+      } else {
+        uint32_t h[4 * W];
+#pragma unroll
+        for (int j = 0; j < 4 * W; ++j) {
+          if constexpr (sizeof(TQ) == 2)
+            h[j] = (uint32_t)__bfloat16_as_ushort(src[2 * j]) | (uint32_t)__bfloat16_as_ushort(src[2 * j + 1]) << 16;
+          else
+            h[j] = __float_as_uint(src[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[u][j] = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+      }
     }
-    uint4 parts[3];
-    if constexpr (S::QP == 1) {  // bf16 as they are
-      uint32_t h[4];
+    if (i0 == warp && !ready()) return false;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = __byte_perm(__float_as_uint(x[2 * j]), __float_as_uint(x[2 * j + 1]), 0x7632);
-      parts[0] = make_uint4(h[0], h[1], h[2], h[3]);
-    } else {
-      split8(x, parts);
-    }
-    for (int r = 0; r < R; ++r) {
-      const uint32_t to = q0 + swizzled(c, r * per + qi, S::ROWS);
+    for (int u = 0; u < U; ++u) {
+      int qi, c;
+      if (!place(i0 + u * warps, &qi, &c)) continue;
+      uint4 parts[3];
+      if constexpr (S::QP == 1) {
+        const uint32_t flip = a.q_flip ? 0x80008000u : 0u;
+        parts[0] = make_uint4(x[u][0].x ^ flip, x[u][0].y ^ flip, x[u][0].z ^ flip, x[u][0].w ^ flip);
+      } else {
+        float y[8];
 #pragma unroll
-      for (int p = 0; p < S::QP; ++p) sts16(to + p * S::kQPart, parts[p]);
+        for (int j = 0; j < W; ++j) {
+          const uint32_t h[4] = {x[u][j].x, x[u][j].y, x[u][j].z, x[u][j].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (sizeof(TQ) == 2)
+              y[2 * e] = __uint_as_float(h[e] << 16), y[2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
+            else
+              y[4 * j + e] = __uint_as_float(h[e]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = a.q_flip ? -y[j] : y[j];
+        split8(y, parts);
+      }
+      for (int r = 0; r < R; ++r) {
+        const uint32_t to = q0 + swizzled(c, r * per + qi, S::ROWS);
+#pragma unroll
+        for (int p = 0; p < S::QP; ++p) sts16(to + p * S::kQPart, parts[p]);
+      }
     }
   }
+  if (warp >= items && !ready()) return false;
   __syncwarp();
   async_fence();
   __syncwarp();
+  return true;
 }
 
 template <typename S, typename TC, typename TQ>
@@ -343,12 +393,16 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   float* stage = reinterpret_cast<float*>(raw + (raw0 + S::RS * S::kRawSlot - smem_u32(raw)));
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < KS; ++i) mbar_init(&s.kfull[i], S::kFixWarps), mbar_init(&s.kempty[i], 1);
-    for (int i = 0; i < VS; ++i)
-      mbar_init(&s.vfull[i], S::kFixWarps), mbar_init(&s.vempty[i], 1), mbar_init(&s.raw[i], 1), mbar_init(&s.looked[i], S::kFixWarps);
-    for (int i = 0; i < S::RS; ++i) mbar_init(&s.rfull[i], 1), mbar_init(&s.rempty[i], S::kFixWarps);
+    for (int i = 0; i < KS; ++i) mbar_init(&s.kfull[i], S::KP == 1 ? 1 : S::kSplitWarps), mbar_init(&s.kempty[i], 1);
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&s.vfull[i], S::kLookWarps);
+      mbar_init(&s.vempty[i], 1);
+      mbar_init(&s.raw[i], 1);
+      mbar_init(&s.looked[i], S::kLookWarps);
+    }
+    for (int i = 0; i < S::RS; ++i) mbar_init(&s.rfull[i], 1), mbar_init(&s.rempty[i], S::kSplitWarps);
     mbar_init(&s.qfirst, kIssueWarp);
-    mbar_init(&s.qfull, kSoftmaxWarps);
+    mbar_init(&s.qfull, S::kQueryWarps);
     mbar_init(&s.qfree, 1);
     for (int i = 0; i < SB; ++i) mbar_init(&s.sfull[i], 1), mbar_init(&s.pfull[i], kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) {
@@ -381,7 +435,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   const TreeWalk& w = s.walk[warp];
   auto next = [&](bool first) { return tree_next(a, s.run, &s.walk[warp], first, S::ROWS / 32); };
   if (warp < kIssueWarp && next(true)) {  // the first unit's queries by the warps that have nothing to do yet
-    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp);
+    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp, [] { return true; });
     arrive(s.qfirst);
   }
 
@@ -392,18 +446,18 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     Ring<VS> v_ring;
 #pragma unroll 1
     for (bool go = next(true); go && !s.abort; go = next(false), ++unit) {
-      if (unit > 0) {  // the first one's are on their way
-        if (!wait(s.qfree, (unit - 1) & 1)) break;
-        load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps);
+      if (S::KP > 1 && unit > 0) {  // the first one's are on their way
+        if (!load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps, [&] { return wait(s.qfree, (unit - 1) & 1); })) break;
         arrive(s.qfull);
       }
       const int R = w.replicas, per = S::ROWS / R, row = threadIdx.x, len = w.e.len, lo = w.lo, hi = w.hi;
       const int qi = row % per, slice = row < S::ROWS ? row / per : 0;
       const bool mine = row < S::ROWS && qi < w.live, live = __any_sync(0xffffffffu, mine);
       uint32_t* sees = s.sees[row < S::ROWS ? row : 0];
+      float m = -INFINITY, l = 0.f;
       // the rows' masks, where this CTA meets drafted keys
-      const bool drafted = hi * TK > len;
-      if (drafted) {
+      bool masked = false;
+      auto mask = [&]() {
         for (int i = threadIdx.x; i < w.e.nodes; i += kSoftmaxWarps * 32) {
           int p = a.parents[w.e.first + i];
           if (p < -1 || p >= i) {
@@ -414,16 +468,50 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           s.parents[masks & 1][i] = (int16_t)p;
         }
         arrive(s.masked);
-        if (!wait(s.masked, masks & 1)) break;
+        if (!wait(s.masked, masks & 1)) return false;
         if (row < S::ROWS)
           for (int i = 0; i < 9; ++i) sees[i] = 0;
         if (mine)
-          for (int p = (w.q0 + qi) / a.group; p >= 0; p = s.parents[masks & 1][p]) sees[p >> 5] |= 1u << (p & 31);
+          for (int p = tree_node(a, w.q0 + qi); p >= 0; p = s.parents[masks & 1][p]) sees[p >> 5] |= 1u << (p & 31);
+        if (s.bad_tree[masks & 1] == masks + 1) l = __int_as_float(0x7fc00000);
         ++masks;
         __syncwarp();
-      }
-      float m = -INFINITY, l = 0.f;
-      if (drafted && s.bad_tree[(masks - 1) & 1] == masks) l = __int_as_float(0x7fc00000);
+        return masked = true;
+      };
+      // values of drafted keys, and of places behind the last one, in shared memory: zero where they are no numbers,
+      // for the rows that do not see them, and marked for those that do
+      auto look = [&](int t, int slot) {
+        const uint32_t to = v0 + slot * S::kVSlot;
+        const int vv = (min(S::VD, d - w.ch0) + 15) / 16 * 2, r0 = len - t * TK, r9 = len + w.e.nodes - t * TK;
+        uint32_t marks[TK / 32] = {};
+#pragma unroll
+        for (int h = 0; h < S::VD / 64; ++h) {
+          const int c = h * 8 + (lane & 7);
+          uint4 v[TK / 16];
+#pragma unroll
+          for (int j = 0; j < TK / 16; ++j) v[j] = lds16(to + swizzled(c, j * 16 + warp * 4 + lane / 8, TK));
+#pragma unroll
+          for (int j = 0; j < TK / 16; ++j) {
+            const int r = j * 16 + warp * 4 + lane / 8;
+            const uint32_t e[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            uint32_t bad = 0;  // whether an exponent is all ones
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bad |= ((e[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+            if (r < r0 || c >= vv || !(bad || r >= r9)) continue;
+            sts16(to + swizzled(c, r, TK), make_uint4(0, 0, 0, 0));
+            if (bad) marks[j / 2] |= 1u << (r & 31);
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < TK / 32; ++i) {
+          marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
+          if (lane == 0) s.vbad[slot][warp][i] = marks[i];
+        }
+        async_fence();
+        arrive(s.vfull[slot]);
+        arrive(s.looked[slot]);
+      };
       const uint32_t sp0 = tmem + ((uint32_t)(warp * 32) << 16);
       // N scores of this row into x: those of the keys from key on of tile t, -inf where the row does not see them
       auto scores = [&](auto& x, int t, int key) {
@@ -446,7 +534,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             for (int j = c; j < N && j < c + 32; ++j)
               if (!(see >> (j - c) & 1)) x[j] = 0xff800000u;
             uint32_t vb = 0;
-            for (int i = 0; i < S::kFixWarps; ++i) vb |= s.vbad[v_ring.at][i][(key + c) >> 5] >> ((key + c) & 31);
+            for (int i = 0; i < S::kLookWarps; ++i) vb |= s.vbad[v_ring.at][i][(key + c) >> 5] >> ((key + c) & 31);
             spoils |= vb & see & (N < 32 ? (1u << (N & 31)) - 1 : 0xffffffffu);
           }
           if (spoils) l = __int_as_float(0x7fc00000);
@@ -528,8 +616,14 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 #pragma unroll 1
       for (int t = lo; t < hi; ++t, ++it, sp_ring.next(), v_ring.next()) {
         if (!(ok = wait(s.sfull[sp_ring.at], sp_ring.turn))) break;
-        if ((t + 1) * TK > len) {  // its values have been looked at
-          if (!(ok = wait(s.looked[v_ring.at], looks >> v_ring.at & 1))) break;
+        if ((t + 1) * TK > len) {  // its values are looked at first
+          const uint32_t turn = looks >> v_ring.at & 1;
+          if (!masked && !(ok = mask())) break;
+          if (S::KP == 1) {
+            if (!(ok = wait(s.raw[v_ring.at], turn))) break;
+            look(t, v_ring.at);
+          }
+          if (!(ok = wait(s.looked[v_ring.at], turn))) break;
           looks ^= 1 << v_ring.at;
         }
         tc_fence_after();
@@ -553,7 +647,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     }
   } else if (warp < kIssueWarp) {
     // ---- sums: a thread a row, of half of the channels
-    constexpr int CH = S::VD / 2;
+    constexpr int CH = S::VD / 2, EC = S::EC, kStagePitch = S::kStagePitch;
     const int row = (warp & 3) * 32 + lane, half = (warp - kSoftmaxWarps) >> 2, id = threadIdx.x - kSoftmaxWarps * 32;
     int it = 0;
     Ring<OB> o_ring;
@@ -597,25 +691,25 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         arrive(s.ofree[ob]);
       }
       if (!ok) break;
-      // the replicas' rows joined: 16 channels of each half at a time by way of shared memory
+      // the replicas' rows joined, by way of shared memory
       const bool whole = w.lo == 0 && w.hi == w.u.tiles, begins = w.lo == 0;
       if (!whole && begins && id == 0)
         a.cut[blockIdx.x] = TreeCut{w.e.first, w.head, w.q0, w.live, w.u.tiles, w.ch0, w.pos, s.run.total};
       const long long piece = (long long)blockIdx.x * 2 + begins;
 #pragma unroll
-      for (int c0 = 0; c0 < CH; c0 += 16) {
+      for (int c0 = 0; c0 < CH; c0 += EC) {
         if (there) {
-          float* mine = stage + row * kStagePitch + half * 16;
+          float* mine = stage + row * kStagePitch + half * EC;
 #pragma unroll
-          for (int j = 0; j < 16; j += 4)
+          for (int j = 0; j < EC; j += 4)
             *reinterpret_cast<ulonglong2*>(mine + j) = make_ulonglong2(o[(c0 + j) / 2], o[(c0 + j) / 2 + 1]);
-          if (c0 == 0 && half == 0) *reinterpret_cast<float2*>(stage + row * kStagePitch + 32) = ml;
+          if (c0 == 0 && half == 0) *reinterpret_cast<float2*>(stage + row * kStagePitch + 2 * EC) = ml;
         }
         arrive(s.staged);
         if (!(ok = wait(s.staged, stages))) break;
         stages ^= 1;
-        for (int i = id; i < w.live * 8; i += kSumWarps * 32) {
-          const int qi = i >> 3, hh = i >> 2 & 1, v = i & 3, ch = hh * CH + c0 + v * 4;
+        for (int i = id; i < w.live * (EC / 2); i += kSumWarps * 32) {
+          const int qi = i / (EC / 2), hh = i / (EC / 4) & 1, v = i % (EC / 4), ch = hh * CH + c0 + v * 4;
           if (ch >= vd) continue;
           float2 p[4];
           float4 x[4];
@@ -626,8 +720,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < R) {
               const float* at = stage + (r * per + qi) * kStagePitch;
-              p[r] = *reinterpret_cast<const float2*>(at + 32);
-              x[r] = *reinterpret_cast<const float4*>(at + hh * 16 + v * 4);
+              p[r] = *reinterpret_cast<const float2*>(at + 2 * EC);
+              x[r] = *reinterpret_cast<const float4*>(at + hh * EC + v * 4);
             }
             top = fmaxf(top, p[r].x);
           }
@@ -639,7 +733,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             fma4(acc, x[r], by);
           }
           if (whole) {
-            const int q = w.q0 + qi, node = q / a.group, g = q - node * a.group;
+            const int q = w.q0 + qi, node = tree_node(a, q), g = q - node * a.group;
             const long long at = (long long)(w.e.first + node) * a.heads + w.head * a.group + g;
             kv_store4((TQ*)a.out + at * d + w.ch0 + ch, acc, sum);
           } else {
@@ -658,7 +752,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     const int ksteps = (d + 15) / 16;
     const uint32_t is = idesc_bf16(TK, 0), one = elected();
     int unit = 0, scored = 0, summed = 0;  // tiles
-    uint32_t io = 0;
     constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
     Ring<SB> sp_ring, p_ring;           // of the tile whose scores, whose values are next
     Ring<OB> o_ring;
@@ -670,7 +763,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       if (summed >= OB && !wait(s.ofree[b], o_ring.turn ^ 1)) return false;
       tc_fence_after();
       uint32_t v = desc_low(v0 + v_ring.at * S::kVSlot, TK * 128);
-      uint32_t to = tmem + SB * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = io;
+      uint32_t to = tmem + SB * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = s.io[p_ring.at];
       // put together here: descriptors that the compiler kept from before the waits' calls came out wrong
       asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
       // the small products first
@@ -695,15 +788,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     bool ok = true;
 #pragma unroll 1
     for (bool go = next(true); go && ok; go = next(false), ++unit) {
-      while (scored > summed && (ok = values())) {
-      }
-      if (!ok) break;
-      io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
-      if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
+      const uint32_t io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
+      // while its queries are on their way, the tiles of the unit before
+      while (ok && unit && scored > summed && !__all_sync(0xffffffffu, bar_is_done(smem_u32(&s.qfull), (unit - 1) & 1)))
+        ok = values();
+      if (!ok || !(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
       const int hi = w.hi;
 #pragma unroll 1
       for (int t = w.lo; t < hi; ++t) {
         if (!(ok = wait(s.kfull[k_ring.at], k_ring.turn))) break;
+        if (lane == 0) s.io[sp_ring.at] = io;
+        __syncwarp();
         tc_fence_after();
         uint32_t kd = desc_low(k0 + k_ring.at * S::kKSlot, 16), qd = desc_low(q0, 16);
         uint32_t to = tmem + sp_ring.at * S::kSP, id = is;
@@ -804,7 +899,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   } else if (S::KP == 1 && warp <= kIssueWarp + 2) {
     // ---- copies of keys, or of values: boxes of as many positions as lie in one page
     const bool values = warp == kIssueWarp + 2;
-    const int rows = a.box_rows, boxes = TK / rows, ring = values ? VS : KS;
+    const int rows = a.box_rows, boxes = TK / rows, box_shift = __ffs(boxes) - 1, ring = values ? VS : KS;
     const CUtensorMap* map = values ? &vmap : &kmap;
     const uint32_t one = elected(), slots0 = values ? v0 : k0, slot_bytes = values ? S::kVSlot : S::kKSlot;
     int unit = 0, it = 0, at_slot = 0;
@@ -813,37 +908,30 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 #pragma unroll 1
     for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
       const int32_t* pages = a.kv.pages_of(w.e.seq);
-      const int keys = w.e.len + w.e.nodes, x0 = values ? w.ch0 : 0;
+      const int len = w.e.len, keys = len + w.e.nodes, x0 = values ? w.ch0 : 0;
       const int chunks = ((values ? min(S::VD, d - w.ch0) : d) + 63) / 64;
-      auto page_of = [&](int t, int i) {  // of box i; behind the last key none
-        const int key = t * TK + i * rows;
-        return i < boxes && key < keys ? pages[a.kv.ordinal(key)] : a.kv.num_pages;
+      // the pages of the unit's boxes, one after another: the lanes hold 32 of them and the 32 behind those
+      const int hi = w.hi, lo = w.lo, head = w.head;
+      auto pages_from = [&](int first) {
+        const int n = first + lane, key = (lo + (n >> box_shift)) * TK + (n & (boxes - 1)) * rows;
+        if (lo + (n >> box_shift) >= hi || key >= keys) return a.kv.num_pages;
+        const int page = pages[a.kv.ordinal(key)];
+        if (page >= 0 && page < a.kv.num_pages) return page;
+        kv_report(a.status, ER_KV_BAD_PAGE);
+        s.bad_unit[unit & 15] = unit + 1;
+        return a.kv.num_pages;  // outside the pool: zeros
       };
-      constexpr int B = TK / 32;  // boxes of a lane at most
-      int next[B];
-#pragma unroll
-      for (int j = 0; j < B; ++j) next[j] = page_of(w.lo, lane + 32 * j);
+      int now = pages_from(0), then = pages_from(32), n = 0, first = 0;
 #pragma unroll 1
-      for (int t = w.lo; t < w.hi; ++t, ++it) {
-        int page[B];
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < B; ++j) {
-          page[j] = next[j];
-          const int i = lane + 32 * j;
-          if (i < boxes && (page[j] < 0 || page[j] >= a.kv.num_pages)) {
-            bad |= t * TK + i * rows < keys;
-            page[j] = a.kv.num_pages;  // outside the pool: zeros
-          }
-          if (t + 1 < w.hi) next[j] = page_of(t + 1, i);
-        }
-        if (__any_sync(0xffffffffu, bad) && lane == 0) {
-          kv_report(a.status, ER_KV_BAD_PAGE);
-          s.bad_unit[unit & 15] = unit + 1;
-        }
+      for (int t = lo; t < hi; ++t, ++it) {
+        __syncwarp();
         if (it >= ring && !(ok = wait(values ? s.vempty[at_slot] : s.kempty[at_slot], turn ^ 1))) break;
         // values of a tile with drafted keys are looked at before they count
-        const uint32_t bar = smem_u32(!values ? &s.kfull[at_slot] : (t + 1) * TK > w.e.len ? &s.raw[at_slot] : &s.vfull[at_slot]);
+        const bool whole = !values || (t + 1) * TK <= len;
+        const uint32_t bar = smem_u32(!values ? &s.kfull[at_slot] : whole ? &s.vfull[at_slot] : &s.raw[at_slot]);
+        if (values && whole && one)
+          for (int i = 1; i < S::kLookWarps; ++i) bar_arrive(bar);
+        __syncwarp();
         asm volatile(
             "{\n\t.reg .pred g;\n\tsetp.ne.b32 g, %2, 0;\n\t"
             "@g mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
@@ -854,27 +942,26 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         auto box = [&](int pg) {
 #pragma unroll
           for (int c = 0; c < S::DP / 64; ++c)
-            if (c < chunks) tma_box(one, to + c * (TK * 128), map, bar, x0 + c * 64, at, w.head, pg);
+            if (c < chunks) tma_box(one, to + c * (TK * 128), map, bar, x0 + c * 64, at, head, pg);
           to += rows * 128;
           at = at + rows == a.kv.page_size ? 0 : at + rows;
         };
         if (boxes <= 4) {  // their pages first: each exchange would be waited for
           int pg[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, page[0], i);
+          for (int i = 0; i < 4; ++i) pg[i] = __shfl_sync(0xffffffffu, now, n + i);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (i < boxes) box(pg[i]);
+          n += boxes;
         } else {
 #pragma unroll 1
-          for (int i = 0; i < boxes; ++i) {
-            int mine = page[0];
-#pragma unroll
-            for (int j = 1; j < B; ++j)
-              if (i >> 5 == j) mine = page[j];
-            box(__shfl_sync(0xffffffffu, mine, i & 31));
+          for (int i = 0; i < boxes; ++i, ++n) {
+            if (n == 32) n = 0, now = then, first += 32, then = pages_from(first + 32);
+            box(__shfl_sync(0xffffffffu, now, n));
           }
         }
+        if (n == 32) n = 0, now = then, first += 32, then = pages_from(first + 32);
         if (++at_slot == ring) at_slot = 0, turn ^= 1;
       }
     }
@@ -884,10 +971,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
     }
   } else {
-    // ---- queries, and drafted values (bf16 caches) or all keys and values (fp32 caches)
-    const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kFixWarps);
+    // ---- the next unit's queries (bf16 caches), or keys and values split into parts (fp32 caches)
+    const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kSplitWarps);
     const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
-    int unit = 0, it = 0, looks = 0, k_item = 0;
+    int unit = 0, it = 0, k_item = 0;
     Ring<KS> k_ring;
     Ring<VS> v_ring;
     Ring<S::kRaw ? S::RS : 1> r_ring;
@@ -900,47 +987,13 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
       const int keys = w.e.len + w.e.nodes;
       if constexpr (S::KP == 1) {
-        for (int t = w.lo; t < w.hi; ++t, v_ring.next()) {
-          if ((t + 1) * TK <= w.e.len) continue;  // neither drafted keys nor places behind the last
-          const int slot = v_ring.at;
-          if (!(ok = wait(s.raw[slot], looks >> slot & 1))) break;
-          looks ^= 1 << slot;
-          const uint32_t to = v0 + slot * S::kVSlot;
-          uint32_t marks[TK / 32] = {};
-          const int vv = (min(S::VD, d - w.ch0) + 15) / 16 * 2, r0 = max(0, w.e.len - t * TK);
-          // eight lanes a row; 32 rows of one 64 channels at a time
-          for (int c = lane & 7; c - (lane & 7) < vv; c += 8)
-#pragma unroll 1
-            for (int r1 = r0 & ~31; r1 < TK; r1 += 32) {
-              uint4 v[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = lds16(to + swizzled(c, r1 + j * 4 + lane / 8, TK));
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int r = r1 + j * 4 + lane / 8;
-                const uint32_t h[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-                uint32_t bad = 0;  // whether an exponent is all ones
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bad |= ((h[e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                // no numbers: zero, for the rows that do not see them, and marked for those that do
-                if (r >= r0 && c < vv && (bad || t * TK + r >= keys)) sts16(to + swizzled(c, r, TK), make_uint4(0, 0, 0, 0));
-#pragma unroll
-                for (int e = 0; e < TK / 32; ++e)
-                  if (bad && r >= r0 && c < vv && r >> 5 == e) marks[e] |= 1u << (r & 31);
-              }
-            }
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < TK / 32; ++i) {
-            marks[i] = __reduce_or_sync(0xffffffffu, marks[i]);
-            if (lane == 0) s.vbad[slot][loader][i] = marks[i];
-          }
-          signal(s.vfull[slot]);
-          arrive(s.looked[slot]);
+        if (unit > 0) {  // the first one's are on their way
+          if (!(ok = load_queries<S, TQ>(a, w, q0, 0, 1, [&] { return wait(s.qfree, (unit - 1) & 1); }))) break;
+          arrive(s.qfull);
         }
       } else if constexpr (S::kRaw) {
         const int len = w.e.len, hi = w.hi;
-        constexpr int ITEMS = (S::kRawRows / 4 * (S::DP / 64) + S::kFixWarps - 1) / S::kFixWarps;  // four rows, 64 channels
+        constexpr int ITEMS = (S::kRawRows / 4 * (S::DP / 64) + S::kSplitWarps - 1) / S::kSplitWarps;  // four rows, 64 channels
         auto split = [&](int t, const uint64_t& full, uint32_t to, int part, bool look, int slot) {
           uint32_t marks[TK / 32] = {};
 #pragma unroll 1
@@ -952,7 +1005,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             const uint32_t swap = (lane & 4) * 4;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-              const int n = loader + i * S::kFixWarps, r = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
+              const int n = loader + i * S::kSplitWarps, r = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
               if (r >= S::kRawRows) continue;
               u[i] = lds16(from + r * (S::DP * 4) + c * 32 + swap);
               v[i] = lds16(from + r * (S::DP * 4) + c * 32 + (swap ^ 16));
@@ -960,7 +1013,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
             arrive(s.rempty[r_ring.at]);
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
-              const int n = loader + i * S::kFixWarps, r0 = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
+              const int n = loader + i * S::kSplitWarps, r0 = n / (S::DP / 64) * 4 + lane / 8, c = n % (S::DP / 64) * 8 + (lane & 7);
               const int r = h * S::kRawRows + r0;
               if (r0 >= S::kRawRows) continue;
               const uint4 x = swap ? v[i] : u[i], z = swap ? u[i] : v[i];
@@ -1011,10 +1064,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         }
       } else {
         // a step: up to 128 channels of the rows in groups of four, eight lanes a row and 64 channels
-        constexpr int GROUPS = (TK / 4 + S::kFixWarps - 1) / S::kFixWarps;
+        constexpr int GROUPS = (TK / 4 + S::kSplitWarps - 1) / S::kSplitWarps;
         const int32_t* pages = a.kv.pages_of(w.e.seq);
         const int hi = w.hi, len = w.e.len;
-        auto row_of = [&](int i) { return (loader + i * S::kFixWarps) * 4; };
+        auto row_of = [&](int i) { return (loader + i * S::kSplitWarps) * 4; };
         const int own = row_of(lane >> 2) + (lane & 3);  // the row that this lane looks up
         const bool looks_up = lane < GROUPS * 4 && own < TK;
         auto page_of = [&](int t) {
