@@ -6,58 +6,93 @@ namespace er {
 
 namespace {
 
-// Joins the units that several CTAs share: a warp a query row, the rows of the
-// unit that begins in CTA blockIdx.x's run. Also writes the rows of trees that
-// something is wrong with, which no attention CTA meets.
-constexpr int kJoinWarps = 8;
+// Joins the units that several CTAs share: CTA (x, y) takes every gridDim.x-th
+// of them from x on, of its rows every gridDim.y-th. Of many pieces the warps
+// share a row's, of few each takes rows of its own. Also writes the rows of
+// trees that something is wrong with, which no attention CTA meets.
+constexpr int kJoinWarps = 8, kJoinMost = 1024;  // CTAs that may share a line at most
 
 template <typename TQ>
 __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv_tree_join_kernel(const __grid_constant__ TreeArgs a) {
+  __shared__ int cuts[kJoinMost], found;
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float2 tops[kJoinWarps];
   kv_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
-  for (int t = blockIdx.y * a.grid + blockIdx.x; t < a.trees; t += a.grid * gridDim.y) {
+  for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.trees; t += gridDim.x * gridDim.y) {
     const Tree e = kv_tree(a, t);
     if (!e.bad) continue;
     TQ* out = (TQ*)a.out + (long long)e.first * a.heads * d;
     for (long long i = threadIdx.x; i < (long long)e.nodes * a.heads * d; i += kJoinWarps * 32)
       out[i] = kv_round<TQ>(__int_as_float(0x7fc00000));
   }
-  const TreeCut c = a.cut[blockIdx.x];
-  if (c.live == 0) return;
-  const int shares = tree_shares(a, c.total), i0 = blockIdx.x;
-  const int n = kv_share_of(c.total, shares, c.begin + kTreeCost + c.tiles - 1) - i0 + 1;  // pieces
-  const int width = min(a.channels, d - c.ch0);
-  const bool mine = lane * 4 < width;
-  for (int r = blockIdx.y * kJoinWarps + warp; r < c.live; r += gridDim.y * kJoinWarps) {
-    auto at = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * a.piece_rows + r; };
-    float top = -INFINITY;
-    for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[at(k) * 2]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int N = 8;  // pieces under way
-#pragma unroll 1
-    for (int k0 = 0; k0 < n; k0 += N) {
-      float2 ml[N];
-      float4 x[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (k0 + j >= n) continue;
-        ml[j] = *reinterpret_cast<const float2*>(a.part_ml + at(k0 + j) * 2);
-        if (mine) x[j] = *reinterpret_cast<const float4*>(a.part_o + at(k0 + j) * a.channels + lane * 4);
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (k0 + j >= n) continue;
-        const float weight = piece_weight(ml[j].x, top);
-        sum = fmaf(ml[j].y, weight, sum);  // a spoilt piece's sum is NaN
-        if (mine) fma4(acc, x[j], weight);
-      }
+  if (warp == 0) {  // the CTAs in whose runs such a unit begins
+    int n = 0;
+    for (int c0 = 0; c0 < a.grid; c0 += 32) {
+      const bool cut = c0 + lane < a.grid && a.cut[c0 + lane].live > 0;
+      const uint32_t all = __ballot_sync(0xffffffffu, cut);
+      if (cut) cuts[n + __popc(all & ((1u << lane) - 1))] = c0 + lane;
+      n += __popc(all);
     }
-    const int q = c.q0 + r, node = q / a.group, g = q - node * a.group;
-    if (mine)
-      kv_store4((TQ*)a.out + ((long long)(c.first + node) * a.heads + c.head * a.group + g) * d + c.ch0 + lane * 4, acc, sum);
+    if (lane == 0) found = n;
+  }
+  __syncthreads();
+  constexpr int N = 8;  // pieces under way
+#pragma unroll 1
+  for (int f = blockIdx.x; f < found; f += gridDim.x) {
+    const int i0 = cuts[f];
+    const TreeCut c = a.cut[i0];
+    const int n = kv_share_of(c.total, tree_shares(a, c.total), c.begin + a.unit_cost + c.tiles - 1) - i0 + 1;  // pieces
+    const bool together = n > 2 * N;
+    const int step = together ? gridDim.y : gridDim.y * kJoinWarps, k1 = together ? warp : 0, by = together ? kJoinWarps : 1;
+    const int width = min(a.channels, d - c.ch0);
+    const bool mine = lane * 4 < width;
+#pragma unroll 1
+    for (int r = together ? blockIdx.y : blockIdx.y * kJoinWarps + warp; r < c.live; r += step) {
+      auto at = [&](int k) { return ((long long)(i0 + k) * 2 + (k == 0 ? 1 : 0)) * a.piece_rows + r; };
+      float top = -INFINITY;
+      for (int k = k1 + lane * by; k < n; k += 32 * by) top = fmaxf(top, a.part_ml[at(k) * 2]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int k0 = k1; k0 < n; k0 += N * by) {
+        float2 ml[N];
+        float4 x[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (k0 + j * by >= n) continue;
+          ml[j] = *reinterpret_cast<const float2*>(a.part_ml + at(k0 + j * by) * 2);
+          if (mine) x[j] = *reinterpret_cast<const float4*>(a.part_o + at(k0 + j * by) * a.channels + lane * 4);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (k0 + j * by >= n) continue;
+          const float weight = piece_weight(ml[j].x, top);
+          sum = fmaf(ml[j].y, weight, sum);  // a spoilt piece's sum is NaN
+          if (mine) fma4(acc, x[j], weight);
+        }
+      }
+      if (together) {
+        __syncthreads();
+        sums[warp][lane] = acc;
+        if (lane == 0) tops[warp] = make_float2(top, sum);
+        __syncthreads();
+        if (warp > 0) continue;
+        for (int i = 1; i < kJoinWarps; ++i) top = fmaxf(top, tops[i].x);
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+        for (int i = 0; i < kJoinWarps; ++i) {
+          const float weight = piece_weight(tops[i].x, top);
+          sum = fmaf(tops[i].y, weight, sum);
+          fma4(acc, sums[i][lane], weight);
+        }
+      }
+      const int q = c.q0 + r, node = tree_node(a, q), g = q - node * a.group;
+      if (mine)
+        kv_store4((TQ*)a.out + ((long long)(c.first + node) * a.heads + c.head * a.group + g) * d + c.ch0 + lane * 4, acc, sum);
+    }
   }
 }
 
@@ -148,6 +183,7 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   if ((uintptr_t)io->out & 15) return fail(ER_EINVAL, "er_kv_tree: out must be 16-byte aligned");
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
+  if (sms > kJoinMost) sms = kJoinMost;
   const TreeLayout L = tree_layout(*cache, *io, sms);
   if (!workspace || workspace_bytes < L.bytes)
     return fail(ER_ENOSPACE, "er_kv_tree: workspace %zu bytes, need %zu", workspace_bytes, L.bytes);
@@ -174,6 +210,9 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   a.part_o = (float*)(ws + L.o);
   while (1 << a.tile_shift < L.shape.tile) ++a.tile_shift;
   while (1 << a.block_shift < L.shape.rows) ++a.block_shift;
+  // 24 trees of up to 4097 positions, 16 heads, bf16: 4 tiles 147 us, 8 141, 14 139, 24 140; 6 of up to 2500, fp32,
+  // whose tiles take four times as long: 150, 151, 157 and 169
+  a.unit_cost = cb ? 12 : 4;
   a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
   CUtensorMap maps[2] = {};
   if (L.shape.box_rows) {
@@ -183,11 +222,13 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
     if (int rc = tree_map(&maps[1], *cache, cache->v, a.box_rows, L.shape.box_channels)) return rc;
   }
   if (int rc = cb ? tree_bf16(a, io->q_dtype, maps, st) : tree_f32(a, io->q_dtype, maps, st)) return rc;
-  // as many units as CTAs: each is cut in two or three pieces, and few CTAs do for its rows
-  int parts = (L.piece_rows + kJoinWarps - 1) / kJoinWarps;
-  const int most = (long long)io->trees * cache->kv_heads >= sms ? 4 : 16;
-  if (parts > most) parts = most;
-  const dim3 grid(sms, parts);
+  // few units: many pieces each, and a CTA a row for them
+  const long long blocks = ((long long)(io->rows < kMaxNodes ? io->rows : kMaxNodes) * a.group + a.block_rows - 1) / a.block_rows;
+  const long long units = (long long)io->trees * cache->kv_heads * blocks * a.halves;
+  const int across = units < sms ? (int)units : sms;
+  int parts = 4 * sms / across;
+  if (parts > L.piece_rows) parts = L.piece_rows;
+  const dim3 grid(across, parts);
   return qb ? kv_launch(kv_tree_join_kernel<bf>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a)
             : kv_launch(kv_tree_join_kernel<float>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a);
 }

@@ -36,6 +36,7 @@ struct TreeArgs {
   int q_wide;              // rows of q on 16-byte boundaries
   int q_flip, q_zero;      // the scale was negative, or zero: queries change their sign, or are zero
   int tile_shift;          // log2 of a tile's keys
+  int unit_cost;           // what a unit takes beside its tiles, in tiles
   int block_rows, block_shift;  // query rows of a unit at most (a power of two), and its log2
   int channels, halves;    // of the values: those of a unit, units beside each other for all of them
   int box_rows;            // positions that a copy takes: they lie in one page wherever it begins
@@ -78,9 +79,9 @@ __device__ __forceinline__ Tree kv_tree(const TreeArgs& a, int t) {
 
 // The line that the CTAs share. A unit is a block of at most block_rows query
 // rows (nodes x group, in equal blocks) of one key head of a tree, and of at
-// most 128 channels of its values; it takes its tiles and kTreeCost of the
+// most 128 channels of its values; it takes its tiles and unit_cost of the
 // line, for its queries, masks and result.
-constexpr int kTreeCost = 4, kTreeMinShare = 2;
+constexpr int kTreeMinShare = 2;
 
 // the node that a key head's query row belongs to
 __device__ __forceinline__ int tree_node(const TreeArgs& a, int q) { return a.group == 1 ? q : q / a.group; }
@@ -122,7 +123,7 @@ __device__ __forceinline__ void tree_run(const TreeArgs& a, TreeRun& run, TreeSc
     const Tree e = kv_tree(a, t);
     if (blockIdx.x == 0 && e.bad) kv_report(a.status, e.bad);
     const TreeUnits u = tree_units(a, e);
-    mine += (long long)u.units * (u.tiles + kTreeCost);
+    mine += (long long)u.units * (u.tiles + a.unit_cost);
   }
   long long in = mine;
 #pragma unroll
@@ -147,7 +148,7 @@ __device__ __forceinline__ void tree_run(const TreeArgs& a, TreeRun& run, TreeSc
         int t = t0;
         for (; t < t1; ++t) {
           const TreeUnits u = tree_units(a, kv_tree(a, t));
-          const long long c = (long long)u.units * (u.tiles + kTreeCost);
+          const long long c = (long long)u.units * (u.tiles + a.unit_cost);
           if (from < at + c) break;
           at += c;
         }
@@ -179,12 +180,12 @@ static __device__ __noinline__ bool tree_next(const TreeArgs& a, const TreeRun& 
     w.t = run.t;
     w.e = kv_tree(a, w.t);
     w.u = tree_units(a, w.e);
-    const int c = w.u.tiles + kTreeCost;
+    const int c = w.u.tiles + a.unit_cost;
     w.unit = (int)kv_div(run.from - run.at, c);
     w.pos = run.at + (long long)w.unit * c;
   } else {
     w = *walk;
-    w.pos += w.u.tiles + kTreeCost;
+    w.pos += w.u.tiles + a.unit_cost;
     ++w.unit;
   }
   for (;;) {
@@ -197,11 +198,11 @@ static __device__ __noinline__ bool tree_next(const TreeArgs& a, const TreeRun& 
       } while (w.u.units == 0);
       w.unit = 0;
     }
-    const long long tile0 = w.pos + kTreeCost;
+    const long long tile0 = w.pos + a.unit_cost;
     w.lo = run.from > tile0 ? (int)(run.from - tile0 < w.u.tiles ? run.from - tile0 : w.u.tiles) : 0;
     w.hi = run.to < tile0 + w.u.tiles ? (int)(run.to > tile0 ? run.to - tile0 : 0) : w.u.tiles;
     if (w.hi > w.lo) break;
-    w.pos += w.u.tiles + kTreeCost;
+    w.pos += w.u.tiles + a.unit_cost;
     ++w.unit;
   }
   const int beside = w.u.blocks * a.halves;

@@ -1055,12 +1055,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           k_ring.next();
           ++k_item;
         };
+        auto values_of = [&](int t) {
+          if (it >= VS && !(ok = wait(s.vempty[v_ring.at], v_ring.turn ^ 1))) return;
+          split(t, s.vfull[v_ring.at], v0 + v_ring.at * S::kVSlot, S::kVPart, (t + 1) * TK > len, v_ring.at);
+          v_ring.next();
+          ++it;
+        };
         keys_of(w.lo);
 #pragma unroll 1
-        for (int t = w.lo; t < hi && ok; ++t, ++it, v_ring.next()) {
+        for (int t = w.lo; t < hi && ok; ++t) {
           if (t + 1 < hi) keys_of(t + 1);
-          if (!ok || (it >= VS && !(ok = wait(s.vempty[v_ring.at], v_ring.turn ^ 1)))) break;
-          split(t, s.vfull[v_ring.at], v0 + v_ring.at * S::kVSlot, S::kVPart, (t + 1) * TK > len, v_ring.at);
+          if (ok) values_of(t);
         }
       } else {
         // a step: up to 128 channels of the rows in groups of four, eight lanes a row and 64 channels
