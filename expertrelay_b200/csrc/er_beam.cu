@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kScanThreads = 256, kEach = 16, kTile = kScanThreads * kEach;  // logits a tile
 constexpr int kMaxCount = 128, kMaxBeams = 1024;
-constexpr int kHeld = kTile + kMaxCount;  // what a CTA may hold before it has to choose
+constexpr int kMaxKeep = 2 * kMaxCount, kHeld = kTile + kMaxKeep;  // what a CTA may hold before it has to choose
 
 struct BeamArgs {
   const void* logits;
@@ -27,7 +27,8 @@ struct BeamArgs {
   int parts, part;  // of a row, and logits of each (a multiple of the tile)
   double* sums;     // [rows][parts] of 2^.. relative to maxima
   float* maxima;    // [rows][parts]
-  unsigned long long* kept;  // [rows][parts][count]: rank key of the logit, then ~token; 0 behind the last
+  int keep;                  // of a part, at most: count at the least where there are as many
+  unsigned long long* kept;  // [rows][parts][keep]: rank key of the logit, then ~token; 0 behind the last
   float* scores_out;
   int32_t *beams_out, *tokens_out;
 };
@@ -55,16 +56,15 @@ struct BlockCount {
   }
 };
 
-// A bound that exactly `want` of the block's distinct keys reach (has(t): how
-// many of the thread's keys are >= t), by halving; `least` .. `most`: such that
-// all, or more than `want`, reach the one and less than `want` the other + 1.
+// A bound that at least `want` of the block's keys reach and, where that can be, at most `enough` (has(t): how many
+// of the thread's keys are >= t), by halving. `least`: one that `want` reach; `most`: none above it is reached by as many.
 template <typename Has>
-__device__ __forceinline__ unsigned long long bound_of(int want, unsigned long long least, unsigned long long most,
-                                                       BlockCount& count, Has has) {
+__device__ __forceinline__ unsigned long long bound_of(int want, int enough, unsigned long long least,
+                                                       unsigned long long most, BlockCount& count, Has has) {
   while (least < most) {
     const unsigned long long mid = least + (most - least) / 2 + 1;
     const int n = count(has(mid));
-    if (n == want) return mid;
+    if (n >= want && n <= enough) return mid;
     if (n > want)
       least = mid;
     else
@@ -73,115 +73,183 @@ __device__ __forceinline__ unsigned long long bound_of(int want, unsigned long l
   return least;
 }
 
-template <typename T>
-__device__ __forceinline__ void load_tile(const T* row, int i0, int end, bool wide, float (&x)[kEach]) {
-  // thread t has logits 4 t .. 4 t + 3 of each fourth of the tile, however the row is aligned: equal rows
-  // give equal sums
-#pragma unroll
-  for (int j = 0; j < kEach / 4; ++j) {
-    const int i = i0 + j * kScanThreads * 4 + threadIdx.x * 4;
-    if (wide && i + 4 <= end) {
-      const float4 v = load4(row + i);
-      x[j * 4] = v.x, x[j * 4 + 1] = v.y, x[j * 4 + 2] = v.z, x[j * 4 + 3] = v.w;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[j * 4 + e] = i + e < end ? to_f32(row[i + e]) : -INFINITY;
-    }
-  }
+// Appends the keys of the threads that have one to a list in shared memory, a warp at a time.
+__device__ __forceinline__ int place_of(bool mine, int* n) {
+  const uint32_t all = __ballot_sync(0xffffffffu, mine);
+  int base = 0;
+  if ((threadIdx.x & 31) == 0 && all) base = atomicAdd(n, __popc(all));
+  return __shfl_sync(0xffffffffu, base, 0) + __popc(all & ((1u << (threadIdx.x & 31)) - 1));
 }
 
+// Sixteen logits of a tile, runs of kRun: thread t has runs t, t + 256, ... however the row is aligned, so that equal
+// rows give equal sums. Those behind the end are -inf.
 template <typename T>
-__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
+struct Logits {
+  static constexpr int kRun = 16 / (int)sizeof(T), kRuns = kEach / kRun;
+  uint4 raw[kRuns];
+
+  __device__ __forceinline__ static int at(int j) { return (j / kRun) * kScanThreads * kRun + threadIdx.x * kRun + j % kRun; }
+  __device__ __forceinline__ void load(const T* row, int i0, int end, bool wide) {
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      const int i = i0 + at(r * kRun);
+      if (wide && i + kRun <= end) {
+        raw[r] = __ldg(reinterpret_cast<const uint4*>(row + i));
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 4) {
+            h[e] = i + e < end ? __float_as_uint(row[i + e]) : 0xff800000u;
+          } else {
+            const uint32_t lo = i + 2 * e < end ? __bfloat16_as_ushort(row[i + 2 * e]) : 0xff80u;
+            const uint32_t hi = i + 2 * e + 1 < end ? __bfloat16_as_ushort(row[i + 2 * e + 1]) : 0xff80u;
+            h[e] = lo | hi << 16;
+          }
+        }
+        raw[r] = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    }
+  }
+  __device__ __forceinline__ void floats(float (&x)[kEach]) const {
+#pragma unroll
+    for (int r = 0; r < kRuns; ++r) {
+      const uint32_t h[4] = {raw[r].x, raw[r].y, raw[r].z, raw[r].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) {
+          x[r * kRun + e] = __uint_as_float(h[e]);
+        } else {
+          x[r * kRun + 2 * e] = __uint_as_float(h[e] << 16);
+          x[r * kRun + 2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
+        }
+      }
+    }
+  }
+};
+
+// e^x for x <= 0 in 32 bits: within 2^-22 and |x| 2^-25 of it
+__device__ __forceinline__ float exp_below(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  return y;
+}
+
+// Of every logit: a maximum, a subtraction, a product, an exponential and a sum; whether it can be among the best is
+// asked of a thread's greatest, and only a thread that has one looks again. Sums of 16 go to 64 bits.
+template <typename T>
+__global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid_constant__ BeamArgs a) {
   kv_enter();
   __shared__ unsigned long long held[kHeld];
   __shared__ int red[64], held_n;
+  __shared__ uint32_t warp_least[kScanThreads / 32];
   __shared__ double sums[kScanThreads / 32];
   __shared__ float tops[kScanThreads / 32];
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int begin = blockIdx.x * a.part, end = min(a.vocab, begin + a.part);
   const T* logits = (const T*)a.logits + row * a.stride;
-  const bool wide = ((uintptr_t)logits & (4 * sizeof(T) - 1)) == 0;
+  const bool wide = ((uintptr_t)logits & 15) == 0;
   BlockCount count{red, 0};
+  Logits<T> next;
+  next.load(logits, begin, end, wide);
   if (threadIdx.x == 0) held_n = 0;
   float m = -INFINITY;
   double sum = 0.0;
   unsigned long long bound = 0;  // what has to be reached to be held
-  bool nan = false;
-  // the best a.count of what is held, moved to its front
+  float least = -INFINITY;       // its logit (NaN where it has none: everything may)
+  int most_held = 0;             // the same in all threads, and no less than is held
+  // the best of what is held, a.count to a.keep of them, moved to its front
   auto choose = [&]() {
     __syncthreads();
     const int n = held_n;
-    if (n <= a.count) return;
-    constexpr int E = (kHeld + kScanThreads - 1) / kScanThreads;
-    unsigned long long mine[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) mine[j] = threadIdx.x + j * kScanThreads < n ? held[threadIdx.x + j * kScanThreads] : 0;
-    bound = bound_of(a.count, bound, ~0ull - 1, count, [&](unsigned long long t) {
+    if (n <= a.keep) return;
+    bound = bound_of(a.count, a.keep, bound, ~0ull - 1, count, [&](unsigned long long t) {
       int c = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j) c += mine[j] >= t;
+      for (int i = threadIdx.x; i < n; i += kScanThreads) c += held[i] >= t;
       return c;
     });
-    __syncthreads();
+    least = unrank((uint32_t)(bound >> 32));
     if (threadIdx.x == 0) held_n = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < E; ++j)
-      if (mine[j] >= bound && mine[j]) held[atomicAdd(&held_n, 1)] = mine[j];
-    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += kScanThreads) {
+      // entries in front of i0 were read before, and no more of them than of those can have been kept
+      const unsigned long long mine = i0 + (int)threadIdx.x < n ? held[i0 + threadIdx.x] : 0;
+      __syncthreads();
+      const bool take = mine && mine >= bound;
+      const int at = place_of(take, &held_n);
+      if (take) held[at] = mine;
+      __syncthreads();
+    }
   };
 #pragma unroll 1
   for (int i0 = begin; i0 < end; i0 += kTile) {
     float x[kEach];
-    load_tile(logits, i0, end, wide, x);
+    next.floats(x);
+    if (i0 + kTile < end) next.load(logits, i0 + kTile, end, wide);
     float top = x[0];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      nan |= x[j] != x[j];
-      top = fmaxf(top, x[j]);
-    }
+    for (int j = 1; j < kEach; ++j) top = fmaxf(top, x[j]);
     if (top > m) {
-      sum *= (double)expf(m - top);  // 0 where m is -inf
+      sum *= (double)exp_below(m - top);  // 0 where m is -inf
       m = top;
     }
-    if (m != -INFINITY) {
+    // a thread whose logits are all -inf, or NaN among them, so far: its sum stays 0, or becomes NaN
+    const float ref = m == -INFINITY ? 0.f : m;
+    float part[4];
 #pragma unroll
-      for (int j = 0; j < kEach; j += 4)
-        sum += (double)(expf(x[j] - m) + expf(x[j + 1] - m) + (expf(x[j + 2] - m) + expf(x[j + 3] - m)));
-    }
-    unsigned long long best = 0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const int i = i0 + (j / 4) * kScanThreads * 4 + threadIdx.x * 4 + j % 4;
-      if (i < end) best = max(best, pack(x[j], i));
-    }
+    for (int j = 0; j < 4; ++j)
+      part[j] = (exp_below(x[j] - ref) + exp_below(x[j + 4] - ref)) + (exp_below(x[j + 8] - ref) + exp_below(x[j + 12] - ref));
+    sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
     if (i0 == begin) {
-      // at least a.count logits reach the a.count-th of the threads' best, and at most kEach times as many
-      bound = bound_of(a.count, 0, ~0ull - 1, count, [&](unsigned long long t) { return (int)(best >= t); });
+      // as many of each warp's threads as make a.count of the block's: what their greatest logits reach, at least
+      // a.count do
+      uint32_t key = begin + Logits<T>::at(0) < end ? rank_key(top) : 0u, r = 0;
+      for (int k = 0; k < a.count; k += kScanThreads / 32) {
+        r = __reduce_max_sync(0xffffffffu, key);
+        const uint32_t who = __ballot_sync(0xffffffffu, key == r);
+        if (lane == __ffs(who) - 1) key = 0;
+      }
+      if (lane == 0) warp_least[warp] = r;
+      __syncthreads();
+      r = warp_least[0];
+      for (int w = 1; w < kScanThreads / 32; ++w) r = min(r, warp_least[w]);
+      bound = (unsigned long long)r << 32;
+      least = unrank(r);
     }
-    if (best >= bound) {
+    bool look = !(top < least);
+    const int lookers = __syncthreads_count(look) * kEach;  // what was held before is there, too
+    if (most_held + lookers > kHeld) {
+      most_held = held_n;
+      __syncthreads();
+      if (most_held + lookers > kHeld) {
+        choose();
+        most_held = a.keep;
+        look = !(top < least);
+      }
+    }
+    most_held += lookers;
+    if (look) {
+      uint32_t which = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) which |= (uint32_t)!(x[j] < least) << j;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) {
-        const int i = i0 + (j / 4) * kScanThreads * 4 + threadIdx.x * 4 + j % 4;
-        if (i >= end) continue;
+        const int i = i0 + Logits<T>::at(j);
+        if (!(which >> j & 1) || i >= end) continue;
         const unsigned long long p = pack(x[j], i);
         if (p >= bound) held[atomicAdd(&held_n, 1)] = p;
       }
     }
-    __syncthreads();
-    if (held_n > kMaxCount) choose();  // the next tile may add kTile
-    __syncthreads();
   }
   choose();
   __syncthreads();
-  unsigned long long* kept = a.kept + ((long long)row * a.parts + blockIdx.x) * a.count;
-  for (int i = threadIdx.x; i < a.count; i += kScanThreads) kept[i] = i < held_n ? held[i] : 0;
+  unsigned long long* kept = a.kept + ((long long)row * a.parts + blockIdx.x) * a.keep;
+  for (int i = threadIdx.x; i < a.keep; i += kScanThreads) kept[i] = i < held_n ? held[i] : 0;
   // the threads' sums, in an order that does not change
   float top = m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (m != -INFINITY) sum *= (double)expf(m - top);
-  if (nan) sum = __longlong_as_double(0x7ff8000000000000ll);
+  if (m != -INFINITY) sum *= (double)exp_below(m - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum, tops[warp] = top;
@@ -190,14 +258,14 @@ __global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const __grid_co
     float all = tops[0];
     for (int w = 1; w < kScanThreads / 32; ++w) all = fmaxf(all, tops[w]);
     double s = 0.0;
-    for (int w = 0; w < kScanThreads / 32; ++w) s += tops[w] == -INFINITY ? sums[w] : sums[w] * (double)expf(tops[w] - all);
+    for (int w = 0; w < kScanThreads / 32; ++w) s += tops[w] == -INFINITY ? sums[w] : sums[w] * (double)exp_below(tops[w] - all);
     a.sums[(long long)row * a.parts + blockIdx.x] = s;
     a.maxima[(long long)row * a.parts + blockIdx.x] = all;
   }
 }
 
 // ---- the choice over a batch's beams
-constexpr int kPickThreads = 512, kPickChunk = 4096;
+constexpr int kPickThreads = 512, kPickEach = 4, kPickChunk = kPickThreads * kPickEach, kFew = 512;
 
 // the order of doubles as unsigned integers (no NaN comes here; the zeros alike)
 __device__ __forceinline__ unsigned long long rank_key64(double v) {
@@ -214,16 +282,29 @@ struct PickShared {
   int red[64], n;
 };
 
-// Grid: a CTA a batch.
+// Grid: a CTA a batch. It goes over what was kept kPickChunk at a time: those that may be among the best join the best
+// so far in shared memory, and the best of them are found by a bound on their values, then by their ranks.
 __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_constant__ BeamArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   PickShared& s = *reinterpret_cast<PickShared*>(smem);
   kv_enter();
   const int batch = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int each = a.parts * a.keep;  // of a beam
+  const long long total = (long long)each * a.beams;
+  unsigned long long kept[kPickEach];
+  auto fetch = [&](long long c0) {
+#pragma unroll
+    for (int i = 0; i < kPickEach; ++i) {
+      const long long c = c0 + i * kPickThreads + threadIdx.x;
+      kept[i] = c < total ? a.kept[(long long)batch * total + c] : 0;
+    }
+  };
+  fetch(0);
   BlockCount count{s.red, 0};
   if (threadIdx.x == 0) s.n = 0;
+  const long long row0 = (long long)batch * a.beams;
   for (int b = warp; b < a.beams; b += kPickThreads / 32) {
-    const long long at = ((long long)batch * a.beams + b) * a.parts;
+    const long long at = (row0 + b) * a.parts;
     float top = -INFINITY;
     for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.maxima[at + p]);
 #pragma unroll
@@ -231,43 +312,50 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
     double sum = 0.0;
     for (int p = lane; p < a.parts; p += 32) {
       const float m = a.maxima[at + p];
-      sum += m == -INFINITY ? a.sums[at + p] : a.sums[at + p] * (double)expf(m - top);
+      sum += m == -INFINITY ? a.sums[at + p] : a.sums[at + p] * exp((double)m - (double)top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s.lse[b] = (double)top + log(sum);
   }
   __syncthreads();
-  const long long each = (long long)a.parts * a.count, total = each * a.beams;
+  const int few = min(kFew, 2 * a.count + 32);
   unsigned long long least = 0;  // a value that a.count of what is held reach
-  constexpr int E = (kPickChunk + kMaxCount + kPickThreads - 1) / kPickThreads;
+  constexpr int E = kPickEach + 1;
 #pragma unroll 1
   for (long long c0 = 0; c0 < total; c0 += kPickChunk) {
-    for (int i = threadIdx.x; i < kPickChunk && c0 + i < total; i += kPickThreads) {
-      const long long c = c0 + i;
-      const int b = (int)(c / each), j = (int)(c - b * each);
-      const float score = a.scores[(long long)batch * a.beams + b];
-      const double lse = s.lse[b];
-      unsigned long long p = a.kept[(long long)batch * total + c];
-      double v = -INFINITY;
-      int token = ~(int)(uint32_t)p;
-      if (!(fabs(lse) < INFINITY) || !(score < INFINITY) || score == -INFINITY) {
-        // a beam that offers nothing: of its tokens, all -inf, the first ones
-        if (j >= a.count || j >= a.vocab) continue;
-        token = j;
-      } else {
-        if (!p) continue;
-        v = (double)score + ((double)unrank((uint32_t)(p >> 32)) - lse);
+#pragma unroll
+    for (int i = 0; i < kPickEach; ++i) {
+      const long long c = c0 + i * kPickThreads + threadIdx.x;
+      bool take = c < total;
+      unsigned long long key = 0, place = 0;
+      if (take) {
+        const int b = (int)(c >> 32 ? c / each : (uint32_t)c / (uint32_t)each), j = (int)(c - (long long)b * each);
+        const float score = a.scores[row0 + b];
+        const double lse = s.lse[b];
+        const unsigned long long p = kept[i];
+        double v = -INFINITY;
+        int token = ~(int)(uint32_t)p;
+        if (!(fabs(lse) < INFINITY) || !(score < INFINITY) || score == -INFINITY) {
+          // a beam that offers nothing: of its tokens, all -inf, the first ones
+          take = j < a.count && j < a.vocab;
+          token = j;
+        } else {
+          take = p != 0;
+          v = (double)score + ((double)unrank((uint32_t)(p >> 32)) - lse);
+        }
+        key = rank_key64(v);
+        place = ~((unsigned long long)b * a.vocab + token);
+        take = take && key >= least;
       }
-      const unsigned long long key = rank_key64(v);
-      if (key < least) continue;
-      const int at = atomicAdd(&s.n, 1);
-      s.value[at] = key;
-      s.place[at] = ~((unsigned long long)b * a.vocab + token);
+      const int at = place_of(take, &s.n);
+      if (take) s.value[at] = key, s.place[at] = place;
     }
+    if (c0 + kPickChunk < total) fetch(c0 + kPickChunk);
     __syncthreads();
     const int n = s.n;
-    if (n > a.count) {
+    const bool last = c0 + kPickChunk >= total;
+    if (n > (last ? few : a.count)) {  // a few are ranked as they are
       unsigned long long value[E], place[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -275,21 +363,21 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
         value[j] = i < n ? s.value[i] : 0;
         place[j] = i < n ? s.place[i] : 0;
       }
-      least = bound_of(a.count, least, ~0ull - 1, count, [&](unsigned long long t) {
+      least = bound_of(a.count, last ? few : a.count, least, ~0ull - 1, count, [&](unsigned long long t) {
         int k = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) k += value[j] >= t;
         return k;
       });
-      // of equal values at the bound, those of the lowest places
+      // of equal values at the bound, where they are many, those of the lowest places
       int above = 0, reach = 0;
 #pragma unroll
       for (int j = 0; j < E; ++j) above += value[j] > least, reach += value[j] >= least;
       above = count(above);
       reach = count(reach);
       unsigned long long first = 0;
-      if (reach > a.count)
-        first = bound_of(a.count - above, 0, ~0ull - 1, count, [&](unsigned long long t) {
+      if (above < a.count && reach > (last ? few : a.count))
+        first = bound_of(a.count - above, a.count - above, 0, ~0ull - 1, count, [&](unsigned long long t) {
           int k = 0;
 #pragma unroll
           for (int j = 0; j < E; ++j) k += value[j] == least && place[j] >= t;
@@ -299,30 +387,36 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
       if (threadIdx.x == 0) s.n = 0;
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (value[j] > least || (value[j] == least && value[j] && place[j] >= first)) {
-          const int at = atomicAdd(&s.n, 1);
-          s.value[at] = value[j];
-          s.place[at] = place[j];
-        }
+      for (int j = 0; j < E; ++j) {
+        const bool take = value[j] > least || (value[j] == least && value[j] && place[j] >= first);
+        const int at = place_of(take, &s.n);
+        if (take) s.value[at] = value[j], s.place[at] = place[j];
+      }
     }
     __syncthreads();
   }
-  // the chosen, each to its rank
+  // the best of them, each to its rank
   const int n = s.n;
   for (int i = threadIdx.x; i < n; i += kPickThreads) {
     const unsigned long long v = s.value[i], p = s.place[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s.value[j] > v || (s.value[j] == v && s.place[j] > p);
-    const long long out = (long long)batch * a.count + rank, at = (long long)~p;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const unsigned long long u = s.value[j];
+      rank += u > v || (u == v && s.place[j] > p);
+    }
+    if (rank >= a.count) continue;
+    const long long out = (long long)batch * a.count + rank;
+    const unsigned long long at = ~p;
+    const int b = (int)(at >> 32 ? at / (unsigned)a.vocab : (uint32_t)at / (uint32_t)a.vocab);
     a.scores_out[out] = (float)unrank64(v);
-    a.beams_out[out] = (int)(at / a.vocab);
-    a.tokens_out[out] = (int)(at % a.vocab);
+    a.beams_out[out] = b;
+    a.tokens_out[out] = (int)(at - (unsigned long long)b * a.vocab);
   }
 }
 
 struct BeamLayout {
-  int parts, part;
+  int parts, part, keep;
   size_t sums, maxima, kept, bytes;
 };
 
@@ -344,7 +438,8 @@ BeamLayout beam_layout(int rows, int vocab, int count, int sms) {
   const size_t n = (size_t)rows * L.parts;
   L.sums = take(n * 8);
   L.maxima = take(n * 4);
-  L.kept = take(n * count * 8);
+  L.keep = 2 * count;
+  L.kept = take(n * L.keep * 8);
   L.bytes = at;
   return L;
 }
@@ -389,7 +484,7 @@ extern "C" int er_beam_select(const void* logits, int dtype, long long row_strid
   if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_beam_select: workspace must be 256-byte aligned");
   char* ws = (char*)workspace;
   BeamArgs a = {logits, row_stride, scores, batch, beams, vocab, count, L.parts, L.part, (double*)(ws + L.sums),
-                (float*)(ws + L.maxima), (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
+                (float*)(ws + L.maxima), L.keep, (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(L.parts, rows);
   int rc = dtype == ER_DTYPE_BF16
