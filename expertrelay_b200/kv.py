@@ -171,7 +171,7 @@ class PagedKV:
 
     def check(self) -> None:
         """Raises ValueError if a call since the last check met a bad page id,
-        length or sequence on the device. Waits for the stream's work."""
+        length, sequence or tree on the device. Waits for the stream's work."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
@@ -179,6 +179,8 @@ class PagedKV:
                                    (_lib.KV_BAD_LENGTH, "a length, position or count outside its table"),
                                    (_lib.KV_BAD_SEQ, "a sequence outside the table"),
                                    (_lib.KV_BAD_TREE, "a tree's rows or parents out of order")) if bits & b]
+            if bits & _lib.KV_GAVE_UP:
+                raise RuntimeError(", ".join(["paged cache: attend_tree gave up waiting, its results are no good", *what]))
             raise ValueError("paged cache: " + ", ".join(what))
 
 

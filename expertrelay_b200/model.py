@@ -18,7 +18,9 @@ cache, as in the reference.
 
 With a PagedKVCache in place of a KVCache, the keys and values of many
 sequences lie in pages (fp32 or bf16): one call may carry tokens of several
-sequences, and attention runs over the pages (expertrelay_b200.kv).
+sequences, or trees of drafted tokens, and attention runs over the pages
+(expertrelay_b200.kv). On it stand generate_drafted (several tokens a call,
+where a draft has guessed them) and beam_search.
 """
 
 from __future__ import annotations
@@ -29,7 +31,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, beam, draft as drafts
 from .cache import HbmExpertCache, HostRecords
 from .kv_cache import PagedKVCache
 from .paged import PagedMoeStack
@@ -190,11 +192,14 @@ class QwenMoeModel:
         return self._linear(out, w["o_proj"])
 
     def forward(self, token_ids, kv: KVCache | PagedKVCache, *, all_logits: bool = False, expert_trace=None,
-                seqs=None) -> torch.Tensor:
+                seqs=None, parents=None) -> torch.Tensor:
         """Run `token_ids` after what `kv` holds; logits [vocab] of the last
         position (or [n, vocab] with all_logits), on the device. With a
         PagedKVCache, `seqs` names the sequence of every token (default: all
-        of sequence 0), and a call that raises leaves it as it was."""
+        of sequence 0), and a call that raises leaves it as it was. `parents`
+        makes the tokens trees of drafted ones (PagedKVCache.step): each sees
+        its sequence, its ancestors and itself; kv.drafted is then the step
+        that kv.accept needs."""
         c = self.c
         ids = torch.as_tensor(np.asarray(token_ids, dtype=np.int64)).to(self.device)
         n = ids.shape[0]
@@ -204,15 +209,17 @@ class QwenMoeModel:
                 raise ValueError(f"seqs: one sequence for each of {n} tokens, got {seqs.shape}")
             if expert_trace is not None and len(np.unique(seqs)) > 1:
                 raise ValueError("a trace follows one sequence")
-            step = kv.step(seqs)
+            if expert_trace is not None and parents is not None:
+                raise ValueError("a trace follows one text: not with parents")
+            step = kv.step(seqs, parents)
             try:
                 return self._forward(token_ids, ids, kv, step, int(kv.pages.position[seqs[0]]) - n, all_logits,
                                      expert_trace)
             except BaseException:  # the places of a call that fails hold nothing, or not in every layer
                 kv.undo(step)
                 raise
-        if seqs is not None:
-            raise ValueError("seqs: only with a PagedKVCache")
+        if seqs is not None or parents is not None:
+            raise ValueError("seqs, parents: only with a PagedKVCache")
         if kv.length + n > kv.max_seq:
             raise ValueError(f"sequence length {kv.length + n} exceeds the KV cache ({kv.max_seq})")
         # causal: query start + i sees keys 0 .. start + i (the same for every layer)
@@ -272,3 +279,74 @@ class QwenMoeModel:
             step.append(time.perf_counter() - t1)
             out.append(tok)
         return out, t_prompt, step
+
+    def generate_drafted(self, prompt, new_tokens: int, draft=drafts.from_text, *, kv: PagedKVCache | None = None,
+                         seq: int = 0):
+        """Greedy decoding, several tokens a call where `draft` has guessed them:
+        draft(text) gets the prompt and what has come so far and returns (tokens,
+        parents), a tree of guesses at what comes next (kv.attend_tree's order; -1:
+        the text's last token; none is fine). One call runs them all, and the
+        path that greedy decoding would have taken stays. Returns (generated ids,
+        calls after the prompt's). kv: a cache of one's own, its sequence `seq`
+        empty (room for the prompt, new_tokens and a call's guesses)."""
+        prompt = [int(t) for t in prompt]
+        if new_tokens < 1:
+            raise ValueError(f"new_tokens: at least 1, got {new_tokens}")
+        if kv is None:
+            kv, seq = self.new_paged_cache(1, len(prompt) + new_tokens + 256), 0
+        out, calls = [int(torch.argmax(self.forward(prompt, kv, seqs=[seq] * len(prompt))).item())], 0
+        while len(out) < new_tokens:
+            tokens, parents = draft(prompt + out)
+            # the last token, its guesses behind it; no more than the cache takes, a child never before its parent
+            most = min(256, max(1, kv.room(seq)))
+            tokens = [out[-1], *map(int, tokens)][:most]
+            parents = [-1, *(int(p) + 1 for p in parents)][:most]
+            logits = self.forward(tokens, kv, all_logits=True, seqs=[seq] * len(tokens), parents=parents)
+            next_of = torch.argmax(logits, dim=1).tolist()
+            path, had = [0], len(out)
+            while len(out) < new_tokens:
+                out.append(next_of[path[-1]])
+                child = next((i for i in range(path[-1] + 1, len(tokens))
+                              if parents[i] == path[-1] and tokens[i] == out[-1]), None)
+                if child is None:
+                    break
+                path.append(child)
+            kv.accept(kv.drafted, [path[:len(out) - had]])  # like generate's, the cache ends before the last token
+            calls += 1
+        return out, calls
+
+    def beam_search(self, prompt, beams: int, new_tokens: int, *, end: int | None = None,
+                    kv: PagedKVCache | None = None) -> list[tuple[list[int], float]]:
+        """The `beams` best continuations of `prompt` by the sum of their tokens' log
+        probabilities that a search of that breadth finds, best first: [(ids, sum)].
+        They have new_tokens tokens, or end with `end`. kv: a cache of one's own
+        with sequences 0 .. beams - 1 empty, for their use."""
+        prompt = [int(t) for t in prompt]
+        if beams < 1 or new_tokens < 1:
+            raise ValueError(f"{beams} beams of {new_tokens} tokens: at least one each")
+        if kv is None:
+            kv = self.new_paged_cache(beams, len(prompt) + new_tokens)
+        kv.pages.known([beams - 1])
+        count = beams if end is None else 2 * beams  # as many that go on, whichever of them end
+        if count > 128:
+            raise ValueError(f"{beams} beams: at most {128 * beams // count}")
+        logits = self.forward(prompt, kv)[None]
+        scores, texts, done, live = torch.zeros((1, 1), device=self.device), [[]], [], [0]
+        for n in range(new_tokens):
+            best, of, tokens = beam.select(logits, scores, min(count, logits.numel()))
+            going = []
+            for value, i, t in zip(best[0].tolist(), of[0].tolist(), tokens[0].tolist()):
+                if t == end or n + 1 == new_tokens:
+                    done.append((texts[i] + [t], value))
+                elif len(going) < beams:
+                    going.append((value, i, t))
+            done = sorted(done, key=lambda d: -d[1])[:beams]
+            # sums only fall: nothing that goes on can pass what has ended
+            if not going or len(done) == beams and done[-1][1] >= going[0][0]:
+                break
+            kv.reorder(list(range(len(going))), [live[i] for _, i, _ in going])
+            live = list(range(len(going)))
+            texts = [texts[i] + [t] for _, i, t in going]
+            scores = torch.tensor([[value for value, _, _ in going]], device=self.device)
+            logits = self.forward([t for _, _, t in going], kv, all_logits=True, seqs=live)
+        return done
