@@ -6,7 +6,7 @@ from __future__ import annotations
 import numpy as np
 import pytest
 import torch
-from kv_ref import make_cache
+from kv_ref import U, attend_exact, make_cache, result_bound, result_error
 from tree_ref import check_trees
 
 from expertrelay_b200 import kv
@@ -216,7 +216,8 @@ def test_refusals(cuda):
     for change, words in (({"lens": ln.long()}, "lens"), ({"lens": _i32([1, 2])}, "lens"), ({"starts": starts[:0]}, "starts"),
                           ({"starts": starts.float()}, "starts"), ({"starts": None}, "starts"), ({"parents": parents[:1]}, "parents"),
                           ({"q": q.half()}, "q:"), ({"q": q[:, :3]}, "heads"), ({"seqs": starts}, "seqs"),
-                          ({"out": q[:1].clone()}, "out")):
+                          ({"out": q[:1].clone()}, "out"),
+                          ({"workspace": torch.empty(0, dtype=torch.uint8, device="cuda")}, "workspace")):
         args = {"q": q, "lens": ln, "starts": starts, "parents": parents, **change}
         with pytest.raises(ValueError, match=words):
             kv.attend_tree(cache, args.pop("q"), args.pop("lens"), args.pop("starts"), args.pop("parents"), **args)
@@ -224,3 +225,92 @@ def test_refusals(cuda):
         kv.attend_tree(cache, q, _i32([1, 1]), _i32([0, 1, 2]), parents)
     assert kv.attend_tree(cache, q, ln[:0], starts[:1], parents).shape == q.shape
     assert kv.attend_tree(cache, q[:0], _i32([0]), _i32([0, 0]), parents[:0]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_one_sequence_in_two_trees(cuda, cache_dtype, q_dtype):
+    """Two trees over the same places, among others, and the same pages under other sequences: as each alone."""
+    rng = np.random.default_rng(6)
+    lens, trees = [150, 90], [_tree(rng, 6), _tree(rng, 6)]
+    cache, q, _, _, parents = _case(6, lens, trees, 2, 2, 64, 16, cache_dtype, q_dtype)
+    two = kv.PagedKV(cache.k, cache.v, torch.cat([cache.table, cache.table[:1]]))
+    q3 = torch.cat([q[:6], q[6:], q[:6] * 0.5, q[:6]])
+    p3 = torch.cat([parents[:6], parents[6:], parents[:6], parents[:6]])
+    lens4, seqs = [150, 90, 150, 150], [0, 1, 0, 2]
+    out = kv.attend_tree(two, q3, _i32(lens4), _i32([0, 6, 12, 18, 24]), p3, seqs=_i32(seqs))
+    check_trees(two, q3, lens4, [trees[0], trees[1], trees[0], trees[0]], out, seqs=seqs)
+    assert torch.equal(out[:6], out[18:])
+    cache.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 2.0])
+def test_scales(cuda, cache_dtype, q_dtype, scale):
+    rng = np.random.default_rng(8)
+    lens, trees = [100, 3], [_tree(rng, 9), _tree(rng, 2)]
+    cache, q, ln, starts, parents = _case(8, lens, trees, 2, 3, 72, 16, cache_dtype, q_dtype)
+    check_trees(cache, q, lens, trees, kv.attend_tree(cache, q, ln, starts, parents, scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize("off", [1, 2, 4])
+def test_queries_off_16_bytes(cuda, cache_dtype, q_dtype, off):
+    """Rows at odd strides and addresses: only out and the cache have to lie on 16 bytes."""
+    rng = np.random.default_rng(off)
+    lens, trees = [70, 33], [_tree(rng, 7), _tree(rng, 12)]
+    cache, q, ln, starts, parents = _case(off, lens, trees, 2, 2, 64, 16, cache_dtype, q_dtype)
+    flat = torch.zeros(19 * 259 + off, dtype=q_dtype, device="cuda")
+    odd = flat[off:].view(19, 259)[:, :256]
+    odd.copy_(q.reshape(19, 256))
+    out = kv.attend_tree(cache, odd.view(19, 4, 64), ln, starts, parents)
+    assert torch.equal(out, kv.attend_tree(cache, q, ln, starts, parents))
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+def test_a_chain_is_a_piece_of_a_text(cuda, cache_dtype, q_dtype):
+    """attend over the same places, row by row: two kernels, each within its rounding of the definition."""
+    lens, trees = [517], [_tree(None, 100, "chain")]
+    cache, q, ln, starts, parents = _case(12, lens, trees, 2, 4, 128, 16, cache_dtype, q_dtype)
+    got = kv.attend_tree(cache, q, ln, starts, parents).double()
+    want = kv.attend(cache, q, _i32([518 + i for i in range(100)]), seqs=_i32([0] * 100)).double()
+    # a step of the results' type, where both round, or a few of 32 bits' of the row's greatest
+    step = torch.finfo(q_dtype).eps if q_dtype == BF16 else 2.0 ** -18
+    assert torch.all((got - want).abs() <= step * want.abs().amax(-1, keepdim=True))
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("kv_heads", "group", "n", "d", "nodes"), [
+    (4, 4, 1008, 64, 16), (4, 2, 1008, 128, 60), (2, 3, 2000, 256, 20), (1, 1, 4800, 128, 1), (2, 16, 480, 96, 9), (4, 1, 20000, 64, 4),
+])
+@pytest.mark.parametrize("size", [1.0, 0.02])
+def test_trees_are_as_exact_as_32_bits(cuda, cache_dtype, q_dtype, kv_heads, group, n, d, nodes, size):
+    """size: the spread of the scores. result_bound counts d / 8 products for a score and two sums over 16 keys; here
+    they are d / 16 and 64 / 16, for each pair of the operands' parts that is multiplied: 1 and 2 of bf16 queries over a
+    bf16 cache, 3 and 3 of fp32 ones, 6 and 6 over an fp32 cache. Each cuts up to U of a sum that grows as it is
+    added up: half of that. Weights in two parts, where the result has 8 bits, lack 2^-18 at the most."""
+    score, value = (6, 6) if cache_dtype == F32 else (3, 3) if q_dtype == F32 else (1, 2)
+    bound = result_bound(d, n, size) + (score * d / 32 * size + value * 4 / 2) * U
+    if cache_dtype == q_dtype == BF16:
+        bound += 2.0 ** -18
+    gen = torch.Generator(device="cuda").manual_seed(n + d)
+    trees = max(1, min(64, 3000000 // (n * d)))
+    each = -(-(n + nodes) // 16)
+    k, v = (torch.randn((trees * each, kv_heads, 16, d), generator=gen, device="cuda").to(cache_dtype) for _ in range(2))
+    table = torch.randperm(trees * each, generator=gen, device="cuda").to(torch.int32).view(trees, each)
+    cache = kv.PagedKV(k, v, table)
+    seen = [x[table.long()].transpose(1, 2).reshape(trees, kv_heads, each * 16, d) for x in (k, v)]
+    calls = 1 if q_dtype == F32 else max(1, min(40, 400000 // (trees * nodes * kv_heads * group * d)))
+    outs, wants = [], []
+    for _ in range(calls):
+        q = torch.randn((trees * nodes, kv_heads * group, d), generator=gen, device="cuda").to(q_dtype)
+        starts = torch.arange(trees + 1, dtype=torch.int32, device="cuda") * nodes
+        outs.append(kv.attend_tree(cache, q, _i32([n] * trees), starts, _i32([-1] * (trees * nodes)), scale=size * d ** -0.5))
+        of = q.view(trees, nodes, kv_heads, group, d)
+        want = torch.empty(of.shape, dtype=torch.float64, device="cuda")
+        for i in range(nodes):  # the context and the node's own place
+            kk, vv = (torch.cat([x[:, :, :n], x[:, :, n + i:n + i + 1]], 2) for x in seen)
+            want[:, i] = attend_exact(of[:, i], kk, vv, size * d ** -0.5)
+        wants.append(want.view(q.shape))
+    got = result_error(torch.stack(outs), torch.stack(wants), q_dtype)
+    assert got <= bound, f"{got:.3g} of the result, {bound:.3g} allowed"
+    cache.check()
