@@ -10,6 +10,7 @@
 // their beams' log-sums, whose rounding in 32 bits would decide close ones.
 // 4 bytes a candidate and about a dozen instructions: memory bounds it.
 #include "er_kv.cuh"
+#include "er_ptx.cuh"
 
 namespace er {
 
@@ -17,7 +18,7 @@ namespace {
 
 constexpr int kScanThreads = 256, kEach = 16, kTile = kScanThreads * kEach;  // logits a tile
 constexpr int kMaxCount = 128, kMaxBeams = 1024;
-constexpr int kMaxKeep = 2 * kMaxCount, kHeld = kTile + kMaxKeep;  // what a CTA may hold before it has to choose
+constexpr int kHeld = kTile + kScanThreads;  // what a CTA may hold before it has to choose
 
 struct BeamArgs {
   const void* logits;
@@ -27,8 +28,7 @@ struct BeamArgs {
   int parts, part;  // of a row, and logits of each (a multiple of the tile)
   double* sums;     // [rows][parts] of 2^.. relative to maxima
   float* maxima;    // [rows][parts]
-  int keep;                  // of a part, at most: count at the least where there are as many
-  unsigned long long* kept;  // [rows][parts][keep]: rank key of the logit, then ~token; 0 behind the last
+  unsigned long long* kept;  // [rows][parts][count]: rank key of the logit, then ~token; 0 behind the last
   float* scores_out;
   int32_t *beams_out, *tokens_out;
 };
@@ -129,11 +129,7 @@ struct Logits {
 };
 
 // e^x for x <= 0 in 32 bits: within 2^-22 and |x| 2^-25 of it
-__device__ __forceinline__ float exp_below(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
-  return y;
-}
+__device__ __forceinline__ float exp_below(float x) { return ex2(x * 1.44269504f); }
 
 // Of every logit: a maximum, a subtraction, a product, an exponential and a sum; whether it can be among the best is
 // asked of a thread's greatest, and only a thread that has one looks again. Sums of 16 go to 64 bits.
@@ -156,14 +152,14 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   float m = -INFINITY;
   double sum = 0.0;
   unsigned long long bound = 0;  // what has to be reached to be held
-  float least = -INFINITY;       // its logit (NaN where it has none: everything may)
+  float least = -INFINITY;       // its logit (what is not below it may be held)
   int most_held = 0;             // the same in all threads, and no less than is held
-  // the best of what is held, a.count to a.keep of them, moved to its front
+  // the best of what is held, a.count to kScanThreads of them, moved to its front
   auto choose = [&]() {
     __syncthreads();
     const int n = held_n;
-    if (n <= a.keep) return;
-    bound = bound_of(a.count, a.keep, bound, ~0ull - 1, count, [&](unsigned long long t) {
+    if (n <= kScanThreads) return;
+    bound = bound_of(a.count, kScanThreads, bound, ~0ull - 1, count, [&](unsigned long long t) {
       int c = 0;
       for (int i = threadIdx.x; i < n; i += kScanThreads) c += held[i] >= t;
       return c;
@@ -182,7 +178,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     }
   };
 #pragma unroll 1
-  for (int i0 = begin; i0 < end; i0 += kTile) {
+  for (int tile = 0; begin + tile * kTile < end; ++tile) {
+    const int i0 = begin + tile * kTile;
     float x[kEach];
     next.floats(x);
     if (i0 + kTile < end) next.load(logits, i0 + kTile, end, wide);
@@ -195,15 +192,21 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     }
     // a thread whose logits are all -inf, or NaN among them, so far: its sum stays 0, or becomes NaN
     const float ref = m == -INFINITY ? 0.f : m;
-    float part[4];
+    const uint64_t off = pack2(-ref, -ref), unit = pack2(1.44269504f, 1.44269504f);
+    uint64_t part[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      part[j] = (exp_below(x[j] - ref) + exp_below(x[j + 4] - ref)) + (exp_below(x[j + 8] - ref) + exp_below(x[j + 12] - ref));
-    sum += (double)((part[0] + part[1]) + (part[2] + part[3]));
-    if (i0 == begin) {
-      // as many of each warp's threads as make a.count of the block's: what their greatest logits reach, at least
-      // a.count do
-      uint32_t key = begin + Logits<T>::at(0) < end ? rank_key(top) : 0u, r = 0;
+    for (int j = 0; j < kEach; j += 2) {
+      float u, v;  // e^(x - m): within 2^-22 and |x - m| 2^-25 of it
+      unpack2(fma2(add2(pack2(x[j], x[j + 1]), off), unit, 0), u, v);
+      part[j / 2 & 1] = add2(part[j / 2 & 1], pack2(ex2(u), ex2(v)));
+    }
+    float even, odd;
+    unpack2(add2(part[0], part[1]), even, odd);
+    sum += (double)(even + odd);
+    if ((tile & (tile - 1)) == 0) {
+      // A bound from the threads' greatest so far, renewed as the tiles double: as many of each warp's as make a.count
+      // of the block's reach the least of what the warps' do.
+      uint32_t key = begin + Logits<T>::at(0) < end ? rank_key(m) : 0u, r = 0;
       for (int k = 0; k < a.count; k += kScanThreads / 32) {
         r = __reduce_max_sync(0xffffffffu, key);
         const uint32_t who = __ballot_sync(0xffffffffu, key == r);
@@ -213,8 +216,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
       __syncthreads();
       r = warp_least[0];
       for (int w = 1; w < kScanThreads / 32; ++w) r = min(r, warp_least[w]);
-      bound = (unsigned long long)r << 32;
-      least = unrank(r);
+      const unsigned long long now = (unsigned long long)r << 32;
+      if (now > bound) bound = now, least = unrank(r);
     }
     bool look = !(top < least);
     const int lookers = __syncthreads_count(look) * kEach;  // what was held before is there, too
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
       __syncthreads();
       if (most_held + lookers > kHeld) {
         choose();
-        most_held = a.keep;
+        most_held = kScanThreads;
         look = !(top < least);
       }
     }
@@ -232,19 +235,26 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
       uint32_t which = 0;
 #pragma unroll
       for (int j = 0; j < kEach; ++j) which |= (uint32_t)!(x[j] < least) << j;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        const int i = i0 + Logits<T>::at(j);
-        if (!(which >> j & 1) || i >= end) continue;
-        const unsigned long long p = pack(x[j], i);
+      for (; which; which &= which - 1) {  // few: read again
+        const int i = i0 + Logits<T>::at(__ffs(which) - 1);
+        if (i >= end) continue;
+        const unsigned long long p = pack((float)logits[i], i);
         if (p >= bound) held[atomicAdd(&held_n, 1)] = p;
       }
     }
   }
   choose();
-  __syncthreads();
-  unsigned long long* kept = a.kept + ((long long)row * a.parts + blockIdx.x) * a.keep;
-  for (int i = threadIdx.x; i < a.keep; i += kScanThreads) kept[i] = i < held_n ? held[i] : 0;
+  // the best of them, a thread each, to its rank (no two keys are alike)
+  unsigned long long* kept = a.kept + ((long long)row * a.parts + blockIdx.x) * a.count;
+  const int n = held_n;
+  const unsigned long long mine = (int)threadIdx.x < n ? held[threadIdx.x] : 0;
+  if (__any_sync(0xffffffffu, mine && mine >= bound)) {
+    int rank = mine && mine >= bound ? 0 : kHeld;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) rank += held[i] > mine;
+    if (rank < a.count) kept[rank] = mine;
+  }
+  if ((int)threadIdx.x >= n && (int)threadIdx.x < a.count) kept[threadIdx.x] = 0;
   // the threads' sums, in an order that does not change
   float top = m;
 #pragma unroll
@@ -265,7 +275,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
 }
 
 // ---- the choice over a batch's beams
-constexpr int kPickThreads = 512, kPickEach = 4, kPickChunk = kPickThreads * kPickEach, kFew = 512;
+constexpr int kPickThreads = 512, kPickEach = 4, kPickChunk = kPickThreads * kPickEach, kFew = 128;
 
 // the order of doubles as unsigned integers (no NaN comes here; the zeros alike)
 __device__ __forceinline__ unsigned long long rank_key64(double v) {
@@ -280,6 +290,7 @@ struct PickShared {
   unsigned long long value[kPickChunk + kMaxCount], place[kPickChunk + kMaxCount];  // place: ~(beam * vocab + token)
   double lse[kMaxBeams];
   int red[64], n;
+  uint32_t warp_least[kPickThreads / 32];
 };
 
 // Grid: a CTA a batch. It goes over what was kept kPickChunk at a time: those that may be among the best join the best
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
   PickShared& s = *reinterpret_cast<PickShared*>(smem);
   kv_enter();
   const int batch = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = a.parts * a.keep;  // of a beam
+  const int each = a.parts * a.count;  // of a beam
   const long long total = (long long)each * a.beams;
   unsigned long long kept[kPickEach];
   auto fetch = [&](long long c0) {
@@ -312,23 +323,37 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
     double sum = 0.0;
     for (int p = lane; p < a.parts; p += 32) {
       const float m = a.maxima[at + p];
-      sum += m == -INFINITY ? a.sums[at + p] : a.sums[at + p] * exp((double)m - (double)top);
+      sum += m == -INFINITY ? a.sums[at + p] : a.sums[at + p] * (double)exp_below(m - top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s.lse[b] = (double)top + log(sum);
   }
   __syncthreads();
-  const int few = min(kFew, 2 * a.count + 32);
+  // Of the threads' greatest values (their upper words), as many of each warp's as make a.count of the block's reach the
+  // least of what the warps' do.
+  auto bound_above = [&](uint32_t key) {
+    uint32_t r = 0;
+    for (int k = 0; k < a.count; k += kPickThreads / 32) {
+      r = __reduce_max_sync(0xffffffffu, key);
+      const uint32_t who = __ballot_sync(0xffffffffu, key == r);
+      if (lane == __ffs(who) - 1) key = 0;
+    }
+    if (lane == 0) s.warp_least[warp] = r;
+    __syncthreads();
+    return (unsigned long long)__reduce_min_sync(0xffffffffu, s.warp_least[lane & (kPickThreads / 32 - 1)]) << 32;
+  };
   unsigned long long least = 0;  // a value that a.count of what is held reach
   constexpr int E = kPickEach + 1;
 #pragma unroll 1
   for (long long c0 = 0; c0 < total; c0 += kPickChunk) {
+    unsigned long long key[kPickEach], place[kPickEach];
+    uint32_t best = 0;
 #pragma unroll
     for (int i = 0; i < kPickEach; ++i) {
       const long long c = c0 + i * kPickThreads + threadIdx.x;
       bool take = c < total;
-      unsigned long long key = 0, place = 0;
+      place[i] = key[i] = 0;
       if (take) {
         const int b = (int)(c >> 32 ? c / each : (uint32_t)c / (uint32_t)each), j = (int)(c - (long long)b * each);
         const float score = a.scores[row0 + b];
@@ -344,18 +369,23 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
           take = p != 0;
           v = (double)score + ((double)unrank((uint32_t)(p >> 32)) - lse);
         }
-        key = rank_key64(v);
-        place = ~((unsigned long long)b * a.vocab + token);
-        take = take && key >= least;
+        if (take) key[i] = rank_key64(v);
+        place[i] = ~((unsigned long long)b * a.vocab + token);
       }
+      best = max(best, (uint32_t)(key[i] >> 32));
+    }
+    least = max(least, bound_above(best));
+#pragma unroll
+    for (int i = 0; i < kPickEach; ++i) {
+      const bool take = key[i] && key[i] >= least;
       const int at = place_of(take, &s.n);
-      if (take) s.value[at] = key, s.place[at] = place;
+      if (take) s.value[at] = key[i], s.place[at] = place[i];
     }
     if (c0 + kPickChunk < total) fetch(c0 + kPickChunk);
     __syncthreads();
     const int n = s.n;
-    const bool last = c0 + kPickChunk >= total;
-    if (n > (last ? few : a.count)) {  // a few are ranked as they are
+    const int enough = c0 + kPickChunk < total ? a.count : a.count + kFew;
+    if (n > enough) {  // a few are ranked as they are
       unsigned long long value[E], place[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -363,12 +393,13 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
         value[j] = i < n ? s.value[i] : 0;
         place[j] = i < n ? s.place[i] : 0;
       }
-      least = bound_of(a.count, last ? few : a.count, least, ~0ull - 1, count, [&](unsigned long long t) {
+      auto reaching = [&](unsigned long long t) {
         int k = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) k += value[j] >= t;
         return k;
-      });
+      };
+      least = bound_of(a.count, enough, least, ~0ull - 1, count, reaching);
       // of equal values at the bound, where they are many, those of the lowest places
       int above = 0, reach = 0;
 #pragma unroll
@@ -376,7 +407,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
       above = count(above);
       reach = count(reach);
       unsigned long long first = 0;
-      if (above < a.count && reach > (last ? few : a.count))
+      if (above < a.count && reach > enough)
         first = bound_of(a.count - above, a.count - above, 0, ~0ull - 1, count, [&](unsigned long long t) {
           int k = 0;
 #pragma unroll
@@ -397,15 +428,16 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
   }
   // the best of them, each to its rank
   const int n = s.n;
-  for (int i = threadIdx.x; i < n; i += kPickThreads) {
+  for (int i = warp; i < n; i += kPickThreads / 32) {
     const unsigned long long v = s.value[i], p = s.place[i];
     int rank = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
+    for (int j = lane; j < n; j += 32) {
       const unsigned long long u = s.value[j];
       rank += u > v || (u == v && s.place[j] > p);
     }
-    if (rank >= a.count) continue;
+    rank = __reduce_add_sync(0xffffffffu, rank);
+    if (rank >= a.count || lane) continue;
     const long long out = (long long)batch * a.count + rank;
     const unsigned long long at = ~p;
     const int b = (int)(at >> 32 ? at / (unsigned)a.vocab : (uint32_t)at / (uint32_t)a.vocab);
@@ -416,7 +448,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
 }
 
 struct BeamLayout {
-  int parts, part, keep;
+  int parts, part;
   size_t sums, maxima, kept, bytes;
 };
 
@@ -438,8 +470,7 @@ BeamLayout beam_layout(int rows, int vocab, int count, int sms) {
   const size_t n = (size_t)rows * L.parts;
   L.sums = take(n * 8);
   L.maxima = take(n * 4);
-  L.keep = 2 * count;
-  L.kept = take(n * L.keep * 8);
+  L.kept = take(n * count * 8);
   L.bytes = at;
   return L;
 }
@@ -484,7 +515,7 @@ extern "C" int er_beam_select(const void* logits, int dtype, long long row_strid
   if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_beam_select: workspace must be 256-byte aligned");
   char* ws = (char*)workspace;
   BeamArgs a = {logits, row_stride, scores, batch, beams, vocab, count, L.parts, L.part, (double*)(ws + L.sums),
-                (float*)(ws + L.maxima), L.keep, (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
+                (float*)(ws + L.maxima), (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(L.parts, rows);
   int rc = dtype == ER_DTYPE_BF16

@@ -192,23 +192,6 @@ __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
-// Two floats at a time: the arithmetic of the weights is bound by instructions.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // two floats rounded to bf16, packed, the first one low
 __device__ __forceinline__ uint32_t round2(uint64_t v) {
   float x, y;
@@ -274,11 +257,6 @@ __device__ __forceinline__ uint32_t seen_from(const uint32_t* sees, int node0) {
   return __funnelshift_r(w < 8 ? sees[w] : 0u, w < 7 ? sees[w + 1] : 0u, node0 & 31);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // (issued by the lane whose `go` is not zero)
 __device__ __forceinline__ void tma_box(uint32_t go, uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int slot,
                                         int head, int page) {
