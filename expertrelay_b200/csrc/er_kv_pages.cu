@@ -88,28 +88,49 @@ struct CompactArgs {
   const int32_t *seqs, *start, *keep, *counts;
   int rows, most;    // most: entries of a row's list
   long long keep_stride;
-  int heads;         // of one CTA
+  int heads, cuts;   // of one CTA: key heads, or one of so many parts of a head's channels
   int32_t* lens_out;
   int* status;
 };
 
-// Grid (blocks of key heads, 2 layers, rows). Place start + keep[j] goes to
-// start + j. keep ascends, so keep[j] >= j: what is written at j is read only
-// for entries up to j, and a CTA that takes the list in order, loading a batch
-// before it stores it, needs no second copy. Batches cannot be shared between
-// CTAs that way, so a CTA takes as few columns as keep its threads busy.
-constexpr int kBatchRows = 512;
+// Grid (columns, 2 layers, rows). Place start + keep[j] goes to start + j. keep
+// ascends, so keep[j] >= j: what is written at j is read only for entries up to
+// j, and a CTA that takes the list in order, loading a batch before it stores
+// it, needs no second copy. Batches cannot be shared between CTAs that way, so
+// a CTA takes as few columns as keep its threads busy: several key heads of a
+// short list, 128 bytes of one head of a long one (twelve lists of up to 1501
+// places, 490 MB in all: 114 us, with whole heads 125, with 64 bytes 118). DRAM
+// bounds it; the last CTAs are those of the shortest lists (104 us, 4.7 TB/s:
+// before and behind a batch's barrier only loads or only stores are under way).
+// An accepted draft's 5 places in 24 layers: 5.4 us, latency.
+constexpr int kBatchRows = 512, kCut = 8;  // kCut: vectors of a place a CTA has at least
 
 __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_constant__ CompactArgs a) {
   kv_enter();
   __shared__ long long from[2][kBatchRows], to[2][kBatchRows];
   const KvView& kv = a.l.kv;
-  const int layer = blockIdx.y >> 1, h0 = blockIdx.x * a.heads, heads = min(a.heads, kv.kv_heads - h0);
-  char* pool = (blockIdx.y & 1 ? kv.v : kv.k) + layer * a.l.layer_stride + h0 * kv.head_stride;
-  const int width = heads * a.l.row16;  // vectors of a place
+  const int layer = blockIdx.y >> 1, column = blockIdx.x / a.cuts, row16 = a.l.row16 / a.cuts;
+  const int h0 = column * a.heads, heads = min(a.heads, kv.kv_heads - h0);
+  char* pool = (blockIdx.y & 1 ? kv.v : kv.k) + layer * a.l.layer_stride + h0 * kv.head_stride +
+               (blockIdx.x - column * a.cuts) * row16 * 16;
+  const int width = heads * row16;  // vectors of a place
   const int batch = min(kBatchRows, kThreads * kMany / width);
+  int z = blockIdx.z;
+  if (a.rows > 1 && a.rows <= kThreads) {  // the longest lists first
+    __shared__ int all[kThreads], which;
+    const int mine = (int)threadIdx.x < a.rows ? a.counts[threadIdx.x] : 0;
+    all[threadIdx.x] = mine;
+    __syncthreads();
+    if ((int)threadIdx.x < a.rows) {
+      int rank = 0;
+      for (int i = 0; i < a.rows; ++i) rank += all[i] > mine || (all[i] == mine && i < (int)threadIdx.x);
+      if (rank == z) which = threadIdx.x;
+    }
+    __syncthreads();
+    z = which;
+  }
 #pragma unroll 1
-  for (int row = blockIdx.z; row < a.rows; row += gridDim.z) {
+  for (int row = z; row < a.rows; row += gridDim.z) {
     const int seq = a.seqs ? a.seqs[row] : row, start = a.start[row], n = a.counts[row];
     const int32_t* keep = a.keep + row * a.keep_stride;
     int bad = 0;
@@ -150,8 +171,8 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_const
       for (int u = 0; u < kMany; ++u) {
         const int i = threadIdx.x + u * kThreads;
         if (i >= total) continue;
-        const int r = i / width, c = i - r * width, h = c / a.l.row16;
-        v[u] = load16(pool + from[b][r] + h * kv.head_stride + (c - h * a.l.row16) * 16);
+        const int r = i / width, c = i - r * width, h = c / row16;
+        v[u] = load16(pool + from[b][r] + h * kv.head_stride + (c - h * row16) * 16);
       }
       if (j0 + batch < n) look(j0 + batch, b ^ 1);
       __syncthreads();  // all of the batch is read, and the next one's places are known
@@ -159,8 +180,8 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_const
       for (int u = 0; u < kMany; ++u) {
         const int i = threadIdx.x + u * kThreads;
         if (i >= total) continue;
-        const int r = i / width, c = i - r * width, h = c / a.l.row16;
-        store16(pool + to[b][r] + h * kv.head_stride + (c - h * a.l.row16) * 16, v[u]);
+        const int r = i / width, c = i - r * width, h = c / row16;
+        store16(pool + to[b][r] + h * kv.head_stride + (c - h * row16) * 16, v[u]);
       }
     }
     __syncthreads();  // the places of the last batch are used no more
@@ -216,7 +237,10 @@ extern "C" int er_kv_compact(const er_kv_cache* cache, int layers, long long lay
   const long long fill = (long long)kThreads * kMany / ((long long)(most ? most : 1) * a.l.row16);
   a.heads = fill < 1 ? 1 : fill > cache->kv_heads ? cache->kv_heads : (int)fill;
   if (a.heads > kThreads * kMany / a.l.row16) a.heads = kThreads * kMany / a.l.row16;
-  const int blocks = (cache->kv_heads + a.heads - 1) / a.heads;
+  a.cuts = 1;
+  if (fill < 1)
+    while (a.l.row16 % (2 * a.cuts) == 0 && a.l.row16 / (2 * a.cuts) >= kCut) a.cuts *= 2;
+  const int blocks = (cache->kv_heads + a.heads - 1) / a.heads * a.cuts;
   return kv_launch(kv_compact_kernel, dim3(blocks, 2 * layers, rows < 65535 ? rows : 65535), kThreads, 0, false,
                    (cudaStream_t)stream, "kv_compact_kernel", a);
 }
