@@ -22,7 +22,8 @@ struct TreeShape {
   static constexpr int kKPart = TK * DP * 2, kVPart = TK * VD * 2;  // bytes of one part of a tile
   static constexpr int kKSlot = kKPart * KP, kVSlot = kVPart * KP;
   static constexpr int kQPart = ROWS * DP * 2, kQ = kQPart * QP;
-  // columns of a tile's scores, then of its weights: by 64 keys, two parts over the scores, a third one behind them
+  static_assert(TK == 64, "weights' parts lie 32 columns apart");
+  // columns of a tile's scores, then of its weights: two parts over the scores, a third one behind them
   static constexpr int kSP = PP > 2 ? TK * 3 / 2 : TK;
   // tiles of scores (the products' warp issues them ahead), and results of a tile, kept while they are read
   static constexpr int SB = 3 * kSP + 2 * VD <= 512 ? 3 : 2, OB = SB * kSP + 2 * VD <= 512 ? 2 : 1;
@@ -42,8 +43,6 @@ struct TreeShape {
   // the warps that look at values of drafted keys
   static constexpr int kLookWarps = KP == 1 ? kSoftmaxWarps : kSplitWarps;
   static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
-  // the column of a tile's weights: part p of the 64 keys from 64 h on
-  static __device__ __forceinline__ constexpr int column(int h, int p) { return p < 2 ? h * 64 + p * 32 : TK + h * 32; }
 };
 
 template <typename S>
@@ -518,8 +517,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           if (spoils) l = __int_as_float(0x7fc00000);
         }
       };
-      // the weights of N scores, as they are multiplied: in parts, into column c of the 64 keys from 64 h on; their sum
-      auto weights = [&](auto& x, float shift, int h, int c) {
+      // the weights of N scores, as they are multiplied: in parts, from column c on; their sum
+      auto weights = [&](auto& x, float shift, int c) {
         constexpr int N = sizeof(x) / 4;
         const uint32_t sp = sp0 + sp_ring.at * S::kSP + c;
         const uint64_t scale = pack2(a.scale, a.scale), by = pack2(shift, shift);
@@ -542,7 +541,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
               y[j] = round2(p[j]);
               if (part + 1 < S::PP) p[j] = rest2(p[j], y[j]);
             }
-            tmem_st8(sp + S::column(h, part) + i, y);
+            tmem_st8(sp + part * 32 + i, y);
           }
         }
         float even, odd;
@@ -560,26 +559,15 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         return by;
       };
       auto tile = [&](auto replicas, int t) {
-        constexpr int RR = decltype(replicas)::value, KPT = TK / RR, N = KPT < 64 ? KPT : 64;
-        uint32_t x[N];
+        constexpr int RR = decltype(replicas)::value, KPT = TK / RR;
+        uint32_t x[KPT];
         float top = m, shift;
         const int key = slice * KPT;
         scores(x, t, key);
 #pragma unroll
-        for (int j = 0; j < N; ++j) top = fmaxf(top, __uint_as_float(x[j]));
-        if constexpr (KPT == 128) {  // the other half; then the first one's scores once more
-          scores(x, t, 64);
-#pragma unroll
-          for (int j = 0; j < N; ++j) top = fmaxf(top, __uint_as_float(x[j]));
-          const float by = rise(top, &shift);
-          float sum = weights(x, shift, 1, 0);
-          scores(x, t, 0);
-          sum += weights(x, shift, 0, 0);
-          l = l * by + sum;
-        } else {
-          const float by = rise(top, &shift);
-          l = l * by + weights(x, shift, key >> 6, (key & 63) / 2);
-        }
+        for (int j = 0; j < KPT; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+        const float by = rise(top, &shift);
+        l = l * by + weights(x, shift, key / 2);
         // the other keys are other replicas'
         const uint32_t zero[8] = {};
         const uint32_t sp = sp0 + sp_ring.at * S::kSP;
@@ -587,7 +575,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         for (int c = KPT / 2; c < TK / 2; c += 8) {
           const int at = (key / 2 + c) & (TK / 2 - 1);
 #pragma unroll
-          for (int part = 0; part < S::PP; ++part) tmem_st8(sp + S::column(at >> 5, part) + (at & 31), zero);
+          for (int part = 0; part < S::PP; ++part) tmem_st8(sp + part * 32 + at, zero);
         }
       };
       bool ok = true;
@@ -752,7 +740,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           if (kThree && pp + kp > 2) continue;
 #pragma unroll
           for (int k = 0; k < TK / 16; ++k)
-            mma_f16_ts(one, to, p + S::column(k >> 2, pp) + (k & 3) * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
+            mma_f16_ts(one, to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
                        !(pp == S::PP - 1 && kp == (kThree ? 2 - pp : 0) && k == 0));
         }
       commit_on(one, smem_u32(&s.ofull[b]));
@@ -951,7 +939,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   } else {
     // ---- the next unit's queries (bf16 caches), or keys and values split into parts (fp32 caches)
     const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kSplitWarps);
-    const int vecs = (d + 15) / 16 * 2;  // 16-byte vectors of a row of bf16, padded to whole products
     int unit = 0, it = 0, k_item = 0;
     Ring<KS> k_ring;
     Ring<VS> v_ring;
