@@ -7,9 +7,17 @@ the rows of a text's beams come together, and select picks the continuations.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib, kv
+
+
+@functools.lru_cache(maxsize=1024)
+def _bytes(device: int, *sizes: int) -> int:
+    """The workspace of a call of these sizes on a device (the current one)."""
+    return _lib.lib().er_beam_workspace_bytes(*sizes)
 
 
 def select(logits: torch.Tensor, scores: torch.Tensor, count: int, *,
@@ -44,11 +52,11 @@ def select(logits: torch.Tensor, scores: torch.Tensor, count: int, *,
             return select(logits, scores, count, workspace=workspace)
     lib = _lib.lib()
     best = scores.new_empty((batch, count))
-    which = torch.empty((2, batch, count), dtype=torch.int32, device=logits.device)
-    need = lib.er_beam_workspace_bytes(batch, beams, vocab, count)
+    beams_out, tokens_out = torch.empty((2, batch, count), dtype=torch.int32, device=logits.device).unbind(0)
+    need = _bytes(index, batch, beams, vocab, count)
     ws = kv._scratch(need, workspace, logits.device) if need else None
     _lib.check(lib.er_beam_select(logits.data_ptr(), kv._DTYPES[logits.dtype], logits.stride(0) if rows > 1 else vocab,
-                                  scores.data_ptr(), batch, beams, vocab, count, best.data_ptr(), which[0].data_ptr(),
-                                  which[1].data_ptr(), ws.data_ptr() if need else None, need,
+                                  scores.data_ptr(), batch, beams, vocab, count, best.data_ptr(), beams_out.data_ptr(),
+                                  tokens_out.data_ptr(), ws.data_ptr() if need else None, need,
                                   torch._C._cuda_getCurrentRawStream(index)), "er_beam_select")
-    return best, which[0], which[1]
+    return best, beams_out, tokens_out

@@ -193,8 +193,7 @@ class PagedLayers:
         if k.dim() != 5 or k.shape[0] == 0 or v.shape != k.shape or v.stride() != k.stride():
             raise ValueError(f"k, v: expected [layers, pages, kv_heads, page_size, head_dim] with strides alike, "
                              f"got {tuple(k.shape)} by {k.stride()}, {tuple(v.shape)} by {v.stride()}")
-        first = PagedKV(k[0], v[0], table, status)
-        self.layers = [first] + [PagedKV(k[i], v[i], table, first.status) for i in range(1, k.shape[0])]
+        first = self._first = PagedKV(k[0], v[0], table, status)
         self.k, self.v, self.table, self.status = k, v, table, first.status
         self.device, self.dtype, self.seqs, self.page_size = first.device, first.dtype, first.seqs, first.page_size
         self._index, self._ref, self._status = first._index, first._ref, first._status
@@ -204,9 +203,14 @@ class PagedLayers:
 
     _stream, _writable = PagedKV._stream, PagedKV._writable
 
+    @functools.cached_property
+    def layers(self) -> list[PagedKV]:
+        """Each layer's cache, all with this one's table and status (made when first asked for)."""
+        return [self._first] + [PagedKV(k, v, self.table, self.status) for k, v in zip(self.k[1:], self.v[1:])]
+
     def check(self) -> None:
         """PagedKV.check() of all layers."""
-        self.layers[0].check()
+        self._first.check()
 
 
 class PageBounds:
