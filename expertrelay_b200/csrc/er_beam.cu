@@ -8,7 +8,13 @@
 // exponentials; a second kernel joins the parts' sums and chooses among what
 // was kept, by values in 64 bits: candidates of different beams compare through
 // their beams' log-sums, whose rounding in 32 bits would decide close ones.
-// 4 bytes a candidate and about a dozen instructions: memory bounds it.
+// 2 or 4 bytes a candidate and about a dozen instructions: 256 rows of 151936
+// bf16 logits take 36 us (0.33 of the copy rate), the instructions and the
+// barrier of a tile; then the choice over 32 batches 12 us, a chain of
+// dependent steps in one CTA a batch, most of it fetching code. 4 fp32 rows:
+// 15 us for both kernels (a tile a CTA; 19 as called), 140 rows of 50257: 33 us.
+// Sums of exponentials of a tile of a thread's 16 are in 32 bits, relative to
+// the thread's greatest (2^-22 off each); all sums above that in 64.
 #include "er_kv.cuh"
 #include "er_ptx.cuh"
 
@@ -26,7 +32,7 @@ struct BeamArgs {
   const float* scores;
   int batch, beams, vocab, count;
   int parts, part;  // of a row, and logits of each (a multiple of the tile)
-  double* sums;     // [rows][parts] of 2^.. relative to maxima
+  double* sums;     // [rows][parts] of exponentials, relative to the maxima
   float* maxima;    // [rows][parts]
   unsigned long long* kept;  // [rows][parts][count]: rank key of the logit, then ~token; 0 behind the last
   float* scores_out;

@@ -5,6 +5,8 @@ namespace er {
 
 namespace {
 using bf = __nv_bfloat16;
+// By head_dim, as much as fits: 128 rows of queries, tiles of keys and of values under way. fp32 queries take three
+// times the room.
 using B64 = TreeShape<1, 1, 2, 64, 128, 64, 6, 6>;
 using B128 = TreeShape<1, 1, 2, 128, 128, 64, 4, 4>;
 using B256 = TreeShape<1, 1, 2, 256, 128, 64, 2, 2>;

@@ -4,6 +4,7 @@
 namespace er {
 
 namespace {
+// Three parts of everything: fewer rows and tiles the wider the heads.
 using S64 = TreeShape<3, 3, 3, 64, 128, 64, 2, 2>;
 using S128 = TreeShape<3, 3, 3, 128, 64, 64, 1, 1>;
 using S256 = TreeShape<3, 3, 3, 256, 32, 64, 1, 1>;

@@ -29,8 +29,8 @@ torch's allocator on that stream unless given one.
 
 Infinities: an infinite or NaN key or value behind a row's length changes
 nothing. One that is seen makes the row's results what the formula gives,
-infinite or NaN; over an fp32 cache they may be NaN where the formula gives an
-infinity. Scores of -inf weigh nothing.
+infinite or NaN; over an fp32 cache, and from attend_tree, they may be NaN where
+the formula gives an infinity. Scores of -inf weigh nothing.
 """
 
 from __future__ import annotations
