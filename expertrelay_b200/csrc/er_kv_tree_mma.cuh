@@ -15,26 +15,28 @@
 // One persistent CTA an SM; all units (tree, key head, block of rows) lie in one
 // line of tiles of which each CTA takes an equal share, whatever the lengths.
 // Warps by their work, joined by mbarriers: 4 turn scores into weights (a thread
-// a row), 8 keep the sums, 1 issues products, 3 bring keys, values and the next
-// unit's queries by TMA (fp32 caches: 1 brings, 4 split into parts; above 128
-// channels 7 split from registers). A draft of few rows lies in shared memory
-// two or four times, each copy taking a share of a tile's keys, so that the
-// weights' threads all have work; the copies' sums are joined at a unit's end.
-// Waits have a limit, after which the CTA reports and ends.
+// a row), 8 keep the sums, 2 issue products, 2 bring keys, values and the next
+// unit's queries (fp32 caches: 1 brings, 4 split into parts; above 128 channels
+// 7 split from registers). A draft of few rows lies in shared memory two or four
+// times, each copy taking a share of a tile's keys, so that the weights' threads
+// all have work; the copies' sums are joined at a unit's end. Waits have a
+// limit, after which the CTA reports and ends.
 //
-// Measured (captured calls; of the bytes' time at the measured copy rate):
-// 24 drafts of 23 after up to 4097 positions, 16 heads of 128, bf16: 138 us
-// (0.48): a copy's issue (200 clocks for 16 rows of a page), 7000 clocks
-// between a CTA's units. 8 drafts of 64 after 32768, 4 key heads of 8, bf16:
-// 530 us, 0.52 PFLOP/s, 633 in a long run under the power cap: the steps of a
-// tile, 1800 clocks, of which the products' are 1050. Two groups of weights'
-// warps that take the tiles in turn: 682 us, 180 for the batch (96 registers a
-// thread in place of 128, and the greatest scores handed over every tile). A
-// chain of 16 after 131071, 2 key heads of 6 of 64, fp32 queries: 56-63 us
-// (0.17): three parts of queries and weights, 14 tiles a CTA, then the join.
+// Measured (queued calls; of the bytes' time at the measured copy rate):
+// 24 drafts of 23 after up to 4097 positions, 16 heads of 128, bf16: 140-145 us
+// (0.47): a copy's issue (200 clocks for 16 rows of a page) and what lies
+// between a CTA's units (queries, masks, result: 5000 clocks and more).
+// 8 drafts of 64 after 32768, 4 key heads of 8, bf16: 575-600 us under the power
+// cap, 0.47 PFLOP/s (495 in a short run): the weights' warps, 1650 clocks a
+// tile; products 1050. With one warp for both kinds of products 1790 and 627 us.
+// Two groups of weights' warps that take the tiles in turn: 682 us in a short
+// run (96 registers a thread in place of 128); 544 threads in place of 512: 788.
+// A chain of 16 after 131071, 2 key heads of 6 of 64, fp32 queries: 53-55 us
+// (0.19): three parts of queries and weights, 14 tiles a CTA, then the join, 9.
 // 6 fp32 drafts of 37 after up to 2500: 156 us, six products a pair of operands
 // (48 for a tile's scores, 67 clocks each) and the splitting. A draft of 8
-// after 631 positions: 30 us, the chain from launch to result.
+// after 631 positions: 32 us, two tiles a CTA, each step of which is fetched and
+// run for the first time.
 #pragma once
 
 #include <type_traits>
@@ -46,7 +48,7 @@ namespace er {
 
 namespace {
 
-constexpr int kSoftmaxWarps = 4, kSumWarps = 8, kIssueWarp = kSoftmaxWarps + kSumWarps;
+constexpr int kSoftmaxWarps = 4, kSumWarps = 8, kIssueWarp = kSoftmaxWarps + kSumWarps, kLoadWarp = kIssueWarp + 2;
 
 // KP: bf16 parts of a key or value in shared memory (1: as they come from a bf16 cache, 3: of fp32), QP of a query,
 // PP of a weight. DP: head_dim padded. ROWS: rows of queries in shared memory (of 128 of a product; the others are
@@ -61,30 +63,28 @@ struct TreeShape {
   static_assert(TK == 64, "weights' parts lie 32 columns apart");
   // columns of a tile's scores, then of its weights: two parts over the scores, a third one behind them
   static constexpr int kSP = PP > 2 ? TK * 3 / 2 : TK;
-  // tiles of scores (the products' warp issues them ahead), and results of a tile, kept while they are read
+  // tiles of scores (their products are issued ahead, over a unit's end too), and results of a tile, kept while they are read
   static constexpr int SB = 3 * kSP + 2 * VD <= 512 ? 3 : 2, OB = SB * kSP + 2 * VD <= 512 ? 2 : 1;
-  // the products' warp goes SB - 1 tiles ahead, over a unit's end too, and the last tile's values are looked at before
-  // its weights
-  static_assert(VS >= SB - 1, "a unit's last values would wait for products behind the next one's queries");
   // the epilogue's exchange: EC channels of each half at a time, and 4 floats of padding a row
   static constexpr int EC = KP == 1 && QP > 1 && DP == 128 ? 16 : 32, kStagePitch = 2 * EC + 4;
   // fp32 caches, up to 128 channels: RS half tiles as they come, to be split into parts from there
   static constexpr bool kRaw = KP > 1 && DP <= 128;
   static constexpr int RS = kRaw ? 3 : 0, kRawRows = TK / 2, kRawSlot = kRawRows * DP * 4;
   static constexpr int kSmem = kQ + KS * kKSlot + VS * kVSlot + RS * kRawSlot + ROWS * kStagePitch * 4;
-  // warps that fill shared memory. bf16 caches: one that issues the keys' copies, one the values' and one for the next
-  // unit's queries. fp32: one that issues copies and four that split, or seven that split from registers.
-  static constexpr int kLoadWarps = KP == 1 ? 3 : kRaw ? 5 : 7, kSplitWarps = KP == 1 ? 0 : kRaw ? 4 : 7;
-  static constexpr int kQueryWarps = KP == 1 ? 1 : kSoftmaxWarps;  // of all units but a CTA's first
+  // Warps that fill shared memory. bf16 caches: one that issues the keys' copies, and one the values', which shares the
+  // next unit's queries with the scores' products' warp. fp32: one that issues copies and four that split, or seven
+  // that split from registers.
+  static constexpr int kLoadWarps = KP == 1 ? 2 : kRaw ? 5 : 7, kSplitWarps = KP == 1 ? 0 : kRaw ? 4 : 7;
+  static constexpr int kQueryWarps = KP == 1 ? 2 : kSoftmaxWarps;  // of all units but a CTA's first
   // the warps that look at values of drafted keys
   static constexpr int kLookWarps = KP == 1 ? kSoftmaxWarps : kSplitWarps;
-  static constexpr int kThreads = (kIssueWarp + 1 + kLoadWarps) * 32;
+  static constexpr int kThreads = (kLoadWarp + kLoadWarps) * 32;
 };
 
 template <typename S>
 struct TreeShared {
   uint64_t kfull[S::KS], kempty[S::KS], vfull[S::VS], vempty[S::VS], raw[S::VS], looked[S::VS], rfull[S::RS + 1], rempty[S::RS + 1];
-  uint64_t qfirst, qfull, qfree, sfull[S::SB], pfull[S::SB], ofull[2], ofree[2], staged, masked, drain;
+  uint64_t qfirst, qfull, qfree, sfull[S::SB], pfull[S::SB], pfree[S::SB], ofull[2], ofree[2], staged, masked, drain[2];
   uint32_t tmem;
   volatile int abort;
   TreeRun run;
@@ -98,7 +98,6 @@ struct TreeShared {
   // of tiles in turn: five may be between the weights' warps and the sums'
   float by[8][S::ROWS];             // what a tile's sums so far are multiplied by
   float2 ml[8][S::ROWS];            // maximum and sum of a unit's last tile
-  uint32_t io[S::SB];               // what kind of product a tile's values take
 };
 
 // Descriptors of operands in shared memory, 128-byte swizzle, eight-row groups 1024 bytes apart: the upper word is
@@ -309,79 +308,101 @@ __device__ __forceinline__ uint32_t swizzled(int c, int r, int rows) {
   return (c >> 3) * (rows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// A unit's queries into shared memory, by `warps` warps of which this is one: eight lanes take 64 channels of a
-// query, which is row qi of every replica. Several loads are under way at once, the first ones before ready() says
+// the whole warp waits, with a limit; false once any wait of the CTA has given up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, bar_done(bar, parity))) return true;
+  return bar_wait_slow(bar, parity, abort_flag);
+}
+
+// A unit's queries into shared memory, by `warps` warps of which this is one: eight lanes take a query, which is row
+// qi of every replica. Several loads are under way at once, the first ones before the barrier `free` (0: none) says
 // that the queries there are used no more.
-template <typename S, typename TQ, typename Ready>
-__device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps, Ready ready) {
+template <typename S, typename TQ>
+__device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps,
+                                             uint32_t free, uint32_t parity, volatile int* abort_flag) {
   const int lane = threadIdx.x & 31, d = a.kv.d, R = w.replicas, per = S::ROWS / R, live = w.live;
-  constexpr int chunks = S::DP / 64;
-  const int items = (live + 3) / 4 * chunks;  // of four queries
-  constexpr int U = S::QP == 1 ? 8 : 4, W = sizeof(TQ) / 2;  // W: 16-byte words of eight elements
-  auto place = [&](int i, int* qi, int* c) {
-    const int g = i / chunks;
-    *qi = g * 4 + lane / 8;
-    *c = (i - g * chunks) * 8 + (lane & 7);
-    return i < items && *qi < live && *c * 8 < (d + 15) / 16 * 16;
-  };
+  // C: 16-byte vectors of bf16 of a lane's query, U queries under way; W: 16-byte words of eight elements
+  constexpr int C = S::DP / 64, U = (S::QP == 1 ? 8 : 4) / C > 1 ? (S::QP == 1 ? 8 : 4) / C : 1, W = sizeof(TQ) / 2;
+  const int items = (live + 3) / 4, c0 = lane & 7;  // of four queries
+  auto ready = [&]() { return free == 0 || bar_wait(free, parity, abort_flag); };
 #pragma unroll 1
   for (int i0 = warp; i0 < items; i0 += warps * U) {
-    uint4 x[U][W];
+    uint4 x[U][C][W];
+    const TQ* src[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int qi, c;
+      const int qi = (i0 + u * warps) * 4 + lane / 8, q = w.q0 + qi, node = tree_node(a, q);
+      src[u] = (const TQ*)a.q + (long long)(w.e.first + node) * a.q_stride +
+               (long long)(w.head * a.group + q - node * a.group) * d + c0 * 8;
 #pragma unroll
-      for (int j = 0; j < W; ++j) x[u][j] = make_uint4(0, 0, 0, 0);
-      if (!place(i0 + u * warps, &qi, &c) || c * 8 >= d || a.q_zero) continue;
-      const int q = w.q0 + qi, node = tree_node(a, q);
-      const TQ* src = (const TQ*)a.q + (long long)(w.e.first + node) * a.q_stride +
-                      (long long)(w.head * a.group + q - node * a.group) * d + c * 8;
-      if (a.q_wide) {
+      for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[u][j] = reinterpret_cast<const uint4*>(src)[j];
-      } else {
-        uint32_t h[4 * W];
+        for (int j = 0; j < W; ++j) x[u][c][j] = make_uint4(0, 0, 0, 0);
+    }
+    auto there = [&](int u, int c) { return (i0 + u * warps) * 4 + lane / 8 < live && (c * 8 + c0) * 8 < d; };
+    if (a.q_zero) {
+    } else if (a.q_wide) {
 #pragma unroll
-        for (int j = 0; j < 4 * W; ++j) {
-          if constexpr (sizeof(TQ) == 2)
-            h[j] = (uint32_t)__bfloat16_as_ushort(src[2 * j]) | (uint32_t)__bfloat16_as_ushort(src[2 * j + 1]) << 16;
-          else
-            h[j] = __float_as_uint(src[j]);
-        }
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[u][j] = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
-      }
+        for (int c = 0; c < C; ++c)
+          if (there(u, c))
+#pragma unroll
+            for (int j = 0; j < W; ++j) x[u][c][j] = reinterpret_cast<const uint4*>(src[u] + c * 64)[j];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          if (there(u, c))
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+              uint32_t h[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(TQ) == 2)
+                  h[e] = (uint32_t)__bfloat16_as_ushort(src[u][c * 64 + 2 * e]) |
+                         (uint32_t)__bfloat16_as_ushort(src[u][c * 64 + 2 * e + 1]) << 16;
+                else
+                  h[e] = __float_as_uint(src[u][c * 64 + 4 * j + e]);
+              }
+              x[u][c][j] = make_uint4(h[0], h[1], h[2], h[3]);
+            }
     }
     if (i0 == warp && !ready()) return false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int qi, c;
-      if (!place(i0 + u * warps, &qi, &c)) continue;
-      uint4 parts[3];
-      if constexpr (S::QP == 1) {
-        const uint32_t flip = a.q_flip ? 0x80008000u : 0u;
-        parts[0] = make_uint4(x[u][0].x ^ flip, x[u][0].y ^ flip, x[u][0].z ^ flip, x[u][0].w ^ flip);
-      } else {
-        float y[8];
+      const int qi = (i0 + u * warps) * 4 + lane / 8;
+      if (qi >= live) continue;
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t h[4] = {x[u][j].x, x[u][j].y, x[u][j].z, x[u][j].w};
+      for (int c = 0; c < C; ++c) {
+        if (c * 8 + c0 >= (d + 15) / 16 * 2) continue;
+        uint4 parts[3];
+        if constexpr (S::QP == 1) {
+          const uint32_t flip = a.q_flip ? 0x80008000u : 0u;
+          parts[0] = make_uint4(x[u][c][0].x ^ flip, x[u][c][0].y ^ flip, x[u][c][0].z ^ flip, x[u][c][0].w ^ flip);
+        } else {
+          float y[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (sizeof(TQ) == 2)
-              y[2 * e] = __uint_as_float(h[e] << 16), y[2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
-            else
-              y[4 * j + e] = __uint_as_float(h[e]);
+          for (int j = 0; j < W; ++j) {
+            const uint32_t h[4] = {x[u][c][j].x, x[u][c][j].y, x[u][c][j].z, x[u][c][j].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (sizeof(TQ) == 2)
+                y[2 * e] = __uint_as_float(h[e] << 16), y[2 * e + 1] = __uint_as_float(h[e] & 0xffff0000u);
+              else
+                y[4 * j + e] = __uint_as_float(h[e]);
+            }
           }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = a.q_flip ? -y[j] : y[j];
+          split8(y, parts);
         }
+        for (int r = 0; r < R; ++r) {
+          const uint32_t to = q0 + swizzled(c * 8 + c0, r * per + qi, S::ROWS);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = a.q_flip ? -y[j] : y[j];
-        split8(y, parts);
-      }
-      for (int r = 0; r < R; ++r) {
-        const uint32_t to = q0 + swizzled(c, r * per + qi, S::ROWS);
-#pragma unroll
-        for (int p = 0; p < S::QP; ++p) sts16(to + p * S::kQPart, parts[p]);
+          for (int p = 0; p < S::QP; ++p) sts16(to + p * S::kQPart, parts[p]);
+        }
       }
     }
   }
@@ -390,6 +411,14 @@ __device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& 
   async_fence();
   __syncwarp();
   return true;
+}
+
+// The same for later units, one copy for the warps that share it: in place, it costs the weights' warps registers or
+// the compiler's order (8 trees of 64 after 32768 604 us in place of 575, but 24 of 23 after 4097 132 in place of 140).
+template <typename S, typename TQ>
+static __device__ __noinline__ bool next_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps,
+                                                 uint32_t free, uint32_t parity, volatile int* abort_flag) {
+  return load_queries<S, TQ>(a, w, q0, warp, warps, free, parity, abort_flag);
 }
 
 template <typename S, typename TC, typename TQ>
@@ -417,14 +446,14 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     mbar_init(&s.qfirst, kIssueWarp);
     mbar_init(&s.qfull, S::kQueryWarps);
     mbar_init(&s.qfree, 1);
-    for (int i = 0; i < SB; ++i) mbar_init(&s.sfull[i], 1), mbar_init(&s.pfull[i], kSoftmaxWarps);
+    for (int i = 0; i < SB; ++i) mbar_init(&s.sfull[i], 1), mbar_init(&s.pfull[i], kSoftmaxWarps), mbar_init(&s.pfree[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.ofull[i], 1);
       mbar_init(&s.ofree[i], kSumWarps);
     }
     mbar_init(&s.staged, kSumWarps);
     mbar_init(&s.masked, kSoftmaxWarps);
-    mbar_init(&s.drain, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s.drain[i], 1);
     s.abort = 0;
     s.bad_tree[0] = s.bad_tree[1] = 0;
     for (int i = 0; i < 16; ++i) s.bad_unit[i] = 0;
@@ -435,12 +464,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   tree_run(a, s.run, s.scratch);  // all threads; ends with a barrier
   tc_fence_after();
   const uint32_t tmem = s.tmem;
-  // the whole warp waits, with a limit; false once any wait of the CTA has given up
-  auto wait = [&](const uint64_t& b, uint32_t parity) {
-    const uint32_t bar = smem_u32(&b);
-    if (__all_sync(0xffffffffu, bar_done(bar, parity))) return true;
-    return bar_wait_slow(bar, parity, &s.abort);
-  };
+  auto wait = [&](const uint64_t& b, uint32_t parity) { return bar_wait(smem_u32(&b), parity, &s.abort); };
   auto arrive = [&](const uint64_t& b) {  // the warp's one arrival, after all its lanes
     __syncwarp();
     if (lane == 0) bar_arrive(smem_u32(&b));
@@ -448,7 +472,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   const TreeWalk& w = s.walk[warp];
   auto next = [&](bool first) { return tree_next(a, s.run, &s.walk[warp], first, S::ROWS / 32); };
   if (warp < kIssueWarp && next(true)) {  // the first unit's queries by the warps that have nothing to do yet
-    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp, [] { return true; });
+    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp, 0, 0, &s.abort);
     arrive(s.qfirst);
   }
 
@@ -460,7 +484,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 #pragma unroll 1
     for (bool go = next(true); go && !s.abort; go = next(false), ++unit) {
       if (S::KP > 1 && unit > 0) {  // the first one's are on their way
-        if (!load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps, [&] { return wait(s.qfree, (unit - 1) & 1); })) break;
+        if (!load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort)) break;
         arrive(s.qfull);
       }
       const int R = w.replicas, per = S::ROWS / R, row = threadIdx.x, len = w.e.len, lo = w.lo, hi = w.hi;
@@ -674,7 +698,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
           const float by1 = there ? s.by[it & 7][row] : 0.f;
           const uint64_t by = pack2(by1, by1);
           const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SB * S::kSP + ob * S::VD + half * CH;
-          constexpr int N = S::kThreads > 512 ? 16 : 32;  // registers
+          constexpr int N = S::KP > 1 ? 16 : 32;  // registers
 #pragma unroll
           for (int c = 0; c < CH; c += N) {
             uint32_t x[N];
@@ -749,92 +773,101 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
       if (!ok) break;
     }
-  } else if (warp == kIssueWarp) {
-    // ---- products
-    const int ksteps = (d + 15) / 16;
-    const uint32_t is = idesc_bf16(TK, 0), one = elected();
-    int unit = 0, scored = 0, summed = 0;  // tiles
+  } else if (warp <= kIssueWarp + 1) {
+    // ---- products: a warp's for scores, another's for results, so that neither waits for what the other needs
     constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
-    Ring<SB> sp_ring, p_ring;           // of the tile whose scores, whose values are next
-    Ring<OB> o_ring;
-    Ring<KS> k_ring;
-    Ring<VS> v_ring;
-    auto values = [&]() {  // out += P V of the first tile that has not been
-      const int b = o_ring.at;
-      if (!wait(s.pfull[p_ring.at], p_ring.turn) || !wait(s.vfull[v_ring.at], v_ring.turn)) return false;
-      if (summed >= OB && !wait(s.ofree[b], o_ring.turn ^ 1)) return false;
-      tc_fence_after();
-      uint32_t v = desc_low(v0 + v_ring.at * S::kVSlot, TK * 128);
-      uint32_t to = tmem + SB * S::kSP + b * S::VD, p = tmem + p_ring.at * S::kSP, id = s.io[p_ring.at];
-      // put together here: descriptors that the compiler kept from before the waits' calls came out wrong
-      asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
-      // the small products first
-#pragma unroll
-      for (int pp = S::PP - 1; pp >= 0; --pp)
-#pragma unroll
-        for (int kp = S::KP - 1; kp >= 0; --kp) {
-          if (kThree && pp + kp > 2) continue;
-#pragma unroll
-          for (int k = 0; k < TK / 16; ++k)
-            mma_f16_ts(one, to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
-                       !(pp == S::PP - 1 && kp == (kThree ? 2 - pp : 0) && k == 0));
-        }
-      commit_on(one, smem_u32(&s.ofull[b]));
-      commit_on(one, smem_u32(&s.vempty[v_ring.at]));
-      p_ring.next();
-      o_ring.next();
-      v_ring.next();
-      ++summed;
-      return true;
-    };
+    const uint32_t one = elected();
+    Ring<SB> ring;  // of tiles of scores or weights
+    int tiles = 0;
     bool ok = true;
+    // Descriptors are put together where they are used, from words the compiler cannot know before: those that it kept
+    // over the waits' calls came out wrong. The small products first.
+    if (warp == kIssueWarp) {
+      const int ksteps = (d + 15) / 16;
+      const uint32_t is = idesc_bf16(TK, 0);
+      int unit = 0;
+      Ring<KS> k_ring, last_k;
 #pragma unroll 1
-    for (bool go = next(true); go && ok; go = next(false), ++unit) {
-      const uint32_t io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
-      // while its queries are on their way, the tiles of the unit before
-      while (ok && unit && scored > summed && !__all_sync(0xffffffffu, bar_is_done(smem_u32(&s.qfull), (unit - 1) & 1)))
-        ok = values();
-      if (!ok || !(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
-      const int hi = w.hi;
+      for (bool go = next(true); go && ok; go = next(false), ++unit) {
+        if (S::KP == 1 && unit > 0) {  // half of its queries, which nothing goes on without
+          if (!(ok = next_queries<S, TQ>(a, w, q0, 1, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort))) break;
+          arrive(s.qfull);
+        }
+        if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
+        const int hi = w.hi;
 #pragma unroll 1
-      for (int t = w.lo; t < hi; ++t) {
-        if (!(ok = wait(s.kfull[k_ring.at], k_ring.turn))) break;
-        if (lane == 0) s.io[sp_ring.at] = io;
-        __syncwarp();
-        tc_fence_after();
-        uint32_t kd = desc_low(k0 + k_ring.at * S::kKSlot, 16), qd = desc_low(q0, 16);
-        uint32_t to = tmem + sp_ring.at * S::kSP, id = is;
-        asm volatile("" : "+r"(kd), "+r"(qd), "+r"(to), "+r"(id));
+        for (int t = w.lo; t < hi; ++t, ++tiles, ring.next(), k_ring.next()) {
+          if (tiles >= SB && !(ok = wait(s.pfree[ring.at], ring.turn ^ 1))) break;
+          if (!(ok = wait(s.kfull[k_ring.at], k_ring.turn))) break;
+          tc_fence_after();
+          uint32_t kd = desc_low(k0 + k_ring.at * S::kKSlot, 16), qd = desc_low(q0, 16);
+          uint32_t to = tmem + ring.at * S::kSP, id = is;
+          asm volatile("" : "+r"(kd), "+r"(qd), "+r"(to), "+r"(id));
 #pragma unroll
-        for (int qp = S::QP - 1; qp >= 0; --qp)
+          for (int qp = S::QP - 1; qp >= 0; --qp)
 #pragma unroll
-          for (int kp = S::KP - 1; kp >= 0; --kp) {
-            if (kThree && qp + kp > 2) continue;
+            for (int kp = S::KP - 1; kp >= 0; --kp) {
+              if (kThree && qp + kp > 2) continue;
 #pragma unroll
-            for (int k = 0; k < S::DP / 16; ++k)
-              mma_f16_ss(k < ksteps ? one : 0u, to, qd + ((qp * S::kQPart + (k >> 2) * (S::ROWS * 128) + (k & 3) * 32) >> 4),
-                         kd + ((kp * S::kKPart + (k >> 2) * (TK * 128) + (k & 3) * 32) >> 4), id,
-                         !(qp == S::QP - 1 && kp == (kThree ? 2 - qp : 0) && k == 0));
-          }
-        commit_on(one, smem_u32(&s.sfull[sp_ring.at]));
-        commit_on(one, smem_u32(&s.kempty[k_ring.at]));
-        if (t + 1 == hi) commit_on(one, smem_u32(&s.qfree));
-        sp_ring.next();
-        k_ring.next();
-        ++scored;
-        if (scored - summed == SB && !(ok = values())) break;
+              for (int k = 0; k < S::DP / 16; ++k)
+                mma_f16_ss(k < ksteps ? one : 0u, to, qd + ((qp * S::kQPart + (k >> 2) * (S::ROWS * 128) + (k & 3) * 32) >> 4),
+                           kd + ((kp * S::kKPart + (k >> 2) * (TK * 128) + (k & 3) * 32) >> 4), id,
+                           !(qp == S::QP - 1 && kp == (kThree ? 2 - qp : 0) && k == 0));
+            }
+          commit_on(one, smem_u32(&s.sfull[ring.at]));
+          commit_on(one, smem_u32(&s.kempty[k_ring.at]));
+          if (t + 1 == hi) commit_on(one, smem_u32(&s.qfree));
+          last_k = k_ring;
+        }
+        if (!ok) break;
       }
-      if (!ok) break;
+      // no arrival is under way when the CTA ends
+      if (ok && unit > 0) ok = wait(s.kempty[last_k.at], last_k.turn) && wait(s.qfree, (unit - 1) & 1);
+    } else {
+      Ring<OB> o_ring;
+      Ring<VS> v_ring, last_v;
+      Ring<SB> last;
+#pragma unroll 1
+      for (bool go = next(true); go && ok; go = next(false)) {
+        const uint32_t io = idesc_bf16((min(S::VD, d - w.ch0) + 15) / 16 * 16, 1);
+        const int hi = w.hi;
+#pragma unroll 1
+        for (int t = w.lo; t < hi; ++t, ++tiles, ring.next(), o_ring.next(), v_ring.next()) {
+          const int b = o_ring.at;
+          if (!(ok = wait(s.vfull[v_ring.at], v_ring.turn))) break;
+          if (tiles >= OB && !(ok = wait(s.ofree[b], o_ring.turn ^ 1))) break;
+          if (!(ok = wait(s.pfull[ring.at], ring.turn))) break;
+          tc_fence_after();
+          uint32_t v = desc_low(v0 + v_ring.at * S::kVSlot, TK * 128);
+          uint32_t to = tmem + SB * S::kSP + b * S::VD, p = tmem + ring.at * S::kSP, id = io;
+          asm volatile("" : "+r"(v), "+r"(to), "+r"(p), "+r"(id));
+#pragma unroll
+          for (int pp = S::PP - 1; pp >= 0; --pp)
+#pragma unroll
+            for (int kp = S::KP - 1; kp >= 0; --kp) {
+              if (kThree && pp + kp > 2) continue;
+#pragma unroll
+              for (int k = 0; k < TK / 16; ++k)
+                mma_f16_ts(one, to, p + pp * 32 + k * 8, v + ((kp * S::kVPart + k * 2048) >> 4), id,
+                           !(pp == S::PP - 1 && kp == (kThree ? 2 - pp : 0) && k == 0));
+            }
+          commit_on(one, smem_u32(&s.ofull[b]));
+          commit_on(one, smem_u32(&s.pfree[ring.at]));
+          commit_on(one, smem_u32(&s.vempty[v_ring.at]));
+          last = ring;
+          last_v = v_ring;
+        }
+        if (!ok) break;
+      }
+      if (ok && tiles > 0) ok = wait(s.pfree[last.at], last.turn) && wait(s.vempty[last_v.at], last_v.turn);
     }
-    Ring<VS> last = v_ring;
-    while (ok && scored > summed) last = v_ring, ok = values();
-    if (ok && summed > 0) ok = wait(s.vempty[last.at], last.turn);
     if (!ok) {  // the products under way end before their memory goes
-      commit_on(one, smem_u32(&s.drain));
-      mbar_drain(&s.drain, 0, kDefaultWaitNs);
+      uint64_t* drain = &s.drain[warp - kIssueWarp];
+      commit_on(one, smem_u32(drain));
+      mbar_drain(drain, 0, kDefaultWaitNs);
     }
     __syncwarp();
-  } else if (S::kRaw && warp == kIssueWarp + 1) {
+  } else if (S::kRaw && warp == kLoadWarp) {
     // ---- copies of fp32 keys and values, half a tile each, in the order in which they are split: the next tile's
     // keys before a tile's values
     const int rows = a.box_rows, each = S::kRawRows / rows;
@@ -898,9 +931,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       while (globaltimer() - t0 < 2000000ull) {
       }
     }
-  } else if (S::KP == 1 && warp <= kIssueWarp + 2) {
-    // ---- copies of keys, or of values: boxes of as many positions as lie in one page
-    const bool values = warp == kIssueWarp + 2;
+  } else if constexpr (S::KP == 1) {
+    // ---- copies of keys, or of values and a unit's queries: boxes of as many positions as lie in one page
+    const bool values = warp == kLoadWarp + 1;
     const int rows = a.box_rows, boxes = TK / rows, box_shift = __ffs(boxes) - 1, ring = values ? VS : KS;
     const CUtensorMap* map = values ? &vmap : &kmap;
     const uint32_t one = elected(), slots0 = values ? v0 : k0, slot_bytes = values ? S::kVSlot : S::kKSlot;
@@ -909,6 +942,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     bool ok = true;
 #pragma unroll 1
     for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
+      if (values && unit > 0) {  // its queries first; the first unit's are on their way
+        if (!(ok = next_queries<S, TQ>(a, w, q0, 0, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort))) break;
+        arrive(s.qfull);
+      }
       const int32_t* pages = a.kv.pages_of(w.e.seq);
       const int len = w.e.len, keys = len + w.e.nodes, x0 = values ? w.ch0 : 0;
       const int chunks = ((values ? min(S::VD, d - w.ch0) : d) + 63) / 64;
@@ -973,8 +1010,8 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
     }
   } else {
-    // ---- the next unit's queries (bf16 caches), or keys and values split into parts (fp32 caches)
-    const int loader = warp - (kIssueWarp + 1 + S::kLoadWarps - S::kSplitWarps);
+    // ---- keys and values split into parts (fp32 caches)
+    const int loader = warp - (kLoadWarp + S::kLoadWarps - S::kSplitWarps);
     int unit = 0, it = 0, k_item = 0;
     Ring<KS> k_ring;
     Ring<VS> v_ring;
@@ -987,12 +1024,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 #pragma unroll 1
     for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
       const int keys = w.e.len + w.e.nodes;
-      if constexpr (S::KP == 1) {
-        if (unit > 0) {  // the first one's are on their way
-          if (!(ok = load_queries<S, TQ>(a, w, q0, 0, 1, [&] { return wait(s.qfree, (unit - 1) & 1); }))) break;
-          arrive(s.qfull);
-        }
-      } else if constexpr (S::kRaw) {
+      if constexpr (S::kRaw) {
         const int len = w.e.len, hi = w.hi;
         constexpr int ITEMS = (S::kRawRows / 4 * (S::DP / 64) + S::kSplitWarps - 1) / S::kSplitWarps;  // four rows, 64 channels
         auto split = [&](int t, const uint64_t& full, uint32_t to, int part, bool look, int slot) {
