@@ -13,7 +13,7 @@ from conftest import golden
 from golden.make_golden import MODEL_CASES, MODEL_NEW
 from kv_ref import tokens
 
-from expertrelay_b200 import _lib, draft, synth
+from expertrelay_b200 import _lib, draft, kv, synth
 from expertrelay_b200.kv_cache import PagedKVCache
 from expertrelay_b200.model import QwenMoeModel
 from oracle.moe_oracle import rel_l2
@@ -145,6 +145,75 @@ def test_texts_that_go_on_from_shared_pages(options, cuda):
         kv.release(s)
     assert sorted(kv.pages.free) == list(range(len(kv.pages.uses)))
     kv.check()
+    model.close()
+
+
+def test_bounds_follow_accepted_drafts_and_forks(cuda):
+    """Rejected drafts leave nothing in the bounds that page choices go by: after each step that appends, they are those
+    of the keys that are there."""
+    shape = SimpleNamespace(num_layers=2, num_kv_heads=2, head_dim=16)
+    cache = PagedKVCache(shape, 3, 40, page_size=4, select=(3, 1, 1), device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+
+    def run(seqs, parents=None, loud=1.0):
+        step = cache.step(seqs, parents)
+        for layer in range(2):
+            qkv = torch.randn((len(seqs), 6 * 16), generator=gen, device=cuda)
+            cache.attend(layer, step, qkv * loud, 2, 1e4)
+        return step
+
+    def right():
+        lens = torch.tensor(cache.pages.length, dtype=torch.int32, device=cuda)
+        for layer in range(2):
+            fresh = kv.PageBounds.new(cache.layers[layer])
+            kv.page_bounds(cache.layers[layer], fresh, lens, torch.zeros_like(lens))
+            used = [int(p) for s in range(3) for p in cache.pages.table[s, :-(-cache.length(s) // 4)]]
+            assert torch.equal(fresh.codes[used], cache.bounds[layer].codes[used])
+            assert torch.equal(fresh.scales[used], cache.bounds[layer].scales[used])
+
+    run([0] * 9 + [1] * 3)
+    right()
+    step = run([0] * 8 + [1] * 2, [-1, 0, 1, 0, 3, 4, 5, 2, -1, -1], loud=50.0)
+    cache.accept(step, [[0, 3, 4, 5, 6], [1]])
+    right()
+    cache.undo(run([0] * 4, [-1] * 4, loud=500.0))
+    right()
+    cache.accept(run([1] * 4, [-1] * 4, loud=500.0), [[]])
+    right()
+    cache.reorder([2], [0])
+    run([0, 1, 2])
+    right()
+    cache.reorder([0, 1, 2], [2, 2, 0])
+    run([2, 1, 0])
+    right()
+    cache.check()
+
+
+@pytest.mark.parametrize("at", [0, 1])
+def test_drafted_calls_that_raise_can_be_made_again(at, cuda):
+    """Nothing stays of a call that fails between layers, and a draft of tokens that there are none of is refused."""
+    model = _model(0, cuda)
+    kv, fresh = (model.new_paged_cache(2, 32, page_size=4) for _ in range(2))
+    for c in (kv, fresh):
+        model.forward([1, 2, 3, 4, 5], c, seqs=[1] * 5)
+    before = (kv.pages.table.copy(), kv.pages.length.copy(), kv.pages.position.copy(), list(kv.pages.free))
+    stack = model.stack
+
+    class Fails:
+        def moe(self, layer, *args, **kwargs):
+            if layer == at:
+                raise RuntimeError("no room")
+            return stack.moe(layer, *args, **kwargs)
+
+    for tokens, error in (([7, 8, 9], RuntimeError), ([7, model.c.vocab_size, 9], ValueError)):
+        model.stack = Fails() if error is RuntimeError else stack
+        with pytest.raises(error):
+            model.forward(tokens, kv, all_logits=True, seqs=[1] * 3, parents=[-1, 0, 0])
+        model.stack = stack
+        assert kv.drafted is None and (kv.pages.table == before[0]).all() and (kv.pages.length == before[1]).all()
+        assert (kv.pages.position == before[2]).all() and kv.pages.free == before[3]
+    got, want = (model.forward([7, 8, 9], c, all_logits=True, seqs=[1] * 3, parents=[-1, 0, 0]) for c in (kv, fresh))
+    assert torch.equal(got, want)
     model.close()
 
 
