@@ -13,7 +13,6 @@
 namespace er {
 
 constexpr int kMaxTrees = 4096, kMaxNodes = 256;
-constexpr int kTreeRows = 128;  // of a matrix product
 constexpr int kTreeChannels = 128;  // of the values, at most, that a unit has
 
 // A unit whose tiles several CTAs share: the first of them writes it, the join reads it.
@@ -75,7 +74,6 @@ __device__ __forceinline__ Tree kv_tree(const TreeArgs& a, int t) {
   }
   return e;
 }
-
 
 // The line that the CTAs share. A unit is a block of at most block_rows query
 // rows (nodes x group, in equal blocks) of one key head of a tree, and of at

@@ -124,6 +124,67 @@ def test_compact(cuda, dtype, layout, layers, heads, ps, d, span, most):
     cache.check()
 
 
+@pytest.mark.parametrize("rows", [255, 256, 257, 700])
+def test_compact_many_rows(cuda, rows):
+    """Lists of all lengths, in every order; a bad one among them."""
+    rng = np.random.default_rng(rows)
+    ps, width, span = 8, 5, 30
+    start = rng.integers(0, 10, rows).tolist()
+    counts = rng.integers(0, 13, rows).tolist()
+    keep = [sorted(rng.choice(span, n, replace=False).tolist()) for n in counts]
+    both, k, v, table = _pools(2, rows * width, 2, ps, 64, BF16, "hnd", rows, width)
+    table.copy_(torch.from_numpy(rng.permutation(rows * width).reshape(rows, width)))
+    cache = kv.PagedLayers(k, v, table)
+    lists = torch.full((rows, 12), -5, dtype=torch.int32, device="cuda")
+    for i, row in enumerate(keep):
+        lists[i, :len(row)] = _i32(row)
+    bad, good = rows // 2, list(counts)
+    counts[bad], good[bad] = 13, 0
+    pages = table.tolist()
+    wk, wv = (_compacted(x, pages, range(rows), start, keep, good, ps) for x in (k, v))
+    lens = kv.compact(cache, _i32(start), lists, _i32(counts))
+    assert lens.tolist() == [-1 if i == bad else a + n for i, (a, n) in enumerate(zip(start, counts))]
+    assert _same(k, wk) and _same(v, wv)
+    with pytest.raises(ValueError, match="length"):
+        cache.check()
+
+
+def test_captured_and_on_another_stream(cuda):
+    """One graph of a fork and an acceptance, replayed over other pages, lists and counts."""
+    ps, width = 4, 6
+    both, k, v, table = _pools(3, 3 * width, 2, ps, 32, F32, "hnd", 2, width)
+    table.copy_(torch.arange(2 * width).view(2, width))
+    cache = kv.PagedLayers(k, v, table)
+    src, dst, used = _i32([0, 6]), _i32([12, 13]), _i32([4, 2])
+    start, keep, counts = _i32([3, 0]), _i32([[1, 2, 5], [0, 4, 9]]), _i32([3, 2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    was = both.clone()
+    with torch.cuda.stream(side):
+        kv.copy_pages(cache, src, dst, used=used)
+        kv.compact(cache, start, keep, counts)
+    torch.cuda.current_stream().wait_stream(side)
+    both.copy_(was)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kv.copy_pages(cache, src, dst, used=used)
+        lens = kv.compact(cache, start, keep, counts)
+    for pairs, lists, n in (([(0, 12, 4), (6, 13, 2)], [[1, 2, 5], [0, 4, 9]], [3, 2]), ([(3, 16, 1), (-1, 0, 4)], [[0, 1, 2], [7, 8, 11]], [1, 3])):
+        both.copy_(was)
+        for t, new in zip((src, dst, used), zip(*pairs)):
+            t.copy_(_i32(list(new)))
+        keep.copy_(_i32(lists))
+        counts.copy_(_i32(n))
+        want = was.clone()
+        for a, b, m in pairs:
+            if a >= 0:
+                want[:, :, b, :, :m] = want[:, :, a, :, :m]
+        wk, wv = (_compacted(x, table.tolist(), [0, 1], [3, 0], lists, n, ps) for x in want)
+        g.replay()
+        assert _same(both[0], wk) and _same(both[1], wv) and lens.tolist() == [3 + n[0], n[1]]
+    cache.check()
+
+
 def test_bad_rows_stay_unwritten(cuda):
     both, k, v, table = _pools(2, 12, 2, 4, 16, F32, "hnd", 3, 4)
     table.copy_(torch.arange(12).reshape(3, 4))

@@ -314,3 +314,29 @@ def test_trees_are_as_exact_as_32_bits(cuda, cache_dtype, q_dtype, kv_heads, gro
     got = result_error(torch.stack(outs), torch.stack(wants), q_dtype)
     assert got <= bound, f"{got:.3g} of the result, {bound:.3g} allowed"
     cache.check()
+
+
+@pytest.mark.parametrize(("cache_dtype", "d"), [(BF16, 128), (F32, 128), (F32, 256)])
+def test_pools_past_32_bits(cuda, cache_dtype, d):
+    """The last pages of pools of 4.3 GB each: attention, copies and places moved, as in a pool of those pages alone."""
+    ps, pages = 64, 10
+    rng = np.random.default_rng(4)
+    lens, trees = [300, 211], [_tree(rng, 9), _tree(rng, 20)]
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    many = (2**32 + 2**26) // (ps * d * cache_dtype.itemsize)
+    big = [torch.empty((many, 1, ps, d), dtype=cache_dtype, device=cuda) for _ in range(2)]
+    small = [torch.randn((pages + 1, 1, ps, d), generator=gen, device=cuda).to(cache_dtype) for _ in range(2)]
+    for a, b in zip(big, small):
+        a[many - pages - 1:] = b
+    table = _i32(rng.permutation(pages).reshape(2, 5).tolist())
+    caches = [kv.PagedKV(*small, table), kv.PagedKV(*big, table + (many - pages - 1))]
+    q = torch.randn((29, 4, d), generator=gen, device=cuda).to(cache_dtype)
+    args = _i32(lens), _i32([0, 9, 29]), _i32(trees[0] + trees[1])
+    want, got = (kv.attend_tree(c, q, *args) for c in caches)
+    assert torch.equal(want, got)
+    for c, first in zip(caches, (0, many - pages - 1)):
+        kv.copy_pages(c, _i32([first + 2]), _i32([first + pages]))
+        kv.compact(c, _i32([250, 200]), _i32([[3, 40, 41], [0, 9, 30]]), _i32([3, 3]))
+        c.check()
+    for a, b in zip(big, small):
+        assert torch.equal(a[many - pages - 1:], b)
