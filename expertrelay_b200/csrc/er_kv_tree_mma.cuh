@@ -6,8 +6,8 @@
 // queries a key head, which is what a matrix product of 128 rows wants: S = Q K^T
 // (both in shared memory) and out = P V (P over its own scores in tensor memory)
 // take bf16 operands. What is not bf16 goes in as bf16 parts: fp32 caches and
-// queries in three, 24 bits; weights in three where the result is fp32, in two
-// (16 bits, 2^-18 off at the most) where it has 8. Products of parts whose
+// queries in three, 24 bits; weights in three, or in two (16 bits, 2^-18 off at
+// the most) where cache and result are bf16. Products of parts whose
 // places add up to three or more are left out: 2^-24 of the whole. A tile's
 // result is added to sums in registers, in rounded fp32: the tensor cores' own
 // accumulators cut every addition, which tells after some hundred tiles.
