@@ -110,7 +110,7 @@ constexpr int kBatchRows = 512, kCut = 8;  // kCut: vectors of a place a CTA has
 
 __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_constant__ CompactArgs a) {
   kv_enter();
-  __shared__ long long from[2][kBatchRows], to[2][kBatchRows];
+  __shared__ long long from[3][kBatchRows], to[3][kBatchRows];
   const KvView& kv = a.l.kv;
   const int layer = blockIdx.y >> 1, column = blockIdx.x / a.cuts, row16 = a.l.row16 / a.cuts;
   const int h0 = column * a.heads, heads = min(a.heads, kv.kv_heads - h0);
@@ -165,9 +165,13 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_const
     };
     look(0, 0);
     __syncthreads();
+    // Places in three buffers, for one barrier a batch: the places that batch i + 1 gets were batch i - 2's. Those were
+    // read last by i - 2's stores, before a thread's barrier of batch i - 1, and are written behind that barrier. In two
+    // they would be batch i - 1's, which a warp behind the others may still have to read for its stores.
     int b = 0;
 #pragma unroll 1
-    for (int j0 = 0; j0 < n; j0 += batch, b ^= 1) {
+    for (int j0 = 0; j0 < n; j0 += batch) {
+      const int following = b == 2 ? 0 : b + 1;
       const int total = min(batch, n - j0) * width;
       uint4 v[kMany];
 #pragma unroll
@@ -177,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_const
         const int r = i / width, c = i - r * width, h = c / row16;
         v[u] = load16(pool + from[b][r] + h * kv.head_stride + (c - h * row16) * 16);
       }
-      if (j0 + batch < n) look(j0 + batch, b ^ 1);
+      if (j0 + batch < n) look(j0 + batch, following);
       __syncthreads();  // all of the batch is read, and the next one's places are known
 #pragma unroll
       for (int u = 0; u < kMany; ++u) {
@@ -186,6 +190,7 @@ __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_const
         const int r = i / width, c = i - r * width, h = c / row16;
         store16(pool + to[b][r] + h * kv.head_stride + (c - h * row16) * 16, v[u]);
       }
+      b = following;
     }
     __syncthreads();  // the places of the last batch are used no more
   }

@@ -236,3 +236,36 @@ def test_refusals(cuda):
             call()
     assert kv.compact(cache, i[:0], _i32([]).view(0, 3), i[:0]).shape == (0,)
     assert kv.compact(cache, i, _i32([]).view(2, 0), _i32([0, 0])).tolist() == [0, 1]
+
+
+@pytest.mark.parametrize(("heads", "ps", "d", "dtype", "most"), [
+    (4, 32, 128, BF16, 2100), (2, 16, 64, F32, 1300), (1, 64, 8, BF16, 3000), (3, 24, 136, BF16, 500), (1, 16, 248, F32, 260),
+    (8, 32, 256, F32, 1100),
+])
+def test_lists_of_many_batches(cuda, heads, ps, d, dtype, most):
+    """Many long lists in many layers at once, so that the warps of a CTA are not abreast: every key and value in its
+    place, several times over."""
+    rng = np.random.default_rng(most + d)
+    layers, rows, span = 6, 24, most + most // 3
+    start = rng.integers(0, 3 * ps, rows)
+    counts = [most, 0, 1, *rng.integers(most // 2, most + 1, rows - 3).tolist()]
+    width = -(-(int(start.max()) + span) // ps)
+    both, k, v, table = _pools(layers, rows * width, heads, ps, d, dtype, "hnd", rows, width)
+    table.copy_(torch.from_numpy(rng.permutation(rows * width).reshape(rows, width)))
+    lists = np.full((rows, most), -1)
+    for i, n in enumerate(counts):
+        lists[i, :n] = np.sort(rng.choice(span, n, replace=False))
+    row, j = (torch.from_numpy(x).cuda() for x in np.nonzero(lists >= 0))
+    frm = torch.from_numpy(start[row.cpu()] + lists[lists >= 0]).cuda()
+    to = torch.from_numpy(start).cuda()[row] + j
+    pages = table.long()
+    want = both.clone()
+    want[:, :, pages[row, to // ps], :, to % ps] = both[:, :, pages[row, frm // ps], :, frm % ps]
+    cache, was = kv.PagedLayers(k, v, table), both.clone()
+    args = _i32(start.tolist()), _i32(lists.tolist()), _i32(counts)
+    for _ in range(6):
+        both.copy_(was)
+        lens = kv.compact(cache, *args)
+        assert _same(both, want)
+        assert lens.tolist() == [int(a) + n for a, n in zip(start, counts)]
+    cache.check()
