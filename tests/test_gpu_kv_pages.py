@@ -269,3 +269,21 @@ def test_lists_of_many_batches(cuda, heads, ps, d, dtype, most):
         assert _same(both, want)
         assert lens.tolist() == [int(a) + n for a, n in zip(start, counts)]
     cache.check()
+
+
+def test_bad_rows_leave_values_too(cuda):
+    """Keys and values of a bad row stay as they were, and the other rows' are moved."""
+    both, k, v, table = _pools(3, 12, 2, 4, 16, BF16, "hnd", 3, 4)
+    table.copy_(torch.arange(12).reshape(3, 4))
+    was, start, counts = both.clone(), [3, 4, 2], [3, 2, 3]
+    for keep0, page in (([1, 3, 3], None), ([1, 3, 14], None), ([-1, 3, 4], None), ([1, 3, 5], 12), ([1, 3, 5], -1)):
+        both.copy_(was)
+        keep, pages = [keep0, [0, 2, 3], [4, 5, 6]], table.clone()
+        if page is not None:
+            pages[0, 1] = page
+        cache = kv.PagedLayers(k, v, pages)
+        assert kv.compact(cache, _i32(start), _i32(keep), _i32(counts)).tolist() == [-1, 6, 5]
+        for pool, old in zip(both, was):
+            assert _same(pool, _compacted(old, table.tolist(), [1, 2], start[1:], keep[1:], counts[1:], 4))
+        with pytest.raises(ValueError, match="page" if page is not None else "length"):
+            cache.check()
