@@ -223,6 +223,7 @@ SIGNATURES: dict[str, tuple] = {
                          C.c_longlong, C.c_longlong, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "er_kv_tree_workspace_bytes": (C.c_size_t, [C.POINTER(KvCache), C.POINTER(KvTreeIO)]),
     "er_kv_tree": (_i, [C.POINTER(KvCache), C.POINTER(KvTreeIO), _vp, C.c_size_t, _vp]),
+    "er_kv_tree_test_stall": (_i, [C.c_ulonglong, _i]),
     "er_kv_copy_pages": (_i, [C.POINTER(KvCache), _i, C.c_longlong, _vp, _vp, _vp, _i, _vp, _vp]),
     "er_kv_compact": (_i, [C.POINTER(KvCache), _i, C.c_longlong, _vp, _vp, _vp, C.c_longlong, _i, _vp, _i, _vp, _vp, _vp]),
     "er_beam_workspace_bytes": (C.c_size_t, [_i, _i, _i, _i]),

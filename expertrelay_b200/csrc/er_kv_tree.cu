@@ -9,7 +9,8 @@ namespace {
 // Joins the units that several CTAs share: CTA (x, y) takes every gridDim.x-th
 // of them from x on, of its rows every gridDim.y-th. Of many pieces the warps
 // share a row's, of few each takes rows of its own. Also writes the rows of
-// trees that something is wrong with, which no attention CTA meets.
+// trees that something is wrong with, which no attention CTA meets, and of all
+// trees where an attention CTA gave up.
 constexpr int kJoinWarps = 8, kJoinMost = 1024;  // CTAs that may share a line at most
 
 template <typename TQ>
@@ -19,24 +20,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv_tree_join_kernel(const 
   __shared__ float2 tops[kJoinWarps];
   kv_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
+  if (warp == 0) {  // the CTAs in whose runs such a unit begins
+    int n = 0;
+    bool gave_up = false;
+    for (int c0 = 0; c0 < a.grid; c0 += 32) {
+      const int live = c0 + lane < a.grid ? a.cut[c0 + lane].live : 0;
+      const uint32_t all = __ballot_sync(0xffffffffu, live > 0);
+      if (live > 0) cuts[n + __popc(all & ((1u << lane) - 1))] = c0 + lane;
+      n += __popc(all);
+      gave_up |= live < 0;
+    }
+    gave_up = __any_sync(0xffffffffu, gave_up);
+    if (lane == 0) found = gave_up ? -1 : n;
+  }
+  __syncthreads();
   for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.trees; t += gridDim.x * gridDim.y) {
     const Tree e = kv_tree(a, t);
-    if (!e.bad) continue;
+    if (!e.bad && found >= 0) continue;
     TQ* out = (TQ*)a.out + (long long)e.first * a.heads * d;
     for (long long i = threadIdx.x; i < (long long)e.nodes * a.heads * d; i += kJoinWarps * 32)
       out[i] = kv_round<TQ>(__int_as_float(0x7fc00000));
   }
-  if (warp == 0) {  // the CTAs in whose runs such a unit begins
-    int n = 0;
-    for (int c0 = 0; c0 < a.grid; c0 += 32) {
-      const bool cut = c0 + lane < a.grid && a.cut[c0 + lane].live > 0;
-      const uint32_t all = __ballot_sync(0xffffffffu, cut);
-      if (cut) cuts[n + __popc(all & ((1u << lane) - 1))] = c0 + lane;
-      n += __popc(all);
-    }
-    if (lane == 0) found = n;
-  }
-  __syncthreads();
   constexpr int N = 8;  // pieces under way
 #pragma unroll 1
   for (int f = blockIdx.x; f < found; f += gridDim.x) {
@@ -117,6 +121,10 @@ int tree_check(const er_kv_cache* c, const er_kv_tree_io* io) {
 using namespace er;
 
 namespace {
+
+// er_kv_tree_test_stall: the limit of a wait, and whether the attention kernel's CTAs end with one that runs out
+unsigned long long tree_wait_ns = kDefaultWaitNs;
+int tree_stall = 0;
 
 struct TreeLayout {
   TreeLaunch shape;
@@ -213,6 +221,7 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   // 24 trees of up to 4097 positions, 16 heads, bf16: 4 tiles 147 us, 8 141, 14 139, 24 140; 6 of up to 2500, fp32,
   // whose tiles take four times as long: 150, 151, 157 and 169
   a.unit_cost = cb ? 12 : 4;
+  a.wait_ns = tree_wait_ns, a.stall = tree_stall;
   a.block_rows = L.shape.rows, a.channels = L.shape.channels, a.halves = L.shape.halves;
   CUtensorMap maps[2] = {};
   if (L.shape.box_rows) {
@@ -231,4 +240,11 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   const dim3 grid(across, parts);
   return qb ? kv_launch(kv_tree_join_kernel<bf>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a)
             : kv_launch(kv_tree_join_kernel<float>, grid, kJoinWarps * 32, 0, false, st, "kv_tree_join_kernel", a);
+}
+
+extern "C" int er_kv_tree_test_stall(unsigned long long wait_ns, int stall) {
+  if (stall < 0 || stall > 1) return fail(ER_EINVAL, "er_kv_tree_test_stall: stall %d (0 or 1)", stall);
+  tree_wait_ns = wait_ns ? wait_ns : kDefaultWaitNs;
+  tree_stall = stall;
+  return ER_OK;
 }

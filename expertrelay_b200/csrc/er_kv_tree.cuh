@@ -17,7 +17,7 @@ constexpr int kTreeChannels = 128;  // of the values, at most, that a unit has
 
 // A unit whose tiles several CTAs share: the first of them writes it, the join reads it.
 struct TreeCut {
-  int first, head, q0, live;  // live 0: none begins here and ends behind
+  int first, head, q0, live;  // live 0: none begins here and ends behind; -1: a wait of the CTA gave up
   int tiles, ch0;
   long long begin, total;  // the unit's place in the line, and the line's length
 };
@@ -44,6 +44,8 @@ struct TreeArgs {
   TreeCut* cut;            // [grid]
   float* part_ml;          // [2 grid][piece_rows][2]: m, l of a CTA's first piece and of one that begins in it
   float* part_o;           // [2 grid][piece_rows][channels]
+  unsigned long long wait_ns;  // limit of a wait
+  int stall;               // test hook (er_kv_tree_test_stall): a wait at a CTA's end that runs out
 };
 
 // A tree: its rows first .. first + nodes - 1 and its context. Where its rows

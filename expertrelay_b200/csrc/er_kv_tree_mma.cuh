@@ -20,7 +20,7 @@
 // 7 split from registers). A draft of few rows lies in shared memory two or four
 // times, each copy taking a share of a tile's keys, so that the weights' threads
 // all have work; the copies' sums are joined at a unit's end. Waits have a
-// limit, after which the CTA reports and ends.
+// limit, after which the CTA reports, ends, and leaves the join to spoil all of the call's rows.
 //
 // Measured (queued calls; of the bytes' time at the measured copy rate):
 // 24 drafts of 23 after up to 4097 positions, 16 heads of 128, bf16: 140-145 us
@@ -81,12 +81,18 @@ struct TreeShape {
   static constexpr int kThreads = (kLoadWarp + kLoadWarps) * 32;
 };
 
+// What every wait of a CTA goes by: whether one has given up, and after how many ns one does.
+struct TreeWaits {
+  volatile int abort;
+  unsigned long long limit;
+};
+
 template <typename S>
 struct TreeShared {
   uint64_t kfull[S::KS], kempty[S::KS], vfull[S::VS], vempty[S::VS], raw[S::VS], looked[S::VS], rfull[S::RS + 1], rempty[S::RS + 1];
   uint64_t qfirst, qfull, qfree, sfull[S::SB], pfull[S::SB], pfree[S::SB], ofull[2], ofree[2], staged, masked, drain[2];
   uint32_t tmem;
-  volatile int abort;
+  TreeWaits waits;
   TreeRun run;
   TreeScratch scratch;
   TreeWalk walk[S::kThreads / 32];
@@ -170,13 +176,13 @@ __device__ __forceinline__ bool bar_done_asleep(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, TreeWaits* waits) {
   if (__all_sync(0xffffffffu, bar_done_asleep(bar, parity))) return true;
   const unsigned long long t0 = globaltimer();
   bool ok = true;
   while (!bar_done_asleep(bar, parity)) {
-    if (*abort_flag || globaltimer() - t0 > kDefaultWaitNs) {
-      *abort_flag = 1;
+    if (waits->abort || globaltimer() - t0 > waits->limit) {
+      waits->abort = 1;
       ok = false;
       break;
     }
@@ -309,9 +315,9 @@ __device__ __forceinline__ uint32_t swizzled(int c, int r, int rows) {
 }
 
 // the whole warp waits, with a limit; false once any wait of the CTA has given up
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, TreeWaits* waits) {
   if (__all_sync(0xffffffffu, bar_done(bar, parity))) return true;
-  return bar_wait_slow(bar, parity, abort_flag);
+  return bar_wait_slow(bar, parity, waits);
 }
 
 // A unit's queries into shared memory, by `warps` warps of which this is one: eight lanes take a query, which is row
@@ -319,12 +325,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // that the queries there are used no more.
 template <typename S, typename TQ>
 __device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps,
-                                             uint32_t free, uint32_t parity, volatile int* abort_flag) {
+                                             uint32_t free, uint32_t parity, TreeWaits* waits) {
   const int lane = threadIdx.x & 31, d = a.kv.d, R = w.replicas, per = S::ROWS / R, live = w.live;
   // C: 16-byte vectors of bf16 of a lane's query, U queries under way; W: 16-byte words of eight elements
   constexpr int C = S::DP / 64, U = (S::QP == 1 ? 8 : 4) / C > 1 ? (S::QP == 1 ? 8 : 4) / C : 1, W = sizeof(TQ) / 2;
   const int items = (live + 3) / 4, c0 = lane & 7;  // of four queries
-  auto ready = [&]() { return free == 0 || bar_wait(free, parity, abort_flag); };
+  auto ready = [&]() { return free == 0 || bar_wait(free, parity, waits); };
 #pragma unroll 1
   for (int i0 = warp; i0 < items; i0 += warps * U) {
     uint4 x[U][C][W];
@@ -417,8 +423,8 @@ __device__ __forceinline__ bool load_queries(const TreeArgs& a, const TreeWalk& 
 // the compiler's order (8 trees of 64 after 32768 604 us in place of 575, but 24 of 23 after 4097 132 in place of 140).
 template <typename S, typename TQ>
 static __device__ __noinline__ bool next_queries(const TreeArgs& a, const TreeWalk& w, uint32_t q0, int warp, int warps,
-                                                 uint32_t free, uint32_t parity, volatile int* abort_flag) {
-  return load_queries<S, TQ>(a, w, q0, warp, warps, free, parity, abort_flag);
+                                                 uint32_t free, uint32_t parity, TreeWaits* waits) {
+  return load_queries<S, TQ>(a, w, q0, warp, warps, free, parity, waits);
 }
 
 template <typename S, typename TC, typename TQ>
@@ -454,7 +460,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     mbar_init(&s.staged, kSumWarps);
     mbar_init(&s.masked, kSoftmaxWarps);
     for (int i = 0; i < 2; ++i) mbar_init(&s.drain[i], 1);
-    s.abort = 0;
+    s.waits.abort = 0, s.waits.limit = a.wait_ns;
     s.bad_tree[0] = s.bad_tree[1] = 0;
     for (int i = 0; i < 16; ++i) s.bad_unit[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   tree_run(a, s.run, s.scratch);  // all threads; ends with a barrier
   tc_fence_after();
   const uint32_t tmem = s.tmem;
-  auto wait = [&](const uint64_t& b, uint32_t parity) { return bar_wait(smem_u32(&b), parity, &s.abort); };
+  auto wait = [&](const uint64_t& b, uint32_t parity) { return bar_wait(smem_u32(&b), parity, &s.waits); };
   auto arrive = [&](const uint64_t& b) {  // the warp's one arrival, after all its lanes
     __syncwarp();
     if (lane == 0) bar_arrive(smem_u32(&b));
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
   const TreeWalk& w = s.walk[warp];
   auto next = [&](bool first) { return tree_next(a, s.run, &s.walk[warp], first, S::ROWS / 32); };
   if (warp < kIssueWarp && next(true)) {  // the first unit's queries by the warps that have nothing to do yet
-    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp, 0, 0, &s.abort);
+    load_queries<S, TQ>(a, w, q0, warp, kIssueWarp, 0, 0, &s.waits);
     arrive(s.qfirst);
   }
 
@@ -482,9 +488,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     Ring<SB> sp_ring;
     Ring<VS> v_ring;
 #pragma unroll 1
-    for (bool go = next(true); go && !s.abort; go = next(false), ++unit) {
+    for (bool go = next(true); go && !s.waits.abort; go = next(false), ++unit) {
       if (S::KP > 1 && unit > 0) {  // the first one's are on their way
-        if (!load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort)) break;
+        if (!load_queries<S, TQ>(a, w, q0, warp, kSoftmaxWarps, smem_u32(&s.qfree), (unit - 1) & 1, &s.waits)) break;
         arrive(s.qfull);
       }
       const int R = w.replicas, per = S::ROWS / R, row = threadIdx.x, len = w.e.len, lo = w.lo, hi = w.hi;
@@ -680,7 +686,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     uint32_t stages = 0;
     if (id == 0) a.cut[blockIdx.x].live = 0;
 #pragma unroll 1
-    for (bool go = next(true); go && !s.abort; go = next(false)) {
+    for (bool go = next(true); go && !s.waits.abort; go = next(false)) {
       uint64_t o[CH / 2];  // two channels each
 #pragma unroll
       for (int c = 0; c < CH / 2; ++c) o[c] = 0;
@@ -773,6 +779,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
       if (!ok) break;
     }
+    if (a.stall) wait(s.drain[0], 0);  // which nothing completes
   } else if (warp <= kIssueWarp + 1) {
     // ---- products: a warp's for scores, another's for results, so that neither waits for what the other needs
     constexpr bool kThree = S::KP > 1;  // products of parts i and j: those with i + j > 2 are under 2^-24 of the whole
@@ -790,7 +797,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
 #pragma unroll 1
       for (bool go = next(true); go && ok; go = next(false), ++unit) {
         if (S::KP == 1 && unit > 0) {  // half of its queries, which nothing goes on without
-          if (!(ok = next_queries<S, TQ>(a, w, q0, 1, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort))) break;
+          if (!(ok = next_queries<S, TQ>(a, w, q0, 1, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.waits))) break;
           arrive(s.qfull);
         }
         if (!(ok = unit ? wait(s.qfull, (unit - 1) & 1) : wait(s.qfirst, 0))) break;
@@ -876,7 +883,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     int unit = 0, item = 0;
     bool ok = true;
 #pragma unroll 1
-    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
+    for (bool go = next(true); go && ok && !s.waits.abort; go = next(false), ++unit) {
       const int32_t* pages = a.kv.pages_of(w.e.seq);
       const int keys = w.e.len + w.e.nodes, hi = w.hi, head = w.head;
       auto page_of = [&](int t, int i) {  // of box i; behind the last key none
@@ -926,11 +933,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         for (int j = 0; j < 2; ++j) now[j] = then[j], then[j] = page_of(t + 2, lane + 32 * j);
       }
     }
-    if (!ok || s.abort) {  // no copy is under way when the CTA's memory goes: they take microseconds
-      const unsigned long long t0 = globaltimer();
-      while (globaltimer() - t0 < 2000000ull) {
-      }
-    }
   } else if constexpr (S::KP == 1) {
     // ---- copies of keys, or of values and a unit's queries: boxes of as many positions as lie in one page
     const bool values = warp == kLoadWarp + 1;
@@ -941,9 +943,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     uint32_t turn = 0;
     bool ok = true;
 #pragma unroll 1
-    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
+    for (bool go = next(true); go && ok && !s.waits.abort; go = next(false), ++unit) {
       if (values && unit > 0) {  // its queries first; the first unit's are on their way
-        if (!(ok = next_queries<S, TQ>(a, w, q0, 0, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.abort))) break;
+        if (!(ok = next_queries<S, TQ>(a, w, q0, 0, 2, smem_u32(&s.qfree), (unit - 1) & 1, &s.waits))) break;
         arrive(s.qfull);
       }
       const int32_t* pages = a.kv.pages_of(w.e.seq);
@@ -1004,11 +1006,6 @@ __global__ void __launch_bounds__(S::kThreads, 1)
         if (++at_slot == ring) at_slot = 0, turn ^= 1;
       }
     }
-    if (!ok || s.abort) {  // no copy is under way when the CTA's memory goes: they take microseconds
-      const unsigned long long t0 = globaltimer();
-      while (globaltimer() - t0 < 2000000ull) {
-      }
-    }
   } else {
     // ---- keys and values split into parts (fp32 caches)
     const int loader = warp - (kLoadWarp + S::kLoadWarps - S::kSplitWarps);
@@ -1022,7 +1019,7 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       arrive(b);
     };
 #pragma unroll 1
-    for (bool go = next(true); go && ok && !s.abort; go = next(false), ++unit) {
+    for (bool go = next(true); go && ok && !s.waits.abort; go = next(false), ++unit) {
       const int keys = w.e.len + w.e.nodes;
       if constexpr (S::kRaw) {
         const int len = w.e.len, hi = w.hi;
@@ -1210,10 +1207,17 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       }
     }
   }
-  if (s.abort && threadIdx.x == 0) kv_report(a.status, ER_KV_GAVE_UP);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (s.waits.abort && threadIdx.x == 0) {  // no warp can give up from here on
+    // nor is a copy under way when the CTA's memory goes: they take microseconds
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < 2000000ull) {
+    }
+    a.cut[blockIdx.x].live = -1;
+    kv_report(a.status, ER_KV_GAVE_UP);
+  }
   if (warp == kIssueWarp) tmem_dealloc<1>(tmem, 512);
 }
 

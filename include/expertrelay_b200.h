@@ -405,7 +405,7 @@ typedef struct er_kv_cache {
 #define ER_KV_BAD_LENGTH 2     /* a length, position or count outside its table */
 #define ER_KV_BAD_SEQ 4        /* a sequence index outside [0, seqs) */
 #define ER_KV_BAD_TREE 8       /* a tree's rows or parents */
-#define ER_KV_GAVE_UP 16       /* a wait of the kernel ran out (2 s): its results are not to be used */
+#define ER_KV_GAVE_UP 16       /* a wait of the kernel ran out (2 s): all of the call's rows are NaN */
 
 /* RoPE and the write of new tokens' rows into the pages: row i of qkv
  * [n, (heads + 2 kv_heads) head_dim] (q | k | v, dtype qkv_dtype, row stride
@@ -521,6 +521,13 @@ typedef struct er_kv_tree_io {
 ER_API size_t er_kv_tree_workspace_bytes(const er_kv_cache* cache, const er_kv_tree_io* io);
 ER_API int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, void* workspace, size_t workspace_bytes,
                       void* stream);
+/* Test hook of er_kv_tree's waits: in every later call each has the limit
+ * wait_ns (0: the default, 2 s), and with stall = 1 the warps of a CTA that end
+ * last wait for what never comes, when nothing else of the CTA is under way:
+ * the call ends with ER_KV_GAVE_UP.
+ * (0, 0) restores normal operation. Process-wide, not thread-safe; for tests of
+ * that path only. */
+ER_API int er_kv_tree_test_stall(unsigned long long wait_ns, int stall);
 
 /* Copies of pages in `layers` pools at once (layer l's pages begin
  * l * layer_stride elements behind cache->k and cache->v): the first used[i]

@@ -9,7 +9,7 @@ import torch
 from kv_ref import U, attend_exact, make_cache, result_bound, result_error
 from tree_ref import check_trees
 
-from expertrelay_b200 import kv
+from expertrelay_b200 import _lib, kv
 
 pytestmark = pytest.mark.gpu
 
@@ -340,3 +340,30 @@ def test_pools_past_32_bits(cuda, cache_dtype, d):
         c.check()
     for a, b in zip(big, small):
         assert torch.equal(a[many - pages - 1:], b)
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("lens", "kv_heads", "d"), [([40, 3], 2, 64), ([5000], 2, 128), ([200, 700, 90], 8, 256)])
+def test_a_wait_that_runs_out_is_reported_and_spoils_every_row(cuda, cache_dtype, q_dtype, lens, kv_heads, d):
+    """The warps that keep the sums wait for what never comes, when their CTA's other warps are through: the call ends,
+    with its rows NaN and a RuntimeError from check(); the next one is as ever."""
+    rng = np.random.default_rng(3)
+    trees = [_tree(rng, 5) for _ in lens]
+    cache, q, ln, starts, parents = _case(13, lens, trees, kv_heads, 2, d, 16, cache_dtype, q_dtype)
+    want = kv.attend_tree(cache, q, ln, starts, parents)
+    out, lib = torch.full((q.shape[0] + 1, *q.shape[1:]), 7.0, dtype=q_dtype, device="cuda"), _lib.lib()
+    _lib.check(lib.er_kv_tree_test_stall(1000000, 1), "er_kv_tree_test_stall")
+    try:
+        more = torch.cat([q, q[:1]]), torch.cat([parents, _i32([-1])])
+        kv.attend_tree(cache, more[0], ln, starts, more[1], out=out)
+    finally:
+        _lib.check(lib.er_kv_tree_test_stall(0, 0), "er_kv_tree_test_stall")
+    assert torch.isnan(out[:-1]).all() and torch.all(out[-1] == 7.0)
+    with pytest.raises(RuntimeError, match="gave up"):
+        cache.check()
+    assert torch.equal(kv.attend_tree(cache, q, ln, starts, parents), want)
+    cache.check()
+
+
+def test_the_stall_of_waits_has_two_modes():
+    assert _lib.lib().er_kv_tree_test_stall(0, 2) == _lib.ER_EINVAL and _lib.lib().er_kv_tree_test_stall(0, -1) == _lib.ER_EINVAL
