@@ -303,6 +303,11 @@ class QwenMoeModel:
             parents = [-1, *(int(p) + 1 for p in parents)][:most]
             logits = self.forward(tokens, kv, all_logits=True, seqs=[seq] * len(tokens), parents=parents)
             next_of = torch.argmax(logits, dim=1).tolist()
+            try:
+                kv.check()
+            except BaseException:  # the logits are no good
+                kv.undo(kv.drafted)
+                raise
             path, had = [0], len(out)
             while len(out) < new_tokens:
                 out.append(next_of[path[-1]])
@@ -333,9 +338,10 @@ class QwenMoeModel:
         logits = self.forward(prompt, kv)[None]
         scores, texts, done, live = torch.zeros((1, 1), device=self.device), [[]], [], [0]
         for n in range(new_tokens):
-            best, of, tokens = beam.select(logits, scores, min(count, logits.numel()))
+            best, of, tokens = (x[0].tolist() for x in beam.select(logits, scores, min(count, logits.numel())))
+            kv.check()
             going = []
-            for value, i, t in zip(best[0].tolist(), of[0].tolist(), tokens[0].tolist()):
+            for value, i, t in zip(best, of, tokens):
                 if t == end or n + 1 == new_tokens:
                     done.append((texts[i] + [t], value))
                 elif len(going) < beams:

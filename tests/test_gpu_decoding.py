@@ -327,3 +327,31 @@ def test_decoding_refusals(cuda):
     with pytest.raises(ValueError, match="at least 1"):
         model.generate_drafted([1], 0)
     model.close()
+
+
+def test_a_call_that_the_device_found_wrong_ends_the_decoding(cuda):
+    """Attention that gave up waiting, or met a bad page: no token comes of it, and the draft's places are given back."""
+    model = _model(0, cuda)
+    prompt = [1, 2, 3, 4, 5]
+    want = model.generate(prompt, 4)[0]
+    kv = model.new_paged_cache(2, 32, page_size=4)
+
+    def spoils(text):
+        kv.status.fill_(_lib.KV_GAVE_UP)
+        return [7, 8], [-1, 0]
+
+    with pytest.raises(RuntimeError, match="gave up"):
+        model.generate_drafted(prompt, 4, spoils, kv=kv)
+    assert kv.drafted is None and kv.length(0) == len(prompt)
+    _whole(kv)
+    kv.release(0)
+    assert model.generate_drafted(prompt, 4, lambda text: ([7, 8], [-1, 0]), kv=kv)[0] == want
+    kv.release(0)
+    for bit, error in ((_lib.KV_GAVE_UP, RuntimeError), (_lib.KV_BAD_PAGE, ValueError)):
+        kv.status.fill_(bit)
+        with pytest.raises(error, match="paged cache"):
+            model.beam_search(prompt, 2, 4, kv=kv)
+        for s in range(2):
+            kv.release(s)
+    assert model.beam_search(prompt, 1, 4, kv=kv)[0][0] == want
+    model.close()
