@@ -287,13 +287,16 @@ class QwenMoeModel:
         parents), a tree of guesses at what comes next (kv.attend_tree's order; -1:
         the text's last token; none is fine). One call runs them all, and the
         path that greedy decoding would have taken stays. Returns (generated ids,
-        calls after the prompt's). kv: a cache of one's own, its sequence `seq`
-        empty (room for the prompt, new_tokens and a call's guesses)."""
+        calls after the prompt's). kv: a cache of one's own, without accumulated
+        weights; the prompt goes on from what its sequence `seq` holds (room for
+        the prompt, new_tokens and a call's guesses)."""
         prompt = [int(t) for t in prompt]
         if new_tokens < 1:
             raise ValueError(f"new_tokens: at least 1, got {new_tokens}")
         if kv is None:
             kv, seq = self.new_paged_cache(1, len(prompt) + new_tokens + 256), 0
+        if kv.mass is not None:
+            raise ValueError("generate_drafted: not over a cache made with mass=True, which takes no drafted tokens")
         out, calls = [int(torch.argmax(self.forward(prompt, kv, seqs=[seq] * len(prompt))).item())], 0
         while len(out) < new_tokens:
             tokens, parents = draft(prompt + out)
@@ -324,14 +327,19 @@ class QwenMoeModel:
                     kv: PagedKVCache | None = None) -> list[tuple[list[int], float]]:
         """The `beams` best continuations of `prompt` by the sum of their tokens' log
         probabilities that a search of that breadth finds, best first: [(ids, sum)].
-        They have new_tokens tokens, or end with `end`. kv: a cache of one's own
-        with sequences 0 .. beams - 1 empty, for their use."""
+        They have new_tokens tokens, or end with `end`. kv: a cache of one's own;
+        the prompt goes on from what sequence 0 holds, and sequences 1 .. beams - 1
+        are empty, for the search's use. What sequences 0 .. beams - 1 hold afterwards
+        are beams of its last step: release them."""
         prompt = [int(t) for t in prompt]
         if beams < 1 or new_tokens < 1:
             raise ValueError(f"{beams} beams of {new_tokens} tokens: at least one each")
         if kv is None:
             kv = self.new_paged_cache(beams, len(prompt) + new_tokens)
         kv.pages.known([beams - 1])
+        full = [s for s in range(1, beams) if kv.length(s)]
+        if full:
+            raise ValueError(f"beam_search: sequences {full} of the cache are not empty")
         count = beams if end is None else 2 * beams  # as many that go on, whichever of them end
         if count > 128:
             raise ValueError(f"{beams} beams: at most {128 * beams // count}")

@@ -355,3 +355,36 @@ def test_a_call_that_the_device_found_wrong_ends_the_decoding(cuda):
             kv.release(s)
     assert model.beam_search(prompt, 1, 4, kv=kv)[0][0] == want
     model.close()
+
+
+def test_searches_go_on_from_what_the_cache_holds(cuda):
+    """A text in two parts gives what it gives in one, and no sequence's text is written over."""
+    model = _model(1, cuda)
+    text = [3, 1, 4, 1, 5, 9, 2, 6]
+    want = model.generate(text, 5)[0]
+
+    def fresh(**options):
+        kv = model.new_paged_cache(4, 32, page_size=4, **options)
+        model.forward(text[:5], kv, seqs=[0] * 5)
+        return kv
+
+    kv = fresh()
+    assert model.generate_drafted(text[5:], 5, lambda t: ([want[0], 7], [-1, 0]), kv=kv)[0] == want
+    assert kv.length(0) == len(text) + 4
+    kv = fresh()
+    assert model.beam_search(text[5:], 1, 5, kv=kv)[0][0] == want
+    one, two = model.beam_search(text, 3, 5), model.beam_search(text[5:], 3, 5, kv=fresh())
+    assert [t for t, _ in one] == [t for t, _ in two]
+    np.testing.assert_allclose([v for _, v in one], [v for _, v in two], rtol=1e-4)
+    for s in (1, 2):
+        kv = fresh()
+        model.forward([7, 7], kv, seqs=[s, s])
+        before = (kv.pages.table.copy(), kv.pages.length.copy())
+        with pytest.raises(ValueError, match="not empty"):
+            model.beam_search(text[5:], 3, 5, kv=kv)
+        assert (kv.pages.table == before[0]).all() and (kv.pages.length == before[1]).all()
+    kv = fresh(mass=True)
+    with pytest.raises(ValueError, match="mass=True"):
+        model.generate_drafted(text[5:], 5, kv=kv)
+    assert kv.length(0) == 5
+    model.close()
