@@ -32,8 +32,8 @@ struct BeamArgs {
   const float* scores;
   int batch, beams, vocab, count;
   int parts, part;  // of a row, and logits of each (a multiple of the tile)
-  double* sums;     // [rows][parts] of exponentials, relative to the maxima
-  float* maxima;    // [rows][parts]
+  double* sums;     // [rows][parts] of exponentials, relative to e^refs
+  float* refs;      // [rows][parts]
   unsigned long long* kept;  // [rows][parts][count]: rank key of the logit, then ~token; 0 behind the last
   float* scores_out;
   int32_t *beams_out, *tokens_out;
@@ -134,8 +134,23 @@ struct Logits {
   }
 };
 
-// e^x for x <= 0 in 32 bits: within 2^-22 and |x| 2^-25 of it
-__device__ __forceinline__ float exp_below(float x) { return ex2(x * 1.44269504f); }
+// Sums of exponentials are relative to whole numbers, no less than the logits and under one more than the greatest:
+// what one is multiplied by when its reference rises is a power of 1/e, within 2^-46 however often that happens.
+__device__ __forceinline__ double relative_to(double sum, float from, float to) {
+  const float by = to - from;
+  if (!(by > 0.f)) return sum;  // NaN: none of the two is finite
+  double power = 0.36787944117144233;
+  // e^-63 is less than the last bit of any sum; mostly 1 or 2
+  for (int n = by < 63.f ? (int)by : 63; n; n >>= 1, power *= power)
+    if (n & 1) sum *= power;
+  return sum;
+}
+
+// the greatest of the warp's (NaN where that is what a lane has)
+__device__ __forceinline__ float warp_max(float x) {
+  auto order = [](int b) { return b ^ (b >> 31 & 0x7fffffff); };
+  return __int_as_float(order(__reduce_max_sync(0xffffffffu, order(__float_as_int(x)))));
+}
 
 // Of every logit: a maximum, a subtraction, a product, an exponential and a sum; whether it can be among the best is
 // asked of a thread's greatest, and only a thread that has one looks again. Sums of 16 go to 64 bits.
@@ -146,7 +161,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   __shared__ int red[64], held_n;
   __shared__ uint32_t warp_least[kScanThreads / 32];
   __shared__ double sums[kScanThreads / 32];
-  __shared__ float tops[kScanThreads / 32];
+  __shared__ float refs[kScanThreads / 32];
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int begin = blockIdx.x * a.part, end = min(a.vocab, begin + a.part);
   const T* logits = (const T*)a.logits + row * a.stride;
@@ -155,7 +170,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   Logits<T> next;
   next.load(logits, begin, end, wide);
   if (threadIdx.x == 0) held_n = 0;
-  float m = -INFINITY;
+  float m = -INFINITY, ref = -INFINITY;  // the thread's greatest logit, and what the warp's sums are relative to
   double sum = 0.0;
   unsigned long long bound = 0;  // what has to be reached to be held
   float least = -INFINITY;       // its logit (what is not below it may be held)
@@ -192,17 +207,20 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < kEach; ++j) top = fmaxf(top, x[j]);
-    if (top > m) {
-      sum *= (double)exp_below(m - top);  // 0 where m is -inf
-      m = top;
+    m = fmaxf(m, top);
+    const float warp_top = warp_max(top);
+    if (warp_top > ref) {
+      const float up = ceilf(warp_top);
+      if (ref != -INFINITY) sum = relative_to(sum, ref, up);  // 0, or NaN, where it is
+      ref = up;
     }
-    // a thread whose logits are all -inf, or NaN among them, so far: its sum stays 0, or becomes NaN
-    const float ref = m == -INFINITY ? 0.f : m;
-    const uint64_t off = pack2(-ref, -ref), unit = pack2(1.44269504f, 1.44269504f);
+    // a warp whose logits are all -inf, or NaN among them, so far: its sums stay 0, or become NaN
+    const float from = ref == -INFINITY ? 0.f : ref;
+    const uint64_t off = pack2(-from, -from), unit = pack2(1.44269504f, 1.44269504f);
     uint64_t part[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) {
-      float u, v;  // e^(x - m): within 2^-22 and |x - m| 2^-25 of it
+      float u, v;  // e^(x - ref): within 2^-22 and |x - ref| 2^-23 of it
       unpack2(fma2(add2(pack2(x[j], x[j + 1]), off), unit, 0), u, v);
       part[j / 2 & 1] = add2(part[j / 2 & 1], pack2(ex2(u), ex2(v)));
     }
@@ -262,21 +280,17 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   }
   if ((int)threadIdx.x >= n && (int)threadIdx.x < a.count) kept[threadIdx.x] = 0;
   // the threads' sums, in an order that does not change
-  float top = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (m != -INFINITY) sum *= (double)exp_below(m - top);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) sums[warp] = sum, tops[warp] = top;
+  if (lane == 0) sums[warp] = sum, refs[warp] = ref;
   __syncthreads();
   if (threadIdx.x == 0) {
-    float all = tops[0];
-    for (int w = 1; w < kScanThreads / 32; ++w) all = fmaxf(all, tops[w]);
+    float all = refs[0];
+    for (int w = 1; w < kScanThreads / 32; ++w) all = fmaxf(all, refs[w]);
     double s = 0.0;
-    for (int w = 0; w < kScanThreads / 32; ++w) s += tops[w] == -INFINITY ? sums[w] : sums[w] * (double)exp_below(tops[w] - all);
+    for (int w = 0; w < kScanThreads / 32; ++w) s += refs[w] == -INFINITY ? sums[w] : relative_to(sums[w], refs[w], all);
     a.sums[(long long)row * a.parts + blockIdx.x] = s;
-    a.maxima[(long long)row * a.parts + blockIdx.x] = all;
+    a.refs[(long long)row * a.parts + blockIdx.x] = all;
   }
 }
 
@@ -323,13 +337,13 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
   for (int b = warp; b < a.beams; b += kPickThreads / 32) {
     const long long at = (row0 + b) * a.parts;
     float top = -INFINITY;
-    for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.maxima[at + p]);
+    for (int p = lane; p < a.parts; p += 32) top = fmaxf(top, a.refs[at + p]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     double sum = 0.0;
     for (int p = lane; p < a.parts; p += 32) {
-      const float m = a.maxima[at + p];
-      sum += m == -INFINITY ? a.sums[at + p] : a.sums[at + p] * (double)exp_below(m - top);
+      const float ref = a.refs[at + p];
+      sum += ref == -INFINITY ? a.sums[at + p] : relative_to(a.sums[at + p], ref, top);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -455,7 +469,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
 
 struct BeamLayout {
   int parts, part;
-  size_t sums, maxima, kept, bytes;
+  size_t sums, refs, kept, bytes;
 };
 
 BeamLayout beam_layout(int rows, int vocab, int count, int sms) {
@@ -475,7 +489,7 @@ BeamLayout beam_layout(int rows, int vocab, int count, int sms) {
   };
   const size_t n = (size_t)rows * L.parts;
   L.sums = take(n * 8);
-  L.maxima = take(n * 4);
+  L.refs = take(n * 4);
   L.kept = take(n * count * 8);
   L.bytes = at;
   return L;
@@ -521,7 +535,7 @@ extern "C" int er_beam_select(const void* logits, int dtype, long long row_strid
   if ((uintptr_t)workspace & 255) return fail(ER_EINVAL, "er_beam_select: workspace must be 256-byte aligned");
   char* ws = (char*)workspace;
   BeamArgs a = {logits, row_stride, scores, batch, beams, vocab, count, L.parts, L.part, (double*)(ws + L.sums),
-                (float*)(ws + L.maxima), (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
+                (float*)(ws + L.refs), (unsigned long long*)(ws + L.kept), scores_out, beams_out, tokens_out};
   cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(L.parts, rows);
   int rc = dtype == ER_DTYPE_BF16

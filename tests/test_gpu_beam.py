@@ -131,3 +131,24 @@ def test_refusals(cuda):
         with pytest.raises(ValueError, match=words):
             call()
     assert [tuple(t.shape) for t in beam.select(x[:0], s[:0], 4)] == [(0, 4)] * 3
+
+
+def test_rows_that_rise_with_every_tile(cuda):
+    """Log-sums to the bound that _check states wherever a row's greatest come: every tile of 4096 here has a new
+    maximum, a little above the last one. The scores make the values near zero, so that no rounding hides the sum's."""
+    rows, vocab = 600, 500003
+    up = torch.linspace(2e-4, 0.08, rows, dtype=torch.float64, device="cuda")
+    tile = torch.arange(vocab, device="cuda") // 4096
+    logits = torch.empty((rows, vocab), device="cuda")
+    want, scores = [], []
+    for r in range(0, rows, 100):
+        logits[r:r + 100] = (up[r:r + 100, None] * tile).float()
+        x = logits[r:r + 100].double()
+        lse = torch.logsumexp(x, -1)
+        scores.append((lse - x[:, -1]).float())
+        want.append(scores[-1].double() + (x[:, -1] - lse))
+    want, scores = torch.cat(want), torch.cat(scores)
+    got, beams, tokens = beam.select(logits, scores[:, None], 1)
+    assert torch.all(beams == 0) and torch.all(tokens[:, 0] == int(torch.nonzero(tile == tile[-1])[0]))
+    off = (got[:, 0].double() - want).abs().max().item()
+    assert off <= 2.0 ** -21, f"{off * 2 ** 21:.3g} of the bound"
