@@ -27,7 +27,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, count: int, *,
     value is scores[b, i] + log_softmax(logits[b * beams + i])[token]; scores
     [batch, beams] float32, logits [batch * beams, vocab] float32 or bfloat16
     (rows may be strided). Values are compared in 64 bits; ties go to the lower
-    beam, then the lower token, and within a beam the higher logit wins. A beam
+    beam, then the lower token, and within a beam the higher logit wins. A beam's
+    log-sum is good to 2^-20, so candidates of different beams that are closer
+    than that may come in either order (equal rows of equal score tie). A beam
     whose score is infinite or NaN, or whose logits hold a NaN or +inf or
     nothing but -inf, offers nothing: its candidates have value -inf, like
     logits of -inf. count: at most 128 and beams x vocab; at most 1024 beams and

@@ -6,15 +6,18 @@
 // CTA that reads a part of a row keeps the part's best `count` logits (the
 // other candidates cannot be chosen) beside the part's maximum and sum of
 // exponentials; a second kernel joins the parts' sums and chooses among what
-// was kept, by values in 64 bits: candidates of different beams compare through
-// their beams' log-sums, whose rounding in 32 bits would decide close ones.
+// was kept, by values in 64 bits: candidates of one beam keep the order of
+// their logits, those of different beams compare through their beams' log-sums.
 // 2 or 4 bytes a candidate and about a dozen instructions: 256 rows of 151936
 // bf16 logits take 36 us (0.33 of the copy rate), the instructions and the
 // barrier of a tile; then the choice over 32 batches 12 us, a chain of
 // dependent steps in one CTA a batch, most of it fetching code. 4 fp32 rows:
 // 15 us for both kernels (a tile a CTA; 19 as called), 140 rows of 50257: 33 us.
-// Sums of exponentials of a tile of a thread's 16 are in 32 bits, relative to
-// the thread's greatest (2^-22 off each); all sums above that in 64.
+// Exponentials, relative to a whole number that is no less than a warp's logits
+// and mostly under one more than the greatest, are in 32 bits (2^-22 off, and
+// |x - ref| 2^-22), and so is the sum of a thread's 16 of a tile; all sums above
+// that, and what they are multiplied by when a reference rises, are in 64. A
+// log-sum is good to 2^-20: beams whose values are closer may go either way.
 #include "er_kv.cuh"
 #include "er_ptx.cuh"
 
@@ -134,8 +137,8 @@ struct Logits {
   }
 };
 
-// Sums of exponentials are relative to whole numbers, no less than the logits and under one more than the greatest:
-// what one is multiplied by when its reference rises is a power of 1/e, within 2^-46 however often that happens.
+// What a sum is multiplied by when its reference rises by a whole number: a power of 1/e, within 2^-46. (As an
+// exponential in 32 bits it is 2^-22 off, and rows that rise with every tile gather that: 123 tiles 7 x 2^-21.)
 __device__ __forceinline__ double relative_to(double sum, float from, float to) {
   const float by = to - from;
   if (!(by > 0.f)) return sum;  // NaN: none of the two is finite
@@ -220,7 +223,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
     uint64_t part[2] = {0, 0};
 #pragma unroll
     for (int j = 0; j < kEach; j += 2) {
-      float u, v;  // e^(x - ref): within 2^-22 and |x - ref| 2^-23 of it
+      float u, v;  // e^(x - ref): within 2^-22 and |x - ref| 2^-22 of it
       unpack2(fma2(add2(pack2(x[j], x[j + 1]), off), unit, 0), u, v);
       part[j / 2 & 1] = add2(part[j / 2 & 1], pack2(ex2(u), ex2(v)));
     }

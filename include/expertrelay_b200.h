@@ -553,7 +553,7 @@ ER_API int er_kv_compact(const er_kv_cache* cache, int layers, long long layer_s
  * logits[batch * beams + beam, token] - log(sum over tokens of exp(logits)), the
  * best `count` in descending order: scores_out, beams_out, tokens_out [batch,
  * count]. Values are compared in 64 bits (within a beam by the logit), ties go to
- * the lower beam, then the lower token. Candidates of a beam whose score is NaN
+ * the lower beam, then the lower token; a log-sum is good to 2^-20. Candidates of a beam whose score is NaN
  * or infinite or whose log-sum is none (a NaN or +inf logit, nothing but -inf),
  * and logits of -inf, have value -inf. logits ER_DTYPE_F32 / ER_DTYPE_BF16, rows
  * row_stride elements apart on any element boundary. At most 1024 beams, 65535
