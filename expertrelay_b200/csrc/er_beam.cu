@@ -310,7 +310,9 @@ __device__ __forceinline__ double unrank64(unsigned long long k) {
 }
 
 struct PickShared {
-  unsigned long long value[kPickChunk + kMaxCount], place[kPickChunk + kMaxCount];  // place: ~(beam * vocab + token)
+  // candidates, by what they are ordered by: the value, kMaxBeams - 1 - beam, the logit's rank and ~token
+  unsigned long long value[kPickChunk + kMaxCount], logit[kPickChunk + kMaxCount];
+  uint16_t beam[kPickChunk + kMaxCount];
   double lse[kMaxBeams];
   int red[64], n;
   uint32_t warp_least[kPickThreads / 32];
@@ -370,30 +372,32 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
   constexpr int E = kPickEach + 1;
 #pragma unroll 1
   for (long long c0 = 0; c0 < total; c0 += kPickChunk) {
-    unsigned long long key[kPickEach], place[kPickEach];
+    unsigned long long key[kPickEach], logit[kPickEach];
+    int beam[kPickEach];
     uint32_t best = 0;
 #pragma unroll
     for (int i = 0; i < kPickEach; ++i) {
       const long long c = c0 + i * kPickThreads + threadIdx.x;
       bool take = c < total;
-      place[i] = key[i] = 0;
+      logit[i] = key[i] = 0;
+      beam[i] = 0;
       if (take) {
         const int b = (int)(c >> 32 ? c / each : (uint32_t)c / (uint32_t)each), j = (int)(c - (long long)b * each);
         const float score = a.scores[row0 + b];
         const double lse = s.lse[b];
         const unsigned long long p = kept[i];
         double v = -INFINITY;
-        int token = ~(int)(uint32_t)p;
+        logit[i] = p;
+        beam[i] = kMaxBeams - 1 - b;
         if (!(fabs(lse) < INFINITY) || !(score < INFINITY) || score == -INFINITY) {
           // a beam that offers nothing: of its tokens, all -inf, the first ones
           take = j < a.count && j < a.vocab;
-          token = j;
+          logit[i] = (uint32_t)~j;
         } else {
           take = p != 0;
           v = (double)score + ((double)unrank((uint32_t)(p >> 32)) - lse);
         }
         if (take) key[i] = rank_key64(v);
-        place[i] = ~((unsigned long long)b * a.vocab + token);
       }
       best = max(best, (uint32_t)(key[i] >> 32));
     }
@@ -402,19 +406,21 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
     for (int i = 0; i < kPickEach; ++i) {
       const bool take = key[i] && key[i] >= least;
       const int at = place_of(take, &s.n);
-      if (take) s.value[at] = key[i], s.place[at] = place[i];
+      if (take) s.value[at] = key[i], s.logit[at] = logit[i], s.beam[at] = (uint16_t)beam[i];
     }
     if (c0 + kPickChunk < total) fetch(c0 + kPickChunk);
     __syncthreads();
     const int n = s.n;
     const int enough = c0 + kPickChunk < total ? a.count : a.count + kFew;
     if (n > enough) {  // a few are ranked as they are
-      unsigned long long value[E], place[E];
+      unsigned long long value[E], logit[E];
+      int beam[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int i = threadIdx.x + j * kPickThreads;
         value[j] = i < n ? s.value[i] : 0;
-        place[j] = i < n ? s.place[i] : 0;
+        logit[j] = i < n ? s.logit[i] : 0;
+        beam[j] = i < n ? s.beam[i] : 0;
       }
       auto reaching = [&](unsigned long long t) {
         int k = 0;
@@ -423,28 +429,41 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
         return k;
       };
       least = bound_of(a.count, enough, least, ~0ull - 1, count, reaching);
-      // of equal values at the bound, where they are many, those of the lowest places
+      // of equal values at the bound, where they are many, those of the lowest beams, of the last of these the greatest logits
       int above = 0, reach = 0;
 #pragma unroll
       for (int j = 0; j < E; ++j) above += value[j] > least, reach += value[j] >= least;
       above = count(above);
       reach = count(reach);
+      int last = -1;
       unsigned long long first = 0;
-      if (above < a.count && reach > enough)
-        first = bound_of(a.count - above, a.count - above, 0, ~0ull - 1, count, [&](unsigned long long t) {
+      if (above < a.count && reach > enough) {
+        int want = a.count - above, before = 0;
+        last = (int)bound_of(want, want, 0, kMaxBeams - 1, count, [&](unsigned long long t) {
           int k = 0;
 #pragma unroll
-          for (int j = 0; j < E; ++j) k += value[j] == least && place[j] >= t;
+          for (int j = 0; j < E; ++j) k += value[j] == least && beam[j] >= (int)t;
           return k;
         });
+#pragma unroll
+        for (int j = 0; j < E; ++j) before += value[j] == least && beam[j] > last;
+        want -= count(before);
+        first = bound_of(want, want, 0, ~0ull - 1, count, [&](unsigned long long t) {
+          int k = 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j) k += value[j] == least && beam[j] == last && logit[j] >= t;
+          return k;
+        });
+      }
       __syncthreads();
       if (threadIdx.x == 0) s.n = 0;
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const bool take = value[j] > least || (value[j] == least && value[j] && place[j] >= first);
+        const bool take = value[j] > least ||
+                          (value[j] == least && value[j] && (beam[j] > last || (beam[j] == last && logit[j] >= first)));
         const int at = place_of(take, &s.n);
-        if (take) s.value[at] = value[j], s.place[at] = place[j];
+        if (take) s.value[at] = value[j], s.logit[at] = logit[j], s.beam[at] = (uint16_t)beam[j];
       }
     }
     __syncthreads();
@@ -452,21 +471,20 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const __grid_co
   // the best of them, each to its rank
   const int n = s.n;
   for (int i = warp; i < n; i += kPickThreads / 32) {
-    const unsigned long long v = s.value[i], p = s.place[i];
+    const unsigned long long v = s.value[i], p = s.logit[i];
+    const int b = s.beam[i];
     int rank = 0;
 #pragma unroll 4
     for (int j = lane; j < n; j += 32) {
       const unsigned long long u = s.value[j];
-      rank += u > v || (u == v && s.place[j] > p);
+      rank += u > v || (u == v && (s.beam[j] > b || (s.beam[j] == b && s.logit[j] > p)));
     }
     rank = __reduce_add_sync(0xffffffffu, rank);
     if (rank >= a.count || lane) continue;
     const long long out = (long long)batch * a.count + rank;
-    const unsigned long long at = ~p;
-    const int b = (int)(at >> 32 ? at / (unsigned)a.vocab : (uint32_t)at / (uint32_t)a.vocab);
     a.scores_out[out] = (float)unrank64(v);
-    a.beams_out[out] = b;
-    a.tokens_out[out] = (int)(at - (unsigned long long)b * a.vocab);
+    a.beams_out[out] = kMaxBeams - 1 - b;
+    a.tokens_out[out] = (int)~(uint32_t)p;
   }
 }
 

@@ -152,3 +152,23 @@ def test_rows_that_rise_with_every_tile(cuda):
     assert torch.all(beams == 0) and torch.all(tokens[:, 0] == int(torch.nonzero(tile == tile[-1])[0]))
     off = (got[:, 0].double() - want).abs().max().item()
     assert off <= 2.0 ** -21, f"{off * 2 ** 21:.3g} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize(("beams", "vocab", "count"), [(1, 5000, 20), (3, 5000, 128), (4, 5, 17), (300, 9, 100), (2, 30011, 1)])
+def test_within_a_beam_the_higher_logit_wins(cuda, dtype, beams, vocab, count):
+    """Scores so far from zero that 64 bits hold no difference of the logits: all values of beams of one score are equal,
+    and the lower beam's come first, by logit, then token."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab + beams)
+    logits = (torch.randn((2 * beams, vocab), generator=gen, device="cuda") * 3).to(dtype)
+    scores = torch.full((2, beams), -1.0e20, device="cuda")
+    if beams > 1:
+        scores[1, 0] = -2.0e20  # behind all others
+    value, which, token = beam.select(logits, scores, count)
+    for b, order in enumerate((list(range(beams)), [*range(1, beams), 0])):
+        want = []
+        for i in order:
+            row = logits[b * beams + i].double()
+            want += [(i, int(t)) for t in torch.sort(row, descending=True, stable=True).indices[:count]]
+        assert list(zip(which[b].tolist(), token[b].tolist())) == want[:count]
+        assert torch.equal(value[b], scores[b][which[b].long()])
