@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) beam_scan_kernel(const __grid
   __shared__ double sums[kScanThreads / 32];
   __shared__ float refs[kScanThreads / 32];
   const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int begin = blockIdx.x * a.part, end = min(a.vocab, begin + a.part);
+  const int begin = blockIdx.x * a.part, end = begin + min(a.vocab - begin, a.part);
   const T* logits = (const T*)a.logits + row * a.stride;
   const bool wide = ((uintptr_t)logits & 15) == 0;
   BlockCount count{red, 0};

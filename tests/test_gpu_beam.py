@@ -172,3 +172,18 @@ def test_within_a_beam_the_higher_logit_wins(cuda, dtype, beams, vocab, count):
             want += [(i, int(t)) for t in torch.sort(row, descending=True, stable=True).indices[:count]]
         assert list(zip(which[b].tolist(), token[b].tolist())) == want[:count]
         assert torch.equal(value[b], scores[b][which[b].long()])
+
+
+def test_the_longest_rows(cuda):
+    """The last part of a row that ends 65536 short of 2^31."""
+    vocab = 0x7fff0000
+    logits = torch.full((1, vocab), -INF, dtype=BF16, device="cuda")
+    at = {vocab - 1: 2.0, 3: 1.0, vocab - 4097: 1.5, vocab - 2000000: -1.0}
+    for token, x in at.items():
+        logits[0, token] = x
+    value, _, token = beam.select(logits, torch.zeros((1, 1), device="cuda"), 4)
+    assert token[0].tolist() == sorted(at, key=at.get, reverse=True)
+    x = torch.tensor(sorted(at.values(), reverse=True), dtype=torch.float64)
+    torch.testing.assert_close(value[0].cpu().double(), x - torch.logsumexp(x, 0), rtol=0, atol=2.0 ** -20)
+    with pytest.raises(ValueError, match="vocabulary"):
+        beam.select(torch.empty((1, vocab + 1), dtype=BF16, device="cuda"), torch.zeros((1, 1), device="cuda"), 4)
