@@ -14,20 +14,41 @@ def from_text(text: list[int], *, nodes: int = 32, length: int = 8, match: int =
     tokens: list[int] = []
     parents: list[int] = []
     children: dict[tuple[int, int], int] = {}
-    n = len(text)
-    for m in range(min(match, n - 1), 0, -1):
-        for at in range(n - m - 1, -1, -1):
-            if text[at:at + m] != text[n - m:]:
-                continue
-            parent = -1
-            for t in text[at + m:at + m + length]:
-                if (parent, t) not in children:
-                    if len(tokens) == nodes:
-                        return tokens, parents
-                    children[parent, t] = len(tokens)
-                    tokens.append(t)
-                    parents.append(parent)
-                parent = children[parent, t]
-        if tokens:
+
+    def add(at: int) -> bool:
+        """The guesses text[at:at + length]; False once there are `nodes`."""
+        parent = -1
+        for t in text[at:at + length]:
+            if (parent, t) not in children:
+                if len(tokens) == nodes:
+                    return False
+                children[parent, t] = len(tokens)
+                tokens.append(t)
+                parents.append(parent)
+            parent = children[parent, t]
+        return True
+
+    # the places where the last token occurred before, the latest first, by list.index (100000 tokens in a millisecond),
+    # and how many tokens up to there recur
+    n, back, at = len(text), text[::-1], 0
+    most, found = 1, []
+    while match > 0 and n:
+        try:
+            at = back.index(back[0], at + 1)
+        except ValueError:
             break
+        m = 1
+        while m < match and at + m < n and back[at + m] == back[m]:
+            m += 1
+        if m == match:
+            if not add(n - at):
+                return tokens, parents
+        elif m > most:
+            most, found = m, [at]
+        elif m == most:
+            found.append(at)
+    if not tokens:
+        for at in found:
+            if not add(n - at):
+                break
     return tokens, parents

@@ -177,3 +177,50 @@ def test_a_text_that_repeats_itself():
     tokens, parents = draft.from_text(long, nodes=5, length=20)
     assert tokens == [0, 1, 2, 3, 4] and parents == [-1, 0, 1, 2, 3]
     assert all(p < i for i, p in enumerate(parents))
+
+
+def _from_text(text, nodes, length, match):
+    """draft.from_text by its definition."""
+    tokens, parents, children, n = [], [], {}, len(text)
+    for m in range(min(match, n - 1), 0, -1):
+        for at in range(n - m - 1, -1, -1):
+            parent = -1
+            for t in text[at + m:at + m + length] if text[at:at + m] == text[n - m:] else ():
+                if (parent, t) not in children:
+                    if len(tokens) == nodes:
+                        return tokens, parents
+                    children[parent, t] = len(tokens)
+                    tokens.append(t)
+                    parents.append(parent)
+                parent = children[parent, t]
+        if tokens:
+            break
+    return tokens, parents
+
+
+class _Counted(list):
+    """A list that counts how often its elements are asked for, and those of its copies."""
+
+    asked = [0]
+
+    def __getitem__(self, at):
+        self.asked[0] += 1
+        got = super().__getitem__(at)
+        return _Counted(got) if isinstance(at, slice) else got
+
+
+def test_drafts_from_short_texts_of_few_tokens():
+    rng = np.random.default_rng(0)
+    for _ in range(3000):
+        text = rng.integers(0, rng.integers(1, 6), rng.integers(0, 30)).tolist()
+        nodes, length, match = (int(rng.integers(0, top)) for top in (10, 6, 5))
+        assert draft.from_text(text, nodes=nodes, length=length, match=match) == _from_text(text, nodes, length, match)
+
+
+@pytest.mark.parametrize(("vocab", "most"), [(1000000, 100), (300, 6000), (2, 1000)])
+def test_a_draft_looks_only_where_the_last_token_recurs(vocab, most):
+    """A long text in which little or nothing recurs: a draft is made for every call, and costs less than one."""
+    text = _Counted(np.random.default_rng(vocab).integers(0, vocab, 100000).tolist())
+    _Counted.asked[0] = 0
+    draft.from_text(text)
+    assert _Counted.asked[0] <= most
