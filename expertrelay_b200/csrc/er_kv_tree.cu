@@ -189,6 +189,14 @@ extern "C" int er_kv_tree(const er_kv_cache* cache, const er_kv_tree_io* io, voi
   if (!io->q || !io->out || !io->lens || !io->starts || !io->parents)
     return fail(ER_EINVAL, "er_kv_tree: null pointer");
   if ((uintptr_t)io->out & 15) return fail(ER_EINVAL, "er_kv_tree: out must be 16-byte aligned");
+  // A unit's queries are read by its own CTAs alone, and before its rows are written: results may take the place of
+  // their own queries, but for heads that two units share.
+  const long long each = (long long)io->heads * cache->head_dim, es = io->q_dtype == ER_DTYPE_BF16 ? 2 : 4;
+  const uintptr_t q = (uintptr_t)io->q, out = (uintptr_t)io->out;
+  if (q < out + io->rows * each * es && out < q + ((io->rows - 1) * io->q_stride + each) * es &&
+      (q != out || (io->rows > 1 && io->q_stride != each) || cache->head_dim > kTreeChannels))
+    return fail(ER_EINVAL, "er_kv_tree: q and out share memory (only the same rows may, of at most %d channels a head)",
+                kTreeChannels);
   int sms = 0;
   if (int rc = device_sms(&sms)) return rc;
   if (sms > kJoinMost) sms = kJoinMost;

@@ -445,7 +445,8 @@ def attend_tree(cache: PagedKV, q: torch.Tensor, lens: torch.Tensor, starts: tor
     4096 trees of at most 256 nodes; a chain (each node the next one's parent) is
     a piece of a text.
 
-    Rows of no tree are left as they were in `out`. scale, workspace: as for attend."""
+    Rows of no tree are left as they were in `out`, which may be q itself (contiguous, head_dim up to 128) or shares no
+    memory with it. scale, workspace: as for attend."""
     rows, heads, stride = _queries(cache, q)
     if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] == 0:
         raise ValueError("starts: expected [trees + 1] int32")

@@ -508,7 +508,8 @@ typedef struct er_kv_tree_io {
   const void* q;               /* [rows, heads, head_dim], row stride q_stride elements */
   int q_dtype;                 /* ER_DTYPE_F32 / ER_DTYPE_BF16; out has it too */
   long long q_stride;
-  void* out;                   /* [rows, heads, head_dim] contiguous, 16-byte aligned */
+  void* out;                   /* [rows, heads, head_dim] contiguous, 16-byte aligned; q itself, if contiguous and of
+                                  head_dim <= 128, or apart from it */
   int rows, heads;             /* heads <= 65536 */
   int trees;
   const int32_t* starts;       /* [trees + 1] */

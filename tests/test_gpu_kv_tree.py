@@ -367,3 +367,22 @@ def test_a_wait_that_runs_out_is_reported_and_spoils_every_row(cuda, cache_dtype
 
 def test_the_stall_of_waits_has_two_modes():
     assert _lib.lib().er_kv_tree_test_stall(0, 2) == _lib.ER_EINVAL and _lib.lib().er_kv_tree_test_stall(0, -1) == _lib.ER_EINVAL
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("lens", "d"), [([700, 20, 0], 128), ([9000], 64)])
+def test_results_in_the_place_of_their_queries(cuda, cache_dtype, q_dtype, lens, d):
+    rng = np.random.default_rng(2)
+    trees = [_tree(rng, 70) for _ in lens]
+    cache, q, ln, starts, parents = _case(15, lens, trees, 2, 3, d, 16, cache_dtype, q_dtype)
+    want = kv.attend_tree(cache, q, ln, starts, parents)
+    assert kv.attend_tree(cache, q, ln, starts, parents, out=q) is q and torch.equal(q, want)
+
+
+def test_results_over_other_queries_are_refused(cuda):
+    cache, q, ln, starts, parents = _case(15, [30], [[-1, 0]], 2, 3, 256, 16, BF16, BF16)
+    both = torch.empty((3, 6, 256), dtype=BF16, device="cuda")
+    for queries, out in ((q, q), (both[:2], both[1:])):
+        with pytest.raises(ValueError, match="share memory"):
+            kv.attend_tree(cache, queries, ln, starts, parents, out=out)
+    assert kv.attend_tree(cache, both[:2], ln, starts, parents, out=q) is q

@@ -224,3 +224,12 @@ def test_a_draft_looks_only_where_the_last_token_recurs(vocab, most):
     _Counted.asked[0] = 0
     draft.from_text(text)
     assert _Counted.asked[0] <= most
+
+
+@pytest.mark.parametrize(("cache", "change"), [
+    ({}, {"out": P + 16}), ({}, {"out": P, "q": P + 5 * 4 * 64 * 2 - 2}), ({}, {"q_stride": 4 * 64 + 8}),
+    ({}, {"out": P + 4 * (4 * 64 + 8) * 2, "q_stride": 4 * 64 + 8}),
+    ({"head_dim": 136, "slot_stride": 136, "head_stride": 16 * 136, "page_stride": 2 * 16 * 136}, {"q_stride": 4 * 136}),
+])
+def test_results_over_other_queries_are_refused(cache, change):
+    _fails(_lib.lib().er_kv_tree(C.byref(_cache(**cache)), C.byref(_tree(**change)), None, 0, None), "share memory")
