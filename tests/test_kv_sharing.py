@@ -233,3 +233,11 @@ def test_a_draft_looks_only_where_the_last_token_recurs(vocab, most):
 ])
 def test_results_over_other_queries_are_refused(cache, change):
     _fails(_lib.lib().er_kv_tree(C.byref(_cache(**cache)), C.byref(_tree(**change)), None, 0, None), "share memory")
+
+
+def test_lengths_over_what_a_compaction_reads_are_refused():
+    """rows 3, lists of 4 by a stride of 5, at addresses of their own; lens_out over each in turn."""
+    L, c = _lib.lib(), _cache()
+    seqs, start, keep, counts = (P * i for i in (1, 2, 3, 4))
+    for out in (seqs, start, start + 8, start - 8, keep, keep + 4 * 13, counts, counts - 4):
+        _fails(L.er_kv_compact(C.byref(c), 2, 1 << 16, seqs, start, keep, 5, 4, counts, 3, out, None, None), "lens_out")
