@@ -240,6 +240,10 @@ extern "C" int er_kv_compact(const er_kv_cache* cache, int layers, long long lay
     return fail(ER_EINVAL, "er_kv_compact: %d rows, %d sequences", rows, cache->seqs);
   if (rows == 0) return ER_OK;
   if (!start || !counts || (most > 0 && !keep)) return fail(ER_EINVAL, "er_kv_compact: null pointer");
+  // one CTA of a row writes its length when others may not have read what the row is to do
+  auto meets = [&](const int32_t* p, long long n) { return p && lens_out && p < lens_out + rows && lens_out < p + n; };
+  if (meets(start, rows) || meets(counts, rows) || meets(seqs, rows) || meets(keep, (rows - 1) * keep_stride + most))
+    return fail(ER_EINVAL, "er_kv_compact: lens_out shares memory with what the call reads");
   a.seqs = seqs, a.start = start, a.keep = keep, a.counts = counts, a.rows = rows, a.most = most;
   a.keep_stride = keep_stride, a.lens_out = lens_out, a.status = status;
   const long long fill = (long long)kThreads * kMany / ((long long)(most ? most : 1) * a.l.row16);

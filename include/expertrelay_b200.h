@@ -543,8 +543,9 @@ ER_API int er_kv_copy_pages(const er_kv_cache* cache, int layers, long long laye
  * start[r] + keep[r * keep_stride + j] of sequence seqs[r] (seqs NULL: r) goes
  * to place start[r] + j, j < counts[r] <= most; keep ascends, from 0 at the
  * least. lens_out[r] (optional) = start[r] + counts[r], or -1 where something is
- * wrong with the row, which then stays as it was. A sequence may occur once in
- * a call, and the pages that it writes belong to it alone. */
+ * wrong with the row, which then stays as it was; it is none of the call's other
+ * arrays. A sequence may occur once in a call, and the pages that it writes
+ * belong to it alone. */
 ER_API int er_kv_compact(const er_kv_cache* cache, int layers, long long layer_stride, const int32_t* seqs,
                          const int32_t* start, const int32_t* keep, long long keep_stride, int most,
                          const int32_t* counts, int rows, int32_t* lens_out, int* status, void* stream);
