@@ -617,8 +617,10 @@ __global__ void __launch_bounds__(S::kThreads, 1)
       // what the sums so far are multiplied by, once the greatest score is `top`, and the exponents' shift
       auto rise = [&](float top, float* shift) {
         const float ref = top == -INFINITY ? 0.f : top;
-        *shift = -ref * a.scale;
-        const float by = ex2(fmaf(m, a.scale, *shift));
+        *shift = __fmul_rn(-ref, a.scale);
+        // by the difference of the two shifts as they are, rounded: 1 where the greatest score stays. (With a product
+        // that is not rounded it is 1 and what the shift's rounding took, once a tile: 1e-5 of a result of 32768 keys.)
+        const float by = ex2(__fadd_rn(__fmul_rn(m, a.scale), *shift));
         m = top;
         if (row < S::ROWS) s.by[it & 7][row] = by;
         __syncwarp();

@@ -386,3 +386,35 @@ def test_results_over_other_queries_are_refused(cuda):
         with pytest.raises(ValueError, match="share memory"):
             kv.attend_tree(cache, queries, ln, starts, parents, out=out)
     assert kv.attend_tree(cache, both[:2], ln, starts, parents, out=q) is q
+
+
+@pytest.mark.parametrize(("cache_dtype", "q_dtype"), TYPES)
+@pytest.mark.parametrize(("trees", "kv_heads", "group", "n", "d", "nodes"), [(4, 40, 1, 20000, 64, 3), (6, 32, 2, 8000, 128, 9), (3, 64, 4, 5000, 256, 2)])
+def test_long_units_of_one_cta_are_as_exact(cuda, cache_dtype, q_dtype, trees, kv_heads, group, n, d, nodes):
+    """More units than CTAs, so that one goes through a unit's hundreds of tiles by itself: the bound of
+    test_trees_are_as_exact_as_32_bits."""
+    score, value = (6, 6) if cache_dtype == F32 else (3, 3) if q_dtype == F32 else (1, 2)
+    bound = result_bound(d, n) + (score * d / 32 + value * 4 / 2) * U
+    if cache_dtype == q_dtype == BF16:
+        bound += 2.0 ** -18
+    gen = torch.Generator(device="cuda").manual_seed(n + d)
+    each = -(-(n + nodes) // 16)
+    k, v = (torch.randn((trees * each, kv_heads, 16, d), generator=gen, device="cuda").to(cache_dtype) for _ in range(2))
+    table = torch.randperm(trees * each, generator=gen, device="cuda").to(torch.int32).view(trees, each)
+    cache = kv.PagedKV(k, v, table)
+    outs, wants = [], []
+    for _ in range(1 if q_dtype == F32 else 12):  # enough of them that cross a border between two bf16 values
+        q = torch.randn((trees * nodes, kv_heads * group, d), generator=gen, device="cuda").to(q_dtype)
+        starts = torch.arange(trees + 1, dtype=torch.int32, device="cuda") * nodes
+        outs.append(kv.attend_tree(cache, q, _i32([n] * trees), starts, _i32([-1] * (trees * nodes))))
+        of = q.view(trees, nodes, kv_heads, group, d)
+        want = torch.empty(of.shape, dtype=torch.float64, device="cuda")
+        for t in range(trees):
+            kk, vv = (x[table[t].long()].transpose(0, 1).reshape(1, kv_heads, each * 16, d) for x in (k, v))
+            for i in range(nodes):
+                see = [torch.cat([x[:, :, :n], x[:, :, n + i:n + i + 1]], 2) for x in (kk, vv)]
+                want[t, i] = attend_exact(of[t, i][None], *see, d ** -0.5)[0]
+        wants.append(want.view(q.shape))
+    got = result_error(torch.stack(outs), torch.stack(wants), q_dtype)
+    assert got <= bound, f"{got:.3g} of the result, {bound:.3g} allowed"
+    cache.check()
