@@ -9,10 +9,11 @@
 // was kept, by values in 64 bits: candidates of one beam keep the order of
 // their logits, those of different beams compare through their beams' log-sums.
 // 2 or 4 bytes a candidate and about a dozen instructions: 256 rows of 151936
-// bf16 logits take 36 us (0.33 of the copy rate), the instructions and the
-// barrier of a tile; then the choice over 32 batches 12 us, a chain of
-// dependent steps in one CTA a batch, most of it fetching code. 4 fp32 rows:
-// 15 us for both kernels (a tile a CTA; 19 as called), 140 rows of 50257: 33 us.
+// bf16 logits take 37 us (0.32 of the copy rate): 19 of instructions at the full
+// rate, the barrier of a tile, and 768 CTAs for the 592 that run at once; then the
+// choice over 32 batches 13 us, a chain of dependent steps in one CTA a batch, most
+// of it fetching code. 4 fp32 rows: 15.5 us for both kernels (a tile a CTA; 19 as
+// called), 140 rows of 50257: 33 us (700 CTAs, and a load an element).
 // Exponentials, relative to a whole number that is no less than a warp's logits
 // and mostly under one more than the greatest, are in 32 bits (2^-22 off, and
 // |x - ref| 2^-22), and so is the sum of a thread's 16 of a tile; all sums above

@@ -105,7 +105,7 @@ struct CompactArgs {
 // places, 490 MB in all: 114 us, with whole heads 125, with 64 bytes 118). DRAM
 // bounds it; the last CTAs are those of the shortest lists (104 us, 4.7 TB/s:
 // before and behind a batch's barrier only loads or only stores are under way).
-// An accepted draft's 5 places in 24 layers: 5.4 us, latency.
+// An accepted draft's 5 places in 24 layers: 5.5 us, latency.
 constexpr int kBatchRows = 512, kCut = 8;  // kCut: vectors of a place a CTA has at least
 
 __global__ void __launch_bounds__(kThreads) kv_compact_kernel(const __grid_constant__ CompactArgs a) {

@@ -23,20 +23,26 @@
 // limit, after which the CTA reports, ends, and leaves the join to spoil all of the call's rows.
 //
 // Measured (queued calls; of the bytes' time at the measured copy rate):
-// 24 drafts of 23 after up to 4097 positions, 16 heads of 128, bf16: 140-145 us
-// (0.47): a copy's issue (200 clocks for 16 rows of a page) and what lies
+// 24 drafts of 23 after up to 4097 positions, 16 heads of 128, bf16: 129-138 us
+// (0.48-0.52): a copy's issue (200 clocks for 16 rows of a page) and what lies
 // between a CTA's units (queries, masks, result: 5000 clocks and more).
-// 8 drafts of 64 after 32768, 4 key heads of 8, bf16: 575-600 us under the power
-// cap, 0.47 PFLOP/s (495 in a short run): the weights' warps, 1650 clocks a
-// tile; products 1050. With one warp for both kinds of products 1790 and 627 us.
+// 8 drafts of 64 after 32768, 4 key heads of 8, bf16: 575-603 us under the power
+// cap, 0.46 PFLOP/s (503 in a short run): the weights' warps, 1650 clocks a
+// tile; products 1050. Its keys and values are read once for each 128 rows, four times. With one warp for both kinds of products 1790 and 627 us.
 // Two groups of weights' warps that take the tiles in turn: 682 us in a short
-// run (96 registers a thread in place of 128); 544 threads in place of 512: 788.
+// run (96 registers a thread in place of 128, all warps alike: none were moved
+// between them); 544 threads in place of 512: 788.
 // A chain of 16 after 131071, 2 key heads of 6 of 64, fp32 queries: 53-55 us
 // (0.19): three parts of queries and weights, 14 tiles a CTA, then the join, 9.
-// 6 fp32 drafts of 37 after up to 2500: 156 us, six products a pair of operands
+// 6 fp32 drafts of 37 after up to 2500: 153-156 us, six products a pair of operands
 // (48 for a tile's scores, 67 clocks each) and the splitting. A draft of 8
 // after 631 positions: 32 us, two tiles a CTA, each step of which is fetched and
-// run for the first time.
+// run for the first time. Forms far from their floor, 8 drafts of 24 after 8000, 4
+// key heads of 2: heads of 256 bf16 107 us (floor 40), with fp32 queries 249; over
+// an fp32 cache 1985 (floor 81; 32 rows a unit, one tile of keys and one of values
+// in shared memory, loads by threads in place of TMA); heads of 128 over an fp32
+// cache 184 (floor 40), and 186 with bf16 queries, whose two lower parts are
+// multiplied although they hold next to nothing.
 #pragma once
 
 #include <type_traits>
@@ -789,8 +795,9 @@ __global__ void __launch_bounds__(S::kThreads, 1)
     Ring<SB> ring;  // of tiles of scores or weights
     int tiles = 0;
     bool ok = true;
-    // Descriptors are put together where they are used, from words the compiler cannot know before: those that it kept
-    // over the waits' calls came out wrong. The small products first.
+    // Descriptors are put together where they are used, from words the compiler cannot know before, so that none lives
+    // over a call (bar_wait_slow, tree_next, next_queries): over those live 32-bit addresses, rings and counts only.
+    // The small products first.
     if (warp == kIssueWarp) {
       const int ksteps = (d + 15) / 16;
       const uint32_t is = idesc_bf16(TK, 0);

@@ -286,7 +286,9 @@ class QwenMoeModel:
         draft(text) gets the prompt and what has come so far and returns (tokens,
         parents), a tree of guesses at what comes next (kv.attend_tree's order; -1:
         the text's last token; none is fine). One call runs them all, and the
-        path that greedy decoding would have taken stays. Returns (generated ids,
+        path that greedy decoding would have taken stays (by that call's logits: they
+        are rounded otherwise than those of a call of one token, and drafted tokens
+        see all pages of a cache with `select`). Returns (generated ids,
         calls after the prompt's). kv: a cache of one's own, without accumulated
         weights; the prompt goes on from what its sequence `seq` holds (room for
         the prompt, new_tokens and a call's guesses)."""
