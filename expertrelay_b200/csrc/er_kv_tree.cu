@@ -20,6 +20,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv_tree_join_kernel(const 
   __shared__ float2 tops[kJoinWarps];
   kv_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = a.kv.d;
+  auto spoil = [&](bool all) {
+    for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.trees; t += gridDim.x * gridDim.y) {
+      const Tree e = kv_tree(a, t);
+      if (!e.bad && !all) continue;
+      TQ* out = (TQ*)a.out + (long long)e.first * a.heads * d;
+      for (long long i = threadIdx.x; i < (long long)e.nodes * a.heads * d; i += kJoinWarps * 32)
+        out[i] = kv_round<TQ>(__int_as_float(0x7fc00000));
+    }
+  };
+  spoil(false);  // beside the other warps' look at the cuts
   if (warp == 0) {  // the CTAs in whose runs such a unit begins
     int n = 0;
     bool gave_up = false;
@@ -34,13 +44,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) kv_tree_join_kernel(const 
     if (lane == 0) found = gave_up ? -1 : n;
   }
   __syncthreads();
-  for (int t = blockIdx.y * gridDim.x + blockIdx.x; t < a.trees; t += gridDim.x * gridDim.y) {
-    const Tree e = kv_tree(a, t);
-    if (!e.bad && found >= 0) continue;
-    TQ* out = (TQ*)a.out + (long long)e.first * a.heads * d;
-    for (long long i = threadIdx.x; i < (long long)e.nodes * a.heads * d; i += kJoinWarps * 32)
-      out[i] = kv_round<TQ>(__int_as_float(0x7fc00000));
-  }
+  if (found < 0) spoil(true);
   constexpr int N = 8;  // pieces under way
 #pragma unroll 1
   for (int f = blockIdx.x; f < found; f += gridDim.x) {
